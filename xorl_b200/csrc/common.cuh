@@ -41,6 +41,7 @@ enum XbKernelId : int {
   XB_K_FP8_GEMM = 10,
   XB_K_FLAG_WAIT_TEST = 11,
   XB_K_RING_ATTN = 12,
+  XB_K_RECURRENCE = 13,
 };
 
 // Kernels receive the per-device status array as an argument (see xb_status_ptr()).

@@ -1,0 +1,1403 @@
+// Gated linear recurrences over packed documents, forward and backward: the gated delta rule (GatedDeltaNet)
+// and the state-space scan with a scalar decay per head (Mamba2).
+//
+//   delta:  S_t = a_t S_{t-1} + k_t (x) u_t,  u_t = b_t (v_t - (a_t S_{t-1})^T k_t),  o_t = S_t^T q_t
+//   scan:   S_t = a_t S_{t-1} + k_t (x) u_t,  u_t = b_t v_t,                          o_t = S_t^T q_t + D v_t
+//
+// (scan: q = C, k = B, v = x, b = dt, log a = dt A.)  S is [dk, dv] per head; q / k heads are shared by groups of v heads.
+// A document is cut into chunks of 64 tokens.  With G the running sum of log a inside a chunk, gamma = e^G,
+// D_ij = e^{G_i - G_j} for j <= i, d_j = e^{G_last - G_j}, and S the state that enters the chunk:
+//
+//   L = diag(b) tril(D o K K^T, -1),  T = (I + L)^-1,  R = diag(b) (V - diag(gamma) K S),  U = T R     (scan: U = diag(b) V)
+//   O = diag(gamma) Q S + tril(D o Q K^T) U,     S' = gamma_last S + K^T diag(d) U
+//
+// and backwards, from dS' and dO, with P = tril(D o Q K^T):
+//
+//   dU = P^T dO + diag(d) K dS',  dR = T^T dU,  dV = diag(b) dR,
+//   dS = gamma_last dS' + Q^T diag(gamma) dO - K^T diag(b gamma) dR
+//   dP = dO U^T,  dL = -dR U^T (strictly below the diagonal),  Z = D o dP,  W = diag(b) (D o dL)
+//   dQ = diag(gamma) dO S^T + Z K,   dK = -diag(b gamma) dR S^T + W K + W^T K + Z^T Q + diag(d) U dS'^T
+//
+// The gradient of G_i is the sum of q.dq and k.dk over the places where row i carries e^{G_i}, minus those where it
+// carries e^{-G_i}; the gradient of log a_t is its suffix sum inside the chunk.
+//
+// Precision: q, k, v and dO are bf16 and enter the products as they are.  Whatever is computed (states, T, U, P and
+// their gradients) is kept in 32 bits and enters a product as the sum of two bf16 values, which keeps 17 bits of its
+// significand: one bf16 value (9 bits) would cost the fp32 gradients of the decay three decimal digits.  Products of
+// two such sums leave out low x low.  Decays are sums in fp64 of log2 units, kept as two floats, so that differences
+// of large sums stay exact.  L2 norms of q and k are row factors and are applied behind the products.
+#include "common.cuh"
+#include "recurrence.h"
+
+namespace {
+
+constexpr int C = 64;         // tokens of a chunk
+constexpr int NV = 32;        // state columns of a CTA of the sequential kernels
+constexpr int HD = 3 * C;     // per chunk and v head: G (two floats each, log2 units), b
+constexpr int RQK = 2 * C;    // per chunk and q / k head: row factors of q and k
+constexpr float MIN_LOG = -120.f;  // e^-120 is 0 in fp32: a stronger decay changes nothing and would cost G its digits
+
+using bf16 = __nv_bfloat16;
+
+// ---- fragments ---------------------------------------------------------------------------------------------
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+               "{%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// two fp32 values as the sums of two bf16 values each
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  hi = pack_bf16x2(x, y);
+  const float2 h = unpack_bf16x2(hi);
+  lo = pack_bf16x2(x - h.x, y - h.y);
+}
+__device__ __forceinline__ float2 join2(uint32_t hi, uint32_t lo) {
+  const float2 h = unpack_bf16x2(hi), l = unpack_bf16x2(lo);
+  return make_float2(h.x + l.x, h.y + l.y);
+}
+
+// A tile is rows of U 16-byte units; unit u of a row lies at u ^ f(row), so that the eight rows that ldmatrix reads
+// at one unit fall into eight different banks.
+template <int U>
+__device__ __forceinline__ uint32_t swz(int row, int u) {
+  return (uint32_t)(row * U + (U == 4 ? (u ^ ((row >> 1) & 3)) : (u ^ (row & 7)))) * 16u;
+}
+// address of two neighbouring bf16 values (col even)
+template <int U>
+__device__ __forceinline__ uint32_t at2(int row, int col) {
+  return swz<U>(row, col >> 3) + (uint32_t)(col & 7) * 2u;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts32(uint32_t a, uint32_t v) {
+  asm volatile("st.shared.b32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+
+// fragment addresses of this lane; m0, n0, k0 are multiples of 8 (16 for the wide ones)
+template <int U>  // A[m][k], k contiguous
+__device__ __forceinline__ uint32_t addr_a(int m0, int k0) {
+  const int l = xb_lane();
+  return swz<U>(m0 + (l & 15), (k0 >> 3) + (l >> 4));
+}
+template <int U>  // A = X^T, X[k][m], m contiguous (transposing load)
+__device__ __forceinline__ uint32_t addr_at(int m0, int k0) {
+  const int l = xb_lane();
+  return swz<U>(k0 + (l & 7) + (l >> 4) * 8, (m0 >> 3) + ((l >> 3) & 1));
+}
+template <int U>  // B of two 8-wide column tiles, X[k][n], n contiguous (transposing load)
+__device__ __forceinline__ uint32_t addr_bt(int k0, int n0) {
+  const int l = xb_lane();
+  return swz<U>(k0 + (l & 15), (n0 >> 3) + (l >> 4));
+}
+template <int U>  // B of two 8-wide column tiles, X[n][k], k contiguous
+__device__ __forceinline__ uint32_t addr_b(int n0, int k0) {
+  const int l = xb_lane();
+  return swz<U>(n0 + (l & 7) + (l >> 4) * 8, (k0 >> 3) + ((l >> 3) & 1));
+}
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// ROWS rows of U units from `src` (row stride ld elements); units behind `cols` and rows behind `rows` become zero
+template <int U, int ROWS, int THREADS>
+__device__ __forceinline__ void load_tile(uint32_t dst, const bf16* src, long long ld, int rows, int cols) {
+#pragma unroll
+  for (int i = 0; i < ROWS * U / THREADS; ++i) {
+    const int idx = i * THREADS + threadIdx.x, r = idx / U, u = idx % U;
+    const bool ok = r < rows && u * 8 < cols;
+    cp16(dst + swz<U>(r, u), ok ? src + r * ld + u * 8 : src, ok);
+  }
+}
+template <int THREADS>
+__device__ __forceinline__ void load_floats(uint32_t dst, const float* src, int n) {
+  for (int i = threadIdx.x; i < n / 4; i += THREADS) cp16(dst + i * 16, src + i * 4, true);
+}
+
+// ---- plan: chunks of the documents -----------------------------------------------------------------------------
+// Documents 0 .. n-1 lie between the boundaries; n is the tail behind the last boundary, n + 1 the rows before the first.
+__device__ __forceinline__ int2 doc_range(const int* cu, int n, int T, int d) {
+  auto cut = [&](int i) { return min(max(cu[i], 0), T); };
+  if (d == n) return make_int2(cut(n), T);
+  if (d == n + 1) return make_int2(0, cut(0));
+  const int s = cut(d);
+  return make_int2(s, max(s, cut(d + 1)));
+}
+
+__global__ void __launch_bounds__(1024) rec_plan(const int* __restrict__ cu, int n, int T, int nc_max, int4* chunks,
+                                                 int* doc_off, int* status) {
+  __shared__ int warp_tot[32];
+  __shared__ int carry;
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, nd = n + 2;
+  if (tid == 0) carry = 0, doc_off[0] = 0;
+  __syncthreads();
+  for (int base = 0; base < nd; base += 1024) {
+    const int d = base + tid;
+    int v = 0;
+    if (d < nd) {
+      const int2 r = doc_range(cu, n, T, d);
+      v = (r.y - r.x + C - 1) / C;
+    }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+    if (lane == 31) warp_tot[w] = v;
+    __syncthreads();
+    if (w == 0) {
+      int t = warp_tot[lane];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, t, o);
+        if (lane >= o) t += u;
+      }
+      warp_tot[lane] = t;
+    }
+    __syncthreads();
+    const int incl = carry + v + (w ? warp_tot[w - 1] : 0);
+    // boundaries that overlap would need more chunks than the rows have: what does not fit is left out and reported
+    if (d < nd) {
+      doc_off[d + 1] = min(incl, nc_max);
+      if (incl > nc_max) xb_report(status, XB_ERR_BAD_ARG, XB_K_RECURRENCE, d);
+    }
+    __syncthreads();
+    if (tid == 0) carry += warp_tot[31];
+    __syncthreads();
+  }
+  const int total = doc_off[nd];
+  for (int c = tid; c < total; c += 1024) {
+    int lo = 0, hi = nd;                                     // doc_off[lo] <= c < doc_off[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (doc_off[mid] <= c) lo = mid; else hi = mid;
+    }
+    const int2 r = doc_range(cu, n, T, lo);
+    const int s = r.x + (c - doc_off[lo]) * C;
+    chunks[c] = make_int4(s, min(C, r.y - s), lo, 0);
+  }
+}
+
+// ---- prepare: what depends on one chunk alone --------------------------------------------------------------------
+template <int DKP, bool DELTA>
+struct PrepSmem {
+  uint8_t q[C * DKP * 2], k[C * DKP * 2];
+  float kk[DELTA ? C * C : 4];
+  float l[DELTA ? 2 : 1][DELTA ? C * C : 4];
+  float ghi[2][C], glo[2][C], b[2][C], rq[C], rk[C];
+};
+
+template <int DKP, bool DELTA>
+__global__ void __launch_bounds__(128) rec_prep(const XbRecArgs p) {
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  PrepSmem<DKP, DELTA>& sm = *reinterpret_cast<PrepSmem<DKP, DELTA>*>(smem_raw);
+  constexpr int U = DKP / 8;
+  const int kh = blockIdx.x % p.Hk, c = blockIdx.x / p.Hk;
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3;
+  if (c >= p.doc_off[p.n_docs + 2]) return;
+  const int4 ch = reinterpret_cast<const int4*>(p.chunks)[c];
+  if (DELTA && ch.z >= p.n_docs) return;
+  const int len = ch.y, rep = p.Hv / p.Hk;
+  const uint32_t sq = xb_smem_u32(sm.q), sk = xb_smem_u32(sm.k);
+  load_tile<U, C, 128>(sq, (const bf16*)p.q + ch.x * p.q_t + kh * p.q_h, p.q_t, len, p.dk);
+  load_tile<U, C, 128>(sk, (const bf16*)p.k + ch.x * p.k_t + kh * p.k_h, p.k_t, len, p.dk);
+  cp_commit();
+  cp_wait<0>();
+  __syncthreads();
+  {  // row factors: thread pair per row, one for q and one for k
+    const int row = tid & 63;
+    const uint32_t base = tid < C ? sq : sk;
+    float ss = 0.f;
+    if (p.l2norm) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const uint4 v = lds128(base + swz<U>(row, u));
+        const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = unpack_bf16x2(x[i]);
+          ss += f.x * f.x + f.y * f.y;
+        }
+      }
+    }
+    float r = p.l2norm ? 1.f / fmaxf(sqrtf(ss), 1e-12f) : 1.f;
+    if (tid < C) r *= p.scale;
+    if (row >= len) r = 0.f;
+    (tid < C ? sm.rq : sm.rk)[row] = r;
+    p.rqk[((long long)c * p.Hk + kh) * RQK + (tid < C ? 0 : C) + row] = r;
+  }
+  __syncthreads();
+  float* qk = p.qk + ((long long)c * p.Hk + kh) * (C * C);
+  float* kkg = DELTA ? p.kk + ((long long)c * p.Hk + kh) * (C * C) : nullptr;
+  const int r0 = w * 16 + g;
+#pragma unroll
+  for (int nt = 0; nt < 8; nt += 2) {
+    if (nt * 8 > w * 16 + 15) break;              // columns above the diagonal block are never read
+    float a1[2][4] = {}, a2[2][4] = {};
+#pragma unroll
+    for (int ks = 0; ks < DKP / 16; ++ks) {
+      uint32_t fq[4], fk[4], fb[4];
+      ldsm4(fb, sk + addr_b<U>(nt * 8, ks * 16));
+      ldsm4(fq, sq + addr_a<U>(w * 16, ks * 16));
+      mma(a1[0], fq, fb[0], fb[1]);
+      mma(a1[1], fq, fb[2], fb[3]);
+      if (DELTA) {
+        ldsm4(fk, sk + addr_a<U>(w * 16, ks * 16));
+        mma(a2[0], fk, fb[0], fb[1]);
+        mma(a2[1], fk, fb[2], fb[3]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        const int row = r0 + hh * 8, col = (nt + j) * 8 + 2 * t;
+        const float c0 = sm.rk[col], c1 = sm.rk[col + 1];
+        *reinterpret_cast<float2*>(qk + row * C + col) =
+            make_float2(sm.rq[row] * c0 * a1[j][2 * hh], sm.rq[row] * c1 * a1[j][2 * hh + 1]);
+        if (DELTA) {
+          const float2 v = make_float2(sm.rk[row] * c0 * a2[j][2 * hh], sm.rk[row] * c1 * a2[j][2 * hh + 1]);
+          *reinterpret_cast<float2*>(kkg + row * C + col) = v;
+          *reinterpret_cast<float2*>(sm.kk + row * C + col) = v;
+        }
+      }
+  }
+  // per v head: running log decays; the inverse of I + L, two heads at a time
+  for (int h0 = 0; h0 < rep; h0 += DELTA ? 2 : 4) {
+    if (!DELTA || w < 2) {
+      const int hh = h0 + w, h = kh * rep + hh;
+      if (hh < rep) {
+        double x[2];
+        float bb[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int row = 2 * lane + i;
+          x[i] = 0.0, bb[i] = 0.f;
+          if (row < len) {
+            const long long tok = ch.x + row;
+            bb[i] = p.b[tok * p.b_t + h * p.b_h];
+            float gv;
+            if (DELTA) {
+              gv = p.g[tok * p.g_t + h * p.g_h];
+              x[i] = (double)(gv < MIN_LOG ? MIN_LOG : gv) * 1.4426950408889634;
+            } else {
+              const double z = (double)bb[i] * (double)p.A[h];
+              x[i] = (z < (double)MIN_LOG ? (double)MIN_LOG : z) * 1.4426950408889634;
+            }
+          }
+        }
+        double s = x[0] + x[1];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double u = __shfl_up_sync(0xffffffffu, s, o);
+          if (lane >= o) s += u;
+        }
+        float* out = p.hd + ((long long)c * p.Hv + h) * HD;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int row = 2 * lane + i;
+          const double G = i ? s : s - x[1];
+          const float hi = (float)G, lo = (float)(G - (double)hi);
+          out[row] = hi, out[C + row] = lo, out[2 * C + row] = bb[i];
+          if (DELTA) sm.ghi[w][row] = hi, sm.glo[w][row] = lo, sm.b[w][row] = bb[i];
+        }
+      }
+    }
+    if (DELTA) {
+      __syncthreads();                        // also: kk is complete, the previous pair's L has been read
+      const int m = tid >> 6, j = tid & 63, hh = h0 + m;
+      if (hh < rep) {
+        // L, one column per thread: rows below the diagonal
+        for (int i = 0; i < C; ++i) {
+          float v = 0.f;
+          if (i > j) v = sm.b[m][i] * xb_ex2((sm.ghi[m][i] - sm.ghi[m][j]) + (sm.glo[m][i] - sm.glo[m][j])) * sm.kk[i * C + j];
+          sm.l[m][i * C + j] = v;
+        }
+      }
+      __syncthreads();
+      if (hh < rep) {
+        // column j of (I + L)^-1 by forward substitution; all threads of a head read the same row of L
+        float x[C];
+        const float4* L4 = reinterpret_cast<const float4*>(sm.l[m]);
+        float* out = p.tm + ((long long)c * p.Hv + kh * rep + hh) * (C * C) + j;
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+          float a0 = i == j ? 1.f : 0.f, a1 = 0.f, a2 = 0.f, a3 = 0.f;
+#pragma unroll
+          for (int k4 = 0; k4 < (i + 3) / 4; ++k4) {
+            const float4 l = L4[i * (C / 4) + k4];
+            a0 -= l.x * x[4 * k4];
+            if (4 * k4 + 1 < i) a1 -= l.y * x[4 * k4 + 1];
+            if (4 * k4 + 2 < i) a2 -= l.z * x[4 * k4 + 2];
+            if (4 * k4 + 3 < i) a3 -= l.w * x[4 * k4 + 3];
+          }
+          x[i] = (a0 + a1) + (a2 + a3);
+          out[i * C] = x[i];
+        }
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// ---- forward: one CTA carries NV columns of one head's state through one document ----------------------------------
+template <int DKP>
+struct SeqStage {
+  uint8_t q[C * DKP * 2], k[C * DKP * 2], v[C * NV * 2];
+  float hd[HD], rqk[RQK];
+};
+template <int DKP, bool DELTA>
+struct FwdSmem {
+  SeqStage<DKP> st[2];
+  uint8_t shi[DKP * NV * 2], slo[DKP * NV * 2];
+  uint8_t xhi[DELTA ? C * NV * 2 : 16], xlo[DELTA ? C * NV * 2 : 16];   // R
+  uint8_t uhi[DELTA ? C * NV * 2 : 16], ulo[DELTA ? C * NV * 2 : 16];   // U
+  uint8_t dhi[C * NV * 2], dlo[C * NV * 2];                             // K's row factor x d x U
+};
+
+__device__ __forceinline__ float ex2_diff(const float* hd, int i, int j) {
+  return xb_ex2((hd[i] - hd[j]) + (hd[C + i] - hd[C + j]));
+}
+__device__ __forceinline__ float ex2_sum(const float* hd, int i) { return xb_ex2(hd[i]) * (1.f + 0.6931472f * hd[C + i]); }
+
+// state [DKP, NV]: warp w holds rows w * DKP / 4 .., as accumulators
+template <int DKP>
+__device__ __forceinline__ void state_to_smem(const float (&s)[DKP / 64][4][4], uint32_t hi, uint32_t lo) {
+  const int lane = xb_lane(), w = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int m = 0; m < DKP / 64; ++m)
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        uint32_t a, b;
+        split2(s[m][n][2 * hh], s[m][n][2 * hh + 1], a, b);
+        const uint32_t off = at2<4>(w * (DKP / 4) + m * 16 + hh * 8 + g, n * 8 + 2 * t);
+        sts32(hi + off, a);
+        sts32(lo + off, b);
+      }
+}
+template <int DKP, bool STORE>
+__device__ __forceinline__ void state_global(float (&s)[DKP / 64][4][4], float* base, long long sk, long long sv, int dk, int cols) {
+  const int lane = xb_lane(), w = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int m = 0; m < DKP / 64; ++m)
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int row = w * (DKP / 4) + m * 16 + (e >> 1) * 8 + g, col = n * 8 + 2 * t + (e & 1);
+        const bool ok = row < dk && col < cols;
+        if (STORE) {
+          if (ok) base[row * sk + col * sv] = s[m][n][e];
+        } else {
+          s[m][n][e] = ok ? base[row * sk + col * sv] : 0.f;
+        }
+      }
+}
+// the two bf16 planes of the state tile to global memory: [plane][DKP][dvp]
+template <int DKP>
+__device__ __forceinline__ void state_save(uint32_t hi, uint32_t lo, bf16* dst, int dvp, int v0) {
+#pragma unroll
+  for (int i = 0; i < DKP * 8 / 128; ++i) {
+    const int idx = i * 128 + threadIdx.x, plane = idx / (DKP * 4), r = (idx / 4) % DKP, u = idx & 3;
+    *reinterpret_cast<uint4*>(dst + ((long long)plane * DKP + r) * dvp + v0 + u * 8) =
+        lds128((plane ? lo : hi) + swz<4>(r, u));
+  }
+}
+
+template <int DKP, bool DELTA, bool SAVE>
+__global__ void __launch_bounds__(128) rec_fwd(const XbRecArgs p) {
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  FwdSmem<DKP, DELTA>& sm = *reinterpret_cast<FwdSmem<DKP, DELTA>*>(smem_raw);
+  constexpr int U = DKP / 8;
+  const int slices = p.dvp / NV, rep = p.Hv / p.Hk;
+  const int sl = blockIdx.x % slices, h = (blockIdx.x / slices) % p.Hv, doc = blockIdx.x / (slices * p.Hv);
+  const int kh = h / rep, v0 = sl * NV, vcols = min(NV, p.dv - v0);
+  const int lane = xb_lane(), w = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int c0 = p.doc_off[doc], c1 = p.doc_off[doc + 1];
+  const int4* chunks = reinterpret_cast<const int4*>(p.chunks);
+  bf16* o = (bf16*)p.o + (long long)h * p.dv + v0;
+  const long long o_t = (long long)p.Hv * p.dv;
+  if (DELTA && doc >= p.n_docs) {                                    // rows outside the documents
+    if (!SAVE)
+      for (int c = c0; c < c1; ++c)
+        for (int i = threadIdx.x; i < chunks[c].y * NV; i += 128)
+          if (i % NV < vcols) o[(chunks[c].x + i / NV) * o_t + i % NV] = __float2bfloat16(0.f);
+    return;
+  }
+  float s[DKP / 64][4][4] = {};
+  const long long soff = ((long long)doc * p.Hv + h) * p.dk * p.dv + v0 * p.s_v;
+  if (p.s_in != nullptr && doc < p.n_docs) state_global<DKP, false>(s, const_cast<float*>(p.s_in) + soff, p.s_k, p.s_v, p.dk, vcols);
+  const uint32_t shi = xb_smem_u32(sm.shi), slo = xb_smem_u32(sm.slo);
+  auto fetch = [&](int c, int b) {
+    const int4 ch = chunks[c];
+    SeqStage<DKP>& st = sm.st[b];
+    load_tile<U, C, 128>(xb_smem_u32(st.k), (const bf16*)p.k + ch.x * p.k_t + kh * p.k_h, p.k_t, ch.y, p.dk);
+    if (!SAVE) load_tile<U, C, 128>(xb_smem_u32(st.q), (const bf16*)p.q + ch.x * p.q_t + kh * p.q_h, p.q_t, ch.y, p.dk);
+    load_tile<4, C, 128>(xb_smem_u32(st.v), (const bf16*)p.v + ch.x * p.v_t + h * p.v_h + v0, p.v_t, ch.y, vcols);
+    load_floats<128>(xb_smem_u32(st.hd), p.hd + ((long long)c * p.Hv + h) * HD, HD);
+    load_floats<128>(xb_smem_u32(st.rqk), p.rqk + ((long long)c * p.Hk + kh) * RQK, RQK);
+  };
+  if (c0 < c1) fetch(c0, 0);
+  cp_commit();
+  state_to_smem<DKP>(s, shi, slo);
+  for (int c = c0; c < c1; ++c) {
+    SeqStage<DKP>& st = sm.st[(c - c0) & 1];
+    const int4 ch = chunks[c];
+    const uint32_t sk = xb_smem_u32(st.k), sq = xb_smem_u32(st.q), sv = xb_smem_u32(st.v);
+    cp_wait<0>();
+    __syncthreads();                       // this chunk's tiles and the state's planes are complete
+    if (c + 1 < c1) fetch(c + 1, (c - c0 + 1) & 1);
+    cp_commit();
+    const long long ch_h = (long long)c * p.Hv + h;
+    if (SAVE) state_save<DKP>(shi, slo, (bf16*)p.s_planes + ch_h * 2 * DKP * p.dvp, p.dvp, v0);
+    const int ra = w * 16 + g;             // this thread's rows: ra and ra + 8
+    float acc_k[4][4] = {}, acc_q[4][4] = {};
+    if (DELTA || !SAVE) {
+#pragma unroll
+      for (int ks = 0; ks < DKP / 16; ++ks) {
+        uint32_t fk[4], fq[4], bh[2][4], bl[2][4];
+        if (DELTA) ldsm4(fk, sk + addr_a<U>(w * 16, ks * 16));
+        if (!SAVE) ldsm4(fq, sq + addr_a<U>(w * 16, ks * 16));
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          ldsm4t(bh[n], shi + addr_bt<4>(ks * 16, n * 16));
+          ldsm4t(bl[n], slo + addr_bt<4>(ks * 16, n * 16));
+        }
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const int a = n >> 1, b = (n & 1) * 2;
+          if (DELTA) {
+            mma(acc_k[n], fk, bl[a][b], bl[a][b + 1]);
+            mma(acc_k[n], fk, bh[a][b], bh[a][b + 1]);
+          }
+          if (!SAVE) {
+            mma(acc_q[n], fq, bl[a][b], bl[a][b + 1]);
+            mma(acc_q[n], fq, bh[a][b], bh[a][b + 1]);
+          }
+        }
+      }
+    }
+    if (DELTA) {
+      // R = b (V - gamma rk K S)
+      const uint32_t xhi = xb_smem_u32(sm.xhi), xlo = xb_smem_u32(sm.xlo);
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        const int row = ra + hh * 8;
+        const float b = st.hd[2 * C + row], f = ex2_sum(st.hd, row) * st.rqk[C + row];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const uint32_t off = at2<4>(row, n * 8 + 2 * t);
+          const float2 v = unpack_bf16x2(lds32(sv + off));
+          uint32_t hi, lo;
+          split2(b * (v.x - f * acc_k[n][2 * hh]), b * (v.y - f * acc_k[n][2 * hh + 1]), hi, lo);
+          sts32(xhi + off, hi);
+          sts32(xlo + off, lo);
+        }
+      }
+      __syncthreads();
+      // U = T R, T lower triangular
+      float u[4][4] = {};
+      const float* tm = p.tm + ch_h * (C * C);
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        if (ks <= w) {
+          uint32_t ah[4], al[4], bh[2][4], bl[2][4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 x = *reinterpret_cast<const float2*>(tm + (ra + (e & 1) * 8) * C + ks * 16 + (e >> 1) * 8 + 2 * t);
+            split2(x.x, x.y, ah[e], al[e]);
+          }
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            ldsm4t(bh[n], xhi + addr_bt<4>(ks * 16, n * 16));
+            ldsm4t(bl[n], xlo + addr_bt<4>(ks * 16, n * 16));
+          }
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const int a = n >> 1, b = (n & 1) * 2;
+            mma(u[n], al, bh[a][b], bh[a][b + 1]);
+            mma(u[n], ah, bl[a][b], bl[a][b + 1]);
+            mma(u[n], ah, bh[a][b], bh[a][b + 1]);
+          }
+        }
+      }
+      const uint32_t uhi = xb_smem_u32(sm.uhi), ulo = xb_smem_u32(sm.ulo);
+      const uint32_t dhi = xb_smem_u32(sm.dhi), dlo = xb_smem_u32(sm.dlo);
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        const int row = ra + hh * 8;
+        const float f = ex2_diff(st.hd, C - 1, row) * st.rqk[C + row];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const uint32_t off = at2<4>(row, n * 8 + 2 * t);
+          uint32_t hi, lo;
+          split2(u[n][2 * hh], u[n][2 * hh + 1], hi, lo);
+          if (SAVE) {
+            uint32_t* pl = reinterpret_cast<uint32_t*>((bf16*)p.u_planes + (ch_h * 2 * C + row) * p.dvp + v0 + n * 8 + 2 * t);
+            pl[0] = hi;
+            pl[C * p.dvp / 2] = lo;
+          } else {
+            sts32(uhi + off, hi);
+            sts32(ulo + off, lo);
+          }
+          split2(f * u[n][2 * hh], f * u[n][2 * hh + 1], hi, lo);
+          sts32(dhi + off, hi);
+          sts32(dlo + off, lo);
+        }
+      }
+    } else {
+      // b d V, two neighbouring values per thread
+      const uint32_t dhi = xb_smem_u32(sm.dhi), dlo = xb_smem_u32(sm.dlo);
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        const int row = ra + hh * 8;
+        const float f = ex2_diff(st.hd, C - 1, row) * st.hd[2 * C + row];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const uint32_t off = at2<4>(row, n * 8 + 2 * t);
+          const float2 v = unpack_bf16x2(lds32(sv + off));
+          uint32_t hi, lo;
+          split2(f * v.x, f * v.y, hi, lo);
+          sts32(dhi + off, hi);
+          sts32(dlo + off, lo);
+        }
+      }
+    }
+    __syncthreads();
+    if (!SAVE) {
+      // O = gamma rq Q S + P U
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        const float f = ex2_sum(st.hd, ra + hh * 8) * st.rqk[ra + hh * 8];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) acc_q[n][2 * hh] *= f, acc_q[n][2 * hh + 1] *= f;
+      }
+      const float* qk = p.qk + ((long long)c * p.Hk + kh) * (C * C);
+      const uint32_t uhi = DELTA ? xb_smem_u32(sm.uhi) : sv, ulo = xb_smem_u32(sm.ulo);
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        if (ks <= w) {
+          uint32_t ah[4], al[4], bh[2][4], bl[2][4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int row = ra + (e & 1) * 8, col = ks * 16 + (e >> 1) * 8 + 2 * t;
+            const float2 x = *reinterpret_cast<const float2*>(qk + row * C + col);
+            float y0 = col <= row ? x.x * ex2_diff(st.hd, row, col) : 0.f;
+            float y1 = col + 1 <= row ? x.y * ex2_diff(st.hd, row, col + 1) : 0.f;
+            if (!DELTA) y0 *= st.hd[2 * C + col], y1 *= st.hd[2 * C + col + 1];
+            split2(y0, y1, ah[e], al[e]);
+          }
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            ldsm4t(bh[n], uhi + addr_bt<4>(ks * 16, n * 16));
+            if (DELTA) ldsm4t(bl[n], ulo + addr_bt<4>(ks * 16, n * 16));
+          }
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const int a = n >> 1, b = (n & 1) * 2;
+            mma(acc_q[n], al, bh[a][b], bh[a][b + 1]);
+            if (DELTA) mma(acc_q[n], ah, bl[a][b], bl[a][b + 1]);
+            mma(acc_q[n], ah, bh[a][b], bh[a][b + 1]);
+          }
+        }
+      }
+      const float skip = DELTA ? 0.f : p.D[h];
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        const int row = ra + hh * 8;
+        if (row < ch.y) {
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const int col = n * 8 + 2 * t;
+            if (col < vcols) {
+              float y0 = acc_q[n][2 * hh], y1 = acc_q[n][2 * hh + 1];
+              if (!DELTA) {
+                const float2 v = unpack_bf16x2(lds32(sv + at2<4>(row, col)));
+                y0 += skip * v.x, y1 += skip * v.y;
+              }
+              *reinterpret_cast<uint32_t*>(o + (ch.x + row) * o_t + col) = pack_bf16x2(y0, y1);
+            }
+          }
+        }
+      }
+    }
+    {  // S = gamma_last S + K^T (d U)
+      const uint32_t dhi = xb_smem_u32(sm.dhi), dlo = xb_smem_u32(sm.dlo);
+      const float f = ex2_sum(st.hd, C - 1);
+#pragma unroll
+      for (int m = 0; m < DKP / 64; ++m)
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[m][n][e] *= f;
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        uint32_t bh[2][4], bl[2][4];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          ldsm4t(bh[n], dhi + addr_bt<4>(ks * 16, n * 16));
+          ldsm4t(bl[n], dlo + addr_bt<4>(ks * 16, n * 16));
+        }
+#pragma unroll
+        for (int m = 0; m < DKP / 64; ++m) {
+          uint32_t fa[4];
+          ldsm4t(fa, sk + addr_at<U>(w * (DKP / 4) + m * 16, ks * 16));
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const int a = n >> 1, b = (n & 1) * 2;
+            mma(s[m][n], fa, bl[a][b], bl[a][b + 1]);
+            mma(s[m][n], fa, bh[a][b], bh[a][b + 1]);
+          }
+        }
+      }
+      state_to_smem<DKP>(s, shi, slo);     // the old planes were last read before the barrier above
+    }
+  }
+  cp_wait<0>();
+  if (p.s_out != nullptr && doc < p.n_docs) state_global<DKP, true>(s, p.s_out + soff, p.s_k, p.s_v, p.dk, vcols);
+}
+
+// ---- backward, sequential part: the state's gradient through one document, last chunk first -----------------------
+template <int DKP>
+struct BwdStage {
+  uint8_t q[C * DKP * 2], k[C * DKP * 2], dy[C * NV * 2];
+  float hd[HD], rqk[RQK];
+};
+template <int DKP, bool DELTA>
+struct BwdSmem {
+  BwdStage<DKP> st[2];
+  uint8_t shi[DKP * NV * 2], slo[DKP * NV * 2];                         // dS'
+  uint8_t uhi[DELTA ? C * NV * 2 : 16], ulo[DELTA ? C * NV * 2 : 16];   // dU
+  uint8_t xhi[DELTA ? C * NV * 2 : 16], xlo[DELTA ? C * NV * 2 : 16];   // -b gamma rk dR
+  uint8_t yhi[C * NV * 2], ylo[C * NV * 2];                             // gamma rq dO
+};
+
+template <int DKP, bool DELTA>
+__global__ void __launch_bounds__(128) rec_bwd(const XbRecArgs p) {
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  BwdSmem<DKP, DELTA>& sm = *reinterpret_cast<BwdSmem<DKP, DELTA>*>(smem_raw);
+  constexpr int U = DKP / 8;
+  const int slices = p.dvp / NV, rep = p.Hv / p.Hk;
+  const int sl = blockIdx.x % slices, h = (blockIdx.x / slices) % p.Hv, doc = blockIdx.x / (slices * p.Hv);
+  const int kh = h / rep, v0 = sl * NV, vcols = min(NV, p.dv - v0);
+  const int lane = xb_lane(), w = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int c0 = p.doc_off[doc], c1 = p.doc_off[doc + 1];
+  const int4* chunks = reinterpret_cast<const int4*>(p.chunks);
+  bf16* dv = (bf16*)p.dv_out + (long long)h * p.dv + v0;
+  const long long dv_t = (long long)p.Hv * p.dv;
+  if (DELTA && doc >= p.n_docs) {
+    for (int c = c0; c < c1; ++c)
+      for (int i = threadIdx.x; i < chunks[c].y * NV; i += 128)
+        if (i % NV < vcols) dv[(chunks[c].x + i / NV) * dv_t + i % NV] = __float2bfloat16(0.f);
+    return;
+  }
+  float s[DKP / 64][4][4] = {};
+  const long long soff = ((long long)doc * p.Hv + h) * p.dk * p.dv + v0 * p.s_v;
+  if (p.ds_out != nullptr && doc < p.n_docs) state_global<DKP, false>(s, const_cast<float*>(p.ds_out) + soff, p.s_k, p.s_v, p.dk, vcols);
+  const uint32_t shi = xb_smem_u32(sm.shi), slo = xb_smem_u32(sm.slo);
+  auto fetch = [&](int c, int b) {
+    const int4 ch = chunks[c];
+    BwdStage<DKP>& st = sm.st[b];
+    load_tile<U, C, 128>(xb_smem_u32(st.k), (const bf16*)p.k + ch.x * p.k_t + kh * p.k_h, p.k_t, ch.y, p.dk);
+    load_tile<U, C, 128>(xb_smem_u32(st.q), (const bf16*)p.q + ch.x * p.q_t + kh * p.q_h, p.q_t, ch.y, p.dk);
+    load_tile<4, C, 128>(xb_smem_u32(st.dy), (const bf16*)p.dy + ch.x * p.dy_t + h * p.dy_h + v0, p.dy_t, ch.y, vcols);
+    load_floats<128>(xb_smem_u32(st.hd), p.hd + ((long long)c * p.Hv + h) * HD, HD);
+    load_floats<128>(xb_smem_u32(st.rqk), p.rqk + ((long long)c * p.Hk + kh) * RQK, RQK);
+  };
+  if (c0 < c1) fetch(c1 - 1, 0);
+  cp_commit();
+  state_to_smem<DKP>(s, shi, slo);
+  for (int c = c1 - 1; c >= c0; --c) {
+    BwdStage<DKP>& st = sm.st[(c1 - 1 - c) & 1];
+    const int4 ch = chunks[c];
+    const uint32_t sk = xb_smem_u32(st.k), sq = xb_smem_u32(st.q), sy = xb_smem_u32(st.dy);
+    const uint32_t yhi = xb_smem_u32(sm.yhi), ylo = xb_smem_u32(sm.ylo);
+    cp_wait<0>();
+    __syncthreads();
+    if (c > c0) fetch(c - 1, (c1 - c) & 1);
+    cp_commit();
+    const long long ch_h = (long long)c * p.Hv + h;
+    state_save<DKP>(shi, slo, (bf16*)p.ds_planes + ch_h * 2 * DKP * p.dvp, p.dvp, v0);
+    const int ra = w * 16 + g;
+    // K dS'
+    float du[4][4] = {};
+#pragma unroll
+    for (int ks = 0; ks < DKP / 16; ++ks) {
+      uint32_t fk[4], bh[2][4], bl[2][4];
+      ldsm4(fk, sk + addr_a<U>(w * 16, ks * 16));
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        ldsm4t(bh[n], shi + addr_bt<4>(ks * 16, n * 16));
+        ldsm4t(bl[n], slo + addr_bt<4>(ks * 16, n * 16));
+      }
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const int a = n >> 1, b = (n & 1) * 2;
+        mma(du[n], fk, bl[a][b], bl[a][b + 1]);
+        mma(du[n], fk, bh[a][b], bh[a][b + 1]);
+      }
+    }
+    // dU = d rk K dS' + P^T dO; beside it gamma rq dO for the state
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      const int row = ra + hh * 8;
+      const float f = ex2_diff(st.hd, C - 1, row) * st.rqk[C + row], y = ex2_sum(st.hd, row) * st.rqk[row];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        du[n][2 * hh] *= f, du[n][2 * hh + 1] *= f;
+        const uint32_t off = at2<4>(row, n * 8 + 2 * t);
+        const float2 v = unpack_bf16x2(lds32(sy + off));
+        uint32_t hi, lo;
+        split2(y * v.x, y * v.y, hi, lo);
+        sts32(yhi + off, hi);
+        sts32(ylo + off, lo);
+      }
+    }
+    const float* qk = p.qk + ((long long)c * p.Hk + kh) * (C * C);
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      if (ks >= w) {
+        uint32_t ah[4], al[4], bh[2][4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = ra + (e & 1) * 8, i = ks * 16 + (e >> 1) * 8 + 2 * t;     // element (j, i) of P^T
+          const float y0 = i >= j ? qk[i * C + j] * ex2_diff(st.hd, i, j) : 0.f;
+          const float y1 = i + 1 >= j ? qk[(i + 1) * C + j] * ex2_diff(st.hd, i + 1, j) : 0.f;
+          split2(y0, y1, ah[e], al[e]);
+        }
+#pragma unroll
+        for (int n = 0; n < 2; ++n) ldsm4t(bh[n], sy + addr_bt<4>(ks * 16, n * 16));
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const int a = n >> 1, b = (n & 1) * 2;
+          mma(du[n], al, bh[a][b], bh[a][b + 1]);
+          mma(du[n], ah, bh[a][b], bh[a][b + 1]);
+        }
+      }
+    }
+    if (DELTA) {
+      const uint32_t uhi = xb_smem_u32(sm.uhi), ulo = xb_smem_u32(sm.ulo), xhi = xb_smem_u32(sm.xhi), xlo = xb_smem_u32(sm.xlo);
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const uint32_t off = at2<4>(ra + hh * 8, n * 8 + 2 * t);
+          uint32_t hi, lo;
+          split2(du[n][2 * hh], du[n][2 * hh + 1], hi, lo);
+          sts32(uhi + off, hi);
+          sts32(ulo + off, lo);
+        }
+      __syncthreads();
+      // dR = T^T dU
+      float dr[4][4] = {};
+      const float* tm = p.tm + ch_h * (C * C);
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        if (ks >= w) {
+          uint32_t ah[4], al[4], bh[2][4], bl[2][4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int j = ra + (e & 1) * 8, i = ks * 16 + (e >> 1) * 8 + 2 * t;
+            split2(tm[i * C + j], tm[(i + 1) * C + j], ah[e], al[e]);
+          }
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            ldsm4t(bh[n], uhi + addr_bt<4>(ks * 16, n * 16));
+            ldsm4t(bl[n], ulo + addr_bt<4>(ks * 16, n * 16));
+          }
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const int a = n >> 1, b = (n & 1) * 2;
+            mma(dr[n], al, bh[a][b], bh[a][b + 1]);
+            mma(dr[n], ah, bl[a][b], bl[a][b + 1]);
+            mma(dr[n], ah, bh[a][b], bh[a][b + 1]);
+          }
+        }
+      }
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        const int row = ra + hh * 8;
+        const float b = st.hd[2 * C + row], f = -b * ex2_sum(st.hd, row) * st.rqk[C + row];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const int col = n * 8 + 2 * t;
+          const uint32_t off = at2<4>(row, col);
+          const float y0 = dr[n][2 * hh], y1 = dr[n][2 * hh + 1];
+          uint32_t hi, lo;
+          split2(y0, y1, hi, lo);
+          uint32_t* pl = reinterpret_cast<uint32_t*>((bf16*)p.dr_planes + (ch_h * 2 * C + row) * p.dvp + v0 + col);
+          pl[0] = hi;
+          pl[C * p.dvp / 2] = lo;
+          split2(f * y0, f * y1, hi, lo);
+          sts32(xhi + off, hi);
+          sts32(xlo + off, lo);
+          if (row < ch.y && col < vcols)
+            *reinterpret_cast<uint32_t*>(dv + (ch.x + row) * dv_t + col) = pack_bf16x2(b * y0, b * y1);
+        }
+      }
+    } else {
+      const float skip = p.D[h];
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        const int row = ra + hh * 8;
+        const float b = st.hd[2 * C + row];
+        if (row < ch.y) {
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const int col = n * 8 + 2 * t;
+            if (col < vcols) {
+              const float2 y = unpack_bf16x2(lds32(sy + at2<4>(row, col)));
+              *reinterpret_cast<uint32_t*>(dv + (ch.x + row) * dv_t + col) =
+                  pack_bf16x2(b * du[n][2 * hh] + skip * y.x, b * du[n][2 * hh + 1] + skip * y.y);
+            }
+          }
+        }
+      }
+    }
+    __syncthreads();
+    {  // dS = gamma_last dS' + Q^T (gamma rq dO) + K^T (-b gamma rk dR)
+      const float f = ex2_sum(st.hd, C - 1);
+#pragma unroll
+      for (int m = 0; m < DKP / 64; ++m)
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[m][n][e] *= f;
+#pragma unroll
+      for (int part = 0; part < (DELTA ? 2 : 1); ++part) {
+        const uint32_t base = part ? sk : sq, bhi = part ? xb_smem_u32(sm.xhi) : yhi, blo = part ? xb_smem_u32(sm.xlo) : ylo;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+          uint32_t bh[2][4], bl[2][4];
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            ldsm4t(bh[n], bhi + addr_bt<4>(ks * 16, n * 16));
+            ldsm4t(bl[n], blo + addr_bt<4>(ks * 16, n * 16));
+          }
+#pragma unroll
+          for (int m = 0; m < DKP / 64; ++m) {
+            uint32_t fa[4];
+            ldsm4t(fa, base + addr_at<U>(w * (DKP / 4) + m * 16, ks * 16));
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              const int a = n >> 1, b = (n & 1) * 2;
+              mma(s[m][n], fa, bl[a][b], bl[a][b + 1]);
+              mma(s[m][n], fa, bh[a][b], bh[a][b + 1]);
+            }
+          }
+        }
+      }
+      state_to_smem<DKP>(s, shi, slo);
+    }
+  }
+  cp_wait<0>();
+  if (p.ds_in != nullptr && doc < p.n_docs) state_global<DKP, true>(s, p.ds_in + soff, p.s_k, p.s_v, p.dk, vcols);
+}
+
+// ---- backward, parallel part: gradients of q, k, the decay and b of one chunk ---------------------------------------
+constexpr int GV = 64;        // state columns of one pass
+template <int DKP, bool DELTA>
+struct GradSmem {
+  uint8_t q[C * DKP * 2], k[C * DKP * 2];
+  uint8_t dy[C * GV * 2], v[C * GV * 2];
+  uint8_t u[DELTA ? 2 : 1][DELTA ? C * GV * 2 : 16], r[DELTA ? 2 : 1][DELTA ? C * GV * 2 : 16];
+  uint8_t s[2][DKP * GV * 2], ds[2][DKP * GV * 2];
+  uint8_t z[2][C * C * 2], w[DELTA ? 2 : 1][DELTA ? C * C * 2 : 16];
+  float hd[HD], rqk[RQK];
+  float rd[3][2][C];          // row sums of q.t1, k.t2, k.t3 by column half
+  float er[2][C], ec[4][C];   // row and column sums of dP o P (scan: without b)
+  float fr[2][C], fc[4][C];   // the same of dL o A
+  float rv[C], sdot[8];
+  float dot[2][2][C];         // q.dq and k.dk of the finished rows
+};
+
+template <int DKP, bool DELTA>
+__global__ void __launch_bounds__(256) rec_grad(const XbRecArgs p) {
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  GradSmem<DKP, DELTA>& sm = *reinterpret_cast<GradSmem<DKP, DELTA>*>(smem_raw);
+  constexpr int U = DKP / 8, NT = DKP / 16;
+  const int kh = blockIdx.x % p.Hk, c = blockIdx.x / p.Hk, rep = p.Hv / p.Hk;
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int rb = w & 3, cb = w >> 2, ra = rb * 16 + g, n0 = cb * (DKP / 2);
+  if (c >= p.doc_off[p.n_docs + 2]) return;
+  const int4 ch = reinterpret_cast<const int4*>(p.chunks)[c];
+  const int len = ch.y;
+  bf16* dq = (bf16*)p.dq + (ch.x * (long long)p.Hk + kh) * p.dk;
+  bf16* dk = (bf16*)p.dk_out + (ch.x * (long long)p.Hk + kh) * p.dk;
+  const long long d_t = (long long)p.Hk * p.dk;
+  if (DELTA && ch.z >= p.n_docs) {                                   // rows outside the documents
+    for (int i = tid; i < len * p.dk; i += 256) {
+      dq[(i / p.dk) * d_t + i % p.dk] = __float2bfloat16(0.f);
+      dk[(i / p.dk) * d_t + i % p.dk] = __float2bfloat16(0.f);
+    }
+    for (int i = tid; i < len * rep; i += 256) {
+      const long long at = (long long)(ch.x + i / rep) * p.Hv + kh * rep + i % rep;
+      p.dg[at] = 0.f, p.db[at] = 0.f;
+    }
+    return;
+  }
+  const uint32_t sq = xb_smem_u32(sm.q), sk = xb_smem_u32(sm.k), sy = xb_smem_u32(sm.dy), sv = xb_smem_u32(sm.v);
+  load_tile<U, C, 256>(sq, (const bf16*)p.q + ch.x * p.q_t + kh * p.q_h, p.q_t, len, p.dk);
+  load_tile<U, C, 256>(sk, (const bf16*)p.k + ch.x * p.k_t + kh * p.k_h, p.k_t, len, p.dk);
+  load_floats<256>(xb_smem_u32(sm.rqk), p.rqk + ((long long)c * p.Hk + kh) * RQK, RQK);
+  float aq[NT][4] = {}, ak[NT][4] = {};                              // rq dq, rk dk over the heads of the group
+  for (int hh = 0; hh < rep; ++hh) {
+    const int h = kh * rep + hh;
+    const long long ch_h = (long long)c * p.Hv + h;
+    float dp[4][4] = {}, dl[4][4] = {}, rd1[2] = {}, rd2[2] = {}, rd3[2] = {};
+    float sdot = 0.f, rv = 0.f;
+    for (int v0 = 0; v0 < p.dv; v0 += GV) {
+      __syncthreads();                                               // the tiles of the pass before have been read
+      const int vcols = min(GV, p.dv - v0), pcols = min(GV, p.dvp - v0);
+      load_tile<8, C, 256>(sy, (const bf16*)p.dy + ch.x * p.dy_t + h * p.dy_h + v0, p.dy_t, len, vcols);
+      load_tile<8, C, 256>(sv, (const bf16*)p.v + ch.x * p.v_t + h * p.v_h + v0, p.v_t, len, vcols);
+#pragma unroll
+      for (int pl = 0; pl < 2; ++pl) {
+        if (DELTA) {
+          load_tile<8, C, 256>(xb_smem_u32(sm.u[pl]), (const bf16*)p.u_planes + (ch_h * 2 + pl) * C * p.dvp + v0, p.dvp, C, pcols);
+          load_tile<8, C, 256>(xb_smem_u32(sm.r[pl]), (const bf16*)p.dr_planes + (ch_h * 2 + pl) * C * p.dvp + v0, p.dvp, C, pcols);
+        }
+        load_tile<8, DKP, 256>(xb_smem_u32(sm.s[pl]), (const bf16*)p.s_planes + (ch_h * 2 + pl) * DKP * p.dvp + v0, p.dvp, DKP, pcols);
+        load_tile<8, DKP, 256>(xb_smem_u32(sm.ds[pl]), (const bf16*)p.ds_planes + (ch_h * 2 + pl) * DKP * p.dvp + v0, p.dvp, DKP, pcols);
+      }
+      if (v0 == 0) load_floats<256>(xb_smem_u32(sm.hd), p.hd + ch_h * HD, HD);
+      cp_commit();
+      cp_wait<0>();
+      __syncthreads();
+      // dP = dO U^T (scan: dO V^T), -dL = dR U^T, this warp's 16 x 32 part
+      const uint32_t ub[2] = {DELTA ? xb_smem_u32(sm.u[0]) : sv, xb_smem_u32(sm.u[1 % (DELTA ? 2 : 1)])};
+      const uint32_t rr[2] = {xb_smem_u32(sm.r[0]), xb_smem_u32(sm.r[1 % (DELTA ? 2 : 1)])};
+      if (cb * 32 <= rb * 16 + 15) {
+#pragma unroll
+        for (int ks = 0; ks < GV / 16; ++ks) {
+          uint32_t fy[4], fr[2][4];
+          ldsm4(fy, sy + addr_a<8>(rb * 16, ks * 16));
+          if (DELTA) {
+            ldsm4(fr[0], rr[0] + addr_a<8>(rb * 16, ks * 16));
+            ldsm4(fr[1], rr[1] + addr_a<8>(rb * 16, ks * 16));
+          }
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            uint32_t bh[4], bl[4];
+            ldsm4(bh, ub[0] + addr_b<8>(cb * 32 + n * 16, ks * 16));
+            if (DELTA) ldsm4(bl, ub[1] + addr_b<8>(cb * 32 + n * 16, ks * 16));
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float(&d)[4] = dp[2 * n + e];
+              if (DELTA) {
+                mma(d, fy, bl[2 * e], bl[2 * e + 1]);
+                mma(dl[2 * n + e], fr[1], bh[2 * e], bh[2 * e + 1]);
+                mma(dl[2 * n + e], fr[0], bl[2 * e], bl[2 * e + 1]);
+                mma(dl[2 * n + e], fr[0], bh[2 * e], bh[2 * e + 1]);
+              }
+              mma(d, fy, bh[2 * e], bh[2 * e + 1]);
+            }
+          }
+        }
+      }
+      // t1 = dO S^T, t2 = dR S^T, t3 = U dS'^T (scan: V dS'^T), one after the other in the same registers
+#pragma unroll
+      for (int which = 0; which < 3; ++which) {
+        if (!DELTA && which == 1) continue;
+        const uint32_t a0 = which == 0 ? sy : which == 1 ? rr[0] : ub[0], a1 = which == 1 ? rr[1] : ub[1];
+        const bool two = DELTA && which > 0;
+        const uint32_t b0 = xb_smem_u32(which == 2 ? sm.ds[0] : sm.s[0]), b1 = xb_smem_u32(which == 2 ? sm.ds[1] : sm.s[1]);
+        float x[NT][4] = {};
+#pragma unroll
+        for (int ks = 0; ks < GV / 16; ++ks) {
+          uint32_t fa[4], fl[4];
+          ldsm4(fa, a0 + addr_a<8>(rb * 16, ks * 16));
+          if (two) ldsm4(fl, a1 + addr_a<8>(rb * 16, ks * 16));
+#pragma unroll
+          for (int n = 0; n < NT; n += 2) {
+            uint32_t bh[4], bl[4];
+            ldsm4(bh, b0 + addr_b<8>(n0 + n * 8, ks * 16));
+            ldsm4(bl, b1 + addr_b<8>(n0 + n * 8, ks * 16));
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              if (two) mma(x[n + e], fl, bh[2 * e], bh[2 * e + 1]);
+              mma(x[n + e], fa, bl[2 * e], bl[2 * e + 1]);
+              mma(x[n + e], fa, bh[2 * e], bh[2 * e + 1]);
+            }
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int row = ra + r * 8;
+          const float b = sm.hd[2 * C + row];
+          float f;
+          if (which == 0) f = ex2_sum(sm.hd, row) * sm.rqk[row];
+          else if (which == 1) f = -b * ex2_sum(sm.hd, row) * sm.rqk[C + row];
+          else f = ex2_diff(sm.hd, C - 1, row) * sm.rqk[C + row] * (DELTA ? 1.f : b);
+          float sum = 0.f;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const float2 y = unpack_bf16x2(lds32((which == 0 ? sq : sk) + at2<U>(row, n0 + n * 8 + 2 * t)));
+            sum += y.x * x[n][2 * r] + y.y * x[n][2 * r + 1];
+            float(&d)[4] = which == 0 ? aq[n] : ak[n];
+            d[2 * r] += f * x[n][2 * r], d[2 * r + 1] += f * x[n][2 * r + 1];
+          }
+          (which == 0 ? rd1 : which == 1 ? rd2 : rd3)[r] += sum;
+        }
+      }
+      // <S, dS'> and the rows' dR.v (scan: dO.v)
+#pragma unroll
+      for (int i = 0; i < DKP * 8 / 256; ++i) {
+        const int idx = i * 256 + tid, r = idx >> 3, u = idx & 7;
+        const uint32_t off = swz<8>(r, u);
+        const uint4 a = lds128(xb_smem_u32(sm.s[0]) + off), al = lds128(xb_smem_u32(sm.s[1]) + off);
+        const uint4 b = lds128(xb_smem_u32(sm.ds[0]) + off), bl = lds128(xb_smem_u32(sm.ds[1]) + off);
+        const uint32_t xa[4] = {a.x, a.y, a.z, a.w}, xl[4] = {al.x, al.y, al.z, al.w};
+        const uint32_t ya[4] = {b.x, b.y, b.z, b.w}, yl[4] = {bl.x, bl.y, bl.z, bl.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 m = join2(xa[e], xl[e]), n = join2(ya[e], yl[e]);
+          sdot += m.x * n.x + m.y * n.y;
+        }
+      }
+      {
+        const int row = tid >> 2;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const uint32_t off = swz<8>(row, (tid & 3) * 2 + u);
+          const uint4 a = DELTA ? lds128(rr[0] + off) : lds128(sy + off), al = DELTA ? lds128(rr[1] + off) : a, b = lds128(sv + off);
+          const uint32_t xa[4] = {a.x, a.y, a.z, a.w}, xl[4] = {al.x, al.y, al.z, al.w}, ya[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 m = DELTA ? join2(xa[e], xl[e]) : unpack_bf16x2(xa[e]), n = unpack_bf16x2(ya[e]);
+            rv += m.x * n.x + m.y * n.y;
+          }
+        }
+      }
+    }
+    // Z = D o dP and W = D o dL with the row factors of both sides, and the sums of their products with P and A
+    {
+      const float* qk = p.qk + ((long long)c * p.Hk + kh) * (C * C);
+      const float* kk = DELTA ? p.kk + ((long long)c * p.Hk + kh) * (C * C) : nullptr;
+      float er[2] = {}, fr[2] = {};
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const int col = cb * 32 + n * 8 + 2 * t;
+        float ec[2] = {}, fc[2] = {};
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int row = ra + r * 8;
+          float z[2] = {}, y[2] = {};
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int j = col + e;
+            if (j <= row) {
+              const float d = ex2_diff(sm.hd, row, j), b = sm.hd[2 * C + (DELTA ? row : j)], m = d * dp[n][2 * r + e];
+              const float v = m * qk[row * C + j];
+              er[r] += DELTA ? v : b * v;
+              ec[e] += v;
+              z[e] = m * sm.rqk[row] * sm.rqk[C + j] * (DELTA ? 1.f : b);
+              if (DELTA && j < row) {
+                const float l = -d * dl[n][2 * r + e], q = l * kk[row * C + j];
+                fr[r] += q;
+                fc[e] += b * q;
+                y[e] = b * l * sm.rqk[C + row] * sm.rqk[C + j];
+              }
+            }
+          }
+          const uint32_t off = at2<8>(row, col);
+          uint32_t hi, lo;
+          split2(z[0], z[1], hi, lo);
+          sts32(xb_smem_u32(sm.z[0]) + off, hi);
+          sts32(xb_smem_u32(sm.z[1]) + off, lo);
+          if (DELTA) {
+            split2(y[0], y[1], hi, lo);
+            sts32(xb_smem_u32(sm.w[0]) + off, hi);
+            sts32(xb_smem_u32(sm.w[DELTA ? 1 : 0]) + off, lo);
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) {
+            ec[e] += __shfl_xor_sync(0xffffffffu, ec[e], o);
+            if (DELTA) fc[e] += __shfl_xor_sync(0xffffffffu, fc[e], o);
+          }
+          if (g == 0) {
+            sm.ec[rb][col + e] = ec[e];
+            if (DELTA) sm.fc[rb][col + e] = fc[e];
+          }
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+          er[r] += __shfl_xor_sync(0xffffffffu, er[r], o);
+          fr[r] += __shfl_xor_sync(0xffffffffu, fr[r], o);
+          rd1[r] += __shfl_xor_sync(0xffffffffu, rd1[r], o);
+          rd2[r] += __shfl_xor_sync(0xffffffffu, rd2[r], o);
+          rd3[r] += __shfl_xor_sync(0xffffffffu, rd3[r], o);
+        }
+        if (t == 0) {
+          const int row = ra + r * 8;
+          sm.er[cb][row] = er[r], sm.fr[cb][row] = fr[r];
+          sm.rd[0][cb][row] = rd1[r], sm.rd[1][cb][row] = rd2[r], sm.rd[2][cb][row] = rd3[r];
+        }
+      }
+      sdot = warp_sum(sdot);
+      if (lane == 0) sm.sdot[w] = sdot;
+      rv += __shfl_xor_sync(0xffffffffu, rv, 1);
+      rv += __shfl_xor_sync(0xffffffffu, rv, 2);
+      if ((tid & 3) == 0) sm.rv[tid >> 2] = rv;
+    }
+    __syncthreads();
+    // dq += Z K, dk += Z^T Q + W K + W^T K
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      const bool row_role = ks <= rb, col_role = ks >= rb;
+      uint32_t zh[4], zl[4], wh[4], wl[4], th[4], tl[4], vh[4], vl[4];
+      if (row_role) {
+        ldsm4(zh, xb_smem_u32(sm.z[0]) + addr_a<8>(rb * 16, ks * 16));
+        ldsm4(zl, xb_smem_u32(sm.z[1]) + addr_a<8>(rb * 16, ks * 16));
+        if (DELTA) {
+          ldsm4(wh, xb_smem_u32(sm.w[0]) + addr_a<8>(rb * 16, ks * 16));
+          ldsm4(wl, xb_smem_u32(sm.w[DELTA ? 1 : 0]) + addr_a<8>(rb * 16, ks * 16));
+        }
+      }
+      if (col_role) {
+        ldsm4t(th, xb_smem_u32(sm.z[0]) + addr_at<8>(rb * 16, ks * 16));
+        ldsm4t(tl, xb_smem_u32(sm.z[1]) + addr_at<8>(rb * 16, ks * 16));
+        if (DELTA) {
+          ldsm4t(vh, xb_smem_u32(sm.w[0]) + addr_at<8>(rb * 16, ks * 16));
+          ldsm4t(vl, xb_smem_u32(sm.w[DELTA ? 1 : 0]) + addr_at<8>(rb * 16, ks * 16));
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; n += 2) {
+        uint32_t bk[4], bq[4];
+        ldsm4t(bk, sk + addr_bt<U>(ks * 16, n0 + n * 8));
+        if (col_role) ldsm4t(bq, sq + addr_bt<U>(ks * 16, n0 + n * 8));
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          if (row_role) {
+            mma(aq[n + e], zl, bk[2 * e], bk[2 * e + 1]);
+            mma(aq[n + e], zh, bk[2 * e], bk[2 * e + 1]);
+            if (DELTA) {
+              mma(ak[n + e], wl, bk[2 * e], bk[2 * e + 1]);
+              mma(ak[n + e], wh, bk[2 * e], bk[2 * e + 1]);
+            }
+          }
+          if (col_role) {
+            mma(ak[n + e], tl, bq[2 * e], bq[2 * e + 1]);
+            mma(ak[n + e], th, bq[2 * e], bq[2 * e + 1]);
+            if (DELTA) {
+              mma(ak[n + e], vl, bk[2 * e], bk[2 * e + 1]);
+              mma(ak[n + e], vh, bk[2 * e], bk[2 * e + 1]);
+            }
+          }
+        }
+      }
+    }
+    // gradients of the log decay (suffix sums of dG) and of b, two rows per lane of one warp
+    if (w == 0) {
+      double x[2], last = 0.0, dsum = 0.0;
+      float db[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = 2 * lane + i;
+        const float b = sm.hd[2 * C + row], gam = ex2_sum(sm.hd, row), d = ex2_diff(sm.hd, C - 1, row);
+        const float rq = sm.rqk[row], rk = sm.rqk[C + row];
+        const float q1 = gam * rq * (sm.rd[0][0][row] + sm.rd[0][1][row]);
+        const float k2 = gam * rk * (sm.rd[1][0][row] + sm.rd[1][1][row]);
+        const float k3 = d * rk * (sm.rd[2][0][row] + sm.rd[2][1][row]);
+        const float e1 = sm.er[0][row] + sm.er[1][row];
+        const float e2 = (sm.ec[0][row] + sm.ec[1][row]) + (sm.ec[2][row] + sm.ec[3][row]);
+        if (DELTA) {
+          const float f1 = sm.fr[0][row] + sm.fr[1][row];
+          const float f2 = (sm.fc[0][row] + sm.fc[1][row]) + (sm.fc[2][row] + sm.fc[3][row]);
+          x[i] = (double)q1 + (double)e1 - (double)e2 + (double)(b * f1) - (double)f2 - (double)(b * k2) - (double)k3;
+          last += k3;
+          db[i] = sm.rv[row] - k2 + f1;
+        } else {
+          x[i] = (double)q1 + (double)e1 - (double)(b * e2) - (double)(b * k3);
+          last += (double)(b * k3);
+          db[i] = e2 + k3;
+          dsum += sm.rv[row];
+        }
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        last += __shfl_xor_sync(0xffffffffu, last, o);
+        dsum += __shfl_xor_sync(0xffffffffu, dsum, o);
+      }
+      float sd = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sd += sm.sdot[i];
+      last += (double)(ex2_sum(sm.hd, C - 1) * sd);
+      double s = x[0] + x[1];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double y = __shfl_down_sync(0xffffffffu, s, o);
+        if (lane + o < 32) s += y;
+      }
+      double da = 0.0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = 2 * lane + i;
+        const float dg = (float)((i ? x[1] + (s - x[0] - x[1]) : s) + last);
+        if (row < len) {
+          const long long at = (long long)(ch.x + row) * p.Hv + h;
+          if (DELTA) {
+            p.dg[at] = dg, p.db[at] = db[i];
+          } else {
+            p.db[at] = db[i] + dg * p.A[h];
+            da += (double)(dg * sm.hd[2 * C + row]);
+          }
+        }
+      }
+      if (!DELTA) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) da += __shfl_xor_sync(0xffffffffu, da, o);
+        if (lane == 0) p.part[ch_h * 2] = (float)da, p.part[ch_h * 2 + 1] = (float)dsum;
+      }
+    }
+  }
+  // gradient through the L2 norms: dq - q^ (q^ . dq), rows of norm below 1e-12 excepted
+  if (p.l2norm) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int row = ra + r * 8;
+      float a = 0.f, b = 0.f;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const uint32_t off = at2<U>(row, n0 + n * 8 + 2 * t);
+        const float2 q = unpack_bf16x2(lds32(sq + off)), k = unpack_bf16x2(lds32(sk + off));
+        a += q.x * aq[n][2 * r] + q.y * aq[n][2 * r + 1];
+        b += k.x * ak[n][2 * r] + k.y * ak[n][2 * r + 1];
+      }
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) {
+        a += __shfl_xor_sync(0xffffffffu, a, o);
+        b += __shfl_xor_sync(0xffffffffu, b, o);
+      }
+      if (t == 0) sm.dot[0][cb][row] = a, sm.dot[1][cb][row] = b;
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int row = ra + r * 8;
+    if (row >= len) continue;
+    float fq = 0.f, fk = 0.f;
+    if (p.l2norm) {
+      const float rq = sm.rqk[row] / p.scale, rk = sm.rqk[C + row];
+      if (rq < 0.99e12f) fq = rq * rq * (sm.dot[0][0][row] + sm.dot[0][1][row]);
+      if (rk < 0.99e12f) fk = rk * rk * (sm.dot[1][0][row] + sm.dot[1][1][row]);
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int col = n0 + n * 8 + 2 * t;
+      if (col < p.dk) {
+        const float2 q = unpack_bf16x2(lds32(sq + at2<U>(row, col))), k = unpack_bf16x2(lds32(sk + at2<U>(row, col)));
+        *reinterpret_cast<uint32_t*>(dq + row * d_t + col) = pack_bf16x2(aq[n][2 * r] - fq * q.x, aq[n][2 * r + 1] - fq * q.y);
+        *reinterpret_cast<uint32_t*>(dk + row * d_t + col) = pack_bf16x2(ak[n][2 * r] - fk * k.x, ak[n][2 * r + 1] - fk * k.y);
+      }
+    }
+  }
+}
+
+// dA and dD: sums of the chunks' parts, in a fixed order
+__global__ void __launch_bounds__(128) rec_reduce(const XbRecArgs p) {
+  __shared__ double red[2][4];
+  const int h = blockIdx.x, n = p.doc_off[p.n_docs + 2], lane = threadIdx.x & 31;
+  double a = 0.0, b = 0.0;
+  for (int c = threadIdx.x; c < n; c += 128) {
+    const float2 v = *reinterpret_cast<const float2*>(p.part + ((long long)c * p.Hv + h) * 2);
+    a += v.x, b += v.y;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    a += __shfl_xor_sync(0xffffffffu, a, o);
+    b += __shfl_xor_sync(0xffffffffu, b, o);
+  }
+  if (lane == 0) red[0][threadIdx.x >> 5] = a, red[1][threadIdx.x >> 5] = b;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    p.dA[h] = (float)((red[0][0] + red[0][1]) + (red[0][2] + red[0][3]));
+    p.dD[h] = (float)((red[1][0] + red[1][1]) + (red[1][2] + red[1][3]));
+  }
+}
+
+template <typename K>
+int launch(K kernel, long long blocks, int threads, size_t smem, const XbRecArgs& a, cudaStream_t st) {
+  if (blocks <= 0) return 0;
+  if (blocks > 0x7fffffffLL) return -4;
+  if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
+    cudaGetLastError();
+    return -5;
+  }
+  kernel<<<(unsigned)blocks, threads, smem, st>>>(a);
+  return cudaGetLastError() == cudaSuccess ? 0 : -11;
+}
+
+bool bad_args(const XbRecArgs& a) {
+  return a.T < 0 || a.n_docs < 0 || a.Hk <= 0 || a.Hv <= 0 || a.Hv % a.Hk || a.dk <= 0 || a.dk > 128 || a.dk % 8 || a.dv <= 0 ||
+         a.dv % 8 || a.dvp != (a.dv + NV - 1) / NV * NV || a.nc_max < a.T / C + a.n_docs + 2;
+}
+
+template <int DKP, bool DELTA>
+int forward(const XbRecArgs& a, cudaStream_t st) {
+  const long long seq = (long long)(a.n_docs + 2) * a.Hv * (a.dvp / NV);
+  rec_plan<<<1, 1024, 0, st>>>(a.cu, a.n_docs, a.T, a.nc_max, (int4*)a.chunks, a.doc_off, xb_status_ptr());
+  if (cudaGetLastError() != cudaSuccess) return -11;
+  if (int rc = launch(rec_prep<DKP, DELTA>, (long long)a.nc_max * a.Hk, 128, sizeof(PrepSmem<DKP, DELTA>), a, st)) return rc;
+  return launch(rec_fwd<DKP, DELTA, false>, seq, 128, sizeof(FwdSmem<DKP, DELTA>), a, st);
+}
+
+template <int DKP, bool DELTA>
+int backward(const XbRecArgs& a, cudaStream_t st) {
+  const long long seq = (long long)(a.n_docs + 2) * a.Hv * (a.dvp / NV);
+  XbRecArgs again = a;
+  again.s_out = nullptr;
+  if (int rc = launch(rec_fwd<DKP, DELTA, true>, seq, 128, sizeof(FwdSmem<DKP, DELTA>), again, st)) return rc;
+  if (int rc = launch(rec_bwd<DKP, DELTA>, seq, 128, sizeof(BwdSmem<DKP, DELTA>), a, st)) return rc;
+  if (int rc = launch(rec_grad<DKP, DELTA>, (long long)a.nc_max * a.Hk, 256, sizeof(GradSmem<DKP, DELTA>), a, st)) return rc;
+  return DELTA ? 0 : launch(rec_reduce, a.Hv, 128, 0, a, st);
+}
+
+}  // namespace
+
+XB_API int xb_recurrence_chunk() { return C; }
+
+XB_API int xb_recurrence_fwd(const XbRecArgs* a, int delta, void* stream) {
+  if (a == nullptr || bad_args(*a)) return -1;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (a->dk <= 64) return delta ? forward<64, true>(*a, st) : forward<64, false>(*a, st);
+  return delta ? forward<128, true>(*a, st) : forward<128, false>(*a, st);
+}
+
+XB_API int xb_recurrence_bwd(const XbRecArgs* a, int delta, void* stream) {
+  if (a == nullptr || bad_args(*a)) return -1;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (a->dk <= 64) return delta ? backward<64, true>(*a, st) : backward<64, false>(*a, st);
+  return delta ? backward<128, true>(*a, st) : backward<128, false>(*a, st);
+}

@@ -1,0 +1,35 @@
+// Arguments of the gated linear recurrences (recurrence.cu).  Plain data; the Python side mirrors the order.
+#pragma once
+
+struct XbRecArgs {
+  // inputs: bf16 [T, heads, dim] with element strides of token and head (dim contiguous)
+  const void *q, *k, *v, *dy;
+  long long q_t, q_h, k_t, k_h, v_t, v_h, dy_t, dy_h;
+  const float *g, *b;            // [T, Hv]: log decay (delta rule only), beta or dt
+  long long g_t, g_h, b_t, b_h;
+  const float *A, *D;            // [Hv], scan only
+  const int* cu;                 // n_docs + 1 boundaries
+  // states: fp32, [n_docs, Hv, dk * dv] with element strides s_k, s_v inside a head
+  const float* s_in;
+  float* s_out;
+  const float* ds_out;           // gradient of the final states
+  float* ds_in;
+  long long s_k, s_v;
+  // outputs
+  void *o;                       // bf16 [T, Hv, dv]
+  void *dq, *dk_out, *dv_out;    // bf16, contiguous
+  float *dg, *db;                // [T, Hv]
+  float *dA, *dD;                // [Hv]
+  // workspaces
+  void* chunks;                  // int4 [nc_max]: first token, tokens, document
+  int* doc_off;                  // [n_docs + 3]: first chunk of every document
+  float* hd;                     // [nc_max, Hv, 192]
+  float* rqk;                    // [nc_max, Hk, 128]
+  float *qk, *kk;                // [nc_max, Hk, 64, 64] (kk: delta rule only)
+  float* tm;                     // [nc_max, Hv, 64, 64] (delta rule only)
+  void *s_planes, *ds_planes;    // bf16 [nc_max, Hv, 2, 64 or 128, dvp]
+  void *u_planes, *dr_planes;    // bf16 [nc_max, Hv, 2, 64, dvp] (delta rule only)
+  float* part;                   // [nc_max, Hv, 2] (scan only)
+  int T, n_docs, Hk, Hv, dk, dv, dvp, nc_max, l2norm;
+  float scale;
+};

@@ -112,6 +112,9 @@ _SIGNATURES = {
     "xb_causal_conv1d_fwd": [P, L, P, P, P, P, L, I, I, I, I, P],
     "xb_causal_conv1d_bwd_chunks": [I],
     "xb_causal_conv1d_bwd": [P, L, P, L, P, P, P, P, P, L, P, I, I, I, I, P],
+    "xb_recurrence_chunk": [],
+    "xb_recurrence_fwd": [P, I, P],
+    "xb_recurrence_bwd": [P, I, P],
     "xb_dequant4": [P, P, P, P, L, I, I, P],
     "xb_quant4": [P, I, P, P, P, P, L, I, I, P],
     "xb_mirror_lower": [P, L, I, I, I, P],
