@@ -7,6 +7,7 @@ loaded, so no operator can silently fall back to a PyTorch implementation there.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -112,6 +113,9 @@ _SIGNATURES = {
     "xb_causal_conv1d_fwd": [P, L, P, P, P, P, L, I, I, I, I, P],
     "xb_causal_conv1d_bwd_chunks": [I],
     "xb_causal_conv1d_bwd": [P, L, P, L, P, P, P, P, P, L, P, I, I, I, I, P],
+    "xb_gated_norm_partial_rows": [I, I, I],
+    "xb_gated_norm_fwd": [P, L, P, L, P, I, I, P, P, I, I, I, F, I, P],
+    "xb_gated_norm_bwd": [P, L, P, L, P, L, P, I, I, P, P, P, P, P, I, I, I, I, P],
     "xb_recurrence_chunk": [],
     "xb_recurrence_fwd": [P, I, P],
     "xb_recurrence_bwd": [P, I, P],
@@ -175,6 +179,13 @@ def host_lib():
 def stream_ptr() -> int:
     """Handle of the current stream of the current device."""
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
+def on_device(t: torch.Tensor):
+    """Makes the tensor's device the current one for a launch whose caller has another one selected."""
+    if t.device.index != torch._C._cuda_getDevice():
+        return torch.cuda.device(t.device)
+    return contextlib.nullcontext()
 
 
 def current_stream() -> torch.cuda.Stream:

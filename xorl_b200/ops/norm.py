@@ -112,3 +112,95 @@ def rmsnorm(x: torch.Tensor, w: torch.Tensor, eps: float = 1e-6,
     if residual is not None:
         return y, h
     return y
+
+
+def _gated_rms_norm_ref(x, gate, weight, group_size, eps, norm_first):
+    act = torch.nn.functional.silu(gate.float())
+    h = x.float() if norm_first else x.float() * act
+    h = h.unflatten(-1, (-1, group_size))
+    h = h * torch.rsqrt(h.pow(2).mean(-1, keepdim=True) + eps) * weight.float().view(-1, group_size)
+    h = h.flatten(-2)
+    return (h * act if norm_first else h).to(x.dtype)
+
+
+def _norm_rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` [T, W] with rows that suit 16-byte loads: itself or a copy."""
+    if t.stride(1) != 1 or t.stride(0) % 8 or t.data_ptr() % 16:
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+class _GatedRMSNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate, w, group_size, eps, norm_first):
+        global _launches
+        shape = x.shape
+        W = shape[-1]
+        x2, z2 = _norm_rows(x.reshape(-1, W)), _norm_rows(gate.reshape(-1, W))
+        wc = w.detach().contiguous()
+        T, groups = x2.shape[0], W // group_size
+        y = torch.empty((T, W), dtype=x.dtype, device=x.device)
+        keep = any(ctx.needs_input_grad)
+        rstd = torch.empty((T, groups), dtype=torch.float32, device=x.device) if keep else None
+        with _lib.on_device(x):
+            _lib.check(_lib.cuda_lib().xb_gated_norm_fwd(
+                x2.data_ptr(), x2.stride(0), z2.data_ptr(), z2.stride(0), wc.data_ptr(),
+                int(w.dtype == torch.float32), int(w.numel() == group_size), y.data_ptr(), _lib.ptr(rstd), T, groups,
+                group_size, float(eps), int(norm_first), _lib.stream_ptr()), "xb_gated_norm_fwd")
+        _launches += 1
+        ctx.save_for_backward(x2, z2, wc, rstd)
+        ctx.w, ctx.conf, ctx.shape = w, (group_size, norm_first), shape
+        return y.reshape(shape)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        global _launches
+        x, z, wc, rstd = ctx.saved_tensors
+        group_size, norm_first = ctx.conf
+        T, W = x.shape
+        groups = W // group_size
+        lib = _lib.cuda_lib()
+        want = ctx.needs_input_grad[2]
+        with _lib.on_device(x):
+            dy = _norm_rows(dy.reshape(T, W))
+            dx, dz = torch.empty((T, W), dtype=x.dtype, device=x.device), torch.empty((T, W), dtype=x.dtype, device=x.device)
+            part = dw = None
+            if want:
+                rows = lib.xb_gated_norm_partial_rows(T, groups, group_size)
+                part = torch.empty((max(rows, 1), W), dtype=torch.float32, device=x.device)
+                dw = torch.empty(wc.numel(), dtype=torch.float32, device=x.device)
+            _lib.check(lib.xb_gated_norm_bwd(
+                dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), z.data_ptr(), z.stride(0), wc.data_ptr(),
+                int(wc.dtype == torch.float32), int(wc.numel() == group_size), rstd.data_ptr(), dx.data_ptr(),
+                dz.data_ptr(), _lib.ptr(part), _lib.ptr(dw), T, groups, group_size, int(norm_first),
+                _lib.stream_ptr()), "xb_gated_norm_bwd")
+        _launches += 1 + int(want)
+        return dx.reshape(ctx.shape), dz.reshape(ctx.shape), deliver_param_grad(ctx.w, dw) if want else None, None, None, None
+
+
+GATED_NORM_MAX_GROUP = 8192
+
+
+def gated_rms_norm(x: torch.Tensor, gate: torch.Tensor, weight: torch.Tensor, group_size: int, eps: float = 1e-6,
+                   norm_first: bool = True) -> torch.Tensor:
+    """RMS norm over groups of ``group_size`` columns with a SiLU gate, statistics in fp32, rounded once.
+
+    ``norm_first``: ``rms(x) * weight * silu(gate)`` (the GatedDeltaNet output norm), else
+    ``rms(x * silu(gate)) * weight`` (the Mamba2 one, src/xorl/ops/ssm/modules/gated_norm.py).  x and gate are [..., W]
+    of one shape and type, any row stride; weight has W elements or ``group_size`` that all groups share.  The CUDA
+    kernels (``csrc/gated_norm.cu``) take bf16 rows with a bf16 or fp32 weight and groups of a multiple of 8 columns,
+    8192 at most; elsewhere the same arithmetic runs as tensor ops."""
+    W = x.shape[-1]
+    if gate.shape != x.shape or gate.device != x.device or weight.device != x.device:
+        raise ValueError(f"gated_rms_norm: x and gate have one shape on one device with the weight (got {tuple(x.shape)} "
+                         f"on {x.device}, {tuple(gate.shape)} on {gate.device}, weight on {weight.device})")
+    if group_size <= 0 or W == 0 or W % group_size:
+        raise ValueError(f"gated_rms_norm: groups of {group_size} columns do not divide rows of {W}")
+    if weight.numel() not in (group_size, W):
+        raise ValueError(f"gated_rms_norm: weight has {weight.numel()} elements, expected {group_size} or {W}")
+    if (not x.is_cuda or x.dtype != torch.bfloat16 or gate.dtype != torch.bfloat16 or group_size % 8
+            or weight.dtype not in (torch.bfloat16, torch.float32) or group_size > GATED_NORM_MAX_GROUP
+            or W // group_size > 65535):
+        return _gated_rms_norm_ref(x, gate, weight, group_size, eps, norm_first)
+    return _lib.apply(_GatedRMSNorm, x, gate, weight, int(group_size), float(eps), bool(norm_first))

@@ -13,7 +13,6 @@ read strided inputs in place when the last dimension is contiguous and rows star
 others.  A call allocates its workspace; it does not synchronise and may be captured into a CUDA graph."""
 from __future__ import annotations
 
-import contextlib
 import ctypes
 from typing import Optional
 
@@ -53,13 +52,6 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     if x.stride(2) != 1 or x.stride(0) % 8 or x.stride(1) % 8 or x.data_ptr() % 16:
         return x.contiguous() if not x.is_contiguous() else x.clone()
     return x
-
-
-def _on(t: torch.Tensor):
-    """Makes the tensor's device current for a call whose caller has another one selected."""
-    if t.device.index != torch._C._cuda_getDevice():
-        return torch.cuda.device(t.device)
-    return contextlib.nullcontext()
 
 
 def _pieces(sizes):
@@ -110,7 +102,7 @@ class _Recurrence(torch.autograd.Function):
         q, k, v = _rows(q), _rows(k), _rows(v)
         T, Hv, dv = v.shape
         a = _Args()
-        with _on(q):
+        with _lib.on_device(q):
             ws = _fill(a, q, k, v, g, b, A, D, cu, s_in, None, delta, scale, l2norm)
             o = torch.empty((T, Hv, dv), dtype=v.dtype, device=v.device)
             shape = (cu.numel() - 1, Hv) + ((q.shape[2], dv) if delta else (dv, q.shape[2]))
@@ -134,7 +126,7 @@ class _Recurrence(torch.autograd.Function):
         Hv, dv = v.shape[1], v.shape[2]
         dev = q.device
         a = _Args()
-        with _on(q):
+        with _lib.on_device(q):
             dy = torch.zeros((T, Hv, dv), dtype=v.dtype, device=dev) if dy is None else _rows(dy)
             _fill(a, q, k, v, g, b, A, D, cu, s_in, ws, delta, scale, l2norm)
             a.dy, a.dy_t, a.dy_h = dy.data_ptr(), dy.stride(0), dy.stride(1)
