@@ -16,15 +16,17 @@ the deltas u_t = beta_t (v_t - (exp(g_t) S_{t-1})^T k_t) solve a unit lower-tria
 j < i and gamma the running decay product, so every chunk costs a handful of batched matrix
 products and only one [d_k, d_v] state per head crosses chunk borders (the chunked formulation of
 src/xorl/ops/linear_attention/ops/gated_delta_rule/chunk.py).  Documents of the packed batch are cut
-into chunks separately, so neither the state nor the convolution crosses a document start.  The
-short convolutions run on the CUDA kernel of ``ops/seqmix.py`` when the activations are bf16 on a
-GPU."""
+into chunks separately, so neither the state nor the convolution crosses a document start.  With bf16
+activations on a GPU the short convolutions, the recurrence (L2 norms included) and the gated norm run
+on the CUDA kernels of ``ops/seqmix.py``, ``ops/recurrence.py`` and ``ops/norm.py``."""
 from __future__ import annotations
 
 import torch
 import torch.nn.functional as F
 from torch import nn
 
+from ..ops import recurrence
+from ..ops.norm import gated_rms_norm
 from ..ops.seqmix import causal_conv1d
 from .config import ModelConfig
 from .context import StepContext
@@ -201,16 +203,17 @@ class GatedDeltaNet(nn.Module):
         v = conv(self.v_proj(x), self.v_conv1d)
         beta = torch.sigmoid(self.b_proj(x).float())
         g = -torch.exp(self.A_log.float()) * F.softplus(self.a_proj(x).float() + self.dt_bias.float())
-        q = F.normalize(q.view(T, self.Hk, self.dk).float(), dim=-1) * self.dk ** -0.5
-        k = F.normalize(k.view(T, self.Hk, self.dk).float(), dim=-1)
-        if self.Hv > self.Hk:
-            rep = self.Hv // self.Hk
-            q, k = q.repeat_interleave(rep, 1), k.repeat_interleave(rep, 1)
+        q, k = q.view(T, self.Hk, self.dk), k.view(T, self.Hk, self.dk)
+        v = v.view(T, self.Hv, self.dv)
         if cp_group is not None:
-            o = gated_delta_rule_cp_docs(q, k, v.view(T, self.Hv, self.dv), g, beta, cu, cp_group).float()
+            q = F.normalize(q.float(), dim=-1) * self.dk ** -0.5
+            k = F.normalize(k.float(), dim=-1)
+            if self.Hv > self.Hk:
+                rep = self.Hv // self.Hk
+                q, k = q.repeat_interleave(rep, 1), k.repeat_interleave(rep, 1)
+            o = gated_delta_rule_cp_docs(q, k, v, g, beta, cu, cp_group)
         else:
-            o = gated_delta_rule_chunked(q, k, v.view(T, self.Hv, self.dv), g, beta, cu).float()
-        z = self.g_proj(x).view(T, self.Hv, self.dv).float()
-        o = o * torch.rsqrt(o.pow(2).mean(-1, keepdim=True) + self.eps) * self.o_norm_weight.float()
-        o = (o * F.silu(z)).to(x.dtype)
-        return self.o_proj(o.reshape(T, self.value_dim))
+            o = recurrence.gated_delta_rule(q, k, v, g, beta, cu, scale=self.dk ** -0.5, qk_l2norm=True)
+        o = gated_rms_norm(o.reshape(T, self.value_dim), self.g_proj(x), self.o_norm_weight, self.dv, self.eps,
+                           norm_first=True)
+        return self.o_proj(o.to(x.dtype))

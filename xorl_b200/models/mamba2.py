@@ -15,7 +15,8 @@ The layer follows the layout of the reference's mixer (src/xorl/ops/ssm/layers/m
 one input projection producing ``[gate | x | B | C | dt]``, a causal depthwise convolution + SiLU
 over ``[x | B | C]``, ``dt = clamp(softplus(dt + dt_bias))``, the scan, a gated grouped RMSNorm
 (``weight * group_rmsnorm(y * silu(gate))``, src/xorl/ops/ssm/modules/gated_norm.py) and the output
-projection.
+projection.  With bf16 activations on a GPU the scan and the gated norm run on the CUDA kernels of
+``ops/recurrence.py`` and ``ops/norm.py``.
 """
 from __future__ import annotations
 
@@ -28,6 +29,8 @@ from torch import nn
 
 from .config import ModelConfig
 from .context import StepContext
+from ..ops.norm import gated_rms_norm
+from ..ops.recurrence import ssd_scan
 from ..ops.seqmix import causal_conv1d
 from .layers import Linear
 
@@ -173,11 +176,13 @@ class Mamba2Mixer(nn.Module):
             y = ssd_cp_docs(x.reshape(T, self.H, self.P), dt, A, B.reshape(T, self.G, self.N),
                             C.reshape(T, self.G, self.N), self.D, local_cu, cp_group, self.chunk)
         else:
-            seg = segment_ids(ctx.cu_seqlens, T)
-            y = ssd_chunked(x.reshape(T, self.H, self.P), dt, A, B.reshape(T, self.G, self.N),
-                            C.reshape(T, self.G, self.N), self.D, seg, self.chunk)
-        y = gated_group_rmsnorm(y.reshape(T, self.d_inner).to(h.dtype), gate, self.norm_weight,
-                                self.d_inner // self.G, self.eps)
+            y = ssd_scan(x.reshape(T, self.H, self.P), dt, A, B.reshape(T, self.G, self.N),
+                         C.reshape(T, self.G, self.N), self.D, ctx.cu_seqlens, chunk=self.chunk)
+        y, group = y.reshape(T, self.d_inner).to(h.dtype), self.d_inner // self.G
+        if h.is_cuda and h.dtype == torch.bfloat16:
+            y = gated_rms_norm(y, gate, self.norm_weight, group, self.eps, norm_first=False)   # rounds once
+        else:
+            y = gated_group_rmsnorm(y, gate, self.norm_weight, group, self.eps)
         return self.out_proj(y.to(h.dtype))
 
 

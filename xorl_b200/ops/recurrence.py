@@ -258,19 +258,19 @@ def ssd_scan_reference(x, dt, A, B, C, D, cu_seqlens, *, initial_state=None, ret
 
 def ssd_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, D: torch.Tensor,
              cu_seqlens: torch.Tensor, *, initial_state: Optional[torch.Tensor] = None,
-             return_final_state: bool = False):
+             return_final_state: bool = False, chunk: int = 128):
     """S_t = e^{dt_t A} S_{t-1} + dt_t x_t (x) B_t;  y_t = S_t C_t + D x_t.
 
     x [T, H, P], dt [T, H] (behind softplus and clamp), A, D [H], B, C [T, G, N] shared by the H / G heads of a group.
     Returns y [T, H, P] in x's type, with ``return_final_state`` also the states [documents, H, P, N] (fp32) that
     leave the documents; ``initial_state`` of the same shape enters them (zeros if None).  Rows before the first and
-    behind the last boundary are documents of their own, without states."""
+    behind the last boundary are documents of their own, without states.  ``chunk``: chunk length of the tensor-op form."""
     T, H = x.shape[0], x.shape[1] if x.dim() == 3 else 0
     _check("ssd_scan", B, C, x, [("dt", dt, (T, H)), ("A", A, (H,)), ("D", D, (H,))], cu_seqlens, initial_state,
            (cu_seqlens.numel() - 1, H, x.shape[-1], B.shape[-1]), ("B", "C", "x"))
     if not _kernel_ok(B, C, x):
         return ssd_scan_reference(x, dt, A, B, C, D, cu_seqlens, initial_state=initial_state,
-                                  return_final_state=return_final_state)
+                                  return_final_state=return_final_state, chunk=chunk)
     s_in = None if initial_state is None else initial_state.float().contiguous()
     y, s = _lib.apply(_Recurrence, C, B, x, None, dt.float(), A.float().contiguous(), D.float().contiguous(), s_in,
                       _boundaries(cu_seqlens, x.device), False, 1.0, False, bool(return_final_state))
