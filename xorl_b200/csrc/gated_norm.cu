@@ -8,10 +8,10 @@
 //   gate first:  dn = dy w,    dh = r (dn - n mean(dn n)),  dx = dh s,  dz = dh x s',  dw = sum dy n
 //
 // Memory-bound: forward reads x and z and writes y, backward reads x, z and dy and writes dx and dz, each once.  A
-// team of lanes owns one group of one row in registers, 16 bytes per lane and load (up to 64 bytes of each input in
-// flight per lane), so the statistics cost shuffles only up to 1024 columns; wider groups add up through shared
-// memory.  A lane keeps its columns from row to row, so the weight's gradient is summed in registers and written once
-// per block; a second kernel adds the blocks' parts in a fixed order.
+// team of lanes owns one group of one row in registers, 16 bytes per lane and load; the next row's loads are issued
+// before a row is worked on.  Statistics cost shuffles up to 256 columns and one barrier of the team beyond.  A lane
+// keeps its columns from row to row, so the weight's gradient is summed in registers and written once per block; a
+// second kernel adds the blocks' parts in a fixed order.
 #include "common.cuh"
 
 namespace {
@@ -40,61 +40,87 @@ __device__ __forceinline__ void unpack8(const uint4 u, float (&v)[8]) {
 __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
   return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
 }
-__device__ __forceinline__ float sigm(float x) { return 1.f / (1.f + __expf(-x)); }
+// 1 / (1 + e^-x) with the fast divide: a denominator above 2^126 gives 0, where the value is below 2^-126
+__device__ __forceinline__ float sigm(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
 
-// sum over the LG lanes of a team, or over all NW warps of a block (WIDE)
-template <int LG, bool WIDE>
-__device__ __forceinline__ float team_sum(float v, float* red, int& phase) {
+// Where a thread works: teams of L lanes own a group each; the teams of a block cover `gpw` neighbouring groups (a
+// window of at most 256 U units) of `rows` rows, so that a block reads contiguous row segments.
+template <int L, int U>
+struct Place {
+  int l, row, rows, g, phase = 0;
+  bool on;                       // false: a team without a group
+  int c[U];                      // first column of each unit inside the group
+  bool ok[U];
+  __device__ Place(const Args& a) {
+    constexpr int TEAMS = 256 / L;
+    const int team = threadIdx.x / L, gpw = min(a.groups, TEAMS);
+    l = threadIdx.x % L, rows = TEAMS / gpw, row = team / gpw, g = blockIdx.y * gpw + team % gpw;
+    on = row < rows && g < a.groups;
 #pragma unroll
-  for (int o = LG / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if (WIDE) {
-    const int w = threadIdx.x >> 5, nw = blockDim.x >> 5;
-    float* r = red + (phase & 1) * 32;       // two buffers: one barrier per sum
-    ++phase;
-    if ((threadIdx.x & 31) == 0) r[w] = v;
-    __syncthreads();
-    v = 0.f;
-    for (int i = 0; i < nw; ++i) v += r[i];
+    for (int u = 0; u < U; ++u) c[u] = (u * L + l) * 8, ok[u] = on && c[u] < a.d;
   }
-  return v;
-}
+  // sum over the team; wide teams meet at a barrier of their own, two buffers take turns
+  __device__ float sum(float v, float* red) {
+#pragma unroll
+    for (int o = (L < 32 ? L : 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (L > 32) {
+      constexpr int NW = L > 32 ? L / 32 : 1;
+      const int team = threadIdx.x / L;
+      float* r = red + (phase & 1) * 8 + team * NW;
+      ++phase;
+      if ((threadIdx.x & 31) == 0) r[(threadIdx.x / 32) % NW] = v;
+      asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(L) : "memory");
+      v = r[0];
+#pragma unroll
+      for (int i = 1; i < NW; ++i) v += r[i];
+    }
+    return v;
+  }
+};
 
-template <int U>
-__device__ __forceinline__ void load_weight(const Args& a, int g, const int (&c)[U], const bool (&ok)[U], float (&w)[U][8]) {
+template <int L, int U>
+__device__ __forceinline__ void load_weight(const Args& a, const Place<L, U>& p, float (&w)[U][8]) {
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const long long at = (a.w_shared ? 0 : (long long)g * a.d) + c[u];
+    const long long at = (a.w_shared ? 0 : (long long)p.g * a.d) + p.c[u];
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      w[u][i] = !ok[u] ? 0.f : a.w_f32 ? ((const float*)a.w)[at + i] : __bfloat162float(((const bf16*)a.w)[at + i]);
+      w[u][i] = !p.ok[u] ? 0.f : a.w_f32 ? ((const float*)a.w)[at + i] : __bfloat162float(((const bf16*)a.w)[at + i]);
   }
 }
+template <int L, int U>
+__device__ __forceinline__ void load_row(const Place<L, U>& p, const bf16* base, long long ld, long long t, int T, int d, uint4 (&r)[U]) {
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    r[u] = t < T && p.ok[u] ? __ldcs(reinterpret_cast<const uint4*>(base + t * ld + p.g * d + p.c[u])) : make_uint4(0, 0, 0, 0);
+}
 
-// LG lanes per group (WIDE: the whole block), U 16-byte units per lane
-template <int LG, int U, bool WIDE, bool FIRST>
-__global__ void __launch_bounds__(256) gated_norm_fwd(const Args a) {
-  __shared__ float red[64];
-  int phase = 0;
-  const int lanes = WIDE ? blockDim.x : LG, team = WIDE ? 0 : threadIdx.x / LG, teams = WIDE ? 1 : blockDim.x / LG;
-  const int l = threadIdx.x % lanes, g = blockIdx.y, W = a.groups * a.d;
-  int c[U];
-  bool ok[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u) c[u] = (u * lanes + l) * 8, ok[u] = c[u] < a.d;
+template <int L, int U, bool FIRST>
+__global__ void __launch_bounds__(256, U == 1 ? 4 : 2) gated_norm_fwd(const Args a) {
+  __shared__ float red[16];
+  Place<L, U> p(a);
+  const long long W = (long long)a.groups * a.d, step = (long long)gridDim.x * p.rows;
   float w[U][8];
-  load_weight<U>(a, g, c, ok, w);
+  load_weight(a, p, w);
   const float inv = 1.f / (float)a.d;
-  for (long long t0 = (long long)blockIdx.x * teams; t0 < a.T; t0 += (long long)gridDim.x * teams) {
-    const long long t = t0 + team;
-    const bool row = t < a.T;                        // all lanes take part in the sums
+  long long t = (long long)blockIdx.x * p.rows + p.row;
+  constexpr bool AHEAD = U < 4;                      // four units would not leave the registers for it
+  uint4 nx[U], nz[U];
+  if (AHEAD) {
+    load_row(p, a.x, a.ldx, t, a.T, a.d, nx);
+    load_row(p, a.z, a.ldz, t, a.T, a.d, nz);
+  }
+  for (long long t0 = (long long)blockIdx.x * p.rows; t0 < a.T; t0 += step, t += step) {
     uint4 rx[U], rz[U];
+    if (!AHEAD) {
+      load_row(p, a.x, a.ldx, t, a.T, a.d, nx);
+      load_row(p, a.z, a.ldz, t, a.T, a.d, nz);
+    }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      rx[u] = rz[u] = make_uint4(0, 0, 0, 0);
-      if (row && ok[u]) {
-        rx[u] = *reinterpret_cast<const uint4*>(a.x + t * a.ldx + g * a.d + c[u]);
-        rz[u] = *reinterpret_cast<const uint4*>(a.z + t * a.ldz + g * a.d + c[u]);
-      }
+    for (int u = 0; u < U; ++u) rx[u] = nx[u], rz[u] = nz[u];
+    if (AHEAD) {                                     // the next row travels while this one is worked on
+      load_row(p, a.x, a.ldx, t + step, a.T, a.d, nx);
+      load_row(p, a.z, a.ldz, t + step, a.T, a.d, nz);
     }
     float h[U][8], ss = 0.f;
 #pragma unroll
@@ -109,106 +135,117 @@ __global__ void __launch_bounds__(256) gated_norm_fwd(const Args a) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) ss += h[u][i] * h[u][i];
     }
-    const float r = rsqrtf(team_sum<LG, WIDE>(ss, red, phase) * inv + a.eps);
-    if (!row) continue;
-    if (l == 0 && a.rstd != nullptr) a.rstd[t * a.groups + g] = r;
+    const float r = rsqrtf(p.sum(ss, red) * inv + a.eps);
+    if (t < a.T) {
+      if (p.on && p.l == 0 && a.rstd != nullptr) a.rstd[t * a.groups + p.g] = r;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float y[8], z[8];
-      if (FIRST) unpack8(rz[u], z);
+      for (int u = 0; u < U; ++u) {
+        float y[8], z[8];
+        if (FIRST) unpack8(rz[u], z);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = h[u][i] * r * w[u][i] * (FIRST ? z[i] * sigm(z[i]) : 1.f);
-      if (ok[u]) *reinterpret_cast<uint4*>(a.y + t * W + g * a.d + c[u]) = pack8(y);
+        for (int i = 0; i < 8; ++i) y[i] = h[u][i] * r * w[u][i] * (FIRST ? z[i] * sigm(z[i]) : 1.f);
+        if (p.ok[u]) *reinterpret_cast<uint4*>(a.y + t * W + p.g * a.d + p.c[u]) = pack8(y);
+      }
     }
   }
 }
 
-template <int LG, int U, bool WIDE, bool FIRST>
-__global__ void __launch_bounds__(256) gated_norm_bwd(const Args a) {
-  extern __shared__ float sums[];                    // teams x d, for the weight's gradient
-  __shared__ float red[64];
-  int phase = 0;
-  const int lanes = WIDE ? blockDim.x : LG, team = WIDE ? 0 : threadIdx.x / LG, teams = WIDE ? 1 : blockDim.x / LG;
-  const int l = threadIdx.x % lanes, g = blockIdx.y, W = a.groups * a.d;
-  int c[U];
-  bool ok[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u) c[u] = (u * lanes + l) * 8, ok[u] = c[u] < a.d;
+template <int L, int U, bool FIRST>
+__global__ void __launch_bounds__(256, U == 1 ? 2 : 1) gated_norm_bwd(const Args a) {
+  __shared__ float sums[U == 1 ? 2048 : 1];          // weight gradients of the block's rows
+  __shared__ float red[16];
+  Place<L, U> p(a);
+  const long long W = (long long)a.groups * a.d, step = (long long)gridDim.x * p.rows;
   float w[U][8], dw[U][8] = {};
-  load_weight<U>(a, g, c, ok, w);
+  load_weight(a, p, w);
   const float inv = 1.f / (float)a.d;
-  for (long long t0 = (long long)blockIdx.x * teams; t0 < a.T; t0 += (long long)gridDim.x * teams) {
-    const long long t = t0 + team;
-    const bool row = t < a.T;
+  long long t = (long long)blockIdx.x * p.rows + p.row;
+  constexpr bool AHEAD = U < 4;
+  uint4 nx[U], nz[U], ny[U];
+  float nr = p.on && t < a.T ? a.rstd[t * a.groups + p.g] : 0.f;
+  if (AHEAD) {
+    load_row(p, a.x, a.ldx, t, a.T, a.d, nx);
+    load_row(p, a.z, a.ldz, t, a.T, a.d, nz);
+    load_row(p, a.dy, a.lddy, t, a.T, a.d, ny);
+  }
+  for (long long t0 = (long long)blockIdx.x * p.rows; t0 < a.T; t0 += step, t += step) {
     uint4 rx[U], rz[U], ry[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      rx[u] = rz[u] = ry[u] = make_uint4(0, 0, 0, 0);
-      if (row && ok[u]) {
-        rx[u] = *reinterpret_cast<const uint4*>(a.x + t * a.ldx + g * a.d + c[u]);
-        rz[u] = *reinterpret_cast<const uint4*>(a.z + t * a.ldz + g * a.d + c[u]);
-        ry[u] = *reinterpret_cast<const uint4*>(a.dy + t * a.lddy + g * a.d + c[u]);
-      }
+    const float r = nr;
+    if (!AHEAD) {
+      load_row(p, a.x, a.ldx, t, a.T, a.d, nx);
+      load_row(p, a.z, a.ldz, t, a.T, a.d, nz);
+      load_row(p, a.dy, a.lddy, t, a.T, a.d, ny);
     }
-    const float r = row ? a.rstd[t * a.groups + g] : 0.f;
-    float n[U][8], dn[U][8], dot = 0.f;
+#pragma unroll
+    for (int u = 0; u < U; ++u) rx[u] = nx[u], rz[u] = nz[u], ry[u] = ny[u];
+    nr = p.on && t + step < a.T ? a.rstd[(t + step) * a.groups + p.g] : 0.f;
+    if (AHEAD) {
+      load_row(p, a.x, a.ldx, t + step, a.T, a.d, nx);
+      load_row(p, a.z, a.ldz, t + step, a.T, a.d, nz);
+      load_row(p, a.dy, a.lddy, t + step, a.T, a.d, ny);
+    }
+    float sg[U][8], dot = 0.f;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       float x[8], z[8], y[8];
       unpack8(rx[u], x), unpack8(rz[u], z), unpack8(ry[u], y);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float s = z[i] * sigm(z[i]);
-        n[u][i] = x[i] * r * (FIRST ? 1.f : s);
-        dn[u][i] = y[i] * w[u][i] * (FIRST ? s : 1.f);
-        dw[u][i] += y[i] * n[u][i] * (FIRST ? s : 1.f);
-        dot += dn[u][i] * n[u][i];
+        sg[u][i] = sigm(z[i]);
+        const float s = z[i] * sg[u][i], f = x[i] * r * s * y[i];      // n dy s or n dy: the same product either way
+        dw[u][i] += f;
+        dot += f * w[u][i];
       }
     }
-    const float m = team_sum<LG, WIDE>(dot, red, phase) * inv;
-    if (!row) continue;
+    const float m = p.sum(dot, red) * inv;
+    if (t < a.T) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float x[8], z[8], y[8], dx[8], dz[8];
-      unpack8(rx[u], x), unpack8(rz[u], z), unpack8(ry[u], y);
+      for (int u = 0; u < U; ++u) {
+        float x[8], z[8], y[8], dx[8], dz[8];
+        unpack8(rx[u], x), unpack8(rz[u], z), unpack8(ry[u], y);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float sg = sigm(z[i]), s = z[i] * sg, slope = sg * (1.f + z[i] * (1.f - sg));
-        const float dh = r * (dn[u][i] - n[u][i] * m);
-        dx[i] = FIRST ? dh : dh * s;
-        dz[i] = (FIRST ? y[i] * n[u][i] * w[u][i] : dh * x[i]) * slope;
-      }
-      if (ok[u]) {
-        *reinterpret_cast<uint4*>(a.dx + t * W + g * a.d + c[u]) = pack8(dx);
-        *reinterpret_cast<uint4*>(a.dz + t * W + g * a.d + c[u]) = pack8(dz);
+        for (int i = 0; i < 8; ++i) {
+          const float s = z[i] * sg[u][i], slope = sg[u][i] * (1.f + z[i] * (1.f - sg[u][i]));
+          const float n = x[i] * r * (FIRST ? 1.f : s), dn = y[i] * w[u][i] * (FIRST ? s : 1.f);
+          const float dh = r * (dn - n * m);
+          dx[i] = FIRST ? dh : dh * s;
+          dz[i] = (FIRST ? y[i] * n * w[u][i] : dh * x[i]) * slope;
+        }
+        if (p.ok[u]) {
+          *reinterpret_cast<uint4*>(a.dx + t * W + p.g * a.d + p.c[u]) = pack8(dx);
+          *reinterpret_cast<uint4*>(a.dz + t * W + p.g * a.d + p.c[u]) = pack8(dz);
+        }
       }
     }
   }
   if (a.part == nullptr) return;
-  float* out = a.part + (long long)blockIdx.x * W + g * a.d;
-  if (teams == 1) {
+  // one row of `part` per block: [gridDim.x, groups * d], or [blocks, d] where the groups share the weight
+  float* out = a.w_shared ? a.part + ((long long)blockIdx.x * gridDim.y + blockIdx.y) * a.d
+                          : a.part + (long long)blockIdx.x * W + (long long)p.g * a.d;
+  if (U == 1) {                                      // teams meet in shared memory: those of other rows, or all
+    const int gpw = min(a.groups, 256 / L), team = threadIdx.x / L;
+    const int mine = a.w_shared ? 0 : team % gpw, n = a.w_shared ? 256 / L : p.rows, stride = a.w_shared ? 1 : gpw;
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (ok[u])
+    for (int i = 0; i < 8; ++i) sums[threadIdx.x * 8 + i] = dw[0][i];          // 0 in teams without a group
+    __syncthreads();
+    if (team != mine || p.c[0] >= a.d || (!a.w_shared && !p.on)) return;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) out[c[u] + i] = dw[u][i];
+    for (int i = 0; i < 8; ++i) {
+      float s = 0.f;
+      for (int j = 0; j < n; ++j) s += sums[((mine + j * stride) * L + p.l) * 8 + i];
+      out[p.c[0] + i] = s;
+    }
     return;
   }
 #pragma unroll
   for (int u = 0; u < U; ++u)
-    if (ok[u])
+    if (p.ok[u])
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sums[team * a.d + c[u] + i] = dw[u][i];
-  __syncthreads();
-  for (int i = threadIdx.x; i < a.d; i += blockDim.x) {
-    float s = 0.f;
-    for (int j = 0; j < teams; ++j) s += sums[j * a.d + i];
-    out[i] = s;
-  }
+      for (int i = 0; i < 8; ++i) out[p.c[u] + i] = dw[u][i];
 }
 
 // dw[c] = sum of `rows` rows of part [rows, n]: 32 columns per block, 8 threads of each share the rows
-__global__ void __launch_bounds__(256) gated_norm_dw(const float* __restrict__ part, float* __restrict__ dw, int rows, int n) {
+__global__ void __launch_bounds__(256) gated_norm_dw(const float* __restrict__ part, void* __restrict__ dw, int f32, int rows, int n) {
   __shared__ float red[8][33];
   const int col = blockIdx.x * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5;
   float s = 0.f;
@@ -219,46 +256,44 @@ __global__ void __launch_bounds__(256) gated_norm_dw(const float* __restrict__ p
   if (k == 0 && col < n) {
 #pragma unroll
     for (int i = 1; i < 8; ++i) s += red[i][threadIdx.x];
-    dw[col] = s;
+    if (f32) ((float*)dw)[col] = s;
+    else ((bf16*)dw)[col] = __float2bfloat16(s);
   }
 }
 
-// Rows that a block walks: enough blocks for `per_sm` of 256 threads on every SM, no more than there are rows.
-dim3 grid_of(int T, int groups, int teams, int per_sm) {
-  const int want = (xb_sm_count() * per_sm + groups - 1) / groups, most = (T + teams - 1) / teams;
-  return dim3((unsigned)max(1, min(want, most)), (unsigned)groups);
+// Lanes per group: the fewest that hold it in one 16-byte unit each, up to 256; wider groups take 2 or 4 units per lane.
+int lanes_of(int d) {
+  int l = 8;
+  while (l < 256 && l * 8 < d) l *= 2;
+  return l;
 }
-
-struct Shape { int lanes, units, threads; bool wide; };
-// Narrow groups: the fewest lanes that hold a group in one 16-byte unit each; from 512 columns a warp with 2, then 4
-// units; wider ones a block of warps with 4 units per lane.
-Shape shape_of(int d) {
-  const int units = d / 8;
-  if (units <= 8) return {8, 1, 256, false};
-  if (units <= 16) return {16, 1, 256, false};
-  if (units <= 32) return {32, 1, 256, false};
-  if (units <= 64) return {32, 2, 256, false};
-  if (units <= 128) return {32, 4, 256, false};
-  return {32, 4, (units + 127) / 128 * 32, true};
+// Blocks side by side over the groups, and enough along the rows to fill the SMs once.
+dim3 grid_of(int T, int groups, int d, bool bwd) {
+  const int teams = 256 / lanes_of(d), gpw = min(groups, teams), rows = teams / gpw, wy = (groups + gpw - 1) / gpw;
+  const int per_sm = d <= 2048 ? (bwd ? 2 : 4) : (bwd ? 1 : 2);
+  const int want = xb_sm_count() * per_sm / wy, most = (T + rows - 1) / rows;
+  return dim3((unsigned)max(1, min(want, most)), (unsigned)wy);
 }
 
 template <bool BWD, bool FIRST>
 int run(const Args& a, cudaStream_t st) {
-  const Shape s = shape_of(a.d);
-  const int teams = s.wide ? 1 : s.threads / s.lanes;
-  const dim3 grid = grid_of(a.T, a.groups, teams, BWD ? 4 : 8);
-  const size_t smem = BWD && a.part != nullptr && teams > 1 ? (size_t)teams * a.d * 4 : 0;
-#define XB_RUN(L, U, WD)                                                        \
-  do {                                                                          \
-    if (BWD) gated_norm_bwd<L, U, WD, FIRST><<<grid, s.threads, smem, st>>>(a); \
-    else gated_norm_fwd<L, U, WD, FIRST><<<grid, s.threads, 0, st>>>(a);        \
+  const dim3 grid = grid_of(a.T, a.groups, a.d, BWD);
+#define XB_RUN(L, U)                                                  \
+  do {                                                                \
+    if (BWD) gated_norm_bwd<L, U, FIRST><<<grid, 256, 0, st>>>(a);    \
+    else gated_norm_fwd<L, U, FIRST><<<grid, 256, 0, st>>>(a);        \
   } while (0)
-  if (s.wide) XB_RUN(32, 4, true);
-  else if (s.units == 4) XB_RUN(32, 4, false);
-  else if (s.units == 2) XB_RUN(32, 2, false);
-  else if (s.lanes == 32) XB_RUN(32, 1, false);
-  else if (s.lanes == 16) XB_RUN(16, 1, false);
-  else XB_RUN(8, 1, false);
+  switch (lanes_of(a.d)) {
+    case 8: XB_RUN(8, 1); break;
+    case 16: XB_RUN(16, 1); break;
+    case 32: XB_RUN(32, 1); break;
+    case 64: XB_RUN(64, 1); break;
+    case 128: XB_RUN(128, 1); break;
+    default:
+      if (a.d <= 2048) XB_RUN(256, 1);
+      else if (a.d <= 4096) XB_RUN(256, 2);
+      else XB_RUN(256, 4);
+  }
 #undef XB_RUN
   return cudaGetLastError() == cudaSuccess ? 0 : -11;
 }
@@ -269,11 +304,11 @@ bool bad(const Args& a) {
 
 }  // namespace
 
-// Rows of the buffer that the backward pass needs for the weight's gradient.
-XB_API int xb_gated_norm_partial_rows(int T, int groups, int d) {
+// fp32 values of the buffer that the backward pass needs for the weight's gradient.
+XB_API int xb_gated_norm_partial(int T, int groups, int d, int w_shared) {
   if (T <= 0 || groups <= 0 || d <= 0 || d % 8) return 0;
-  const Shape s = shape_of(d);
-  return (int)grid_of(T, groups, s.wide ? 1 : s.threads / s.lanes, 4).x;
+  const dim3 g = grid_of(T, groups, d, true);
+  return (int)(w_shared ? g.x * g.y * d : g.x * groups * d);
 }
 
 XB_API int xb_gated_norm_fwd(const void* x, long long ldx, const void* z, long long ldz, const void* w, int w_f32,
@@ -287,10 +322,10 @@ XB_API int xb_gated_norm_fwd(const void* x, long long ldx, const void* z, long l
   return norm_first ? run<false, true>(a, (cudaStream_t)stream) : run<false, false>(a, (cudaStream_t)stream);
 }
 
-// dw: fp32 [d] (shared weight) or [groups * d]; with part null it is not computed.
+// dw: [d] (shared weight) or [groups * d], fp32 or bf16; with part null it is not computed.
 XB_API int xb_gated_norm_bwd(const void* dy, long long lddy, const void* x, long long ldx, const void* z, long long ldz,
                              const void* w, int w_f32, int w_shared, const float* rstd, void* dx, void* dz, float* part,
-                             float* dw, int T, int groups, int d, int norm_first, void* stream) {
+                             void* dw, int dw_f32, int T, int groups, int d, int norm_first, void* stream) {
   Args a{};
   a.dy = (const bf16*)dy, a.lddy = lddy;
   a.x = (const bf16*)x, a.z = (const bf16*)z, a.ldx = ldx, a.ldz = ldz, a.w = w, a.w_f32 = w_f32, a.w_shared = w_shared;
@@ -302,7 +337,7 @@ XB_API int xb_gated_norm_bwd(const void* dy, long long lddy, const void* x, long
     if (rc) return rc;
   }
   if (part == nullptr) return 0;
-  const int rows = xb_gated_norm_partial_rows(T, groups, d) * (w_shared ? groups : 1), n = w_shared ? d : groups * d;
-  gated_norm_dw<<<(n + 31) / 32, 256, 0, st>>>(part, dw, rows, n);
+  const int n = w_shared ? d : groups * d, rows = xb_gated_norm_partial(T, groups, d, w_shared) / n;
+  gated_norm_dw<<<(n + 31) / 32, 256, 0, st>>>(part, dw, dw_f32, rows, n);
   return cudaGetLastError() == cudaSuccess ? 0 : -11;
 }

@@ -166,14 +166,16 @@ class _GatedRMSNorm(torch.autograd.Function):
             dy = _norm_rows(dy.reshape(T, W))
             dx, dz = torch.empty((T, W), dtype=x.dtype, device=x.device), torch.empty((T, W), dtype=x.dtype, device=x.device)
             part = dw = None
+            shared = int(wc.numel() == group_size)
             if want:
-                rows = lib.xb_gated_norm_partial_rows(T, groups, group_size)
-                part = torch.empty((max(rows, 1), W), dtype=torch.float32, device=x.device)
-                dw = torch.empty(wc.numel(), dtype=torch.float32, device=x.device)
+                part = torch.empty(max(lib.xb_gated_norm_partial(T, groups, group_size, shared), 1), dtype=torch.float32,
+                                   device=x.device)
+                # an engine's buffer takes fp32 sums; a gradient that autograd gets is rounded where it is summed
+                dw = torch.empty(wc.shape, dtype=wc.dtype if grad_target(ctx.w)[0] is None else torch.float32, device=x.device)
             _lib.check(lib.xb_gated_norm_bwd(
                 dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), z.data_ptr(), z.stride(0), wc.data_ptr(),
-                int(wc.dtype == torch.float32), int(wc.numel() == group_size), rstd.data_ptr(), dx.data_ptr(),
-                dz.data_ptr(), _lib.ptr(part), _lib.ptr(dw), T, groups, group_size, int(norm_first),
+                int(wc.dtype == torch.float32), shared, rstd.data_ptr(), dx.data_ptr(), dz.data_ptr(), _lib.ptr(part),
+                _lib.ptr(dw), int(want and dw.dtype == torch.float32), T, groups, group_size, int(norm_first),
                 _lib.stream_ptr()), "xb_gated_norm_bwd")
         _launches += 1 + int(want)
         return dx.reshape(ctx.shape), dz.reshape(ctx.shape), deliver_param_grad(ctx.w, dw) if want else None, None, None, None
