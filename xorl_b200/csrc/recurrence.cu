@@ -26,114 +26,9 @@
 // significand: one bf16 value (9 bits) would cost the fp32 gradients of the decay three decimal digits.  Products of
 // two such sums leave out low x low.  Decays are sums in fp64 of log2 units, kept as two floats, so that differences
 // of large sums stay exact.  L2 norms of q and k are row factors and are applied behind the products.
-#include "common.cuh"
-#include "recurrence.h"
+#include "recurrence_core.cuh"
 
 namespace {
-
-constexpr int C = 64;         // tokens of a chunk
-constexpr int NV = 32;        // state columns of a CTA of the sequential kernels
-constexpr int HD = 3 * C;     // per chunk and v head: G (two floats each, log2 units), b
-constexpr int RQK = 2 * C;    // per chunk and q / k head: row factors of q and k
-constexpr float MIN_LOG = -120.f;  // e^-120 is 0 in fp32: a stronger decay changes nothing and would cost G its digits
-
-using bf16 = __nv_bfloat16;
-
-// ---- fragments ---------------------------------------------------------------------------------------------
-__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-               "{%0, %1, %2, %3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-// two fp32 values as the sums of two bf16 values each
-__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
-  hi = pack_bf16x2(x, y);
-  const float2 h = unpack_bf16x2(hi);
-  lo = pack_bf16x2(x - h.x, y - h.y);
-}
-__device__ __forceinline__ float2 join2(uint32_t hi, uint32_t lo) {
-  const float2 h = unpack_bf16x2(hi), l = unpack_bf16x2(lo);
-  return make_float2(h.x + l.x, h.y + l.y);
-}
-
-// A tile is rows of U 16-byte units; unit u of a row lies at u ^ f(row), so that the eight rows that ldmatrix reads
-// at one unit fall into eight different banks.
-template <int U>
-__device__ __forceinline__ uint32_t swz(int row, int u) {
-  return (uint32_t)(row * U + (U == 4 ? (u ^ ((row >> 1) & 3)) : (u ^ (row & 7)))) * 16u;
-}
-// address of two neighbouring bf16 values (col even)
-template <int U>
-__device__ __forceinline__ uint32_t at2(int row, int col) {
-  return swz<U>(row, col >> 3) + (uint32_t)(col & 7) * 2u;
-}
-__device__ __forceinline__ uint32_t lds32(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-  return v;
-}
-__device__ __forceinline__ void sts32(uint32_t a, uint32_t v) {
-  asm volatile("st.shared.b32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
-}
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
-  return v;
-}
-
-// fragment addresses of this lane; m0, n0, k0 are multiples of 8 (16 for the wide ones)
-template <int U>  // A[m][k], k contiguous
-__device__ __forceinline__ uint32_t addr_a(int m0, int k0) {
-  const int l = xb_lane();
-  return swz<U>(m0 + (l & 15), (k0 >> 3) + (l >> 4));
-}
-template <int U>  // A = X^T, X[k][m], m contiguous (transposing load)
-__device__ __forceinline__ uint32_t addr_at(int m0, int k0) {
-  const int l = xb_lane();
-  return swz<U>(k0 + (l & 7) + (l >> 4) * 8, (m0 >> 3) + ((l >> 3) & 1));
-}
-template <int U>  // B of two 8-wide column tiles, X[k][n], n contiguous (transposing load)
-__device__ __forceinline__ uint32_t addr_bt(int k0, int n0) {
-  const int l = xb_lane();
-  return swz<U>(k0 + (l & 15), (n0 >> 3) + (l >> 4));
-}
-template <int U>  // B of two 8-wide column tiles, X[n][k], k contiguous
-__device__ __forceinline__ uint32_t addr_b(int n0, int k0) {
-  const int l = xb_lane();
-  return swz<U>(n0 + (l & 7) + (l >> 4) * 8, (k0 >> 3) + ((l >> 3) & 1));
-}
-
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-// ROWS rows of U units from `src` (row stride ld elements); units behind `cols` and rows behind `rows` become zero
-template <int U, int ROWS, int THREADS>
-__device__ __forceinline__ void load_tile(uint32_t dst, const bf16* src, long long ld, int rows, int cols) {
-#pragma unroll
-  for (int i = 0; i < ROWS * U / THREADS; ++i) {
-    const int idx = i * THREADS + threadIdx.x, r = idx / U, u = idx % U;
-    const bool ok = r < rows && u * 8 < cols;
-    cp16(dst + swz<U>(r, u), ok ? src + r * ld + u * 8 : src, ok);
-  }
-}
-template <int THREADS>
-__device__ __forceinline__ void load_floats(uint32_t dst, const float* src, int n) {
-  for (int i = threadIdx.x; i < n / 4; i += THREADS) cp16(dst + i * 16, src + i * 4, true);
-}
 
 // ---- plan: chunks of the documents -----------------------------------------------------------------------------
 // Documents 0 .. n-1 lie between the boundaries; n is the tail behind the last boundary, n + 1 the rows before the first.
@@ -340,7 +235,7 @@ __global__ void __launch_bounds__(128) rec_prep(const XbRecArgs p) {
         // column j of (I + L)^-1 by forward substitution; all threads of a head read the same row of L
         float x[C];
         const float4* L4 = reinterpret_cast<const float4*>(sm.l[m]);
-        float* out = p.tm + ((long long)c * p.Hv + kh * rep + hh) * (C * C) + j;
+        float* out = ((float*)p.pt) + ((long long)c * p.Hv + kh * rep + hh) * (C * C) + j;
 #pragma unroll
         for (int i = 0; i < C; ++i) {
           float a0 = i == j ? 1.f : 0.f, a1 = 0.f, a2 = 0.f, a3 = 0.f;
@@ -375,57 +270,6 @@ struct FwdSmem {
   uint8_t uhi[DELTA ? C * NV * 2 : 16], ulo[DELTA ? C * NV * 2 : 16];   // U
   uint8_t dhi[C * NV * 2], dlo[C * NV * 2];                             // K's row factor x d x U
 };
-
-__device__ __forceinline__ float ex2_diff(const float* hd, int i, int j) {
-  return xb_ex2((hd[i] - hd[j]) + (hd[C + i] - hd[C + j]));
-}
-__device__ __forceinline__ float ex2_sum(const float* hd, int i) { return xb_ex2(hd[i]) * (1.f + 0.6931472f * hd[C + i]); }
-
-// state [DKP, NV]: warp w holds rows w * DKP / 4 .., as accumulators
-template <int DKP>
-__device__ __forceinline__ void state_to_smem(const float (&s)[DKP / 64][4][4], uint32_t hi, uint32_t lo) {
-  const int lane = xb_lane(), w = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-#pragma unroll
-  for (int m = 0; m < DKP / 64; ++m)
-#pragma unroll
-    for (int n = 0; n < 4; ++n)
-#pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
-        uint32_t a, b;
-        split2(s[m][n][2 * hh], s[m][n][2 * hh + 1], a, b);
-        const uint32_t off = at2<4>(w * (DKP / 4) + m * 16 + hh * 8 + g, n * 8 + 2 * t);
-        sts32(hi + off, a);
-        sts32(lo + off, b);
-      }
-}
-template <int DKP, bool STORE>
-__device__ __forceinline__ void state_global(float (&s)[DKP / 64][4][4], float* base, long long sk, long long sv, int dk, int cols) {
-  const int lane = xb_lane(), w = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-#pragma unroll
-  for (int m = 0; m < DKP / 64; ++m)
-#pragma unroll
-    for (int n = 0; n < 4; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int row = w * (DKP / 4) + m * 16 + (e >> 1) * 8 + g, col = n * 8 + 2 * t + (e & 1);
-        const bool ok = row < dk && col < cols;
-        if (STORE) {
-          if (ok) base[row * sk + col * sv] = s[m][n][e];
-        } else {
-          s[m][n][e] = ok ? base[row * sk + col * sv] : 0.f;
-        }
-      }
-}
-// the two bf16 planes of the state tile to global memory: [plane][DKP][dvp]
-template <int DKP>
-__device__ __forceinline__ void state_save(uint32_t hi, uint32_t lo, bf16* dst, int dvp, int v0) {
-#pragma unroll
-  for (int i = 0; i < DKP * 8 / 128; ++i) {
-    const int idx = i * 128 + threadIdx.x, plane = idx / (DKP * 4), r = (idx / 4) % DKP, u = idx & 3;
-    *reinterpret_cast<uint4*>(dst + ((long long)plane * DKP + r) * dvp + v0 + u * 8) =
-        lds128((plane ? lo : hi) + swz<4>(r, u));
-  }
-}
 
 template <int DKP, bool DELTA, bool SAVE>
 __global__ void __launch_bounds__(128) rec_fwd(const XbRecArgs p) {
@@ -520,7 +364,7 @@ __global__ void __launch_bounds__(128) rec_fwd(const XbRecArgs p) {
       __syncthreads();
       // U = T R, T lower triangular
       float u[4][4] = {};
-      const float* tm = p.tm + ch_h * (C * C);
+      const float* tm = ((float*)p.pt) + ch_h * (C * C);
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
         if (ks <= w) {
@@ -813,7 +657,7 @@ __global__ void __launch_bounds__(128) rec_bwd(const XbRecArgs p) {
       __syncthreads();
       // dR = T^T dU
       float dr[4][4] = {};
-      const float* tm = p.tm + ch_h * (C * C);
+      const float* tm = ((float*)p.pt) + ch_h * (C * C);
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
         if (ks >= w) {
@@ -1347,41 +1191,35 @@ __global__ void __launch_bounds__(128) rec_reduce(const XbRecArgs p) {
   }
 }
 
-template <typename K>
-int launch(K kernel, long long blocks, int threads, size_t smem, const XbRecArgs& a, cudaStream_t st) {
-  if (blocks <= 0) return 0;
-  if (blocks > 0x7fffffffLL) return -4;
-  if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
-    cudaGetLastError();
-    return -5;
-  }
-  kernel<<<(unsigned)blocks, threads, smem, st>>>(a);
-  return cudaGetLastError() == cudaSuccess ? 0 : -11;
-}
-
 bool bad_args(const XbRecArgs& a) {
   return a.T < 0 || a.n_docs < 0 || a.Hk <= 0 || a.Hv <= 0 || a.Hv % a.Hk || a.dk <= 0 || a.dk > 128 || a.dk % 8 || a.dv <= 0 ||
          a.dv % 8 || a.dvp != (a.dv + NV - 1) / NV * NV || a.nc_max < a.T / C + a.n_docs + 2;
 }
 
-template <int DKP, bool DELTA>
-int forward(const XbRecArgs& a, cudaStream_t st) {
-  const long long seq = (long long)(a.n_docs + 2) * a.Hv * (a.dvp / NV);
+int plan(const XbRecArgs& a, cudaStream_t st) {
   rec_plan<<<1, 1024, 0, st>>>(a.cu, a.n_docs, a.T, a.nc_max, (int4*)a.chunks, a.doc_off, xb_status_ptr());
-  if (cudaGetLastError() != cudaSuccess) return -11;
-  if (int rc = launch(rec_prep<DKP, DELTA>, (long long)a.nc_max * a.Hk, 128, sizeof(PrepSmem<DKP, DELTA>), a, st)) return rc;
-  return launch(rec_fwd<DKP, DELTA, false>, seq, 128, sizeof(FwdSmem<DKP, DELTA>), a, st);
+  return cudaGetLastError() == cudaSuccess ? 0 : -11;
 }
 
-template <int DKP, bool DELTA>
-int backward(const XbRecArgs& a, cudaStream_t st) {
+template <int DKP>
+int scan_fwd(const XbRecArgs& a, cudaStream_t st) {
+  const long long seq = (long long)(a.n_docs + 2) * a.Hv * (a.dvp / NV);
+  if (int rc = rec_launch(rec_prep<DKP, false>, (long long)a.nc_max * a.Hk, 128, sizeof(PrepSmem<DKP, false>), a, st)) return rc;
+  return rec_launch(rec_fwd<DKP, false, false>, seq, 128, sizeof(FwdSmem<DKP, false>), a, st);
+}
+
+template <int DKP>
+int scan_bwd(const XbRecArgs& a, cudaStream_t st) {
   const long long seq = (long long)(a.n_docs + 2) * a.Hv * (a.dvp / NV);
   XbRecArgs again = a;
   again.s_out = nullptr;
-  if (int rc = launch(rec_fwd<DKP, DELTA, true>, seq, 128, sizeof(FwdSmem<DKP, DELTA>), again, st)) return rc;
-  if (int rc = launch(rec_bwd<DKP, DELTA>, seq, 128, sizeof(BwdSmem<DKP, DELTA>), a, st)) return rc;
-  if (int rc = launch(rec_grad<DKP, DELTA>, (long long)a.nc_max * a.Hk, 256, sizeof(GradSmem<DKP, DELTA>), a, st)) return rc;
-  return DELTA ? 0 : launch(rec_reduce, a.Hv, 128, 0, a, st);
+  if (int rc = rec_launch(rec_fwd<DKP, false, true>, seq, 128, sizeof(FwdSmem<DKP, false>), again, st)) return rc;
+  return rec_launch(rec_bwd<DKP, false>, seq, 128, sizeof(BwdSmem<DKP, false>), a, st);
+}
+
+template <int DKP, bool DELTA>
+int grad(const XbRecArgs& a, cudaStream_t st) {
+  return rec_launch(rec_grad<DKP, DELTA>, (long long)a.nc_max * a.Hk, 256, sizeof(GradSmem<DKP, DELTA>), a, st);
 }
 
 }  // namespace
@@ -1391,13 +1229,19 @@ XB_API int xb_recurrence_chunk() { return C; }
 XB_API int xb_recurrence_fwd(const XbRecArgs* a, int delta, void* stream) {
   if (a == nullptr || bad_args(*a)) return -1;
   cudaStream_t st = (cudaStream_t)stream;
-  if (a->dk <= 64) return delta ? forward<64, true>(*a, st) : forward<64, false>(*a, st);
-  return delta ? forward<128, true>(*a, st) : forward<128, false>(*a, st);
+  if (int rc = plan(*a, st)) return rc;
+  if (delta) return xb_delta_fwd(*a, st);
+  return a->dk <= 64 ? scan_fwd<64>(*a, st) : scan_fwd<128>(*a, st);
 }
 
 XB_API int xb_recurrence_bwd(const XbRecArgs* a, int delta, void* stream) {
   if (a == nullptr || bad_args(*a)) return -1;
   cudaStream_t st = (cudaStream_t)stream;
-  if (a->dk <= 64) return delta ? backward<64, true>(*a, st) : backward<64, false>(*a, st);
-  return delta ? backward<128, true>(*a, st) : backward<128, false>(*a, st);
+  if (delta) {
+    if (int rc = xb_delta_bwd(*a, st)) return rc;
+    return a->dk <= 64 ? grad<64, true>(*a, st) : grad<128, true>(*a, st);
+  }
+  if (int rc = a->dk <= 64 ? scan_bwd<64>(*a, st) : scan_bwd<128>(*a, st)) return rc;
+  if (int rc = a->dk <= 64 ? grad<64, false>(*a, st) : grad<128, false>(*a, st)) return rc;
+  return rec_launch(rec_reduce, a->Hv, 128, 0, *a, st);
 }

@@ -25,8 +25,8 @@ struct XbRecArgs {
   int* doc_off;                  // [n_docs + 3]: first chunk of every document
   float* hd;                     // [nc_max, Hv, 192]
   float* rqk;                    // [nc_max, Hk, 128]
-  float *qk, *kk;                // [nc_max, Hk, 64, 64] (kk: delta rule only)
-  float* tm;                     // [nc_max, Hv, 64, 64] (delta rule only)
+  float *qk, *kk;                // [nc_max, Hk, 64, 64] (delta rule: for the backward pass, null without one)
+  void* pt;                      // [nc_max, Hv]: P and T in packed planes, 20480 bytes (delta rule only)
   void *s_planes, *ds_planes;    // bf16 [nc_max, Hv, 2, 64 or 128, dvp]
   void *u_planes, *dr_planes;    // bf16 [nc_max, Hv, 2, 64, dvp] (delta rule only)
   float* part;                   // [nc_max, Hv, 2] (scan only)

@@ -26,6 +26,7 @@ _launches = 0
 CHUNK = 64              # tokens of a chunk of the kernels (csrc/recurrence.cu)
 SLICE = 32              # columns of the state that one CTA carries
 MAX_STATE_ROWS = 128
+PACKED = 20480          # bytes of P and T of one chunk and head
 
 
 def launch_count() -> int:
@@ -41,7 +42,7 @@ class _Args(ctypes.Structure):
                 + [(n, ctypes.c_void_p) for n in ("A", "D", "cu", "s_in", "s_out", "ds_out", "ds_in")]
                 + [(n, ctypes.c_longlong) for n in ("s_k", "s_v")]
                 + [(n, ctypes.c_void_p) for n in ("o", "dq", "dk_out", "dv_out", "dg", "db", "dA", "dD", "chunks",
-                                                  "doc_off", "hd", "rqk", "qk", "kk", "tm", "s_planes", "ds_planes",
+                                                  "doc_off", "hd", "rqk", "qk", "kk", "pt", "s_planes", "ds_planes",
                                                   "u_planes", "dr_planes", "part")]
                 + [(n, ctypes.c_int) for n in ("T", "n_docs", "Hk", "Hv", "dk", "dv", "dvp", "nc_max", "l2norm")]
                 + [("scale", ctypes.c_float)])
@@ -63,7 +64,7 @@ def _pieces(sizes):
     return out, at
 
 
-def _fill(a: _Args, q, k, v, g, b, A, D, cu, s_in, ws, delta: bool, scale: float, l2norm: bool) -> torch.Tensor:
+def _fill(a: _Args, q, k, v, g, b, A, D, cu, s_in, ws, keep: bool, delta: bool, scale: float, l2norm: bool) -> torch.Tensor:
     """Inputs, sizes and the kept workspace (allocated if ``ws`` is None), which is returned."""
     T, Hk, dk = q.shape
     Hv, dv = v.shape[1], v.shape[2]
@@ -83,12 +84,18 @@ def _fill(a: _Args, q, k, v, g, b, A, D, cu, s_in, ws, delta: bool, scale: float
     a.nc_max = T // CHUNK + cu.numel() + 1
     a.l2norm, a.scale = int(l2norm), scale
     nc = a.nc_max
-    offs, total = _pieces([nc * 16, (cu.numel() + 2) * 4, nc * Hv * 3 * CHUNK * 4, nc * Hk * 2 * CHUNK * 4,
-                           nc * Hk * CHUNK * CHUNK * 4] + ([nc * Hk * CHUNK * CHUNK * 4, nc * Hv * CHUNK * CHUNK * 4]
-                                                           if delta else []))
+    sizes = [("chunks", nc * 16), ("doc_off", (cu.numel() + 2) * 4), ("hd", nc * Hv * 3 * CHUNK * 4),
+             ("rqk", nc * Hk * 2 * CHUNK * 4)]
+    if delta:
+        sizes.append(("pt", nc * Hv * PACKED))
+    if keep or not delta:
+        sizes.append(("qk", nc * Hk * CHUNK * CHUNK * 4))
+    if keep and delta:
+        sizes.append(("kk", nc * Hk * CHUNK * CHUNK * 4))
+    offs, total = _pieces([n for _, n in sizes])
     if ws is None:
         ws = torch.empty(total, dtype=torch.uint8, device=q.device)
-    for name, off in zip(("chunks", "doc_off", "hd", "rqk", "qk", "kk", "tm"), offs):
+    for (name, _), off in zip(sizes, offs):
         setattr(a, name, ws.data_ptr() + off)
     return ws
 
@@ -103,7 +110,7 @@ class _Recurrence(torch.autograd.Function):
         T, Hv, dv = v.shape
         a = _Args()
         with _lib.on_device(q):
-            ws = _fill(a, q, k, v, g, b, A, D, cu, s_in, None, delta, scale, l2norm)
+            ws = _fill(a, q, k, v, g, b, A, D, cu, s_in, None, any(ctx.needs_input_grad), delta, scale, l2norm)
             o = torch.empty((T, Hv, dv), dtype=v.dtype, device=v.device)
             shape = (cu.numel() - 1, Hv) + ((q.shape[2], dv) if delta else (dv, q.shape[2]))
             s_out = torch.empty(shape, dtype=torch.float32, device=v.device) if final else None
@@ -128,7 +135,7 @@ class _Recurrence(torch.autograd.Function):
         a = _Args()
         with _lib.on_device(q):
             dy = torch.zeros((T, Hv, dv), dtype=v.dtype, device=dev) if dy is None else _rows(dy)
-            _fill(a, q, k, v, g, b, A, D, cu, s_in, ws, delta, scale, l2norm)
+            _fill(a, q, k, v, g, b, A, D, cu, s_in, ws, True, delta, scale, l2norm)
             a.dy, a.dy_t, a.dy_h = dy.data_ptr(), dy.stride(0), dy.stride(1)
             ds_out = None if ds_out is None else ds_out.contiguous()
             ds_in = torch.empty_like(s_in) if ctx.needs_input_grad[7] else None
