@@ -1193,11 +1193,11 @@ __global__ void __launch_bounds__(128) rec_reduce(const XbRecArgs p) {
 
 bool bad_args(const XbRecArgs& a) {
   return a.T < 0 || a.n_docs < 0 || a.Hk <= 0 || a.Hv <= 0 || a.Hv % a.Hk || a.dk <= 0 || a.dk > 128 || a.dk % 8 || a.dv <= 0 ||
-         a.dv % 8 || a.dvp != (a.dv + NV - 1) / NV * NV || a.nc_max < a.T / C + a.n_docs + 2;
+         a.dv % 8 || a.dvp != (a.dv + NV - 1) / NV * NV || a.dkp != (a.dk <= 64 ? 64 : 128) || a.nc_max < a.T / C + a.n_docs + 2;
 }
 
 int plan(const XbRecArgs& a, cudaStream_t st) {
-  rec_plan<<<1, 1024, 0, st>>>(a.cu, a.n_docs, a.T, a.nc_max, (int4*)a.chunks, a.doc_off, xb_status_ptr());
+  rec_plan<<<1, 1024, 0, st>>>(a.cu, a.n_docs, a.T, a.nc_max, (int4*)a.chunks, a.doc_off, a.status);
   return cudaGetLastError() == cudaSuccess ? 0 : -11;
 }
 
@@ -1226,16 +1226,20 @@ int grad(const XbRecArgs& a, cudaStream_t st) {
 
 XB_API int xb_recurrence_chunk() { return C; }
 
-XB_API int xb_recurrence_fwd(const XbRecArgs* a, int delta, void* stream) {
-  if (a == nullptr || bad_args(*a)) return -1;
+XB_API int xb_recurrence_fwd(const XbRecArgs* args, int delta, void* stream) {
+  if (args == nullptr || bad_args(*args)) return -1;
+  XbRecArgs mine = *args, *a = &mine;
+  mine.status = xb_status_ptr();
   cudaStream_t st = (cudaStream_t)stream;
   if (int rc = plan(*a, st)) return rc;
   if (delta) return xb_delta_fwd(*a, st);
   return a->dk <= 64 ? scan_fwd<64>(*a, st) : scan_fwd<128>(*a, st);
 }
 
-XB_API int xb_recurrence_bwd(const XbRecArgs* a, int delta, void* stream) {
-  if (a == nullptr || bad_args(*a)) return -1;
+XB_API int xb_recurrence_bwd(const XbRecArgs* args, int delta, void* stream) {
+  if (args == nullptr || bad_args(*args)) return -1;
+  XbRecArgs mine = *args, *a = &mine;
+  mine.status = xb_status_ptr();
   cudaStream_t st = (cudaStream_t)stream;
   if (delta) {
     if (int rc = xb_delta_bwd(*a, st)) return rc;

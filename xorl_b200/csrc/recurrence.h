@@ -26,10 +26,11 @@ struct XbRecArgs {
   float* hd;                     // [nc_max, Hv, 192]
   float* rqk;                    // [nc_max, Hk, 128]
   float *qk, *kk;                // [nc_max, Hk, 64, 64] (delta rule: for the backward pass, null without one)
-  void* pt;                      // [nc_max, Hv]: P and T in packed planes, 20480 bytes (delta rule only)
+  void* pt;                      // [nc_max, Hv]: operand tile [T; P T], two planes, 32768 bytes (delta rule only)
   void *s_planes, *ds_planes;    // bf16 [nc_max, Hv, 2, 64 or 128, dvp]
   void *u_planes, *dr_planes;    // bf16 [nc_max, Hv, 2, 64, dvp] (delta rule only)
   float* part;                   // [nc_max, Hv, 2] (scan only)
-  int T, n_docs, Hk, Hv, dk, dv, dvp, nc_max, l2norm;
+  int* status;                   // filled in by the entry points
+  int T, n_docs, Hk, Hv, dk, dv, dkp, dvp, nc_max, l2norm;   // dkp: 64 or 128, dvp: a multiple of 32
   float scale;
 };

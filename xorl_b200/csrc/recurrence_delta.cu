@@ -3,26 +3,33 @@
 //
 // A chunk's chain  K S -> R -> U = T R -> S' = gamma S + K^T d U  is sequential, and with one long document there are
 // only heads x column slices of them (32 x 4 for 32 heads of 128), less than one per SM: the time of a step is what
-// counts.  So a CTA of eight warps carries 32 state columns; four warps run the chain, the other four what hangs on it
-// (forward: Q S and P U; backward: the state's own update).  Everything that depends on the chunk alone is made once,
-// by the prepare kernel, in the form that the products read: P = tril(D o Q K^T) and T = (I + L)^-1 as two bf16 parts
-// in blocks of 16 x 16, lower triangle only, so the chain has no exponentials, no splits of T and no loads that it
-// waits for.  mma.sync and not tcgen05: operands change hands between registers three times per step on 64 x 32 tiles,
-// and a round trip through tensor memory (commit, wait, load) costs more than the 100 to 500 cycles that such a
-// product takes on the register path.
+// counts.  A CTA carries 32 state columns through three products per step, all of them 128 rows high:
+//
+//   forward   [K; Q] S        -> R (rows of K), gamma Q S (rows of Q)
+//             [T; P T] R      -> U, and P U = (P T) R beside it
+//             K^T (d U)       -> added to the state, whose 128 rows live in the registers of 128 x 2 threads
+//   backward  [K; .] dS'      -> Y = d K dS'
+//             [T; P T]^T [Y; dO] -> dR = T^T (Y + P^T dO)
+//             [K; Q]^T [-b gamma dR; gamma dO] -> added to dS  (the dO part is issued early)
+//
+// A computed operand enters as two bf16 parts side by side, [hi | lo], 64 columns of one product; the parts of T and
+// P T are two products into the same accumulator.  P = tril(D o Q K^T), T = (I + L)^-1 and P T depend on the chunk
+// alone and come from the prepare kernel as operand tiles.  Eight warps work on the accumulators, one row and 16
+// columns per thread (row factors are scalars there); a ninth issues the loads and the products.  mma.sync spent 5800
+// cycles on a forward step (1100 of them on cp.async, 2300 in the tensor pipe): 789 us for 16384 tokens of 32 heads.
 #include "recurrence_core.cuh"
 
 namespace {
 
-constexpr int BLK = 512;                    // bytes of a 16 x 16 bf16 block: four 8 x 8 matrices in fragment order
-constexpr int TRI = 10 * 2 * BLK;           // lower triangle of a 64 x 64 matrix, two planes
-__device__ __forceinline__ int blk_of(int rb, int cb) { return (rb * (rb + 1) / 2 + cb) * 2 * BLK; }
-// A fragment of a block, and of its transpose
-__device__ __forceinline__ uint32_t addr_blk(int l) { return (uint32_t)l * 16u; }
-__device__ __forceinline__ uint32_t addr_blk_t(int l) { return (uint32_t)((l & 7) + ((l >> 3) & 1) * 16 + (l >> 4) * 8) * 16u; }
-
-__device__ __forceinline__ void bar(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
-__device__ __forceinline__ void bar_arrive(int id, int n) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(n) : "memory"); }
+// named barriers want whole warps
+__device__ __forceinline__ void bar(int id, int n) {
+  __syncwarp();
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(int id, int n) {
+  __syncwarp();
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(n) : "memory");
+}
 
 // ---- prepare -----------------------------------------------------------------------------------------------------
 constexpr int LS = 72;                      // row stride of L: rows of a fragment fall into different banks
@@ -36,6 +43,23 @@ struct DPrepSmem {
   float hd[2][3][C];
   float rq[C], rk[C];
 };
+
+// 64 x 64 values per head to rows 64 * part .. of its operand tile: two planes of [128 rows][128 bytes] whose 16-byte
+// units are swizzled as the tensor core reads them
+constexpr int TP_PLANE = 128 * 128;
+__device__ __forceinline__ void put_tile(const XbRecArgs& p, const float (&l)[2][C * LS], int part, int c, int h, int heads) {
+  for (int it = threadIdx.x; it < 2 * C * 8; it += 128) {
+    const int mm = it / (C * 8), r = (it >> 3) % C, u = it & 7;
+    if (mm >= heads) break;
+    const float4* src = reinterpret_cast<const float4*>(&l[mm][r * LS + u * 8]);
+    const float4 a = src[0], b = src[1];
+    uint4 hi, lo;
+    split2(a.x, a.y, hi.x, lo.x), split2(a.z, a.w, hi.y, lo.y), split2(b.x, b.y, hi.z, lo.z), split2(b.z, b.w, hi.w, lo.w);
+    uint8_t* dst = (uint8_t*)p.pt + ((long long)c * p.Hv + h + mm) * (2 * TP_PLANE) + (part * C + r) * 128 + ((u ^ (r & 7)) << 4);
+    *reinterpret_cast<uint4*>(dst) = hi;
+    *reinterpret_cast<uint4*>(dst + TP_PLANE) = lo;
+  }
+}
 
 // x = column j of (I + L)^-1, whose first FROM rows are zero
 template <int FROM>
@@ -176,7 +200,6 @@ __global__ void __launch_bounds__(128, 3) delta_prep(const XbRecArgs p) {
     for (int m = 0; m < 2; ++m) {
       if (h0 + m >= rep) break;
       const float* hd = sm.hd[m][0];
-      uint8_t* pl = (uint8_t*)p.pt + ((long long)c * p.Hv + kh * rep + h0 + m) * (2 * TRI);
 #pragma unroll
       for (int nt = 0; nt < 8; ++nt) {
         if (nt > 2 * w + 1) break;
@@ -184,13 +207,8 @@ __global__ void __launch_bounds__(128, 3) delta_prep(const XbRecArgs p) {
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
           const int row = r0 + hh * 8;
-          const float2 x = sm.qk[(nt * 2 + hh) * 128 + tid], y = sm.kk[(nt * 2 + hh) * 128 + tid];
+          const float2 y = sm.kk[(nt * 2 + hh) * 128 + tid];
           const float d0 = ex2_diff(hd, row, col), d1 = ex2_diff(hd, row, col + 1), b = hd[2 * C + row];
-          uint32_t hi, lo;
-          split2(col <= row ? d0 * x.x : 0.f, col + 1 <= row ? d1 * x.y : 0.f, hi, lo);
-          uint32_t* dst = reinterpret_cast<uint32_t*>(pl + blk_of(w, nt >> 1) + (hh + 2 * (nt & 1)) * 128 + g * 16 + t * 4);
-          dst[0] = hi;
-          dst[BLK / 4] = lo;
           *reinterpret_cast<float2*>(&sm.l[m][row * LS + col]) =
               make_float2(col < row ? b * d0 * y.x : 0.f, col + 1 < row ? b * d1 * y.y : 0.f);
         }
@@ -211,434 +229,553 @@ __global__ void __launch_bounds__(128, 3) delta_prep(const XbRecArgs p) {
       for (int i = 0; i < C; ++i) sm.l[m][i * LS + j] = x[i];
     }
     __syncthreads();
-    for (int it = tid; it < 2 * 320; it += 128) {
-      const int mm = it / 320, e = it % 320, blk = e >> 5, mat = (e >> 3) & 3, r = e & 7;
+    put_tile(p, sm.l, 0, c, kh * rep + h0, rep - h0);
+    // P T, this warp's 16 rows: P from the fragments of Q K^T, T from shared memory
+    float pt[2][8][4] = {};
+#pragma unroll
+    for (int mm = 0; mm < 2; ++mm) {
       if (h0 + mm >= rep) break;
-      const int rb = blk < 1 ? 0 : blk < 3 ? 1 : blk < 6 ? 2 : 3, cb = blk - rb * (rb + 1) / 2;
-      const float4* src = reinterpret_cast<const float4*>(&sm.l[mm][(rb * 16 + (mat & 1) * 8 + r) * LS + cb * 16 + (mat >> 1) * 8]);
-      const float4 a = src[0], b = src[1];
-      uint4 hi, lo;
-      split2(a.x, a.y, hi.x, lo.x), split2(a.z, a.w, hi.y, lo.y), split2(b.x, b.y, hi.z, lo.z), split2(b.z, b.w, hi.w, lo.w);
-      uint8_t* dst = (uint8_t*)p.pt + ((long long)c * p.Hv + kh * rep + h0 + mm) * (2 * TRI) + TRI + blk * 2 * BLK + mat * 128 + r * 16;
-      *reinterpret_cast<uint4*>(dst) = hi;
-      *reinterpret_cast<uint4*>(dst + BLK) = lo;
-    }
-  }
-}
-
-// ---- what a step reads ---------------------------------------------------------------------------------------------
-template <int DKP>
-struct DStage {
-  uint8_t q[C * DKP * 2], k[C * DKP * 2], x[C * NV * 2];      // x: v, or dO
-  uint8_t pt[2 * TRI];                                        // P, T
-  float hd[HD], rqk[RQK];
-};
-template <int THREADS>
-__device__ __forceinline__ void load_bytes(uint32_t dst, const uint8_t* src, int n) {
-  for (int i = threadIdx.x; i < n / 16; i += THREADS) cp16(dst + i * 16, src + i * 16, true);
-}
-template <int DKP, int THREADS, bool Q, bool P>
-__device__ __forceinline__ void fetch_stage(const XbRecArgs& p, DStage<DKP>& st, const int4 ch, int c, int h, int kh, const bf16* x,
-                                            long long x_t, int vcols) {
-  constexpr int U = DKP / 8;
-  load_tile<U, C, THREADS>(xb_smem_u32(st.k), (const bf16*)p.k + ch.x * p.k_t + kh * p.k_h, p.k_t, ch.y, p.dk);
-  if (Q) load_tile<U, C, THREADS>(xb_smem_u32(st.q), (const bf16*)p.q + ch.x * p.q_t + kh * p.q_h, p.q_t, ch.y, p.dk);
-  load_tile<4, C, THREADS>(xb_smem_u32(st.x), x, x_t, ch.y, vcols);
-  const uint8_t* pt = (const uint8_t*)p.pt + ((long long)c * p.Hv + h) * (2 * TRI);
-  load_bytes<THREADS>(xb_smem_u32(st.pt) + (P ? 0 : TRI), pt + (P ? 0 : TRI), P ? 2 * TRI : TRI);
-  load_floats<THREADS>(xb_smem_u32(st.hd), p.hd + ((long long)c * p.Hv + h) * HD, HD);
-  load_floats<THREADS>(xb_smem_u32(st.rqk), p.rqk + ((long long)c * p.Hk + kh) * RQK, RQK);
-}
-
-// B fragments of two planes of a [rows][NV] tile: 16 rows, all four column tiles
-struct BFrag { uint32_t h[2][4], l[2][4]; };
-__device__ __forceinline__ void load_b(BFrag& b, uint32_t hi, uint32_t lo, int k0) {
-#pragma unroll
-  for (int n = 0; n < 2; ++n) {
-    ldsm4t(b.h[n], hi + addr_bt<4>(k0, n * 16));
-    ldsm4t(b.l[n], lo + addr_bt<4>(k0, n * 16));
-  }
-}
-__device__ __forceinline__ void mma2(float (&d)[4][4], const uint32_t (&a)[4], const BFrag& b) {          // a exact
-#pragma unroll
-  for (int n = 0; n < 4; ++n) mma(d[n], a, b.l[n >> 1][(n & 1) * 2], b.l[n >> 1][(n & 1) * 2 + 1]);
-#pragma unroll
-  for (int n = 0; n < 4; ++n) mma(d[n], a, b.h[n >> 1][(n & 1) * 2], b.h[n >> 1][(n & 1) * 2 + 1]);
-}
-__device__ __forceinline__ void mma3(float (&d)[4][4], const uint32_t (&ah)[4], const uint32_t (&al)[4], const BFrag& b) {
-#pragma unroll
-  for (int n = 0; n < 4; ++n) mma(d[n], al, b.h[n >> 1][(n & 1) * 2], b.h[n >> 1][(n & 1) * 2 + 1]);
-  mma2(d, ah, b);
-}
-// 64 x 32 accumulators, scaled by row, to two planes
-__device__ __forceinline__ void put_planes(const float (&d)[4][4], float f0, float f1, uint32_t hi, uint32_t lo, int row0, int t) {
-#pragma unroll
-  for (int hh = 0; hh < 2; ++hh)
-#pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      const uint32_t off = at2<4>(row0 + hh * 8, n * 8 + 2 * t);
-      const float f = hh ? f1 : f0;
-      uint32_t a, b;
-      split2(f * d[n][2 * hh], f * d[n][2 * hh + 1], a, b);
-      sts32(hi + off, a);
-      sts32(lo + off, b);
-    }
-}
-
-// ---- forward -------------------------------------------------------------------------------------------------------
-template <int DKP>
-struct DFwdSmem {
-  DStage<DKP> st[2];
-  uint8_t s[2][2][DKP * NV * 2];            // the state's planes, this chunk's and the next one's
-  uint8_t r[2][C * NV * 2], u[2][C * NV * 2], d[2][C * NV * 2];
-};
-
-template <int DKP, bool SAVE>
-__global__ void __launch_bounds__(SAVE ? 128 : 256, 1) delta_fwd(const XbRecArgs p) {
-  extern __shared__ __align__(128) uint8_t smem_raw[];
-  DFwdSmem<DKP>& sm = *reinterpret_cast<DFwdSmem<DKP>*>(smem_raw);
-  constexpr int U = DKP / 8, THREADS = SAVE ? 128 : 256;
-  const int slices = p.dvp / NV, rep = p.Hv / p.Hk;
-  const int sl = blockIdx.x % slices, h = (blockIdx.x / slices) % p.Hv, doc = blockIdx.x / (slices * p.Hv);
-  const int kh = h / rep, v0 = sl * NV, vcols = min(NV, p.dv - v0);
-  const int lane = xb_lane(), warp = threadIdx.x >> 5, w = warp & 3, g = lane >> 2, t = lane & 3, ra = w * 16 + g;
-  const int c0 = p.doc_off[doc], c1 = p.doc_off[doc + 1];
-  const int4* chunks = reinterpret_cast<const int4*>(p.chunks);
-  bf16* o = (bf16*)p.o + (long long)h * p.dv + v0;
-  const long long o_t = (long long)p.Hv * p.dv;
-  if (doc >= p.n_docs) {                                             // rows outside the documents
-    if (!SAVE)
-      for (int c = c0; c < c1; ++c)
-        for (int i = threadIdx.x; i < chunks[c].y * NV; i += THREADS)
-          if (i % NV < vcols) o[(chunks[c].x + i / NV) * o_t + i % NV] = __float2bfloat16(0.f);
-    return;
-  }
-  float s[DKP / 64][4][4] = {};
-  const long long soff = ((long long)doc * p.Hv + h) * p.dk * p.dv + v0 * p.s_v;
-  auto fetch = [&](int c, int b) {
-    const int4 ch = chunks[c];
-    fetch_stage<DKP, THREADS, !SAVE, !SAVE>(p, sm.st[b], ch, c, h, kh, (const bf16*)p.v + ch.x * p.v_t + h * p.v_h + v0, p.v_t, vcols);
-  };
-  if (c0 < c1) fetch(c0, 0);
-  cp_commit();
-  if (warp < 4) {
-    if (p.s_in != nullptr) state_global<DKP, false>(s, const_cast<float*>(p.s_in) + soff, p.s_k, p.s_v, p.dk, vcols);
-    state_to_smem<DKP>(s, xb_smem_u32(sm.s[0][0]), xb_smem_u32(sm.s[0][1]));
-  }
-  for (int c = c0; c < c1; ++c) {
-    const int par = (c - c0) & 1;
-    DStage<DKP>& st = sm.st[par];
-    const uint32_t sk = xb_smem_u32(st.k), sq = xb_smem_u32(st.q), sv = xb_smem_u32(st.x), spt = xb_smem_u32(st.pt);
-    const uint32_t shi = xb_smem_u32(sm.s[par][0]), slo = xb_smem_u32(sm.s[par][1]);
-    const uint32_t uhi = xb_smem_u32(sm.u[0]), ulo = xb_smem_u32(sm.u[1]);
-    cp_wait<0>();
-    __syncthreads();                       // this chunk's tiles and the state's planes are complete
-    if (c + 1 < c1) fetch(c + 1, par ^ 1);
-    cp_commit();
-    const long long ch_h = (long long)c * p.Hv + h;
-    if (warp < 4) {
-      if (SAVE) state_save<DKP>(shi, slo, (bf16*)p.s_planes + ch_h * 2 * DKP * p.dvp, p.dvp, v0);
-      float acc[4][4] = {};
-#pragma unroll
-      for (int ks = 0; ks < DKP / 16; ++ks) {
-        uint32_t fk[4];
-        BFrag b;
-        ldsm4(fk, sk + addr_a<U>(w * 16, ks * 16));
-        load_b(b, shi, slo, ks * 16);
-        mma2(acc, fk, b);
-      }
-      // R = b (V - gamma rk K S)
-      const uint32_t rhi = xb_smem_u32(sm.r[0]), rlo = xb_smem_u32(sm.r[1]);
-#pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
-        const int row = ra + hh * 8;
-        const float b = st.hd[2 * C + row], f = ex2_sum(st.hd, row) * st.rqk[C + row];
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const uint32_t off = at2<4>(row, n * 8 + 2 * t);
-          const float2 v = unpack_bf16x2(lds32(sv + off));
-          uint32_t hi, lo;
-          split2(b * (v.x - f * acc[n][2 * hh]), b * (v.y - f * acc[n][2 * hh + 1]), hi, lo);
-          sts32(rhi + off, hi);
-          sts32(rlo + off, lo);
-        }
-      }
-      bar(1, 128);
-      // U = T R
-      float u[4][4] = {};
+      const float* hd = sm.hd[mm][0];
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
-        if (ks <= w) {
-          uint32_t ah[4], al[4];
-          BFrag b;
-          ldsm4(ah, spt + TRI + blk_of(w, ks) + addr_blk(lane));
-          ldsm4(al, spt + TRI + blk_of(w, ks) + BLK + addr_blk(lane));
-          load_b(b, rhi, rlo, ks * 16);
-          mma3(u, ah, al, b);
+        if (ks > w) break;
+        uint32_t ah[4], al[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int row = r0 + (e & 1) * 8, col = ks * 16 + (e >> 1) * 8 + 2 * t;
+          const float2 x = sm.qk[((ks * 2 + (e >> 1)) * 2 + (e & 1)) * 128 + tid];
+          split2(col <= row ? ex2_diff(hd, row, col) * x.x : 0.f, col + 1 <= row ? ex2_diff(hd, row, col + 1) * x.y : 0.f, ah[e], al[e]);
+        }
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+          if (n > 2 * ks + 1) break;
+          const float* T = &sm.l[mm][(ks * 16 + 2 * t) * LS + n * 8 + g];
+          uint32_t bh[2], bl[2];
+          split2(T[0], T[LS], bh[0], bl[0]);
+          split2(T[8 * LS], T[9 * LS], bh[1], bl[1]);
+          mma(pt[mm][n], al, bh[0], bh[1]);
+          mma(pt[mm][n], ah, bl[0], bl[1]);
+          mma(pt[mm][n], ah, bh[0], bh[1]);
         }
       }
-      const uint32_t dhi = xb_smem_u32(sm.d[0]), dlo = xb_smem_u32(sm.d[1]);
-      if (SAVE) {
+    }
+    __syncthreads();
+#pragma unroll
+    for (int mm = 0; mm < 2; ++mm)
+#pragma unroll
+      for (int n = 0; n < 8; ++n)
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh)
-#pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            uint32_t* pl = reinterpret_cast<uint32_t*>((bf16*)p.u_planes + (ch_h * 2 * C + ra + hh * 8) * p.dvp + v0 + n * 8 + 2 * t);
-            split2(u[n][2 * hh], u[n][2 * hh + 1], pl[0], pl[C * p.dvp / 2]);
-          }
-      } else {
-        put_planes(u, 1.f, 1.f, uhi, ulo, ra, t);
-        bar_arrive(3, 256);                // the output warps may read U
-      }
-      put_planes(u, ex2_diff(st.hd, C - 1, ra) * st.rqk[C + ra], ex2_diff(st.hd, C - 1, ra + 8) * st.rqk[C + ra + 8], dhi, dlo, ra, t);
-      const float f = ex2_sum(st.hd, C - 1);
-#pragma unroll
-      for (int m = 0; m < DKP / 64; ++m)
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[m][n][e] *= f;
-      bar(2, 128);
-      // S = gamma_last S + K^T (rk d U)
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        BFrag b;
-        load_b(b, dhi, dlo, ks * 16);
-#pragma unroll
-        for (int m = 0; m < DKP / 64; ++m) {
-          uint32_t fa[4];
-          ldsm4t(fa, sk + addr_at<U>(w * (DKP / 4) + m * 16, ks * 16));
-          mma2(s[m], fa, b);
-        }
-      }
-      state_to_smem<DKP>(s, xb_smem_u32(sm.s[par ^ 1][0]), xb_smem_u32(sm.s[par ^ 1][1]));
-    } else {
-      // O = gamma rq Q S + P U
-      const int4 ch = chunks[c];
-      float acc[4][4] = {};
-#pragma unroll
-      for (int ks = 0; ks < DKP / 16; ++ks) {
-        uint32_t fq[4];
-        BFrag b;
-        ldsm4(fq, sq + addr_a<U>(w * 16, ks * 16));
-        load_b(b, shi, slo, ks * 16);
-        mma2(acc, fq, b);
-      }
-#pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
-        const float f = ex2_sum(st.hd, ra + hh * 8) * st.rqk[ra + hh * 8];
-#pragma unroll
-        for (int n = 0; n < 4; ++n) acc[n][2 * hh] *= f, acc[n][2 * hh + 1] *= f;
-      }
-      bar(3, 256);
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        if (ks <= w) {
-          uint32_t ah[4], al[4];
-          BFrag b;
-          ldsm4(ah, spt + blk_of(w, ks) + addr_blk(lane));
-          ldsm4(al, spt + blk_of(w, ks) + BLK + addr_blk(lane));
-          load_b(b, uhi, ulo, ks * 16);
-          mma3(acc, ah, al, b);
-        }
-      }
-#pragma unroll
-      for (int hh = 0; hh < 2; ++hh)
-        if (ra + hh * 8 < ch.y)
-#pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            const int col = n * 8 + 2 * t;
-            if (col < vcols)
-              *reinterpret_cast<uint32_t*>(o + (ch.x + ra + hh * 8) * o_t + col) = pack_bf16x2(acc[n][2 * hh], acc[n][2 * hh + 1]);
-          }
-    }
+          *reinterpret_cast<float2*>(&sm.l[mm][(r0 + hh * 8) * LS + n * 8 + 2 * t]) = make_float2(pt[mm][n][2 * hh], pt[mm][n][2 * hh + 1]);
+    __syncthreads();
+    put_tile(p, sm.l, 1, c, kh * rep + h0, rep - h0);
   }
-  cp_wait<0>();
-  if (warp < 4 && p.s_out != nullptr) state_global<DKP, true>(s, p.s_out + soff, p.s_k, p.s_v, p.dk, vcols);
 }
 
-// ---- backward, sequential part: dS through one document, last chunk first -----------------------------------------
-template <int DKP>
-struct DBwdSmem {
-  DStage<DKP> st[2];
-  uint8_t s[2][DKP * NV * 2];               // dS'
-  uint8_t u[2][C * NV * 2];                 // dU
-  uint8_t x[2][C * NV * 2], y[2][C * NV * 2];   // -b gamma rk dR, gamma rq dO
+// ---- the step of both directions ------------------------------------------------------------------------------------
+constexpr int HALF = 128 * 128;             // [128 rows][64 bf16]: K rows 0 .. 63, Q rows 64 .. 127
+constexpr int ST_KQ = 0, ST_TP = 2 * HALF, ST_X = ST_TP + 2 * TP_PLANE, ST_HD = ST_X + C * NV * 2, ST_RQK = ST_HD + HD * 4;
+constexpr int STAGE = (ST_RQK + RQK * 4 + 1023) / 1024 * 1024;
+constexpr int STAGE_BYTES = ST_RQK + RQK * 4;      // what the loads bring, boxes outside a tensor included
+constexpr int SM_S = 2 * STAGE, SM_B2 = SM_S + HALF, SM_B3 = SM_B2 + HALF, SM_BAR = SM_B3 + HALF;
+constexpr int SMEM = SM_BAR + 128 + 1024;
+constexpr int WORKERS = 256, THREADS = WORKERS + 32;
+constexpr int TMEM_COLS = 256, D1 = 0, D2 = 64, D3 = 128;     // accumulators, 64 columns each
+
+struct __align__(8) Bars {
+  uint64_t full[2], done[3];
+  uint32_t tmem;
+  int abort_flag;
+};
+static_assert(sizeof(Bars) <= 128, "barriers");
+
+// What every thread of a step knows.
+struct Cta {
+  uint8_t* smem;
+  Bars* bars;
+  uint32_t tmem;
+  int h, kh, doc, v0, vcols, c0, c1;
+  int* status;
+  __device__ void wait1(uint64_t* b, uint32_t parity, int detail) {         // one thread
+    mbar_wait(b, parity, &bars->abort_flag, status, XB_K_RECURRENCE, detail);
+  }
+  __device__ void wait(uint64_t* b, uint32_t parity, int detail) {          // a whole warp: what follows is collective
+    wait1(b, parity, detail);
+    __syncwarp();
+  }
 };
 
-template <int DKP>
-__global__ void __launch_bounds__(256, 1) delta_bwd(const XbRecArgs p) {
-  extern __shared__ __align__(128) uint8_t smem_raw[];
-  DBwdSmem<DKP>& sm = *reinterpret_cast<DBwdSmem<DKP>*>(smem_raw);
-  constexpr int U = DKP / 8;
-  const int slices = p.dvp / NV, rep = p.Hv / p.Hk;
-  const int sl = blockIdx.x % slices, h = (blockIdx.x / slices) % p.Hv, doc = blockIdx.x / (slices * p.Hv);
-  const int kh = h / rep, v0 = sl * NV, vcols = min(NV, p.dv - v0);
-  const int lane = xb_lane(), warp = threadIdx.x >> 5, w = warp & 3, g = lane >> 2, t = lane & 3, ra = w * 16 + g;
-  const int c0 = p.doc_off[doc], c1 = p.doc_off[doc + 1];
-  const int4* chunks = reinterpret_cast<const int4*>(p.chunks);
-  bf16* dv = (bf16*)p.dv_out + (long long)h * p.dv + v0;
-  const long long dv_t = (long long)p.Hv * p.dv;
-  if (doc >= p.n_docs) {
-    for (int c = c0; c < c1; ++c)
-      for (int i = threadIdx.x; i < chunks[c].y * NV; i += 256)
-        if (i % NV < vcols) dv[(chunks[c].x + i / NV) * dv_t + i % NV] = __float2bfloat16(0.f);
-    return;
+// The loads of one chunk, by one thread.
+__device__ __forceinline__ void load_stage(const XbRecArgs& p, const Cta& a, const CUtensorMap* mk, const CUtensorMap* mq,
+                                           const CUtensorMap* mx, int c, int s) {
+  uint8_t* st = a.smem + s * STAGE;
+  uint64_t* full = &a.bars->full[s];
+  const int t0 = reinterpret_cast<const int4*>(p.chunks)[c].x;
+  mbar_expect_tx(full, STAGE_BYTES);
+  for (int i = 0; i < 2; ++i) {
+    tma_load_3d(st + ST_KQ + i * HALF, mk, full, i * 64, a.kh, t0);
+    tma_load_3d(st + ST_KQ + i * HALF + HALF / 2, mq, full, i * 64, a.kh, t0);
   }
-  float s[DKP / 64][4][4] = {};             // warps 4 .. 7: the state's gradient
-  const long long soff = ((long long)doc * p.Hv + h) * p.dk * p.dv + v0 * p.s_v;
-  auto fetch = [&](int c, int b) {
-    const int4 ch = chunks[c];
-    fetch_stage<DKP, 256, true, true>(p, sm.st[b], ch, c, h, kh, (const bf16*)p.dy + ch.x * p.dy_t + h * p.dy_h + v0, p.dy_t, vcols);
-  };
-  if (c0 < c1) fetch(c1 - 1, 0);
-  cp_commit();
-  const uint32_t shi = xb_smem_u32(sm.s[0]), slo = xb_smem_u32(sm.s[1]), xhi = xb_smem_u32(sm.x[0]), xlo = xb_smem_u32(sm.x[1]);
-  if (warp >= 4) {
-    if (p.ds_out != nullptr) state_global<DKP, false>(s, const_cast<float*>(p.ds_out) + soff, p.s_k, p.s_v, p.dk, vcols);
-    state_to_smem<DKP>(s, shi, slo);
+  tma_load_3d(st + ST_X, mx, full, a.v0, a.h, t0);
+  bulk_load(st + ST_TP, (const uint8_t*)p.pt + ((long long)c * p.Hv + a.h) * (2 * TP_PLANE), 2 * TP_PLANE, full);
+  bulk_load(st + ST_HD, p.hd + ((long long)c * p.Hv + a.h) * HD, HD * 4, full);
+  bulk_load(st + ST_RQK, p.rqk + ((long long)c * p.Hk + a.kh) * RQK, RQK * 4, full);
+}
+
+// Rows of K and Q behind the document's end: they hold the next document's, and 0 x Inf is NaN.
+__device__ __forceinline__ void clear_rows(uint8_t* st, int len) {
+  const int n = (C - len) * 8;
+  for (int i = threadIdx.x; i < 4 * n; i += WORKERS) {
+    const int part = i / n, r = len + (i % n) / 8;
+    reinterpret_cast<uint4*>(st + ST_KQ + part * (HALF / 2) + r * 128)[i & 7] = make_uint4(0, 0, 0, 0);
   }
-  for (int c = c1 - 1; c >= c0; --c) {
-    DStage<DKP>& st = sm.st[(c1 - 1 - c) & 1];
-    const int4 ch = chunks[c];
-    const uint32_t sk = xb_smem_u32(st.k), sq = xb_smem_u32(st.q), sy = xb_smem_u32(st.x), spt = xb_smem_u32(st.pt);
-    cp_wait<0>();
-    __syncthreads();
-    if (c > c0) fetch(c - 1, (c1 - c) & 1);
-    cp_commit();
-    const long long ch_h = (long long)c * p.Hv + h;
-    if (warp < 4) {
-      // dU = d rk K dS' + P^T dO
-      float du[4][4] = {};
+}
+
+// 16 values of a row as [hi | lo] of a [rows][128 bytes] operand tile; columns 16 * half ..
+__device__ __forceinline__ void put_row(uint8_t* tile, int row, int half, const float (&x)[16], uint32_t (&hi)[8], uint32_t (&lo)[8]) {
 #pragma unroll
-      for (int ks = 0; ks < DKP / 16; ++ks) {
-        uint32_t fk[4];
-        BFrag b;
-        ldsm4(fk, sk + addr_a<U>(w * 16, ks * 16));
-        load_b(b, shi, slo, ks * 16);
-        mma2(du, fk, b);
-      }
+  for (int i = 0; i < 8; ++i) split2(x[2 * i], x[2 * i + 1], hi[i], lo[i]);
+  uint8_t* r = tile + row * 128;
 #pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
-        const float f = ex2_diff(st.hd, C - 1, ra + hh * 8) * st.rqk[C + ra + hh * 8];
+  for (int i = 0; i < 2; ++i) {
+    const int u = half * 2 + i;
+    *reinterpret_cast<uint4*>(r + ((u ^ (row & 7)) << 4)) = make_uint4(hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
+    *reinterpret_cast<uint4*>(r + (((u + 4) ^ (row & 7)) << 4)) = make_uint4(lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
+  }
+}
+__device__ __forceinline__ void store16(bf16* dst, const uint32_t (&v)[8]) {
+  reinterpret_cast<uint4*>(dst)[0] = make_uint4(v[0], v[1], v[2], v[3]);
+  reinterpret_cast<uint4*>(dst)[1] = make_uint4(v[4], v[5], v[6], v[7]);
+}
+// the sum of an accumulator's two halves, 16 columns of this thread's row
+__device__ __forceinline__ void read_acc(uint32_t addr, float (&x)[16]) {
+  uint32_t a[16], b[16];
+  tmem_ld_32x16(addr, a);
+  tmem_ld_32x16(addr + 32, b);
+  tc_wait_ld();
 #pragma unroll
-        for (int n = 0; n < 4; ++n) du[n][2 * hh] *= f, du[n][2 * hh + 1] *= f;
-      }
+  for (int i = 0; i < 16; ++i) x[i] = __uint_as_float(a[i]) + __uint_as_float(b[i]);
+}
+// 16 bf16 values of a row of the [64][64 bytes] tile of v or dO
+__device__ __forceinline__ void read_x(const uint8_t* tile, int row, int half, bool on, uint4 (&v)[2]) {
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        if (ks >= w) {
-          uint32_t ah[4], al[4], by[2][4];
-          ldsm4t(ah, spt + blk_of(ks, w) + addr_blk_t(lane));
-          ldsm4t(al, spt + blk_of(ks, w) + BLK + addr_blk_t(lane));
+  for (int i = 0; i < 2; ++i)
+    v[i] = on ? *reinterpret_cast<const uint4*>(tile + swz<4>(row, half * 2 + i)) : make_uint4(0, 0, 0, 0);
+}
+__device__ __forceinline__ void floats(const uint4 (&v)[2], float (&x)[16]) {
 #pragma unroll
-          for (int n = 0; n < 2; ++n) ldsm4t(by[n], sy + addr_bt<4>(ks * 16, n * 16));
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
-          for (int n = 0; n < 4; ++n) mma(du[n], al, by[n >> 1][(n & 1) * 2], by[n >> 1][(n & 1) * 2 + 1]);
-#pragma unroll
-          for (int n = 0; n < 4; ++n) mma(du[n], ah, by[n >> 1][(n & 1) * 2], by[n >> 1][(n & 1) * 2 + 1]);
-        }
-      }
-      const uint32_t uhi = xb_smem_u32(sm.u[0]), ulo = xb_smem_u32(sm.u[1]);
-      put_planes(du, 1.f, 1.f, uhi, ulo, ra, t);
-      bar(1, 128);
-      // dR = T^T dU
-      float dr[4][4] = {};
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        if (ks >= w) {
-          uint32_t ah[4], al[4];
-          BFrag b;
-          ldsm4t(ah, spt + TRI + blk_of(ks, w) + addr_blk_t(lane));
-          ldsm4t(al, spt + TRI + blk_of(ks, w) + BLK + addr_blk_t(lane));
-          load_b(b, uhi, ulo, ks * 16);
-          mma3(dr, ah, al, b);
-        }
-      }
-      const float b0 = st.hd[2 * C + ra], b1 = st.hd[2 * C + ra + 8];
-      put_planes(dr, -b0 * ex2_sum(st.hd, ra) * st.rqk[C + ra], -b1 * ex2_sum(st.hd, ra + 8) * st.rqk[C + ra + 8], xhi, xlo, ra, t);
-      bar_arrive(2, 256);
-#pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
-        const int row = ra + hh * 8;
-        const float b = hh ? b1 : b0;
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const int col = n * 8 + 2 * t;
-          const float y0 = dr[n][2 * hh], y1 = dr[n][2 * hh + 1];
-          uint32_t* pl = reinterpret_cast<uint32_t*>((bf16*)p.dr_planes + (ch_h * 2 * C + row) * p.dvp + v0 + col);
-          split2(y0, y1, pl[0], pl[C * p.dvp / 2]);
-          if (row < ch.y && col < vcols) *reinterpret_cast<uint32_t*>(dv + (ch.x + row) * dv_t + col) = pack_bf16x2(b * y0, b * y1);
-        }
-      }
-    } else {
-      // dS = gamma_last dS' + Q^T (gamma rq dO) + K^T (-b gamma rk dR)
-      const uint32_t yhi = xb_smem_u32(sm.y[0]), ylo = xb_smem_u32(sm.y[1]);
-#pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
-        const int row = ra + hh * 8;
-        const float y = ex2_sum(st.hd, row) * st.rqk[row];
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const uint32_t off = at2<4>(row, n * 8 + 2 * t);
-          const float2 v = unpack_bf16x2(lds32(sy + off));
-          uint32_t hi, lo;
-          split2(y * v.x, y * v.y, hi, lo);
-          sts32(yhi + off, hi);
-          sts32(ylo + off, lo);
-        }
-      }
-      bar(3, 128);
-      const float f = ex2_sum(st.hd, C - 1);
-#pragma unroll
-      for (int m = 0; m < DKP / 64; ++m)
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[m][n][e] *= f;
-      state_save<DKP>(shi, slo, (bf16*)p.ds_planes + ch_h * 2 * DKP * p.dvp, p.dvp, v0);
-#pragma unroll
-      for (int part = 0; part < 2; ++part) {
-        const uint32_t a = part ? sk : sq;
-        if (part) bar(2, 256);               // dR is there, and dS' has been read
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-          BFrag b;
-          load_b(b, part ? xhi : yhi, part ? xlo : ylo, ks * 16);
-#pragma unroll
-          for (int m = 0; m < DKP / 64; ++m) {
-            uint32_t fa[4];
-            ldsm4t(fa, a + addr_at<U>(w * (DKP / 4) + m * 16, ks * 16));
-            mma2(s[m], fa, b);
-          }
-        }
-      }
-      state_to_smem<DKP>(s, shi, slo);
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = unpack_bf16x2(w[j]);
+      x[8 * i + 2 * j] = f.x, x[8 * i + 2 * j + 1] = f.y;
     }
   }
-  cp_wait<0>();
-  if (warp >= 4 && p.ds_in != nullptr) state_global<DKP, true>(s, p.ds_in + soff, p.s_k, p.s_v, p.dk, vcols);
+}
+// 16 fp32 values of a state row in global memory
+__device__ __forceinline__ void state_row(float* base, long long sk, long long sv, int row, int dk, int col, int cols, bool store, float (&s)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    float* at = base + row * sk + (col + i) * sv;
+    const bool on = row < dk && col + i < cols;
+    if (store) {
+      if (on) *at = s[i];
+    } else {
+      s[i] = on ? *at : 0.f;
+    }
+  }
+}
+
+constexpr uint64_t KMAJ = xb_smem_desc_base_sw128(16, 1024), MNMAJ = xb_smem_desc_base_sw128(HALF, 1024);
+
+__device__ __forceinline__ bool cta_setup(const XbRecArgs& p, Cta& a, uint8_t* raw) {
+  const int slices = p.dvp / NV, rep = p.Hv / p.Hk;
+  a.smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  a.bars = reinterpret_cast<Bars*>(a.smem + SM_BAR);
+  const int sl = blockIdx.x % slices;
+  a.h = (blockIdx.x / slices) % p.Hv, a.doc = blockIdx.x / (slices * p.Hv), a.kh = a.h / rep;
+  a.v0 = sl * NV, a.vcols = min(NV, p.dv - a.v0);
+  a.c0 = p.doc_off[a.doc], a.c1 = p.doc_off[a.doc + 1];
+  a.status = p.status;
+  return a.doc < p.n_docs;
+}
+__device__ __forceinline__ void cta_begin(Cta& a) {
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) mbar_init(&a.bars->full[i], 1);
+    for (int i = 0; i < 3; ++i) mbar_init(&a.bars->done[i], 1);
+    a.bars->abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (threadIdx.x >= WORKERS) {
+    tmem_alloc(&a.bars->tmem, TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  a.tmem = a.bars->tmem;
+}
+__device__ __forceinline__ void cta_end(Cta& a) {
+  // after a wait that ran out, loads and products may still be on their way: give them 0.2 s
+  if (*(volatile int*)&a.bars->abort_flag && threadIdx.x == 0)
+    for (const uint64_t t0 = xb_globaltimer(); xb_globaltimer() - t0 < 200000000ull;) {}
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x >= WORKERS) {
+    tc_fence_after();
+    tmem_dealloc(a.tmem, TMEM_COLS);
+  }
+}
+// rows outside the documents: zeros
+__device__ __forceinline__ void zero_rows(const XbRecArgs& p, const Cta& a, bf16* out, long long ld) {
+  const int4* chunks = reinterpret_cast<const int4*>(p.chunks);
+  for (int c = a.c0; c < a.c1; ++c)
+    for (int i = threadIdx.x; i < chunks[c].y * NV; i += THREADS)
+      if (i % NV < a.vcols) out[(chunks[c].x + i / NV) * ld + i % NV] = __float2bfloat16(0.f);
+}
+
+// Workers tell the issuing warp through barriers 1 (state tile and this chunk's loads), 2 and 3 (operands of the second
+// and third product) that operands are written, and learn through done[0 .. 2] that a product is complete.  A wait
+// that runs out raises a flag; everybody then walks through the remaining steps without waiting, so that no barrier
+// is left with a thread missing.
+
+template <bool SAVE>
+__global__ void __launch_bounds__(THREADS, 1)
+delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mv,
+          const __grid_constant__ XbRecArgs p) {
+  extern __shared__ uint8_t smem_raw[];
+  Cta a;
+  const bool inside = cta_setup(p, a, smem_raw);
+  bf16* o = (bf16*)p.o + (long long)a.h * p.dv + a.v0;
+  const long long o_t = (long long)p.Hv * p.dv;
+  if (!inside) {
+    if (!SAVE) zero_rows(p, a, o, o_t);
+    return;
+  }
+  cta_begin(a);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp == WORKERS / 32) {
+    const bool one = lane == 0;
+    if (one && a.c0 < a.c1) load_stage(p, a, &mk, &mq, &mv, a.c0, 0);
+    if (one && a.c0 + 1 < a.c1) load_stage(p, a, &mk, &mq, &mv, a.c0 + 1, 1);
+    for (int n = 0; n < a.c1 - a.c0; ++n) {
+      const uint32_t st = xb_smem_u32(a.smem + (n & 1) * STAGE), b1 = xb_smem_u32(a.smem + SM_S), b2 = xb_smem_u32(a.smem + SM_B2),
+                     b3 = xb_smem_u32(a.smem + SM_B3);
+      bar(1, THREADS);
+      if (one) {
+        a.wait1(&a.bars->full[n & 1], (n >> 1) & 1, 1);
+        tc_fence_after();
+        constexpr uint32_t id = xb_idesc(1, 1, 128, 64, 0, 1);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          tc_mma_f16_ss(a.tmem + D1, xb_smem_desc(KMAJ, st + ST_KQ + (k >> 2) * HALF + (k & 3) * 32), xb_smem_desc(MNMAJ, b1 + k * 2048), id, k > 0);
+        tc_commit(&a.bars->done[0]);
+      }
+      bar(2, THREADS);
+      if (one) {
+        tc_fence_after();
+        constexpr uint32_t id = xb_idesc(1, 1, 128, 64, 0, 1);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          tc_mma_f16_ss(a.tmem + D2, xb_smem_desc(KMAJ, st + ST_TP + (k >> 2) * TP_PLANE + (k & 3) * 32), xb_smem_desc(MNMAJ, b2 + (k & 3) * 2048), id, k > 0);
+        tc_commit(&a.bars->done[1]);
+      }
+      bar(3, THREADS);
+      if (one) {
+        tc_fence_after();
+        constexpr uint32_t id = xb_idesc(1, 1, 128, 64, 1, 1);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          tc_mma_f16_ss(a.tmem + D3, xb_smem_desc(MNMAJ, st + ST_KQ + k * 2048), xb_smem_desc(MNMAJ, b3 + k * 2048), id, k > 0);
+        tc_commit(&a.bars->done[2]);
+        if (n + 2 < a.c1 - a.c0) {           // the stage is free when the last product has read it
+          a.wait1(&a.bars->done[2], n & 1, 2);
+          load_stage(p, a, &mk, &mq, &mv, a.c0 + n + 2, n & 1);
+        }
+      }
+      __syncwarp();
+    }
+  } else {
+    const int q4 = warp & 3, half = warp >> 2, r = q4 * 32 + lane, i = r & 63;
+    const bool krow = r < C;
+    const uint32_t acc = a.tmem + ((uint32_t)(q4 * 32) << 16) + half * 16;
+    const long long soff = ((long long)a.doc * p.Hv + a.h) * p.dk * p.dv + a.v0 * p.s_v;
+    float s[16] = {};
+    uint32_t hi[8], lo[8];
+    if (p.s_in != nullptr) state_row(const_cast<float*>(p.s_in) + soff, p.s_k, p.s_v, r, p.dk, half * 16, a.vcols, false, s);
+    for (int n = 0; n < a.c1 - a.c0; ++n) {
+      const int c = a.c0 + n, len = reinterpret_cast<const int4*>(p.chunks)[c].y;
+      const long long ch_h = (long long)c * p.Hv + a.h, t0 = reinterpret_cast<const int4*>(p.chunks)[c].x;
+      uint8_t* st = a.smem + (n & 1) * STAGE;
+      const float* hd = reinterpret_cast<const float*>(st + ST_HD);
+      const float* rqk = reinterpret_cast<const float*>(st + ST_RQK);
+      put_row(a.smem + SM_S, r, half, s, hi, lo);
+      if (SAVE && r < p.dkp) {
+        bf16* pl = (bf16*)p.s_planes + (ch_h * 2 * p.dkp + r) * p.dvp + a.v0 + half * 16;
+        store16(pl, hi);
+        store16(pl + (long long)p.dkp * p.dvp, lo);
+      }
+      a.wait(&a.bars->full[n & 1], (n >> 1) & 1, 3);
+      if (len < C) clear_rows(st, len);
+      fence_proxy_async_smem();
+      tc_fence_before();
+      bar_arrive(1, THREADS);
+      // row factors, and v, while the first product runs
+      const float gam = ex2_sum(hd, i), dec = ex2_diff(hd, C - 1, i), last = ex2_sum(hd, C - 1), b = hd[2 * C + i];
+      const float rq = rqk[i], rk = rqk[C + i];
+      uint4 xv[2];
+      read_x(st + ST_X, i, half, krow && i < len, xv);
+      float x[16], y[16];
+      a.wait(&a.bars->done[0], n & 1, 4);
+      tc_fence_after();
+      read_acc(acc + D1, y);
+      if (krow) {                            // R = b (V - gamma rk K S)
+        floats(xv, x);
+        const float f = gam * rk;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = b * (x[e] - f * y[e]);
+        put_row(a.smem + SM_B2, i, half, x, hi, lo);
+      }
+      fence_proxy_async_smem();
+      tc_fence_before();
+      bar_arrive(2, THREADS);
+      a.wait(&a.bars->done[1], n & 1, 5);
+      tc_fence_after();
+      read_acc(acc + D2, x);
+      if (krow) {                            // d rk U
+        if (SAVE) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) split2(x[2 * e], x[2 * e + 1], hi[e], lo[e]);
+          bf16* pl = (bf16*)p.u_planes + (ch_h * 2 * C + i) * p.dvp + a.v0 + half * 16;
+          store16(pl, hi);
+          store16(pl + (long long)C * p.dvp, lo);
+        }
+        const float f = dec * rk;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] *= f;
+        put_row(a.smem + SM_B3, i, half, x, hi, lo);
+      }
+      fence_proxy_async_smem();
+      tc_fence_before();
+      bar_arrive(3, THREADS);
+      if (!SAVE && !krow && i < len) {       // O = gamma rq Q S + (P T) R
+        const float f = gam * rq;
+        bf16* dst = o + (t0 + i) * o_t + half * 16;
+#pragma unroll
+        for (int e = 0; e < 16; e += 8)
+          if (half * 16 + e < a.vcols)
+            *reinterpret_cast<uint4*>(dst + e) =
+                make_uint4(pack_bf16x2(f * y[e] + x[e], f * y[e + 1] + x[e + 1]), pack_bf16x2(f * y[e + 2] + x[e + 2], f * y[e + 3] + x[e + 3]),
+                           pack_bf16x2(f * y[e + 4] + x[e + 4], f * y[e + 5] + x[e + 5]), pack_bf16x2(f * y[e + 6] + x[e + 6], f * y[e + 7] + x[e + 7]));
+      }
+      __syncwarp();
+      a.wait(&a.bars->done[2], n & 1, 6);
+      tc_fence_after();
+      read_acc(acc + D3, y);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[e] = last * s[e] + y[e];
+    }
+    if (p.s_out != nullptr) state_row(p.s_out + soff, p.s_k, p.s_v, r, p.dk, half * 16, a.vcols, true, s);
+  }
+  cta_end(a);
+}
+
+// dS through one document, last chunk first.
+__global__ void __launch_bounds__(THREADS, 1)
+delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap my,
+          const __grid_constant__ XbRecArgs p) {
+  extern __shared__ uint8_t smem_raw[];
+  Cta a;
+  const bool inside = cta_setup(p, a, smem_raw);
+  bf16* dv = (bf16*)p.dv_out + (long long)a.h * p.dv + a.v0;
+  const long long dv_t = (long long)p.Hv * p.dv;
+  if (!inside) {
+    zero_rows(p, a, dv, dv_t);
+    return;
+  }
+  cta_begin(a);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, steps = a.c1 - a.c0;
+  if (warp == WORKERS / 32) {
+    const bool one = lane == 0;
+    if (one && steps > 0) load_stage(p, a, &mk, &mq, &my, a.c1 - 1, 0);
+    if (one && steps > 1) load_stage(p, a, &mk, &mq, &my, a.c1 - 2, 1);
+    for (int n = 0; n < steps; ++n) {
+      const uint32_t st = xb_smem_u32(a.smem + (n & 1) * STAGE), b1 = xb_smem_u32(a.smem + SM_S), b2 = xb_smem_u32(a.smem + SM_B2),
+                     b3 = xb_smem_u32(a.smem + SM_B3);
+      constexpr uint32_t id3 = xb_idesc(1, 1, 128, 64, 1, 1);
+      bar(1, THREADS);
+      if (one) {
+        a.wait1(&a.bars->full[n & 1], (n >> 1) & 1, 1);
+        tc_fence_after();
+        constexpr uint32_t id = xb_idesc(1, 1, 128, 64, 0, 1);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          tc_mma_f16_ss(a.tmem + D1, xb_smem_desc(KMAJ, st + ST_KQ + (k >> 2) * HALF + (k & 3) * 32), xb_smem_desc(MNMAJ, b1 + k * 2048), id, k > 0);
+        tc_commit(&a.bars->done[0]);
+#pragma unroll
+        for (int k = 4; k < 8; ++k)          // rows of Q
+          tc_mma_f16_ss(a.tmem + D3, xb_smem_desc(MNMAJ, st + ST_KQ + k * 2048), xb_smem_desc(MNMAJ, b3 + k * 2048), id3, k > 4);
+      }
+      bar(2, THREADS);
+      if (one) {
+        tc_fence_after();
+        constexpr uint32_t id = xb_idesc(1, 1, 64, 64, 1, 1);
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+          tc_mma_f16_ss(a.tmem + D2, xb_smem_desc(MNMAJ, st + ST_TP + (k >> 3) * TP_PLANE + (k & 7) * 2048), xb_smem_desc(MNMAJ, b2 + (k & 7) * 2048), id, k > 0);
+        tc_commit(&a.bars->done[1]);
+      }
+      bar(3, THREADS);
+      if (one) {
+        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < 4; ++k)          // rows of K
+          tc_mma_f16_ss(a.tmem + D3, xb_smem_desc(MNMAJ, st + ST_KQ + k * 2048), xb_smem_desc(MNMAJ, b3 + k * 2048), id3, 1);
+        tc_commit(&a.bars->done[2]);
+        if (n + 2 < steps) {
+          a.wait1(&a.bars->done[2], n & 1, 2);
+          load_stage(p, a, &mk, &mq, &my, a.c1 - 1 - (n + 2), n & 1);
+        }
+      }
+      __syncwarp();
+    }
+  } else {
+    const int q4 = warp & 3, half = warp >> 2, r = q4 * 32 + lane, i = r & 63;
+    const bool krow = r < C;
+    const int ri = q4 * 16 + (lane & 15);    // row of a 64-row accumulator: 16 lanes of every warp
+    const uint32_t acc = a.tmem + ((uint32_t)(q4 * 32) << 16) + half * 16;
+    const long long soff = ((long long)a.doc * p.Hv + a.h) * p.dk * p.dv + a.v0 * p.s_v;
+    float s[16] = {}, x[16];
+    uint32_t hi[8], lo[8];
+    if (p.ds_out != nullptr) state_row(const_cast<float*>(p.ds_out) + soff, p.s_k, p.s_v, r, p.dk, half * 16, a.vcols, false, s);
+    // operands that need dO alone: [dO | 0] of the second product, gamma rq dO of the third (threads of Q's rows)
+    auto put_dy = [&](int n) {
+      const int c = a.c1 - 1 - n, len = reinterpret_cast<const int4*>(p.chunks)[c].y;
+      uint8_t* st = a.smem + (n & 1) * STAGE;
+      a.wait(&a.bars->full[n & 1], (n >> 1) & 1, 3);
+      if (len < C) clear_rows(st, len);
+      if (krow) return;
+      uint4 v[2];
+      read_x(st + ST_X, i, half, i < len, v);
+      uint8_t* row = a.smem + SM_B2 + r * 128;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) *reinterpret_cast<uint4*>(row + (((half * 2 + e) ^ (r & 7)) << 4)) = v[e];
+      const float f = ex2_sum(reinterpret_cast<const float*>(st + ST_HD), i) * reinterpret_cast<const float*>(st + ST_RQK)[i];
+      floats(v, x);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[e] *= f;
+      put_row(a.smem + SM_B3, r, half, x, hi, lo);
+    };
+    if (!krow)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        *reinterpret_cast<uint4*>(a.smem + SM_B2 + r * 128 + (((4 + half * 2 + e) ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+    if (steps > 0) put_dy(0);
+    for (int n = 0; n < steps; ++n) {
+      const int c = a.c1 - 1 - n, len = reinterpret_cast<const int4*>(p.chunks)[c].y;
+      const long long ch_h = (long long)c * p.Hv + a.h, t0 = reinterpret_cast<const int4*>(p.chunks)[c].x;
+      uint8_t* st = a.smem + (n & 1) * STAGE;
+      const float* hd = reinterpret_cast<const float*>(st + ST_HD);
+      const float* rqk = reinterpret_cast<const float*>(st + ST_RQK);
+      put_row(a.smem + SM_S, r, half, s, hi, lo);
+      if (r < p.dkp) {
+        bf16* pl = (bf16*)p.ds_planes + (ch_h * 2 * p.dkp + r) * p.dvp + a.v0 + half * 16;
+        store16(pl, hi);
+        store16(pl + (long long)p.dkp * p.dvp, lo);
+      }
+      fence_proxy_async_smem();
+      tc_fence_before();
+      bar_arrive(1, THREADS);
+      const float last = ex2_sum(hd, C - 1), f1 = ex2_diff(hd, C - 1, i) * rqk[C + i];
+      const float b = hd[2 * C + ri], f2 = -b * ex2_sum(hd, ri) * rqk[C + ri];
+      a.wait(&a.bars->done[0], n & 1, 4);
+      tc_fence_after();
+      if (q4 < 2) {                          // Y = d rk K dS'
+        read_acc(acc + D1, x);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] *= f1;
+        put_row(a.smem + SM_B2, i, half, x, hi, lo);
+      }
+      fence_proxy_async_smem();
+      tc_fence_before();
+      bar_arrive(2, THREADS);
+      a.wait(&a.bars->done[1], n & 1, 5);
+      tc_fence_after();
+      float dr[16];
+      read_acc(acc + D2, dr);
+      if (lane < 16) {                       // -b gamma rk dR
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = f2 * dr[e];
+        put_row(a.smem + SM_B3, ri, half, x, hi, lo);
+      }
+      fence_proxy_async_smem();
+      tc_fence_before();
+      bar_arrive(3, THREADS);
+      if (lane < 16) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) split2(dr[2 * e], dr[2 * e + 1], hi[e], lo[e]);
+        bf16* pl = (bf16*)p.dr_planes + (ch_h * 2 * C + ri) * p.dvp + a.v0 + half * 16;
+        store16(pl, hi);
+        store16(pl + (long long)C * p.dvp, lo);
+        if (ri < len) {
+          bf16* dst = dv + (t0 + ri) * dv_t + half * 16;
+#pragma unroll
+          for (int e = 0; e < 16; e += 8)
+            if (half * 16 + e < a.vcols)
+              *reinterpret_cast<uint4*>(dst + e) = make_uint4(pack_bf16x2(b * dr[e], b * dr[e + 1]), pack_bf16x2(b * dr[e + 2], b * dr[e + 3]),
+                                                              pack_bf16x2(b * dr[e + 4], b * dr[e + 5]), pack_bf16x2(b * dr[e + 6], b * dr[e + 7]));
+        }
+      }
+      __syncwarp();
+      if (n + 1 < steps) put_dy(n + 1);      // beside the third product: the first two have read these rows
+      __syncwarp();
+      a.wait(&a.bars->done[2], n & 1, 6);
+      tc_fence_after();
+      read_acc(acc + D3, x);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[e] = last * s[e] + x[e];
+    }
+    if (p.ds_in != nullptr) state_row(p.ds_in + soff, p.s_k, p.s_v, r, p.dk, half * 16, a.vcols, true, s);
+  }
+  cta_end(a);
+}
+
+// [T, heads, cols] bf16, boxes of 64 rows of one head
+int tile_map(CUtensorMap* m, const void* base, int T, int heads, int cols, long long ld_t, long long ld_h, int box, CUtensorMapSwizzle swz) {
+  return xb_make_tmap_3d(m, base, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, T, heads, cols, T > 1 ? ld_t : 8, heads > 1 ? ld_h : 8, C, 1, box, swz);
+}
+template <typename K>
+int run(K kernel, const XbRecArgs& a, const void* x, long long x_t, long long x_h, cudaStream_t st) {
+  const long long blocks = (long long)(a.n_docs + 2) * a.Hv * (a.dvp / NV);
+  if (blocks > 0x7fffffffLL) return -4;
+  CUtensorMap mk{}, mq{}, mx{};
+  if (a.T > 0 && (tile_map(&mk, a.k, a.T, a.Hk, a.dk, a.k_t, a.k_h, 64, CU_TENSOR_MAP_SWIZZLE_128B) ||
+                  tile_map(&mq, a.q, a.T, a.Hk, a.dk, a.q_t, a.q_h, 64, CU_TENSOR_MAP_SWIZZLE_128B) ||
+                  tile_map(&mx, x, a.T, a.Hv, a.dv, x_t, x_h, NV, CU_TENSOR_MAP_SWIZZLE_64B)))
+    return -2;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess) {
+    cudaGetLastError();
+    return -5;
+  }
+  kernel<<<(unsigned)blocks, THREADS, SMEM, st>>>(mk, mq, mx, a);
+  return cudaGetLastError() == cudaSuccess ? 0 : -11;
 }
 
 template <int DKP>
-int forward(const XbRecArgs& a, long long seq, cudaStream_t st) {
-  if (int rc = rec_launch(delta_prep<DKP>, (long long)a.nc_max * a.Hk, 128, sizeof(DPrepSmem<DKP>), a, st)) return rc;
-  return rec_launch(delta_fwd<DKP, false>, seq, 256, sizeof(DFwdSmem<DKP>), a, st);
-}
-template <int DKP>
-int backward(const XbRecArgs& a, long long seq, cudaStream_t st) {
-  XbRecArgs again = a;
-  again.s_out = nullptr;
-  if (int rc = rec_launch(delta_fwd<DKP, true>, seq, 128, sizeof(DFwdSmem<DKP>), again, st)) return rc;
-  return rec_launch(delta_bwd<DKP>, seq, 256, sizeof(DBwdSmem<DKP>), a, st);
+int prep(const XbRecArgs& a, cudaStream_t st) {
+  return rec_launch(delta_prep<DKP>, (long long)a.nc_max * a.Hk, 128, sizeof(DPrepSmem<DKP>), a, st);
 }
 
 }  // namespace
 
 int xb_delta_fwd(const XbRecArgs& a, cudaStream_t st) {
-  const long long seq = (long long)(a.n_docs + 2) * a.Hv * (a.dvp / NV);
-  return a.dk <= 64 ? forward<64>(a, seq, st) : forward<128>(a, seq, st);
+  if (int rc = a.dk <= 64 ? prep<64>(a, st) : prep<128>(a, st)) return rc;
+  return run(delta_fwd<false>, a, a.v, a.v_t, a.v_h, st);
 }
 int xb_delta_bwd(const XbRecArgs& a, cudaStream_t st) {
-  const long long seq = (long long)(a.n_docs + 2) * a.Hv * (a.dvp / NV);
-  return a.dk <= 64 ? backward<64>(a, seq, st) : backward<128>(a, seq, st);
+  XbRecArgs again = a;
+  again.s_out = nullptr;
+  if (int rc = run(delta_fwd<true>, again, a.v, a.v_t, a.v_h, st)) return rc;
+  return run(delta_bwd, a, a.dy, a.dy_t, a.dy_h, st);
 }

@@ -26,7 +26,7 @@ _launches = 0
 CHUNK = 64              # tokens of a chunk of the kernels (csrc/recurrence.cu)
 SLICE = 32              # columns of the state that one CTA carries
 MAX_STATE_ROWS = 128
-PACKED = 20480          # bytes of P and T of one chunk and head
+OPERANDS = 32768        # bytes of the operand tile that the delta rule prepares per chunk and head
 
 
 def launch_count() -> int:
@@ -43,14 +43,14 @@ class _Args(ctypes.Structure):
                 + [(n, ctypes.c_longlong) for n in ("s_k", "s_v")]
                 + [(n, ctypes.c_void_p) for n in ("o", "dq", "dk_out", "dv_out", "dg", "db", "dA", "dD", "chunks",
                                                   "doc_off", "hd", "rqk", "qk", "kk", "pt", "s_planes", "ds_planes",
-                                                  "u_planes", "dr_planes", "part")]
-                + [(n, ctypes.c_int) for n in ("T", "n_docs", "Hk", "Hv", "dk", "dv", "dvp", "nc_max", "l2norm")]
+                                                  "u_planes", "dr_planes", "part", "status")]
+                + [(n, ctypes.c_int) for n in ("T", "n_docs", "Hk", "Hv", "dk", "dv", "dkp", "dvp", "nc_max", "l2norm")]
                 + [("scale", ctypes.c_float)])
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """``x`` [T, heads, dim] as the kernels read it: itself, or a copy where its strides do not suit 16-byte loads."""
-    if x.stride(2) != 1 or x.stride(0) % 8 or x.stride(1) % 8 or x.data_ptr() % 16:
+    if x.stride(2) != 1 or x.stride(0) % 8 or x.stride(1) % 8 or x.stride(0) <= 0 or x.stride(1) <= 0 or x.data_ptr() % 16:
         return x.contiguous() if not x.is_contiguous() else x.clone()
     return x
 
@@ -80,14 +80,14 @@ def _fill(a: _Args, q, k, v, g, b, A, D, cu, s_in, ws, keep: bool, delta: bool, 
         a.s_k, a.s_v = 1, dk
     a.cu, a.s_in = cu.data_ptr(), _lib.ptr(s_in)
     a.T, a.n_docs, a.Hk, a.Hv, a.dk, a.dv = T, cu.numel() - 1, Hk, Hv, dk, dv
-    a.dvp = -(-dv // SLICE) * SLICE
+    a.dkp, a.dvp = 64 if dk <= 64 else 128, -(-dv // SLICE) * SLICE
     a.nc_max = T // CHUNK + cu.numel() + 1
     a.l2norm, a.scale = int(l2norm), scale
     nc = a.nc_max
     sizes = [("chunks", nc * 16), ("doc_off", (cu.numel() + 2) * 4), ("hd", nc * Hv * 3 * CHUNK * 4),
              ("rqk", nc * Hk * 2 * CHUNK * 4)]
     if delta:
-        sizes.append(("pt", nc * Hv * PACKED))
+        sizes.append(("pt", nc * Hv * OPERANDS))
     if keep or not delta:
         sizes.append(("qk", nc * Hk * CHUNK * CHUNK * 4))
     if keep and delta:
@@ -149,7 +149,7 @@ class _Recurrence(torch.autograd.Function):
             dD = None if delta else torch.empty(Hv, dtype=torch.float32, device=dev)
             a.dq, a.dk_out, a.dv_out, a.db = dq.data_ptr(), dkk.data_ptr(), dvv.data_ptr(), db.data_ptr()
             a.dg, a.dA, a.dD = _lib.ptr(dg), _lib.ptr(dA), _lib.ptr(dD)
-            state = a.nc_max * Hv * 2 * (64 if dk <= 64 else 128) * a.dvp * 2
+            state = a.nc_max * Hv * 2 * a.dkp * a.dvp * 2
             plane = a.nc_max * Hv * 2 * CHUNK * a.dvp * 2
             offs, total = _pieces([state, state] + ([plane, plane] if delta else [a.nc_max * Hv * 2 * 4]))
             tmp = torch.empty(total, dtype=torch.uint8, device=dev)
