@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(128) rec_fwd(const XbRecArgs p) {
     if (c + 1 < c1) fetch(c + 1, (c - c0 + 1) & 1);
     cp_commit();
     const long long ch_h = (long long)c * p.Hv + h;
-    if (SAVE) state_save<DKP>(shi, slo, (bf16*)p.s_planes + ch_h * 2 * DKP * p.dvp, p.dvp, v0);
+    if (SAVE) state_save<DKP>(shi, slo, (uint8_t*)p.s_tiles + (ch_h * slices + sl) * HALF);
     const int ra = w * 16 + g;             // this thread's rows: ra and ra + 8
     float acc_k[4][4] = {}, acc_q[4][4] = {};
     if (DELTA || !SAVE) {
@@ -400,9 +400,6 @@ __global__ void __launch_bounds__(128) rec_fwd(const XbRecArgs p) {
           uint32_t hi, lo;
           split2(u[n][2 * hh], u[n][2 * hh + 1], hi, lo);
           if (SAVE) {
-            uint32_t* pl = reinterpret_cast<uint32_t*>((bf16*)p.u_planes + (ch_h * 2 * C + row) * p.dvp + v0 + n * 8 + 2 * t);
-            pl[0] = hi;
-            pl[C * p.dvp / 2] = lo;
           } else {
             sts32(uhi + off, hi);
             sts32(ulo + off, lo);
@@ -584,7 +581,7 @@ __global__ void __launch_bounds__(128) rec_bwd(const XbRecArgs p) {
     if (c > c0) fetch(c - 1, (c1 - c) & 1);
     cp_commit();
     const long long ch_h = (long long)c * p.Hv + h;
-    state_save<DKP>(shi, slo, (bf16*)p.ds_planes + ch_h * 2 * DKP * p.dvp, p.dvp, v0);
+    state_save<DKP>(shi, slo, (uint8_t*)p.ds_tiles + (ch_h * slices + sl) * HALF);
     const int ra = w * 16 + g;
     // K dS'
     float du[4][4] = {};
@@ -692,9 +689,6 @@ __global__ void __launch_bounds__(128) rec_bwd(const XbRecArgs p) {
           const float y0 = dr[n][2 * hh], y1 = dr[n][2 * hh + 1];
           uint32_t hi, lo;
           split2(y0, y1, hi, lo);
-          uint32_t* pl = reinterpret_cast<uint32_t*>((bf16*)p.dr_planes + (ch_h * 2 * C + row) * p.dvp + v0 + col);
-          pl[0] = hi;
-          pl[C * p.dvp / 2] = lo;
           split2(f * y0, f * y1, hi, lo);
           sts32(xhi + off, hi);
           sts32(xlo + off, lo);
@@ -761,414 +755,6 @@ __global__ void __launch_bounds__(128) rec_bwd(const XbRecArgs p) {
   if (p.ds_in != nullptr && doc < p.n_docs) state_global<DKP, true>(s, p.ds_in + soff, p.s_k, p.s_v, p.dk, vcols);
 }
 
-// ---- backward, parallel part: gradients of q, k, the decay and b of one chunk ---------------------------------------
-constexpr int GV = 64;        // state columns of one pass
-template <int DKP, bool DELTA>
-struct GradSmem {
-  uint8_t q[C * DKP * 2], k[C * DKP * 2];
-  uint8_t dy[C * GV * 2], v[C * GV * 2];
-  uint8_t u[DELTA ? 2 : 1][DELTA ? C * GV * 2 : 16], r[DELTA ? 2 : 1][DELTA ? C * GV * 2 : 16];
-  uint8_t s[2][DKP * GV * 2], ds[2][DKP * GV * 2];
-  uint8_t z[2][C * C * 2], w[DELTA ? 2 : 1][DELTA ? C * C * 2 : 16];
-  float hd[HD], rqk[RQK];
-  float rd[3][2][C];          // row sums of q.t1, k.t2, k.t3 by column half
-  float er[2][C], ec[4][C];   // row and column sums of dP o P (scan: without b)
-  float fr[2][C], fc[4][C];   // the same of dL o A
-  float rv[C], sdot[8];
-  float dot[2][2][C];         // q.dq and k.dk of the finished rows
-};
-
-template <int DKP, bool DELTA>
-__global__ void __launch_bounds__(256) rec_grad(const XbRecArgs p) {
-  extern __shared__ __align__(128) uint8_t smem_raw[];
-  GradSmem<DKP, DELTA>& sm = *reinterpret_cast<GradSmem<DKP, DELTA>*>(smem_raw);
-  constexpr int U = DKP / 8, NT = DKP / 16;
-  const int kh = blockIdx.x % p.Hk, c = blockIdx.x / p.Hk, rep = p.Hv / p.Hk;
-  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3;
-  const int rb = w & 3, cb = w >> 2, ra = rb * 16 + g, n0 = cb * (DKP / 2);
-  if (c >= p.doc_off[p.n_docs + 2]) return;
-  const int4 ch = reinterpret_cast<const int4*>(p.chunks)[c];
-  const int len = ch.y;
-  bf16* dq = (bf16*)p.dq + (ch.x * (long long)p.Hk + kh) * p.dk;
-  bf16* dk = (bf16*)p.dk_out + (ch.x * (long long)p.Hk + kh) * p.dk;
-  const long long d_t = (long long)p.Hk * p.dk;
-  if (DELTA && ch.z >= p.n_docs) {                                   // rows outside the documents
-    for (int i = tid; i < len * p.dk; i += 256) {
-      dq[(i / p.dk) * d_t + i % p.dk] = __float2bfloat16(0.f);
-      dk[(i / p.dk) * d_t + i % p.dk] = __float2bfloat16(0.f);
-    }
-    for (int i = tid; i < len * rep; i += 256) {
-      const long long at = (long long)(ch.x + i / rep) * p.Hv + kh * rep + i % rep;
-      p.dg[at] = 0.f, p.db[at] = 0.f;
-    }
-    return;
-  }
-  const uint32_t sq = xb_smem_u32(sm.q), sk = xb_smem_u32(sm.k), sy = xb_smem_u32(sm.dy), sv = xb_smem_u32(sm.v);
-  load_tile<U, C, 256>(sq, (const bf16*)p.q + ch.x * p.q_t + kh * p.q_h, p.q_t, len, p.dk);
-  load_tile<U, C, 256>(sk, (const bf16*)p.k + ch.x * p.k_t + kh * p.k_h, p.k_t, len, p.dk);
-  load_floats<256>(xb_smem_u32(sm.rqk), p.rqk + ((long long)c * p.Hk + kh) * RQK, RQK);
-  float aq[NT][4] = {}, ak[NT][4] = {};                              // rq dq, rk dk over the heads of the group
-  for (int hh = 0; hh < rep; ++hh) {
-    const int h = kh * rep + hh;
-    const long long ch_h = (long long)c * p.Hv + h;
-    float dp[4][4] = {}, dl[4][4] = {}, rd1[2] = {}, rd2[2] = {}, rd3[2] = {};
-    float sdot = 0.f, rv = 0.f;
-    for (int v0 = 0; v0 < p.dv; v0 += GV) {
-      __syncthreads();                                               // the tiles of the pass before have been read
-      const int vcols = min(GV, p.dv - v0), pcols = min(GV, p.dvp - v0);
-      load_tile<8, C, 256>(sy, (const bf16*)p.dy + ch.x * p.dy_t + h * p.dy_h + v0, p.dy_t, len, vcols);
-      load_tile<8, C, 256>(sv, (const bf16*)p.v + ch.x * p.v_t + h * p.v_h + v0, p.v_t, len, vcols);
-#pragma unroll
-      for (int pl = 0; pl < 2; ++pl) {
-        if (DELTA) {
-          load_tile<8, C, 256>(xb_smem_u32(sm.u[pl]), (const bf16*)p.u_planes + (ch_h * 2 + pl) * C * p.dvp + v0, p.dvp, C, pcols);
-          load_tile<8, C, 256>(xb_smem_u32(sm.r[pl]), (const bf16*)p.dr_planes + (ch_h * 2 + pl) * C * p.dvp + v0, p.dvp, C, pcols);
-        }
-        load_tile<8, DKP, 256>(xb_smem_u32(sm.s[pl]), (const bf16*)p.s_planes + (ch_h * 2 + pl) * DKP * p.dvp + v0, p.dvp, DKP, pcols);
-        load_tile<8, DKP, 256>(xb_smem_u32(sm.ds[pl]), (const bf16*)p.ds_planes + (ch_h * 2 + pl) * DKP * p.dvp + v0, p.dvp, DKP, pcols);
-      }
-      if (v0 == 0) load_floats<256>(xb_smem_u32(sm.hd), p.hd + ch_h * HD, HD);
-      cp_commit();
-      cp_wait<0>();
-      __syncthreads();
-      // dP = dO U^T (scan: dO V^T), -dL = dR U^T, this warp's 16 x 32 part
-      const uint32_t ub[2] = {DELTA ? xb_smem_u32(sm.u[0]) : sv, xb_smem_u32(sm.u[1 % (DELTA ? 2 : 1)])};
-      const uint32_t rr[2] = {xb_smem_u32(sm.r[0]), xb_smem_u32(sm.r[1 % (DELTA ? 2 : 1)])};
-      if (cb * 32 <= rb * 16 + 15) {
-#pragma unroll
-        for (int ks = 0; ks < GV / 16; ++ks) {
-          uint32_t fy[4], fr[2][4];
-          ldsm4(fy, sy + addr_a<8>(rb * 16, ks * 16));
-          if (DELTA) {
-            ldsm4(fr[0], rr[0] + addr_a<8>(rb * 16, ks * 16));
-            ldsm4(fr[1], rr[1] + addr_a<8>(rb * 16, ks * 16));
-          }
-#pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            uint32_t bh[4], bl[4];
-            ldsm4(bh, ub[0] + addr_b<8>(cb * 32 + n * 16, ks * 16));
-            if (DELTA) ldsm4(bl, ub[1] + addr_b<8>(cb * 32 + n * 16, ks * 16));
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float(&d)[4] = dp[2 * n + e];
-              if (DELTA) {
-                mma(d, fy, bl[2 * e], bl[2 * e + 1]);
-                mma(dl[2 * n + e], fr[1], bh[2 * e], bh[2 * e + 1]);
-                mma(dl[2 * n + e], fr[0], bl[2 * e], bl[2 * e + 1]);
-                mma(dl[2 * n + e], fr[0], bh[2 * e], bh[2 * e + 1]);
-              }
-              mma(d, fy, bh[2 * e], bh[2 * e + 1]);
-            }
-          }
-        }
-      }
-      // t1 = dO S^T, t2 = dR S^T, t3 = U dS'^T (scan: V dS'^T), one after the other in the same registers
-#pragma unroll
-      for (int which = 0; which < 3; ++which) {
-        if (!DELTA && which == 1) continue;
-        const uint32_t a0 = which == 0 ? sy : which == 1 ? rr[0] : ub[0], a1 = which == 1 ? rr[1] : ub[1];
-        const bool two = DELTA && which > 0;
-        const uint32_t b0 = xb_smem_u32(which == 2 ? sm.ds[0] : sm.s[0]), b1 = xb_smem_u32(which == 2 ? sm.ds[1] : sm.s[1]);
-        float x[NT][4] = {};
-#pragma unroll
-        for (int ks = 0; ks < GV / 16; ++ks) {
-          uint32_t fa[4], fl[4];
-          ldsm4(fa, a0 + addr_a<8>(rb * 16, ks * 16));
-          if (two) ldsm4(fl, a1 + addr_a<8>(rb * 16, ks * 16));
-#pragma unroll
-          for (int n = 0; n < NT; n += 2) {
-            uint32_t bh[4], bl[4];
-            ldsm4(bh, b0 + addr_b<8>(n0 + n * 8, ks * 16));
-            ldsm4(bl, b1 + addr_b<8>(n0 + n * 8, ks * 16));
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              if (two) mma(x[n + e], fl, bh[2 * e], bh[2 * e + 1]);
-              mma(x[n + e], fa, bl[2 * e], bl[2 * e + 1]);
-              mma(x[n + e], fa, bh[2 * e], bh[2 * e + 1]);
-            }
-          }
-        }
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int row = ra + r * 8;
-          const float b = sm.hd[2 * C + row];
-          float f;
-          if (which == 0) f = ex2_sum(sm.hd, row) * sm.rqk[row];
-          else if (which == 1) f = -b * ex2_sum(sm.hd, row) * sm.rqk[C + row];
-          else f = ex2_diff(sm.hd, C - 1, row) * sm.rqk[C + row] * (DELTA ? 1.f : b);
-          float sum = 0.f;
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const float2 y = unpack_bf16x2(lds32((which == 0 ? sq : sk) + at2<U>(row, n0 + n * 8 + 2 * t)));
-            sum += y.x * x[n][2 * r] + y.y * x[n][2 * r + 1];
-            float(&d)[4] = which == 0 ? aq[n] : ak[n];
-            d[2 * r] += f * x[n][2 * r], d[2 * r + 1] += f * x[n][2 * r + 1];
-          }
-          (which == 0 ? rd1 : which == 1 ? rd2 : rd3)[r] += sum;
-        }
-      }
-      // <S, dS'> and the rows' dR.v (scan: dO.v)
-#pragma unroll
-      for (int i = 0; i < DKP * 8 / 256; ++i) {
-        const int idx = i * 256 + tid, r = idx >> 3, u = idx & 7;
-        const uint32_t off = swz<8>(r, u);
-        const uint4 a = lds128(xb_smem_u32(sm.s[0]) + off), al = lds128(xb_smem_u32(sm.s[1]) + off);
-        const uint4 b = lds128(xb_smem_u32(sm.ds[0]) + off), bl = lds128(xb_smem_u32(sm.ds[1]) + off);
-        const uint32_t xa[4] = {a.x, a.y, a.z, a.w}, xl[4] = {al.x, al.y, al.z, al.w};
-        const uint32_t ya[4] = {b.x, b.y, b.z, b.w}, yl[4] = {bl.x, bl.y, bl.z, bl.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 m = join2(xa[e], xl[e]), n = join2(ya[e], yl[e]);
-          sdot += m.x * n.x + m.y * n.y;
-        }
-      }
-      {
-        const int row = tid >> 2;
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const uint32_t off = swz<8>(row, (tid & 3) * 2 + u);
-          const uint4 a = DELTA ? lds128(rr[0] + off) : lds128(sy + off), al = DELTA ? lds128(rr[1] + off) : a, b = lds128(sv + off);
-          const uint32_t xa[4] = {a.x, a.y, a.z, a.w}, xl[4] = {al.x, al.y, al.z, al.w}, ya[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 m = DELTA ? join2(xa[e], xl[e]) : unpack_bf16x2(xa[e]), n = unpack_bf16x2(ya[e]);
-            rv += m.x * n.x + m.y * n.y;
-          }
-        }
-      }
-    }
-    // Z = D o dP and W = D o dL with the row factors of both sides, and the sums of their products with P and A
-    {
-      const float* qk = p.qk + ((long long)c * p.Hk + kh) * (C * C);
-      const float* kk = DELTA ? p.kk + ((long long)c * p.Hk + kh) * (C * C) : nullptr;
-      float er[2] = {}, fr[2] = {};
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const int col = cb * 32 + n * 8 + 2 * t;
-        float ec[2] = {}, fc[2] = {};
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int row = ra + r * 8;
-          float z[2] = {}, y[2] = {};
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int j = col + e;
-            if (j <= row) {
-              const float d = ex2_diff(sm.hd, row, j), b = sm.hd[2 * C + (DELTA ? row : j)], m = d * dp[n][2 * r + e];
-              const float v = m * qk[row * C + j];
-              er[r] += DELTA ? v : b * v;
-              ec[e] += v;
-              z[e] = m * sm.rqk[row] * sm.rqk[C + j] * (DELTA ? 1.f : b);
-              if (DELTA && j < row) {
-                const float l = -d * dl[n][2 * r + e], q = l * kk[row * C + j];
-                fr[r] += q;
-                fc[e] += b * q;
-                y[e] = b * l * sm.rqk[C + row] * sm.rqk[C + j];
-              }
-            }
-          }
-          const uint32_t off = at2<8>(row, col);
-          uint32_t hi, lo;
-          split2(z[0], z[1], hi, lo);
-          sts32(xb_smem_u32(sm.z[0]) + off, hi);
-          sts32(xb_smem_u32(sm.z[1]) + off, lo);
-          if (DELTA) {
-            split2(y[0], y[1], hi, lo);
-            sts32(xb_smem_u32(sm.w[0]) + off, hi);
-            sts32(xb_smem_u32(sm.w[DELTA ? 1 : 0]) + off, lo);
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-#pragma unroll
-          for (int o = 4; o < 32; o <<= 1) {
-            ec[e] += __shfl_xor_sync(0xffffffffu, ec[e], o);
-            if (DELTA) fc[e] += __shfl_xor_sync(0xffffffffu, fc[e], o);
-          }
-          if (g == 0) {
-            sm.ec[rb][col + e] = ec[e];
-            if (DELTA) sm.fc[rb][col + e] = fc[e];
-          }
-        }
-      }
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-#pragma unroll
-        for (int o = 1; o < 4; o <<= 1) {
-          er[r] += __shfl_xor_sync(0xffffffffu, er[r], o);
-          fr[r] += __shfl_xor_sync(0xffffffffu, fr[r], o);
-          rd1[r] += __shfl_xor_sync(0xffffffffu, rd1[r], o);
-          rd2[r] += __shfl_xor_sync(0xffffffffu, rd2[r], o);
-          rd3[r] += __shfl_xor_sync(0xffffffffu, rd3[r], o);
-        }
-        if (t == 0) {
-          const int row = ra + r * 8;
-          sm.er[cb][row] = er[r], sm.fr[cb][row] = fr[r];
-          sm.rd[0][cb][row] = rd1[r], sm.rd[1][cb][row] = rd2[r], sm.rd[2][cb][row] = rd3[r];
-        }
-      }
-      sdot = warp_sum(sdot);
-      if (lane == 0) sm.sdot[w] = sdot;
-      rv += __shfl_xor_sync(0xffffffffu, rv, 1);
-      rv += __shfl_xor_sync(0xffffffffu, rv, 2);
-      if ((tid & 3) == 0) sm.rv[tid >> 2] = rv;
-    }
-    __syncthreads();
-    // dq += Z K, dk += Z^T Q + W K + W^T K
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      const bool row_role = ks <= rb, col_role = ks >= rb;
-      uint32_t zh[4], zl[4], wh[4], wl[4], th[4], tl[4], vh[4], vl[4];
-      if (row_role) {
-        ldsm4(zh, xb_smem_u32(sm.z[0]) + addr_a<8>(rb * 16, ks * 16));
-        ldsm4(zl, xb_smem_u32(sm.z[1]) + addr_a<8>(rb * 16, ks * 16));
-        if (DELTA) {
-          ldsm4(wh, xb_smem_u32(sm.w[0]) + addr_a<8>(rb * 16, ks * 16));
-          ldsm4(wl, xb_smem_u32(sm.w[DELTA ? 1 : 0]) + addr_a<8>(rb * 16, ks * 16));
-        }
-      }
-      if (col_role) {
-        ldsm4t(th, xb_smem_u32(sm.z[0]) + addr_at<8>(rb * 16, ks * 16));
-        ldsm4t(tl, xb_smem_u32(sm.z[1]) + addr_at<8>(rb * 16, ks * 16));
-        if (DELTA) {
-          ldsm4t(vh, xb_smem_u32(sm.w[0]) + addr_at<8>(rb * 16, ks * 16));
-          ldsm4t(vl, xb_smem_u32(sm.w[DELTA ? 1 : 0]) + addr_at<8>(rb * 16, ks * 16));
-        }
-      }
-#pragma unroll
-      for (int n = 0; n < NT; n += 2) {
-        uint32_t bk[4], bq[4];
-        ldsm4t(bk, sk + addr_bt<U>(ks * 16, n0 + n * 8));
-        if (col_role) ldsm4t(bq, sq + addr_bt<U>(ks * 16, n0 + n * 8));
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          if (row_role) {
-            mma(aq[n + e], zl, bk[2 * e], bk[2 * e + 1]);
-            mma(aq[n + e], zh, bk[2 * e], bk[2 * e + 1]);
-            if (DELTA) {
-              mma(ak[n + e], wl, bk[2 * e], bk[2 * e + 1]);
-              mma(ak[n + e], wh, bk[2 * e], bk[2 * e + 1]);
-            }
-          }
-          if (col_role) {
-            mma(ak[n + e], tl, bq[2 * e], bq[2 * e + 1]);
-            mma(ak[n + e], th, bq[2 * e], bq[2 * e + 1]);
-            if (DELTA) {
-              mma(ak[n + e], vl, bk[2 * e], bk[2 * e + 1]);
-              mma(ak[n + e], vh, bk[2 * e], bk[2 * e + 1]);
-            }
-          }
-        }
-      }
-    }
-    // gradients of the log decay (suffix sums of dG) and of b, two rows per lane of one warp
-    if (w == 0) {
-      double x[2], last = 0.0, dsum = 0.0;
-      float db[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int row = 2 * lane + i;
-        const float b = sm.hd[2 * C + row], gam = ex2_sum(sm.hd, row), d = ex2_diff(sm.hd, C - 1, row);
-        const float rq = sm.rqk[row], rk = sm.rqk[C + row];
-        const float q1 = gam * rq * (sm.rd[0][0][row] + sm.rd[0][1][row]);
-        const float k2 = gam * rk * (sm.rd[1][0][row] + sm.rd[1][1][row]);
-        const float k3 = d * rk * (sm.rd[2][0][row] + sm.rd[2][1][row]);
-        const float e1 = sm.er[0][row] + sm.er[1][row];
-        const float e2 = (sm.ec[0][row] + sm.ec[1][row]) + (sm.ec[2][row] + sm.ec[3][row]);
-        if (DELTA) {
-          const float f1 = sm.fr[0][row] + sm.fr[1][row];
-          const float f2 = (sm.fc[0][row] + sm.fc[1][row]) + (sm.fc[2][row] + sm.fc[3][row]);
-          x[i] = (double)q1 + (double)e1 - (double)e2 + (double)(b * f1) - (double)f2 - (double)(b * k2) - (double)k3;
-          last += k3;
-          db[i] = sm.rv[row] - k2 + f1;
-        } else {
-          x[i] = (double)q1 + (double)e1 - (double)(b * e2) - (double)(b * k3);
-          last += (double)(b * k3);
-          db[i] = e2 + k3;
-          dsum += sm.rv[row];
-        }
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        last += __shfl_xor_sync(0xffffffffu, last, o);
-        dsum += __shfl_xor_sync(0xffffffffu, dsum, o);
-      }
-      float sd = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) sd += sm.sdot[i];
-      last += (double)(ex2_sum(sm.hd, C - 1) * sd);
-      double s = x[0] + x[1];
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double y = __shfl_down_sync(0xffffffffu, s, o);
-        if (lane + o < 32) s += y;
-      }
-      double da = 0.0;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int row = 2 * lane + i;
-        const float dg = (float)((i ? x[1] + (s - x[0] - x[1]) : s) + last);
-        if (row < len) {
-          const long long at = (long long)(ch.x + row) * p.Hv + h;
-          if (DELTA) {
-            p.dg[at] = dg, p.db[at] = db[i];
-          } else {
-            p.db[at] = db[i] + dg * p.A[h];
-            da += (double)(dg * sm.hd[2 * C + row]);
-          }
-        }
-      }
-      if (!DELTA) {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) da += __shfl_xor_sync(0xffffffffu, da, o);
-        if (lane == 0) p.part[ch_h * 2] = (float)da, p.part[ch_h * 2 + 1] = (float)dsum;
-      }
-    }
-  }
-  // gradient through the L2 norms: dq - q^ (q^ . dq), rows of norm below 1e-12 excepted
-  if (p.l2norm) {
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int row = ra + r * 8;
-      float a = 0.f, b = 0.f;
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const uint32_t off = at2<U>(row, n0 + n * 8 + 2 * t);
-        const float2 q = unpack_bf16x2(lds32(sq + off)), k = unpack_bf16x2(lds32(sk + off));
-        a += q.x * aq[n][2 * r] + q.y * aq[n][2 * r + 1];
-        b += k.x * ak[n][2 * r] + k.y * ak[n][2 * r + 1];
-      }
-#pragma unroll
-      for (int o = 1; o < 4; o <<= 1) {
-        a += __shfl_xor_sync(0xffffffffu, a, o);
-        b += __shfl_xor_sync(0xffffffffu, b, o);
-      }
-      if (t == 0) sm.dot[0][cb][row] = a, sm.dot[1][cb][row] = b;
-    }
-    __syncthreads();
-  }
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const int row = ra + r * 8;
-    if (row >= len) continue;
-    float fq = 0.f, fk = 0.f;
-    if (p.l2norm) {
-      const float rq = sm.rqk[row] / p.scale, rk = sm.rqk[C + row];
-      if (rq < 0.99e12f) fq = rq * rq * (sm.dot[0][0][row] + sm.dot[0][1][row]);
-      if (rk < 0.99e12f) fk = rk * rk * (sm.dot[1][0][row] + sm.dot[1][1][row]);
-    }
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int col = n0 + n * 8 + 2 * t;
-      if (col < p.dk) {
-        const float2 q = unpack_bf16x2(lds32(sq + at2<U>(row, col))), k = unpack_bf16x2(lds32(sk + at2<U>(row, col)));
-        *reinterpret_cast<uint32_t*>(dq + row * d_t + col) = pack_bf16x2(aq[n][2 * r] - fq * q.x, aq[n][2 * r + 1] - fq * q.y);
-        *reinterpret_cast<uint32_t*>(dk + row * d_t + col) = pack_bf16x2(ak[n][2 * r] - fk * k.x, ak[n][2 * r + 1] - fk * k.y);
-      }
-    }
-  }
-}
-
 // dA and dD: sums of the chunks' parts, in a fixed order
 __global__ void __launch_bounds__(128) rec_reduce(const XbRecArgs p) {
   __shared__ double red[2][4];
@@ -1193,7 +779,7 @@ __global__ void __launch_bounds__(128) rec_reduce(const XbRecArgs p) {
 
 bool bad_args(const XbRecArgs& a) {
   return a.T < 0 || a.n_docs < 0 || a.Hk <= 0 || a.Hv <= 0 || a.Hv % a.Hk || a.dk <= 0 || a.dk > 128 || a.dk % 8 || a.dv <= 0 ||
-         a.dv % 8 || a.dvp != (a.dv + NV - 1) / NV * NV || a.dkp != (a.dk <= 64 ? 64 : 128) || a.nc_max < a.T / C + a.n_docs + 2;
+         a.dv % 8 || a.dvp != (a.dv + 63) / 64 * 64 || a.dkp != (a.dk <= 64 ? 64 : 128) || a.nc_max < a.T / C + a.n_docs + 2;
 }
 
 int plan(const XbRecArgs& a, cudaStream_t st) {
@@ -1217,11 +803,6 @@ int scan_bwd(const XbRecArgs& a, cudaStream_t st) {
   return rec_launch(rec_bwd<DKP, false>, seq, 128, sizeof(BwdSmem<DKP, false>), a, st);
 }
 
-template <int DKP, bool DELTA>
-int grad(const XbRecArgs& a, cudaStream_t st) {
-  return rec_launch(rec_grad<DKP, DELTA>, (long long)a.nc_max * a.Hk, 256, sizeof(GradSmem<DKP, DELTA>), a, st);
-}
-
 }  // namespace
 
 XB_API int xb_recurrence_chunk() { return C; }
@@ -1243,9 +824,9 @@ XB_API int xb_recurrence_bwd(const XbRecArgs* args, int delta, void* stream) {
   cudaStream_t st = (cudaStream_t)stream;
   if (delta) {
     if (int rc = xb_delta_bwd(*a, st)) return rc;
-    return a->dk <= 64 ? grad<64, true>(*a, st) : grad<128, true>(*a, st);
+    return xb_recurrence_grad(*a, 1, st);
   }
   if (int rc = a->dk <= 64 ? scan_bwd<64>(*a, st) : scan_bwd<128>(*a, st)) return rc;
-  if (int rc = a->dk <= 64 ? grad<64, false>(*a, st) : grad<128, false>(*a, st)) return rc;
+  if (int rc = xb_recurrence_grad(*a, 0, st)) return rc;
   return rec_launch(rec_reduce, a->Hv, 128, 0, *a, st);
 }

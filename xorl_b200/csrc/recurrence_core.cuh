@@ -6,6 +6,7 @@
 namespace {
 
 constexpr int C = 64;         // tokens of a chunk
+constexpr int HALF = 128 * 128;   // bytes of an operand tile of 128 rows of 128 bytes
 constexpr int NV = 32;        // state columns of a CTA of the sequential kernels
 constexpr int HD = 3 * C;     // per chunk and v head: G (two floats each, log2 units), b
 constexpr int RQK = 2 * C;    // per chunk and q / k head: row factors of q and k
@@ -149,15 +150,20 @@ __device__ __forceinline__ void state_global(float (&s)[DKP / 64][4][4], float* 
         }
       }
 }
-// the two bf16 planes of the state tile to global memory: [plane][DKP][dvp]
+// the two bf16 planes of the state tile to global memory, as a tile of [128 rows][hi | lo]
 template <int DKP>
-__device__ __forceinline__ void state_save(uint32_t hi, uint32_t lo, bf16* dst, int dvp, int v0) {
+__device__ __forceinline__ void state_save(uint32_t hi, uint32_t lo, uint8_t* dst) {
 #pragma unroll
-  for (int i = 0; i < DKP * 8 / 128; ++i) {
-    const int idx = i * 128 + (threadIdx.x & 127), plane = idx / (DKP * 4), r = (idx / 4) % DKP, u = idx & 3;
-    *reinterpret_cast<uint4*>(dst + ((long long)plane * DKP + r) * dvp + v0 + u * 8) =
-        lds128((plane ? lo : hi) + swz<4>(r, u));
+  for (int i = 0; i < 128 * 8 / 128; ++i) {
+    const int idx = i * 128 + (threadIdx.x & 127), r = idx >> 3, u = idx & 7;
+    const uint4 v = r < DKP ? lds128((u >= 4 ? lo : hi) + swz<4>(r, u & 3)) : make_uint4(0, 0, 0, 0);
+    *reinterpret_cast<uint4*>(dst + r * 128 + ((u ^ (r & 7)) << 4)) = v;
   }
+}
+
+// [T, heads, cols] bf16, boxes of 64 rows of one head
+inline int rec_tile_map(CUtensorMap* m, const void* base, int T, int heads, int cols, long long ld_t, long long ld_h, int box, CUtensorMapSwizzle swz) {
+  return xb_make_tmap_3d(m, base, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, T, heads, cols, T > 1 ? ld_t : 8, heads > 1 ? ld_h : 8, C, 1, box, swz);
 }
 
 template <typename K>
@@ -177,3 +183,5 @@ int rec_launch(K kernel, long long blocks, int threads, size_t smem, const XbRec
 // recurrence_delta.cu: prepare and forward; forward again with the states kept, and the state's gradient
 int xb_delta_fwd(const XbRecArgs& a, cudaStream_t st);
 int xb_delta_bwd(const XbRecArgs& a, cudaStream_t st);
+// recurrence_grad.cu: gradients of q, k, the decay and b from the kept tiles
+int xb_recurrence_grad(const XbRecArgs& a, int delta, cudaStream_t st);

@@ -273,11 +273,12 @@ __global__ void __launch_bounds__(128, 3) delta_prep(const XbRecArgs p) {
 }
 
 // ---- the step of both directions ------------------------------------------------------------------------------------
-constexpr int HALF = 128 * 128;             // [128 rows][64 bf16]: K rows 0 .. 63, Q rows 64 .. 127
+// HALF: [128 rows][64 bf16], K rows 0 .. 63, Q rows 64 .. 127
 constexpr int ST_KQ = 0, ST_TP = 2 * HALF, ST_X = ST_TP + 2 * TP_PLANE, ST_HD = ST_X + C * NV * 2, ST_RQK = ST_HD + HD * 4;
 constexpr int STAGE = (ST_RQK + RQK * 4 + 1023) / 1024 * 1024;
 constexpr int STAGE_BYTES = ST_RQK + RQK * 4;      // what the loads bring, boxes outside a tensor included
-constexpr int SM_S = 2 * STAGE, SM_B2 = SM_S + HALF, SM_B3 = SM_B2 + HALF, SM_BAR = SM_B3 + HALF;
+constexpr int SM_S = 2 * STAGE, SM_B2 = SM_S + HALF, SM_B3 = SM_B2 + HALF, SM_U = SM_B3 + HALF,
+              SM_BAR = SM_U + HALF / 2;
 constexpr int SMEM = SM_BAR + 128 + 1024;
 constexpr int WORKERS = 256, THREADS = WORKERS + 32;
 constexpr int TMEM_COLS = 256, D1 = 0, D2 = 64, D3 = 128;     // accumulators, 64 columns each
@@ -320,6 +321,14 @@ __device__ __forceinline__ void load_stage(const XbRecArgs& p, const Cta& a, con
   bulk_load(st + ST_TP, (const uint8_t*)p.pt + ((long long)c * p.Hv + a.h) * (2 * TP_PLANE), 2 * TP_PLANE, full);
   bulk_load(st + ST_HD, p.hd + ((long long)c * p.Hv + a.h) * HD, HD * 4, full);
   bulk_load(st + ST_RQK, p.rqk + ((long long)c * p.Hk + a.kh) * RQK, RQK * 4, full);
+}
+
+// The state tile of chunk `cs` and the 64-row tile of chunk `cu` to global memory, as they are (-1: none).
+__device__ __forceinline__ void keep_tiles(const XbRecArgs& p, const Cta& a, void* states, void* rows, int cs, int cu) {
+  const int slices = p.dvp / NV, sl = a.v0 / NV;
+  if (cs >= 0) bulk_store((uint8_t*)states + (((long long)cs * p.Hv + a.h) * slices + sl) * HALF, a.smem + SM_S, HALF);
+  if (cu >= 0) bulk_store((uint8_t*)rows + (((long long)cu * p.Hv + a.h) * slices + sl) * (HALF / 2), a.smem + SM_U, HALF / 2);
+  tma_store_commit();
 }
 
 // Rows of K and Q behind the document's end: they hold the next document's, and 0 x Inf is NaN.
@@ -471,10 +480,12 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
         for (int k = 0; k < 8; ++k)
           tc_mma_f16_ss(a.tmem + D1, xb_smem_desc(KMAJ, st + ST_KQ + (k >> 2) * HALF + (k & 3) * 32), xb_smem_desc(MNMAJ, b1 + k * 2048), id, k > 0);
         tc_commit(&a.bars->done[0]);
+        if (SAVE) keep_tiles(p, a, p.s_tiles, p.u_tiles, a.c0 + n, n > 0 ? a.c0 + n - 1 : -1);
       }
       bar(2, THREADS);
       if (one) {
         tc_fence_after();
+        if (SAVE) tma_store_wait_read<0>();
         constexpr uint32_t id = xb_idesc(1, 1, 128, 64, 0, 1);
 #pragma unroll
         for (int k = 0; k < 8; ++k)
@@ -496,6 +507,13 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       }
       __syncwarp();
     }
+    if (SAVE && a.c0 < a.c1) {
+      bar(1, THREADS);
+      if (one) {
+        keep_tiles(p, a, p.s_tiles, p.u_tiles, -1, a.c1 - 1);
+        tma_store_wait_read<0>();
+      }
+    }
   } else {
     const int q4 = warp & 3, half = warp >> 2, r = q4 * 32 + lane, i = r & 63;
     const bool krow = r < C;
@@ -506,16 +524,11 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
     if (p.s_in != nullptr) state_row(const_cast<float*>(p.s_in) + soff, p.s_k, p.s_v, r, p.dk, half * 16, a.vcols, false, s);
     for (int n = 0; n < a.c1 - a.c0; ++n) {
       const int c = a.c0 + n, len = reinterpret_cast<const int4*>(p.chunks)[c].y;
-      const long long ch_h = (long long)c * p.Hv + a.h, t0 = reinterpret_cast<const int4*>(p.chunks)[c].x;
+      const long long t0 = reinterpret_cast<const int4*>(p.chunks)[c].x;
       uint8_t* st = a.smem + (n & 1) * STAGE;
       const float* hd = reinterpret_cast<const float*>(st + ST_HD);
       const float* rqk = reinterpret_cast<const float*>(st + ST_RQK);
       put_row(a.smem + SM_S, r, half, s, hi, lo);
-      if (SAVE && r < p.dkp) {
-        bf16* pl = (bf16*)p.s_planes + (ch_h * 2 * p.dkp + r) * p.dvp + a.v0 + half * 16;
-        store16(pl, hi);
-        store16(pl + (long long)p.dkp * p.dvp, lo);
-      }
       a.wait(&a.bars->full[n & 1], (n >> 1) & 1, 3);
       if (len < C) clear_rows(st, len);
       fence_proxy_async_smem();
@@ -544,13 +557,7 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       tc_fence_after();
       read_acc(acc + D2, x);
       if (krow) {                            // d rk U
-        if (SAVE) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) split2(x[2 * e], x[2 * e + 1], hi[e], lo[e]);
-          bf16* pl = (bf16*)p.u_planes + (ch_h * 2 * C + i) * p.dvp + a.v0 + half * 16;
-          store16(pl, hi);
-          store16(pl + (long long)C * p.dvp, lo);
-        }
+        if (SAVE) put_row(a.smem + SM_U, i, half, x, hi, lo);
         const float f = dec * rk;
 #pragma unroll
         for (int e = 0; e < 16; ++e) x[e] *= f;
@@ -576,6 +583,8 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] = last * s[e] + y[e];
     }
+    fence_proxy_async_smem();
+    if (SAVE && a.c0 < a.c1) bar_arrive(1, THREADS);
     if (p.s_out != nullptr) state_row(p.s_out + soff, p.s_k, p.s_v, r, p.dk, half * 16, a.vcols, true, s);
   }
   cta_end(a);
@@ -616,10 +625,12 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
 #pragma unroll
         for (int k = 4; k < 8; ++k)          // rows of Q
           tc_mma_f16_ss(a.tmem + D3, xb_smem_desc(MNMAJ, st + ST_KQ + k * 2048), xb_smem_desc(MNMAJ, b3 + k * 2048), id3, k > 4);
+        keep_tiles(p, a, p.ds_tiles, p.dr_tiles, a.c1 - 1 - n, n > 0 ? a.c1 - n : -1);
       }
       bar(2, THREADS);
       if (one) {
         tc_fence_after();
+        tma_store_wait_read<0>();
         constexpr uint32_t id = xb_idesc(1, 1, 64, 64, 1, 1);
 #pragma unroll
         for (int k = 0; k < 16; ++k)
@@ -639,6 +650,13 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
         }
       }
       __syncwarp();
+    }
+    if (steps > 0) {
+      bar(1, THREADS);
+      if (one) {
+        keep_tiles(p, a, p.ds_tiles, p.dr_tiles, -1, a.c0);
+        tma_store_wait_read<0>();
+      }
     }
   } else {
     const int q4 = warp & 3, half = warp >> 2, r = q4 * 32 + lane, i = r & 63;
@@ -674,16 +692,11 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
     if (steps > 0) put_dy(0);
     for (int n = 0; n < steps; ++n) {
       const int c = a.c1 - 1 - n, len = reinterpret_cast<const int4*>(p.chunks)[c].y;
-      const long long ch_h = (long long)c * p.Hv + a.h, t0 = reinterpret_cast<const int4*>(p.chunks)[c].x;
+      const long long t0 = reinterpret_cast<const int4*>(p.chunks)[c].x;
       uint8_t* st = a.smem + (n & 1) * STAGE;
       const float* hd = reinterpret_cast<const float*>(st + ST_HD);
       const float* rqk = reinterpret_cast<const float*>(st + ST_RQK);
       put_row(a.smem + SM_S, r, half, s, hi, lo);
-      if (r < p.dkp) {
-        bf16* pl = (bf16*)p.ds_planes + (ch_h * 2 * p.dkp + r) * p.dvp + a.v0 + half * 16;
-        store16(pl, hi);
-        store16(pl + (long long)p.dkp * p.dvp, lo);
-      }
       fence_proxy_async_smem();
       tc_fence_before();
       bar_arrive(1, THREADS);
@@ -713,11 +726,7 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       tc_fence_before();
       bar_arrive(3, THREADS);
       if (lane < 16) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) split2(dr[2 * e], dr[2 * e + 1], hi[e], lo[e]);
-        bf16* pl = (bf16*)p.dr_planes + (ch_h * 2 * C + ri) * p.dvp + a.v0 + half * 16;
-        store16(pl, hi);
-        store16(pl + (long long)C * p.dvp, lo);
+        put_row(a.smem + SM_U, ri, half, dr, hi, lo);
         if (ri < len) {
           bf16* dst = dv + (t0 + ri) * dv_t + half * 16;
 #pragma unroll
@@ -736,23 +745,21 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] = last * s[e] + x[e];
     }
+    fence_proxy_async_smem();
+    if (steps > 0) bar_arrive(1, THREADS);
     if (p.ds_in != nullptr) state_row(p.ds_in + soff, p.s_k, p.s_v, r, p.dk, half * 16, a.vcols, true, s);
   }
   cta_end(a);
 }
 
-// [T, heads, cols] bf16, boxes of 64 rows of one head
-int tile_map(CUtensorMap* m, const void* base, int T, int heads, int cols, long long ld_t, long long ld_h, int box, CUtensorMapSwizzle swz) {
-  return xb_make_tmap_3d(m, base, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, T, heads, cols, T > 1 ? ld_t : 8, heads > 1 ? ld_h : 8, C, 1, box, swz);
-}
 template <typename K>
 int run(K kernel, const XbRecArgs& a, const void* x, long long x_t, long long x_h, cudaStream_t st) {
   const long long blocks = (long long)(a.n_docs + 2) * a.Hv * (a.dvp / NV);
   if (blocks > 0x7fffffffLL) return -4;
   CUtensorMap mk{}, mq{}, mx{};
-  if (a.T > 0 && (tile_map(&mk, a.k, a.T, a.Hk, a.dk, a.k_t, a.k_h, 64, CU_TENSOR_MAP_SWIZZLE_128B) ||
-                  tile_map(&mq, a.q, a.T, a.Hk, a.dk, a.q_t, a.q_h, 64, CU_TENSOR_MAP_SWIZZLE_128B) ||
-                  tile_map(&mx, x, a.T, a.Hv, a.dv, x_t, x_h, NV, CU_TENSOR_MAP_SWIZZLE_64B)))
+  if (a.T > 0 && (rec_tile_map(&mk, a.k, a.T, a.Hk, a.dk, a.k_t, a.k_h, 64, CU_TENSOR_MAP_SWIZZLE_128B) ||
+                  rec_tile_map(&mq, a.q, a.T, a.Hk, a.dk, a.q_t, a.q_h, 64, CU_TENSOR_MAP_SWIZZLE_128B) ||
+                  rec_tile_map(&mx, x, a.T, a.Hv, a.dv, x_t, x_h, NV, CU_TENSOR_MAP_SWIZZLE_64B)))
     return -2;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess) {
     cudaGetLastError();

@@ -1,0 +1,524 @@
+// Gated linear recurrences, the parallel part of the backward pass: gradients of q, k, the log decay and b of one chunk
+// from the states that enter it, the gradients of the states that leave it, U and dR (formulas in recurrence.cu).
+//
+// One CTA per chunk and q / k head.  It walks over the v heads that share the q / k head and over their state columns,
+// 32 at a time, and forms five products in tensor memory, all with 64 rows of tokens:
+//   dP = dO U^T,  dL = dR U^T  [64 x 64];   t1 = dO S^T,  t2 = dR S^T,  t3 = U dS'^T  [64 x 128]
+// (scan: U = V, no dL and t2.)  A computed operand is a tile of [hi 32 | lo 32] columns; the parts of a product are the
+// pairs of 16-column steps hi hi, hi lo, lo hi.  Behind each head the rows of t1 .. t3 are scaled and added up in
+// registers, their dot products with q and k give the gradient of the decay and of b, and D o dP, D o dL are added up;
+// the products with K and Q are the same for all heads of the group and are made once, from the sums.
+// The tiles that it reads (60 KB per head and 32 columns; scan 40 KB) bound it: they are what the two sequential passes
+// keep.  Sixteen worker warps, a loading and an issuing warp; 64-row accumulators lie in 16 lanes of each warp.
+#include "recurrence_core.cuh"
+
+namespace {
+
+constexpr int WORKERS = 512, THREADS = WORKERS + 64;
+constexpr int T64 = HALF / 2;                       // 8 KB: [64 rows][128 bytes]
+template <bool DELTA>
+struct Lay {
+  static constexpr int RING = DELTA ? 2 : 3;
+  static constexpr int ST_S = 0, ST_DS = HALF, ST_U = 2 * HALF, ST_R = 2 * HALF + T64;
+  static constexpr int STAGE = 2 * HALF + (DELTA ? 2 * T64 : 0);
+  static constexpr int DOV = 4 * T64 + 1024;        // dO, V: 128 columns each; the head's decays
+  static constexpr int SM_Q = 0, SM_K = 2 * T64, SM_RING = 4 * T64, SM_DOV = SM_RING + RING * STAGE, SM_RED = SM_DOV + 2 * DOV;
+};
+struct Red {                                        // what meets across warps, one set per head in turn
+  float rd[3][4][C];                                // q.t1, k.t2, k.t3 by column quarter
+  float er[4][C], fr[4][C];                         // row sums of dP o P and dL o A by column quarter (scan: dP o P)
+  float ec[4][C], fc[4][C];                         // column sums by row block
+  float rv[C], sdot[16];
+};
+struct __align__(8) Bars {
+  uint64_t full[3], empty[3], dov_full[2], dov_empty[2], qk_full, acc_full, acc_empty, last;
+  uint32_t tmem;
+  int abort_flag;
+};
+template <bool DELTA>
+constexpr int smem_bytes() { return Lay<DELTA>::SM_RED + 2 * (int)sizeof(Red) + RQK * 4 + 256 + 1024; }
+constexpr int COL_P = 0, COL_L = 64, COL_T1 = 128, COL_T2 = 256, COL_T3 = 384;
+
+__device__ __forceinline__ void wbar() { asm volatile("bar.sync 1, %0;" ::"n"(WORKERS) : "memory"); }
+
+// D (64 x N) += A (64 x 16 of a row of 16-column steps) B^T: one step each
+__device__ __forceinline__ void step(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool first) {
+  constexpr uint64_t kmaj = xb_smem_desc_base_sw128(16, 1024);
+  tc_mma_f16_ss(d, xb_smem_desc(kmaj, a), xb_smem_desc(kmaj, b), idesc, first ? 0u : 1u);
+}
+// hi hi, hi lo, lo hi of two [hi | lo] tiles; EXACT: a is 32 plain columns
+template <bool EXACT>
+__device__ __forceinline__ void product(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool first) {
+  step(d, a, b, idesc, first);
+  step(d, a + 32, b + 32, idesc, false);
+  step(d, a, b + 64, idesc, false);
+  step(d, a + 32, b + 96, idesc, false);
+  if (!EXACT) {
+    step(d, a + 64, b, idesc, false);
+    step(d, a + 96, b + 32, idesc, false);
+  }
+}
+// sum over the 16 lanes of a half warp of 8 values each; lane l keeps the sum of value l % 8
+__device__ __forceinline__ float col_sum(float (&v)[8]) {
+  const int l = threadIdx.x & 15;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], 8);
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < o; ++i) {
+      const float mine = l & o ? v[i + o] : v[i], other = l & o ? v[i] : v[i + o];
+      v[i] = mine + __shfl_xor_sync(0xffffffffu, other, o);
+    }
+  return v[0];
+}
+// A 64-row accumulator lies in lanes 0 .. 15 of each warp; lanes 16 .. 31 take the second half of its 2 N columns.
+template <int N>
+__device__ __forceinline__ void spread(const uint32_t (&t)[2 * N], float (&x)[N]) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const uint32_t far = __shfl_sync(0xffffffffu, t[N + e], threadIdx.x & 15);
+    x[e] = __uint_as_float(threadIdx.x & 16 ? far : t[e]);
+  }
+}
+// 32 bf16 values of row `row` of a [64][256 bytes] tile in two halves of 64 columns
+__device__ __forceinline__ uint4 tile_unit(const uint8_t* tile, int row, int unit) {
+  return *reinterpret_cast<const uint4*>(tile + (unit >> 3) * T64 + row * 128 + (((unit & 7) ^ (row & 7)) << 4));
+}
+__device__ __forceinline__ void floats8(const uint4 u, float (&x)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 f = unpack_bf16x2(w[j]);
+    x[2 * j] = f.x, x[2 * j + 1] = f.y;
+  }
+}
+// acc += f * t over this thread's 16 columns (from unit `unit`) of its row; returns t . (the same columns of `tile`)
+__device__ __forceinline__ float add_rows(uint32_t addr, const uint8_t* tile, int row, int unit, float f, float (&acc)[16]) {
+  uint32_t t[32];
+  float y[16];
+  tmem_ld_32x32(addr, t);
+  tc_wait_ld();
+  spread<16>(t, y);
+  float dot = 0.f;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    float x[8];
+    floats8(tile_unit(tile, row, unit + u), x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      dot += x[e] * y[8 * u + e];
+      acc[8 * u + e] += f * y[8 * u + e];
+    }
+  }
+  return dot + __shfl_xor_sync(0xffffffffu, dot, 16);
+}
+
+template <bool DELTA>
+__global__ void __launch_bounds__(THREADS, 1)
+rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+         const __grid_constant__ CUtensorMap my, const __grid_constant__ XbRecArgs p) {
+  using L = Lay<DELTA>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  Red* red = reinterpret_cast<Red*>(smem + L::SM_RED);
+  float* rqk = reinterpret_cast<float*>(red + 2);
+  Bars* bars = reinterpret_cast<Bars*>(rqk + RQK);
+  const int kh = blockIdx.x % p.Hk, c = blockIdx.x / p.Hk, rep = p.Hv / p.Hk;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (c >= p.doc_off[p.n_docs + 2]) return;
+  const int4 ch = reinterpret_cast<const int4*>(p.chunks)[c];
+  const int len = ch.y;
+  bf16* dq = (bf16*)p.dq + (ch.x * (long long)p.Hk + kh) * p.dk;
+  bf16* dk = (bf16*)p.dk_out + (ch.x * (long long)p.Hk + kh) * p.dk;
+  const long long d_t = (long long)p.Hk * p.dk;
+  if (DELTA && ch.z >= p.n_docs) {                  // rows outside the documents
+    for (int i = tid; i < len * p.dk; i += THREADS) {
+      dq[(i / p.dk) * d_t + i % p.dk] = __float2bfloat16(0.f);
+      dk[(i / p.dk) * d_t + i % p.dk] = __float2bfloat16(0.f);
+    }
+    for (int i = tid; i < len * rep; i += THREADS) {
+      const long long at = (long long)(ch.x + i / rep) * p.Hv + kh * rep + i % rep;
+      p.dg[at] = 0.f, p.db[at] = 0.f;
+    }
+    return;
+  }
+  const int slices = p.dvp / NV, passes = (slices + 3) / 4;
+  if (tid == 0) {
+    for (int i = 0; i < 3; ++i) mbar_init(&bars->full[i], 1), mbar_init(&bars->empty[i], 1 + WORKERS / 32);
+    for (int i = 0; i < 2; ++i) mbar_init(&bars->dov_full[i], 1), mbar_init(&bars->dov_empty[i], 1 + WORKERS / 32);
+    mbar_init(&bars->qk_full, 1), mbar_init(&bars->acc_full, 1), mbar_init(&bars->acc_empty, WORKERS / 32), mbar_init(&bars->last, 1);
+    bars->abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == WORKERS / 32) {
+    tmem_alloc(&bars->tmem, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem;
+  // a wait that runs out raises a flag; from then on waits return at once and every role walks to its end
+  auto wait = [&](uint64_t* b, uint32_t parity, int detail) { mbar_wait(b, parity, &bars->abort_flag, p.status, XB_K_RECURRENCE, detail); };
+
+  if (warp == WORKERS / 32) {
+    // ------------------------------------------------ loads ------------------------------------------------
+    if (xb_elect_one()) {
+      mbar_expect_tx(&bars->qk_full, 4 * T64 + RQK * 4);
+      for (int i = 0; i < 2; ++i) {
+        tma_load_3d(smem + L::SM_Q + i * T64, &mq, &bars->qk_full, i * 64, kh, ch.x);
+        tma_load_3d(smem + L::SM_K + i * T64, &mk, &bars->qk_full, i * 64, kh, ch.x);
+      }
+      bulk_load(rqk, p.rqk + ((long long)c * p.Hk + kh) * RQK, RQK * 4, &bars->qk_full);
+      int n = 0, m = 0;
+      for (int hh = 0; hh < rep; ++hh) {
+        const int h = kh * rep + hh;
+        const long long ch_h = (long long)c * p.Hv + h;
+        for (int pass = 0; pass < passes; ++pass, ++m) {
+          uint8_t* dov = smem + L::SM_DOV + (m & 1) * L::DOV;
+          wait(&bars->dov_empty[m & 1], ((m >> 1) & 1) ^ 1, 20);
+          mbar_expect_tx(&bars->dov_full[m & 1], 4 * T64 + HD * 4);
+          for (int i = 0; i < 2; ++i) {
+            tma_load_3d(dov + i * T64, &my, &bars->dov_full[m & 1], pass * 128 + i * 64, h, ch.x);
+            tma_load_3d(dov + (2 + i) * T64, &mv, &bars->dov_full[m & 1], pass * 128 + i * 64, h, ch.x);
+          }
+          bulk_load(dov + 4 * T64, p.hd + ch_h * HD, HD * 4, &bars->dov_full[m & 1]);
+          for (int sl = pass * 4; sl < min(slices, pass * 4 + 4); ++sl, ++n) {
+            const int s = n % L::RING;
+            uint8_t* st = smem + L::SM_RING + s * L::STAGE;
+            wait(&bars->empty[s], ((n / L::RING) & 1) ^ 1, 21);
+            mbar_expect_tx(&bars->full[s], L::STAGE);
+            const long long at = ch_h * slices + sl;
+            bulk_load(st + L::ST_S, (const uint8_t*)p.s_tiles + at * HALF, HALF, &bars->full[s]);
+            if (DELTA) {
+              bulk_load(st + L::ST_U, (const uint8_t*)p.u_tiles + at * T64, T64, &bars->full[s]);
+              bulk_load(st + L::ST_R, (const uint8_t*)p.dr_tiles + at * T64, T64, &bars->full[s]);
+            }
+            bulk_load(st + L::ST_DS, (const uint8_t*)p.ds_tiles + at * HALF, HALF, &bars->full[s]);
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == WORKERS / 32 + 1) {
+    // ------------------------------------------------ products ----------------------------------------------
+    if (xb_elect_one()) {
+      constexpr uint32_t id64 = xb_idesc(1, 1, 64, 64, 0, 0), id128 = xb_idesc(1, 1, 64, 128, 0, 0);
+      int n = 0, m = 0;
+      for (int hh = 0; hh < rep; ++hh) {
+        wait(&bars->acc_empty, (hh & 1) ^ 1, 30);
+        for (int pass = 0; pass < passes; ++pass, ++m) {
+          const uint32_t y0 = xb_smem_u32(smem + L::SM_DOV + (m & 1) * L::DOV), x0 = y0 + 2 * T64;
+          wait(&bars->dov_full[m & 1], (m >> 1) & 1, 31);
+          for (int sl = pass * 4; sl < min(slices, pass * 4 + 4); ++sl, ++n) {
+            const int s = n % L::RING, q = sl & 3;
+            const uint32_t st = xb_smem_u32(smem + L::SM_RING + s * L::STAGE);
+            const uint32_t y = y0 + (q >> 1) * T64 + (q & 1) * 64, x = x0 + (q >> 1) * T64 + (q & 1) * 64;
+            const bool first = sl == 0;
+            wait(&bars->full[s], (n / L::RING) & 1, 32);
+            tc_fence_after();
+            if (DELTA) {
+              product<true>(tmem + COL_P, y, st + L::ST_U, id64, first);
+              product<false>(tmem + COL_L, st + L::ST_R, st + L::ST_U, id64, first);
+              product<true>(tmem + COL_T1, y, st + L::ST_S, id128, first);
+              product<false>(tmem + COL_T2, st + L::ST_R, st + L::ST_S, id128, first);
+              product<false>(tmem + COL_T3, st + L::ST_U, st + L::ST_DS, id128, first);
+            } else {
+              step(tmem + COL_P, y, x, id64, first);
+              step(tmem + COL_P, y + 32, x + 32, id64, false);
+              product<true>(tmem + COL_T1, y, st + L::ST_S, id128, first);
+              product<true>(tmem + COL_T3, x, st + L::ST_DS, id128, first);
+            }
+            tc_commit(&bars->empty[s]);
+          }
+          tc_commit(&bars->dov_empty[m & 1]);
+        }
+        tc_commit(&bars->acc_full);
+      }
+      // dq = Z K, dk = W K + W^T K + Z^T Q, from the sums over the heads
+      wait(&bars->acc_empty, (rep & 1) ^ 1, 33);
+      tc_fence_after();
+      constexpr uint64_t kmaj = xb_smem_desc_base_sw128(16, 1024), mn = xb_smem_desc_base_sw128(T64, 1024);
+      constexpr uint32_t idr = xb_idesc(1, 1, 64, 128, 0, 1), idc = xb_idesc(1, 1, 64, 128, 1, 1);
+      const uint32_t z = xb_smem_u32(smem + L::SM_RING), sk = xb_smem_u32(smem + L::SM_K), sq = xb_smem_u32(smem + L::SM_Q);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {                  // planes hi, lo; four steps of 16 tokens
+        const uint32_t t = z + (i >> 2) * T64, w = t + 2 * T64, k = (uint32_t)(i & 3);
+        tc_mma_f16_ss(tmem + COL_T1, xb_smem_desc(kmaj, t + k * 32), xb_smem_desc(mn, sk + k * 2048), idr, i > 0);
+        tc_mma_f16_ss(tmem + COL_T2, xb_smem_desc(mn, t + k * 2048), xb_smem_desc(mn, sq + k * 2048), idc, i > 0);
+        if (DELTA) {
+          tc_mma_f16_ss(tmem + COL_T2, xb_smem_desc(kmaj, w + k * 32), xb_smem_desc(mn, sk + k * 2048), idr, 1);
+          tc_mma_f16_ss(tmem + COL_T2, xb_smem_desc(mn, w + k * 2048), xb_smem_desc(mn, sk + k * 2048), idc, 1);
+        }
+      }
+      tc_commit(&bars->last);
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------ workers -----------------------------------------------
+    // row `row`; 16 of 128 columns (from unit cu) of the wide products, 8 of 64 (from j0) of the square ones
+    const int q4 = warp & 3, qd = warp >> 2, row = q4 * 16 + (lane & 15), cu = qd * 4 + (lane >> 4) * 2, j0 = qd * 16 + (lane >> 4) * 8;
+    const bool act = lane < 16;
+    const uint32_t base = tmem + ((uint32_t)(q4 * 32) << 16);
+    float aq[16] = {}, ak[16] = {}, az[8] = {}, aw[8] = {};
+    auto wwait = [&](uint64_t* b, uint32_t parity, int detail) {
+      wait(b, parity, detail);
+      __syncwarp();
+    };
+    auto arrive = [&](uint64_t* b) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(b);
+    };
+    wwait(&bars->qk_full, 0, 40);
+    const float rq = rqk[row], rk = rqk[C + row];
+    const float* qk = p.qk + ((long long)c * p.Hk + kh) * (C * C) + row * C + j0;
+    const float* kk = DELTA ? p.kk + ((long long)c * p.Hk + kh) * (C * C) + row * C + j0 : nullptr;
+    int n = 0, m = 0;
+    for (int hh = 0; hh < rep; ++hh) {
+      const int h = kh * rep + hh;
+      const long long ch_h = (long long)c * p.Hv + h;
+      Red& r = red[hh & 1];
+      float sdot = 0.f, rv = 0.f;
+      const float* hd = nullptr;
+      for (int pass = 0; pass < passes; ++pass, ++m) {
+        const uint8_t* dov = smem + L::SM_DOV + (m & 1) * L::DOV;
+        hd = reinterpret_cast<const float*>(dov + 4 * T64);
+        wwait(&bars->dov_full[m & 1], (m >> 1) & 1, 41);
+        for (int sl = pass * 4; sl < min(slices, pass * 4 + 4); ++sl, ++n) {
+          const int s = n % L::RING;
+          const uint8_t* st = smem + L::SM_RING + s * L::STAGE;
+          wwait(&bars->full[s], (n / L::RING) & 1, 42);
+          {  // <S, dS'>: a unit of eight columns of a row per thread
+            const int sr = tid >> 2, u = tid & 3;
+            const uint32_t hi = (uint32_t)(sr * 128 + ((u ^ (sr & 7)) << 4)), lo = (uint32_t)(sr * 128 + (((u + 4) ^ (sr & 7)) << 4));
+            float a[8], al[8], b[8], bl[8];
+            floats8(*reinterpret_cast<const uint4*>(st + L::ST_S + hi), a), floats8(*reinterpret_cast<const uint4*>(st + L::ST_S + lo), al);
+            floats8(*reinterpret_cast<const uint4*>(st + L::ST_DS + hi), b), floats8(*reinterpret_cast<const uint4*>(st + L::ST_DS + lo), bl);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sdot += (a[e] + al[e]) * (b[e] + bl[e]);
+          }
+          if (tid < 4 * C) {  // dR.v (scan: dO.v)
+            const int sr = tid >> 2, u = tid & 3;
+            float v[8], a[8], al[8];
+            floats8(tile_unit(dov + 2 * T64, sr, (sl & 3) * 4 + u), v);
+            if (DELTA) {
+              floats8(*reinterpret_cast<const uint4*>(st + L::ST_R + sr * 128 + ((u ^ (sr & 7)) << 4)), a);
+              floats8(*reinterpret_cast<const uint4*>(st + L::ST_R + sr * 128 + (((u + 4) ^ (sr & 7)) << 4)), al);
+            } else {
+              floats8(tile_unit(dov, sr, (sl & 3) * 4 + u), a);
+            }
+            if (sr < len)
+#pragma unroll
+              for (int e = 0; e < 8; ++e) rv += (DELTA ? a[e] + al[e] : a[e]) * v[e];
+          }
+          arrive(&bars->empty[s]);
+        }
+        if (pass + 1 < passes) arrive(&bars->dov_empty[m & 1]);     // the last one is given back below: its decays are read
+      }
+      sdot = warp_sum(sdot);
+      if (lane == 0) r.sdot[warp] = sdot;
+      rv += __shfl_xor_sync(0xffffffffu, rv, 1);
+      rv += __shfl_xor_sync(0xffffffffu, rv, 2);
+      if (tid < 4 * C && (tid & 3) == 0) r.rv[tid >> 2] = rv;
+      const float b = hd[2 * C + row], gam = ex2_sum(hd, row), dec = ex2_diff(hd, C - 1, row);
+      wwait(&bars->acc_full, hh & 1, 43);
+      tc_fence_after();
+      {
+        const bool on = row < len;                                    // rows behind the end hold other documents' products
+        const float f1 = on ? gam * rq : 0.f, f2 = on ? -b * gam * rk : 0.f, f3 = on ? dec * rk * (DELTA ? 1.f : b) : 0.f;
+        const float d1 = add_rows(base + COL_T1 + qd * 32, smem + L::SM_Q, row, cu, f1, aq);
+        const float d2 = DELTA ? add_rows(base + COL_T2 + qd * 32, smem + L::SM_K, row, cu, f2, ak) : 0.f;
+        const float d3 = add_rows(base + COL_T3 + qd * 32, smem + L::SM_K, row, cu, f3, ak);
+        if (act) r.rd[0][qd][row] = d1, r.rd[1][qd][row] = d2, r.rd[2][qd][row] = d3;
+      }
+      {
+        uint32_t t[16];
+        float pr[8], lr[8] = {}, ec[8], fc[8], er = 0.f, fr = 0.f;
+        tmem_ld_32x16(base + COL_P + qd * 16, t);
+        tc_wait_ld();
+        spread<8>(t, pr);
+        if (DELTA) {
+          tmem_ld_32x16(base + COL_L + qd * 16, t);
+          tc_wait_ld();
+          spread<8>(t, lr);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int j = j0 + e;
+          ec[e] = fc[e] = 0.f;
+          if (j <= row && row < len) {
+            const float d = ex2_diff(hd, row, j), bj = DELTA ? 1.f : hd[2 * C + j], g = d * pr[e];
+            const float v = g * qk[e];
+            er += bj * v;
+            ec[e] = v;
+            az[e] += g * rq * rqk[C + j] * bj;
+            if (DELTA && j < row) {
+              const float l = -d * lr[e], w = l * kk[e];
+              fr += w;
+              fc[e] = b * w;
+              aw[e] += b * l * rk * rqk[C + j];
+            }
+          }
+        }
+        er += __shfl_xor_sync(0xffffffffu, er, 16), fr += __shfl_xor_sync(0xffffffffu, fr, 16);
+        if (act) r.er[qd][row] = er, r.fr[qd][row] = fr;
+        const float es = col_sum(ec), fs = DELTA ? col_sum(fc) : 0.f;
+        if ((lane & 8) == 0) r.ec[q4][j0 + (lane & 7)] = es, r.fc[q4][j0 + (lane & 7)] = fs;
+      }
+      tc_fence_before();
+      if (hh + 1 < rep) arrive(&bars->acc_empty);
+      wbar();
+      if (warp == 0) {
+        // gradients of the log decay (suffix sums of dG) and of b: two rows per lane
+        double x[2], tail = 0.0, dsum = 0.0;
+        float db[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int t = 2 * lane + i;
+          const float bt = hd[2 * C + t], ga = ex2_sum(hd, t), de = ex2_diff(hd, C - 1, t);
+          const bool on = t < len;
+          auto four = [&](const float (&a)[4][C]) { return (a[0][t] + a[1][t]) + (a[2][t] + a[3][t]); };
+          const float q1 = on ? ga * rqk[t] * four(r.rd[0]) : 0.f, k2 = on && DELTA ? ga * rqk[C + t] * four(r.rd[1]) : 0.f;
+          const float k3 = on ? de * rqk[C + t] * four(r.rd[2]) : 0.f;
+          const float e1 = four(r.er), e2 = four(r.ec), g1 = four(r.fr), g2 = four(r.fc);
+          if (DELTA) {
+            x[i] = (double)q1 + (double)e1 - (double)e2 + (double)(bt * g1) - (double)g2 - (double)(bt * k2) - (double)k3;
+            tail += k3;
+            db[i] = r.rv[t] - k2 + g1;
+          } else {
+            x[i] = (double)q1 + (double)e1 - (double)(bt * e2) - (double)(bt * k3);
+            tail += (double)(bt * k3);
+            db[i] = e2 + k3;
+            dsum += r.rv[t];
+          }
+        }
+        float sd = lane < 16 ? r.sdot[lane] : 0.f;
+        sd = warp_sum(sd);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+          tail += __shfl_xor_sync(0xffffffffu, tail, o);
+          dsum += __shfl_xor_sync(0xffffffffu, dsum, o);
+        }
+        tail += (double)(ex2_sum(hd, C - 1) * sd);
+        double s = x[0] + x[1];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double y = __shfl_down_sync(0xffffffffu, s, o);
+          if (lane + o < 32) s += y;
+        }
+        double da = 0.0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int t = 2 * lane + i;
+          const float dg = (float)((i ? s - x[0] : s) + tail);
+          if (t < len) {
+            const long long at = (long long)(ch.x + t) * p.Hv + h;
+            if (DELTA) {
+              p.dg[at] = dg, p.db[at] = db[i];
+            } else {
+              p.db[at] = db[i] + dg * p.A[h];
+              da += (double)(dg * hd[2 * C + t]);
+            }
+          }
+        }
+        if (!DELTA) {
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) da += __shfl_xor_sync(0xffffffffu, da, o);
+          if (lane == 0) p.part[ch_h * 2] = (float)da, p.part[ch_h * 2 + 1] = (float)dsum;
+        }
+      }
+      arrive(&bars->dov_empty[(m - 1) & 1]);
+    }
+    // Z and W as operand tiles over the ring, whose last tiles have been read; K and Q without rows behind the end
+    {
+      uint8_t* t = smem + L::SM_RING + row * 128;
+#pragma unroll
+      for (int part = 0; part < (DELTA ? 2 : 1); ++part) {
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          split2(part ? aw[2 * e] : az[2 * e], part ? aw[2 * e + 1] : az[2 * e + 1], hi[e], lo[e]);
+        const int off = part * 2 * T64 + (((j0 >> 3) ^ (row & 7)) << 4);
+        *reinterpret_cast<uint4*>(t + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(t + off + T64) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      }
+    }
+    for (int i = tid; i < 4 * (C - len) * 8; i += WORKERS) {
+      const int part = i / ((C - len) * 8), rr = len + (i % ((C - len) * 8)) / 8;
+      reinterpret_cast<uint4*>(smem + L::SM_Q + part * T64 + rr * 128)[i & 7] = make_uint4(0, 0, 0, 0);
+    }
+    fence_proxy_async_smem();
+    tc_fence_before();
+    arrive(&bars->acc_empty);
+    wwait(&bars->last, 0, 44);
+    tc_fence_after();
+    add_rows(base + COL_T1 + qd * 32, smem + L::SM_Q, row, cu, 1.f, aq);
+    add_rows(base + COL_T2 + qd * 32, smem + L::SM_K, row, cu, 1.f, ak);
+    // gradient through the L2 norms: dq - q^ (q^ . dq), rows of norm below 1e-12 excepted
+    float fq = 0.f, fk = 0.f;
+    if (p.l2norm) {
+      float sq = 0.f, sk = 0.f;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        float x[8], y[8];
+        floats8(tile_unit(smem + L::SM_Q, row, cu + u), x), floats8(tile_unit(smem + L::SM_K, row, cu + u), y);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sq += x[e] * aq[8 * u + e], sk += y[e] * ak[8 * u + e];
+      }
+      sq += __shfl_xor_sync(0xffffffffu, sq, 16), sk += __shfl_xor_sync(0xffffffffu, sk, 16);
+      Red& r = red[rep & 1];
+      if (act) r.rd[0][qd][row] = sq, r.rd[1][qd][row] = sk;
+      wbar();
+      const float nq = rq / p.scale;
+      if (nq < 0.99e12f) fq = nq * nq * ((r.rd[0][0][row] + r.rd[0][1][row]) + (r.rd[0][2][row] + r.rd[0][3][row]));
+      if (rk < 0.99e12f) fk = rk * rk * ((r.rd[1][0][row] + r.rd[1][1][row]) + (r.rd[1][2][row] + r.rd[1][3][row]));
+    }
+    if (row < len)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int col = (cu + u) * 8;
+        if (col < p.dk) {
+          float x[8], y[8];
+          floats8(tile_unit(smem + L::SM_Q, row, cu + u), x), floats8(tile_unit(smem + L::SM_K, row, cu + u), y);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = aq[8 * u + e] - fq * x[e], y[e] = ak[8 * u + e] - fk * y[e];
+          *reinterpret_cast<uint4*>(dq + row * d_t + col) =
+              make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+          *reinterpret_cast<uint4*>(dk + row * d_t + col) =
+              make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7]));
+        }
+      }
+  }
+  // after a wait that ran out, loads and products may still be on their way: give them 0.2 s
+  if (*(volatile int*)&bars->abort_flag && tid == 0)
+    for (const uint64_t t0 = xb_globaltimer(); xb_globaltimer() - t0 < 200000000ull;) {}
+  tc_fence_before();
+  __syncthreads();
+  if (warp == WORKERS / 32) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <bool DELTA>
+int run(const XbRecArgs& a, cudaStream_t st) {
+  const long long blocks = (long long)a.nc_max * a.Hk;
+  if (blocks > 0x7fffffffLL) return -4;
+  CUtensorMap mq{}, mk{}, mv{}, my{};
+  if (a.T > 0 && (rec_tile_map(&mq, a.q, a.T, a.Hk, a.dk, a.q_t, a.q_h, 64, CU_TENSOR_MAP_SWIZZLE_128B) ||
+                  rec_tile_map(&mk, a.k, a.T, a.Hk, a.dk, a.k_t, a.k_h, 64, CU_TENSOR_MAP_SWIZZLE_128B) ||
+                  rec_tile_map(&mv, a.v, a.T, a.Hv, a.dv, a.v_t, a.v_h, 64, CU_TENSOR_MAP_SWIZZLE_128B) ||
+                  rec_tile_map(&my, a.dy, a.T, a.Hv, a.dv, a.dy_t, a.dy_h, 64, CU_TENSOR_MAP_SWIZZLE_128B)))
+    return -2;
+  if (cudaFuncSetAttribute(rec_grad<DELTA>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<DELTA>()) != cudaSuccess) {
+    cudaGetLastError();
+    return -5;
+  }
+  rec_grad<DELTA><<<(unsigned)blocks, THREADS, smem_bytes<DELTA>(), st>>>(mq, mk, mv, my, a);
+  return cudaGetLastError() == cudaSuccess ? 0 : -11;
+}
+
+}  // namespace
+
+int xb_recurrence_grad(const XbRecArgs& a, int delta, cudaStream_t st) { return delta ? run<true>(a, st) : run<false>(a, st); }

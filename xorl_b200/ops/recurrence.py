@@ -24,7 +24,8 @@ from . import _lib
 _launches = 0
 
 CHUNK = 64              # tokens of a chunk of the kernels (csrc/recurrence.cu)
-SLICE = 32              # columns of the state that one CTA carries
+SLICE = 32              # columns of the state in one operand tile
+TILE = 16384            # bytes of an operand tile of the state
 MAX_STATE_ROWS = 128
 OPERANDS = 32768        # bytes of the operand tile that the delta rule prepares per chunk and head
 
@@ -42,8 +43,8 @@ class _Args(ctypes.Structure):
                 + [(n, ctypes.c_void_p) for n in ("A", "D", "cu", "s_in", "s_out", "ds_out", "ds_in")]
                 + [(n, ctypes.c_longlong) for n in ("s_k", "s_v")]
                 + [(n, ctypes.c_void_p) for n in ("o", "dq", "dk_out", "dv_out", "dg", "db", "dA", "dD", "chunks",
-                                                  "doc_off", "hd", "rqk", "qk", "kk", "pt", "s_planes", "ds_planes",
-                                                  "u_planes", "dr_planes", "part", "status")]
+                                                  "doc_off", "hd", "rqk", "qk", "kk", "pt", "s_tiles", "ds_tiles",
+                                                  "u_tiles", "dr_tiles", "part", "status")]
                 + [(n, ctypes.c_int) for n in ("T", "n_docs", "Hk", "Hv", "dk", "dv", "dkp", "dvp", "nc_max", "l2norm")]
                 + [("scale", ctypes.c_float)])
 
@@ -80,7 +81,7 @@ def _fill(a: _Args, q, k, v, g, b, A, D, cu, s_in, ws, keep: bool, delta: bool, 
         a.s_k, a.s_v = 1, dk
     a.cu, a.s_in = cu.data_ptr(), _lib.ptr(s_in)
     a.T, a.n_docs, a.Hk, a.Hv, a.dk, a.dv = T, cu.numel() - 1, Hk, Hv, dk, dv
-    a.dkp, a.dvp = 64 if dk <= 64 else 128, -(-dv // SLICE) * SLICE
+    a.dkp, a.dvp = 64 if dk <= 64 else 128, -(-dv // 64) * 64
     a.nc_max = T // CHUNK + cu.numel() + 1
     a.l2norm, a.scale = int(l2norm), scale
     nc = a.nc_max
@@ -149,11 +150,11 @@ class _Recurrence(torch.autograd.Function):
             dD = None if delta else torch.empty(Hv, dtype=torch.float32, device=dev)
             a.dq, a.dk_out, a.dv_out, a.db = dq.data_ptr(), dkk.data_ptr(), dvv.data_ptr(), db.data_ptr()
             a.dg, a.dA, a.dD = _lib.ptr(dg), _lib.ptr(dA), _lib.ptr(dD)
-            state = a.nc_max * Hv * 2 * a.dkp * a.dvp * 2
-            plane = a.nc_max * Hv * 2 * CHUNK * a.dvp * 2
-            offs, total = _pieces([state, state] + ([plane, plane] if delta else [a.nc_max * Hv * 2 * 4]))
+            tiles = a.nc_max * Hv * (a.dvp // SLICE)
+            offs, total = _pieces([tiles * TILE, tiles * TILE]
+                                  + ([tiles * TILE // 2, tiles * TILE // 2] if delta else [a.nc_max * Hv * 2 * 4]))
             tmp = torch.empty(total, dtype=torch.uint8, device=dev)
-            for name, off in zip(("s_planes", "ds_planes") + (("u_planes", "dr_planes") if delta else ("part",)), offs):
+            for name, off in zip(("s_tiles", "ds_tiles") + (("u_tiles", "dr_tiles") if delta else ("part",)), offs):
                 setattr(a, name, tmp.data_ptr() + off)
             _lib.check(_lib.cuda_lib().xb_recurrence_bwd(ctypes.byref(a), int(delta), _lib.stream_ptr()),
                        "xb_recurrence_bwd")
