@@ -9,12 +9,13 @@
 // registers, their dot products with q and k give the gradient of the decay and of b, and D o dP, D o dL are added up;
 // the products with K and Q are the same for all heads of the group and are made once, from the sums.
 // The tiles that it reads (60 KB per head and 32 columns; scan 40 KB) bound it: they are what the two sequential passes
-// keep.  Sixteen worker warps, a loading and an issuing warp; 64-row accumulators lie in 16 lanes of each warp.
+// keep.  Eight worker warps, a loading and an issuing warp, and one that turns the heads' sums into gradients of the
+// decay; 64-row accumulators lie in 16 lanes of each warp.
 #include "recurrence_core.cuh"
 
 namespace {
 
-constexpr int WORKERS = 512, THREADS = WORKERS + 64;
+constexpr int WORKERS = 256, THREADS = WORKERS + 96;
 constexpr int T64 = HALF / 2;                       // 8 KB: [64 rows][128 bytes]
 template <bool DELTA>
 struct Lay {
@@ -25,13 +26,14 @@ struct Lay {
   static constexpr int SM_Q = 0, SM_K = 2 * T64, SM_RING = 4 * T64, SM_DOV = SM_RING + RING * STAGE, SM_RED = SM_DOV + 2 * DOV;
 };
 struct Red {                                        // what meets across warps, one set per head in turn
-  float rd[3][4][C];                                // q.t1, k.t2, k.t3 by column quarter
-  float er[4][C], fr[4][C];                         // row sums of dP o P and dL o A by column quarter (scan: dP o P)
+  float rd[3][2][C];                                // q.t1, k.t2, k.t3 by column half
+  float er[2][C], fr[2][C];                         // row sums of dP o P and dL o A by column half (scan: dP o P)
   float ec[4][C], fc[4][C];                         // column sums by row block
-  float rv[C], sdot[16];
+  float rv[C], sdot[8];
+  float hd[HD];
 };
 struct __align__(8) Bars {
-  uint64_t full[3], empty[3], dov_full[2], dov_empty[2], qk_full, acc_full, acc_empty, last;
+  uint64_t full[3], empty[3], dov_full[2], dov_empty[2], red_full[2], red_empty[2], qk_full, acc_full, acc_empty, last;
   uint32_t tmem;
   int abort_flag;
 };
@@ -62,15 +64,13 @@ __device__ __forceinline__ void product(uint32_t d, uint32_t a, uint32_t b, uint
 __device__ __forceinline__ float col_sum(float (&v)[8]) {
   const int l = threadIdx.x & 15;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], 8);
-#pragma unroll
   for (int o = 4; o > 0; o >>= 1)
 #pragma unroll
     for (int i = 0; i < o; ++i) {
       const float mine = l & o ? v[i + o] : v[i], other = l & o ? v[i] : v[i + o];
       v[i] = mine + __shfl_xor_sync(0xffffffffu, other, o);
     }
-  return v[0];
+  return v[0] + __shfl_xor_sync(0xffffffffu, v[0], 8);
 }
 // A 64-row accumulator lies in lanes 0 .. 15 of each warp; lanes 16 .. 31 take the second half of its 2 N columns.
 template <int N>
@@ -93,25 +93,27 @@ __device__ __forceinline__ void floats8(const uint4 u, float (&x)[8]) {
     x[2 * j] = f.x, x[2 * j + 1] = f.y;
   }
 }
-// acc += f * t over this thread's 16 columns (from unit `unit`) of its row; returns t . (the same columns of `tile`)
-__device__ __forceinline__ float add_rows(uint32_t addr, const uint8_t* tile, int row, int unit, float f, float (&acc)[16]) {
-  uint32_t t[32];
-  float y[16];
-  tmem_ld_32x32(addr, t);
-  tc_wait_ld();
-  spread<16>(t, y);
-  float dot = 0.f;
+// acc += f * t over this thread's columns of its row: 8 of every 16, four times, units `unit` + 2 i; returns t . (the same
+// columns of `tile`).  The next 16 columns are on their way while 8 are worked on.
+__device__ __forceinline__ float add_rows(uint32_t addr, const uint8_t* tile, int row, int unit, float f, float (&acc)[32]) {
+  uint32_t t[2][16];
+  float dot[2] = {0.f, 0.f};
+  tmem_ld_32x16(addr, t[0]);
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    float x[8];
-    floats8(tile_unit(tile, row, unit + u), x);
+  for (int i = 0; i < 4; ++i) {
+    float x[8], y[8];
+    floats8(tile_unit(tile, row, unit + 2 * i), x);
+    tc_wait_ld();
+    if (i < 3) tmem_ld_32x16(addr + 16 * (i + 1), t[(i + 1) & 1]);
+    spread<8>(t[i & 1], y);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      dot += x[e] * y[8 * u + e];
-      acc[8 * u + e] += f * y[8 * u + e];
+      dot[e & 1] += x[e] * y[e];
+      acc[8 * i + e] += f * y[e];
     }
   }
-  return dot + __shfl_xor_sync(0xffffffffu, dot, 16);
+  const float d = dot[0] + dot[1];
+  return d + __shfl_xor_sync(0xffffffffu, d, 16);
 }
 
 template <bool DELTA>
@@ -147,6 +149,7 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
   if (tid == 0) {
     for (int i = 0; i < 3; ++i) mbar_init(&bars->full[i], 1), mbar_init(&bars->empty[i], 1 + WORKERS / 32);
     for (int i = 0; i < 2; ++i) mbar_init(&bars->dov_full[i], 1), mbar_init(&bars->dov_empty[i], 1 + WORKERS / 32);
+    for (int i = 0; i < 2; ++i) mbar_init(&bars->red_full[i], WORKERS / 32), mbar_init(&bars->red_empty[i], 1);
     mbar_init(&bars->qk_full, 1), mbar_init(&bars->acc_full, 1), mbar_init(&bars->acc_empty, WORKERS / 32), mbar_init(&bars->last, 1);
     bars->abort_flag = 0;
     mbar_fence_init();
@@ -255,13 +258,86 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
       tc_commit(&bars->last);
     }
     __syncwarp();
+  } else if (warp == WORKERS / 32 + 2) {
+    // ------------------------------------------------ the heads' sums ---------------------------------------
+    wait(&bars->qk_full, 0, 50);
+    __syncwarp();
+    for (int hh = 0; hh < rep; ++hh) {
+      const int h = kh * rep + hh;
+      const long long ch_h = (long long)c * p.Hv + h;
+      const Red& r = red[hh & 1];
+      const float* hd = r.hd;
+      wait(&bars->red_full[hh & 1], (hh >> 1) & 1, 51);
+      __syncwarp();
+      // gradients of the log decay (suffix sums of dG) and of b: two rows per lane
+      double x[2], tail = 0.0, dsum = 0.0;
+      float db[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int t = 2 * lane + i;
+        const float bt = hd[2 * C + t], ga = ex2_sum(hd, t), de = ex2_diff(hd, C - 1, t);
+        const bool on = t < len;
+        auto four = [&](const float (&a)[4][C]) { return (a[0][t] + a[1][t]) + (a[2][t] + a[3][t]); };
+        auto two = [&](const float (&a)[2][C]) { return a[0][t] + a[1][t]; };
+        const float q1 = on ? ga * rqk[t] * two(r.rd[0]) : 0.f, k2 = on && DELTA ? ga * rqk[C + t] * two(r.rd[1]) : 0.f;
+        const float k3 = on ? de * rqk[C + t] * two(r.rd[2]) : 0.f;
+        const float e1 = two(r.er), e2 = four(r.ec), g1 = DELTA ? two(r.fr) : 0.f, g2 = DELTA ? four(r.fc) : 0.f;
+        if (DELTA) {
+          x[i] = (double)q1 + (double)e1 - (double)e2 + (double)(bt * g1) - (double)g2 - (double)(bt * k2) - (double)k3;
+          tail += k3;
+          db[i] = r.rv[t] - k2 + g1;
+        } else {
+          x[i] = (double)q1 + (double)e1 - (double)(bt * e2) - (double)(bt * k3);
+          tail += (double)(bt * k3);
+          db[i] = e2 + k3;
+          dsum += r.rv[t];
+        }
+      }
+      float sd = lane < 8 ? r.sdot[lane] : 0.f;
+      sd = warp_sum(sd);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        tail += __shfl_xor_sync(0xffffffffu, tail, o);
+        dsum += __shfl_xor_sync(0xffffffffu, dsum, o);
+      }
+      tail += (double)(ex2_sum(hd, C - 1) * sd);
+      double s = x[0] + x[1];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double y = __shfl_down_sync(0xffffffffu, s, o);
+        if (lane + o < 32) s += y;
+      }
+      double da = 0.0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int t = 2 * lane + i;
+        const float dg = (float)((i ? s - x[0] : s) + tail);
+        if (t < len) {
+          const long long at = (long long)(ch.x + t) * p.Hv + h;
+          if (DELTA) {
+            p.dg[at] = dg, p.db[at] = db[i];
+          } else {
+            p.db[at] = db[i] + dg * p.A[h];
+            da += (double)(dg * hd[2 * C + t]);
+          }
+        }
+      }
+      if (!DELTA) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) da += __shfl_xor_sync(0xffffffffu, da, o);
+        if (lane == 0) p.part[ch_h * 2] = (float)da, p.part[ch_h * 2 + 1] = (float)dsum;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->red_empty[hh & 1]);
+    }
   } else {
     // ------------------------------------------------ workers -----------------------------------------------
-    // row `row`; 16 of 128 columns (from unit cu) of the wide products, 8 of 64 (from j0) of the square ones
-    const int q4 = warp & 3, qd = warp >> 2, row = q4 * 16 + (lane & 15), cu = qd * 4 + (lane >> 4) * 2, j0 = qd * 16 + (lane >> 4) * 8;
+    // row `row`; of its warp's half of the columns the lower or upper 8 of every 16: units cu, cu + 2, .. of the wide
+    // products, columns j0 .., j0 + 16 .. of the square ones
+    const int q4 = warp & 3, hf = warp >> 2, row = q4 * 16 + (lane & 15), cu = hf * 8 + (lane >> 4), j0 = hf * 32 + (lane >> 4) * 8;
     const bool act = lane < 16;
     const uint32_t base = tmem + ((uint32_t)(q4 * 32) << 16);
-    float aq[16] = {}, ak[16] = {}, az[8] = {}, aw[8] = {};
+    float aq[32] = {}, ak[32] = {}, az[16] = {}, aw[DELTA ? 16 : 1] = {};
     auto wwait = [&](uint64_t* b, uint32_t parity, int detail) {
       wait(b, parity, detail);
       __syncwarp();
@@ -276,8 +352,6 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
     const float* kk = DELTA ? p.kk + ((long long)c * p.Hk + kh) * (C * C) + row * C + j0 : nullptr;
     int n = 0, m = 0;
     for (int hh = 0; hh < rep; ++hh) {
-      const int h = kh * rep + hh;
-      const long long ch_h = (long long)c * p.Hv + h;
       Red& r = red[hh & 1];
       float sdot = 0.f, rv = 0.f;
       const float* hd = nullptr;
@@ -289,8 +363,9 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
           const int s = n % L::RING;
           const uint8_t* st = smem + L::SM_RING + s * L::STAGE;
           wwait(&bars->full[s], (n / L::RING) & 1, 42);
-          {  // <S, dS'>: a unit of eight columns of a row per thread
-            const int sr = tid >> 2, u = tid & 3;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {  // <S, dS'>: two units of eight columns of a row per thread
+            const int sr = i * 64 + (tid >> 2), u = tid & 3;
             const uint32_t hi = (uint32_t)(sr * 128 + ((u ^ (sr & 7)) << 4)), lo = (uint32_t)(sr * 128 + (((u + 4) ^ (sr & 7)) << 4));
             float a[8], al[8], b[8], bl[8];
             floats8(*reinterpret_cast<const uint4*>(st + L::ST_S + hi), a), floats8(*reinterpret_cast<const uint4*>(st + L::ST_S + lo), al);
@@ -298,7 +373,7 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
 #pragma unroll
             for (int e = 0; e < 8; ++e) sdot += (a[e] + al[e]) * (b[e] + bl[e]);
           }
-          if (tid < 4 * C) {  // dR.v (scan: dO.v)
+          {  // dR.v (scan: dO.v)
             const int sr = tid >> 2, u = tid & 3;
             float v[8], a[8], al[8];
             floats8(tile_unit(dov + 2 * T64, sr, (sl & 3) * 4 + u), v);
@@ -316,118 +391,75 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
         }
         if (pass + 1 < passes) arrive(&bars->dov_empty[m & 1]);     // the last one is given back below: its decays are read
       }
+      wwait(&bars->red_empty[hh & 1], ((hh >> 1) & 1) ^ 1, 45);
+      if (tid < HD) r.hd[tid] = hd[tid];
       sdot = warp_sum(sdot);
       if (lane == 0) r.sdot[warp] = sdot;
       rv += __shfl_xor_sync(0xffffffffu, rv, 1);
       rv += __shfl_xor_sync(0xffffffffu, rv, 2);
-      if (tid < 4 * C && (tid & 3) == 0) r.rv[tid >> 2] = rv;
+      if ((tid & 3) == 0) r.rv[tid >> 2] = rv;
       const float b = hd[2 * C + row], gam = ex2_sum(hd, row), dec = ex2_diff(hd, C - 1, row);
       wwait(&bars->acc_full, hh & 1, 43);
       tc_fence_after();
       {
-        const bool on = row < len;                                    // rows behind the end hold other documents' products
-        const float f1 = on ? gam * rq : 0.f, f2 = on ? -b * gam * rk : 0.f, f3 = on ? dec * rk * (DELTA ? 1.f : b) : 0.f;
-        const float d1 = add_rows(base + COL_T1 + qd * 32, smem + L::SM_Q, row, cu, f1, aq);
-        const float d2 = DELTA ? add_rows(base + COL_T2 + qd * 32, smem + L::SM_K, row, cu, f2, ak) : 0.f;
-        const float d3 = add_rows(base + COL_T3 + qd * 32, smem + L::SM_K, row, cu, f3, ak);
-        if (act) r.rd[0][qd][row] = d1, r.rd[1][qd][row] = d2, r.rd[2][qd][row] = d3;
-      }
-      {
-        uint32_t t[16];
-        float pr[8], lr[8] = {}, ec[8], fc[8], er = 0.f, fr = 0.f;
-        tmem_ld_32x16(base + COL_P + qd * 16, t);
-        tc_wait_ld();
-        spread<8>(t, pr);
-        if (DELTA) {
-          tmem_ld_32x16(base + COL_L + qd * 16, t);
-          tc_wait_ld();
-          spread<8>(t, lr);
-        }
+        float er = 0.f, fr = 0.f;
+        const float gi = hd[row], gl = hd[C + row];
+        const int last = row < len ? row : -1;                        // the row's last column; none behind the end
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int j = j0 + e;
-          ec[e] = fc[e] = 0.f;
-          if (j <= row && row < len) {
-            const float d = ex2_diff(hd, row, j), bj = DELTA ? 1.f : hd[2 * C + j], g = d * pr[e];
-            const float v = g * qk[e];
-            er += bj * v;
-            ec[e] = v;
-            az[e] += g * rq * rqk[C + j] * bj;
-            if (DELTA && j < row) {
-              const float l = -d * lr[e], w = l * kk[e];
+        for (int i = 0; i < 2; ++i) {
+          const int j = j0 + 16 * i;
+          float hi[8], lo[8], kj[8], bj[8], qr[8], kr[8], x[8], v[8];
+          uint32_t t[16], tl[16];
+          auto eight = [&](const float* src, float (&dst)[8]) {
+            const float4 a = reinterpret_cast<const float4*>(src)[0], c4 = reinterpret_cast<const float4*>(src)[1];
+            dst[0] = a.x, dst[1] = a.y, dst[2] = a.z, dst[3] = a.w, dst[4] = c4.x, dst[5] = c4.y, dst[6] = c4.z, dst[7] = c4.w;
+          };
+          tmem_ld_32x16(base + COL_P + hf * 32 + 16 * i, t);
+          if (DELTA) tmem_ld_32x16(base + COL_L + hf * 32 + 16 * i, tl);
+          eight(qk + 16 * i, qr);
+          if (DELTA) eight(kk + 16 * i, kr);
+          eight(hd + j, hi), eight(hd + C + j, lo), eight(rqk + C + j, kj);
+          if (!DELTA) eight(hd + 2 * C + j, bj);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) hi[e] = xb_ex2((gi - hi[e]) + (gl - lo[e]));
+          tc_wait_ld();
+          spread<8>(t, x);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float y = j + e <= last ? hi[e] * x[e] : 0.f, w = j + e <= last ? y * qr[e] : 0.f;
+            er += DELTA ? w : bj[e] * w;
+            v[e] = w;
+            az[8 * i + e] += y * (rq * kj[e]) * (DELTA ? 1.f : bj[e]);
+          }
+          const float es = col_sum(v);
+          if ((lane & 8) == 0) r.ec[q4][j + (lane & 7)] = es;
+          if (DELTA) {
+            spread<8>(tl, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float y = j + e < last ? -hi[e] * x[e] : 0.f, w = j + e < last ? y * kr[e] : 0.f;
               fr += w;
-              fc[e] = b * w;
-              aw[e] += b * l * rk * rqk[C + j];
+              v[e] = b * w;
+              aw[DELTA ? 8 * i + e : 0] += b * y * (rk * kj[e]);
             }
+            const float fs = col_sum(v);
+            if ((lane & 8) == 0) r.fc[q4][j + (lane & 7)] = fs;
           }
         }
         er += __shfl_xor_sync(0xffffffffu, er, 16), fr += __shfl_xor_sync(0xffffffffu, fr, 16);
-        if (act) r.er[qd][row] = er, r.fr[qd][row] = fr;
-        const float es = col_sum(ec), fs = DELTA ? col_sum(fc) : 0.f;
-        if ((lane & 8) == 0) r.ec[q4][j0 + (lane & 7)] = es, r.fc[q4][j0 + (lane & 7)] = fs;
+        if (act) r.er[hf][row] = er, r.fr[hf][row] = fr;
+      }
+      {
+        const bool on = row < len;                                    // rows behind the end hold other documents' products
+        const float f1 = on ? gam * rq : 0.f, f2 = on ? -b * gam * rk : 0.f, f3 = on ? dec * rk * (DELTA ? 1.f : b) : 0.f;
+        const float d1 = add_rows(base + COL_T1 + hf * 64, smem + L::SM_Q, row, cu, f1, aq);
+        const float d2 = DELTA ? add_rows(base + COL_T2 + hf * 64, smem + L::SM_K, row, cu, f2, ak) : 0.f;
+        const float d3 = add_rows(base + COL_T3 + hf * 64, smem + L::SM_K, row, cu, f3, ak);
+        if (act) r.rd[0][hf][row] = d1, r.rd[1][hf][row] = d2, r.rd[2][hf][row] = d3;
       }
       tc_fence_before();
       if (hh + 1 < rep) arrive(&bars->acc_empty);
-      wbar();
-      if (warp == 0) {
-        // gradients of the log decay (suffix sums of dG) and of b: two rows per lane
-        double x[2], tail = 0.0, dsum = 0.0;
-        float db[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int t = 2 * lane + i;
-          const float bt = hd[2 * C + t], ga = ex2_sum(hd, t), de = ex2_diff(hd, C - 1, t);
-          const bool on = t < len;
-          auto four = [&](const float (&a)[4][C]) { return (a[0][t] + a[1][t]) + (a[2][t] + a[3][t]); };
-          const float q1 = on ? ga * rqk[t] * four(r.rd[0]) : 0.f, k2 = on && DELTA ? ga * rqk[C + t] * four(r.rd[1]) : 0.f;
-          const float k3 = on ? de * rqk[C + t] * four(r.rd[2]) : 0.f;
-          const float e1 = four(r.er), e2 = four(r.ec), g1 = four(r.fr), g2 = four(r.fc);
-          if (DELTA) {
-            x[i] = (double)q1 + (double)e1 - (double)e2 + (double)(bt * g1) - (double)g2 - (double)(bt * k2) - (double)k3;
-            tail += k3;
-            db[i] = r.rv[t] - k2 + g1;
-          } else {
-            x[i] = (double)q1 + (double)e1 - (double)(bt * e2) - (double)(bt * k3);
-            tail += (double)(bt * k3);
-            db[i] = e2 + k3;
-            dsum += r.rv[t];
-          }
-        }
-        float sd = lane < 16 ? r.sdot[lane] : 0.f;
-        sd = warp_sum(sd);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-          tail += __shfl_xor_sync(0xffffffffu, tail, o);
-          dsum += __shfl_xor_sync(0xffffffffu, dsum, o);
-        }
-        tail += (double)(ex2_sum(hd, C - 1) * sd);
-        double s = x[0] + x[1];
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const double y = __shfl_down_sync(0xffffffffu, s, o);
-          if (lane + o < 32) s += y;
-        }
-        double da = 0.0;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int t = 2 * lane + i;
-          const float dg = (float)((i ? s - x[0] : s) + tail);
-          if (t < len) {
-            const long long at = (long long)(ch.x + t) * p.Hv + h;
-            if (DELTA) {
-              p.dg[at] = dg, p.db[at] = db[i];
-            } else {
-              p.db[at] = db[i] + dg * p.A[h];
-              da += (double)(dg * hd[2 * C + t]);
-            }
-          }
-        }
-        if (!DELTA) {
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) da += __shfl_xor_sync(0xffffffffu, da, o);
-          if (lane == 0) p.part[ch_h * 2] = (float)da, p.part[ch_h * 2 + 1] = (float)dsum;
-        }
-      }
+      arrive(&bars->red_full[hh & 1]);
       arrive(&bars->dov_empty[(m - 1) & 1]);
     }
     // Z and W as operand tiles over the ring, whose last tiles have been read; K and Q without rows behind the end
@@ -435,13 +467,18 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
       uint8_t* t = smem + L::SM_RING + row * 128;
 #pragma unroll
       for (int part = 0; part < (DELTA ? 2 : 1); ++part) {
-        uint32_t hi[4], lo[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          split2(part ? aw[2 * e] : az[2 * e], part ? aw[2 * e + 1] : az[2 * e + 1], hi[e], lo[e]);
-        const int off = part * 2 * T64 + (((j0 >> 3) ^ (row & 7)) << 4);
-        *reinterpret_cast<uint4*>(t + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<uint4*>(t + off + T64) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        for (int u = 0; u < 2; ++u) {
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int i = 8 * u + 2 * e;
+            split2(part ? aw[DELTA ? i : 0] : az[i], part ? aw[DELTA ? i + 1 : 0] : az[i + 1], hi[e], lo[e]);
+          }
+          const int off = part * 2 * T64 + ((((j0 >> 3) + 2 * u) ^ (row & 7)) << 4);
+          *reinterpret_cast<uint4*>(t + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          *reinterpret_cast<uint4*>(t + off + T64) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
       }
     }
     for (int i = tid; i < 4 * (C - len) * 8; i += WORKERS) {
@@ -453,36 +490,39 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
     arrive(&bars->acc_empty);
     wwait(&bars->last, 0, 44);
     tc_fence_after();
-    add_rows(base + COL_T1 + qd * 32, smem + L::SM_Q, row, cu, 1.f, aq);
-    add_rows(base + COL_T2 + qd * 32, smem + L::SM_K, row, cu, 1.f, ak);
+    add_rows(base + COL_T1 + hf * 64, smem + L::SM_Q, row, cu, 1.f, aq);
+    add_rows(base + COL_T2 + hf * 64, smem + L::SM_K, row, cu, 1.f, ak);
     // gradient through the L2 norms: dq - q^ (q^ . dq), rows of norm below 1e-12 excepted
     float fq = 0.f, fk = 0.f;
     if (p.l2norm) {
       float sq = 0.f, sk = 0.f;
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+      for (int i = 0; i < 4; ++i) {
+        const int unit = cu + 2 * i;
         float x[8], y[8];
-        floats8(tile_unit(smem + L::SM_Q, row, cu + u), x), floats8(tile_unit(smem + L::SM_K, row, cu + u), y);
+        floats8(tile_unit(smem + L::SM_Q, row, unit), x), floats8(tile_unit(smem + L::SM_K, row, unit), y);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sq += x[e] * aq[8 * u + e], sk += y[e] * ak[8 * u + e];
+        for (int e = 0; e < 8; ++e) sq += x[e] * aq[8 * i + e], sk += y[e] * ak[8 * i + e];
       }
       sq += __shfl_xor_sync(0xffffffffu, sq, 16), sk += __shfl_xor_sync(0xffffffffu, sk, 16);
       Red& r = red[rep & 1];
-      if (act) r.rd[0][qd][row] = sq, r.rd[1][qd][row] = sk;
+      wwait(&bars->red_empty[rep & 1], ((rep >> 1) & 1) ^ 1, 46);
+      if (act) r.rd[0][hf][row] = sq, r.rd[1][hf][row] = sk;
       wbar();
       const float nq = rq / p.scale;
-      if (nq < 0.99e12f) fq = nq * nq * ((r.rd[0][0][row] + r.rd[0][1][row]) + (r.rd[0][2][row] + r.rd[0][3][row]));
-      if (rk < 0.99e12f) fk = rk * rk * ((r.rd[1][0][row] + r.rd[1][1][row]) + (r.rd[1][2][row] + r.rd[1][3][row]));
+      if (nq < 0.99e12f) fq = nq * nq * (r.rd[0][0][row] + r.rd[0][1][row]);
+      if (rk < 0.99e12f) fk = rk * rk * (r.rd[1][0][row] + r.rd[1][1][row]);
     }
     if (row < len)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int col = (cu + u) * 8;
+      for (int i = 0; i < 4; ++i) {
+        const int unit = cu + 2 * i, col = unit * 8;
         if (col < p.dk) {
           float x[8], y[8];
-          floats8(tile_unit(smem + L::SM_Q, row, cu + u), x), floats8(tile_unit(smem + L::SM_K, row, cu + u), y);
+          floats8(tile_unit(smem + L::SM_Q, row, unit), x), floats8(tile_unit(smem + L::SM_K, row, unit), y);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = aq[8 * u + e] - fq * x[e], y[e] = ak[8 * u + e] - fk * y[e];
+          for (int e = 0; e < 8; ++e)
+            x[e] = aq[8 * i + e] - fq * x[e], y[e] = ak[8 * i + e] - fk * y[e];
           *reinterpret_cast<uint4*>(dq + row * d_t + col) =
               make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
           *reinterpret_cast<uint4*>(dk + row * d_t + col) =
