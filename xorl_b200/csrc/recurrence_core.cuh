@@ -183,5 +183,8 @@ int rec_launch(K kernel, long long blocks, int threads, size_t smem, const XbRec
 // recurrence_delta.cu: prepare and forward; forward again with the states kept, and the state's gradient
 int xb_delta_fwd(const XbRecArgs& a, cudaStream_t st);
 int xb_delta_bwd(const XbRecArgs& a, cudaStream_t st);
+// recurrence_scan.cu: the same for the scan
+int xb_scan_fwd(const XbRecArgs& a, cudaStream_t st);
+int xb_scan_bwd(const XbRecArgs& a, cudaStream_t st);
 // recurrence_grad.cu: gradients of q, k, the decay and b from the kept tiles
 int xb_recurrence_grad(const XbRecArgs& a, int delta, cudaStream_t st);

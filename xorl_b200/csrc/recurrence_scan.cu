@@ -1,0 +1,423 @@
+// The state-space scan's own kernels: prepare, and one kernel for the sequential part of both directions (the formulas
+// stand in recurrence.cu).  With P_ij = D_ij (Q K^T)_ij b_j for j <= i:
+//
+//   forward   O = gamma Q S + P V + D V,             S' = gamma_last S + K^T (d b V)
+//   backward  dV = d b K dS' + P^T dO + D dO,        dS = gamma_last dS' + Q^T (gamma dO)
+//
+// The two are one computation with Q and K, and the row factors gamma and d b, exchanged, P transposed and the chunks
+// walked the other way.  The state does not feed back into what is added to it, so the products of a step need not wait
+// for one another: a CTA carries 64 state columns of one head through one document, four warps make the operands that
+// depend on the chunk alone (P, and d b V or gamma dO) ahead of the products, eight add up the state and write the
+// outputs, one loads and one issues.  Computed operands are [hi 32 | lo 32] tiles (P: two planes).  Per step and CTA 20
+// products, about 1100 cycles of the tensor pipe, which bounds it next to the split and decay arithmetic.
+#include "recurrence_core.cuh"
+
+namespace {
+
+// ---- prepare: Q K^T of a chunk and group, running decays of the group's heads -----------------------------------------
+template <int DKP>
+__global__ void __launch_bounds__(128) scan_prep(const XbRecArgs p) {
+  __shared__ __align__(128) uint8_t q[C * DKP * 2];
+  __shared__ __align__(128) uint8_t k[C * DKP * 2];
+  constexpr int U = DKP / 8;
+  const int kh = blockIdx.x % p.Hk, c = blockIdx.x / p.Hk;
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3;
+  if (c >= p.doc_off[p.n_docs + 2]) return;
+  const int4 ch = reinterpret_cast<const int4*>(p.chunks)[c];
+  const int len = ch.y, rep = p.Hv / p.Hk;
+  const uint32_t sq = xb_smem_u32(q), sk = xb_smem_u32(k);
+  load_tile<U, C, 128>(sq, (const bf16*)p.q + ch.x * p.q_t + kh * p.q_h, p.q_t, len, p.dk);
+  load_tile<U, C, 128>(sk, (const bf16*)p.k + ch.x * p.k_t + kh * p.k_h, p.k_t, len, p.dk);
+  cp_commit();
+  p.rqk[((long long)c * p.Hk + kh) * RQK + tid] = (tid & 63) < len ? 1.f : 0.f;
+  for (int hh = w; hh < rep; hh += 4) {
+    const int h = kh * rep + hh;
+    double x[2];
+    float bb[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = 2 * lane + i;
+      x[i] = 0.0, bb[i] = 0.f;
+      if (row < len) {
+        bb[i] = p.b[(ch.x + row) * p.b_t + h * p.b_h];
+        const double z = (double)bb[i] * (double)p.A[h];
+        x[i] = (z < (double)MIN_LOG ? (double)MIN_LOG : z) * 1.4426950408889634;
+      }
+    }
+    double s = x[0] + x[1];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double u = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += u;
+    }
+    float* out = p.hd + ((long long)c * p.Hv + h) * HD;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = 2 * lane + i;
+      const double G = i ? s : s - x[1];
+      const float hi = (float)G;
+      out[row] = hi, out[C + row] = (float)(G - (double)hi), out[2 * C + row] = bb[i];
+    }
+  }
+  cp_wait<0>();
+  __syncthreads();
+  float* qk = p.qk + ((long long)c * p.Hk + kh) * (C * C);
+#pragma unroll
+  for (int nt = 0; nt < 8; nt += 2) {
+    if (nt * 8 > w * 16 + 15) break;              // columns above the diagonal block are never used
+    float a[2][4] = {};
+#pragma unroll
+    for (int ks = 0; ks < DKP / 16; ++ks) {
+      uint32_t fq[4], fb[4];
+      ldsm4(fb, sk + addr_b<U>(nt * 8, ks * 16));
+      ldsm4(fq, sq + addr_a<U>(w * 16, ks * 16));
+      mma(a[0], fq, fb[0], fb[1]);
+      mma(a[1], fq, fb[2], fb[3]);
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh)
+        *reinterpret_cast<float2*>(qk + (w * 16 + g + hh * 8) * C + (nt + j) * 8 + 2 * t) = make_float2(a[j][2 * hh], a[j][2 * hh + 1]);
+  }
+}
+
+// ---- the sequential part -------------------------------------------------------------------------------------------
+constexpr int T64 = HALF / 2;
+constexpr int MAKERS = 128, ADDERS = 256, THREADS = MAKERS + ADDERS + 64;
+// K and Q: [64 rows][128 bytes] twice each; v or dO: [64][64 columns]; Q K^T: [64][32 fp32] twice; decays and b
+constexpr int ST_K = 0, ST_Q = 2 * T64, ST_X = 4 * T64, ST_QK = 5 * T64, ST_HD = 7 * T64, STAGE = 7 * T64 + 1024;
+constexpr int SM_S = 2 * STAGE, SM_P = SM_S + 2 * HALF, SM_D = SM_P + 2 * HALF, SM_BAR = SM_D + 2 * HALF;
+constexpr int SMEM = SM_BAR + 256 + 1024;
+constexpr int D1 = 0, D2 = 128, DSTEP = 192, D3 = 384;      // D1, D2 of even and odd steps; D3
+
+struct __align__(8) Bars {
+  uint64_t full[2], empty[2], pd_full[2], pd_empty[2], s_full, s_empty, out_full[2], out_empty[2], d3_full, d3_empty;
+  uint32_t tmem;
+  int abort_flag;
+};
+static_assert(sizeof(Bars) <= 256, "barriers");
+
+// BWD: the direction.  OUT: outputs are wanted.  KEEP: the state tiles of every chunk go to global memory.
+template <bool BWD, bool OUT, bool KEEP>
+__global__ void __launch_bounds__(THREADS, 1)
+scan_seq(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mx,
+         const __grid_constant__ CUtensorMap mqk, const __grid_constant__ XbRecArgs p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  Bars* bars = reinterpret_cast<Bars*>(smem + SM_BAR);
+  const int blocks = p.dvp / 64, rep = p.Hv / p.Hk;
+  const int cb = blockIdx.x % blocks, h = (blockIdx.x / blocks) % p.Hv, doc = blockIdx.x / (blocks * p.Hv);
+  const int kh = h / rep, v0 = cb * 64, c0 = p.doc_off[doc], steps = p.doc_off[doc + 1] - c0;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int4* chunks = reinterpret_cast<const int4*>(p.chunks);
+  auto chunk_of = [&](int n) { return BWD ? c0 + steps - 1 - n : c0 + n; };
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars->full[i], 1), mbar_init(&bars->empty[i], 1 + (MAKERS + ADDERS) / 32);
+      mbar_init(&bars->pd_full[i], MAKERS / 32), mbar_init(&bars->pd_empty[i], 1);
+      mbar_init(&bars->out_full[i], 1), mbar_init(&bars->out_empty[i], ADDERS / 32);
+    }
+    mbar_init(&bars->s_full, ADDERS / 32), mbar_init(&bars->s_empty, (OUT ? 1 : 0) + (KEEP ? 1 : 0));
+    mbar_init(&bars->d3_full, 1), mbar_init(&bars->d3_empty, ADDERS / 32);
+    bars->abort_flag = 0;
+    mbar_fence_init();
+  }
+  constexpr int LOADER = (MAKERS + ADDERS) / 32, ISSUER = LOADER + 1;
+  if (warp == LOADER) {
+    tmem_alloc(&bars->tmem, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem;
+  // a wait that runs out raises a flag; from then on waits return at once and every role walks to its end
+  auto wait = [&](uint64_t* b, uint32_t parity, int detail) { mbar_wait(b, parity, &bars->abort_flag, p.status, XB_K_RECURRENCE, detail); };
+  auto wwait = [&](uint64_t* b, uint32_t parity, int detail) {
+    wait(b, parity, detail);
+    __syncwarp();
+  };
+  auto arrive = [&](uint64_t* b) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(b);
+  };
+
+  if (warp == LOADER) {
+    if (xb_elect_one()) {
+      for (int n = 0; n < steps; ++n) {
+        const int s = n & 1, c = chunk_of(n), t0 = chunks[c].x;
+        uint8_t* st = smem + s * STAGE;
+        uint64_t* full = &bars->full[s];
+        wait(&bars->empty[s], ((n >> 1) & 1) ^ 1, 1);
+        mbar_expect_tx(full, T64 * (OUT ? 7 : 3) + HD * 4);
+        for (int i = 0; i < 2; ++i) {
+          if (OUT || !BWD) tma_load_3d(st + ST_K + i * T64, &mk, full, i * 64, kh, t0);
+          if (OUT || BWD) tma_load_3d(st + ST_Q + i * T64, &mq, full, i * 64, kh, t0);
+          if (OUT) tma_load_2d(st + ST_QK + i * T64, &mqk, full, i * 32, (c * p.Hk + kh) * C);
+        }
+        tma_load_3d(st + ST_X, &mx, full, v0, h, t0);
+        bulk_load(st + ST_HD, p.hd + ((long long)c * p.Hv + h) * HD, HD * 4, full);
+      }
+    }
+    __syncwarp();
+  } else if (warp == ISSUER) {
+    if (xb_elect_one()) {
+      constexpr uint64_t kmaj = xb_smem_desc_base_sw128(16, 1024), mn64 = xb_smem_desc_base_sw128(T64, 1024),
+                         mn128 = xb_smem_desc_base_sw128(HALF, 1024);
+      constexpr uint32_t id1 = xb_idesc(1, 1, 64, 128, 0, 1), id2 = xb_idesc(1, 1, 64, 64, BWD ? 1 : 0, 1), id3 = xb_idesc(1, 1, 128, 128, 1, 1);
+      const uint32_t bs = xb_smem_u32(smem + SM_S);
+      for (int n = 0; n < steps; ++n) {
+        const int s = n & 1;
+        const uint32_t ph = (n >> 1) & 1, st = xb_smem_u32(smem + s * STAGE);
+        const uint32_t pt = xb_smem_u32(smem + SM_P + s * HALF), dt = xb_smem_u32(smem + SM_D + s * HALF);
+        const uint32_t row = st + (BWD ? ST_K : ST_Q), col = st + (BWD ? ST_Q : ST_K);
+        wait(&bars->full[s], ph, 10);
+        wait(&bars->pd_full[s], ph, 11);
+        wait(&bars->d3_empty, (n & 1) ^ 1, 12);
+        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < 4; ++k)          // K^T (d b V), Q^T (gamma dO)
+          tc_mma_f16_ss(tmem + D3, xb_smem_desc(mn64, col + k * 2048), xb_smem_desc(mn64, dt + k * 2048), id3, k > 0);
+        tc_commit(&bars->d3_full);
+        if (OUT) {
+          wait(&bars->out_empty[s], ph ^ 1, 13);
+          tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {      // P V, P^T dO: planes hi, lo
+            const uint32_t a = pt + (k >> 2) * T64;
+            tc_mma_f16_ss(tmem + D2 + s * DSTEP, BWD ? xb_smem_desc(mn64, a + (k & 3) * 2048) : xb_smem_desc(kmaj, a + (k & 3) * 32),
+                          xb_smem_desc(mn64, st + ST_X + (k & 3) * 2048), id2, k > 0);
+          }
+        }
+        tc_commit(&bars->pd_empty[s]);
+        wait(&bars->s_full, n & 1, 14);
+        tc_fence_after();
+        if (KEEP) {
+          const int slices = p.dvp / NV;
+          uint8_t* dst = (uint8_t*)(BWD ? p.ds_tiles : p.s_tiles) + (((long long)chunk_of(n) * p.Hv + h) * slices + 2 * cb) * HALF;
+          bulk_store(dst, smem + SM_S, 2 * HALF);
+          tma_store_commit();
+        }
+        if (OUT) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)        // Q S, K dS'
+            tc_mma_f16_ss(tmem + D1 + s * DSTEP, xb_smem_desc(kmaj, row + (k >> 2) * T64 + (k & 3) * 32), xb_smem_desc(mn128, bs + k * 2048), id1, k > 0);
+          tc_commit(&bars->s_empty);
+          tc_commit(&bars->out_full[s]);
+        }
+        tc_commit(&bars->empty[s]);
+        if (KEEP) {
+          tma_store_wait_read<0>();
+          mbar_arrive(&bars->s_empty);
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp >= ADDERS / 32) {
+    // ------------------------------------ operands that depend on the chunk alone ------------------------------------
+    const int t = tid - ADDERS, row = t & 63, half = t >> 6;
+    for (int n = 0; n < steps; ++n) {
+      const int s = n & 1, len = chunks[chunk_of(n)].y;
+      uint8_t* st = smem + s * STAGE;
+      const float* hd = reinterpret_cast<const float*>(st + ST_HD);
+      wwait(&bars->full[s], (n >> 1) & 1, 20);
+      // rows behind the document's end hold the next one's: they must not meet a product's zeros (0 x Inf is NaN)
+      for (int i = t; i < 5 * (C - len) * 8; i += MAKERS) {
+        const int part = i / ((C - len) * 8), r = len + (i % ((C - len) * 8)) / 8;
+        reinterpret_cast<uint4*>(st + ST_K + part * T64 + r * 128)[i & 7] = make_uint4(0, 0, 0, 0);
+      }
+      if (len < C) asm volatile("bar.sync 1, %0;" ::"n"(MAKERS) : "memory");
+      wwait(&bars->pd_empty[s], ((n >> 1) & 1) ^ 1, 21);
+      {  // gamma dO, or d b V: 32 columns of a row
+        const float f = BWD ? ex2_sum(hd, row) : ex2_diff(hd, C - 1, row) * hd[2 * C + row];
+        uint8_t* dst = smem + SM_D + s * HALF + half * T64 + row * 128;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const uint4 v = *reinterpret_cast<const uint4*>(st + ST_X + row * 128 + (((half * 4 + u) ^ (row & 7)) << 4));
+          const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 y = unpack_bf16x2(x[e]);
+            split2(f * y.x, f * y.y, hi[e], lo[e]);
+          }
+          *reinterpret_cast<uint4*>(dst + ((u ^ (row & 7)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          *reinterpret_cast<uint4*>(dst + (((u + 4) ^ (row & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+      }
+      if (OUT) {  // P: 32 columns of a row
+        uint8_t* dst = smem + SM_P + s * HALF + row * 128;
+        const float gi = hd[row], gl = hd[C + row];
+        const uint8_t* src = st + ST_QK + half * T64 + row * 128;
+        const bool none = half * 32 > (row | 31);                     // the warp's rows end before these columns
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          uint32_t hi[4] = {}, lo[4] = {};
+          if (!none)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              const int j = half * 32 + u * 8 + q * 4;
+              const float4 x = *reinterpret_cast<const float4*>(src + (((u * 2 + q) ^ (row & 7)) << 4));
+              const float4 a = *reinterpret_cast<const float4*>(hd + j), b = *reinterpret_cast<const float4*>(hd + C + j);
+              const float4 w = *reinterpret_cast<const float4*>(hd + 2 * C + j);
+              const float y0 = j <= row ? x.x * w.x * xb_ex2((gi - a.x) + (gl - b.x)) : 0.f;
+              const float y1 = j + 1 <= row ? x.y * w.y * xb_ex2((gi - a.y) + (gl - b.y)) : 0.f;
+              const float y2 = j + 2 <= row ? x.z * w.z * xb_ex2((gi - a.z) + (gl - b.z)) : 0.f;
+              const float y3 = j + 3 <= row ? x.w * w.w * xb_ex2((gi - a.w) + (gl - b.w)) : 0.f;
+              split2(y0, y1, hi[2 * q], lo[2 * q]);
+              split2(y2, y3, hi[2 * q + 1], lo[2 * q + 1]);
+            }
+          const int off = ((half * 4 + u) ^ (row & 7)) << 4;
+          *reinterpret_cast<uint4*>(dst + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          *reinterpret_cast<uint4*>(dst + T64 + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+      }
+      fence_proxy_async_smem();
+      arrive(&bars->pd_full[s]);
+      arrive(&bars->empty[s]);
+    }
+  } else {
+    // ------------------------------------ the state, and the outputs -------------------------------------------------
+    const int q4 = warp & 3, sl = warp >> 2, r = q4 * 32 + lane, orow = q4 * 16 + (lane & 15);
+    const uint32_t base = tmem + ((uint32_t)(q4 * 32) << 16);
+    const int cols = min(NV, p.dv - v0 - sl * NV);
+    const long long soff = ((long long)doc * p.Hv + h) * p.dk * p.dv + (v0 + sl * NV) * p.s_v + r * p.s_k;
+    const float* from = BWD ? p.ds_out : p.s_in;
+    float* to = BWD ? p.ds_in : p.s_out;
+    float x[32];
+#pragma unroll
+    for (int e = 0; e < 32; ++e) x[e] = from != nullptr && doc < p.n_docs && r < p.dk && e < cols ? from[soff + e * p.s_v] : 0.f;
+    auto put = [&]() {                       // the state's row as [hi | lo]
+      uint8_t* dst = smem + SM_S + sl * HALF + r * 128;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) split2(x[8 * u + 2 * e], x[8 * u + 2 * e + 1], hi[e], lo[e]);
+        *reinterpret_cast<uint4*>(dst + ((u ^ (r & 7)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(dst + (((u + 4) ^ (r & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      }
+      fence_proxy_async_smem();
+      tc_fence_before();
+      arrive(&bars->s_full);
+    };
+    if (steps > 0) put();
+    const float skip = p.D[h];
+    bf16* out = (bf16*)(BWD ? p.dv_out : p.o);
+    for (int n = 0; n < steps; ++n) {
+      const int s = n & 1;
+      const int4 ch = chunks[chunk_of(n)];
+      const uint8_t* st = smem + s * STAGE;
+      const float* hd = reinterpret_cast<const float*>(st + ST_HD);
+      wwait(&bars->full[s], (n >> 1) & 1, 30);
+      const float f = BWD ? ex2_diff(hd, C - 1, orow) * hd[2 * C + orow] : ex2_sum(hd, orow), last = ex2_sum(hd, C - 1);
+      wwait(&bars->d3_full, n & 1, 31);
+      tc_fence_after();
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+        uint32_t a[16], b[16];
+        tmem_ld_32x16(base + D3 + sl * 64 + part * 16, a);
+        tmem_ld_32x16(base + D3 + sl * 64 + 32 + part * 16, b);
+        tc_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[part * 16 + e] = last * x[part * 16 + e] + (__uint_as_float(a[e]) + __uint_as_float(b[e]));
+      }
+      tc_fence_before();
+      arrive(&bars->d3_empty);
+      if (n + 1 < steps) {
+        wwait(&bars->s_empty, n & 1, 32);    // the tile's readers are done
+        put();
+      }
+      if (OUT) {
+        // lanes 0 .. 15 hold the rows of 64-row accumulators; lanes 16 .. 31 take the second half of the columns
+        const int u0 = sl * 4 + (lane >> 4) * 2;
+        uint4 xv[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) xv[u] = *reinterpret_cast<const uint4*>(st + ST_X + orow * 128 + (((u0 + u) ^ (orow & 7)) << 4));
+        wwait(&bars->out_full[s], (n >> 1) & 1, 33);
+        tc_fence_after();
+        float y[16];
+        {
+          uint32_t a[32], b[32];
+          tmem_ld_32x32(base + D1 + s * DSTEP + sl * 64, a);
+          tmem_ld_32x32(base + D1 + s * DSTEP + sl * 64 + 32, b);
+          tc_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) a[e] = __float_as_uint(f * (__uint_as_float(a[e]) + __uint_as_float(b[e])));
+          tmem_ld_32x32(base + D2 + s * DSTEP + sl * 32, b);
+          tc_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) a[e] = __float_as_uint(__uint_as_float(a[e]) + __uint_as_float(b[e]));
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const uint32_t far = __shfl_sync(0xffffffffu, a[16 + e], lane & 15);
+            y[e] = __uint_as_float(lane & 16 ? far : a[e]);
+          }
+        }
+        tc_fence_before();
+        arrive(&bars->out_empty[s]);
+        if (orow < ch.y)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int col = v0 + (u0 + u) * 8;
+            const uint32_t w[4] = {xv[u].x, xv[u].y, xv[u].z, xv[u].w};
+            uint32_t z[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 v = unpack_bf16x2(w[e]);
+              z[e] = pack_bf16x2(y[8 * u + 2 * e] + skip * v.x, y[8 * u + 2 * e + 1] + skip * v.y);
+            }
+            if (col < p.dv)
+              *reinterpret_cast<uint4*>(out + ((long long)(ch.x + orow) * p.Hv + h) * p.dv + col) = make_uint4(z[0], z[1], z[2], z[3]);
+          }
+      }
+      arrive(&bars->empty[s]);
+    }
+    if (to != nullptr && doc < p.n_docs && r < p.dk)
+#pragma unroll
+      for (int e = 0; e < 32; ++e)
+        if (e < cols) to[soff + e * p.s_v] = x[e];
+  }
+  // after a wait that ran out, loads and products may still be on their way: give them 0.2 s
+  if (*(volatile int*)&bars->abort_flag && tid == 0)
+    for (const uint64_t t0 = xb_globaltimer(); xb_globaltimer() - t0 < 200000000ull;) {}
+  tc_fence_before();
+  __syncthreads();
+  if (warp == LOADER) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <bool BWD, bool OUT, bool KEEP>
+int run(const XbRecArgs& a, const void* x, long long x_t, long long x_h, cudaStream_t st) {
+  const long long blocks = (long long)(a.n_docs + 2) * a.Hv * (a.dvp / 64);
+  if (blocks > 0x7fffffffLL) return -4;
+  CUtensorMap mk{}, mq{}, mx{}, mqk{};
+  if (a.T > 0 && (rec_tile_map(&mk, a.k, a.T, a.Hk, a.dk, a.k_t, a.k_h, 64, CU_TENSOR_MAP_SWIZZLE_128B) ||
+                  rec_tile_map(&mq, a.q, a.T, a.Hk, a.dk, a.q_t, a.q_h, 64, CU_TENSOR_MAP_SWIZZLE_128B) ||
+                  rec_tile_map(&mx, x, a.T, a.Hv, a.dv, x_t, x_h, 64, CU_TENSOR_MAP_SWIZZLE_128B) ||
+                  xb_make_tmap_2d(&mqk, a.qk, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, (uint64_t)a.nc_max * a.Hk * C, C, C, C, 32, CU_TENSOR_MAP_SWIZZLE_128B)))
+    return -2;
+  if (cudaFuncSetAttribute(scan_seq<BWD, OUT, KEEP>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess) {
+    cudaGetLastError();
+    return -5;
+  }
+  scan_seq<BWD, OUT, KEEP><<<(unsigned)blocks, THREADS, SMEM, st>>>(mk, mq, mx, mqk, a);
+  return cudaGetLastError() == cudaSuccess ? 0 : -11;
+}
+
+}  // namespace
+
+int xb_scan_fwd(const XbRecArgs& a, cudaStream_t st) {
+  const long long blocks = (long long)a.nc_max * a.Hk;
+  if (int rc = a.dk <= 64 ? rec_launch(scan_prep<64>, blocks, 128, 0, a, st) : rec_launch(scan_prep<128>, blocks, 128, 0, a, st)) return rc;
+  return run<false, true, false>(a, a.v, a.v_t, a.v_h, st);
+}
+int xb_scan_bwd(const XbRecArgs& a, cudaStream_t st) {
+  XbRecArgs again = a;
+  again.s_out = nullptr;
+  if (int rc = run<false, false, true>(again, a.v, a.v_t, a.v_h, st)) return rc;
+  return run<true, true, true>(a, a.dy, a.dy_t, a.dy_h, st);
+}
