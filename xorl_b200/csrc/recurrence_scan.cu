@@ -6,8 +6,8 @@
 //
 // The two are one computation with Q and K, and the row factors gamma and d b, exchanged, P transposed and the chunks
 // walked the other way.  The state does not feed back into what is added to it, so the products of a step need not wait
-// for one another: a CTA carries 64 state columns of one head through one document, four warps make the operands that
-// depend on the chunk alone (P, and d b V or gamma dO) ahead of the products, eight add up the state and write the
+// for one another: a CTA carries 64 state columns of one head through one document, ten warps make the operands that
+// depend on the chunk alone (P, and d b V or gamma dO) ahead of the products, sixteen add up the state and write the
 // outputs, one loads and one issues.  Computed operands are [hi 32 | lo 32] tiles (P: two planes).  Per step and CTA 20
 // products, about 1100 cycles of the tensor pipe, which bounds it next to the split and decay arithmetic.
 #include "recurrence_core.cuh"
@@ -84,7 +84,8 @@ __global__ void __launch_bounds__(128) scan_prep(const XbRecArgs p) {
 
 // ---- the sequential part -------------------------------------------------------------------------------------------
 constexpr int T64 = HALF / 2;
-constexpr int MAKERS = 128, ADDERS = 256, THREADS = MAKERS + ADDERS + 64;
+// warps: 16 add up the state and write outputs, 6 make P (a block of 32 rows and 16 columns each), 4 the other operand
+constexpr int ADDERS = 512, PMAKERS = 192, XMAKERS = 128, MAKERS = PMAKERS + XMAKERS, THREADS = ADDERS + MAKERS + 64;
 // K and Q: [64 rows][128 bytes] twice each; v or dO: [64][64 columns]; Q K^T: [64][32 fp32] twice; decays and b
 constexpr int ST_K = 0, ST_Q = 2 * T64, ST_X = 4 * T64, ST_QK = 5 * T64, ST_HD = 7 * T64, STAGE = 7 * T64 + 1024;
 constexpr int SM_S = 2 * STAGE, SM_P = SM_S + 2 * HALF, SM_D = SM_P + 2 * HALF, SM_BAR = SM_D + 2 * HALF;
@@ -114,8 +115,8 @@ scan_seq(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtenso
   auto chunk_of = [&](int n) { return BWD ? c0 + steps - 1 - n : c0 + n; };
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bars->full[i], 1), mbar_init(&bars->empty[i], 1 + (MAKERS + ADDERS) / 32);
-      mbar_init(&bars->pd_full[i], MAKERS / 32), mbar_init(&bars->pd_empty[i], 1);
+      mbar_init(&bars->full[i], 1), mbar_init(&bars->empty[i], 1 + ((OUT ? MAKERS : XMAKERS) + ADDERS) / 32);
+      mbar_init(&bars->pd_full[i], (OUT ? MAKERS : XMAKERS) / 32), mbar_init(&bars->pd_empty[i], 1);
       mbar_init(&bars->out_full[i], 1), mbar_init(&bars->out_empty[i], ADDERS / 32);
     }
     mbar_init(&bars->s_full, ADDERS / 32), mbar_init(&bars->s_empty, (OUT ? 1 : 0) + (KEEP ? 1 : 0));
@@ -214,97 +215,124 @@ scan_seq(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtenso
       }
     }
     __syncwarp();
-  } else if (warp >= ADDERS / 32) {
-    // ------------------------------------ operands that depend on the chunk alone ------------------------------------
-    const int t = tid - ADDERS, row = t & 63, half = t >> 6;
+  } else if (warp >= (ADDERS + PMAKERS) / 32) {
+    // ------------------------------------ gamma dO, or d b V: 32 columns of a row ------------------------------------
+    const int t = tid - ADDERS - PMAKERS, row = t & 63, half = t >> 6;
     for (int n = 0; n < steps; ++n) {
       const int s = n & 1, len = chunks[chunk_of(n)].y;
       uint8_t* st = smem + s * STAGE;
       const float* hd = reinterpret_cast<const float*>(st + ST_HD);
       wwait(&bars->full[s], (n >> 1) & 1, 20);
       // rows behind the document's end hold the next one's: they must not meet a product's zeros (0 x Inf is NaN)
-      for (int i = t; i < 5 * (C - len) * 8; i += MAKERS) {
-        const int part = i / ((C - len) * 8), r = len + (i % ((C - len) * 8)) / 8;
-        reinterpret_cast<uint4*>(st + ST_K + part * T64 + r * 128)[i & 7] = make_uint4(0, 0, 0, 0);
+      if (len < C) {
+        for (int i = t; i < 5 * (C - len) * 8; i += XMAKERS) {
+          const int part = i / ((C - len) * 8), r = len + (i % ((C - len) * 8)) / 8;
+          reinterpret_cast<uint4*>(st + ST_K + part * T64 + r * 128)[i & 7] = make_uint4(0, 0, 0, 0);
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(XMAKERS) : "memory");
       }
-      if (len < C) asm volatile("bar.sync 1, %0;" ::"n"(MAKERS) : "memory");
+      const float f = BWD ? ex2_sum(hd, row) : ex2_diff(hd, C - 1, row) * hd[2 * C + row];
+      uint4 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const uint4*>(st + ST_X + row * 128 + (((half * 4 + u) ^ (row & 7)) << 4));
       wwait(&bars->pd_empty[s], ((n >> 1) & 1) ^ 1, 21);
-      {  // gamma dO, or d b V: 32 columns of a row
-        const float f = BWD ? ex2_sum(hd, row) : ex2_diff(hd, C - 1, row) * hd[2 * C + row];
-        uint8_t* dst = smem + SM_D + s * HALF + half * T64 + row * 128;
+      uint8_t* dst = smem + SM_D + s * HALF + half * T64 + row * 128;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const uint4 v = *reinterpret_cast<const uint4*>(st + ST_X + row * 128 + (((half * 4 + u) ^ (row & 7)) << 4));
-          const uint32_t x[4] = {v.x, v.y, v.z, v.w};
-          uint32_t hi[4], lo[4];
+      for (int u = 0; u < 4; ++u) {
+        const uint32_t x[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+        uint32_t hi[4], lo[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 y = unpack_bf16x2(x[e]);
-            split2(f * y.x, f * y.y, hi[e], lo[e]);
-          }
-          *reinterpret_cast<uint4*>(dst + ((u ^ (row & 7)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          *reinterpret_cast<uint4*>(dst + (((u + 4) ^ (row & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        for (int e = 0; e < 4; ++e) {
+          const float2 y = unpack_bf16x2(x[e]);
+          split2(f * y.x, f * y.y, hi[e], lo[e]);
         }
-      }
-      if (OUT) {  // P: 32 columns of a row
-        uint8_t* dst = smem + SM_P + s * HALF + row * 128;
-        const float gi = hd[row], gl = hd[C + row];
-        const uint8_t* src = st + ST_QK + half * T64 + row * 128;
-        const bool none = half * 32 > (row | 31);                     // the warp's rows end before these columns
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          uint32_t hi[4] = {}, lo[4] = {};
-          if (!none)
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              const int j = half * 32 + u * 8 + q * 4;
-              const float4 x = *reinterpret_cast<const float4*>(src + (((u * 2 + q) ^ (row & 7)) << 4));
-              const float4 a = *reinterpret_cast<const float4*>(hd + j), b = *reinterpret_cast<const float4*>(hd + C + j);
-              const float4 w = *reinterpret_cast<const float4*>(hd + 2 * C + j);
-              const float y0 = j <= row ? x.x * w.x * xb_ex2((gi - a.x) + (gl - b.x)) : 0.f;
-              const float y1 = j + 1 <= row ? x.y * w.y * xb_ex2((gi - a.y) + (gl - b.y)) : 0.f;
-              const float y2 = j + 2 <= row ? x.z * w.z * xb_ex2((gi - a.z) + (gl - b.z)) : 0.f;
-              const float y3 = j + 3 <= row ? x.w * w.w * xb_ex2((gi - a.w) + (gl - b.w)) : 0.f;
-              split2(y0, y1, hi[2 * q], lo[2 * q]);
-              split2(y2, y3, hi[2 * q + 1], lo[2 * q + 1]);
-            }
-          const int off = ((half * 4 + u) ^ (row & 7)) << 4;
-          *reinterpret_cast<uint4*>(dst + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          *reinterpret_cast<uint4*>(dst + T64 + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        }
+        *reinterpret_cast<uint4*>(dst + ((u ^ (row & 7)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(dst + (((u + 4) ^ (row & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
       fence_proxy_async_smem();
       arrive(&bars->pd_full[s]);
       arrive(&bars->empty[s]);
     }
+  } else if (warp >= ADDERS / 32) {
+    // ------------------------------------ P: 16 columns of a row -----------------------------------------------------
+    // blocks of 32 rows and 16 columns on and below the diagonal: two of the upper rows, four of the lower ones
+    const int m = warp - ADDERS / 32, row = (m < 2 ? 0 : 32) + lane, j0 = (m < 2 ? m : m - 2) * 16;
+    if (OUT && m < 2)                                                 // the two above it stay zero
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          *reinterpret_cast<uint4*>(smem + SM_P + i * HALF + (u >> 1) * T64 + row * 128 + (((4 + m * 2 + (u & 1)) ^ (row & 7)) << 4)) =
+              make_uint4(0, 0, 0, 0);
+    for (int n = 0; OUT && n < steps; ++n) {
+      const int s = n & 1;
+      const uint8_t* st = smem + s * STAGE;
+      const float* hd = reinterpret_cast<const float*>(st + ST_HD);
+      wwait(&bars->full[s], (n >> 1) & 1, 22);
+      const float gi = hd[row], gl = hd[C + row];
+      const uint8_t* src = st + ST_QK + (j0 >> 5) * T64 + row * 128;
+      float y[16];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int j = j0 + q * 4;
+        const float4 x = *reinterpret_cast<const float4*>(src + ((((j & 31) >> 2) ^ (row & 7)) << 4));
+        const float4 a = *reinterpret_cast<const float4*>(hd + j), b = *reinterpret_cast<const float4*>(hd + C + j);
+        const float4 w = *reinterpret_cast<const float4*>(hd + 2 * C + j);
+        y[4 * q] = j <= row ? x.x * w.x * xb_ex2((gi - a.x) + (gl - b.x)) : 0.f;
+        y[4 * q + 1] = j + 1 <= row ? x.y * w.y * xb_ex2((gi - a.y) + (gl - b.y)) : 0.f;
+        y[4 * q + 2] = j + 2 <= row ? x.z * w.z * xb_ex2((gi - a.z) + (gl - b.z)) : 0.f;
+        y[4 * q + 3] = j + 3 <= row ? x.w * w.w * xb_ex2((gi - a.w) + (gl - b.w)) : 0.f;
+      }
+      arrive(&bars->empty[s]);
+      uint32_t hi[8], lo[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) split2(y[2 * e], y[2 * e + 1], hi[e], lo[e]);
+      wwait(&bars->pd_empty[s], ((n >> 1) & 1) ^ 1, 23);
+      uint8_t* dst = smem + SM_P + s * HALF + row * 128;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int off = (((j0 >> 3) + u) ^ (row & 7)) << 4;
+        *reinterpret_cast<uint4*>(dst + off) = make_uint4(hi[4 * u], hi[4 * u + 1], hi[4 * u + 2], hi[4 * u + 3]);
+        *reinterpret_cast<uint4*>(dst + T64 + off) = make_uint4(lo[4 * u], lo[4 * u + 1], lo[4 * u + 2], lo[4 * u + 3]);
+      }
+      fence_proxy_async_smem();
+      arrive(&bars->pd_full[s]);
+    }
   } else {
     // ------------------------------------ the state, and the outputs -------------------------------------------------
-    const int q4 = warp & 3, sl = warp >> 2, r = q4 * 32 + lane, orow = q4 * 16 + (lane & 15);
+    // a row of the state and 16 of its columns; 16 lanes of each warp hold the rows of the 64-row accumulators, the other
+    // 16 take half of their columns
+    const int q4 = warp & 3, sl = warp >> 3, part = (warp >> 2) & 1, r = q4 * 32 + lane, orow = q4 * 16 + (lane & 15);
     const uint32_t base = tmem + ((uint32_t)(q4 * 32) << 16);
-    const int cols = min(NV, p.dv - v0 - sl * NV);
-    const long long soff = ((long long)doc * p.Hv + h) * p.dk * p.dv + (v0 + sl * NV) * p.s_v + r * p.s_k;
+    const int col = v0 + sl * NV + part * 16, cols = p.dv - col;
+    const long long soff = ((long long)doc * p.Hv + h) * p.dk * p.dv + col * p.s_v + r * p.s_k;
     const float* from = BWD ? p.ds_out : p.s_in;
     float* to = BWD ? p.ds_in : p.s_out;
-    float x[32];
+    float x[16];
 #pragma unroll
-    for (int e = 0; e < 32; ++e) x[e] = from != nullptr && doc < p.n_docs && r < p.dk && e < cols ? from[soff + e * p.s_v] : 0.f;
+    for (int e = 0; e < 16; ++e) x[e] = from != nullptr && doc < p.n_docs && r < p.dk && e < cols ? from[soff + e * p.s_v] : 0.f;
+    uint32_t hi[8], lo[8];
+    auto split_row = [&]() {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) split2(x[2 * e], x[2 * e + 1], hi[e], lo[e]);
+    };
     auto put = [&]() {                       // the state's row as [hi | lo]
       uint8_t* dst = smem + SM_S + sl * HALF + r * 128;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) split2(x[8 * u + 2 * e], x[8 * u + 2 * e + 1], hi[e], lo[e]);
-        *reinterpret_cast<uint4*>(dst + ((u ^ (r & 7)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<uint4*>(dst + (((u + 4) ^ (r & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      for (int i = 0; i < 2; ++i) {
+        const int u = part * 2 + i;
+        *reinterpret_cast<uint4*>(dst + ((u ^ (r & 7)) << 4)) = make_uint4(hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
+        *reinterpret_cast<uint4*>(dst + (((u + 4) ^ (r & 7)) << 4)) = make_uint4(lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
       }
       fence_proxy_async_smem();
       tc_fence_before();
       arrive(&bars->s_full);
     };
+    split_row();
     if (steps > 0) put();
     const float skip = p.D[h];
-    bf16* out = (bf16*)(BWD ? p.dv_out : p.o);
+    const int u0 = sl * 4 + part * 2 + (lane >> 4), ocol = v0 + u0 * 8;
+    bf16* out = (bf16*)(BWD ? p.dv_out : p.o) + (long long)h * p.dv + ocol;
     for (int n = 0; n < steps; ++n) {
       const int s = n & 1;
       const int4 ch = chunks[chunk_of(n)];
@@ -312,71 +340,59 @@ scan_seq(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtenso
       const float* hd = reinterpret_cast<const float*>(st + ST_HD);
       wwait(&bars->full[s], (n >> 1) & 1, 30);
       const float f = BWD ? ex2_diff(hd, C - 1, orow) * hd[2 * C + orow] : ex2_sum(hd, orow), last = ex2_sum(hd, C - 1);
+      uint4 xv = make_uint4(0, 0, 0, 0);
+      if (OUT) xv = *reinterpret_cast<const uint4*>(st + ST_X + orow * 128 + ((u0 ^ (orow & 7)) << 4));
+      arrive(&bars->empty[s]);
       wwait(&bars->d3_full, n & 1, 31);
       tc_fence_after();
-#pragma unroll
-      for (int part = 0; part < 2; ++part) {
+      {
         uint32_t a[16], b[16];
         tmem_ld_32x16(base + D3 + sl * 64 + part * 16, a);
         tmem_ld_32x16(base + D3 + sl * 64 + 32 + part * 16, b);
         tc_wait_ld();
+        tc_fence_before();
+        arrive(&bars->d3_empty);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[part * 16 + e] = last * x[part * 16 + e] + (__uint_as_float(a[e]) + __uint_as_float(b[e]));
+        for (int e = 0; e < 16; ++e) x[e] = last * x[e] + (__uint_as_float(a[e]) + __uint_as_float(b[e]));
       }
-      tc_fence_before();
-      arrive(&bars->d3_empty);
       if (n + 1 < steps) {
+        split_row();
         wwait(&bars->s_empty, n & 1, 32);    // the tile's readers are done
         put();
       }
       if (OUT) {
-        // lanes 0 .. 15 hold the rows of 64-row accumulators; lanes 16 .. 31 take the second half of the columns
-        const int u0 = sl * 4 + (lane >> 4) * 2;
-        uint4 xv[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) xv[u] = *reinterpret_cast<const uint4*>(st + ST_X + orow * 128 + (((u0 + u) ^ (orow & 7)) << 4));
         wwait(&bars->out_full[s], (n >> 1) & 1, 33);
         tc_fence_after();
-        float y[16];
-        {
-          uint32_t a[32], b[32];
-          tmem_ld_32x32(base + D1 + s * DSTEP + sl * 64, a);
-          tmem_ld_32x32(base + D1 + s * DSTEP + sl * 64 + 32, b);
-          tc_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 32; ++e) a[e] = __float_as_uint(f * (__uint_as_float(a[e]) + __uint_as_float(b[e])));
-          tmem_ld_32x32(base + D2 + s * DSTEP + sl * 32, b);
-          tc_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 32; ++e) a[e] = __float_as_uint(__uint_as_float(a[e]) + __uint_as_float(b[e]));
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const uint32_t far = __shfl_sync(0xffffffffu, a[16 + e], lane & 15);
-            y[e] = __uint_as_float(lane & 16 ? far : a[e]);
-          }
-        }
+        uint32_t a[16], b[16], d[16];
+        tmem_ld_32x16(base + D1 + s * DSTEP + sl * 64 + part * 16, a);
+        tmem_ld_32x16(base + D1 + s * DSTEP + sl * 64 + 32 + part * 16, b);
+        tmem_ld_32x16(base + D2 + s * DSTEP + sl * 32 + part * 16, d);
+        tc_wait_ld();
         tc_fence_before();
         arrive(&bars->out_empty[s]);
-        if (orow < ch.y)
+        float y[8];
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int col = v0 + (u0 + u) * 8;
-            const uint32_t w[4] = {xv[u].x, xv[u].y, xv[u].z, xv[u].w};
-            uint32_t z[4];
+        for (int e = 0; e < 16; ++e) a[e] = __float_as_uint(f * (__uint_as_float(a[e]) + __uint_as_float(b[e])) + __uint_as_float(d[e]));
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float2 v = unpack_bf16x2(w[e]);
-              z[e] = pack_bf16x2(y[8 * u + 2 * e] + skip * v.x, y[8 * u + 2 * e + 1] + skip * v.y);
-            }
-            if (col < p.dv)
-              *reinterpret_cast<uint4*>(out + ((long long)(ch.x + orow) * p.Hv + h) * p.dv + col) = make_uint4(z[0], z[1], z[2], z[3]);
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t far = __shfl_sync(0xffffffffu, a[8 + e], lane & 15);
+          y[e] = __uint_as_float(lane & 16 ? far : a[e]);
+        }
+        if (orow < ch.y && ocol < p.dv) {
+          const uint32_t w[4] = {xv.x, xv.y, xv.z, xv.w};
+          uint32_t z[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 v = unpack_bf16x2(w[e]);
+            z[e] = pack_bf16x2(y[2 * e] + skip * v.x, y[2 * e + 1] + skip * v.y);
           }
+          *reinterpret_cast<uint4*>(out + (long long)(ch.x + orow) * p.Hv * p.dv) = make_uint4(z[0], z[1], z[2], z[3]);
+        }
       }
-      arrive(&bars->empty[s]);
     }
     if (to != nullptr && doc < p.n_docs && r < p.dk)
 #pragma unroll
-      for (int e = 0; e < 32; ++e)
+      for (int e = 0; e < 16; ++e)
         if (e < cols) to[soff + e * p.s_v] = x[e];
   }
   // after a wait that ran out, loads and products may still be on their way: give them 0.2 s
