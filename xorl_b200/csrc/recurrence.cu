@@ -140,16 +140,17 @@ XB_API int xb_recurrence_fwd(const XbRecArgs* args, int delta, void* stream) {
   return xb_scan_fwd(*a, st);
 }
 
-XB_API int xb_recurrence_bwd(const XbRecArgs* args, int delta, void* stream) {
+// tiles: the forward pass has left its tiles in s_tiles (and u_tiles); else they are made again.
+XB_API int xb_recurrence_bwd(const XbRecArgs* args, int delta, int tiles, void* stream) {
   if (args == nullptr || bad_args(*args)) return -1;
   XbRecArgs mine = *args, *a = &mine;
   mine.status = xb_status_ptr();
   cudaStream_t st = (cudaStream_t)stream;
   if (delta) {
-    if (int rc = xb_delta_bwd(*a, st)) return rc;
+    if (int rc = xb_delta_bwd(*a, tiles, st)) return rc;
     return xb_recurrence_grad(*a, 1, st);
   }
-  if (int rc = xb_scan_bwd(*a, st)) return rc;
+  if (int rc = xb_scan_bwd(*a, tiles, st)) return rc;
   if (int rc = xb_recurrence_grad(*a, 0, st)) return rc;
   return rec_launch(rec_reduce, a->Hv, 128, 0, *a, st);
 }

@@ -449,7 +449,8 @@ __device__ __forceinline__ void zero_rows(const XbRecArgs& p, const Cta& a, bf16
 // that runs out raises a flag; everybody then walks through the remaining steps without waiting, so that no barrier
 // is left with a thread missing.
 
-template <bool SAVE>
+// OUT: outputs are wanted.  SAVE: the tiles of the states and of U go to global memory.
+template <bool OUT, bool SAVE>
 __global__ void __launch_bounds__(THREADS, 1)
 delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mv,
           const __grid_constant__ XbRecArgs p) {
@@ -459,7 +460,7 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
   bf16* o = (bf16*)p.o + (long long)a.h * p.dv + a.v0;
   const long long o_t = (long long)p.Hv * p.dv;
   if (!inside) {
-    if (!SAVE) zero_rows(p, a, o, o_t);
+    if (OUT) zero_rows(p, a, o, o_t);
     return;
   }
   cta_begin(a);
@@ -566,7 +567,7 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       fence_proxy_async_smem();
       tc_fence_before();
       bar_arrive(3, THREADS);
-      if (!SAVE && !krow && i < len) {       // O = gamma rq Q S + (P T) R
+      if (OUT && !krow && i < len) {       // O = gamma rq Q S + (P T) R
         const float f = gam * rq;
         bf16* dst = o + (t0 + i) * o_t + half * 16;
 #pragma unroll
@@ -778,11 +779,13 @@ int prep(const XbRecArgs& a, cudaStream_t st) {
 
 int xb_delta_fwd(const XbRecArgs& a, cudaStream_t st) {
   if (int rc = a.dk <= 64 ? prep<64>(a, st) : prep<128>(a, st)) return rc;
-  return run(delta_fwd<false>, a, a.v, a.v_t, a.v_h, st);
+  return a.s_tiles != nullptr ? run(delta_fwd<true, true>, a, a.v, a.v_t, a.v_h, st) : run(delta_fwd<true, false>, a, a.v, a.v_t, a.v_h, st);
 }
-int xb_delta_bwd(const XbRecArgs& a, cudaStream_t st) {
-  XbRecArgs again = a;
-  again.s_out = nullptr;
-  if (int rc = run(delta_fwd<true>, again, a.v, a.v_t, a.v_h, st)) return rc;
+int xb_delta_bwd(const XbRecArgs& a, int tiles, cudaStream_t st) {
+  if (!tiles) {
+    XbRecArgs again = a;
+    again.s_out = nullptr;
+    if (int rc = run(delta_fwd<false, true>, again, a.v, a.v_t, a.v_h, st)) return rc;
+  }
   return run(delta_bwd, a, a.dy, a.dy_t, a.dy_h, st);
 }

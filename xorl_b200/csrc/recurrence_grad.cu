@@ -9,13 +9,15 @@
 // registers, their dot products with q and k give the gradient of the decay and of b, and D o dP, D o dL are added up;
 // the products with K and Q are the same for all heads of the group and are made once, from the sums.
 // The tiles that it reads (60 KB per head and 32 columns; scan 40 KB) bound it: they are what the two sequential passes
-// keep.  Eight worker warps, a loading and an issuing warp, and one that turns the heads' sums into gradients of the
+// keep.  Sixteen worker warps, a loading and an issuing warp, and one that turns the heads' sums into gradients of the
 // decay; 64-row accumulators lie in 16 lanes of each warp.
 #include "recurrence_core.cuh"
 
 namespace {
 
-constexpr int WORKERS = 256, THREADS = WORKERS + 96;
+constexpr int WORKERS = 512, THREADS = WORKERS + 96;
+constexpr int PARTS = WORKERS / 128;                // column parts of the wide products: 128 / PARTS columns per warp
+constexpr int WIDE = 8 / PARTS, SQUARE = 4 / PARTS;  // pieces of 16 columns of a warp's part
 constexpr int T64 = HALF / 2;                       // 8 KB: [64 rows][128 bytes]
 template <bool DELTA>
 struct Lay {
@@ -26,10 +28,10 @@ struct Lay {
   static constexpr int SM_Q = 0, SM_K = 2 * T64, SM_RING = 4 * T64, SM_DOV = SM_RING + RING * STAGE, SM_RED = SM_DOV + 2 * DOV;
 };
 struct Red {                                        // what meets across warps, one set per head in turn
-  float rd[3][2][C];                                // q.t1, k.t2, k.t3 by column half
-  float er[2][C], fr[2][C];                         // row sums of dP o P and dL o A by column half (scan: dP o P)
+  float rd[3][PARTS][C];                            // q.t1, k.t2, k.t3 by column part
+  float er[PARTS][C], fr[PARTS][C];                 // row sums of dP o P and dL o A by column part (scan: dP o P)
   float ec[4][C], fc[4][C];                         // column sums by row block
-  float rv[C], sdot[8];
+  float rv[C], sdot[WORKERS / 32];
   float hd[HD];
 };
 struct __align__(8) Bars {
@@ -41,6 +43,12 @@ template <bool DELTA>
 constexpr int smem_bytes() { return Lay<DELTA>::SM_RED + 2 * (int)sizeof(Red) + RQK * 4 + 256 + 1024; }
 constexpr int COL_P = 0, COL_L = 64, COL_T1 = 128, COL_T2 = 256, COL_T3 = 384;
 
+__device__ __forceinline__ float parts(const float (&a)[PARTS][C], int t) {
+  float s = a[0][t] + a[1][t];
+#pragma unroll
+  for (int i = 2; i < PARTS; i += 2) s += a[i][t] + a[i + 1][t];
+  return s;
+}
 __device__ __forceinline__ void wbar() { asm volatile("bar.sync 1, %0;" ::"n"(WORKERS) : "memory"); }
 
 // D (64 x N) += A (64 x 16 of a row of 16-column steps) B^T: one step each
@@ -93,18 +101,18 @@ __device__ __forceinline__ void floats8(const uint4 u, float (&x)[8]) {
     x[2 * j] = f.x, x[2 * j + 1] = f.y;
   }
 }
-// acc += f * t over this thread's columns of its row: 8 of every 16, four times, units `unit` + 2 i; returns t . (the same
+// acc += f * t over this thread's columns of its row: 8 of every 16, units `unit` + 2 i; returns t . (the same
 // columns of `tile`).  The next 16 columns are on their way while 8 are worked on.
-__device__ __forceinline__ float add_rows(uint32_t addr, const uint8_t* tile, int row, int unit, float f, float (&acc)[32]) {
+__device__ __forceinline__ float add_rows(uint32_t addr, const uint8_t* tile, int row, int unit, float f, float (&acc)[8 * WIDE]) {
   uint32_t t[2][16];
   float dot[2] = {0.f, 0.f};
   tmem_ld_32x16(addr, t[0]);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < WIDE; ++i) {
     float x[8], y[8];
     floats8(tile_unit(tile, row, unit + 2 * i), x);
     tc_wait_ld();
-    if (i < 3) tmem_ld_32x16(addr + 16 * (i + 1), t[(i + 1) & 1]);
+    if (i + 1 < WIDE) tmem_ld_32x16(addr + 16 * (i + 1), t[(i + 1) & 1]);
     spread<8>(t[i & 1], y);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -278,7 +286,7 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
         const float bt = hd[2 * C + t], ga = ex2_sum(hd, t), de = ex2_diff(hd, C - 1, t);
         const bool on = t < len;
         auto four = [&](const float (&a)[4][C]) { return (a[0][t] + a[1][t]) + (a[2][t] + a[3][t]); };
-        auto two = [&](const float (&a)[2][C]) { return a[0][t] + a[1][t]; };
+        auto two = [&](const float (&a)[PARTS][C]) { return parts(a, t); };
         const float q1 = on ? ga * rqk[t] * two(r.rd[0]) : 0.f, k2 = on && DELTA ? ga * rqk[C + t] * two(r.rd[1]) : 0.f;
         const float k3 = on ? de * rqk[C + t] * two(r.rd[2]) : 0.f;
         const float e1 = two(r.er), e2 = four(r.ec), g1 = DELTA ? two(r.fr) : 0.f, g2 = DELTA ? four(r.fc) : 0.f;
@@ -293,7 +301,7 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
           dsum += r.rv[t];
         }
       }
-      float sd = lane < 8 ? r.sdot[lane] : 0.f;
+      float sd = lane < WORKERS / 32 ? r.sdot[lane] : 0.f;
       sd = warp_sum(sd);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
@@ -332,12 +340,16 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
     }
   } else {
     // ------------------------------------------------ workers -----------------------------------------------
-    // row `row`; of its warp's half of the columns the lower or upper 8 of every 16: units cu, cu + 2, .. of the wide
+    // row `row`; of its warp's part of the columns the lower or upper 8 of every 16: units cu, cu + 2, .. of the wide
     // products, columns j0 .., j0 + 16 .. of the square ones
-    const int q4 = warp & 3, hf = warp >> 2, row = q4 * 16 + (lane & 15), cu = hf * 8 + (lane >> 4), j0 = hf * 32 + (lane >> 4) * 8;
+    const int q4 = warp & 3, hf = warp >> 2, row = q4 * 16 + (lane & 15), cu = hf * 2 * WIDE + (lane >> 4), j0 = hf * 16 * SQUARE + (lane >> 4) * 8;
     const bool act = lane < 16;
     const uint32_t base = tmem + ((uint32_t)(q4 * 32) << 16);
-    float aq[32] = {}, ak[32] = {}, az[16] = {}, aw[DELTA ? 16 : 1] = {};
+    float aq[8 * WIDE] = {}, ak[8 * WIDE] = {}, az[8 * SQUARE] = {}, aw[DELTA ? 8 * SQUARE : 1] = {};
+    for (int i = 0; i < SQUARE; ++i) {               // first use is behind the first head's products
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(p.qk + ((long long)c * p.Hk + kh) * (C * C) + row * C + j0 + 16 * i));
+      if (DELTA) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.kk + ((long long)c * p.Hk + kh) * (C * C) + row * C + j0 + 16 * i));
+    }
     auto wwait = [&](uint64_t* b, uint32_t parity, int detail) {
       wait(b, parity, detail);
       __syncwarp();
@@ -364,7 +376,7 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
           const uint8_t* st = smem + L::SM_RING + s * L::STAGE;
           wwait(&bars->full[s], (n / L::RING) & 1, 42);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {  // <S, dS'>: two units of eight columns of a row per thread
+          for (int i = 0; i < 512 / WORKERS; ++i) {  // <S, dS'>: units of eight columns of a row
             const int sr = i * 64 + (tid >> 2), u = tid & 3;
             const uint32_t hi = (uint32_t)(sr * 128 + ((u ^ (sr & 7)) << 4)), lo = (uint32_t)(sr * 128 + (((u + 4) ^ (sr & 7)) << 4));
             float a[8], al[8], b[8], bl[8];
@@ -373,7 +385,7 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
 #pragma unroll
             for (int e = 0; e < 8; ++e) sdot += (a[e] + al[e]) * (b[e] + bl[e]);
           }
-          {  // dR.v (scan: dO.v)
+          if (tid < 4 * C) {  // dR.v (scan: dO.v)
             const int sr = tid >> 2, u = tid & 3;
             float v[8], a[8], al[8];
             floats8(tile_unit(dov + 2 * T64, sr, (sl & 3) * 4 + u), v);
@@ -397,7 +409,7 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
       if (lane == 0) r.sdot[warp] = sdot;
       rv += __shfl_xor_sync(0xffffffffu, rv, 1);
       rv += __shfl_xor_sync(0xffffffffu, rv, 2);
-      if ((tid & 3) == 0) r.rv[tid >> 2] = rv;
+      if (tid < 4 * C && (tid & 3) == 0) r.rv[tid >> 2] = rv;
       const float b = hd[2 * C + row], gam = ex2_sum(hd, row), dec = ex2_diff(hd, C - 1, row);
       wwait(&bars->acc_full, hh & 1, 43);
       tc_fence_after();
@@ -406,7 +418,7 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
         const float gi = hd[row], gl = hd[C + row];
         const int last = row < len ? row : -1;                        // the row's last column; none behind the end
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < SQUARE; ++i) {
           const int j = j0 + 16 * i;
           float hi[8], lo[8], kj[8], bj[8], qr[8], kr[8], x[8], v[8];
           uint32_t t[16], tl[16];
@@ -414,8 +426,8 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
             const float4 a = reinterpret_cast<const float4*>(src)[0], c4 = reinterpret_cast<const float4*>(src)[1];
             dst[0] = a.x, dst[1] = a.y, dst[2] = a.z, dst[3] = a.w, dst[4] = c4.x, dst[5] = c4.y, dst[6] = c4.z, dst[7] = c4.w;
           };
-          tmem_ld_32x16(base + COL_P + hf * 32 + 16 * i, t);
-          if (DELTA) tmem_ld_32x16(base + COL_L + hf * 32 + 16 * i, tl);
+          tmem_ld_32x16(base + COL_P + hf * 16 * SQUARE + 16 * i, t);
+          if (DELTA) tmem_ld_32x16(base + COL_L + hf * 16 * SQUARE + 16 * i, tl);
           eight(qk + 16 * i, qr);
           if (DELTA) eight(kk + 16 * i, kr);
           eight(hd + j, hi), eight(hd + C + j, lo), eight(rqk + C + j, kj);
@@ -452,9 +464,9 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
       {
         const bool on = row < len;                                    // rows behind the end hold other documents' products
         const float f1 = on ? gam * rq : 0.f, f2 = on ? -b * gam * rk : 0.f, f3 = on ? dec * rk * (DELTA ? 1.f : b) : 0.f;
-        const float d1 = add_rows(base + COL_T1 + hf * 64, smem + L::SM_Q, row, cu, f1, aq);
-        const float d2 = DELTA ? add_rows(base + COL_T2 + hf * 64, smem + L::SM_K, row, cu, f2, ak) : 0.f;
-        const float d3 = add_rows(base + COL_T3 + hf * 64, smem + L::SM_K, row, cu, f3, ak);
+        const float d1 = add_rows(base + COL_T1 + hf * 16 * WIDE, smem + L::SM_Q, row, cu, f1, aq);
+        const float d2 = DELTA ? add_rows(base + COL_T2 + hf * 16 * WIDE, smem + L::SM_K, row, cu, f2, ak) : 0.f;
+        const float d3 = add_rows(base + COL_T3 + hf * 16 * WIDE, smem + L::SM_K, row, cu, f3, ak);
         if (act) r.rd[0][hf][row] = d1, r.rd[1][hf][row] = d2, r.rd[2][hf][row] = d3;
       }
       tc_fence_before();
@@ -468,7 +480,7 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
 #pragma unroll
       for (int part = 0; part < (DELTA ? 2 : 1); ++part) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < SQUARE; ++u) {
           uint32_t hi[4], lo[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -490,14 +502,14 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
     arrive(&bars->acc_empty);
     wwait(&bars->last, 0, 44);
     tc_fence_after();
-    add_rows(base + COL_T1 + hf * 64, smem + L::SM_Q, row, cu, 1.f, aq);
-    add_rows(base + COL_T2 + hf * 64, smem + L::SM_K, row, cu, 1.f, ak);
+    add_rows(base + COL_T1 + hf * 16 * WIDE, smem + L::SM_Q, row, cu, 1.f, aq);
+    add_rows(base + COL_T2 + hf * 16 * WIDE, smem + L::SM_K, row, cu, 1.f, ak);
     // gradient through the L2 norms: dq - q^ (q^ . dq), rows of norm below 1e-12 excepted
     float fq = 0.f, fk = 0.f;
     if (p.l2norm) {
       float sq = 0.f, sk = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < WIDE; ++i) {
         const int unit = cu + 2 * i;
         float x[8], y[8];
         floats8(tile_unit(smem + L::SM_Q, row, unit), x), floats8(tile_unit(smem + L::SM_K, row, unit), y);
@@ -510,12 +522,12 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
       if (act) r.rd[0][hf][row] = sq, r.rd[1][hf][row] = sk;
       wbar();
       const float nq = rq / p.scale;
-      if (nq < 0.99e12f) fq = nq * nq * (r.rd[0][0][row] + r.rd[0][1][row]);
-      if (rk < 0.99e12f) fk = rk * rk * (r.rd[1][0][row] + r.rd[1][1][row]);
+      if (nq < 0.99e12f) fq = nq * nq * parts(r.rd[0], row);
+      if (rk < 0.99e12f) fk = rk * rk * parts(r.rd[1], row);
     }
     if (row < len)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < WIDE; ++i) {
         const int unit = cu + 2 * i, col = unit * 8;
         if (col < p.dk) {
           float x[8], y[8];

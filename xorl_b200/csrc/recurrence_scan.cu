@@ -429,11 +429,13 @@ int run(const XbRecArgs& a, const void* x, long long x_t, long long x_h, cudaStr
 int xb_scan_fwd(const XbRecArgs& a, cudaStream_t st) {
   const long long blocks = (long long)a.nc_max * a.Hk;
   if (int rc = a.dk <= 64 ? rec_launch(scan_prep<64>, blocks, 128, 0, a, st) : rec_launch(scan_prep<128>, blocks, 128, 0, a, st)) return rc;
-  return run<false, true, false>(a, a.v, a.v_t, a.v_h, st);
+  return a.s_tiles != nullptr ? run<false, true, true>(a, a.v, a.v_t, a.v_h, st) : run<false, true, false>(a, a.v, a.v_t, a.v_h, st);
 }
-int xb_scan_bwd(const XbRecArgs& a, cudaStream_t st) {
-  XbRecArgs again = a;
-  again.s_out = nullptr;
-  if (int rc = run<false, false, true>(again, a.v, a.v_t, a.v_h, st)) return rc;
+int xb_scan_bwd(const XbRecArgs& a, int tiles, cudaStream_t st) {
+  if (!tiles) {
+    XbRecArgs again = a;
+    again.s_out = nullptr;
+    if (int rc = run<false, false, true>(again, a.v, a.v_t, a.v_h, st)) return rc;
+  }
   return run<true, true, true>(a, a.dy, a.dy_t, a.dy_h, st);
 }

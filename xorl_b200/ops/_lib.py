@@ -118,7 +118,7 @@ _SIGNATURES = {
     "xb_gated_norm_bwd": [P, L, P, L, P, L, P, I, I, P, P, P, P, P, I, I, I, I, I, P],
     "xb_recurrence_chunk": [],
     "xb_recurrence_fwd": [P, I, P],
-    "xb_recurrence_bwd": [P, I, P],
+    "xb_recurrence_bwd": [P, I, I, P],
     "xb_dequant4": [P, P, P, P, L, I, I, P],
     "xb_quant4": [P, I, P, P, P, P, L, I, I, P],
     "xb_mirror_lower": [P, L, I, I, I, P],

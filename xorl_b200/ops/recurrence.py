@@ -27,6 +27,9 @@ CHUNK = 64              # tokens of a chunk of the kernels (csrc/recurrence.cu)
 SLICE = 32              # columns of the state in one operand tile
 TILE = 16384            # bytes of an operand tile of the state
 MAX_STATE_ROWS = 128
+# The states of all chunks are kept for the backward pass up to this size (4096 tokens of 32 heads of 128 x 128: 207 MB);
+# a longer call makes them again, which is the forward pass without its outputs once more.
+KEEP_BYTES = 1 << 30
 OPERANDS = 32768        # bytes of the operand tile that the delta rule prepares per chunk and head
 
 
@@ -63,6 +66,21 @@ def _pieces(sizes):
         out.append(at)
         at += (s + 255) // 256 * 256
     return out, at
+
+
+def _tiles(a: _Args, delta: bool):
+    """(field, bytes) of the operand tiles that the gradients read: one set from the forward pass, one from the backward."""
+    n = a.nc_max * a.Hv * (a.dvp // SLICE) * TILE
+    return [("s_tiles", n)] + ([("u_tiles", n // 2)] if delta else []), [("ds_tiles", n)] + (
+        [("dr_tiles", n // 2)] if delta else [("part", a.nc_max * a.Hv * 2 * 4)])
+
+
+def _place(a: _Args, fields, device) -> torch.Tensor:
+    offs, total = _pieces([n for _, n in fields])
+    buf = torch.empty(total, dtype=torch.uint8, device=device)
+    for (name, _), off in zip(fields, offs):
+        setattr(a, name, buf.data_ptr() + off)
+    return buf
 
 
 def _fill(a: _Args, q, k, v, g, b, A, D, cu, s_in, ws, keep: bool, delta: bool, scale: float, l2norm: bool) -> torch.Tensor:
@@ -111,15 +129,19 @@ class _Recurrence(torch.autograd.Function):
         T, Hv, dv = v.shape
         a = _Args()
         with _lib.on_device(q):
-            ws = _fill(a, q, k, v, g, b, A, D, cu, s_in, None, any(ctx.needs_input_grad), delta, scale, l2norm)
+            keep = any(ctx.needs_input_grad)
+            ws = _fill(a, q, k, v, g, b, A, D, cu, s_in, None, keep, delta, scale, l2norm)
             o = torch.empty((T, Hv, dv), dtype=v.dtype, device=v.device)
             shape = (cu.numel() - 1, Hv) + ((q.shape[2], dv) if delta else (dv, q.shape[2]))
             s_out = torch.empty(shape, dtype=torch.float32, device=v.device) if final else None
             a.o, a.s_out = o.data_ptr(), _lib.ptr(s_out)
+            tiles = None
+            if keep and sum(n for _, n in _tiles(a, delta)[0]) <= KEEP_BYTES:
+                tiles = _place(a, _tiles(a, delta)[0], v.device)
             _lib.check(_lib.cuda_lib().xb_recurrence_fwd(ctypes.byref(a), int(delta), _lib.stream_ptr()),
                        "xb_recurrence_fwd")
         _launches += 3
-        ctx.save_for_backward(q, k, v, g, b, A, D, s_in, cu, ws)
+        ctx.save_for_backward(q, k, v, g, b, A, D, s_in, cu, ws, tiles)
         ctx.conf = (delta, scale, l2norm)
         ctx.set_materialize_grads(False)
         return o, s_out
@@ -128,7 +150,7 @@ class _Recurrence(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy, ds_out):
         global _launches
-        q, k, v, g, b, A, D, s_in, cu, ws = ctx.saved_tensors
+        q, k, v, g, b, A, D, s_in, cu, ws, tiles = ctx.saved_tensors
         delta, scale, l2norm = ctx.conf
         T, Hk, dk = q.shape
         Hv, dv = v.shape[1], v.shape[2]
@@ -150,15 +172,17 @@ class _Recurrence(torch.autograd.Function):
             dD = None if delta else torch.empty(Hv, dtype=torch.float32, device=dev)
             a.dq, a.dk_out, a.dv_out, a.db = dq.data_ptr(), dkk.data_ptr(), dvv.data_ptr(), db.data_ptr()
             a.dg, a.dA, a.dD = _lib.ptr(dg), _lib.ptr(dA), _lib.ptr(dD)
-            tiles = a.nc_max * Hv * (a.dvp // SLICE)
-            offs, total = _pieces([tiles * TILE, tiles * TILE]
-                                  + ([tiles * TILE // 2, tiles * TILE // 2] if delta else [a.nc_max * Hv * 2 * 4]))
-            tmp = torch.empty(total, dtype=torch.uint8, device=dev)
-            for name, off in zip(("s_tiles", "ds_tiles") + (("u_tiles", "dr_tiles") if delta else ("part",)), offs):
-                setattr(a, name, tmp.data_ptr() + off)
-            _lib.check(_lib.cuda_lib().xb_recurrence_bwd(ctypes.byref(a), int(delta), _lib.stream_ptr()),
+            first, second = _tiles(a, delta)
+            if tiles is None:
+                tmp = _place(a, first + second, dev)
+            else:
+                tmp = _place(a, second, dev)
+                for (name, _), off in zip(first, _pieces([n for _, n in first])[0]):
+                    setattr(a, name, tiles.data_ptr() + off)
+            _lib.check(_lib.cuda_lib().xb_recurrence_bwd(ctypes.byref(a), int(delta), int(tiles is not None), _lib.stream_ptr()),
                        "xb_recurrence_bwd")
-        _launches += 3 if delta else 4
+        del tmp
+        _launches += (2 if delta else 3) + int(tiles is None)
         return dq, dkk, dvv, dg, db, dA, dD, ds_in, None, None, None, None, None
 
 
