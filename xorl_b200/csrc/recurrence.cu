@@ -26,6 +26,8 @@
 // significand: one bf16 value (9 bits) would cost the fp32 gradients of the decay three decimal digits.  Products of
 // two such sums leave out low x low.  Decays are sums in fp64 of log2 units, kept as two floats, so that differences
 // of large sums stay exact.  L2 norms of q and k are row factors and are applied behind the products.
+#include <type_traits>
+
 #include "recurrence_core.cuh"
 
 namespace {
@@ -118,7 +120,7 @@ __global__ void __launch_bounds__(128) rec_reduce(const XbRecArgs p) {
 
 bool bad_args(const XbRecArgs& a) {
   return a.T < 0 || a.n_docs < 0 || a.Hk <= 0 || a.Hv <= 0 || a.Hv % a.Hk || a.dk <= 0 || a.dk > 128 || a.dk % 8 || a.dv <= 0 ||
-         a.dv % 8 || a.dvp != (a.dv + 63) / 64 * 64 || a.dkp != (a.dk <= 64 ? 64 : 128) || a.nc_max < a.T / C + a.n_docs + 2;
+         a.dv % 8 || a.nc_max < a.T / C + a.n_docs + 2;
 }
 
 int plan(const XbRecArgs& a, cudaStream_t st) {
@@ -130,27 +132,41 @@ int plan(const XbRecArgs& a, cudaStream_t st) {
 
 XB_API int xb_recurrence_chunk() { return C; }
 
-XB_API int xb_recurrence_fwd(const XbRecArgs* args, int delta, void* stream) {
-  if (args == nullptr || bad_args(*args)) return -1;
-  XbRecArgs mine = *args, *a = &mine;
-  mine.status = xb_status_ptr();
+// The arguments as 64-bit words, in the order of XbRecArgs up to `part`, then T, n_docs, Hk, Hv, dk, dv, nc_max, l2norm.
+static XbRecArgs unpack(const long long* w, float scale) {
+  XbRecArgs a{};
+  auto ptr = [&](auto& f) { f = reinterpret_cast<std::remove_reference_t<decltype(f)>>(*w++); };
+  auto num = [&](auto& f) { f = static_cast<std::remove_reference_t<decltype(f)>>(*w++); };
+  ptr(a.q), ptr(a.k), ptr(a.v), ptr(a.dy);
+  num(a.q_t), num(a.q_h), num(a.k_t), num(a.k_h), num(a.v_t), num(a.v_h), num(a.dy_t), num(a.dy_h);
+  ptr(a.g), ptr(a.b), num(a.g_t), num(a.g_h), num(a.b_t), num(a.b_h);
+  ptr(a.A), ptr(a.D), ptr(a.cu), ptr(a.s_in), ptr(a.s_out), ptr(a.ds_out), ptr(a.ds_in), num(a.s_k), num(a.s_v);
+  ptr(a.o), ptr(a.dq), ptr(a.dk_out), ptr(a.dv_out), ptr(a.dg), ptr(a.db), ptr(a.dA), ptr(a.dD);
+  ptr(a.chunks), ptr(a.doc_off), ptr(a.hd), ptr(a.rqk), ptr(a.qk), ptr(a.kk), ptr(a.pt);
+  ptr(a.s_tiles), ptr(a.u_tiles), ptr(a.ds_tiles), ptr(a.dr_tiles), ptr(a.part);
+  num(a.T), num(a.n_docs), num(a.Hk), num(a.Hv), num(a.dk), num(a.dv), num(a.nc_max), num(a.l2norm);
+  a.dkp = a.dk <= 64 ? 64 : 128, a.dvp = (a.dv + 63) / 64 * 64;
+  a.scale = scale;
+  a.status = xb_status_ptr();
+  return a;
+}
+
+XB_API int xb_recurrence_fwd(const long long* words, float scale, int delta, void* stream) {
+  if (words == nullptr) return -1;
+  const XbRecArgs a = unpack(words, scale);
+  if (bad_args(a)) return -1;
   cudaStream_t st = (cudaStream_t)stream;
-  if (int rc = plan(*a, st)) return rc;
-  if (delta) return xb_delta_fwd(*a, st);
-  return xb_scan_fwd(*a, st);
+  if (int rc = plan(a, st)) return rc;
+  return delta ? xb_delta_fwd(a, st) : xb_scan_fwd(a, st);
 }
 
 // tiles: the forward pass has left its tiles in s_tiles (and u_tiles); else they are made again.
-XB_API int xb_recurrence_bwd(const XbRecArgs* args, int delta, int tiles, void* stream) {
-  if (args == nullptr || bad_args(*args)) return -1;
-  XbRecArgs mine = *args, *a = &mine;
-  mine.status = xb_status_ptr();
+XB_API int xb_recurrence_bwd(const long long* words, float scale, int delta, int tiles, void* stream) {
+  if (words == nullptr) return -1;
+  const XbRecArgs a = unpack(words, scale);
+  if (bad_args(a)) return -1;
   cudaStream_t st = (cudaStream_t)stream;
-  if (delta) {
-    if (int rc = xb_delta_bwd(*a, tiles, st)) return rc;
-    return xb_recurrence_grad(*a, 1, st);
-  }
-  if (int rc = xb_scan_bwd(*a, tiles, st)) return rc;
-  if (int rc = xb_recurrence_grad(*a, 0, st)) return rc;
-  return rec_launch(rec_reduce, a->Hv, 128, 0, *a, st);
+  if (int rc = delta ? xb_delta_bwd(a, tiles, st) : xb_scan_bwd(a, tiles, st)) return rc;
+  if (int rc = xb_recurrence_grad(a, delta, st)) return rc;
+  return delta ? 0 : rec_launch(rec_reduce, a.Hv, 128, 0, a, st);
 }

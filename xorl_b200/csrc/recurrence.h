@@ -1,4 +1,4 @@
-// Arguments of the gated linear recurrences (recurrence.cu).  Plain data; the Python side mirrors the order.
+// Arguments of the gated linear recurrences, as the kernels get them (recurrence.cu unpacks them).
 #pragma once
 
 struct XbRecArgs {
@@ -29,7 +29,7 @@ struct XbRecArgs {
   void* pt;                      // [nc_max, Hv]: operand tile [T; P T], two planes, 32768 bytes (delta rule only)
   // operand tiles of [rows][hi 32 | lo 32] bf16, [nc_max, Hv, dvp / 32]: states entering and gradients of those leaving
   // the chunks (16 KB), U and dR (8 KB, delta rule only)
-  void *s_tiles, *ds_tiles, *u_tiles, *dr_tiles;
+  void *s_tiles, *u_tiles, *ds_tiles, *dr_tiles;
   float* part;                   // [nc_max, Hv, 2] (scan only)
   int* status;                   // filled in by the entry points
   int T, n_docs, Hk, Hv, dk, dv, dkp, dvp, nc_max, l2norm;   // dkp: 64 or 128, dvp: a multiple of 64

@@ -166,14 +166,23 @@ inline int rec_tile_map(CUtensorMap* m, const void* base, int T, int heads, int 
   return xb_make_tmap_3d(m, base, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, T, heads, cols, T > 1 ? ld_t : 8, heads > 1 ? ld_h : 8, C, 1, box, swz);
 }
 
+// Dynamic shared memory above 48 KB, once per kernel and device.
+template <auto KERNEL>
+bool rec_configure(int smem) {
+  static bool done[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (done[dev & 63]) return true;
+  if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+    cudaGetLastError();
+    return false;
+  }
+  return done[dev & 63] = true;
+}
 template <typename K>
 int rec_launch(K kernel, long long blocks, int threads, size_t smem, const XbRecArgs& a, cudaStream_t st) {
   if (blocks <= 0) return 0;
   if (blocks > 0x7fffffffLL) return -4;
-  if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
-    cudaGetLastError();
-    return -5;
-  }
   kernel<<<(unsigned)blocks, threads, smem, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? 0 : -11;
 }

@@ -277,9 +277,14 @@ __global__ void __launch_bounds__(128, 3) delta_prep(const XbRecArgs p) {
 constexpr int ST_KQ = 0, ST_TP = 2 * HALF, ST_X = ST_TP + 2 * TP_PLANE, ST_HD = ST_X + C * NV * 2, ST_RQK = ST_HD + HD * 4;
 constexpr int STAGE = (ST_RQK + RQK * 4 + 1023) / 1024 * 1024;
 constexpr int STAGE_BYTES = ST_RQK + RQK * 4;      // what the loads bring, boxes outside a tensor included
-constexpr int SM_S = 2 * STAGE, SM_B2 = SM_S + HALF, SM_B3 = SM_B2 + HALF, SM_U = SM_B3 + HALF,
-              SM_BAR = SM_U + HALF / 2;
-constexpr int SMEM = SM_BAR + 128 + 1024;
+// Shared memory.  Backward: two stages, operand tiles of 128 rows.  Forward: tiles of 64 rows; two stages, or one and two
+// CTAs per SM.
+template <bool BWD, int STAGES>
+struct Lay {
+  static constexpr int ROWS = BWD ? HALF : HALF / 2;
+  static constexpr int SM_S = STAGES * STAGE, SM_B2 = SM_S + HALF, SM_B3 = SM_B2 + ROWS, SM_U = SM_B3 + ROWS, SM_BAR = SM_U + HALF / 2;
+  static constexpr int SMEM = SM_BAR + 128 + 1024;
+};
 constexpr int WORKERS = 256, THREADS = WORKERS + 32;
 constexpr int TMEM_COLS = 256, D1 = 0, D2 = 64, D3 = 128;     // accumulators, 64 columns each
 
@@ -296,6 +301,7 @@ struct Cta {
   Bars* bars;
   uint32_t tmem;
   int h, kh, doc, v0, vcols, c0, c1;
+  int sm_s, sm_u;
   int* status;
   __device__ void wait1(uint64_t* b, uint32_t parity, int detail) {         // one thread
     mbar_wait(b, parity, &bars->abort_flag, status, XB_K_RECURRENCE, detail);
@@ -326,8 +332,8 @@ __device__ __forceinline__ void load_stage(const XbRecArgs& p, const Cta& a, con
 // The state tile of chunk `cs` and the 64-row tile of chunk `cu` to global memory, as they are (-1: none).
 __device__ __forceinline__ void keep_tiles(const XbRecArgs& p, const Cta& a, void* states, void* rows, int cs, int cu) {
   const int slices = p.dvp / NV, sl = a.v0 / NV;
-  if (cs >= 0) bulk_store((uint8_t*)states + (((long long)cs * p.Hv + a.h) * slices + sl) * HALF, a.smem + SM_S, HALF);
-  if (cu >= 0) bulk_store((uint8_t*)rows + (((long long)cu * p.Hv + a.h) * slices + sl) * (HALF / 2), a.smem + SM_U, HALF / 2);
+  if (cs >= 0) bulk_store((uint8_t*)states + (((long long)cs * p.Hv + a.h) * slices + sl) * HALF, a.smem + a.sm_s, HALF);
+  if (cu >= 0) bulk_store((uint8_t*)rows + (((long long)cu * p.Hv + a.h) * slices + sl) * (HALF / 2), a.smem + a.sm_u, HALF / 2);
   tma_store_commit();
 }
 
@@ -384,6 +390,19 @@ __device__ __forceinline__ void floats(const uint4 (&v)[2], float (&x)[16]) {
 }
 // 16 fp32 values of a state row in global memory
 __device__ __forceinline__ void state_row(float* base, long long sk, long long sv, int row, int dk, int col, int cols, bool store, float (&s)[16]) {
+  if (sv == 1 && row < dk && col + 16 <= cols) {                     // rows of a multiple of 8 values
+    float4* at = reinterpret_cast<float4*>(base + row * sk + col);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (store) {
+        at[i] = make_float4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
+      } else {
+        const float4 v = at[i];
+        s[4 * i] = v.x, s[4 * i + 1] = v.y, s[4 * i + 2] = v.z, s[4 * i + 3] = v.w;
+      }
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     float* at = base + row * sk + (col + i) * sv;
@@ -398,10 +417,11 @@ __device__ __forceinline__ void state_row(float* base, long long sk, long long s
 
 constexpr uint64_t KMAJ = xb_smem_desc_base_sw128(16, 1024), MNMAJ = xb_smem_desc_base_sw128(HALF, 1024);
 
-__device__ __forceinline__ bool cta_setup(const XbRecArgs& p, Cta& a, uint8_t* raw) {
+__device__ __forceinline__ bool cta_setup(const XbRecArgs& p, Cta& a, uint8_t* raw, int sm_s, int sm_u, int sm_bar) {
   const int slices = p.dvp / NV, rep = p.Hv / p.Hk;
   a.smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-  a.bars = reinterpret_cast<Bars*>(a.smem + SM_BAR);
+  a.bars = reinterpret_cast<Bars*>(a.smem + sm_bar);
+  a.sm_s = sm_s, a.sm_u = sm_u;
   const int sl = blockIdx.x % slices;
   a.h = (blockIdx.x / slices) % p.Hv, a.doc = blockIdx.x / (slices * p.Hv), a.kh = a.h / rep;
   a.v0 = sl * NV, a.vcols = min(NV, p.dv - a.v0);
@@ -450,13 +470,14 @@ __device__ __forceinline__ void zero_rows(const XbRecArgs& p, const Cta& a, bf16
 // is left with a thread missing.
 
 // OUT: outputs are wanted.  SAVE: the tiles of the states and of U go to global memory.
-template <bool OUT, bool SAVE>
-__global__ void __launch_bounds__(THREADS, 1)
+template <bool OUT, bool SAVE, int STAGES>
+__global__ void __launch_bounds__(THREADS, 3 - STAGES)
 delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mv,
           const __grid_constant__ XbRecArgs p) {
+  using L = Lay<false, STAGES>;
   extern __shared__ uint8_t smem_raw[];
   Cta a;
-  const bool inside = cta_setup(p, a, smem_raw);
+  const bool inside = cta_setup(p, a, smem_raw, L::SM_S, L::SM_U, L::SM_BAR);
   bf16* o = (bf16*)p.o + (long long)a.h * p.dv + a.v0;
   const long long o_t = (long long)p.Hv * p.dv;
   if (!inside) {
@@ -467,14 +488,14 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == WORKERS / 32) {
     const bool one = lane == 0;
-    if (one && a.c0 < a.c1) load_stage(p, a, &mk, &mq, &mv, a.c0, 0);
-    if (one && a.c0 + 1 < a.c1) load_stage(p, a, &mk, &mq, &mv, a.c0 + 1, 1);
+    for (int n = 0; n < STAGES; ++n)
+      if (one && a.c0 + n < a.c1) load_stage(p, a, &mk, &mq, &mv, a.c0 + n, n);
     for (int n = 0; n < a.c1 - a.c0; ++n) {
-      const uint32_t st = xb_smem_u32(a.smem + (n & 1) * STAGE), b1 = xb_smem_u32(a.smem + SM_S), b2 = xb_smem_u32(a.smem + SM_B2),
-                     b3 = xb_smem_u32(a.smem + SM_B3);
+      const uint32_t st = xb_smem_u32(a.smem + (n % STAGES) * STAGE), b1 = xb_smem_u32(a.smem + L::SM_S), b2 = xb_smem_u32(a.smem + L::SM_B2),
+                     b3 = xb_smem_u32(a.smem + L::SM_B3);
       bar(1, THREADS);
       if (one) {
-        a.wait1(&a.bars->full[n & 1], (n >> 1) & 1, 1);
+        a.wait1(&a.bars->full[n % STAGES], (n / STAGES) & 1, 1);
         tc_fence_after();
         constexpr uint32_t id = xb_idesc(1, 1, 128, 64, 0, 1);
 #pragma unroll
@@ -501,9 +522,9 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
         for (int k = 0; k < 4; ++k)
           tc_mma_f16_ss(a.tmem + D3, xb_smem_desc(MNMAJ, st + ST_KQ + k * 2048), xb_smem_desc(MNMAJ, b3 + k * 2048), id, k > 0);
         tc_commit(&a.bars->done[2]);
-        if (n + 2 < a.c1 - a.c0) {           // the stage is free when the last product has read it
+        if (n + STAGES < a.c1 - a.c0) {           // the stage is free when the last product has read it
           a.wait1(&a.bars->done[2], n & 1, 2);
-          load_stage(p, a, &mk, &mq, &mv, a.c0 + n + 2, n & 1);
+          load_stage(p, a, &mk, &mq, &mv, a.c0 + n + STAGES, n % STAGES);
         }
       }
       __syncwarp();
@@ -526,11 +547,11 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
     for (int n = 0; n < a.c1 - a.c0; ++n) {
       const int c = a.c0 + n, len = reinterpret_cast<const int4*>(p.chunks)[c].y;
       const long long t0 = reinterpret_cast<const int4*>(p.chunks)[c].x;
-      uint8_t* st = a.smem + (n & 1) * STAGE;
+      uint8_t* st = a.smem + (n % STAGES) * STAGE;
       const float* hd = reinterpret_cast<const float*>(st + ST_HD);
       const float* rqk = reinterpret_cast<const float*>(st + ST_RQK);
-      put_row(a.smem + SM_S, r, half, s, hi, lo);
-      a.wait(&a.bars->full[n & 1], (n >> 1) & 1, 3);
+      put_row(a.smem + L::SM_S, r, half, s, hi, lo);
+      a.wait(&a.bars->full[n % STAGES], (n / STAGES) & 1, 3);
       if (len < C) clear_rows(st, len);
       fence_proxy_async_smem();
       tc_fence_before();
@@ -549,7 +570,7 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
         const float f = gam * rk;
 #pragma unroll
         for (int e = 0; e < 16; ++e) x[e] = b * (x[e] - f * y[e]);
-        put_row(a.smem + SM_B2, i, half, x, hi, lo);
+        put_row(a.smem + L::SM_B2, i, half, x, hi, lo);
       }
       fence_proxy_async_smem();
       tc_fence_before();
@@ -558,11 +579,11 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       tc_fence_after();
       read_acc(acc + D2, x);
       if (krow) {                            // d rk U
-        if (SAVE) put_row(a.smem + SM_U, i, half, x, hi, lo);
+        if (SAVE) put_row(a.smem + L::SM_U, i, half, x, hi, lo);
         const float f = dec * rk;
 #pragma unroll
         for (int e = 0; e < 16; ++e) x[e] *= f;
-        put_row(a.smem + SM_B3, i, half, x, hi, lo);
+        put_row(a.smem + L::SM_B3, i, half, x, hi, lo);
       }
       fence_proxy_async_smem();
       tc_fence_before();
@@ -595,9 +616,10 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
 __global__ void __launch_bounds__(THREADS, 1)
 delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap my,
           const __grid_constant__ XbRecArgs p) {
+  using L = Lay<true, 2>;
   extern __shared__ uint8_t smem_raw[];
   Cta a;
-  const bool inside = cta_setup(p, a, smem_raw);
+  const bool inside = cta_setup(p, a, smem_raw, L::SM_S, L::SM_U, L::SM_BAR);
   bf16* dv = (bf16*)p.dv_out + (long long)a.h * p.dv + a.v0;
   const long long dv_t = (long long)p.Hv * p.dv;
   if (!inside) {
@@ -611,8 +633,8 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
     if (one && steps > 0) load_stage(p, a, &mk, &mq, &my, a.c1 - 1, 0);
     if (one && steps > 1) load_stage(p, a, &mk, &mq, &my, a.c1 - 2, 1);
     for (int n = 0; n < steps; ++n) {
-      const uint32_t st = xb_smem_u32(a.smem + (n & 1) * STAGE), b1 = xb_smem_u32(a.smem + SM_S), b2 = xb_smem_u32(a.smem + SM_B2),
-                     b3 = xb_smem_u32(a.smem + SM_B3);
+      const uint32_t st = xb_smem_u32(a.smem + (n & 1) * STAGE), b1 = xb_smem_u32(a.smem + L::SM_S), b2 = xb_smem_u32(a.smem + L::SM_B2),
+                     b3 = xb_smem_u32(a.smem + L::SM_B3);
       constexpr uint32_t id3 = xb_idesc(1, 1, 128, 64, 1, 1);
       bar(1, THREADS);
       if (one) {
@@ -677,19 +699,19 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       if (krow) return;
       uint4 v[2];
       read_x(st + ST_X, i, half, i < len, v);
-      uint8_t* row = a.smem + SM_B2 + r * 128;
+      uint8_t* row = a.smem + L::SM_B2 + r * 128;
 #pragma unroll
       for (int e = 0; e < 2; ++e) *reinterpret_cast<uint4*>(row + (((half * 2 + e) ^ (r & 7)) << 4)) = v[e];
       const float f = ex2_sum(reinterpret_cast<const float*>(st + ST_HD), i) * reinterpret_cast<const float*>(st + ST_RQK)[i];
       floats(v, x);
 #pragma unroll
       for (int e = 0; e < 16; ++e) x[e] *= f;
-      put_row(a.smem + SM_B3, r, half, x, hi, lo);
+      put_row(a.smem + L::SM_B3, r, half, x, hi, lo);
     };
     if (!krow)
 #pragma unroll
       for (int e = 0; e < 2; ++e)
-        *reinterpret_cast<uint4*>(a.smem + SM_B2 + r * 128 + (((4 + half * 2 + e) ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(a.smem + L::SM_B2 + r * 128 + (((4 + half * 2 + e) ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
     if (steps > 0) put_dy(0);
     for (int n = 0; n < steps; ++n) {
       const int c = a.c1 - 1 - n, len = reinterpret_cast<const int4*>(p.chunks)[c].y;
@@ -697,7 +719,7 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       uint8_t* st = a.smem + (n & 1) * STAGE;
       const float* hd = reinterpret_cast<const float*>(st + ST_HD);
       const float* rqk = reinterpret_cast<const float*>(st + ST_RQK);
-      put_row(a.smem + SM_S, r, half, s, hi, lo);
+      put_row(a.smem + L::SM_S, r, half, s, hi, lo);
       fence_proxy_async_smem();
       tc_fence_before();
       bar_arrive(1, THREADS);
@@ -709,7 +731,7 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
         read_acc(acc + D1, x);
 #pragma unroll
         for (int e = 0; e < 16; ++e) x[e] *= f1;
-        put_row(a.smem + SM_B2, i, half, x, hi, lo);
+        put_row(a.smem + L::SM_B2, i, half, x, hi, lo);
       }
       fence_proxy_async_smem();
       tc_fence_before();
@@ -721,13 +743,13 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       if (lane < 16) {                       // -b gamma rk dR
 #pragma unroll
         for (int e = 0; e < 16; ++e) x[e] = f2 * dr[e];
-        put_row(a.smem + SM_B3, ri, half, x, hi, lo);
+        put_row(a.smem + L::SM_B3, ri, half, x, hi, lo);
       }
       fence_proxy_async_smem();
       tc_fence_before();
       bar_arrive(3, THREADS);
       if (lane < 16) {
-        put_row(a.smem + SM_U, ri, half, dr, hi, lo);
+        put_row(a.smem + L::SM_U, ri, half, dr, hi, lo);
         if (ri < len) {
           bf16* dst = dv + (t0 + ri) * dv_t + half * 16;
 #pragma unroll
@@ -753,8 +775,8 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
   cta_end(a);
 }
 
-template <typename K>
-int run(K kernel, const XbRecArgs& a, const void* x, long long x_t, long long x_h, cudaStream_t st) {
+template <auto KERNEL, int SMEM>
+int run(const XbRecArgs& a, const void* x, long long x_t, long long x_h, cudaStream_t st) {
   const long long blocks = (long long)(a.n_docs + 2) * a.Hv * (a.dvp / NV);
   if (blocks > 0x7fffffffLL) return -4;
   CUtensorMap mk{}, mq{}, mx{};
@@ -762,16 +784,14 @@ int run(K kernel, const XbRecArgs& a, const void* x, long long x_t, long long x_
                   rec_tile_map(&mq, a.q, a.T, a.Hk, a.dk, a.q_t, a.q_h, 64, CU_TENSOR_MAP_SWIZZLE_128B) ||
                   rec_tile_map(&mx, x, a.T, a.Hv, a.dv, x_t, x_h, NV, CU_TENSOR_MAP_SWIZZLE_64B)))
     return -2;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess) {
-    cudaGetLastError();
-    return -5;
-  }
-  kernel<<<(unsigned)blocks, THREADS, SMEM, st>>>(mk, mq, mx, a);
+  if (!rec_configure<KERNEL>(SMEM)) return -5;
+  KERNEL<<<(unsigned)blocks, THREADS, SMEM, st>>>(mk, mq, mx, a);
   return cudaGetLastError() == cudaSuccess ? 0 : -11;
 }
 
 template <int DKP>
 int prep(const XbRecArgs& a, cudaStream_t st) {
+  if (!rec_configure<delta_prep<DKP>>(sizeof(DPrepSmem<DKP>))) return -5;
   return rec_launch(delta_prep<DKP>, (long long)a.nc_max * a.Hk, 128, sizeof(DPrepSmem<DKP>), a, st);
 }
 
@@ -779,13 +799,17 @@ int prep(const XbRecArgs& a, cudaStream_t st) {
 
 int xb_delta_fwd(const XbRecArgs& a, cudaStream_t st) {
   if (int rc = a.dk <= 64 ? prep<64>(a, st) : prep<128>(a, st)) return rc;
-  return a.s_tiles != nullptr ? run(delta_fwd<true, true>, a, a.v, a.v_t, a.v_h, st) : run(delta_fwd<true, false>, a, a.v, a.v_t, a.v_h, st);
+  if (a.s_tiles != nullptr) return run<delta_fwd<true, true, 2>, Lay<false, 2>::SMEM>(a, a.v, a.v_t, a.v_h, st);
+  // Documents of one chunk on average spend their time on the way in and out: two CTAs per SM, one stage each (48
+  // documents of 2 tokens, 32 heads of 128 x 128: SHORT_US).  Longer ones want the next chunk's loads ahead of them.
+  if ((long long)a.n_docs * C >= a.T) return run<delta_fwd<true, false, 1>, Lay<false, 1>::SMEM>(a, a.v, a.v_t, a.v_h, st);
+  return run<delta_fwd<true, false, 2>, Lay<false, 2>::SMEM>(a, a.v, a.v_t, a.v_h, st);
 }
 int xb_delta_bwd(const XbRecArgs& a, int tiles, cudaStream_t st) {
   if (!tiles) {
     XbRecArgs again = a;
     again.s_out = nullptr;
-    if (int rc = run(delta_fwd<false, true>, again, a.v, a.v_t, a.v_h, st)) return rc;
+    if (int rc = run<delta_fwd<false, true, 2>, Lay<false, 2>::SMEM>(again, a.v, a.v_t, a.v_h, st)) return rc;
   }
-  return run(delta_bwd, a, a.dy, a.dy_t, a.dy_h, st);
+  return run<delta_bwd, Lay<true, 2>::SMEM>(a, a.dy, a.dy_t, a.dy_h, st);
 }

@@ -563,10 +563,7 @@ int run(const XbRecArgs& a, cudaStream_t st) {
                   rec_tile_map(&mv, a.v, a.T, a.Hv, a.dv, a.v_t, a.v_h, 64, CU_TENSOR_MAP_SWIZZLE_128B) ||
                   rec_tile_map(&my, a.dy, a.T, a.Hv, a.dv, a.dy_t, a.dy_h, 64, CU_TENSOR_MAP_SWIZZLE_128B)))
     return -2;
-  if (cudaFuncSetAttribute(rec_grad<DELTA>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<DELTA>()) != cudaSuccess) {
-    cudaGetLastError();
-    return -5;
-  }
+  if (!rec_configure<rec_grad<DELTA>>(smem_bytes<DELTA>())) return -5;
   rec_grad<DELTA><<<(unsigned)blocks, THREADS, smem_bytes<DELTA>(), st>>>(mq, mk, mv, my, a);
   return cudaGetLastError() == cudaSuccess ? 0 : -11;
 }

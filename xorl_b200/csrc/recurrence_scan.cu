@@ -416,10 +416,7 @@ int run(const XbRecArgs& a, const void* x, long long x_t, long long x_h, cudaStr
                   rec_tile_map(&mx, x, a.T, a.Hv, a.dv, x_t, x_h, 64, CU_TENSOR_MAP_SWIZZLE_128B) ||
                   xb_make_tmap_2d(&mqk, a.qk, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, (uint64_t)a.nc_max * a.Hk * C, C, C, C, 32, CU_TENSOR_MAP_SWIZZLE_128B)))
     return -2;
-  if (cudaFuncSetAttribute(scan_seq<BWD, OUT, KEEP>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess) {
-    cudaGetLastError();
-    return -5;
-  }
+  if (!rec_configure<scan_seq<BWD, OUT, KEEP>>(SMEM)) return -5;
   scan_seq<BWD, OUT, KEEP><<<(unsigned)blocks, THREADS, SMEM, st>>>(mk, mq, mx, mqk, a);
   return cudaGetLastError() == cudaSuccess ? 0 : -11;
 }

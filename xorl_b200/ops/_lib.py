@@ -7,7 +7,6 @@ loaded, so no operator can silently fall back to a PyTorch implementation there.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 import threading
@@ -117,8 +116,8 @@ _SIGNATURES = {
     "xb_gated_norm_fwd": [P, L, P, L, P, I, I, P, P, I, I, I, F, I, P],
     "xb_gated_norm_bwd": [P, L, P, L, P, L, P, I, I, P, P, P, P, P, I, I, I, I, I, P],
     "xb_recurrence_chunk": [],
-    "xb_recurrence_fwd": [P, I, P],
-    "xb_recurrence_bwd": [P, I, I, P],
+    "xb_recurrence_fwd": [P, F, I, P],
+    "xb_recurrence_bwd": [P, F, I, I, P],
     "xb_dequant4": [P, P, P, P, L, I, I, P],
     "xb_quant4": [P, I, P, P, P, P, L, I, I, P],
     "xb_mirror_lower": [P, L, I, I, I, P],
@@ -181,11 +180,17 @@ def stream_ptr() -> int:
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
-def on_device(t: torch.Tensor):
-    """Makes the tensor's device the current one for a launch whose caller has another one selected."""
-    if t.device.index != torch._C._cuda_getDevice():
-        return torch.cuda.device(t.device)
-    return contextlib.nullcontext()
+def call_on(device: torch.device, name: str, *args) -> None:
+    """Calls an entry point of the kernel library with the current stream of ``device``, which need not be the current
+    device, as its last argument."""
+    fn = getattr(cuda_lib(), name)
+    if device.index == torch._C._cuda_getDevice():
+        rc = fn(*args, stream_ptr())
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, stream_ptr())
+    if rc != 0:
+        check(rc, name)
 
 
 def current_stream() -> torch.cuda.Stream:

@@ -136,49 +136,46 @@ class _GatedRMSNorm(torch.autograd.Function):
         global _launches
         shape = x.shape
         W = shape[-1]
-        x2, z2 = _norm_rows(x.reshape(-1, W)), _norm_rows(gate.reshape(-1, W))
-        wc = w.detach().contiguous()
-        T, groups = x2.shape[0], W // group_size
-        y = torch.empty((T, W), dtype=x.dtype, device=x.device)
-        keep = any(ctx.needs_input_grad)
-        rstd = torch.empty((T, groups), dtype=torch.float32, device=x.device) if keep else None
-        with _lib.on_device(x):
-            _lib.check(_lib.cuda_lib().xb_gated_norm_fwd(
-                x2.data_ptr(), x2.stride(0), z2.data_ptr(), z2.stride(0), wc.data_ptr(),
-                int(w.dtype == torch.float32), int(w.numel() == group_size), y.data_ptr(), _lib.ptr(rstd), T, groups,
-                group_size, float(eps), int(norm_first), _lib.stream_ptr()), "xb_gated_norm_fwd")
+        x2, z2 = (x, gate) if x.dim() == 2 else (x.reshape(-1, W), gate.reshape(-1, W))
+        x2, z2 = _norm_rows(x2), _norm_rows(z2)
+        wc = w if w.is_contiguous() else w.contiguous()
+        T, groups, dev = x2.shape[0], W // group_size, x.device
+        y = torch.empty((T, W), dtype=x.dtype, device=dev)
+        rstd = torch.empty((T, groups), dtype=torch.float32, device=dev) if True in ctx.needs_input_grad else None
+        shared, wide = int(w.numel() == group_size), int(w.dtype == torch.float32)
+        _lib.call_on(dev, "xb_gated_norm_fwd", x2.data_ptr(), x2.stride(0), z2.data_ptr(), z2.stride(0), wc.data_ptr(), wide,
+                     shared, y.data_ptr(), _lib.ptr(rstd), T, groups, group_size, eps, norm_first)
         _launches += 1
         ctx.save_for_backward(x2, z2, wc, rstd)
-        ctx.w, ctx.conf, ctx.shape = w, (group_size, norm_first), shape
-        return y.reshape(shape)
+        ctx.w, ctx.conf = w, (group_size, norm_first, shape, groups, shared, wide)
+        return y if len(shape) == 2 else y.reshape(shape)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         global _launches
         x, z, wc, rstd = ctx.saved_tensors
-        group_size, norm_first = ctx.conf
+        group_size, norm_first, shape, groups, shared, wide = ctx.conf
         T, W = x.shape
-        groups = W // group_size
-        lib = _lib.cuda_lib()
-        want = ctx.needs_input_grad[2]
-        with _lib.on_device(x):
-            dy = _norm_rows(dy.reshape(T, W))
-            dx, dz = torch.empty((T, W), dtype=x.dtype, device=x.device), torch.empty((T, W), dtype=x.dtype, device=x.device)
-            part = dw = None
-            shared = int(wc.numel() == group_size)
-            if want:
-                part = torch.empty(max(lib.xb_gated_norm_partial(T, groups, group_size, shared), 1), dtype=torch.float32,
-                                   device=x.device)
-                # an engine's buffer takes fp32 sums; a gradient that autograd gets is rounded where it is summed
-                dw = torch.empty(wc.shape, dtype=wc.dtype if grad_target(ctx.w)[0] is None else torch.float32, device=x.device)
-            _lib.check(lib.xb_gated_norm_bwd(
-                dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), z.data_ptr(), z.stride(0), wc.data_ptr(),
-                int(wc.dtype == torch.float32), shared, rstd.data_ptr(), dx.data_ptr(), dz.data_ptr(), _lib.ptr(part),
-                _lib.ptr(dw), int(want and dw.dtype == torch.float32), T, groups, group_size, int(norm_first),
-                _lib.stream_ptr()), "xb_gated_norm_bwd")
+        dev = x.device
+        dy = _norm_rows(dy if dy.dim() == 2 else dy.reshape(T, W))
+        dx, dz = torch.empty((T, W), dtype=x.dtype, device=dev), torch.empty((T, W), dtype=x.dtype, device=dev)
+        part = dw = None
+        want, out_wide = ctx.needs_input_grad[2], 0
+        if want:
+            floats = _lib.cuda_lib().xb_gated_norm_partial(T, groups, group_size, shared)
+            part = torch.empty(max(floats, 1), dtype=torch.float32, device=dev)
+            # an engine's buffer takes fp32 sums; a gradient that autograd gets is rounded where it is summed
+            sink = grad_target(ctx.w)[0] is not None
+            dw = torch.empty(wc.shape, dtype=torch.float32 if sink else wc.dtype, device=dev)
+            out_wide = int(sink or wide)
+        _lib.call_on(dev, "xb_gated_norm_bwd", dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), z.data_ptr(), z.stride(0),
+                     wc.data_ptr(), wide, shared, rstd.data_ptr(), dx.data_ptr(), dz.data_ptr(), _lib.ptr(part), _lib.ptr(dw),
+                     out_wide, T, groups, group_size, norm_first)
         _launches += 1 + int(want)
-        return dx.reshape(ctx.shape), dz.reshape(ctx.shape), deliver_param_grad(ctx.w, dw) if want else None, None, None, None
+        if len(shape) != 2:
+            dx, dz = dx.reshape(shape), dz.reshape(shape)
+        return dx, dz, deliver_param_grad(ctx.w, dw) if want else None, None, None, None
 
 
 GATED_NORM_MAX_GROUP = 8192
@@ -205,4 +202,4 @@ def gated_rms_norm(x: torch.Tensor, gate: torch.Tensor, weight: torch.Tensor, gr
             or weight.dtype not in (torch.bfloat16, torch.float32) or group_size > GATED_NORM_MAX_GROUP
             or W // group_size > 65535):
         return _gated_rms_norm_ref(x, gate, weight, group_size, eps, norm_first)
-    return _lib.apply(_GatedRMSNorm, x, gate, weight, int(group_size), float(eps), bool(norm_first))
+    return _lib.apply(_GatedRMSNorm, x, gate, weight, group_size, eps, bool(norm_first))

@@ -14,6 +14,7 @@ others.  A call allocates its workspace; it does not synchronise and may be capt
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional
 
 import torch
@@ -24,7 +25,6 @@ from . import _lib
 _launches = 0
 
 CHUNK = 64              # tokens of a chunk of the kernels (csrc/recurrence.cu)
-SLICE = 32              # columns of the state in one operand tile
 TILE = 16384            # bytes of an operand tile of the state
 MAX_STATE_ROWS = 128
 # The states of all chunks are kept for the backward pass up to this size (4096 tokens of 32 heads of 128 x 128: 207 MB);
@@ -37,86 +37,66 @@ def launch_count() -> int:
     return _launches
 
 
-class _Args(ctypes.Structure):
-    """``XbRecArgs`` of csrc/recurrence.h."""
-    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "dy")]
-                + [(n, ctypes.c_longlong) for n in ("q_t", "q_h", "k_t", "k_h", "v_t", "v_h", "dy_t", "dy_h")]
-                + [(n, ctypes.c_void_p) for n in ("g", "b")]
-                + [(n, ctypes.c_longlong) for n in ("g_t", "g_h", "b_t", "b_h")]
-                + [(n, ctypes.c_void_p) for n in ("A", "D", "cu", "s_in", "s_out", "ds_out", "ds_in")]
-                + [(n, ctypes.c_longlong) for n in ("s_k", "s_v")]
-                + [(n, ctypes.c_void_p) for n in ("o", "dq", "dk_out", "dv_out", "dg", "db", "dA", "dD", "chunks",
-                                                  "doc_off", "hd", "rqk", "qk", "kk", "pt", "s_tiles", "ds_tiles",
-                                                  "u_tiles", "dr_tiles", "part", "status")]
-                + [(n, ctypes.c_int) for n in ("T", "n_docs", "Hk", "Hv", "dk", "dv", "dkp", "dvp", "nc_max", "l2norm")]
-                + [("scale", ctypes.c_float)])
+_Words = ctypes.c_longlong * 55      # the fields of XbRecArgs (csrc/recurrence.cu)
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """``x`` [T, heads, dim] as the kernels read it: itself, or a copy where its strides do not suit 16-byte loads."""
-    if x.stride(2) != 1 or x.stride(0) % 8 or x.stride(1) % 8 or x.stride(0) <= 0 or x.stride(1) <= 0 or x.data_ptr() % 16:
-        return x.contiguous() if not x.is_contiguous() else x.clone()
+    t, h, d = x.stride()
+    if d != 1 or t % 8 or h % 8 or t <= 0 or h <= 0 or x.data_ptr() % 16:
+        return x.clone(memory_format=torch.contiguous_format)
     return x
 
 
-def _pieces(sizes):
-    """Byte offsets of buffers of ``sizes`` in one allocation, and its size."""
-    at, out = 0, []
-    for s in sizes:
-        out.append(at)
-        at += (s + 255) // 256 * 256
-    return out, at
+@functools.lru_cache(maxsize=256)
+def _layout(T: int, docs: int, Hk: int, Hv: int, dk: int, dv: int, delta: bool, train: bool):
+    """Where the workspaces of a call of these sizes lie: (chunks, bytes kept from the forward pass, bytes of the backward
+    pass, whether the state tiles are kept, offsets of chunks .. pt, of the kept tiles, of the backward pass's buffers)."""
+    nc = T // CHUNK + docs + 2
+    square = nc * CHUNK * CHUNK * 4
+    work = [nc * 16, (docs + 3) * 4, nc * Hv * 3 * CHUNK * 4, nc * Hk * 2 * CHUNK * 4,
+            Hk * square if train or not delta else 0, Hk * square if train and delta else 0, nc * Hv * OPERANDS if delta else 0]
+    tiles = nc * Hv * (-(-dv // 64) * 2) * TILE
+    first = [tiles, tiles // 2 if delta else 0]
+    second = [tiles, tiles // 2 if delta else 0, 0 if delta else nc * Hv * 2 * 4]
+    keep = train and sum(first) <= KEEP_BYTES
+
+    def place(sizes):
+        at, out = 0, []
+        for s in sizes:
+            out.append(at if s else -1)                  # -1: no such buffer
+            at += (s + 255) // 256 * 256
+        return out, at
+
+    kept, kept_bytes = place(work + (first if keep else []))
+    later, later_bytes = place(second if keep else second + (first if train else [0, 0]))
+    return nc, kept_bytes, later_bytes, keep, tuple(kept), tuple(later)
 
 
-def _tiles(a: _Args, delta: bool):
-    """(field, bytes) of the operand tiles that the gradients read: one set from the forward pass, one from the backward."""
-    n = a.nc_max * a.Hv * (a.dvp // SLICE) * TILE
-    return [("s_tiles", n)] + ([("u_tiles", n // 2)] if delta else []), [("ds_tiles", n)] + (
-        [("dr_tiles", n // 2)] if delta else [("part", a.nc_max * a.Hv * 2 * 4)])
-
-
-def _place(a: _Args, fields, device) -> torch.Tensor:
-    offs, total = _pieces([n for _, n in fields])
-    buf = torch.empty(total, dtype=torch.uint8, device=device)
-    for (name, _), off in zip(fields, offs):
-        setattr(a, name, buf.data_ptr() + off)
-    return buf
-
-
-def _fill(a: _Args, q, k, v, g, b, A, D, cu, s_in, ws, keep: bool, delta: bool, scale: float, l2norm: bool) -> torch.Tensor:
-    """Inputs, sizes and the kept workspace (allocated if ``ws`` is None), which is returned."""
+def _words(q, k, v, g, b, A, D, cu, s_in, s_out, ds_out, ds_in, dy, outs, ws, tmp, lay, delta, l2norm):
+    """The arguments of the C entry points."""
     T, Hk, dk = q.shape
-    Hv, dv = v.shape[1], v.shape[2]
-    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    a.q_t, a.q_h, a.k_t, a.k_h, a.v_t, a.v_h = (q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0),
-                                                v.stride(1))
-    a.b, a.b_t, a.b_h = b.data_ptr(), b.stride(0), b.stride(1)
-    if delta:
-        a.g, a.g_t, a.g_h = g.data_ptr(), g.stride(0), g.stride(1)
-        a.s_k, a.s_v = dv, 1
-    else:
-        a.A, a.D = A.data_ptr(), D.data_ptr()
-        a.s_k, a.s_v = 1, dk
-    a.cu, a.s_in = cu.data_ptr(), _lib.ptr(s_in)
-    a.T, a.n_docs, a.Hk, a.Hv, a.dk, a.dv = T, cu.numel() - 1, Hk, Hv, dk, dv
-    a.dkp, a.dvp = 64 if dk <= 64 else 128, -(-dv // 64) * 64
-    a.nc_max = T // CHUNK + cu.numel() + 1
-    a.l2norm, a.scale = int(l2norm), scale
-    nc = a.nc_max
-    sizes = [("chunks", nc * 16), ("doc_off", (cu.numel() + 2) * 4), ("hd", nc * Hv * 3 * CHUNK * 4),
-             ("rqk", nc * Hk * 2 * CHUNK * 4)]
-    if delta:
-        sizes.append(("pt", nc * Hv * OPERANDS))
-    if keep or not delta:
-        sizes.append(("qk", nc * Hk * CHUNK * CHUNK * 4))
-    if keep and delta:
-        sizes.append(("kk", nc * Hk * CHUNK * CHUNK * 4))
-    offs, total = _pieces([n for _, n in sizes])
-    if ws is None:
-        ws = torch.empty(total, dtype=torch.uint8, device=q.device)
-    for (name, _), off in zip(sizes, offs):
-        setattr(a, name, ws.data_ptr() + off)
-    return ws
+    _, Hv, dv = v.shape
+    qs, ks, vs, bs = q.stride(), k.stride(), v.stride(), b.stride()
+    nc, _, _, keep, kept, later = lay
+    base = ws.data_ptr()
+    work = [base + o if o >= 0 else 0 for o in kept]
+    back = [0] * 5
+    if tmp is not None:
+        base = tmp.data_ptr()
+        back = [base + o if o >= 0 else 0 for o in later]
+    # state and U tiles come from the forward pass or are made again; dS and dR tiles and partial sums are the backward's
+    work += back[3:] + back[:3] if not keep else back[:3]
+    return _Words(q.data_ptr(), k.data_ptr(), v.data_ptr(), 0 if dy is None else dy.data_ptr(), qs[0], qs[1], ks[0], ks[1],
+                  vs[0], vs[1], *((0, 0) if dy is None else dy.stride()[:2]),
+                  0 if g is None else g.data_ptr(), b.data_ptr(), *((0, 0) if g is None else g.stride()), bs[0], bs[1],
+                  _ptr(A), _ptr(D), cu.data_ptr(), _ptr(s_in), _ptr(s_out), _ptr(ds_out), _ptr(ds_in),
+                  *((dv, 1) if delta else (1, dk)), *outs, *work,
+                  T, cu.shape[0] - 1, Hk, Hv, dk, dv, nc, l2norm)
+
+
+def _ptr(t) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 class _Recurrence(torch.autograd.Function):
@@ -126,23 +106,20 @@ class _Recurrence(torch.autograd.Function):
     def forward(ctx, q, k, v, g, b, A, D, s_in, cu, delta, scale, l2norm, final):
         global _launches
         q, k, v = _rows(q), _rows(k), _rows(v)
-        T, Hv, dv = v.shape
-        a = _Args()
-        with _lib.on_device(q):
-            keep = any(ctx.needs_input_grad)
-            ws = _fill(a, q, k, v, g, b, A, D, cu, s_in, None, keep, delta, scale, l2norm)
-            o = torch.empty((T, Hv, dv), dtype=v.dtype, device=v.device)
-            shape = (cu.numel() - 1, Hv) + ((q.shape[2], dv) if delta else (dv, q.shape[2]))
-            s_out = torch.empty(shape, dtype=torch.float32, device=v.device) if final else None
-            a.o, a.s_out = o.data_ptr(), _lib.ptr(s_out)
-            tiles = None
-            if keep and sum(n for _, n in _tiles(a, delta)[0]) <= KEEP_BYTES:
-                tiles = _place(a, _tiles(a, delta)[0], v.device)
-            _lib.check(_lib.cuda_lib().xb_recurrence_fwd(ctypes.byref(a), int(delta), _lib.stream_ptr()),
-                       "xb_recurrence_fwd")
+        T, Hk, dk = q.shape
+        _, Hv, dv = v.shape
+        dev = v.device
+        docs = cu.shape[0] - 1
+        lay = _layout(T, docs, Hk, Hv, dk, dv, delta, True in ctx.needs_input_grad)
+        ws = torch.empty(lay[1], dtype=torch.uint8, device=dev)
+        o = torch.empty((T, Hv, dv), dtype=v.dtype, device=dev)
+        s_out = torch.empty((docs, Hv, dk, dv) if delta else (docs, Hv, dv, dk), dtype=torch.float32, device=dev) if final else None
+        _lib.call_on(dev, "xb_recurrence_fwd", _words(q, k, v, g, b, A, D, cu, s_in, s_out, None, None, None,
+                                                      (o.data_ptr(), 0, 0, 0, 0, 0, 0, 0), ws, None, lay, delta, l2norm),
+                     scale, delta)
         _launches += 3
-        ctx.save_for_backward(q, k, v, g, b, A, D, s_in, cu, ws, tiles)
-        ctx.conf = (delta, scale, l2norm)
+        ctx.save_for_backward(q, k, v, g, b, A, D, s_in, cu, ws)
+        ctx.conf = (delta, scale, l2norm, lay)
         ctx.set_materialize_grads(False)
         return o, s_out
 
@@ -150,39 +127,29 @@ class _Recurrence(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy, ds_out):
         global _launches
-        q, k, v, g, b, A, D, s_in, cu, ws, tiles = ctx.saved_tensors
-        delta, scale, l2norm = ctx.conf
+        q, k, v, g, b, A, D, s_in, cu, ws = ctx.saved_tensors
+        delta, scale, l2norm, lay = ctx.conf
         T, Hk, dk = q.shape
-        Hv, dv = v.shape[1], v.shape[2]
+        _, Hv, dv = v.shape
         dev = q.device
-        a = _Args()
-        with _lib.on_device(q):
-            dy = torch.zeros((T, Hv, dv), dtype=v.dtype, device=dev) if dy is None else _rows(dy)
-            _fill(a, q, k, v, g, b, A, D, cu, s_in, ws, True, delta, scale, l2norm)
-            a.dy, a.dy_t, a.dy_h = dy.data_ptr(), dy.stride(0), dy.stride(1)
-            ds_out = None if ds_out is None else ds_out.contiguous()
-            ds_in = torch.empty_like(s_in) if ctx.needs_input_grad[7] else None
-            a.ds_out, a.ds_in = _lib.ptr(ds_out), _lib.ptr(ds_in)
-            dq = torch.empty((T, Hk, dk), dtype=q.dtype, device=dev)
-            dkk = torch.empty((T, Hk, dk), dtype=q.dtype, device=dev)
-            dvv = torch.empty((T, Hv, dv), dtype=v.dtype, device=dev)
-            db = torch.empty((T, Hv), dtype=torch.float32, device=dev)
-            dg = torch.empty((T, Hv), dtype=torch.float32, device=dev) if delta else None
-            dA = None if delta else torch.empty(Hv, dtype=torch.float32, device=dev)
-            dD = None if delta else torch.empty(Hv, dtype=torch.float32, device=dev)
-            a.dq, a.dk_out, a.dv_out, a.db = dq.data_ptr(), dkk.data_ptr(), dvv.data_ptr(), db.data_ptr()
-            a.dg, a.dA, a.dD = _lib.ptr(dg), _lib.ptr(dA), _lib.ptr(dD)
-            first, second = _tiles(a, delta)
-            if tiles is None:
-                tmp = _place(a, first + second, dev)
-            else:
-                tmp = _place(a, second, dev)
-                for (name, _), off in zip(first, _pieces([n for _, n in first])[0]):
-                    setattr(a, name, tiles.data_ptr() + off)
-            _lib.check(_lib.cuda_lib().xb_recurrence_bwd(ctypes.byref(a), int(delta), int(tiles is not None), _lib.stream_ptr()),
-                       "xb_recurrence_bwd")
-        del tmp
-        _launches += (2 if delta else 3) + int(tiles is None)
+        dy = torch.zeros((T, Hv, dv), dtype=v.dtype, device=dev) if dy is None else _rows(dy)
+        ds_out = None if ds_out is None else ds_out.contiguous()
+        ds_in = torch.empty_like(s_in) if ctx.needs_input_grad[7] else None
+        dq = torch.empty((T, Hk, dk), dtype=q.dtype, device=dev)
+        dkk = torch.empty((T, Hk, dk), dtype=q.dtype, device=dev)
+        dvv = torch.empty((T, Hv, dv), dtype=v.dtype, device=dev)
+        db = torch.empty((T, Hv), dtype=torch.float32, device=dev)
+        if delta:
+            dg, dA, dD = torch.empty((T, Hv), dtype=torch.float32, device=dev), None, None
+        else:
+            dg = None
+            dA, dD = (torch.empty(Hv, dtype=torch.float32, device=dev) for _ in range(2))
+        tmp = torch.empty(lay[2], dtype=torch.uint8, device=dev)
+        _lib.call_on(dev, "xb_recurrence_bwd", _words(q, k, v, g, b, A, D, cu, s_in, None, ds_out, ds_in, dy,
+                                               (0, dq.data_ptr(), dkk.data_ptr(), dvv.data_ptr(), _ptr(dg), db.data_ptr(),
+                                                _ptr(dA), _ptr(dD)), ws, tmp, lay, delta, l2norm),
+              scale, delta, lay[3])
+        _launches += (2 if delta else 3) + (not lay[3])
         return dq, dkk, dvv, dg, db, dA, dD, ds_in, None, None, None, None, None
 
 
@@ -192,16 +159,18 @@ def _check(what: str, q, k, v, per_head, cu, s_in, state_shape, names) -> None:
                          f"[T, heads, dim] with the same T (got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)})")
     if q.shape[1] == 0 or v.shape[1] % q.shape[1] or not (q.shape[2] and v.shape[2] and v.shape[1]):
         raise ValueError(f"{what}: {v.shape[1]} heads of {names[2]} cannot share {q.shape[1]} heads of {names[0]}")
-    for name, t, shape in per_head:
-        if tuple(t.shape) != shape:
-            raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected {shape}")
-    if cu.dim() != 1 or cu.numel() < 1 or cu.is_floating_point():
+    if cu.dim() != 1 or cu.shape[0] < 1 or cu.is_floating_point():
         raise ValueError(f"{what}: cu_seqlens is a vector of integers, one more than there are documents")
-    if s_in is not None and tuple(s_in.shape) != state_shape:
-        raise ValueError(f"{what}: initial_state has shape {tuple(s_in.shape)}, expected {state_shape}")
-    for t in [q, k, v] + [t for _, t, _ in per_head] + ([s_in] if s_in is not None else []):
-        if t.device != q.device:
-            raise ValueError(f"{what}: inputs on different devices ({q.device} and {t.device})")
+    dev = q.device
+    if k.device != dev or v.device != dev:
+        raise ValueError(f"{what}: inputs on different devices")
+    for name, t, shape in per_head:
+        if t.shape != shape:
+            raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected {shape}")
+        if t.device != dev:
+            raise ValueError(f"{what}: {name} is on {t.device}, {names[0]} on {dev}")
+    if s_in is not None and (s_in.shape != state_shape or s_in.device != dev):
+        raise ValueError(f"{what}: initial_state is {tuple(s_in.shape)} on {s_in.device}, expected {state_shape} on {dev}")
 
 
 def _kernel_ok(q, k, v) -> bool:
@@ -249,7 +218,7 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
                                           initial_state=initial_state, return_final_state=return_final_state)
     s_in = None if initial_state is None else initial_state.float().contiguous()
     o, s = _lib.apply(_Recurrence, q, k, v, g.float(), beta.float(), None, None, s_in,
-                      _boundaries(cu_seqlens, q.device), True, scale, bool(qk_l2norm), bool(return_final_state))
+                      _boundaries(cu_seqlens, q.device), True, scale, bool(qk_l2norm), return_final_state)
     return (o, s) if return_final_state else o
 
 
@@ -305,5 +274,5 @@ def ssd_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor
                                   return_final_state=return_final_state, chunk=chunk)
     s_in = None if initial_state is None else initial_state.float().contiguous()
     y, s = _lib.apply(_Recurrence, C, B, x, None, dt.float(), A.float().contiguous(), D.float().contiguous(), s_in,
-                      _boundaries(cu_seqlens, x.device), False, 1.0, False, bool(return_final_state))
+                      _boundaries(cu_seqlens, x.device), False, 1.0, False, return_final_state)
     return (y, s) if return_final_state else y
