@@ -39,51 +39,134 @@ struct DPrepSmem {
     struct { uint8_t q[C * DKP * 2], k[C * DKP * 2]; };
     float l[2][C * LS];
   };
-  float2 qk[8 * 2 * 128], kk[8 * 2 * 128];  // Q K^T and K K^T, each thread's own fragments
+  float2 qk[8 * 2 * 128], kk[8 * 2 * 128];  // Q K^T and K K^T as fragments
   float hd[2][3][C];
   float rq[C], rk[C];
 };
 
-// 64 x 64 values per head to rows 64 * part .. of its operand tile: two planes of [128 rows][128 bytes] whose 16-byte
+// 64 x 64 values per head to the upper half of its operand tile: two planes of [128 rows][128 bytes] whose 16-byte
 // units are swizzled as the tensor core reads them
 constexpr int TP_PLANE = 128 * 128;
-__device__ __forceinline__ void put_tile(const XbRecArgs& p, const float (&l)[2][C * LS], int part, int c, int h, int heads) {
+__device__ __forceinline__ void put_tile(const XbRecArgs& p, const float (&l)[2][C * LS], int c, int h, int heads) {
   for (int it = threadIdx.x; it < 2 * C * 8; it += 128) {
     const int mm = it / (C * 8), r = (it >> 3) % C, u = it & 7;
     if (mm >= heads) break;
     const float4* src = reinterpret_cast<const float4*>(&l[mm][r * LS + u * 8]);
-    const float4 a = src[0], b = src[1];
+    const bool above = (u >> 1) > (r >> 4);            // blocks above the diagonal are not written by anybody
+    const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f), a = above ? zero : src[0], b = above ? zero : src[1];
     uint4 hi, lo;
     split2(a.x, a.y, hi.x, lo.x), split2(a.z, a.w, hi.y, lo.y), split2(b.x, b.y, hi.z, lo.z), split2(b.z, b.w, hi.w, lo.w);
-    uint8_t* dst = (uint8_t*)p.pt + ((long long)c * p.Hv + h + mm) * (2 * TP_PLANE) + (part * C + r) * 128 + ((u ^ (r & 7)) << 4);
+    uint8_t* dst = (uint8_t*)p.pt + ((long long)c * p.Hv + h + mm) * (2 * TP_PLANE) + r * 128 + ((u ^ (r & 7)) << 4);
     *reinterpret_cast<uint4*>(dst) = hi;
     *reinterpret_cast<uint4*>(dst + TP_PLANE) = lo;
   }
 }
 
-// x = column j of (I + L)^-1, whose first FROM rows are zero
-template <int FROM>
-__device__ __forceinline__ void solve(float (&x)[C], const float* L, int j) {
-  const float4* L4 = reinterpret_cast<const float4*>(L);
+// d (16 x 16, two column tiles) += A B of blocks in shared memory (row stride LS).  Three bf16 parts of each operand keep
+// the 24 bits of its significand, so the inverse is as exact as fp32 makes it.
+__device__ __forceinline__ void split3(float x, float y, uint32_t (&p)[3]) {
+  p[0] = pack_bf16x2(x, y);
+  const float2 h = unpack_bf16x2(p[0]);
+  x -= h.x, y -= h.y;
+  p[1] = pack_bf16x2(x, y);
+  const float2 m = unpack_bf16x2(p[1]);
+  p[2] = pack_bf16x2(x - m.x, y - m.y);
+}
+__device__ __forceinline__ void block_mma(float (&d)[2][4], const float* A, const float* B) {
+  const int lane = xb_lane(), g = lane >> 2, t = lane & 3;
+  uint32_t a[3][4];
 #pragma unroll
-  for (int i = 0; i < FROM; ++i) x[i] = 0.f;
-#pragma unroll
-  for (int i = FROM; i < C; ++i) {
-    float a0 = i == j ? 1.f : 0.f, a1 = 0.f, a2 = 0.f, a3 = 0.f;
-#pragma unroll
-    for (int k4 = FROM / 4; k4 < (i + 3) / 4; ++k4) {
-      const float4 l = L4[i * (LS / 4) + k4];
-      a0 -= l.x * x[4 * k4];
-      if (4 * k4 + 1 < i) a1 -= l.y * x[4 * k4 + 1];
-      if (4 * k4 + 2 < i) a2 -= l.z * x[4 * k4 + 2];
-      if (4 * k4 + 3 < i) a3 -= l.w * x[4 * k4 + 3];
-    }
-    x[i] = (a0 + a1) + (a2 + a3);
+  for (int e = 0; e < 4; ++e) {
+    const float2 x = *reinterpret_cast<const float2*>(A + (g + (e & 1) * 8) * LS + (e >> 1) * 8 + 2 * t);
+    uint32_t q[3];
+    split3(x.x, x.y, q);
+    a[0][e] = q[0], a[1][e] = q[1], a[2][e] = q[2];
   }
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    const float* b = B + 2 * t * LS + n * 8 + g;
+    uint32_t b0[3], b1[3];
+    split3(b[0], b[LS], b0);
+    split3(b[8 * LS], b[9 * LS], b1);
+    mma(d[n], a[2], b0[0], b1[0]);
+    mma(d[n], a[0], b0[2], b1[2]);
+    mma(d[n], a[1], b0[1], b1[1]);
+    mma(d[n], a[1], b0[0], b1[0]);
+    mma(d[n], a[0], b0[1], b1[1]);
+    mma(d[n], a[0], b0[0], b1[0]);
+  }
+}
+__device__ __forceinline__ void block_put(float* dst, const float (&d)[2][4], float sign) {
+  const int lane = xb_lane(), g = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int n = 0; n < 2; ++n)
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh)
+      *reinterpret_cast<float2*>(dst + (g + hh * 8) * LS + n * 8 + 2 * t) = make_float2(sign * d[n][2 * hh], sign * d[n][2 * hh + 1]);
+}
+// L (strictly lower, two heads) becomes (I + L)^-1 in place: the four diagonal blocks by substitution, one column per
+// thread, then T21 = -T22 L21 T11 for blocks of 16 and of 32.  (Substitution down all 64 rows is 2000 multiply-adds of
+// straight-line code for a thread, which ran at the speed of the instruction cache: 28,000 cycles.)
+__device__ __forceinline__ void invert(float (&l)[2][C * LS]) {
+  const int tid = threadIdx.x, w = tid >> 5, m = tid >> 6;
+  float* L = l[m];
+  {
+    const int blk = (tid & 63) >> 4, j = tid & 15;
+    float* D = L + blk * 16 * (LS + 1);
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float s0 = i == j ? 1.f : 0.f, s1 = 0.f;
+#pragma unroll
+      for (int k = 0; k < i; ++k) {
+        if (k & 1) s1 -= D[i * LS + k] * x[k];
+        else s0 -= D[i * LS + k] * x[k];
+      }
+      x[i] = s0 + s1;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) D[i * LS + j] = x[i];
+  }
+  __syncthreads();
+  {  // blocks of 16: one pair per warp
+    float* T11 = L + (w & 1) * 32 * (LS + 1);
+    float* L21 = T11 + 16 * LS;
+    float* T22 = L21 + 16;
+    float d[2][4] = {}, e[2][4] = {};
+    block_mma(d, L21, T11);
+    __syncwarp();
+    block_put(L21, d, 1.f);
+    __syncwarp();
+    block_mma(e, T22, L21);
+    __syncwarp();
+    block_put(L21, e, -1.f);
+  }
+  __syncthreads();
+  {  // blocks of 32: a warp has 16 of the 32 rows
+    const int i = w & 1;
+    float* row = L + (32 + 16 * i) * LS;
+    float d[2][2][4] = {}, e[2][2][4] = {};
+    block_mma(d[0], row, L);
+    block_mma(d[0], row + 16, L + 16 * LS);
+    block_mma(d[1], row + 16, L + 16 * LS + 16);
+    __syncwarp();
+    block_put(row, d[0], 1.f), block_put(row + 16, d[1], 1.f);
+    __syncthreads();
+    const float* M = L + 32 * LS;
+#pragma unroll 1
+    for (int k = 0; k <= i; ++k) {
+      block_mma(e[0], row + 32 + 16 * k, M + 16 * k * LS);
+      block_mma(e[1], row + 32 + 16 * k, M + 16 * k * LS + 16);
+    }
+    __syncthreads();
+    block_put(row, e[0], -1.f), block_put(row + 16, e[1], -1.f);
+  }
+  __syncthreads();
 }
 
 template <int DKP>
-__global__ void __launch_bounds__(128, 3) delta_prep(const XbRecArgs p) {
+__global__ void __launch_bounds__(128, 4) delta_prep(const XbRecArgs p) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   DPrepSmem<DKP>& sm = *reinterpret_cast<DPrepSmem<DKP>*>(smem_raw);
   constexpr int U = DKP / 8;
@@ -215,60 +298,52 @@ __global__ void __launch_bounds__(128, 3) delta_prep(const XbRecArgs p) {
       }
     }
     __syncthreads();
-    // column j of (I + L)^-1 by forward substitution: all threads of a head read the same row of L, and a warp of
-    // columns 32 .. 63 starts at row 32
-    const int m = tid >> 6, j = tid & 63;
-    float x[C];
-    if (h0 + m < rep) {
-      if (w & 1) solve<32>(x, sm.l[m], j);
-      else solve<0>(x, sm.l[m], j);
-    }
-    __syncthreads();
-    if (h0 + m < rep) {
-#pragma unroll
-      for (int i = 0; i < C; ++i) sm.l[m][i * LS + j] = x[i];
-    }
-    __syncthreads();
-    put_tile(p, sm.l, 0, c, kh * rep + h0, rep - h0);
-    // P T, this warp's 16 rows: P from the fragments of Q K^T, T from shared memory
-    float pt[2][8][4] = {};
-#pragma unroll
-    for (int mm = 0; mm < 2; ++mm) {
-      if (h0 + mm >= rep) break;
+    invert(sm.l);
+    put_tile(p, sm.l, c, kh * rep + h0, rep - h0);
+    // P T: two warps per head, 16 rows at a time (blocks 0 and 3, or 1 and 2); P from the fragments of Q K^T that the
+    // thread of the same lane in warp rb left, T from shared memory
+    const int mm = w >> 1;
+    if (h0 + mm < rep) {
       const float* hd = sm.hd[mm][0];
+      uint8_t* tile = (uint8_t*)p.pt + ((long long)c * p.Hv + kh * rep + h0 + mm) * (2 * TP_PLANE) + C * 128;
+#pragma unroll 1
+      for (int part = 0; part < 2; ++part) {
+        const int rb = part ? 3 - (w & 1) : (w & 1);
+        float d[8][4] = {};
+#pragma unroll 1
+        for (int ks = 0; ks <= rb; ++ks) {
+          uint32_t ah[4], al[4];
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        if (ks > w) break;
-        uint32_t ah[4], al[4];
+          for (int e = 0; e < 4; ++e) {
+            const int row = rb * 16 + g + (e & 1) * 8, col = ks * 16 + (e >> 1) * 8 + 2 * t;
+            const float2 x = sm.qk[((ks * 2 + (e >> 1)) * 2 + (e & 1)) * 128 + rb * 32 + lane];
+            split2(col <= row ? ex2_diff(hd, row, col) * x.x : 0.f, col + 1 <= row ? ex2_diff(hd, row, col + 1) * x.y : 0.f, ah[e], al[e]);
+          }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int row = r0 + (e & 1) * 8, col = ks * 16 + (e >> 1) * 8 + 2 * t;
-          const float2 x = sm.qk[((ks * 2 + (e >> 1)) * 2 + (e & 1)) * 128 + tid];
-          split2(col <= row ? ex2_diff(hd, row, col) * x.x : 0.f, col + 1 <= row ? ex2_diff(hd, row, col + 1) * x.y : 0.f, ah[e], al[e]);
+          for (int n = 0; n < 8; ++n) {
+            if (n > 2 * ks + 1) break;                 // T is lower triangular
+            const float* T = &sm.l[mm][(ks * 16 + 2 * t) * LS + n * 8 + g];
+            uint32_t bh[2], bl[2];
+            split2(T[0], T[LS], bh[0], bl[0]);
+            split2(T[8 * LS], T[9 * LS], bh[1], bl[1]);
+            mma(d[n], al, bh[0], bh[1]);
+            mma(d[n], ah, bl[0], bl[1]);
+            mma(d[n], ah, bh[0], bh[1]);
+          }
         }
 #pragma unroll
-        for (int n = 0; n < 8; ++n) {
-          if (n > 2 * ks + 1) break;
-          const float* T = &sm.l[mm][(ks * 16 + 2 * t) * LS + n * 8 + g];
-          uint32_t bh[2], bl[2];
-          split2(T[0], T[LS], bh[0], bl[0]);
-          split2(T[8 * LS], T[9 * LS], bh[1], bl[1]);
-          mma(pt[mm][n], al, bh[0], bh[1]);
-          mma(pt[mm][n], ah, bl[0], bl[1]);
-          mma(pt[mm][n], ah, bh[0], bh[1]);
-        }
+        for (int n = 0; n < 8; ++n)
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh) {
+            const int row = rb * 16 + g + hh * 8;
+            uint32_t hi, lo;
+            split2(d[n][2 * hh], d[n][2 * hh + 1], hi, lo);
+            uint8_t* dst = tile + row * 128 + ((n ^ (row & 7)) << 4) + t * 4;
+            *reinterpret_cast<uint32_t*>(dst) = hi;
+            *reinterpret_cast<uint32_t*>(dst + TP_PLANE) = lo;
+          }
       }
     }
-    __syncthreads();
-#pragma unroll
-    for (int mm = 0; mm < 2; ++mm)
-#pragma unroll
-      for (int n = 0; n < 8; ++n)
-#pragma unroll
-        for (int hh = 0; hh < 2; ++hh)
-          *reinterpret_cast<float2*>(&sm.l[mm][(r0 + hh * 8) * LS + n * 8 + 2 * t]) = make_float2(pt[mm][n][2 * hh], pt[mm][n][2 * hh + 1]);
-    __syncthreads();
-    put_tile(p, sm.l, 1, c, kh * rep + h0, rep - h0);
   }
 }
 
