@@ -5,16 +5,18 @@
 // only heads x column slices of them (32 x 4 for 32 heads of 128), less than one per SM: the time of a step is what
 // counts.  A CTA carries 32 state columns through three products per step, all of them 128 rows high:
 //
-//   forward   [K; Q] S        -> R (rows of K), gamma Q S (rows of Q)
-//             [T; P T] R      -> U, and P U = (P T) R beside it
-//             K^T (d U)       -> added to the state, whose 128 rows live in the registers of 128 x 2 threads
-//   backward  [K; .] dS'      -> Y = d K dS'
-//             [T; P T]^T [Y; dO] -> dR = T^T (Y + P^T dO)
+//   forward   [K; Q] S      -> R (rows of K), gamma Q S (rows of Q)
+//             [T; P] R      -> U
+//             K^T (d U)     -> added to the state, whose 128 rows live in the registers of 128 x 2 threads
+//             [T; P] U      -> P U, beside the next step
+//   backward  P^T dO        -> beside the step before
+//             K dS'         -> Y = d K dS' + P^T dO
+//             T^T Y         -> dR
 //             [K; Q]^T [-b gamma dR; gamma dO] -> added to dS  (the dO part is issued early)
 //
 // A computed operand enters as two bf16 parts side by side, [hi | lo], 64 columns of one product; the parts of T and
-// P T are two products into the same accumulator.  P = tril(D o Q K^T), T = (I + L)^-1 and P T depend on the chunk
-// alone and come from the prepare kernel as operand tiles.  Eight warps work on the accumulators, one row and 16
+// P are two products into the same accumulator.  P = tril(D o Q K^T) and T = (I + L)^-1 depend on the chunk alone and
+// come from the prepare kernel as operand tiles.  Eight warps work on the accumulators, one row and 16
 // columns per thread (row factors are scalars there); a ninth issues the loads and the products.  mma.sync spent 5800
 // cycles on a forward step (1100 of them on cp.async, 2300 in the tensor pipe): 789 us for 16384 tokens of 32 heads.
 #include "recurrence_core.cuh"
@@ -39,7 +41,7 @@ struct DPrepSmem {
     struct { uint8_t q[C * DKP * 2], k[C * DKP * 2]; };
     float l[2][C * LS];
   };
-  float2 qk[8 * 2 * 128], kk[8 * 2 * 128];  // Q K^T and K K^T as fragments
+  float2 qk[8 * 2 * 128], kk[8 * 2 * 128];  // Q K^T and K K^T, each thread's own fragments
   float hd[2][3][C];
   float rq[C], rk[C];
 };
@@ -283,15 +285,31 @@ __global__ void __launch_bounds__(128, 4) delta_prep(const XbRecArgs p) {
     for (int m = 0; m < 2; ++m) {
       if (h0 + m >= rep) break;
       const float* hd = sm.hd[m][0];
+      // P as the lower half of the operand tile, L for the inverse
+      uint8_t* tile = (uint8_t*)p.pt + ((long long)c * p.Hv + kh * rep + h0 + m) * (2 * TP_PLANE) + C * 128;
 #pragma unroll
       for (int nt = 0; nt < 8; ++nt) {
-        if (nt > 2 * w + 1) break;
         const int col = nt * 8 + 2 * t;
+        if (nt > 2 * w + 1) {                          // blocks above the diagonal
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh) {
+            const int row = r0 + hh * 8;
+            uint8_t* dst = tile + row * 128 + ((nt ^ (row & 7)) << 4) + t * 4;
+            *reinterpret_cast<uint32_t*>(dst) = 0;
+            *reinterpret_cast<uint32_t*>(dst + TP_PLANE) = 0;
+          }
+          continue;
+        }
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
           const int row = r0 + hh * 8;
-          const float2 y = sm.kk[(nt * 2 + hh) * 128 + tid];
+          const float2 x = sm.qk[(nt * 2 + hh) * 128 + tid], y = sm.kk[(nt * 2 + hh) * 128 + tid];
           const float d0 = ex2_diff(hd, row, col), d1 = ex2_diff(hd, row, col + 1), b = hd[2 * C + row];
+          uint32_t hi, lo;
+          split2(col <= row ? d0 * x.x : 0.f, col + 1 <= row ? d1 * x.y : 0.f, hi, lo);
+          uint8_t* dst = tile + row * 128 + ((nt ^ (row & 7)) << 4) + t * 4;
+          *reinterpret_cast<uint32_t*>(dst) = hi;
+          *reinterpret_cast<uint32_t*>(dst + TP_PLANE) = lo;
           *reinterpret_cast<float2*>(&sm.l[m][row * LS + col]) =
               make_float2(col < row ? b * d0 * y.x : 0.f, col + 1 < row ? b * d1 * y.y : 0.f);
         }
@@ -300,50 +318,6 @@ __global__ void __launch_bounds__(128, 4) delta_prep(const XbRecArgs p) {
     __syncthreads();
     invert(sm.l);
     put_tile(p, sm.l, c, kh * rep + h0, rep - h0);
-    // P T: two warps per head, 16 rows at a time (blocks 0 and 3, or 1 and 2); P from the fragments of Q K^T that the
-    // thread of the same lane in warp rb left, T from shared memory
-    const int mm = w >> 1;
-    if (h0 + mm < rep) {
-      const float* hd = sm.hd[mm][0];
-      uint8_t* tile = (uint8_t*)p.pt + ((long long)c * p.Hv + kh * rep + h0 + mm) * (2 * TP_PLANE) + C * 128;
-#pragma unroll 1
-      for (int part = 0; part < 2; ++part) {
-        const int rb = part ? 3 - (w & 1) : (w & 1);
-        float d[8][4] = {};
-#pragma unroll 1
-        for (int ks = 0; ks <= rb; ++ks) {
-          uint32_t ah[4], al[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int row = rb * 16 + g + (e & 1) * 8, col = ks * 16 + (e >> 1) * 8 + 2 * t;
-            const float2 x = sm.qk[((ks * 2 + (e >> 1)) * 2 + (e & 1)) * 128 + rb * 32 + lane];
-            split2(col <= row ? ex2_diff(hd, row, col) * x.x : 0.f, col + 1 <= row ? ex2_diff(hd, row, col + 1) * x.y : 0.f, ah[e], al[e]);
-          }
-#pragma unroll
-          for (int n = 0; n < 8; ++n) {
-            if (n > 2 * ks + 1) break;                 // T is lower triangular
-            const float* T = &sm.l[mm][(ks * 16 + 2 * t) * LS + n * 8 + g];
-            uint32_t bh[2], bl[2];
-            split2(T[0], T[LS], bh[0], bl[0]);
-            split2(T[8 * LS], T[9 * LS], bh[1], bl[1]);
-            mma(d[n], al, bh[0], bh[1]);
-            mma(d[n], ah, bl[0], bl[1]);
-            mma(d[n], ah, bh[0], bh[1]);
-          }
-        }
-#pragma unroll
-        for (int n = 0; n < 8; ++n)
-#pragma unroll
-          for (int hh = 0; hh < 2; ++hh) {
-            const int row = rb * 16 + g + hh * 8;
-            uint32_t hi, lo;
-            split2(d[n][2 * hh], d[n][2 * hh + 1], hi, lo);
-            uint8_t* dst = tile + row * 128 + ((n ^ (row & 7)) << 4) + t * 4;
-            *reinterpret_cast<uint32_t*>(dst) = hi;
-            *reinterpret_cast<uint32_t*>(dst + TP_PLANE) = lo;
-          }
-      }
-    }
   }
 }
 
@@ -361,10 +335,10 @@ struct Lay {
   static constexpr int SMEM = SM_BAR + 128 + 1024;
 };
 constexpr int WORKERS = 256, THREADS = WORKERS + 32;
-constexpr int TMEM_COLS = 256, D1 = 0, D2 = 64, D3 = 128;     // accumulators, 64 columns each
+constexpr int TMEM_COLS = 256, D1 = 0, D2 = 64, D3 = 128, D4 = 192;     // accumulators, 64 columns each
 
 struct __align__(8) Bars {
-  uint64_t full[2], done[3];
+  uint64_t full[2], done[4];
   uint32_t tmem;
   int abort_flag;
 };
@@ -507,7 +481,7 @@ __device__ __forceinline__ bool cta_setup(const XbRecArgs& p, Cta& a, uint8_t* r
 __device__ __forceinline__ void cta_begin(Cta& a) {
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) mbar_init(&a.bars->full[i], 1);
-    for (int i = 0; i < 3; ++i) mbar_init(&a.bars->done[i], 1);
+    for (int i = 0; i < 4; ++i) mbar_init(&a.bars->done[i], 1);
     a.bars->abort_flag = 0;
     mbar_fence_init();
   }
@@ -540,9 +514,9 @@ __device__ __forceinline__ void zero_rows(const XbRecArgs& p, const Cta& a, bf16
 }
 
 // Workers tell the issuing warp through barriers 1 (state tile and this chunk's loads), 2 and 3 (operands of the second
-// and third product) that operands are written, and learn through done[0 .. 2] that a product is complete.  A wait
-// that runs out raises a flag; everybody then walks through the remaining steps without waiting, so that no barrier
-// is left with a thread missing.
+// and third product) and 4 (of the one beside the chain) that operands are written, and learn through done[0 .. 3] that a
+// product is complete.  A wait that runs out raises a flag; everybody then walks through the remaining steps without
+// waiting, so that no barrier is left with a thread missing.
 
 // OUT: outputs are wanted.  SAVE: the tiles of the states and of U go to global memory.
 template <bool OUT, bool SAVE, int STAGES>
@@ -561,8 +535,15 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
   }
   cta_begin(a);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int4* chunks = reinterpret_cast<const int4*>(p.chunks);
   if (warp == WORKERS / 32) {
     const bool one = lane == 0;
+    // the stage of chunk n is free when the chunk's last product has read it
+    auto refill = [&](int n) {
+      if (n < 0 || n + STAGES >= a.c1 - a.c0) return;
+      a.wait1(&a.bars->done[OUT ? 3 : 2], n & 1, 2);
+      load_stage(p, a, &mk, &mq, &mv, a.c0 + n + STAGES, n % STAGES);
+    };
     for (int n = 0; n < STAGES; ++n)
       if (one && a.c0 + n < a.c1) load_stage(p, a, &mk, &mq, &mv, a.c0 + n, n);
     for (int n = 0; n < a.c1 - a.c0; ++n) {
@@ -578,6 +559,7 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
           tc_mma_f16_ss(a.tmem + D1, xb_smem_desc(KMAJ, st + ST_KQ + (k >> 2) * HALF + (k & 3) * 32), xb_smem_desc(MNMAJ, b1 + k * 2048), id, k > 0);
         tc_commit(&a.bars->done[0]);
         if (SAVE) keep_tiles(p, a, p.s_tiles, p.u_tiles, a.c0 + n, n > 0 ? a.c0 + n - 1 : -1);
+        if (STAGES == 2) refill(n - 1);
       }
       bar(2, THREADS);
       if (one) {
@@ -597,11 +579,20 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
         for (int k = 0; k < 4; ++k)
           tc_mma_f16_ss(a.tmem + D3, xb_smem_desc(MNMAJ, st + ST_KQ + k * 2048), xb_smem_desc(MNMAJ, b3 + k * 2048), id, k > 0);
         tc_commit(&a.bars->done[2]);
-        if (n + STAGES < a.c1 - a.c0) {           // the stage is free when the last product has read it
-          a.wait1(&a.bars->done[2], n & 1, 2);
-          load_stage(p, a, &mk, &mq, &mv, a.c0 + n + STAGES, n % STAGES);
+      }
+      if (OUT) {
+        bar(4, THREADS);
+        if (one) {
+          tc_fence_after();
+          constexpr uint32_t id = xb_idesc(1, 1, 128, 64, 0, 1);
+          const uint32_t u = xb_smem_u32(a.smem + L::SM_U);
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            tc_mma_f16_ss(a.tmem + D4, xb_smem_desc(KMAJ, st + ST_TP + (k >> 2) * TP_PLANE + (k & 3) * 32), xb_smem_desc(MNMAJ, u + (k & 3) * 2048), id, k > 0);
+          tc_commit(&a.bars->done[3]);
         }
       }
+      if (STAGES == 1 && one) refill(n);
       __syncwarp();
     }
     if (SAVE && a.c0 < a.c1) {
@@ -616,27 +607,50 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
     const bool krow = r < C;
     const uint32_t acc = a.tmem + ((uint32_t)(q4 * 32) << 16) + half * 16;
     const long long soff = ((long long)a.doc * p.Hv + a.h) * p.dk * p.dv + a.v0 * p.s_v;
-    float s[16] = {};
+    float s[16] = {}, y[16];
     uint32_t hi[8], lo[8];
     if (p.s_in != nullptr) state_row(const_cast<float*>(p.s_in) + soff, p.s_k, p.s_v, r, p.dk, half * 16, a.vcols, false, s);
-    for (int n = 0; n < a.c1 - a.c0; ++n) {
-      const int c = a.c0 + n, len = reinterpret_cast<const int4*>(p.chunks)[c].y;
-      const long long t0 = reinterpret_cast<const int4*>(p.chunks)[c].x;
+    // O = gamma rq Q S + P U of a chunk, whose Q S waits in y (threads of Q's rows)
+    auto finish = [&](int n, int4 ch, float f) {
+      a.wait(&a.bars->done[3], n & 1, 7);
+      tc_fence_after();
+      float x[16];
+      read_acc(acc + D4, x);
+      if (!krow && i < ch.y) {
+        bf16* dst = o + (long long)(ch.x + i) * o_t + half * 16;
+#pragma unroll
+        for (int e = 0; e < 16; e += 8)
+          if (half * 16 + e < a.vcols)
+            *reinterpret_cast<uint4*>(dst + e) =
+                make_uint4(pack_bf16x2(f * y[e] + x[e], f * y[e + 1] + x[e + 1]), pack_bf16x2(f * y[e + 2] + x[e + 2], f * y[e + 3] + x[e + 3]),
+                           pack_bf16x2(f * y[e + 4] + x[e + 4], f * y[e + 5] + x[e + 5]), pack_bf16x2(f * y[e + 6] + x[e + 6], f * y[e + 7] + x[e + 7]));
+      }
+      tc_fence_before();
+      __syncwarp();
+    };
+    const int steps = a.c1 - a.c0;
+    int4 ch = steps > 0 ? chunks[a.c0] : make_int4(0, 0, 0, 0), old = ch;
+    float fo = 0.f;                          // gamma rq of the chunk before
+    for (int n = 0; n < steps; ++n) {
       uint8_t* st = a.smem + (n % STAGES) * STAGE;
       const float* hd = reinterpret_cast<const float*>(st + ST_HD);
       const float* rqk = reinterpret_cast<const float*>(st + ST_RQK);
       put_row(a.smem + L::SM_S, r, half, s, hi, lo);
       a.wait(&a.bars->full[n % STAGES], (n / STAGES) & 1, 3);
-      if (len < C) clear_rows(st, len);
+      if (ch.y < C) clear_rows(st, ch.y);
       fence_proxy_async_smem();
       tc_fence_before();
       bar_arrive(1, THREADS);
+      if (OUT && q4 >= 2 && n > 0) finish(n - 1, old, fo);
       // row factors, and v, while the first product runs
       const float gam = ex2_sum(hd, i), dec = ex2_diff(hd, C - 1, i), last = ex2_sum(hd, C - 1), b = hd[2 * C + i];
       const float rq = rqk[i], rk = rqk[C + i];
+      const int len = ch.y;
       uint4 xv[2];
       read_x(st + ST_X, i, half, krow && i < len, xv);
-      float x[16], y[16];
+      old = ch, fo = gam * rq;
+      if (n + 1 < steps) ch = chunks[a.c0 + n + 1];
+      float x[16];
       a.wait(&a.bars->done[0], n & 1, 4);
       tc_fence_after();
       read_acc(acc + D1, y);
@@ -652,36 +666,29 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       bar_arrive(2, THREADS);
       a.wait(&a.bars->done[1], n & 1, 5);
       tc_fence_after();
-      read_acc(acc + D2, x);
-      if (krow) {                            // d rk U
-        if (SAVE) put_row(a.smem + L::SM_U, i, half, x, hi, lo);
+      if (krow) {                            // d rk U, then U itself
+        read_acc(acc + D2, x);
+        float z[16];
         const float f = dec * rk;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] *= f;
-        put_row(a.smem + L::SM_B3, i, half, x, hi, lo);
+        for (int e = 0; e < 16; ++e) z[e] = f * x[e];
+        put_row(a.smem + L::SM_B3, i, half, z, hi, lo);
       }
       fence_proxy_async_smem();
       tc_fence_before();
       bar_arrive(3, THREADS);
-      if (OUT && !krow && i < len) {       // O = gamma rq Q S + (P T) R
-        const float f = gam * rq;
-        bf16* dst = o + (t0 + i) * o_t + half * 16;
-#pragma unroll
-        for (int e = 0; e < 16; e += 8)
-          if (half * 16 + e < a.vcols)
-            *reinterpret_cast<uint4*>(dst + e) =
-                make_uint4(pack_bf16x2(f * y[e] + x[e], f * y[e + 1] + x[e + 1]), pack_bf16x2(f * y[e + 2] + x[e + 2], f * y[e + 3] + x[e + 3]),
-                           pack_bf16x2(f * y[e + 4] + x[e + 4], f * y[e + 5] + x[e + 5]), pack_bf16x2(f * y[e + 6] + x[e + 6], f * y[e + 7] + x[e + 7]));
-      }
-      __syncwarp();
+      if (krow) put_row(a.smem + L::SM_U, i, half, x, hi, lo);
+      fence_proxy_async_smem();
+      if (OUT) bar_arrive(4, THREADS);
       a.wait(&a.bars->done[2], n & 1, 6);
       tc_fence_after();
-      read_acc(acc + D3, y);
+      float z[16];
+      read_acc(acc + D3, z);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] = last * s[e] + y[e];
+      for (int e = 0; e < 16; ++e) s[e] = last * s[e] + z[e];
     }
-    fence_proxy_async_smem();
-    if (SAVE && a.c0 < a.c1) bar_arrive(1, THREADS);
+    if (OUT && q4 >= 2 && steps > 0) finish(steps - 1, old, fo);
+    if (SAVE && steps > 0) bar_arrive(1, THREADS);
     if (p.s_out != nullptr) state_row(p.s_out + soff, p.s_k, p.s_v, r, p.dk, half * 16, a.vcols, true, s);
   }
   cta_end(a);
@@ -703,6 +710,7 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
   }
   cta_begin(a);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, steps = a.c1 - a.c0;
+  const int4* chunks = reinterpret_cast<const int4*>(p.chunks);
   if (warp == WORKERS / 32) {
     const bool one = lane == 0;
     if (one && steps > 0) load_stage(p, a, &mk, &mq, &my, a.c1 - 1, 0);
@@ -711,14 +719,22 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       const uint32_t st = xb_smem_u32(a.smem + (n & 1) * STAGE), b1 = xb_smem_u32(a.smem + L::SM_S), b2 = xb_smem_u32(a.smem + L::SM_B2),
                      b3 = xb_smem_u32(a.smem + L::SM_B3);
       constexpr uint32_t id3 = xb_idesc(1, 1, 128, 64, 1, 1);
-      bar(1, THREADS);
+      constexpr uint32_t id1 = xb_idesc(1, 1, 64, 64, 0, 1), id2 = xb_idesc(1, 1, 64, 64, 1, 1), id4 = xb_idesc(1, 1, 64, 32, 1, 1);
+      bar(4, THREADS);
       if (one) {
         a.wait1(&a.bars->full[n & 1], (n >> 1) & 1, 1);
         tc_fence_after();
-        constexpr uint32_t id = xb_idesc(1, 1, 128, 64, 0, 1);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)          // P^T dO
+          tc_mma_f16_ss(a.tmem + D4, xb_smem_desc(MNMAJ, st + ST_TP + (k >> 2) * TP_PLANE + HALF / 2 + (k & 3) * 2048),
+                        xb_smem_desc(MNMAJ, b2 + HALF / 2 + (k & 3) * 2048), id4, k > 0);
+      }
+      bar(1, THREADS);
+      if (one) {
+        tc_fence_after();
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          tc_mma_f16_ss(a.tmem + D1, xb_smem_desc(KMAJ, st + ST_KQ + (k >> 2) * HALF + (k & 3) * 32), xb_smem_desc(MNMAJ, b1 + k * 2048), id, k > 0);
+          tc_mma_f16_ss(a.tmem + D1, xb_smem_desc(KMAJ, st + ST_KQ + (k >> 2) * HALF + (k & 3) * 32), xb_smem_desc(MNMAJ, b1 + k * 2048), id1, k > 0);
         tc_commit(&a.bars->done[0]);
 #pragma unroll
         for (int k = 4; k < 8; ++k)          // rows of Q
@@ -729,10 +745,9 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       if (one) {
         tc_fence_after();
         tma_store_wait_read<0>();
-        constexpr uint32_t id = xb_idesc(1, 1, 64, 64, 1, 1);
 #pragma unroll
-        for (int k = 0; k < 16; ++k)
-          tc_mma_f16_ss(a.tmem + D2, xb_smem_desc(MNMAJ, st + ST_TP + (k >> 3) * TP_PLANE + (k & 7) * 2048), xb_smem_desc(MNMAJ, b2 + (k & 7) * 2048), id, k > 0);
+        for (int k = 0; k < 8; ++k)
+          tc_mma_f16_ss(a.tmem + D2, xb_smem_desc(MNMAJ, st + ST_TP + (k >> 2) * TP_PLANE + (k & 3) * 2048), xb_smem_desc(MNMAJ, b2 + (k & 3) * 2048), id2, k > 0);
         tc_commit(&a.bars->done[1]);
       }
       bar(3, THREADS);
@@ -765,9 +780,9 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
     float s[16] = {}, x[16];
     uint32_t hi[8], lo[8];
     if (p.ds_out != nullptr) state_row(const_cast<float*>(p.ds_out) + soff, p.s_k, p.s_v, r, p.dk, half * 16, a.vcols, false, s);
-    // operands that need dO alone: [dO | 0] of the second product, gamma rq dO of the third (threads of Q's rows)
+    // operands that need dO alone: dO beside Y's tile, gamma rq dO of the third product (threads of Q's rows)
     auto put_dy = [&](int n) {
-      const int c = a.c1 - 1 - n, len = reinterpret_cast<const int4*>(p.chunks)[c].y;
+      const int len = chunks[a.c1 - 1 - n].y;
       uint8_t* st = a.smem + (n & 1) * STAGE;
       a.wait(&a.bars->full[n & 1], (n >> 1) & 1, 3);
       if (len < C) clear_rows(st, len);
@@ -783,14 +798,15 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       for (int e = 0; e < 16; ++e) x[e] *= f;
       put_row(a.smem + L::SM_B3, r, half, x, hi, lo);
     };
-    if (!krow)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        *reinterpret_cast<uint4*>(a.smem + L::SM_B2 + r * 128 + (((4 + half * 2 + e) ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
-    if (steps > 0) put_dy(0);
+    if (steps > 0) {
+      put_dy(0);
+      fence_proxy_async_smem();
+      bar_arrive(4, THREADS);
+    }
+    int4 ch = steps > 0 ? chunks[a.c1 - 1] : make_int4(0, 0, 0, 0);
     for (int n = 0; n < steps; ++n) {
-      const int c = a.c1 - 1 - n, len = reinterpret_cast<const int4*>(p.chunks)[c].y;
-      const long long t0 = reinterpret_cast<const int4*>(p.chunks)[c].x;
+      const int len = ch.y;
+      const long long t0 = ch.x;
       uint8_t* st = a.smem + (n & 1) * STAGE;
       const float* hd = reinterpret_cast<const float*>(st + ST_HD);
       const float* rqk = reinterpret_cast<const float*>(st + ST_RQK);
@@ -798,15 +814,17 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       fence_proxy_async_smem();
       tc_fence_before();
       bar_arrive(1, THREADS);
-      const float last = ex2_sum(hd, C - 1), f1 = ex2_diff(hd, C - 1, i) * rqk[C + i];
+      const float last = ex2_sum(hd, C - 1), f1 = ex2_diff(hd, C - 1, ri) * rqk[C + ri];
       const float b = hd[2 * C + ri], f2 = -b * ex2_sum(hd, ri) * rqk[C + ri];
       a.wait(&a.bars->done[0], n & 1, 4);
       tc_fence_after();
-      if (q4 < 2) {                          // Y = d rk K dS'
+      {                                      // Y = d rk K dS' + P^T dO
+        uint32_t v[16];
+        tmem_ld_32x16(acc + D4, v);
         read_acc(acc + D1, x);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] *= f1;
-        put_row(a.smem + L::SM_B2, i, half, x, hi, lo);
+        for (int e = 0; e < 16; ++e) x[e] = f1 * x[e] + __uint_as_float(v[e]);
+        if (lane < 16) put_row(a.smem + L::SM_B2, ri, half, x, hi, lo);
       }
       fence_proxy_async_smem();
       tc_fence_before();
@@ -835,8 +853,12 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
         }
       }
       __syncwarp();
-      if (n + 1 < steps) put_dy(n + 1);      // beside the third product: the first two have read these rows
-      __syncwarp();
+      if (n + 1 < steps) {                   // beside the third product: the first two have read these rows
+        ch = chunks[a.c1 - 2 - n];
+        put_dy(n + 1);
+        fence_proxy_async_smem();
+        bar_arrive(4, THREADS);
+      }
       a.wait(&a.bars->done[2], n & 1, 6);
       tc_fence_after();
       read_acc(acc + D3, x);
