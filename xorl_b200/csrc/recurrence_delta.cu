@@ -17,7 +17,7 @@
 // A computed operand enters as two bf16 parts side by side, [hi | lo], 64 columns of one product; the parts of T and
 // P are two products into the same accumulator.  P = tril(D o Q K^T) and T = (I + L)^-1 depend on the chunk alone and
 // come from the prepare kernel as operand tiles.  Eight warps work on the accumulators, one row and 16
-// columns per thread (row factors are scalars there); a ninth issues the loads and the products.  mma.sync spent 5800
+// columns per thread (row factors are scalars there), one issues the products, one moves tiles in and out.  mma.sync spent 5800
 // cycles on a forward step (1100 of them on cp.async, 2300 in the tensor pipe): 789 us for 16384 tokens of 32 heads.
 #include "recurrence_core.cuh"
 
@@ -334,11 +334,12 @@ struct Lay {
   static constexpr int SM_S = STAGES * STAGE, SM_B2 = SM_S + HALF, SM_B3 = SM_B2 + ROWS, SM_U = SM_B3 + ROWS, SM_BAR = SM_U + HALF / 2;
   static constexpr int SMEM = SM_BAR + 128 + 1024;
 };
-constexpr int WORKERS = 256, THREADS = WORKERS + 32;
+constexpr int WORKERS = 256, ISSUER = WORKERS / 32, LOADER = ISSUER + 1, THREADS = WORKERS + 64;
+constexpr int MEET = WORKERS + 32;           // workers and the issuing warp
 constexpr int TMEM_COLS = 256, D1 = 0, D2 = 64, D3 = 128, D4 = 192;     // accumulators, 64 columns each
 
 struct __align__(8) Bars {
-  uint64_t full[2], done[4];
+  uint64_t full[2], done[4], kept;
   uint32_t tmem;
   int abort_flag;
 };
@@ -384,6 +385,8 @@ __device__ __forceinline__ void keep_tiles(const XbRecArgs& p, const Cta& a, voi
   if (cs >= 0) bulk_store((uint8_t*)states + (((long long)cs * p.Hv + a.h) * slices + sl) * HALF, a.smem + a.sm_s, HALF);
   if (cu >= 0) bulk_store((uint8_t*)rows + (((long long)cu * p.Hv + a.h) * slices + sl) * (HALF / 2), a.smem + a.sm_u, HALF / 2);
   tma_store_commit();
+  tma_store_wait_read<0>();
+  mbar_arrive(&a.bars->kept);
 }
 
 // Rows of K and Q behind the document's end: they hold the next document's, and 0 x Inf is NaN.
@@ -406,10 +409,6 @@ __device__ __forceinline__ void put_row(uint8_t* tile, int row, int half, const 
     *reinterpret_cast<uint4*>(r + ((u ^ (row & 7)) << 4)) = make_uint4(hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
     *reinterpret_cast<uint4*>(r + (((u + 4) ^ (row & 7)) << 4)) = make_uint4(lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
   }
-}
-__device__ __forceinline__ void store16(bf16* dst, const uint32_t (&v)[8]) {
-  reinterpret_cast<uint4*>(dst)[0] = make_uint4(v[0], v[1], v[2], v[3]);
-  reinterpret_cast<uint4*>(dst)[1] = make_uint4(v[4], v[5], v[6], v[7]);
 }
 // the sum of an accumulator's two halves, 16 columns of this thread's row
 __device__ __forceinline__ void read_acc(uint32_t addr, float (&x)[16]) {
@@ -482,10 +481,11 @@ __device__ __forceinline__ void cta_begin(Cta& a) {
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) mbar_init(&a.bars->full[i], 1);
     for (int i = 0; i < 4; ++i) mbar_init(&a.bars->done[i], 1);
+    mbar_init(&a.bars->kept, 1);
     a.bars->abort_flag = 0;
     mbar_fence_init();
   }
-  if (threadIdx.x >= WORKERS) {
+  if (threadIdx.x / 32 == ISSUER) {
     tmem_alloc(&a.bars->tmem, TMEM_COLS);
     tmem_relinquish();
   }
@@ -500,7 +500,7 @@ __device__ __forceinline__ void cta_end(Cta& a) {
     for (const uint64_t t0 = xb_globaltimer(); xb_globaltimer() - t0 < 200000000ull;) {}
   tc_fence_before();
   __syncthreads();
-  if (threadIdx.x >= WORKERS) {
+  if (threadIdx.x / 32 == ISSUER) {
     tc_fence_after();
     tmem_dealloc(a.tmem, TMEM_COLS);
   }
@@ -536,20 +536,33 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
   cta_begin(a);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int4* chunks = reinterpret_cast<const int4*>(p.chunks);
-  if (warp == WORKERS / 32) {
-    const bool one = lane == 0;
-    // the stage of chunk n is free when the chunk's last product has read it
-    auto refill = [&](int n) {
-      if (n < 0 || n + STAGES >= a.c1 - a.c0) return;
-      a.wait1(&a.bars->done[OUT ? 3 : 2], n & 1, 2);
-      load_stage(p, a, &mk, &mq, &mv, a.c0 + n + STAGES, n % STAGES);
-    };
+  constexpr int FIRST = MEET + (SAVE ? 32 : 0);    // whom barrier 1 brings together
+  if (warp == LOADER) {
+    const bool one = xb_elect_one();
+    const int steps = a.c1 - a.c0;
     for (int n = 0; n < STAGES; ++n)
-      if (one && a.c0 + n < a.c1) load_stage(p, a, &mk, &mq, &mv, a.c0 + n, n);
+      if (one && n < steps) load_stage(p, a, &mk, &mq, &mv, a.c0 + n, n);
+    for (int n = 0; n < steps; ++n) {
+      if (SAVE) {
+        bar(1, FIRST);
+        if (one) keep_tiles(p, a, p.s_tiles, p.u_tiles, a.c0 + n, n > 0 ? a.c0 + n - 1 : -1);
+      }
+      if (one && n + STAGES < steps) {         // the stage is free when the chunk's last product has read it
+        a.wait1(&a.bars->done[OUT ? 3 : 2], n & 1, 2);
+        load_stage(p, a, &mk, &mq, &mv, a.c0 + n + STAGES, n % STAGES);
+      }
+      __syncwarp();
+    }
+    if (SAVE && steps > 0) {
+      bar(1, FIRST);
+      if (one) keep_tiles(p, a, p.s_tiles, p.u_tiles, -1, a.c1 - 1);
+    }
+  } else if (warp == ISSUER) {
+    const bool one = xb_elect_one();
     for (int n = 0; n < a.c1 - a.c0; ++n) {
       const uint32_t st = xb_smem_u32(a.smem + (n % STAGES) * STAGE), b1 = xb_smem_u32(a.smem + L::SM_S), b2 = xb_smem_u32(a.smem + L::SM_B2),
                      b3 = xb_smem_u32(a.smem + L::SM_B3);
-      bar(1, THREADS);
+      bar(1, FIRST);
       if (one) {
         a.wait1(&a.bars->full[n % STAGES], (n / STAGES) & 1, 1);
         tc_fence_after();
@@ -558,20 +571,17 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
         for (int k = 0; k < 8; ++k)
           tc_mma_f16_ss(a.tmem + D1, xb_smem_desc(KMAJ, st + ST_KQ + (k >> 2) * HALF + (k & 3) * 32), xb_smem_desc(MNMAJ, b1 + k * 2048), id, k > 0);
         tc_commit(&a.bars->done[0]);
-        if (SAVE) keep_tiles(p, a, p.s_tiles, p.u_tiles, a.c0 + n, n > 0 ? a.c0 + n - 1 : -1);
-        if (STAGES == 2) refill(n - 1);
       }
-      bar(2, THREADS);
+      bar(2, MEET);
       if (one) {
         tc_fence_after();
-        if (SAVE) tma_store_wait_read<0>();
         constexpr uint32_t id = xb_idesc(1, 1, 128, 64, 0, 1);
 #pragma unroll
         for (int k = 0; k < 8; ++k)
           tc_mma_f16_ss(a.tmem + D2, xb_smem_desc(KMAJ, st + ST_TP + (k >> 2) * TP_PLANE + (k & 3) * 32), xb_smem_desc(MNMAJ, b2 + (k & 3) * 2048), id, k > 0);
         tc_commit(&a.bars->done[1]);
       }
-      bar(3, THREADS);
+      bar(3, MEET);
       if (one) {
         tc_fence_after();
         constexpr uint32_t id = xb_idesc(1, 1, 128, 64, 1, 1);
@@ -581,7 +591,7 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
         tc_commit(&a.bars->done[2]);
       }
       if (OUT) {
-        bar(4, THREADS);
+        bar(4, MEET);
         if (one) {
           tc_fence_after();
           constexpr uint32_t id = xb_idesc(1, 1, 128, 64, 0, 1);
@@ -592,16 +602,9 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
           tc_commit(&a.bars->done[3]);
         }
       }
-      if (STAGES == 1 && one) refill(n);
       __syncwarp();
     }
-    if (SAVE && a.c0 < a.c1) {
-      bar(1, THREADS);
-      if (one) {
-        keep_tiles(p, a, p.s_tiles, p.u_tiles, -1, a.c1 - 1);
-        tma_store_wait_read<0>();
-      }
-    }
+    if (SAVE && a.c0 < a.c1) bar(1, FIRST);
   } else {
     const int q4 = warp & 3, half = warp >> 2, r = q4 * 32 + lane, i = r & 63;
     const bool krow = r < C;
@@ -640,7 +643,7 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       if (ch.y < C) clear_rows(st, ch.y);
       fence_proxy_async_smem();
       tc_fence_before();
-      bar_arrive(1, THREADS);
+      bar_arrive(1, FIRST);
       if (OUT && q4 >= 2 && n > 0) finish(n - 1, old, fo);
       // row factors, and v, while the first product runs
       const float gam = ex2_sum(hd, i), dec = ex2_diff(hd, C - 1, i), last = ex2_sum(hd, C - 1), b = hd[2 * C + i];
@@ -663,7 +666,7 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       }
       fence_proxy_async_smem();
       tc_fence_before();
-      bar_arrive(2, THREADS);
+      bar_arrive(2, MEET);
       a.wait(&a.bars->done[1], n & 1, 5);
       tc_fence_after();
       if (krow) {                            // d rk U, then U itself
@@ -676,10 +679,11 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       }
       fence_proxy_async_smem();
       tc_fence_before();
-      bar_arrive(3, THREADS);
+      bar_arrive(3, MEET);
+      if (SAVE) a.wait(&a.bars->kept, n & 1, 8);          // the tiles on their way out have been read
       if (krow) put_row(a.smem + L::SM_U, i, half, x, hi, lo);
       fence_proxy_async_smem();
-      if (OUT) bar_arrive(4, THREADS);
+      if (OUT) bar_arrive(4, MEET);
       a.wait(&a.bars->done[2], n & 1, 6);
       tc_fence_after();
       float z[16];
@@ -688,7 +692,7 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       for (int e = 0; e < 16; ++e) s[e] = last * s[e] + z[e];
     }
     if (OUT && q4 >= 2 && steps > 0) finish(steps - 1, old, fo);
-    if (SAVE && steps > 0) bar_arrive(1, THREADS);
+    if (SAVE && steps > 0) bar_arrive(1, FIRST);
     if (p.s_out != nullptr) state_row(p.s_out + soff, p.s_k, p.s_v, r, p.dk, half * 16, a.vcols, true, s);
   }
   cta_end(a);
@@ -711,16 +715,32 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
   cta_begin(a);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, steps = a.c1 - a.c0;
   const int4* chunks = reinterpret_cast<const int4*>(p.chunks);
-  if (warp == WORKERS / 32) {
-    const bool one = lane == 0;
-    if (one && steps > 0) load_stage(p, a, &mk, &mq, &my, a.c1 - 1, 0);
-    if (one && steps > 1) load_stage(p, a, &mk, &mq, &my, a.c1 - 2, 1);
+  constexpr int FIRST = MEET + 32;
+  if (warp == LOADER) {
+    const bool one = xb_elect_one();
+    for (int n = 0; n < 2; ++n)
+      if (one && n < steps) load_stage(p, a, &mk, &mq, &my, a.c1 - 1 - n, n);
+    for (int n = 0; n < steps; ++n) {
+      bar(1, FIRST);
+      if (one) keep_tiles(p, a, p.ds_tiles, p.dr_tiles, a.c1 - 1 - n, n > 0 ? a.c1 - n : -1);
+      if (one && n + 2 < steps) {
+        a.wait1(&a.bars->done[2], n & 1, 2);
+        load_stage(p, a, &mk, &mq, &my, a.c1 - 1 - (n + 2), n & 1);
+      }
+      __syncwarp();
+    }
+    if (steps > 0) {
+      bar(1, FIRST);
+      if (one) keep_tiles(p, a, p.ds_tiles, p.dr_tiles, -1, a.c0);
+    }
+  } else if (warp == ISSUER) {
+    const bool one = xb_elect_one();
     for (int n = 0; n < steps; ++n) {
       const uint32_t st = xb_smem_u32(a.smem + (n & 1) * STAGE), b1 = xb_smem_u32(a.smem + L::SM_S), b2 = xb_smem_u32(a.smem + L::SM_B2),
                      b3 = xb_smem_u32(a.smem + L::SM_B3);
       constexpr uint32_t id3 = xb_idesc(1, 1, 128, 64, 1, 1);
       constexpr uint32_t id1 = xb_idesc(1, 1, 64, 64, 0, 1), id2 = xb_idesc(1, 1, 64, 64, 1, 1), id4 = xb_idesc(1, 1, 64, 32, 1, 1);
-      bar(4, THREADS);
+      bar(4, MEET);
       if (one) {
         a.wait1(&a.bars->full[n & 1], (n >> 1) & 1, 1);
         tc_fence_after();
@@ -729,7 +749,7 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
           tc_mma_f16_ss(a.tmem + D4, xb_smem_desc(MNMAJ, st + ST_TP + (k >> 2) * TP_PLANE + HALF / 2 + (k & 3) * 2048),
                         xb_smem_desc(MNMAJ, b2 + HALF / 2 + (k & 3) * 2048), id4, k > 0);
       }
-      bar(1, THREADS);
+      bar(1, FIRST);
       if (one) {
         tc_fence_after();
 #pragma unroll
@@ -739,38 +759,26 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
 #pragma unroll
         for (int k = 4; k < 8; ++k)          // rows of Q
           tc_mma_f16_ss(a.tmem + D3, xb_smem_desc(MNMAJ, st + ST_KQ + k * 2048), xb_smem_desc(MNMAJ, b3 + k * 2048), id3, k > 4);
-        keep_tiles(p, a, p.ds_tiles, p.dr_tiles, a.c1 - 1 - n, n > 0 ? a.c1 - n : -1);
       }
-      bar(2, THREADS);
+      bar(2, MEET);
       if (one) {
         tc_fence_after();
-        tma_store_wait_read<0>();
 #pragma unroll
         for (int k = 0; k < 8; ++k)
           tc_mma_f16_ss(a.tmem + D2, xb_smem_desc(MNMAJ, st + ST_TP + (k >> 2) * TP_PLANE + (k & 3) * 2048), xb_smem_desc(MNMAJ, b2 + (k & 3) * 2048), id2, k > 0);
         tc_commit(&a.bars->done[1]);
       }
-      bar(3, THREADS);
+      bar(3, MEET);
       if (one) {
         tc_fence_after();
 #pragma unroll
         for (int k = 0; k < 4; ++k)          // rows of K
           tc_mma_f16_ss(a.tmem + D3, xb_smem_desc(MNMAJ, st + ST_KQ + k * 2048), xb_smem_desc(MNMAJ, b3 + k * 2048), id3, 1);
         tc_commit(&a.bars->done[2]);
-        if (n + 2 < steps) {
-          a.wait1(&a.bars->done[2], n & 1, 2);
-          load_stage(p, a, &mk, &mq, &my, a.c1 - 1 - (n + 2), n & 1);
-        }
       }
       __syncwarp();
     }
-    if (steps > 0) {
-      bar(1, THREADS);
-      if (one) {
-        keep_tiles(p, a, p.ds_tiles, p.dr_tiles, -1, a.c0);
-        tma_store_wait_read<0>();
-      }
-    }
+    if (steps > 0) bar(1, FIRST);
   } else {
     const int q4 = warp & 3, half = warp >> 2, r = q4 * 32 + lane, i = r & 63;
     const bool krow = r < C;
@@ -801,7 +809,7 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
     if (steps > 0) {
       put_dy(0);
       fence_proxy_async_smem();
-      bar_arrive(4, THREADS);
+      bar_arrive(4, MEET);
     }
     int4 ch = steps > 0 ? chunks[a.c1 - 1] : make_int4(0, 0, 0, 0);
     for (int n = 0; n < steps; ++n) {
@@ -813,7 +821,7 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       put_row(a.smem + L::SM_S, r, half, s, hi, lo);
       fence_proxy_async_smem();
       tc_fence_before();
-      bar_arrive(1, THREADS);
+      bar_arrive(1, FIRST);
       const float last = ex2_sum(hd, C - 1), f1 = ex2_diff(hd, C - 1, ri) * rqk[C + ri];
       const float b = hd[2 * C + ri], f2 = -b * ex2_sum(hd, ri) * rqk[C + ri];
       a.wait(&a.bars->done[0], n & 1, 4);
@@ -828,7 +836,7 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       }
       fence_proxy_async_smem();
       tc_fence_before();
-      bar_arrive(2, THREADS);
+      bar_arrive(2, MEET);
       a.wait(&a.bars->done[1], n & 1, 5);
       tc_fence_after();
       float dr[16];
@@ -840,7 +848,8 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       }
       fence_proxy_async_smem();
       tc_fence_before();
-      bar_arrive(3, THREADS);
+      bar_arrive(3, MEET);
+      a.wait(&a.bars->kept, n & 1, 8);       // the tiles on their way out have been read
       if (lane < 16) {
         put_row(a.smem + L::SM_U, ri, half, dr, hi, lo);
         if (ri < len) {
@@ -857,7 +866,7 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
         ch = chunks[a.c1 - 2 - n];
         put_dy(n + 1);
         fence_proxy_async_smem();
-        bar_arrive(4, THREADS);
+        bar_arrive(4, MEET);
       }
       a.wait(&a.bars->done[2], n & 1, 6);
       tc_fence_after();
@@ -866,7 +875,7 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       for (int e = 0; e < 16; ++e) s[e] = last * s[e] + x[e];
     }
     fence_proxy_async_smem();
-    if (steps > 0) bar_arrive(1, THREADS);
+    if (steps > 0) bar_arrive(1, FIRST);
     if (p.ds_in != nullptr) state_row(p.ds_in + soff, p.s_k, p.s_v, r, p.dk, half * 16, a.vcols, true, s);
   }
   cta_end(a);
