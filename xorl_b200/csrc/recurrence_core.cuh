@@ -59,6 +59,15 @@ __device__ __forceinline__ uint32_t lds32(uint32_t a) {
 __device__ __forceinline__ void sts32(uint32_t a, uint32_t v) {
   asm volatile("st.shared.b32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
 }
+__device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+__device__ __forceinline__ float ldsf(uint32_t a) { return __uint_as_float(lds32(a)); }
+__device__ __forceinline__ float4 ldsf4(uint32_t a) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+  return v;
+}
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
   uint4 v;
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
@@ -114,6 +123,21 @@ __device__ __forceinline__ float ex2_diff(const float* hd, int i, int j) {
   return xb_ex2((hd[i] - hd[j]) + (hd[C + i] - hd[C + j]));
 }
 __device__ __forceinline__ float ex2_sum(const float* hd, int i) { return xb_ex2(hd[i]) * (1.f + 0.6931472f * hd[C + i]); }
+
+// the same from a shared-memory address (pointers into aligned dynamic shared memory become generic ones)
+__device__ __forceinline__ float ex2_diff(uint32_t hd, int i, int j) {
+  return xb_ex2((ldsf(hd + i * 4) - ldsf(hd + j * 4)) + (ldsf(hd + (C + i) * 4) - ldsf(hd + (C + j) * 4)));
+}
+__device__ __forceinline__ float ex2_sum(uint32_t hd, int i) { return xb_ex2(ldsf(hd + i * 4)) * (1.f + 0.6931472f * ldsf(hd + (C + i) * 4)); }
+
+// A bounded wait whose slow path stays out of line: a wait that runs out raises a flag and reports; from then on waits
+// return at once and every role walks to its end.
+__device__ __noinline__ void rec_wait_slow(uint64_t* bar, uint32_t parity, int* abort_flag, int* status, int detail) {
+  mbar_wait(bar, parity, abort_flag, status, XB_K_RECURRENCE, detail);
+}
+__device__ __forceinline__ void rec_wait(uint64_t* bar, uint32_t parity, int* abort_flag, int* status, int detail) {
+  if (!mbar_try_wait(bar, parity)) rec_wait_slow(bar, parity, abort_flag, status, detail);
+}
 
 // state [DKP, NV]: four warps hold DKP / 4 rows each, as accumulators
 template <int DKP>

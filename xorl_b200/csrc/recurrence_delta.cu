@@ -349,12 +349,12 @@ static_assert(sizeof(Bars) <= 128, "barriers");
 struct Cta {
   uint8_t* smem;
   Bars* bars;
-  uint32_t tmem;
+  uint32_t tmem, sm;                         // tensor memory, shared memory
   int h, kh, doc, v0, vcols, c0, c1;
   int sm_s, sm_u;
   int* status;
   __device__ void wait1(uint64_t* b, uint32_t parity, int detail) {         // one thread
-    mbar_wait(b, parity, &bars->abort_flag, status, XB_K_RECURRENCE, detail);
+    rec_wait(b, parity, &bars->abort_flag, status, detail);
   }
   __device__ void wait(uint64_t* b, uint32_t parity, int detail) {          // a whole warp: what follows is collective
     wait1(b, parity, detail);
@@ -390,24 +390,24 @@ __device__ __forceinline__ void keep_tiles(const XbRecArgs& p, const Cta& a, voi
 }
 
 // Rows of K and Q behind the document's end: they hold the next document's, and 0 x Inf is NaN.
-__device__ __forceinline__ void clear_rows(uint8_t* st, int len) {
+__device__ __forceinline__ void clear_rows(uint32_t st, int len) {
   const int n = (C - len) * 8;
   for (int i = threadIdx.x; i < 4 * n; i += WORKERS) {
     const int part = i / n, r = len + (i % n) / 8;
-    reinterpret_cast<uint4*>(st + ST_KQ + part * (HALF / 2) + r * 128)[i & 7] = make_uint4(0, 0, 0, 0);
+    sts128(st + ST_KQ + part * (HALF / 2) + r * 128 + (i & 7) * 16, 0, 0, 0, 0);
   }
 }
 
 // 16 values of a row as [hi | lo] of a [rows][128 bytes] operand tile; columns 16 * half ..
-__device__ __forceinline__ void put_row(uint8_t* tile, int row, int half, const float (&x)[16], uint32_t (&hi)[8], uint32_t (&lo)[8]) {
+__device__ __forceinline__ void put_row(uint32_t tile, int row, int half, const float (&x)[16], uint32_t (&hi)[8], uint32_t (&lo)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) split2(x[2 * i], x[2 * i + 1], hi[i], lo[i]);
-  uint8_t* r = tile + row * 128;
+  const uint32_t r = tile + row * 128;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int u = half * 2 + i;
-    *reinterpret_cast<uint4*>(r + ((u ^ (row & 7)) << 4)) = make_uint4(hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
-    *reinterpret_cast<uint4*>(r + (((u + 4) ^ (row & 7)) << 4)) = make_uint4(lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
+    sts128(r + ((u ^ (row & 7)) << 4), hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
+    sts128(r + (((u + 4) ^ (row & 7)) << 4), lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
   }
 }
 // the sum of an accumulator's two halves, 16 columns of this thread's row
@@ -420,10 +420,10 @@ __device__ __forceinline__ void read_acc(uint32_t addr, float (&x)[16]) {
   for (int i = 0; i < 16; ++i) x[i] = __uint_as_float(a[i]) + __uint_as_float(b[i]);
 }
 // 16 bf16 values of a row of the [64][64 bytes] tile of v or dO
-__device__ __forceinline__ void read_x(const uint8_t* tile, int row, int half, bool on, uint4 (&v)[2]) {
+__device__ __forceinline__ void read_x(uint32_t tile, int row, int half, bool on, uint4 (&v)[2]) {
 #pragma unroll
   for (int i = 0; i < 2; ++i)
-    v[i] = on ? *reinterpret_cast<const uint4*>(tile + swz<4>(row, half * 2 + i)) : make_uint4(0, 0, 0, 0);
+    v[i] = on ? lds128(tile + swz<4>(row, half * 2 + i)) : make_uint4(0, 0, 0, 0);
 }
 __device__ __forceinline__ void floats(const uint4 (&v)[2], float (&x)[16]) {
 #pragma unroll
@@ -469,7 +469,7 @@ __device__ __forceinline__ bool cta_setup(const XbRecArgs& p, Cta& a, uint8_t* r
   const int slices = p.dvp / NV, rep = p.Hv / p.Hk;
   a.smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   a.bars = reinterpret_cast<Bars*>(a.smem + sm_bar);
-  a.sm_s = sm_s, a.sm_u = sm_u;
+  a.sm = xb_smem_u32(a.smem), a.sm_s = sm_s, a.sm_u = sm_u;
   const int sl = blockIdx.x % slices;
   a.h = (blockIdx.x / slices) % p.Hv, a.doc = blockIdx.x / (slices * p.Hv), a.kh = a.h / rep;
   a.v0 = sl * NV, a.vcols = min(NV, p.dv - a.v0);
@@ -635,10 +635,8 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
     int4 ch = steps > 0 ? chunks[a.c0] : make_int4(0, 0, 0, 0), old = ch;
     float fo = 0.f;                          // gamma rq of the chunk before
     for (int n = 0; n < steps; ++n) {
-      uint8_t* st = a.smem + (n % STAGES) * STAGE;
-      const float* hd = reinterpret_cast<const float*>(st + ST_HD);
-      const float* rqk = reinterpret_cast<const float*>(st + ST_RQK);
-      put_row(a.smem + L::SM_S, r, half, s, hi, lo);
+      const uint32_t st = a.sm + (n % STAGES) * STAGE, hd = st + ST_HD, rqk = st + ST_RQK;
+      put_row(a.sm + L::SM_S, r, half, s, hi, lo);
       a.wait(&a.bars->full[n % STAGES], (n / STAGES) & 1, 3);
       if (ch.y < C) clear_rows(st, ch.y);
       fence_proxy_async_smem();
@@ -646,8 +644,8 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       bar_arrive(1, FIRST);
       if (OUT && q4 >= 2 && n > 0) finish(n - 1, old, fo);
       // row factors, and v, while the first product runs
-      const float gam = ex2_sum(hd, i), dec = ex2_diff(hd, C - 1, i), last = ex2_sum(hd, C - 1), b = hd[2 * C + i];
-      const float rq = rqk[i], rk = rqk[C + i];
+      const float gam = ex2_sum(hd, i), dec = ex2_diff(hd, C - 1, i), last = ex2_sum(hd, C - 1), b = ldsf(hd + (2 * C + i) * 4);
+      const float rq = ldsf(rqk + i * 4), rk = ldsf(rqk + (C + i) * 4);
       const int len = ch.y;
       uint4 xv[2];
       read_x(st + ST_X, i, half, krow && i < len, xv);
@@ -662,7 +660,7 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
         const float f = gam * rk;
 #pragma unroll
         for (int e = 0; e < 16; ++e) x[e] = b * (x[e] - f * y[e]);
-        put_row(a.smem + L::SM_B2, i, half, x, hi, lo);
+        put_row(a.sm + L::SM_B2, i, half, x, hi, lo);
       }
       fence_proxy_async_smem();
       tc_fence_before();
@@ -675,13 +673,13 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
         const float f = dec * rk;
 #pragma unroll
         for (int e = 0; e < 16; ++e) z[e] = f * x[e];
-        put_row(a.smem + L::SM_B3, i, half, z, hi, lo);
+        put_row(a.sm + L::SM_B3, i, half, z, hi, lo);
       }
       fence_proxy_async_smem();
       tc_fence_before();
       bar_arrive(3, MEET);
       if (SAVE) a.wait(&a.bars->kept, n & 1, 8);          // the tiles on their way out have been read
-      if (krow) put_row(a.smem + L::SM_U, i, half, x, hi, lo);
+      if (krow) put_row(a.sm + L::SM_U, i, half, x, hi, lo);
       fence_proxy_async_smem();
       if (OUT) bar_arrive(4, MEET);
       a.wait(&a.bars->done[2], n & 1, 6);
@@ -791,20 +789,20 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
     // operands that need dO alone: dO beside Y's tile, gamma rq dO of the third product (threads of Q's rows)
     auto put_dy = [&](int n) {
       const int len = chunks[a.c1 - 1 - n].y;
-      uint8_t* st = a.smem + (n & 1) * STAGE;
+      const uint32_t st = a.sm + (n & 1) * STAGE;
       a.wait(&a.bars->full[n & 1], (n >> 1) & 1, 3);
       if (len < C) clear_rows(st, len);
       if (krow) return;
       uint4 v[2];
       read_x(st + ST_X, i, half, i < len, v);
-      uint8_t* row = a.smem + L::SM_B2 + r * 128;
+      const uint32_t row = a.sm + L::SM_B2 + r * 128;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) *reinterpret_cast<uint4*>(row + (((half * 2 + e) ^ (r & 7)) << 4)) = v[e];
-      const float f = ex2_sum(reinterpret_cast<const float*>(st + ST_HD), i) * reinterpret_cast<const float*>(st + ST_RQK)[i];
+      for (int e = 0; e < 2; ++e) sts128(row + (((half * 2 + e) ^ (r & 7)) << 4), v[e].x, v[e].y, v[e].z, v[e].w);
+      const float f = ex2_sum(st + ST_HD, i) * ldsf(st + ST_RQK + i * 4);
       floats(v, x);
 #pragma unroll
       for (int e = 0; e < 16; ++e) x[e] *= f;
-      put_row(a.smem + L::SM_B3, r, half, x, hi, lo);
+      put_row(a.sm + L::SM_B3, r, half, x, hi, lo);
     };
     if (steps > 0) {
       put_dy(0);
@@ -815,15 +813,13 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
     for (int n = 0; n < steps; ++n) {
       const int len = ch.y;
       const long long t0 = ch.x;
-      uint8_t* st = a.smem + (n & 1) * STAGE;
-      const float* hd = reinterpret_cast<const float*>(st + ST_HD);
-      const float* rqk = reinterpret_cast<const float*>(st + ST_RQK);
-      put_row(a.smem + L::SM_S, r, half, s, hi, lo);
+      const uint32_t st = a.sm + (n & 1) * STAGE, hd = st + ST_HD, rqk = st + ST_RQK;
+      put_row(a.sm + L::SM_S, r, half, s, hi, lo);
       fence_proxy_async_smem();
       tc_fence_before();
       bar_arrive(1, FIRST);
-      const float last = ex2_sum(hd, C - 1), f1 = ex2_diff(hd, C - 1, ri) * rqk[C + ri];
-      const float b = hd[2 * C + ri], f2 = -b * ex2_sum(hd, ri) * rqk[C + ri];
+      const float last = ex2_sum(hd, C - 1), rk = ldsf(rqk + (C + ri) * 4), f1 = ex2_diff(hd, C - 1, ri) * rk;
+      const float b = ldsf(hd + (2 * C + ri) * 4), f2 = -b * ex2_sum(hd, ri) * rk;
       a.wait(&a.bars->done[0], n & 1, 4);
       tc_fence_after();
       {                                      // Y = d rk K dS' + P^T dO
@@ -832,7 +828,7 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
         read_acc(acc + D1, x);
 #pragma unroll
         for (int e = 0; e < 16; ++e) x[e] = f1 * x[e] + __uint_as_float(v[e]);
-        if (lane < 16) put_row(a.smem + L::SM_B2, ri, half, x, hi, lo);
+        if (lane < 16) put_row(a.sm + L::SM_B2, ri, half, x, hi, lo);
       }
       fence_proxy_async_smem();
       tc_fence_before();
@@ -844,14 +840,14 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       if (lane < 16) {                       // -b gamma rk dR
 #pragma unroll
         for (int e = 0; e < 16; ++e) x[e] = f2 * dr[e];
-        put_row(a.smem + L::SM_B3, ri, half, x, hi, lo);
+        put_row(a.sm + L::SM_B3, ri, half, x, hi, lo);
       }
       fence_proxy_async_smem();
       tc_fence_before();
       bar_arrive(3, MEET);
       a.wait(&a.bars->kept, n & 1, 8);       // the tiles on their way out have been read
       if (lane < 16) {
-        put_row(a.smem + L::SM_U, ri, half, dr, hi, lo);
+        put_row(a.sm + L::SM_U, ri, half, dr, hi, lo);
         if (ri < len) {
           bf16* dst = dv + (t0 + ri) * dv_t + half * 16;
 #pragma unroll

@@ -90,8 +90,8 @@ __device__ __forceinline__ void spread(const uint32_t (&t)[2 * N], float (&x)[N]
   }
 }
 // 32 bf16 values of row `row` of a [64][256 bytes] tile in two halves of 64 columns
-__device__ __forceinline__ uint4 tile_unit(const uint8_t* tile, int row, int unit) {
-  return *reinterpret_cast<const uint4*>(tile + (unit >> 3) * T64 + row * 128 + (((unit & 7) ^ (row & 7)) << 4));
+__device__ __forceinline__ uint4 tile_unit(uint32_t tile, int row, int unit) {
+  return lds128(tile + (unit >> 3) * T64 + row * 128 + (((unit & 7) ^ (row & 7)) << 4));
 }
 __device__ __forceinline__ void floats8(const uint4 u, float (&x)[8]) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -103,7 +103,7 @@ __device__ __forceinline__ void floats8(const uint4 u, float (&x)[8]) {
 }
 // acc += f * t over this thread's columns of its row: 8 of every 16, units `unit` + 2 i; returns t . (the same
 // columns of `tile`).  The next 16 columns are on their way while 8 are worked on.
-__device__ __forceinline__ float add_rows(uint32_t addr, const uint8_t* tile, int row, int unit, float f, float (&acc)[8 * WIDE]) {
+__device__ __forceinline__ float add_rows(uint32_t addr, uint32_t tile, int row, int unit, float f, float (&acc)[8 * WIDE]) {
   uint32_t t[2][16];
   float dot[2] = {0.f, 0.f};
   tmem_ld_32x16(addr, t[0]);
@@ -169,9 +169,9 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = bars->tmem;
+  const uint32_t tmem = bars->tmem, sm = xb_smem_u32(smem), srqk = xb_smem_u32(rqk);
   // a wait that runs out raises a flag; from then on waits return at once and every role walks to its end
-  auto wait = [&](uint64_t* b, uint32_t parity, int detail) { mbar_wait(b, parity, &bars->abort_flag, p.status, XB_K_RECURRENCE, detail); };
+  auto wait = [&](uint64_t* b, uint32_t parity, int detail) { rec_wait(b, parity, &bars->abort_flag, p.status, detail); };
 
   if (warp == WORKERS / 32) {
     // ------------------------------------------------ loads ------------------------------------------------
@@ -366,22 +366,22 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
     for (int hh = 0; hh < rep; ++hh) {
       Red& r = red[hh & 1];
       float sdot = 0.f, rv = 0.f;
-      const float* hd = nullptr;
+      uint32_t hd = 0;
       for (int pass = 0; pass < passes; ++pass, ++m) {
-        const uint8_t* dov = smem + L::SM_DOV + (m & 1) * L::DOV;
-        hd = reinterpret_cast<const float*>(dov + 4 * T64);
+        const uint32_t dov = sm + L::SM_DOV + (m & 1) * L::DOV;
+        hd = dov + 4 * T64;
         wwait(&bars->dov_full[m & 1], (m >> 1) & 1, 41);
         for (int sl = pass * 4; sl < min(slices, pass * 4 + 4); ++sl, ++n) {
           const int s = n % L::RING;
-          const uint8_t* st = smem + L::SM_RING + s * L::STAGE;
+          const uint32_t st = sm + L::SM_RING + s * L::STAGE;
           wwait(&bars->full[s], (n / L::RING) & 1, 42);
 #pragma unroll
           for (int i = 0; i < 512 / WORKERS; ++i) {  // <S, dS'>: units of eight columns of a row
             const int sr = i * 64 + (tid >> 2), u = tid & 3;
             const uint32_t hi = (uint32_t)(sr * 128 + ((u ^ (sr & 7)) << 4)), lo = (uint32_t)(sr * 128 + (((u + 4) ^ (sr & 7)) << 4));
             float a[8], al[8], b[8], bl[8];
-            floats8(*reinterpret_cast<const uint4*>(st + L::ST_S + hi), a), floats8(*reinterpret_cast<const uint4*>(st + L::ST_S + lo), al);
-            floats8(*reinterpret_cast<const uint4*>(st + L::ST_DS + hi), b), floats8(*reinterpret_cast<const uint4*>(st + L::ST_DS + lo), bl);
+            floats8(lds128(st + L::ST_S + hi), a), floats8(lds128(st + L::ST_S + lo), al);
+            floats8(lds128(st + L::ST_DS + hi), b), floats8(lds128(st + L::ST_DS + lo), bl);
 #pragma unroll
             for (int e = 0; e < 8; ++e) sdot += (a[e] + al[e]) * (b[e] + bl[e]);
           }
@@ -390,8 +390,8 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
             float v[8], a[8], al[8];
             floats8(tile_unit(dov + 2 * T64, sr, (sl & 3) * 4 + u), v);
             if (DELTA) {
-              floats8(*reinterpret_cast<const uint4*>(st + L::ST_R + sr * 128 + ((u ^ (sr & 7)) << 4)), a);
-              floats8(*reinterpret_cast<const uint4*>(st + L::ST_R + sr * 128 + (((u + 4) ^ (sr & 7)) << 4)), al);
+              floats8(lds128(st + L::ST_R + sr * 128 + ((u ^ (sr & 7)) << 4)), a);
+              floats8(lds128(st + L::ST_R + sr * 128 + (((u + 4) ^ (sr & 7)) << 4)), al);
             } else {
               floats8(tile_unit(dov, sr, (sl & 3) * 4 + u), a);
             }
@@ -404,18 +404,18 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
         if (pass + 1 < passes) arrive(&bars->dov_empty[m & 1]);     // the last one is given back below: its decays are read
       }
       wwait(&bars->red_empty[hh & 1], ((hh >> 1) & 1) ^ 1, 45);
-      if (tid < HD) r.hd[tid] = hd[tid];
+      if (tid < HD) r.hd[tid] = ldsf(hd + tid * 4);
       sdot = warp_sum(sdot);
       if (lane == 0) r.sdot[warp] = sdot;
       rv += __shfl_xor_sync(0xffffffffu, rv, 1);
       rv += __shfl_xor_sync(0xffffffffu, rv, 2);
       if (tid < 4 * C && (tid & 3) == 0) r.rv[tid >> 2] = rv;
-      const float b = hd[2 * C + row], gam = ex2_sum(hd, row), dec = ex2_diff(hd, C - 1, row);
+      const float b = ldsf(hd + (2 * C + row) * 4), gam = ex2_sum(hd, row), dec = ex2_diff(hd, C - 1, row);
       wwait(&bars->acc_full, hh & 1, 43);
       tc_fence_after();
       {
         float er = 0.f, fr = 0.f;
-        const float gi = hd[row], gl = hd[C + row];
+        const float gi = ldsf(hd + row * 4), gl = ldsf(hd + (C + row) * 4);
         const int last = row < len ? row : -1;                        // the row's last column; none behind the end
 #pragma unroll
         for (int i = 0; i < SQUARE; ++i) {
@@ -426,12 +426,16 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
             const float4 a = reinterpret_cast<const float4*>(src)[0], c4 = reinterpret_cast<const float4*>(src)[1];
             dst[0] = a.x, dst[1] = a.y, dst[2] = a.z, dst[3] = a.w, dst[4] = c4.x, dst[5] = c4.y, dst[6] = c4.z, dst[7] = c4.w;
           };
+          auto eight_s = [&](uint32_t src, float (&dst)[8]) {
+            const float4 a = ldsf4(src), c4 = ldsf4(src + 16);
+            dst[0] = a.x, dst[1] = a.y, dst[2] = a.z, dst[3] = a.w, dst[4] = c4.x, dst[5] = c4.y, dst[6] = c4.z, dst[7] = c4.w;
+          };
           tmem_ld_32x16(base + COL_P + hf * 16 * SQUARE + 16 * i, t);
           if (DELTA) tmem_ld_32x16(base + COL_L + hf * 16 * SQUARE + 16 * i, tl);
           eight(qk + 16 * i, qr);
           if (DELTA) eight(kk + 16 * i, kr);
-          eight(hd + j, hi), eight(hd + C + j, lo), eight(rqk + C + j, kj);
-          if (!DELTA) eight(hd + 2 * C + j, bj);
+          eight_s(hd + j * 4, hi), eight_s(hd + (C + j) * 4, lo), eight_s(srqk + (C + j) * 4, kj);
+          if (!DELTA) eight_s(hd + (2 * C + j) * 4, bj);
 #pragma unroll
           for (int e = 0; e < 8; ++e) hi[e] = xb_ex2((gi - hi[e]) + (gl - lo[e]));
           tc_wait_ld();
@@ -464,9 +468,9 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
       {
         const bool on = row < len;                                    // rows behind the end hold other documents' products
         const float f1 = on ? gam * rq : 0.f, f2 = on ? -b * gam * rk : 0.f, f3 = on ? dec * rk * (DELTA ? 1.f : b) : 0.f;
-        const float d1 = add_rows(base + COL_T1 + hf * 16 * WIDE, smem + L::SM_Q, row, cu, f1, aq);
-        const float d2 = DELTA ? add_rows(base + COL_T2 + hf * 16 * WIDE, smem + L::SM_K, row, cu, f2, ak) : 0.f;
-        const float d3 = add_rows(base + COL_T3 + hf * 16 * WIDE, smem + L::SM_K, row, cu, f3, ak);
+        const float d1 = add_rows(base + COL_T1 + hf * 16 * WIDE, sm + L::SM_Q, row, cu, f1, aq);
+        const float d2 = DELTA ? add_rows(base + COL_T2 + hf * 16 * WIDE, sm + L::SM_K, row, cu, f2, ak) : 0.f;
+        const float d3 = add_rows(base + COL_T3 + hf * 16 * WIDE, sm + L::SM_K, row, cu, f3, ak);
         if (act) r.rd[0][hf][row] = d1, r.rd[1][hf][row] = d2, r.rd[2][hf][row] = d3;
       }
       tc_fence_before();
@@ -476,7 +480,7 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
     }
     // Z and W as operand tiles over the ring, whose last tiles have been read; K and Q without rows behind the end
     {
-      uint8_t* t = smem + L::SM_RING + row * 128;
+      const uint32_t t = sm + L::SM_RING + row * 128;
 #pragma unroll
       for (int part = 0; part < (DELTA ? 2 : 1); ++part) {
 #pragma unroll
@@ -488,22 +492,22 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
             split2(part ? aw[DELTA ? i : 0] : az[i], part ? aw[DELTA ? i + 1 : 0] : az[i + 1], hi[e], lo[e]);
           }
           const int off = part * 2 * T64 + ((((j0 >> 3) + 2 * u) ^ (row & 7)) << 4);
-          *reinterpret_cast<uint4*>(t + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          *reinterpret_cast<uint4*>(t + off + T64) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          sts128(t + off, hi[0], hi[1], hi[2], hi[3]);
+          sts128(t + off + T64, lo[0], lo[1], lo[2], lo[3]);
         }
       }
     }
     for (int i = tid; i < 4 * (C - len) * 8; i += WORKERS) {
       const int part = i / ((C - len) * 8), rr = len + (i % ((C - len) * 8)) / 8;
-      reinterpret_cast<uint4*>(smem + L::SM_Q + part * T64 + rr * 128)[i & 7] = make_uint4(0, 0, 0, 0);
+      sts128(sm + L::SM_Q + part * T64 + rr * 128 + (i & 7) * 16, 0, 0, 0, 0);
     }
     fence_proxy_async_smem();
     tc_fence_before();
     arrive(&bars->acc_empty);
     wwait(&bars->last, 0, 44);
     tc_fence_after();
-    add_rows(base + COL_T1 + hf * 16 * WIDE, smem + L::SM_Q, row, cu, 1.f, aq);
-    add_rows(base + COL_T2 + hf * 16 * WIDE, smem + L::SM_K, row, cu, 1.f, ak);
+    add_rows(base + COL_T1 + hf * 16 * WIDE, sm + L::SM_Q, row, cu, 1.f, aq);
+    add_rows(base + COL_T2 + hf * 16 * WIDE, sm + L::SM_K, row, cu, 1.f, ak);
     // gradient through the L2 norms: dq - q^ (q^ . dq), rows of norm below 1e-12 excepted
     float fq = 0.f, fk = 0.f;
     if (p.l2norm) {
@@ -512,7 +516,7 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
       for (int i = 0; i < WIDE; ++i) {
         const int unit = cu + 2 * i;
         float x[8], y[8];
-        floats8(tile_unit(smem + L::SM_Q, row, unit), x), floats8(tile_unit(smem + L::SM_K, row, unit), y);
+        floats8(tile_unit(sm + L::SM_Q, row, unit), x), floats8(tile_unit(sm + L::SM_K, row, unit), y);
 #pragma unroll
         for (int e = 0; e < 8; ++e) sq += x[e] * aq[8 * i + e], sk += y[e] * ak[8 * i + e];
       }
@@ -531,7 +535,7 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
         const int unit = cu + 2 * i, col = unit * 8;
         if (col < p.dk) {
           float x[8], y[8];
-          floats8(tile_unit(smem + L::SM_Q, row, unit), x), floats8(tile_unit(smem + L::SM_K, row, unit), y);
+          floats8(tile_unit(sm + L::SM_Q, row, unit), x), floats8(tile_unit(sm + L::SM_K, row, unit), y);
 #pragma unroll
           for (int e = 0; e < 8; ++e)
             x[e] = aq[8 * i + e] - fq * x[e], y[e] = ak[8 * i + e] - fk * y[e];

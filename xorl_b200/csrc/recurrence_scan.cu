@@ -132,9 +132,9 @@ scan_seq(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtenso
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = bars->tmem;
+  const uint32_t tmem = bars->tmem, sm = xb_smem_u32(smem);
   // a wait that runs out raises a flag; from then on waits return at once and every role walks to its end
-  auto wait = [&](uint64_t* b, uint32_t parity, int detail) { mbar_wait(b, parity, &bars->abort_flag, p.status, XB_K_RECURRENCE, detail); };
+  auto wait = [&](uint64_t* b, uint32_t parity, int detail) { rec_wait(b, parity, &bars->abort_flag, p.status, detail); };
   auto wwait = [&](uint64_t* b, uint32_t parity, int detail) {
     wait(b, parity, detail);
     __syncwarp();
@@ -220,23 +220,22 @@ scan_seq(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtenso
     const int t = tid - ADDERS - PMAKERS, row = t & 63, half = t >> 6;
     for (int n = 0; n < steps; ++n) {
       const int s = n & 1, len = chunks[chunk_of(n)].y;
-      uint8_t* st = smem + s * STAGE;
-      const float* hd = reinterpret_cast<const float*>(st + ST_HD);
+      const uint32_t st = sm + s * STAGE, hd = st + ST_HD;
       wwait(&bars->full[s], (n >> 1) & 1, 20);
       // rows behind the document's end hold the next one's: they must not meet a product's zeros (0 x Inf is NaN)
       if (len < C) {
         for (int i = t; i < 5 * (C - len) * 8; i += XMAKERS) {
           const int part = i / ((C - len) * 8), r = len + (i % ((C - len) * 8)) / 8;
-          reinterpret_cast<uint4*>(st + ST_K + part * T64 + r * 128)[i & 7] = make_uint4(0, 0, 0, 0);
+          sts128(st + ST_K + part * T64 + r * 128 + (i & 7) * 16, 0, 0, 0, 0);
         }
         asm volatile("bar.sync 1, %0;" ::"n"(XMAKERS) : "memory");
       }
-      const float f = BWD ? ex2_sum(hd, row) : ex2_diff(hd, C - 1, row) * hd[2 * C + row];
+      const float f = BWD ? ex2_sum(hd, row) : ex2_diff(hd, C - 1, row) * ldsf(hd + (2 * C + row) * 4);
       uint4 v[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const uint4*>(st + ST_X + row * 128 + (((half * 4 + u) ^ (row & 7)) << 4));
+      for (int u = 0; u < 4; ++u) v[u] = lds128(st + ST_X + row * 128 + (((half * 4 + u) ^ (row & 7)) << 4));
       wwait(&bars->pd_empty[s], ((n >> 1) & 1) ^ 1, 21);
-      uint8_t* dst = smem + SM_D + s * HALF + half * T64 + row * 128;
+      const uint32_t dst = sm + SM_D + s * HALF + half * T64 + row * 128;
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const uint32_t x[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
@@ -246,8 +245,8 @@ scan_seq(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtenso
           const float2 y = unpack_bf16x2(x[e]);
           split2(f * y.x, f * y.y, hi[e], lo[e]);
         }
-        *reinterpret_cast<uint4*>(dst + ((u ^ (row & 7)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<uint4*>(dst + (((u + 4) ^ (row & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        sts128(dst + ((u ^ (row & 7)) << 4), hi[0], hi[1], hi[2], hi[3]);
+        sts128(dst + (((u + 4) ^ (row & 7)) << 4), lo[0], lo[1], lo[2], lo[3]);
       }
       fence_proxy_async_smem();
       arrive(&bars->pd_full[s]);
@@ -262,22 +261,20 @@ scan_seq(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtenso
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int u = 0; u < 4; ++u)
-          *reinterpret_cast<uint4*>(smem + SM_P + i * HALF + (u >> 1) * T64 + row * 128 + (((4 + m * 2 + (u & 1)) ^ (row & 7)) << 4)) =
-              make_uint4(0, 0, 0, 0);
+          sts128(sm + SM_P + i * HALF + (u >> 1) * T64 + row * 128 + (((4 + m * 2 + (u & 1)) ^ (row & 7)) << 4), 0, 0, 0, 0);
     for (int n = 0; OUT && n < steps; ++n) {
       const int s = n & 1;
-      const uint8_t* st = smem + s * STAGE;
-      const float* hd = reinterpret_cast<const float*>(st + ST_HD);
+      const uint32_t st = sm + s * STAGE, hd = st + ST_HD;
       wwait(&bars->full[s], (n >> 1) & 1, 22);
-      const float gi = hd[row], gl = hd[C + row];
-      const uint8_t* src = st + ST_QK + (j0 >> 5) * T64 + row * 128;
+      const float gi = ldsf(hd + row * 4), gl = ldsf(hd + (C + row) * 4);
+      const uint32_t src = st + ST_QK + (j0 >> 5) * T64 + row * 128;
       float y[16];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int j = j0 + q * 4;
-        const float4 x = *reinterpret_cast<const float4*>(src + ((((j & 31) >> 2) ^ (row & 7)) << 4));
-        const float4 a = *reinterpret_cast<const float4*>(hd + j), b = *reinterpret_cast<const float4*>(hd + C + j);
-        const float4 w = *reinterpret_cast<const float4*>(hd + 2 * C + j);
+        const float4 x = ldsf4(src + ((((j & 31) >> 2) ^ (row & 7)) << 4));
+        const float4 a = ldsf4(hd + j * 4), b = ldsf4(hd + (C + j) * 4);
+        const float4 w = ldsf4(hd + (2 * C + j) * 4);
         y[4 * q] = j <= row ? x.x * w.x * xb_ex2((gi - a.x) + (gl - b.x)) : 0.f;
         y[4 * q + 1] = j + 1 <= row ? x.y * w.y * xb_ex2((gi - a.y) + (gl - b.y)) : 0.f;
         y[4 * q + 2] = j + 2 <= row ? x.z * w.z * xb_ex2((gi - a.z) + (gl - b.z)) : 0.f;
@@ -288,12 +285,12 @@ scan_seq(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtenso
 #pragma unroll
       for (int e = 0; e < 8; ++e) split2(y[2 * e], y[2 * e + 1], hi[e], lo[e]);
       wwait(&bars->pd_empty[s], ((n >> 1) & 1) ^ 1, 23);
-      uint8_t* dst = smem + SM_P + s * HALF + row * 128;
+      const uint32_t dst = sm + SM_P + s * HALF + row * 128;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int off = (((j0 >> 3) + u) ^ (row & 7)) << 4;
-        *reinterpret_cast<uint4*>(dst + off) = make_uint4(hi[4 * u], hi[4 * u + 1], hi[4 * u + 2], hi[4 * u + 3]);
-        *reinterpret_cast<uint4*>(dst + T64 + off) = make_uint4(lo[4 * u], lo[4 * u + 1], lo[4 * u + 2], lo[4 * u + 3]);
+        sts128(dst + off, hi[4 * u], hi[4 * u + 1], hi[4 * u + 2], hi[4 * u + 3]);
+        sts128(dst + T64 + off, lo[4 * u], lo[4 * u + 1], lo[4 * u + 2], lo[4 * u + 3]);
       }
       fence_proxy_async_smem();
       arrive(&bars->pd_full[s]);
@@ -317,12 +314,12 @@ scan_seq(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtenso
       for (int e = 0; e < 8; ++e) split2(x[2 * e], x[2 * e + 1], hi[e], lo[e]);
     };
     auto put = [&]() {                       // the state's row as [hi | lo]
-      uint8_t* dst = smem + SM_S + sl * HALF + r * 128;
+      const uint32_t dst = sm + SM_S + sl * HALF + r * 128;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int u = part * 2 + i;
-        *reinterpret_cast<uint4*>(dst + ((u ^ (r & 7)) << 4)) = make_uint4(hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
-        *reinterpret_cast<uint4*>(dst + (((u + 4) ^ (r & 7)) << 4)) = make_uint4(lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
+        sts128(dst + ((u ^ (r & 7)) << 4), hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
+        sts128(dst + (((u + 4) ^ (r & 7)) << 4), lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
       }
       fence_proxy_async_smem();
       tc_fence_before();
@@ -336,12 +333,11 @@ scan_seq(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtenso
     for (int n = 0; n < steps; ++n) {
       const int s = n & 1;
       const int4 ch = chunks[chunk_of(n)];
-      const uint8_t* st = smem + s * STAGE;
-      const float* hd = reinterpret_cast<const float*>(st + ST_HD);
+      const uint32_t st = sm + s * STAGE, hd = st + ST_HD;
       wwait(&bars->full[s], (n >> 1) & 1, 30);
-      const float f = BWD ? ex2_diff(hd, C - 1, orow) * hd[2 * C + orow] : ex2_sum(hd, orow), last = ex2_sum(hd, C - 1);
+      const float f = BWD ? ex2_diff(hd, C - 1, orow) * ldsf(hd + (2 * C + orow) * 4) : ex2_sum(hd, orow), last = ex2_sum(hd, C - 1);
       uint4 xv = make_uint4(0, 0, 0, 0);
-      if (OUT) xv = *reinterpret_cast<const uint4*>(st + ST_X + orow * 128 + ((u0 ^ (orow & 7)) << 4));
+      if (OUT) xv = lds128(st + ST_X + orow * 128 + ((u0 ^ (orow & 7)) << 4));
       arrive(&bars->empty[s]);
       wwait(&bars->d3_full, n & 1, 31);
       tc_fence_after();
