@@ -29,11 +29,46 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// Pairs of fp32 values: one instruction for two on sm_100.
+struct Pair { uint64_t v; };
+__device__ __forceinline__ Pair pair(float x, float y) {
+  Pair p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(x), "f"(y));
+  return p;
+}
+__device__ __forceinline__ Pair pair(uint32_t x, uint32_t y) {
+  Pair p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "r"(x), "r"(y));
+  return p;
+}
+__device__ __forceinline__ float2 both(Pair p) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p.v));
+  return f;
+}
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
+  asm("add.rn.f32x2 %0, %0, %1;" : "+l"(a.v) : "l"(b.v));
+  return a;
+}
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+  asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(a.v) : "l"(b.v));
+  return a;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c.v) : "l"(a.v), "l"(b.v));
+  return c;
+}
 // two fp32 values as the sums of two bf16 values each
 __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
   hi = pack_bf16x2(x, y);
-  const float2 h = unpack_bf16x2(hi);
-  lo = pack_bf16x2(x - h.x, y - h.y);
+  const float2 r = both(fma2(pair(hi << 16, hi & 0xffff0000u), pair(-1.f, -1.f), pair(x, y)));     // exact
+  lo = pack_bf16x2(r.x, r.y);
+}
+__device__ __forceinline__ void split2(Pair x, uint32_t& hi, uint32_t& lo) {
+  const float2 f = both(x);
+  hi = pack_bf16x2(f.x, f.y);
+  const float2 r = both(fma2(pair(hi << 16, hi & 0xffff0000u), pair(-1.f, -1.f), x));
+  lo = pack_bf16x2(r.x, r.y);
 }
 __device__ __forceinline__ float2 join2(uint32_t hi, uint32_t lo) {
   const float2 h = unpack_bf16x2(hi), l = unpack_bf16x2(lo);

@@ -417,7 +417,10 @@ __device__ __forceinline__ void read_acc(uint32_t addr, float (&x)[16]) {
   tmem_ld_32x16(addr + 32, b);
   tc_wait_ld();
 #pragma unroll
-  for (int i = 0; i < 16; ++i) x[i] = __uint_as_float(a[i]) + __uint_as_float(b[i]);
+  for (int i = 0; i < 16; i += 2) {
+    const float2 f = both(pair(a[i], a[i + 1]) + pair(b[i], b[i + 1]));
+    x[i] = f.x, x[i + 1] = f.y;
+  }
 }
 // 16 bf16 values of a row of the [64][64 bytes] tile of v or dO
 __device__ __forceinline__ void read_x(uint32_t tile, int row, int half, bool on, uint4 (&v)[2]) {

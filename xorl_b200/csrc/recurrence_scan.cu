@@ -242,8 +242,7 @@ scan_seq(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtenso
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float2 y = unpack_bf16x2(x[e]);
-          split2(f * y.x, f * y.y, hi[e], lo[e]);
+          split2(pair(f, f) * pair(x[e] << 16, x[e] & 0xffff0000u), hi[e], lo[e]);
         }
         sts128(dst + ((u ^ (row & 7)) << 4), hi[0], hi[1], hi[2], hi[3]);
         sts128(dst + (((u + 4) ^ (row & 7)) << 4), lo[0], lo[1], lo[2], lo[3]);
@@ -305,13 +304,16 @@ scan_seq(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtenso
     const long long soff = ((long long)doc * p.Hv + h) * p.dk * p.dv + col * p.s_v + r * p.s_k;
     const float* from = BWD ? p.ds_out : p.s_in;
     float* to = BWD ? p.ds_in : p.s_out;
-    float x[16];
+    Pair x[8];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) x[e] = from != nullptr && doc < p.n_docs && r < p.dk && e < cols ? from[soff + e * p.s_v] : 0.f;
+    for (int e = 0; e < 8; ++e) {
+      auto at = [&](int i) { return from != nullptr && doc < p.n_docs && r < p.dk && i < cols ? from[soff + i * p.s_v] : 0.f; };
+      x[e] = pair(at(2 * e), at(2 * e + 1));
+    }
     uint32_t hi[8], lo[8];
     auto split_row = [&]() {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) split2(x[2 * e], x[2 * e + 1], hi[e], lo[e]);
+      for (int e = 0; e < 8; ++e) split2(x[e], hi[e], lo[e]);
     };
     auto put = [&]() {                       // the state's row as [hi | lo]
       const uint32_t dst = sm + SM_S + sl * HALF + r * 128;
@@ -349,7 +351,8 @@ scan_seq(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtenso
         tc_fence_before();
         arrive(&bars->d3_empty);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = last * x[e] + (__uint_as_float(a[e]) + __uint_as_float(b[e]));
+        for (int e = 0; e < 8; ++e)
+          x[e] = fma2(pair(last, last), x[e], pair(a[2 * e], a[2 * e + 1]) + pair(b[2 * e], b[2 * e + 1]));
       }
       if (n + 1 < steps) {
         split_row();
@@ -357,7 +360,7 @@ scan_seq(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtenso
         put();
       }
       if (OUT) {
-        wwait(&bars->out_full[s], (n >> 1) & 1, 33);
+        if (n + 1 == steps) wwait(&bars->out_full[s], (n >> 1) & 1, 33);   // else: the wait above was for the same products
         tc_fence_after();
         uint32_t a[16], b[16], d[16];
         tmem_ld_32x16(base + D1 + s * DSTEP + sl * 64 + part * 16, a);
@@ -368,7 +371,10 @@ scan_seq(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtenso
         arrive(&bars->out_empty[s]);
         float y[8];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) a[e] = __float_as_uint(f * (__uint_as_float(a[e]) + __uint_as_float(b[e])) + __uint_as_float(d[e]));
+        for (int e = 0; e < 16; e += 2) {
+          const float2 z = both(fma2(pair(f, f), pair(a[e], a[e + 1]) + pair(b[e], b[e + 1]), pair(d[e], d[e + 1])));
+          a[e] = __float_as_uint(z.x), a[e + 1] = __float_as_uint(z.y);
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const uint32_t far = __shfl_sync(0xffffffffu, a[8 + e], lane & 15);
@@ -388,8 +394,10 @@ scan_seq(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtenso
     }
     if (to != nullptr && doc < p.n_docs && r < p.dk)
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
-        if (e < cols) to[soff + e * p.s_v] = x[e];
+      for (int e = 0; e < 8; ++e) {
+        const float2 f = both(x[e]);
+        if (2 * e < cols) to[soff + 2 * e * p.s_v] = f.x, to[soff + (2 * e + 1) * p.s_v] = f.y;
+      }
   }
   // after a wait that ran out, loads and products may still be on their way: give them 0.2 s
   if (*(volatile int*)&bars->abort_flag && tid == 0)
