@@ -17,30 +17,36 @@ namespace {
 
 constexpr int WORKERS = 512, THREADS = WORKERS + 96;
 constexpr int PARTS = WORKERS / 128;                // column parts of the wide products: 128 / PARTS columns per warp
+static_assert(WORKERS == 512, "one 16 x 16 block of a state tile per warp");
 constexpr int WIDE = 8 / PARTS, SQUARE = 4 / PARTS;  // pieces of 16 columns of a warp's part
 constexpr int T64 = HALF / 2;                       // 8 KB: [64 rows][128 bytes]
 template <bool DELTA>
 struct Lay {
-  static constexpr int RING = DELTA ? 2 : 3;
+  static constexpr int RING = DELTA ? 3 : 4;
   static constexpr int ST_S = 0, ST_DS = HALF, ST_U = 2 * HALF, ST_R = 2 * HALF + T64;
   static constexpr int STAGE = 2 * HALF + (DELTA ? 2 * T64 : 0);
-  static constexpr int DOV = 4 * T64 + 1024;        // dO, V: 128 columns each; the head's decays
-  static constexpr int SM_Q = 0, SM_K = 2 * T64, SM_RING = 4 * T64, SM_DOV = SM_RING + RING * STAGE, SM_RED = SM_DOV + 2 * DOV;
+  // dO and V of a pass: 128 columns each in one buffer, which the next head's loads wait for; scan: 64 columns in two.
+  // The decays of two heads.
+  static constexpr int SL = DELTA ? 4 : 2, NB = DELTA ? 1 : 2, DOV = SL * T64;
+  static constexpr int SM_Q = 0, SM_K = 2 * T64, SM_RING = 4 * T64, SM_DOV = SM_RING + RING * STAGE, SM_HD = SM_DOV + NB * DOV,
+                       SM_RED = SM_HD + 2 * 1024;
 };
 struct Red {                                        // what meets across warps, one set per head in turn
   float rd[3][PARTS][C];                            // q.t1, k.t2, k.t3 by column part
   float er[PARTS][C], fr[PARTS][C];                 // row sums of dP o P and dL o A by column part (scan: dP o P)
   float ec[4][C], fc[4][C];                         // column sums by row block
-  float rv[C], sdot[WORKERS / 32];
-  float hd[HD];
+  float rv[2][C], sdot[WORKERS / 32];                // dR.v (scan: dO.v) by column half of every slice; <S, dS'> by warp
 };
 struct __align__(8) Bars {
-  uint64_t full[3], empty[3], dov_full[2], dov_empty[2], red_full[2], red_empty[2], qk_full, acc_full, acc_empty, last;
+  uint64_t full[4], empty[4], dov_full[2], dov_empty[2], hd_full[2], hd_empty[2], red_full[2], red_empty[2];
+  uint64_t qk_full, acc_full, t3_empty, set_empty[2], z_full, last;
   uint32_t tmem;
   int abort_flag;
 };
 template <bool DELTA>
 constexpr int smem_bytes() { return Lay<DELTA>::SM_RED + 2 * (int)sizeof(Red) + RQK * 4 + 256 + 1024; }
+// Tensor memory: dP, dL, t1, t2, t3 (scan: dP and t1 of even and odd heads, t3; the next head's products start when t3 has
+// been read).  At the end dq and dk in the places of t1 and t2.
 constexpr int COL_P = 0, COL_L = 64, COL_T1 = 128, COL_T2 = 256, COL_T3 = 384;
 
 __device__ __forceinline__ float parts(const float (&a)[PARTS][C], int t) {
@@ -153,12 +159,17 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
     }
     return;
   }
-  const int slices = p.dvp / NV, passes = (slices + 3) / 4;
+  const int slices = p.dvp / NV, passes = (slices + L::SL - 1) / L::SL;
   if (tid == 0) {
-    for (int i = 0; i < 3; ++i) mbar_init(&bars->full[i], 1), mbar_init(&bars->empty[i], 1 + WORKERS / 32);
-    for (int i = 0; i < 2; ++i) mbar_init(&bars->dov_full[i], 1), mbar_init(&bars->dov_empty[i], 1 + WORKERS / 32);
-    for (int i = 0; i < 2; ++i) mbar_init(&bars->red_full[i], WORKERS / 32), mbar_init(&bars->red_empty[i], 1);
-    mbar_init(&bars->qk_full, 1), mbar_init(&bars->acc_full, 1), mbar_init(&bars->acc_empty, WORKERS / 32), mbar_init(&bars->last, 1);
+    constexpr int NW = WORKERS / 32;
+    for (int i = 0; i < 4; ++i) mbar_init(&bars->full[i], 1), mbar_init(&bars->empty[i], 1 + NW);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars->dov_full[i], 1), mbar_init(&bars->dov_empty[i], 1 + NW);
+      mbar_init(&bars->hd_full[i], 1), mbar_init(&bars->hd_empty[i], NW + 1);
+      mbar_init(&bars->red_full[i], NW), mbar_init(&bars->red_empty[i], 1), mbar_init(&bars->set_empty[i], NW);
+    }
+    mbar_init(&bars->qk_full, 1), mbar_init(&bars->acc_full, 1), mbar_init(&bars->t3_empty, NW), mbar_init(&bars->z_full, NW);
+    mbar_init(&bars->last, 1);
     bars->abort_flag = 0;
     mbar_fence_init();
   }
@@ -186,16 +197,19 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
       for (int hh = 0; hh < rep; ++hh) {
         const int h = kh * rep + hh;
         const long long ch_h = (long long)c * p.Hv + h;
+        wait(&bars->hd_empty[hh & 1], ((hh >> 1) & 1) ^ 1, 19);
+        mbar_expect_tx(&bars->hd_full[hh & 1], HD * 4);
+        bulk_load(smem + L::SM_HD + (hh & 1) * 1024, p.hd + ch_h * HD, HD * 4, &bars->hd_full[hh & 1]);
         for (int pass = 0; pass < passes; ++pass, ++m) {
-          uint8_t* dov = smem + L::SM_DOV + (m & 1) * L::DOV;
-          wait(&bars->dov_empty[m & 1], ((m >> 1) & 1) ^ 1, 20);
-          mbar_expect_tx(&bars->dov_full[m & 1], 4 * T64 + HD * 4);
-          for (int i = 0; i < 2; ++i) {
-            tma_load_3d(dov + i * T64, &my, &bars->dov_full[m & 1], pass * 128 + i * 64, h, ch.x);
-            tma_load_3d(dov + (2 + i) * T64, &mv, &bars->dov_full[m & 1], pass * 128 + i * 64, h, ch.x);
+          const int d = m % L::NB;
+          uint8_t* dov = smem + L::SM_DOV + d * L::DOV;
+          wait(&bars->dov_empty[d], ((m / L::NB) & 1) ^ 1, 20);
+          mbar_expect_tx(&bars->dov_full[d], L::DOV);
+          for (int i = 0; i < L::SL / 2; ++i) {
+            tma_load_3d(dov + i * T64, &my, &bars->dov_full[d], pass * L::SL * NV + i * 64, h, ch.x);
+            tma_load_3d(dov + (L::SL / 2 + i) * T64, &mv, &bars->dov_full[d], pass * L::SL * NV + i * 64, h, ch.x);
           }
-          bulk_load(dov + 4 * T64, p.hd + ch_h * HD, HD * 4, &bars->dov_full[m & 1]);
-          for (int sl = pass * 4; sl < min(slices, pass * 4 + 4); ++sl, ++n) {
+          for (int sl = pass * L::SL; sl < min(slices, pass * L::SL + L::SL); ++sl, ++n) {
             const int s = n % L::RING;
             uint8_t* st = smem + L::SM_RING + s * L::STAGE;
             wait(&bars->empty[s], ((n / L::RING) & 1) ^ 1, 21);
@@ -218,12 +232,14 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
       constexpr uint32_t id64 = xb_idesc(1, 1, 64, 64, 0, 0), id128 = xb_idesc(1, 1, 64, 128, 0, 0);
       int n = 0, m = 0;
       for (int hh = 0; hh < rep; ++hh) {
-        wait(&bars->acc_empty, (hh & 1) ^ 1, 30);
+        wait(&bars->t3_empty, (hh & 1) ^ 1, 30);
+        if (!DELTA) wait(&bars->set_empty[hh & 1], ((hh >> 1) & 1) ^ 1, 34);
+        const uint32_t set = DELTA ? 0 : hh & 1;
         for (int pass = 0; pass < passes; ++pass, ++m) {
-          const uint32_t y0 = xb_smem_u32(smem + L::SM_DOV + (m & 1) * L::DOV), x0 = y0 + 2 * T64;
-          wait(&bars->dov_full[m & 1], (m >> 1) & 1, 31);
-          for (int sl = pass * 4; sl < min(slices, pass * 4 + 4); ++sl, ++n) {
-            const int s = n % L::RING, q = sl & 3;
+          const uint32_t y0 = sm + L::SM_DOV + (m % L::NB) * L::DOV, x0 = y0 + L::DOV / 2;
+          wait(&bars->dov_full[m % L::NB], (m / L::NB) & 1, 31);
+          for (int sl = pass * L::SL; sl < min(slices, pass * L::SL + L::SL); ++sl, ++n) {
+            const int s = n % L::RING, q = sl % L::SL;
             const uint32_t st = xb_smem_u32(smem + L::SM_RING + s * L::STAGE);
             const uint32_t y = y0 + (q >> 1) * T64 + (q & 1) * 64, x = x0 + (q >> 1) * T64 + (q & 1) * 64;
             const bool first = sl == 0;
@@ -236,19 +252,19 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
               product<false>(tmem + COL_T2, st + L::ST_R, st + L::ST_S, id128, first);
               product<false>(tmem + COL_T3, st + L::ST_U, st + L::ST_DS, id128, first);
             } else {
-              step(tmem + COL_P, y, x, id64, first);
-              step(tmem + COL_P, y + 32, x + 32, id64, false);
-              product<true>(tmem + COL_T1, y, st + L::ST_S, id128, first);
+              step(tmem + COL_P + set * 64, y, x, id64, first);
+              step(tmem + COL_P + set * 64, y + 32, x + 32, id64, false);
+              product<true>(tmem + COL_T1 + set * 128, y, st + L::ST_S, id128, first);
               product<true>(tmem + COL_T3, x, st + L::ST_DS, id128, first);
             }
             tc_commit(&bars->empty[s]);
           }
-          tc_commit(&bars->dov_empty[m & 1]);
+          tc_commit(&bars->dov_empty[m % L::NB]);
         }
         tc_commit(&bars->acc_full);
       }
       // dq = Z K, dk = W K + W^T K + Z^T Q, from the sums over the heads
-      wait(&bars->acc_empty, (rep & 1) ^ 1, 33);
+      wait(&bars->z_full, 0, 33);
       tc_fence_after();
       constexpr uint64_t kmaj = xb_smem_desc_base_sw128(16, 1024), mn = xb_smem_desc_base_sw128(T64, 1024);
       constexpr uint32_t idr = xb_idesc(1, 1, 64, 128, 0, 1), idc = xb_idesc(1, 1, 64, 128, 1, 1);
@@ -274,7 +290,8 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
       const int h = kh * rep + hh;
       const long long ch_h = (long long)c * p.Hv + h;
       const Red& r = red[hh & 1];
-      const float* hd = r.hd;
+      const float* hd = reinterpret_cast<const float*>(smem + L::SM_HD + (hh & 1) * 1024);
+      wait(&bars->hd_full[hh & 1], (hh >> 1) & 1, 52);
       wait(&bars->red_full[hh & 1], (hh >> 1) & 1, 51);
       __syncwarp();
       // gradients of the log decay (suffix sums of dG) and of b: two rows per lane
@@ -293,12 +310,12 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
         if (DELTA) {
           x[i] = (double)q1 + (double)e1 - (double)e2 + (double)(bt * g1) - (double)g2 - (double)(bt * k2) - (double)k3;
           tail += k3;
-          db[i] = r.rv[t] - k2 + g1;
+          db[i] = (r.rv[0][t] + r.rv[1][t]) - k2 + g1;
         } else {
           x[i] = (double)q1 + (double)e1 - (double)(bt * e2) - (double)(bt * k3);
           tail += (double)(bt * k3);
           db[i] = e2 + k3;
-          dsum += r.rv[t];
+          if (on) dsum += r.rv[0][t] + r.rv[1][t];
         }
       }
       float sd = lane < WORKERS / 32 ? r.sdot[lane] : 0.f;
@@ -336,7 +353,7 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
         if (lane == 0) p.part[ch_h * 2] = (float)da, p.part[ch_h * 2 + 1] = (float)dsum;
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->red_empty[hh & 1]);
+      if (lane == 0) mbar_arrive(&bars->red_empty[hh & 1]), mbar_arrive(&bars->hd_empty[hh & 1]);
     }
   } else {
     // ------------------------------------------------ workers -----------------------------------------------
@@ -358,6 +375,11 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
       __syncwarp();
       if (lane == 0) mbar_arrive(b);
     };
+    // this warp's 16 x 16 block of the state tiles: row block warp & 7, columns 16 (warp >> 3) ..
+    const int sa_r = (warp & 7) * 16 + (lane & 15), sb_r = (warp & 7) * 16 + (lane & 7) + (lane >> 4) * 8, su = (warp >> 3) * 2;
+    const uint32_t a_off = sa_r * 128, b_off = sb_r * 128;
+    const uint32_t a_hi = ((su + (lane >> 4)) ^ (sa_r & 7)) << 4, a_lo = ((su + (lane >> 4) + 4) ^ (sa_r & 7)) << 4;
+    const uint32_t b_hi = ((su + ((lane >> 3) & 1)) ^ (sb_r & 7)) << 4, b_lo = ((su + ((lane >> 3) & 1) + 4) ^ (sb_r & 7)) << 4;
     wwait(&bars->qk_full, 0, 40);
     const float rq = rqk[row], rk = rqk[C + row];
     const float* qk = p.qk + ((long long)c * p.Hk + kh) * (C * C) + row * C + j0;
@@ -365,54 +387,99 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
     int n = 0, m = 0;
     for (int hh = 0; hh < rep; ++hh) {
       Red& r = red[hh & 1];
-      float sdot = 0.f, rv = 0.f;
-      uint32_t hd = 0;
+      float sd[2][4] = {}, rv[2][4] = {};
+      const uint32_t hd = sm + L::SM_HD + (hh & 1) * 1024, set = DELTA ? 0 : hh & 1;
       for (int pass = 0; pass < passes; ++pass, ++m) {
-        const uint32_t dov = sm + L::SM_DOV + (m & 1) * L::DOV;
-        hd = dov + 4 * T64;
-        wwait(&bars->dov_full[m & 1], (m >> 1) & 1, 41);
-        for (int sl = pass * 4; sl < min(slices, pass * 4 + 4); ++sl, ++n) {
+        const uint32_t dov = sm + L::SM_DOV + (m % L::NB) * L::DOV;
+        wwait(&bars->dov_full[m % L::NB], (m / L::NB) & 1, 41);
+        for (int sl = pass * L::SL; sl < min(slices, pass * L::SL + L::SL); ++sl, ++n) {
           const int s = n % L::RING;
           const uint32_t st = sm + L::SM_RING + s * L::STAGE;
           wwait(&bars->full[s], (n / L::RING) & 1, 42);
+          if (DELTA) {
+            {  // <S, dS'>: a unit of eight columns of a row per thread
+              const int sr = tid >> 2, u = tid & 3;
+              const uint32_t hi = (uint32_t)(sr * 128 + ((u ^ (sr & 7)) << 4)), lo = (uint32_t)(sr * 128 + (((u + 4) ^ (sr & 7)) << 4));
+              float a[8], al[8], b[8], bl[8];
+              floats8(lds128(st + L::ST_S + hi), a), floats8(lds128(st + L::ST_S + lo), al);
+              floats8(lds128(st + L::ST_DS + hi), b), floats8(lds128(st + L::ST_DS + lo), bl);
 #pragma unroll
-          for (int i = 0; i < 512 / WORKERS; ++i) {  // <S, dS'>: units of eight columns of a row
-            const int sr = i * 64 + (tid >> 2), u = tid & 3;
-            const uint32_t hi = (uint32_t)(sr * 128 + ((u ^ (sr & 7)) << 4)), lo = (uint32_t)(sr * 128 + (((u + 4) ^ (sr & 7)) << 4));
-            float a[8], al[8], b[8], bl[8];
-            floats8(lds128(st + L::ST_S + hi), a), floats8(lds128(st + L::ST_S + lo), al);
-            floats8(lds128(st + L::ST_DS + hi), b), floats8(lds128(st + L::ST_DS + lo), bl);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) sdot += (a[e] + al[e]) * (b[e] + bl[e]);
-          }
-          if (tid < 4 * C) {  // dR.v (scan: dO.v)
-            const int sr = tid >> 2, u = tid & 3;
-            float v[8], a[8], al[8];
-            floats8(tile_unit(dov + 2 * T64, sr, (sl & 3) * 4 + u), v);
-            if (DELTA) {
+              for (int e = 0; e < 8; ++e) sd[0][0] += (a[e] + al[e]) * (b[e] + bl[e]);
+            }
+            if (tid < 4 * C) {  // dR.v
+              const int sr = tid >> 2, u = tid & 3;
+              float v[8], a[8], al[8];
+              floats8(tile_unit(dov + L::DOV / 2, sr, (sl % L::SL) * 4 + u), v);
               floats8(lds128(st + L::ST_R + sr * 128 + ((u ^ (sr & 7)) << 4)), a);
               floats8(lds128(st + L::ST_R + sr * 128 + (((u + 4) ^ (sr & 7)) << 4)), al);
-            } else {
-              floats8(tile_unit(dov, sr, (sl & 3) * 4 + u), a);
-            }
-            if (sr < len)
 #pragma unroll
-              for (int e = 0; e < 8; ++e) rv += (DELTA ? a[e] + al[e] : a[e]) * v[e];
+              for (int e = 0; e < 8; ++e) rv[0][0] += (a[e] + al[e]) * v[e];
+            }
+          } else {
+            // <S, dS'> and the rows' dO.v are diagonals of products of 16 x 16 blocks: a block per warp.  (Here the state
+            // tiles are most of what a head reads and the workers' time counts; the delta rule's products take longer
+            // and its tensor pipe has no room: 209 us this way, 221 us with diagonals.)
+            {
+              const uint32_t sa = st + L::ST_S + a_off, da = st + L::ST_DS + b_off;
+              uint32_t ah[4], al[4], bh[4], bl[4];
+              ldsm4(ah, sa + a_hi), ldsm4(al, sa + a_lo), ldsm4(bh, da + b_hi), ldsm4(bl, da + b_lo);
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                mma(sd[e], al, bl[2 * e], bl[2 * e + 1]);
+                mma(sd[e], al, bh[2 * e], bh[2 * e + 1]);
+                mma(sd[e], ah, bl[2 * e], bl[2 * e + 1]);
+                mma(sd[e], ah, bh[2 * e], bh[2 * e + 1]);
+              }
+            }
+            if (warp < 8) {
+              const int rb = warp & 3, ks = warp >> 2, unit = (sl % L::SL) * 4 + ks * 2;
+              const int ra = rb * 16 + (lane & 15), rn = rb * 16 + (lane & 7) + (lane >> 4) * 8;
+              const int ub = unit + ((lane >> 3) & 1), ua = unit + (lane >> 4);
+              uint32_t a4[4], b4[4];
+              ldsm4(b4, dov + L::DOV / 2 + (ub >> 3) * T64 + rn * 128 + (((ub & 7) ^ (rn & 7)) << 4));
+              ldsm4(a4, dov + (ua >> 3) * T64 + ra * 128 + (((ua & 7) ^ (ra & 7)) << 4));
+#pragma unroll
+              for (int e = 0; e < 2; ++e) mma(rv[e], a4, b4[2 * e], b4[2 * e + 1]);
+            }
           }
           arrive(&bars->empty[s]);
         }
-        if (pass + 1 < passes) arrive(&bars->dov_empty[m & 1]);     // the last one is given back below: its decays are read
+        arrive(&bars->dov_empty[m % L::NB]);
       }
       wwait(&bars->red_empty[hh & 1], ((hh >> 1) & 1) ^ 1, 45);
-      if (tid < HD) r.hd[tid] = ldsf(hd + tid * 4);
-      sdot = warp_sum(sdot);
-      if (lane == 0) r.sdot[warp] = sdot;
-      rv += __shfl_xor_sync(0xffffffffu, rv, 1);
-      rv += __shfl_xor_sync(0xffffffffu, rv, 2);
-      if (tid < 4 * C && (tid & 3) == 0) r.rv[tid >> 2] = rv;
+      wwait(&bars->hd_full[hh & 1], (hh >> 1) & 1, 47);
+      if (DELTA) {
+        const float sum = warp_sum(sd[0][0]);
+        if (lane == 0) r.sdot[warp] = sum;
+        float v = rv[0][0];
+        v += __shfl_xor_sync(0xffffffffu, v, 1);
+        v += __shfl_xor_sync(0xffffffffu, v, 2);
+        if (tid < 4 * C && (tid & 3) == 0) r.rv[0][tid >> 2] = v, r.rv[1][tid >> 2] = 0.f;
+      } else {
+        // rows 0 .. 7 of a block from the first column tile, 8 .. 15 from the second
+        const int g = lane >> 2, t = lane & 3;
+        const bool d0 = g == 2 * t, d1 = g == 2 * t + 1;
+        const float sum = warp_sum(d0 ? sd[0][0] + sd[1][2] : d1 ? sd[0][1] + sd[1][3] : 0.f);
+        if (lane == 0) r.sdot[warp] = sum;
+        if (warp < 8 && (d0 || d1)) {
+          float* dst = r.rv[warp >> 2] + (warp & 3) * 16 + g;
+          dst[0] = d0 ? rv[0][0] : rv[0][1];
+          dst[8] = d0 ? rv[1][2] : rv[1][3];
+        }
+      }
       const float b = ldsf(hd + (2 * C + row) * 4), gam = ex2_sum(hd, row), dec = ex2_diff(hd, C - 1, row);
       wwait(&bars->acc_full, hh & 1, 43);
       tc_fence_after();
+      const bool on = row < len;                                      // rows behind the end hold other documents' products
+      const float f1 = on ? gam * rq : 0.f, f2 = on ? -b * gam * rk : 0.f, f3 = on ? dec * rk * (DELTA ? 1.f : b) : 0.f;
+      const float d3 = add_rows(base + COL_T3 + hf * 16 * WIDE, sm + L::SM_K, row, cu, f3, ak);
+      if (!DELTA) {
+        tc_fence_before();
+        arrive(&bars->t3_empty);
+      }
+      const float d1 = add_rows(base + COL_T1 + set * 128 + hf * 16 * WIDE, sm + L::SM_Q, row, cu, f1, aq);
+      const float d2 = DELTA ? add_rows(base + COL_T2 + hf * 16 * WIDE, sm + L::SM_K, row, cu, f2, ak) : 0.f;
+      if (act) r.rd[0][hf][row] = d1, r.rd[1][hf][row] = d2, r.rd[2][hf][row] = d3;
       {
         float er = 0.f, fr = 0.f;
         const float gi = ldsf(hd + row * 4), gl = ldsf(hd + (C + row) * 4);
@@ -430,7 +497,7 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
             const float4 a = ldsf4(src), c4 = ldsf4(src + 16);
             dst[0] = a.x, dst[1] = a.y, dst[2] = a.z, dst[3] = a.w, dst[4] = c4.x, dst[5] = c4.y, dst[6] = c4.z, dst[7] = c4.w;
           };
-          tmem_ld_32x16(base + COL_P + hf * 16 * SQUARE + 16 * i, t);
+          tmem_ld_32x16(base + COL_P + set * 64 + hf * 16 * SQUARE + 16 * i, t);
           if (DELTA) tmem_ld_32x16(base + COL_L + hf * 16 * SQUARE + 16 * i, tl);
           eight(qk + 16 * i, qr);
           if (DELTA) eight(kk + 16 * i, kr);
@@ -465,18 +532,10 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
         er += __shfl_xor_sync(0xffffffffu, er, 16), fr += __shfl_xor_sync(0xffffffffu, fr, 16);
         if (act) r.er[hf][row] = er, r.fr[hf][row] = fr;
       }
-      {
-        const bool on = row < len;                                    // rows behind the end hold other documents' products
-        const float f1 = on ? gam * rq : 0.f, f2 = on ? -b * gam * rk : 0.f, f3 = on ? dec * rk * (DELTA ? 1.f : b) : 0.f;
-        const float d1 = add_rows(base + COL_T1 + hf * 16 * WIDE, sm + L::SM_Q, row, cu, f1, aq);
-        const float d2 = DELTA ? add_rows(base + COL_T2 + hf * 16 * WIDE, sm + L::SM_K, row, cu, f2, ak) : 0.f;
-        const float d3 = add_rows(base + COL_T3 + hf * 16 * WIDE, sm + L::SM_K, row, cu, f3, ak);
-        if (act) r.rd[0][hf][row] = d1, r.rd[1][hf][row] = d2, r.rd[2][hf][row] = d3;
-      }
       tc_fence_before();
-      if (hh + 1 < rep) arrive(&bars->acc_empty);
+      arrive(DELTA ? &bars->t3_empty : &bars->set_empty[set]);
       arrive(&bars->red_full[hh & 1]);
-      arrive(&bars->dov_empty[(m - 1) & 1]);
+      arrive(&bars->hd_empty[hh & 1]);
     }
     // Z and W as operand tiles over the ring, whose last tiles have been read; K and Q without rows behind the end
     {
@@ -503,7 +562,7 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
     }
     fence_proxy_async_smem();
     tc_fence_before();
-    arrive(&bars->acc_empty);
+    arrive(&bars->z_full);
     wwait(&bars->last, 0, 44);
     tc_fence_after();
     add_rows(base + COL_T1 + hf * 16 * WIDE, sm + L::SM_Q, row, cu, 1.f, aq);
