@@ -34,6 +34,8 @@ __device__ __forceinline__ void bar_arrive(int id, int n) {
 }
 
 // ---- prepare -----------------------------------------------------------------------------------------------------
+// One CTA per chunk and key head, two v heads at a time with four warps each.
+constexpr int PT = 256;                     // threads
 constexpr int LS = 72;                      // row stride of L: rows of a fragment fall into different banks
 template <int DKP>
 struct DPrepSmem {
@@ -41,16 +43,16 @@ struct DPrepSmem {
     struct { uint8_t q[C * DKP * 2], k[C * DKP * 2]; };
     float l[2][C * LS];
   };
-  float2 qk[8 * 2 * 128], kk[8 * 2 * 128];  // Q K^T and K K^T, each thread's own fragments
+  float2 qk[8 * 2 * 128], kk[8 * 2 * 128];  // Q K^T and K K^T as fragments, by lane of four warps
   float hd[2][3][C];
-  float rq[C], rk[C];
+  float rq[C], rk[C], part[2][2 * C];
 };
 
 // 64 x 64 values per head to the upper half of its operand tile: two planes of [128 rows][128 bytes] whose 16-byte
 // units are swizzled as the tensor core reads them
 constexpr int TP_PLANE = 128 * 128;
 __device__ __forceinline__ void put_tile(const XbRecArgs& p, const float (&l)[2][C * LS], int c, int h, int heads) {
-  for (int it = threadIdx.x; it < 2 * C * 8; it += 128) {
+  for (int it = threadIdx.x; it < 2 * C * 8; it += PT) {
     const int mm = it / (C * 8), r = (it >> 3) % C, u = it & 7;
     if (mm >= heads) break;
     const float4* src = reinterpret_cast<const float4*>(&l[mm][r * LS + u * 8]);
@@ -110,12 +112,12 @@ __device__ __forceinline__ void block_put(float* dst, const float (&d)[2][4], fl
 // thread, then T21 = -T22 L21 T11 for blocks of 16 and of 32.  (Substitution down all 64 rows is 2000 multiply-adds of
 // straight-line code for a thread, which ran at the speed of the instruction cache: 28,000 cycles.)
 __device__ __forceinline__ void invert(float (&l)[2][C * LS]) {
-  const int tid = threadIdx.x, w = tid >> 5, m = tid >> 6;
+  const int tid = threadIdx.x, w = (tid >> 5) & 3, m = tid >> 7;
   float* L = l[m];
-  {
-    const int blk = (tid & 63) >> 4, j = tid & 15;
-    float* D = L + blk * 16 * (LS + 1);
-    float x[16];
+  const int blk = (tid & 63) >> 4, j = tid & 15;
+  float* D = L + blk * 16 * (LS + 1);
+  float x[16];
+  if (w < 2) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       float s0 = i == j ? 1.f : 0.f, s1 = 0.f;
@@ -126,13 +128,15 @@ __device__ __forceinline__ void invert(float (&l)[2][C * LS]) {
       }
       x[i] = s0 + s1;
     }
-    __syncthreads();
+  }
+  __syncthreads();
+  if (w < 2) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) D[i * LS + j] = x[i];
   }
   __syncthreads();
-  {  // blocks of 16: one pair per warp
-    float* T11 = L + (w & 1) * 32 * (LS + 1);
+  if (w < 2) {  // blocks of 16: one pair per warp
+    float* T11 = L + w * 32 * (LS + 1);
     float* L21 = T11 + 16 * LS;
     float* T22 = L21 + 16;
     float d[2][4] = {}, e[2][4] = {};
@@ -145,119 +149,116 @@ __device__ __forceinline__ void invert(float (&l)[2][C * LS]) {
     block_put(L21, e, -1.f);
   }
   __syncthreads();
-  {  // blocks of 32: a warp has 16 of the 32 rows
-    const int i = w & 1;
+  {  // blocks of 32: a warp has 16 of the 32 rows and 16 of the 32 columns
+    const int i = w & 1, c = w >> 1;
     float* row = L + (32 + 16 * i) * LS;
-    float d[2][2][4] = {}, e[2][2][4] = {};
-    block_mma(d[0], row, L);
-    block_mma(d[0], row + 16, L + 16 * LS);
-    block_mma(d[1], row + 16, L + 16 * LS + 16);
-    __syncwarp();
-    block_put(row, d[0], 1.f), block_put(row + 16, d[1], 1.f);
+    const float* M = L + 32 * LS + 16 * c;
+    float d[2][4] = {}, e[2][4] = {};
+    if (c == 0) block_mma(d, row, L);
+    block_mma(d, row + 16, L + 16 * LS + 16 * c);
     __syncthreads();
-    const float* M = L + 32 * LS;
-#pragma unroll 1
-    for (int k = 0; k <= i; ++k) {
-      block_mma(e[0], row + 32 + 16 * k, M + 16 * k * LS);
-      block_mma(e[1], row + 32 + 16 * k, M + 16 * k * LS + 16);
-    }
+    block_put(row + 16 * c, d, 1.f);
     __syncthreads();
-    block_put(row, e[0], -1.f), block_put(row + 16, e[1], -1.f);
+    block_mma(e, row + 32, M);
+    if (i) block_mma(e, row + 48, M + 16 * LS);
+    __syncthreads();
+    block_put(row + 16 * c, e, -1.f);
   }
   __syncthreads();
 }
 
 template <int DKP>
-__global__ void __launch_bounds__(128, 4) delta_prep(const XbRecArgs p) {
+__global__ void __launch_bounds__(PT, 3) delta_prep(const XbRecArgs p) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   DPrepSmem<DKP>& sm = *reinterpret_cast<DPrepSmem<DKP>*>(smem_raw);
   constexpr int U = DKP / 8;
   const int kh = blockIdx.x % p.Hk, c = blockIdx.x / p.Hk;
-  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int tid = threadIdx.x, lane = tid & 31, w = (tid >> 5) & 3, m = tid >> 7, g = lane >> 2, t = lane & 3;
   if (c >= p.doc_off[p.n_docs + 2]) return;
   const int4 ch = reinterpret_cast<const int4*>(p.chunks)[c];
   if (ch.z >= p.n_docs) return;
   const int len = ch.y, rep = p.Hv / p.Hk;
   const uint32_t sq = xb_smem_u32(sm.q), sk = xb_smem_u32(sm.k);
-  load_tile<U, C, 128>(sq, (const bf16*)p.q + ch.x * p.q_t + kh * p.q_h, p.q_t, len, p.dk);
-  load_tile<U, C, 128>(sk, (const bf16*)p.k + ch.x * p.k_t + kh * p.k_h, p.k_t, len, p.dk);
+  load_tile<U, C, PT>(sq, (const bf16*)p.q + ch.x * p.q_t + kh * p.q_h, p.q_t, len, p.dk);
+  load_tile<U, C, PT>(sk, (const bf16*)p.k + ch.x * p.k_t + kh * p.k_h, p.k_t, len, p.dk);
   cp_commit();
-  // warps 0 and 1 own the running decay of one head of a pair each: two rows per lane
+  // the first warp of each head's four owns its running decay: two rows per lane
   float gv[2] = {}, bv[2] = {};
   auto read_head = [&](int hh) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int row = 2 * lane + i;
       gv[i] = bv[i] = 0.f;
-      if (w < 2 && hh < rep && row < len) {
+      if (w == 0 && hh < rep && row < len) {
         const long long tok = ch.x + row;
         gv[i] = p.g[tok * p.g_t + (kh * rep + hh) * p.g_h];
         bv[i] = p.b[tok * p.b_t + (kh * rep + hh) * p.b_h];
       }
     }
   };
-  read_head(w);
+  read_head(m);
   cp_wait<0>();
   __syncthreads();
-  {  // row factors: one thread per row of q and of k
-    const int row = tid & 63;
-    const uint32_t base = tid < C ? sq : sk;
-    float ss = 0.f;
-    if (p.l2norm) {
+  if (p.l2norm) {  // sums of squares: two threads per row of q and of k
+    const int row = tid & 63, half = m;
+    const uint32_t base = tid & 64 ? sk : sq;
+    float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const uint4 v = lds128(base + swz<U>(row, u));
-        const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+    for (int u = 0; u < U / 2; ++u) {
+      const uint4 v = lds128(base + swz<U>(row, half * (U / 2) + u));
+      const uint32_t x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 f = unpack_bf16x2(x[i]);
-          ss += f.x * f.x + f.y * f.y;
-        }
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = unpack_bf16x2(x[i]);
+        s0 += f.x * f.x, s1 += f.y * f.y;
       }
     }
-    float r = p.l2norm ? 1.f / fmaxf(sqrtf(ss), 1e-12f) : 1.f;
+    sm.part[half][tid & 127] = s0 + s1;
+    __syncthreads();
+  }
+  if (tid < 2 * C) {
+    const int row = tid & 63;
+    float r = p.l2norm ? 1.f / fmaxf(sqrtf(sm.part[0][tid] + sm.part[1][tid]), 1e-12f) : 1.f;
     if (tid < C) r *= p.scale;
     if (row >= len) r = 0.f;
     (tid < C ? sm.rq : sm.rk)[row] = r;
-    p.rqk[((long long)c * p.Hk + kh) * RQK + (tid < C ? 0 : C) + row] = r;
+    p.rqk[((long long)c * p.Hk + kh) * RQK + tid] = r;
   }
   __syncthreads();
   const int r0 = w * 16 + g;
-  float* qkg = p.qk == nullptr ? nullptr : p.qk + ((long long)c * p.Hk + kh) * (C * C);
-  float* kkg = p.kk == nullptr ? nullptr : p.kk + ((long long)c * p.Hk + kh) * (C * C);
+  {  // Q K^T by the first four warps, K K^T by the others
+    float* out = m ? p.kk : p.qk;
+    if (out != nullptr) out += ((long long)c * p.Hk + kh) * (C * C);
+    const uint32_t sa = m ? sk : sq;
+    const float* ra = m ? sm.rk : sm.rq;
+    float2* keep = m ? sm.kk : sm.qk;
 #pragma unroll
-  for (int nt = 0; nt < 8; nt += 2) {
-    if (nt * 8 > w * 16 + 15) break;              // columns above the diagonal block are never read
-    float a1[2][4] = {}, a2[2][4] = {};
+    for (int nt = 0; nt < 8; nt += 2) {
+      if (nt * 8 > w * 16 + 15) break;              // columns above the diagonal block are never read
+      float a1[2][4] = {};
 #pragma unroll
-    for (int ks = 0; ks < DKP / 16; ++ks) {
-      uint32_t fq[4], fk[4], fb[4];
-      ldsm4(fb, sk + addr_b<U>(nt * 8, ks * 16));
-      ldsm4(fq, sq + addr_a<U>(w * 16, ks * 16));
-      ldsm4(fk, sk + addr_a<U>(w * 16, ks * 16));
-      mma(a1[0], fq, fb[0], fb[1]);
-      mma(a1[1], fq, fb[2], fb[3]);
-      mma(a2[0], fk, fb[0], fb[1]);
-      mma(a2[1], fk, fb[2], fb[3]);
-    }
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
-        const int row = r0 + hh * 8, col = (nt + j) * 8 + 2 * t;
-        const float c0 = sm.rk[col], c1 = sm.rk[col + 1], fq = sm.rq[row], fk = sm.rk[row];
-        const float2 x = make_float2(fq * c0 * a1[j][2 * hh], fq * c1 * a1[j][2 * hh + 1]);
-        const float2 y = make_float2(fk * c0 * a2[j][2 * hh], fk * c1 * a2[j][2 * hh + 1]);
-        sm.qk[((nt + j) * 2 + hh) * 128 + tid] = x;
-        sm.kk[((nt + j) * 2 + hh) * 128 + tid] = y;
-        if (qkg != nullptr) {
-          *reinterpret_cast<float2*>(qkg + row * C + col) = x;
-          *reinterpret_cast<float2*>(kkg + row * C + col) = y;
-        }
+      for (int ks = 0; ks < DKP / 16; ++ks) {
+        uint32_t fa[4], fb[4];
+        ldsm4(fb, sk + addr_b<U>(nt * 8, ks * 16));
+        ldsm4(fa, sa + addr_a<U>(w * 16, ks * 16));
+        mma(a1[0], fa, fb[0], fb[1]);
+        mma(a1[1], fa, fb[2], fb[3]);
       }
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          const int row = r0 + hh * 8, col = (nt + j) * 8 + 2 * t;
+          const float2 rc = *reinterpret_cast<const float2*>(&sm.rk[col]);
+          const float2 x = make_float2(ra[row] * rc.x * a1[j][2 * hh], ra[row] * rc.y * a1[j][2 * hh + 1]);
+          keep[((nt + j) * 2 + hh) * 128 + w * 32 + lane] = x;
+          if (out != nullptr) *reinterpret_cast<float2*>(out + row * C + col) = x;
+        }
+    }
   }
   for (int h0 = 0; h0 < rep; h0 += 2) {
-    if (w < 2 && h0 + w < rep) {
+    const bool on = h0 + m < rep;
+    if (w == 0 && on) {
       double x[2], s = 0.0;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -269,54 +270,49 @@ __global__ void __launch_bounds__(128, 4) delta_prep(const XbRecArgs p) {
         const double u = __shfl_up_sync(0xffffffffu, s, o);
         if (lane >= o) s += u;
       }
-      float* out = p.hd + ((long long)c * p.Hv + kh * rep + h0 + w) * HD;
+      float* out = p.hd + ((long long)c * p.Hv + kh * rep + h0 + m) * HD;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int row = 2 * lane + i;
         const double G = i ? s : s - x[1];
         const float hi = (float)G, lo = (float)(G - (double)hi);
         out[row] = hi, out[C + row] = lo, out[2 * C + row] = bv[i];
-        sm.hd[w][0][row] = hi, sm.hd[w][1][row] = lo, sm.hd[w][2][row] = bv[i];
+        sm.hd[m][0][row] = hi, sm.hd[m][1][row] = lo, sm.hd[m][2][row] = bv[i];
       }
     }
-    read_head(h0 + 2 + w);
+    read_head(h0 + 2 + m);
     __syncthreads();                              // also: the tiles, or the pair before, have been read
-#pragma unroll 1
-    for (int m = 0; m < 2; ++m) {
-      if (h0 + m >= rep) break;
+    if (on) {
       const float* hd = sm.hd[m][0];
       // P as the lower half of the operand tile, L for the inverse
       uint8_t* tile = (uint8_t*)p.pt + ((long long)c * p.Hv + kh * rep + h0 + m) * (2 * TP_PLANE) + C * 128;
+      float gh[2], gl[2], bb[2];
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) gh[hh] = hd[r0 + hh * 8], gl[hh] = hd[C + r0 + hh * 8], bb[hh] = hd[2 * C + r0 + hh * 8];
 #pragma unroll
       for (int nt = 0; nt < 8; ++nt) {
         const int col = nt * 8 + 2 * t;
-        if (nt > 2 * w + 1) {                          // blocks above the diagonal
-#pragma unroll
-          for (int hh = 0; hh < 2; ++hh) {
-            const int row = r0 + hh * 8;
-            uint8_t* dst = tile + row * 128 + ((nt ^ (row & 7)) << 4) + t * 4;
-            *reinterpret_cast<uint32_t*>(dst) = 0;
-            *reinterpret_cast<uint32_t*>(dst + TP_PLANE) = 0;
-          }
-          continue;
-        }
+        const bool above = nt > 2 * w + 1;            // blocks above the diagonal
+        const float2 ch = *reinterpret_cast<const float2*>(hd + col), cl = *reinterpret_cast<const float2*>(hd + C + col);
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
           const int row = r0 + hh * 8;
-          const float2 x = sm.qk[(nt * 2 + hh) * 128 + tid], y = sm.kk[(nt * 2 + hh) * 128 + tid];
-          const float d0 = ex2_diff(hd, row, col), d1 = ex2_diff(hd, row, col + 1), b = hd[2 * C + row];
-          uint32_t hi, lo;
-          split2(col <= row ? d0 * x.x : 0.f, col + 1 <= row ? d1 * x.y : 0.f, hi, lo);
+          uint32_t hi = 0, lo = 0;
+          if (!above) {
+            const float2 x = sm.qk[(nt * 2 + hh) * 128 + w * 32 + lane], y = sm.kk[(nt * 2 + hh) * 128 + w * 32 + lane];
+            const float d0 = xb_ex2((gh[hh] - ch.x) + (gl[hh] - cl.x)), d1 = xb_ex2((gh[hh] - ch.y) + (gl[hh] - cl.y)), b = bb[hh];
+            split2(col <= row ? d0 * x.x : 0.f, col + 1 <= row ? d1 * x.y : 0.f, hi, lo);
+            *reinterpret_cast<float2*>(&sm.l[m][row * LS + col]) =
+                make_float2(col < row ? b * d0 * y.x : 0.f, col + 1 < row ? b * d1 * y.y : 0.f);
+          }
           uint8_t* dst = tile + row * 128 + ((nt ^ (row & 7)) << 4) + t * 4;
           *reinterpret_cast<uint32_t*>(dst) = hi;
           *reinterpret_cast<uint32_t*>(dst + TP_PLANE) = lo;
-          *reinterpret_cast<float2*>(&sm.l[m][row * LS + col]) =
-              make_float2(col < row ? b * d0 * y.x : 0.f, col + 1 < row ? b * d1 * y.y : 0.f);
         }
       }
     }
     __syncthreads();
-    invert(sm.l);
+    invert(sm.l);                                 // of a missing second head: values that nobody reads
     put_tile(p, sm.l, c, kh * rep + h0, rep - h0);
   }
 }
@@ -897,7 +893,7 @@ int run(const XbRecArgs& a, const void* x, long long x_t, long long x_h, cudaStr
 template <int DKP>
 int prep(const XbRecArgs& a, cudaStream_t st) {
   if (!rec_configure<delta_prep<DKP>>(sizeof(DPrepSmem<DKP>))) return -5;
-  return rec_launch(delta_prep<DKP>, (long long)a.nc_max * a.Hk, 128, sizeof(DPrepSmem<DKP>), a, st);
+  return rec_launch(delta_prep<DKP>, (long long)a.nc_max * a.Hk, PT, sizeof(DPrepSmem<DKP>), a, st);
 }
 
 }  // namespace
