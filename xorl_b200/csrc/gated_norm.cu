@@ -299,7 +299,9 @@ int run(const Args& a, cudaStream_t st) {
 }
 
 bool bad(const Args& a) {
-  return a.T < 0 || a.groups <= 0 || a.groups > 65535 || a.d <= 0 || a.d % 8 || a.d > 8192 || a.ldx % 8 || a.ldz % 8 || a.lddy % 8;
+  uintptr_t at = 0;
+  for (const void* p : {a.x, a.z, a.dy, (const bf16*)a.y, (const bf16*)a.dx, (const bf16*)a.dz}) at |= (uintptr_t)p;
+  return at % 16 || a.T < 0 || a.groups <= 0 || a.groups > 65535 || a.d <= 0 || a.d % 8 || a.d > 8192 || a.ldx % 8 || a.ldz % 8 || a.lddy % 8;
 }
 
 }  // namespace

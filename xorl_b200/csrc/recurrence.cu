@@ -118,8 +118,12 @@ __global__ void __launch_bounds__(128) rec_reduce(const XbRecArgs p) {
   }
 }
 
+// 16-byte loads: rows of q, k, v and dO, and the states of the delta rule
 bool bad_args(const XbRecArgs& a) {
-  return a.T < 0 || a.n_docs < 0 || a.Hk <= 0 || a.Hv <= 0 || a.Hv % a.Hk || a.dk <= 0 || a.dk > 128 || a.dk % 8 || a.dv <= 0 ||
+  const long long strides = a.q_t | a.q_h | a.k_t | a.k_h | a.v_t | a.v_h | a.dy_t | a.dy_h;
+  uintptr_t at = 0;
+  for (const void* p : {a.q, a.k, a.v, a.dy, (const void*)a.s_in, (const void*)a.s_out, (const void*)a.ds_out, (const void*)a.ds_in}) at |= (uintptr_t)p;
+  return strides % 8 || at % 16 || a.T < 0 || a.n_docs < 0 || a.Hk <= 0 || a.Hv <= 0 || a.Hv % a.Hk || a.dk <= 0 || a.dk > 128 || a.dk % 8 || a.dv <= 0 ||
          a.dv % 8 || a.nc_max < a.T / C + a.n_docs + 2;
 }
 
@@ -129,8 +133,6 @@ int plan(const XbRecArgs& a, cudaStream_t st) {
 }
 
 }  // namespace
-
-XB_API int xb_recurrence_chunk() { return C; }
 
 // The arguments as 64-bit words, in the order of XbRecArgs up to `part`, then T, n_docs, Hk, Hv, dk, dv, nc_max, l2norm.
 static XbRecArgs unpack(const long long* w, float scale) {
@@ -145,7 +147,7 @@ static XbRecArgs unpack(const long long* w, float scale) {
   ptr(a.chunks), ptr(a.doc_off), ptr(a.hd), ptr(a.rqk), ptr(a.qk), ptr(a.kk), ptr(a.pt);
   ptr(a.s_tiles), ptr(a.u_tiles), ptr(a.ds_tiles), ptr(a.dr_tiles), ptr(a.part);
   num(a.T), num(a.n_docs), num(a.Hk), num(a.Hv), num(a.dk), num(a.dv), num(a.nc_max), num(a.l2norm);
-  a.dkp = a.dk <= 64 ? 64 : 128, a.dvp = (a.dv + 63) / 64 * 64;
+  a.dvp = (a.dv + 63) / 64 * 64;
   a.scale = scale;
   a.status = xb_status_ptr();
   return a;

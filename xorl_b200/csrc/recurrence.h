@@ -26,12 +26,12 @@ struct XbRecArgs {
   float* hd;                     // [nc_max, Hv, 192]
   float* rqk;                    // [nc_max, Hk, 128]
   float *qk, *kk;                // [nc_max, Hk, 64, 64] (delta rule: for the backward pass, null without one)
-  void* pt;                      // [nc_max, Hv]: operand tile [T; P T], two planes, 32768 bytes (delta rule only)
+  void* pt;                      // [nc_max, Hv]: operand tile [T; P], two planes, 32768 bytes (delta rule only)
   // operand tiles of [rows][hi 32 | lo 32] bf16, [nc_max, Hv, dvp / 32]: states entering and gradients of those leaving
   // the chunks (16 KB), U and dR (8 KB, delta rule only)
   void *s_tiles, *u_tiles, *ds_tiles, *dr_tiles;
   float* part;                   // [nc_max, Hv, 2] (scan only)
   int* status;                   // filled in by the entry points
-  int T, n_docs, Hk, Hv, dk, dv, dkp, dvp, nc_max, l2norm;   // dkp: 64 or 128, dvp: a multiple of 64
+  int T, n_docs, Hk, Hv, dk, dv, dvp, nc_max, l2norm;   // dvp: dv rounded up to 64
   float scale;
 };

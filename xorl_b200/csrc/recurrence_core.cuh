@@ -19,10 +19,6 @@ __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
                "{%0, %1, %2, %3};"
@@ -70,29 +66,16 @@ __device__ __forceinline__ void split2(Pair x, uint32_t& hi, uint32_t& lo) {
   const float2 r = both(fma2(pair(hi << 16, hi & 0xffff0000u), pair(-1.f, -1.f), x));
   lo = pack_bf16x2(r.x, r.y);
 }
-__device__ __forceinline__ float2 join2(uint32_t hi, uint32_t lo) {
-  const float2 h = unpack_bf16x2(hi), l = unpack_bf16x2(lo);
-  return make_float2(h.x + l.x, h.y + l.y);
-}
-
 // A tile is rows of U 16-byte units; unit u of a row lies at u ^ f(row), so that the eight rows that ldmatrix reads
 // at one unit fall into eight different banks.
 template <int U>
 __device__ __forceinline__ uint32_t swz(int row, int u) {
   return (uint32_t)(row * U + (U == 4 ? (u ^ ((row >> 1) & 3)) : (u ^ (row & 7)))) * 16u;
 }
-// address of two neighbouring bf16 values (col even)
-template <int U>
-__device__ __forceinline__ uint32_t at2(int row, int col) {
-  return swz<U>(row, col >> 3) + (uint32_t)(col & 7) * 2u;
-}
 __device__ __forceinline__ uint32_t lds32(uint32_t a) {
   uint32_t v;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
   return v;
-}
-__device__ __forceinline__ void sts32(uint32_t a, uint32_t v) {
-  asm volatile("st.shared.b32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
 }
 __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
@@ -114,16 +97,6 @@ template <int U>  // A[m][k], k contiguous
 __device__ __forceinline__ uint32_t addr_a(int m0, int k0) {
   const int l = xb_lane();
   return swz<U>(m0 + (l & 15), (k0 >> 3) + (l >> 4));
-}
-template <int U>  // A = X^T, X[k][m], m contiguous (transposing load)
-__device__ __forceinline__ uint32_t addr_at(int m0, int k0) {
-  const int l = xb_lane();
-  return swz<U>(k0 + (l & 7) + (l >> 4) * 8, (m0 >> 3) + ((l >> 3) & 1));
-}
-template <int U>  // B of two 8-wide column tiles, X[k][n], n contiguous (transposing load)
-__device__ __forceinline__ uint32_t addr_bt(int k0, int n0) {
-  const int l = xb_lane();
-  return swz<U>(k0 + (l & 15), (n0 >> 3) + (l >> 4));
 }
 template <int U>  // B of two 8-wide column tiles, X[n][k], k contiguous
 __device__ __forceinline__ uint32_t addr_b(int n0, int k0) {
@@ -149,11 +122,6 @@ __device__ __forceinline__ void load_tile(uint32_t dst, const bf16* src, long lo
     cp16(dst + swz<U>(r, u), ok ? src + r * ld + u * 8 : src, ok);
   }
 }
-template <int THREADS>
-__device__ __forceinline__ void load_floats(uint32_t dst, const float* src, int n) {
-  for (int i = threadIdx.x; i < n / 4; i += THREADS) cp16(dst + i * 16, src + i * 4, true);
-}
-
 __device__ __forceinline__ float ex2_diff(const float* hd, int i, int j) {
   return xb_ex2((hd[i] - hd[j]) + (hd[C + i] - hd[C + j]));
 }
@@ -172,52 +140,6 @@ __device__ __noinline__ void rec_wait_slow(uint64_t* bar, uint32_t parity, int* 
 }
 __device__ __forceinline__ void rec_wait(uint64_t* bar, uint32_t parity, int* abort_flag, int* status, int detail) {
   if (!mbar_try_wait(bar, parity)) rec_wait_slow(bar, parity, abort_flag, status, detail);
-}
-
-// state [DKP, NV]: four warps hold DKP / 4 rows each, as accumulators
-template <int DKP>
-__device__ __forceinline__ void state_to_smem(const float (&s)[DKP / 64][4][4], uint32_t hi, uint32_t lo) {
-  const int lane = xb_lane(), w = (threadIdx.x >> 5) & 3, g = lane >> 2, t = lane & 3;
-#pragma unroll
-  for (int m = 0; m < DKP / 64; ++m)
-#pragma unroll
-    for (int n = 0; n < 4; ++n)
-#pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
-        uint32_t a, b;
-        split2(s[m][n][2 * hh], s[m][n][2 * hh + 1], a, b);
-        const uint32_t off = at2<4>(w * (DKP / 4) + m * 16 + hh * 8 + g, n * 8 + 2 * t);
-        sts32(hi + off, a);
-        sts32(lo + off, b);
-      }
-}
-template <int DKP, bool STORE>
-__device__ __forceinline__ void state_global(float (&s)[DKP / 64][4][4], float* base, long long sk, long long sv, int dk, int cols) {
-  const int lane = xb_lane(), w = (threadIdx.x >> 5) & 3, g = lane >> 2, t = lane & 3;
-#pragma unroll
-  for (int m = 0; m < DKP / 64; ++m)
-#pragma unroll
-    for (int n = 0; n < 4; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int row = w * (DKP / 4) + m * 16 + (e >> 1) * 8 + g, col = n * 8 + 2 * t + (e & 1);
-        const bool ok = row < dk && col < cols;
-        if (STORE) {
-          if (ok) base[row * sk + col * sv] = s[m][n][e];
-        } else {
-          s[m][n][e] = ok ? base[row * sk + col * sv] : 0.f;
-        }
-      }
-}
-// the two bf16 planes of the state tile to global memory, as a tile of [128 rows][hi | lo]
-template <int DKP>
-__device__ __forceinline__ void state_save(uint32_t hi, uint32_t lo, uint8_t* dst) {
-#pragma unroll
-  for (int i = 0; i < 128 * 8 / 128; ++i) {
-    const int idx = i * 128 + (threadIdx.x & 127), r = idx >> 3, u = idx & 7;
-    const uint4 v = r < DKP ? lds128((u >= 4 ? lo : hi) + swz<4>(r, u & 3)) : make_uint4(0, 0, 0, 0);
-    *reinterpret_cast<uint4*>(dst + r * 128 + ((u ^ (r & 7)) << 4)) = v;
-  }
 }
 
 // [T, heads, cols] bf16, boxes of 64 rows of one head

@@ -48,6 +48,13 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     return x
 
 
+def _state(x: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """A state as the kernels read it: contiguous, on a 16-byte boundary."""
+    if x is None or (x.is_contiguous() and x.data_ptr() % 16 == 0):
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
+
+
 @functools.lru_cache(maxsize=256)
 def _layout(T: int, docs: int, Hk: int, Hv: int, dk: int, dv: int, delta: bool, train: bool):
     """Where the workspaces of a call of these sizes lie: (chunks, bytes kept from the forward pass, bytes of the backward
@@ -105,7 +112,7 @@ class _Recurrence(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, g, b, A, D, s_in, cu, delta, scale, l2norm, final):
         global _launches
-        q, k, v = _rows(q), _rows(k), _rows(v)
+        q, k, v, s_in = _rows(q), _rows(k), _rows(v), _state(s_in)
         T, Hk, dk = q.shape
         _, Hv, dv = v.shape
         dev = v.device
@@ -133,7 +140,7 @@ class _Recurrence(torch.autograd.Function):
         _, Hv, dv = v.shape
         dev = q.device
         dy = torch.zeros((T, Hv, dv), dtype=v.dtype, device=dev) if dy is None else _rows(dy)
-        ds_out = None if ds_out is None else ds_out.contiguous()
+        ds_out = _state(ds_out)
         ds_in = torch.empty_like(s_in) if ctx.needs_input_grad[7] else None
         dq = torch.empty((T, Hk, dk), dtype=q.dtype, device=dev)
         dkk = torch.empty((T, Hk, dk), dtype=q.dtype, device=dev)
@@ -186,6 +193,10 @@ def gated_delta_rule_reference(q, k, v, g, beta, cu_seqlens, *, scale: float = 1
                                initial_state=None, return_final_state: bool = False):
     """Tensor-op form of ``gated_delta_rule``, in fp32 chunks."""
     from ..models.gated_deltanet import gated_delta_rule_chunked
+    if v.shape[0] == 0:                                          # no rows: the states pass through
+        S = initial_state.float().clone() if initial_state is not None else v.new_zeros(
+            cu_seqlens.numel() - 1, v.shape[1], q.shape[2], v.shape[2], dtype=torch.float32)
+        return (v.clone(), S) if return_final_state else v.clone()
     qf, kf = q.float(), k.float()
     if qk_l2norm:
         qf, kf = torch.nn.functional.normalize(qf, dim=-1), torch.nn.functional.normalize(kf, dim=-1)
@@ -216,7 +227,7 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     if not _kernel_ok(q, k, v):
         return gated_delta_rule_reference(q, k, v, g, beta, cu_seqlens, scale=scale, qk_l2norm=qk_l2norm,
                                           initial_state=initial_state, return_final_state=return_final_state)
-    s_in = None if initial_state is None else initial_state.float().contiguous()
+    s_in = None if initial_state is None else initial_state.float()
     o, s = _lib.apply(_Recurrence, q, k, v, g.float(), beta.float(), None, None, s_in,
                       _boundaries(cu_seqlens, q.device), True, scale, bool(qk_l2norm), return_final_state)
     return (o, s) if return_final_state else o
@@ -272,7 +283,7 @@ def ssd_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor
     if not _kernel_ok(B, C, x):
         return ssd_scan_reference(x, dt, A, B, C, D, cu_seqlens, initial_state=initial_state,
                                   return_final_state=return_final_state, chunk=chunk)
-    s_in = None if initial_state is None else initial_state.float().contiguous()
+    s_in = None if initial_state is None else initial_state.float()
     y, s = _lib.apply(_Recurrence, C, B, x, None, dt.float(), A.float().contiguous(), D.float().contiguous(), s_in,
                       _boundaries(cu_seqlens, x.device), False, 1.0, False, return_final_state)
     return (y, s) if return_final_state else y
