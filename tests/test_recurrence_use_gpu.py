@@ -312,6 +312,40 @@ def test_serving(op):
 
 
 @pytest.mark.parametrize("op", OPS)
+@pytest.mark.parametrize("hk,hv,dk,dv", [(1, 1, 8, 8), (2, 4, 64, 64), (1, 3, 128, 128), (2, 4, 72, 40), (1, 2, 32, 136)])
+@pytest.mark.parametrize("lens", [[1] * 7, [0, 1, 5, 0, 16, 3], [1, 16, 17, 0, 64, 2, 65, 1, 1, 200, 16] + [1] * 20, [1, 0]],
+                         ids=["ones", "short", "mixed", "two"])
+@pytest.mark.parametrize("outside", [(0, 0), (3, 20), (18, 2)])
+def test_few_tokens_per_document(op, hk, hv, dk, dv, lens, outside):
+    """Documents around the length up to which they go token by token, rows outside them on both sides of it too."""
+    from xorl_b200.ops.recurrence import gated_delta_rule, ssd_scan
+    cuts = [outside[0]]
+    for n in lens:
+        cuts.append(cuts[-1] + n)
+    T = cuts[-1] + outside[1]
+    for state in (False, True):
+        if op == "delta":
+            ts = delta_inputs(T, hk, hv, dk, dv, len(lens), seed=4, state=state)
+            o, S = gated_delta_rule(*ts[:5], boundaries(cuts), scale=0.3, qk_l2norm=state, initial_state=ts[5], return_final_state=True)
+            bits = lambda t: t.view(torch.int16)  # noqa: E731  (long keys: what grows without bound ends as NaN in both)
+            assert torch.equal(bits(o), bits(gated_delta_rule(*ts[:5], boundaries(cuts), scale=0.3, qk_l2norm=state, initial_state=ts[5])))
+            ds = [None if t is None else t.double() for t in ts]
+            if not state:                        # short keys
+                ts[1].div_(dk), ts[0].div_(dk)
+                o, S = gated_delta_rule(*ts[:5], boundaries(cuts), scale=0.3, return_final_state=True)
+                ds = [None if t is None else t.double() for t in ts]
+            ro, rS = oracle_delta(*ds[:5], cuts, 0.3, state, ds[5])
+        else:
+            ts = scan_inputs(T, hk, hv, dk, dv, len(lens), seed=4, state=state)
+            o, S = ssd_scan(*ts[:6], boundaries(cuts), initial_state=ts[6], return_final_state=True)
+            assert torch.equal(o, ssd_scan(*ts[:6], boundaries(cuts), initial_state=ts[6]))
+            ds = [None if t is None else t.double() for t in ts]
+            ro, rS = oracle_scan(*ds[:6], cuts, ds[6])
+        check(o, ro, "o")
+        check(S, rS, "S")
+
+
+@pytest.mark.parametrize("op", OPS)
 def test_long_document_in_two_halves(op):
     ts = inputs(op, T=6000, docs=1, state=False, seed=12)
     rows = [i for i, n in enumerate(NAMES[op]) if n not in ("A", "D", "initial_state")]

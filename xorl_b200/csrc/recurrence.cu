@@ -33,50 +33,46 @@
 namespace {
 
 // ---- plan: chunks of the documents -----------------------------------------------------------------------------
-// Documents 0 .. n-1 lie between the boundaries; n is the tail behind the last boundary, n + 1 the rows before the first.
-__device__ __forceinline__ int2 doc_range(const int* cu, int n, int T, int d) {
-  auto cut = [&](int i) { return min(max(cu[i], 0), T); };
-  if (d == n) return make_int2(cut(n), T);
-  if (d == n + 1) return make_int2(0, cut(0));
-  const int s = cut(d);
-  return make_int2(s, max(s, cut(d + 1)));
-}
-
-__global__ void __launch_bounds__(1024) rec_plan(const int* __restrict__ cu, int n, int T, int nc_max, int4* chunks,
-                                                 int* doc_off, int* status) {
-  __shared__ int warp_tot[32];
-  __shared__ int carry;
+// Documents of at most `step` tokens have no chunks.  The scan counts chunks in the lower 40 bits, documents above.
+__global__ void __launch_bounds__(1024) rec_plan(const int* __restrict__ cu, int n, int T, int nc_max, int step, int4* chunks,
+                                                 int* doc_off, int* doc_list, int* status) {
+  __shared__ long long warp_tot[32];
+  __shared__ long long carry;
+  constexpr long long DOC = 1ll << 40;
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, nd = n + 2;
   if (tid == 0) carry = 0, doc_off[0] = 0;
   __syncthreads();
   for (int base = 0; base < nd; base += 1024) {
     const int d = base + tid;
-    int v = 0;
+    long long v = 0;
     if (d < nd) {
       const int2 r = doc_range(cu, n, T, d);
-      v = (r.y - r.x + C - 1) / C;
+      v = r.y - r.x > step ? (r.y - r.x + C - 1) / C + DOC : 0;
     }
+    const bool some = v != 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, v, o);
+      const long long u = __shfl_up_sync(0xffffffffu, v, o);
       if (lane >= o) v += u;
     }
     if (lane == 31) warp_tot[w] = v;
     __syncthreads();
     if (w == 0) {
-      int t = warp_tot[lane];
+      long long t = warp_tot[lane];
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, t, o);
+        const long long u = __shfl_up_sync(0xffffffffu, t, o);
         if (lane >= o) t += u;
       }
       warp_tot[lane] = t;
     }
     __syncthreads();
-    const int incl = carry + v + (w ? warp_tot[w - 1] : 0);
+    const long long all = carry + v + (w ? warp_tot[w - 1] : 0), incl = all & (DOC - 1);
     // boundaries that overlap would need more chunks than the rows have: what does not fit is left out and reported
     if (d < nd) {
-      doc_off[d + 1] = min(incl, nc_max);
+      doc_off[d + 1] = (int)min(incl, (long long)nc_max);
+      if (some) doc_list[all / DOC] = d;
+      if (d == nd - 1) doc_list[0] = (int)(all / DOC);
       if (incl > nc_max) xb_report(status, XB_ERR_BAD_ARG, XB_K_RECURRENCE, d);
     }
     __syncthreads();
@@ -124,17 +120,17 @@ bool bad_args(const XbRecArgs& a) {
   uintptr_t at = 0;
   for (const void* p : {a.q, a.k, a.v, a.dy, (const void*)a.s_in, (const void*)a.s_out, (const void*)a.ds_out, (const void*)a.ds_in}) at |= (uintptr_t)p;
   return strides % 8 || at % 16 || a.T < 0 || a.n_docs < 0 || a.Hk <= 0 || a.Hv <= 0 || a.Hv % a.Hk || a.dk <= 0 || a.dk > 128 || a.dk % 8 || a.dv <= 0 ||
-         a.dv % 8 || a.nc_max < a.T / C + a.n_docs + 2;
+         a.dv % 8 || a.step < 0 || a.step >= C || a.nc_max < a.T / C + rec_docs(a);
 }
 
 int plan(const XbRecArgs& a, cudaStream_t st) {
-  rec_plan<<<1, 1024, 0, st>>>(a.cu, a.n_docs, a.T, a.nc_max, (int4*)a.chunks, a.doc_off, a.status);
+  rec_plan<<<1, 1024, 0, st>>>(a.cu, a.n_docs, a.T, a.nc_max, a.step, (int4*)a.chunks, a.doc_off, a.doc_list, a.status);
   return cudaGetLastError() == cudaSuccess ? 0 : -11;
 }
 
 }  // namespace
 
-// The arguments as 64-bit words, in the order of XbRecArgs up to `part`, then T, n_docs, Hk, Hv, dk, dv, nc_max, l2norm.
+// The arguments as 64-bit words, in the order of XbRecArgs up to `part`, (without doc_list), then T, n_docs, Hk, Hv, dk, dv, nc_max, l2norm, step.
 static XbRecArgs unpack(const long long* w, float scale) {
   XbRecArgs a{};
   auto ptr = [&](auto& f) { f = reinterpret_cast<std::remove_reference_t<decltype(f)>>(*w++); };
@@ -146,7 +142,8 @@ static XbRecArgs unpack(const long long* w, float scale) {
   ptr(a.o), ptr(a.dq), ptr(a.dk_out), ptr(a.dv_out), ptr(a.dg), ptr(a.db), ptr(a.dA), ptr(a.dD);
   ptr(a.chunks), ptr(a.doc_off), ptr(a.hd), ptr(a.rqk), ptr(a.qk), ptr(a.kk), ptr(a.pt);
   ptr(a.s_tiles), ptr(a.u_tiles), ptr(a.ds_tiles), ptr(a.dr_tiles), ptr(a.part);
-  num(a.T), num(a.n_docs), num(a.Hk), num(a.Hv), num(a.dk), num(a.dv), num(a.nc_max), num(a.l2norm);
+  num(a.T), num(a.n_docs), num(a.Hk), num(a.Hv), num(a.dk), num(a.dv), num(a.nc_max), num(a.l2norm), num(a.step);
+  a.doc_list = a.doc_off + a.n_docs + 3;
   a.dvp = (a.dv + 63) / 64 * 64;
   a.scale = scale;
   a.status = xb_status_ptr();
@@ -158,6 +155,9 @@ XB_API int xb_recurrence_fwd(const long long* words, float scale, int delta, voi
   const XbRecArgs a = unpack(words, scale);
   if (bad_args(a)) return -1;
   cudaStream_t st = (cudaStream_t)stream;
+  if (a.step > 0)
+    if (int rc = xb_recurrence_step(a, delta, st)) return rc;
+  if (a.step > 0 && a.T <= a.step) return 0;                  // no document can be longer
   if (int rc = plan(a, st)) return rc;
   return delta ? xb_delta_fwd(a, st) : xb_scan_fwd(a, st);
 }
@@ -166,7 +166,7 @@ XB_API int xb_recurrence_fwd(const long long* words, float scale, int delta, voi
 XB_API int xb_recurrence_bwd(const long long* words, float scale, int delta, int tiles, void* stream) {
   if (words == nullptr) return -1;
   const XbRecArgs a = unpack(words, scale);
-  if (bad_args(a)) return -1;
+  if (bad_args(a) || a.step > 0) return -1;
   cudaStream_t st = (cudaStream_t)stream;
   if (int rc = delta ? xb_delta_bwd(a, tiles, st) : xb_scan_bwd(a, tiles, st)) return rc;
   if (int rc = xb_recurrence_grad(a, delta, st)) return rc;

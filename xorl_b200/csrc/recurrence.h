@@ -23,6 +23,7 @@ struct XbRecArgs {
   // workspaces
   void* chunks;                  // int4 [nc_max]: first token, tokens, document
   int* doc_off;                  // [n_docs + 3]: first chunk of every document
+  int* doc_list;                 // [n_docs + 3], behind doc_off: how many documents have chunks, and which
   float* hd;                     // [nc_max, Hv, 192]
   float* rqk;                    // [nc_max, Hk, 128]
   float *qk, *kk;                // [nc_max, Hk, 64, 64] (delta rule: for the backward pass, null without one)
@@ -32,6 +33,6 @@ struct XbRecArgs {
   void *s_tiles, *u_tiles, *ds_tiles, *dr_tiles;
   float* part;                   // [nc_max, Hv, 2] (scan only)
   int* status;                   // filled in by the entry points
-  int T, n_docs, Hk, Hv, dk, dv, dvp, nc_max, l2norm;   // dvp: dv rounded up to 64
+  int T, n_docs, Hk, Hv, dk, dv, dvp, nc_max, l2norm, step;   // step: documents of so many tokens at most go token by token; dvp: dv rounded up to 64
   float scale;
 };

@@ -147,6 +147,21 @@ inline int rec_tile_map(CUtensorMap* m, const void* base, int T, int heads, int 
   return xb_make_tmap_3d(m, base, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, T, heads, cols, T > 1 ? ld_t : 8, heads > 1 ? ld_h : 8, C, 1, box, swz);
 }
 
+// Documents 0 .. n-1 lie between the boundaries; n is the tail behind the last boundary, n + 1 the rows before the first.
+__device__ __forceinline__ int2 doc_range(const int* cu, int n, int T, int d) {
+  auto cut = [&](int i) { return min(max(cu[i], 0), T); };
+  if (d == n) return make_int2(cut(n), T);
+  if (d == n + 1) return make_int2(0, cut(0));
+  const int s = cut(d);
+  return make_int2(s, max(s, cut(d + 1)));
+}
+// Documents that the grids of the chunked kernels cover: all, or at most those that are too long to go token by token.
+__host__ __device__ inline int rec_docs(const XbRecArgs& a) { return a.step > 0 ? a.T / (a.step + 1) : a.n_docs + 2; }
+// The document of a grid's `i`-th; -1: none.
+__device__ __forceinline__ int rec_doc(const XbRecArgs& a, int i) {
+  return a.step == 0 ? i : i < a.doc_list[0] ? a.doc_list[1 + i] : -1;
+}
+
 // Dynamic shared memory above 48 KB, once per kernel and device.
 template <auto KERNEL>
 bool rec_configure(int smem) {
@@ -174,6 +189,8 @@ int rec_launch(K kernel, long long blocks, int threads, size_t smem, const XbRec
 // unless they are there, and the state's gradient
 int xb_delta_fwd(const XbRecArgs& a, cudaStream_t st);
 int xb_delta_bwd(const XbRecArgs& a, int tiles, cudaStream_t st);
+// recurrence_step.cu: documents of at most `step` tokens, forward only
+int xb_recurrence_step(const XbRecArgs& a, int delta, cudaStream_t st);
 // recurrence_scan.cu: the same for the scan
 int xb_scan_fwd(const XbRecArgs& a, cudaStream_t st);
 int xb_scan_bwd(const XbRecArgs& a, int tiles, cudaStream_t st);

@@ -470,11 +470,12 @@ __device__ __forceinline__ bool cta_setup(const XbRecArgs& p, Cta& a, uint8_t* r
   a.bars = reinterpret_cast<Bars*>(a.smem + sm_bar);
   a.sm = xb_smem_u32(a.smem), a.sm_s = sm_s, a.sm_u = sm_u;
   const int sl = blockIdx.x % slices;
-  a.h = (blockIdx.x / slices) % p.Hv, a.doc = blockIdx.x / (slices * p.Hv), a.kh = a.h / rep;
+  a.h = (blockIdx.x / slices) % p.Hv, a.doc = rec_doc(p, blockIdx.x / (slices * p.Hv)), a.kh = a.h / rep;
   a.v0 = sl * NV, a.vcols = min(NV, p.dv - a.v0);
-  a.c0 = p.doc_off[a.doc], a.c1 = p.doc_off[a.doc + 1];
+  a.c0 = a.c1 = 0;
+  if (a.doc >= 0) a.c0 = p.doc_off[a.doc], a.c1 = p.doc_off[a.doc + 1];
   a.status = p.status;
-  return a.doc < p.n_docs;
+  return a.doc >= 0 && a.doc < p.n_docs;
 }
 __device__ __forceinline__ void cta_begin(Cta& a) {
   if (threadIdx.x == 0) {
@@ -878,8 +879,9 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
 
 template <auto KERNEL, int SMEM>
 int run(const XbRecArgs& a, const void* x, long long x_t, long long x_h, cudaStream_t st) {
-  const long long blocks = (long long)(a.n_docs + 2) * a.Hv * (a.dvp / NV);
+  const long long blocks = (long long)rec_docs(a) * a.Hv * (a.dvp / NV);
   if (blocks > 0x7fffffffLL) return -4;
+  if (blocks == 0) return 0;
   CUtensorMap mk{}, mq{}, mx{};
   if (a.T > 0 && (rec_tile_map(&mk, a.k, a.T, a.Hk, a.dk, a.k_t, a.k_h, 64, CU_TENSOR_MAP_SWIZZLE_128B) ||
                   rec_tile_map(&mq, a.q, a.T, a.Hk, a.dk, a.q_t, a.q_h, 64, CU_TENSOR_MAP_SWIZZLE_128B) ||

@@ -108,7 +108,8 @@ scan_seq(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtenso
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   Bars* bars = reinterpret_cast<Bars*>(smem + SM_BAR);
   const int blocks = p.dvp / 64, rep = p.Hv / p.Hk;
-  const int cb = blockIdx.x % blocks, h = (blockIdx.x / blocks) % p.Hv, doc = blockIdx.x / (blocks * p.Hv);
+  const int cb = blockIdx.x % blocks, h = (blockIdx.x / blocks) % p.Hv, doc = rec_doc(p, blockIdx.x / (blocks * p.Hv));
+  if (doc < 0) return;
   const int kh = h / rep, v0 = cb * 64, c0 = p.doc_off[doc], steps = p.doc_off[doc + 1] - c0;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int4* chunks = reinterpret_cast<const int4*>(p.chunks);
@@ -412,8 +413,9 @@ scan_seq(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtenso
 
 template <bool BWD, bool OUT, bool KEEP>
 int run(const XbRecArgs& a, const void* x, long long x_t, long long x_h, cudaStream_t st) {
-  const long long blocks = (long long)(a.n_docs + 2) * a.Hv * (a.dvp / 64);
+  const long long blocks = (long long)rec_docs(a) * a.Hv * (a.dvp / 64);
   if (blocks > 0x7fffffffLL) return -4;
+  if (blocks == 0) return 0;
   CUtensorMap mk{}, mq{}, mx{}, mqk{};
   if (a.T > 0 && (rec_tile_map(&mk, a.k, a.T, a.Hk, a.dk, a.k_t, a.k_h, 64, CU_TENSOR_MAP_SWIZZLE_128B) ||
                   rec_tile_map(&mq, a.q, a.T, a.Hk, a.dk, a.q_t, a.q_h, 64, CU_TENSOR_MAP_SWIZZLE_128B) ||

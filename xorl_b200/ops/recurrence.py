@@ -30,6 +30,7 @@ MAX_STATE_ROWS = 128
 # The states of all chunks are kept for the backward pass up to this size (4096 tokens of 32 heads of 128 x 128: 207 MB);
 # a longer call makes them again, which is the forward pass without its outputs once more.
 KEEP_BYTES = 1 << 30
+STEP = 16               # without gradients, documents of at most so many tokens go token by token (csrc/recurrence_step.cu)
 OPERANDS = 32768        # bytes of the operand tile that the delta rule prepares per chunk and head
 
 
@@ -37,7 +38,7 @@ def launch_count() -> int:
     return _launches
 
 
-_Words = ctypes.c_longlong * 55      # the fields of XbRecArgs (csrc/recurrence.cu)
+_Words = ctypes.c_longlong * 56      # the fields of XbRecArgs (csrc/recurrence.cu)
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -56,12 +57,12 @@ def _state(x: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
 
 
 @functools.lru_cache(maxsize=256)
-def _layout(T: int, docs: int, Hk: int, Hv: int, dk: int, dv: int, delta: bool, train: bool):
+def _layout(T: int, docs: int, Hk: int, Hv: int, dk: int, dv: int, delta: bool, train: bool, step: int):
     """Where the workspaces of a call of these sizes lie: (chunks, bytes kept from the forward pass, bytes of the backward
     pass, whether the state tiles are kept, offsets of chunks .. pt, of the kept tiles, of the backward pass's buffers)."""
-    nc = T // CHUNK + docs + 2
+    nc = T // CHUNK + (T // (step + 1) if step else docs + 2)
     square = nc * CHUNK * CHUNK * 4
-    work = [nc * 16, (docs + 3) * 4, nc * Hv * 3 * CHUNK * 4, nc * Hk * 2 * CHUNK * 4,
+    work = [nc * 16, 2 * (docs + 3) * 4, nc * Hv * 3 * CHUNK * 4, nc * Hk * 2 * CHUNK * 4,
             Hk * square if train or not delta else 0, Hk * square if train and delta else 0, nc * Hv * OPERANDS if delta else 0]
     tiles = nc * Hv * (-(-dv // 64) * 2) * TILE
     first = [tiles, tiles // 2 if delta else 0]
@@ -80,7 +81,7 @@ def _layout(T: int, docs: int, Hk: int, Hv: int, dk: int, dv: int, delta: bool, 
     return nc, kept_bytes, later_bytes, keep, tuple(kept), tuple(later)
 
 
-def _words(q, k, v, g, b, A, D, cu, s_in, s_out, ds_out, ds_in, dy, outs, ws, tmp, lay, delta, l2norm):
+def _words(q, k, v, g, b, A, D, cu, s_in, s_out, ds_out, ds_in, dy, outs, ws, tmp, lay, delta, l2norm, step=0):
     """The arguments of the C entry points."""
     T, Hk, dk = q.shape
     _, Hv, dv = v.shape
@@ -99,7 +100,7 @@ def _words(q, k, v, g, b, A, D, cu, s_in, s_out, ds_out, ds_in, dy, outs, ws, tm
                   0 if g is None else g.data_ptr(), b.data_ptr(), *((0, 0) if g is None else g.stride()), bs[0], bs[1],
                   _ptr(A), _ptr(D), cu.data_ptr(), _ptr(s_in), _ptr(s_out), _ptr(ds_out), _ptr(ds_in),
                   *((dv, 1) if delta else (1, dk)), *outs, *work,
-                  T, cu.shape[0] - 1, Hk, Hv, dk, dv, nc, l2norm)
+                  T, cu.shape[0] - 1, Hk, Hv, dk, dv, nc, l2norm, step)
 
 
 def _ptr(t) -> int:
@@ -117,14 +118,16 @@ class _Recurrence(torch.autograd.Function):
         _, Hv, dv = v.shape
         dev = v.device
         docs = cu.shape[0] - 1
-        lay = _layout(T, docs, Hk, Hv, dk, dv, delta, True in ctx.needs_input_grad)
+        train = True in ctx.needs_input_grad
+        step = STEP if not train and T <= STEP * max(docs, 1) else 0
+        lay = _layout(T, docs, Hk, Hv, dk, dv, delta, train, step)
         ws = torch.empty(lay[1], dtype=torch.uint8, device=dev)
         o = torch.empty((T, Hv, dv), dtype=v.dtype, device=dev)
         s_out = torch.empty((docs, Hv, dk, dv) if delta else (docs, Hv, dv, dk), dtype=torch.float32, device=dev) if final else None
         _lib.call_on(dev, "xb_recurrence_fwd", _words(q, k, v, g, b, A, D, cu, s_in, s_out, None, None, None,
-                                                      (o.data_ptr(), 0, 0, 0, 0, 0, 0, 0), ws, None, lay, delta, l2norm),
+                                                      (o.data_ptr(), 0, 0, 0, 0, 0, 0, 0), ws, None, lay, delta, l2norm, step),
                      scale, delta)
-        _launches += 3
+        _launches += 3 if not step else 4 if T > step else 1
         ctx.save_for_backward(q, k, v, g, b, A, D, s_in, cu, ws)
         ctx.conf = (delta, scale, l2norm, lay)
         ctx.set_materialize_grads(False)
