@@ -30,7 +30,9 @@ MAX_STATE_ROWS = 128
 # The states of all chunks are kept for the backward pass up to this size (4096 tokens of 32 heads of 128 x 128: 207 MB);
 # a longer call makes them again, which is the forward pass without its outputs once more.
 KEEP_BYTES = 1 << 30
-STEP = 16               # without gradients, documents of at most so many tokens go token by token (csrc/recurrence_step.cu)
+# Without gradients and with at most so many tokens per document on average, documents of at most so many go token by
+# token (csrc/recurrence_step.cu, which gives the times of both ways), the others through the chunked kernels.
+STEP = 16
 OPERANDS = 32768        # bytes of the operand tile that the delta rule prepares per chunk and head
 
 
