@@ -92,6 +92,17 @@ __device__ __forceinline__ uint4 lds128(uint32_t a) {
   return v;
 }
 
+// 16 x 16 bf16 values from fragments (as ldsm4 reads them)
+__device__ __forceinline__ void stsm4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// 16 rows and 16 columns of an accumulator as fragments: r[4 n + 2 h + e] is row g + 8 h, column 8 n + 2 t + e (g = lane / 4,
+// t = lane % 4).  Of a 64-row accumulator, which lies in 16 lanes of each warp, every thread gets values.
+__device__ __forceinline__ void tmem_ld_frag(uint32_t addr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(addr) : "memory");
+}
+
 // fragment addresses of this lane; m0, n0, k0 are multiples of 8 (16 for the wide ones)
 template <int U>  // A[m][k], k contiguous
 __device__ __forceinline__ uint32_t addr_a(int m0, int k0) {

@@ -16,9 +16,9 @@
 namespace {
 
 constexpr int WORKERS = 512, THREADS = WORKERS + 96;
-constexpr int PARTS = WORKERS / 128;                // column parts of the wide products: 128 / PARTS columns per warp
+constexpr int PARTS = WORKERS / 128;                // column parts of the products, 32 and 16 columns per warp
 static_assert(WORKERS == 512, "one 16 x 16 block of a state tile per warp");
-constexpr int WIDE = 8 / PARTS, SQUARE = 4 / PARTS;  // pieces of 16 columns of a warp's part
+constexpr int WIDE = 8 / PARTS;                     // pieces of 16 columns of a warp's part of the wide products
 constexpr int T64 = HALF / 2;                       // 8 KB: [64 rows][128 bytes]
 template <bool DELTA>
 struct Lay {
@@ -55,6 +55,11 @@ __device__ __forceinline__ float parts(const float (&a)[PARTS][C], int t) {
   for (int i = 2; i < PARTS; i += 2) s += a[i][t] + a[i + 1][t];
   return s;
 }
+__device__ __forceinline__ float2 lds2(uint32_t a) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+  return v;
+}
 __device__ __forceinline__ void wbar() { asm volatile("bar.sync 1, %0;" ::"n"(WORKERS) : "memory"); }
 
 // D (64 x N) += A (64 x 16 of a row of 16-column steps) B^T: one step each
@@ -74,26 +79,27 @@ __device__ __forceinline__ void product(uint32_t d, uint32_t a, uint32_t b, uint
     step(d, a + 96, b + 32, idesc, false);
   }
 }
-// sum over the 16 lanes of a half warp of 8 values each; lane l keeps the sum of value l % 8
-__device__ __forceinline__ float col_sum(float (&v)[8]) {
-  const int l = threadIdx.x & 15;
-#pragma unroll
-  for (int o = 4; o > 0; o >>= 1)
-#pragma unroll
-    for (int i = 0; i < o; ++i) {
-      const float mine = l & o ? v[i + o] : v[i], other = l & o ? v[i] : v[i + o];
-      v[i] = mine + __shfl_xor_sync(0xffffffffu, other, o);
-    }
-  return v[0] + __shfl_xor_sync(0xffffffffu, v[0], 8);
+// Fragments: a thread has rows g and g + 8 of its warp's 16 and, of every 8 columns, 2 t and 2 t + 1.
+// The two rows' sums over the four lanes that share them; lane t keeps the one of row t % 2.
+__device__ __forceinline__ float row_sum(float a, float b) {
+  const bool odd = threadIdx.x & 1;
+  const float v = (odd ? b : a) + __shfl_xor_sync(0xffffffffu, odd ? a : b, 1);
+  return v + __shfl_xor_sync(0xffffffffu, v, 2);
 }
-// A 64-row accumulator lies in lanes 0 .. 15 of each warp; lanes 16 .. 31 take the second half of its 2 N columns.
-template <int N>
-__device__ __forceinline__ void spread(const uint32_t (&t)[2 * N], float (&x)[N]) {
-#pragma unroll
-  for (int e = 0; e < N; ++e) {
-    const uint32_t far = __shfl_sync(0xffffffffu, t[N + e], threadIdx.x & 15);
-    x[e] = __uint_as_float(threadIdx.x & 16 ? far : t[e]);
-  }
+// The same of two sums at once: lanes t < 2 keep the first's, the others the second's.
+__device__ __forceinline__ float row_sum2(const float (&a)[2], const float (&b)[2]) {
+  const bool odd = threadIdx.x & 1, up = threadIdx.x & 2;
+  const float x = (odd ? a[1] : a[0]) + __shfl_xor_sync(0xffffffffu, odd ? a[0] : a[1], 1);
+  const float y = (odd ? b[1] : b[0]) + __shfl_xor_sync(0xffffffffu, odd ? b[0] : b[1], 1);
+  return (up ? y : x) + __shfl_xor_sync(0xffffffffu, up ? x : y, 2);
+}
+// Sums over the eight lanes that share columns; lane g keeps column 8 (g & 1) + 2 t + (g >> 1 & 1) of the 16.
+__device__ __forceinline__ float col_sum(const float (&v)[2][2]) {
+  const bool n = threadIdx.x & 4, e = threadIdx.x & 8;
+  const float x = (n ? v[1][0] : v[0][0]) + __shfl_xor_sync(0xffffffffu, n ? v[0][0] : v[1][0], 4);
+  const float y = (n ? v[1][1] : v[0][1]) + __shfl_xor_sync(0xffffffffu, n ? v[0][1] : v[1][1], 4);
+  const float z = (e ? y : x) + __shfl_xor_sync(0xffffffffu, e ? x : y, 8);
+  return z + __shfl_xor_sync(0xffffffffu, z, 16);
 }
 // 32 bf16 values of row `row` of a [64][256 bytes] tile in two halves of 64 columns
 __device__ __forceinline__ uint4 tile_unit(uint32_t tile, int row, int unit) {
@@ -107,27 +113,34 @@ __device__ __forceinline__ void floats8(const uint4 u, float (&x)[8]) {
     x[2 * j] = f.x, x[2 * j + 1] = f.y;
   }
 }
-// acc += f * t over this thread's columns of its row: 8 of every 16, units `unit` + 2 i; returns t . (the same
-// columns of `tile`).  The next 16 columns are on their way while 8 are worked on.
-__device__ __forceinline__ float add_rows(uint32_t addr, uint32_t tile, int row, int unit, float f, float (&acc)[8 * WIDE]) {
-  uint32_t t[2][16];
-  float dot[2] = {0.f, 0.f};
-  tmem_ld_32x16(addr, t[0]);
+// address of a 16 x 16 block of a [64][256 bytes] tile in two halves of 64 columns, for ldsm4 and stsm4
+__device__ __forceinline__ uint32_t block_addr(uint32_t tile, int r0, int col) {
+  const int l = xb_lane(), unit = (col >> 3) + (l >> 4), row = r0 + (l & 15);
+  return tile + (unit >> 3) * T64 + row * 128 + (((unit & 7) ^ (row & 7)) << 4);
+}
+__device__ __forceinline__ Pair bf16_pair(uint32_t v) { return pair(v << 16, v & 0xffff0000u); }
+// acc += f * t over this thread's rows and columns col .. col + 32; returns t . (the same columns of `tile`)
+__device__ __forceinline__ float add_rows(uint32_t addr, uint32_t tile, int r0, int col, const float (&f)[2], Pair (&acc)[WIDE][2][2]) {
+  uint32_t t[2][8];
+  Pair dot[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
+  tmem_ld_frag(addr, t[0]);
 #pragma unroll
   for (int i = 0; i < WIDE; ++i) {
-    float x[8], y[8];
-    floats8(tile_unit(tile, row, unit + 2 * i), x);
+    uint32_t x[4];
+    ldsm4(x, block_addr(tile, r0, col + 16 * i));
     tc_wait_ld();
-    if (i + 1 < WIDE) tmem_ld_32x16(addr + 16 * (i + 1), t[(i + 1) & 1]);
-    spread<8>(t[i & 1], y);
+    if (i + 1 < WIDE) tmem_ld_frag(addr + 16 * (i + 1), t[(i + 1) & 1]);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      dot[e & 1] += x[e] * y[e];
-      acc[8 * i + e] += f * y[e];
-    }
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const Pair y = pair(t[i & 1][4 * n + 2 * h], t[i & 1][4 * n + 2 * h + 1]);
+        dot[h] = fma2(bf16_pair(x[2 * n + h]), y, dot[h]);
+        acc[i][n][h] = fma2(pair(f[h], f[h]), y, acc[i][n][h]);
+      }
   }
-  const float d = dot[0] + dot[1];
-  return d + __shfl_xor_sync(0xffffffffu, d, 16);
+  const float2 a = both(dot[0]), b = both(dot[1]);
+  return row_sum(a.x + a.y, b.x + b.y);
 }
 
 template <bool DELTA>
@@ -357,16 +370,27 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
     }
   } else {
     // ------------------------------------------------ workers -----------------------------------------------
-    // row `row`; of its warp's part of the columns the lower or upper 8 of every 16: units cu, cu + 2, .. of the wide
-    // products, columns j0 .., j0 + 16 .. of the square ones
-    const int q4 = warp & 3, hf = warp >> 2, row = q4 * 16 + (lane & 15), cu = hf * 2 * WIDE + (lane >> 4), j0 = hf * 16 * SQUARE + (lane >> 4) * 8;
-    const bool act = lane < 16;
+    // 16 rows per warp, of the wide products 32 columns and of the square ones 16, as fragments
+    const int q4 = warp & 3, hf = warp >> 2, g = lane >> 2, t = lane & 3, r0 = q4 * 16, j0 = hf * 16, w0 = hf * 16 * WIDE;
+    const int row[2] = {r0 + g, r0 + g + 8}, sum_row = r0 + g + 8 * (t & 1);        // whose sums this lane keeps
     const uint32_t base = tmem + ((uint32_t)(q4 * 32) << 16);
-    float aq[8 * WIDE] = {}, ak[8 * WIDE] = {}, az[8 * SQUARE] = {}, aw[DELTA ? 8 * SQUARE : 1] = {};
-    for (int i = 0; i < SQUARE; ++i) {               // first use is behind the first head's products
-      asm volatile("prefetch.global.L2 [%0];" ::"l"(p.qk + ((long long)c * p.Hk + kh) * (C * C) + row * C + j0 + 16 * i));
-      if (DELTA) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.kk + ((long long)c * p.Hk + kh) * (C * C) + row * C + j0 + 16 * i));
+    Pair aq[WIDE][2][2], ak[WIDE][2][2], az[2][2], aw[2][2];
+    {
+      const Pair zero = pair(0.f, 0.f);
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          az[n][h] = aw[n][h] = zero;
+#pragma unroll
+          for (int i = 0; i < WIDE; ++i) aq[i][n][h] = ak[i][n][h] = zero;
+        }
     }
+    // first use is behind the first head's products
+    const float* qk = p.qk + ((long long)c * p.Hk + kh) * (C * C) + j0 + 2 * t;
+    const float* kk = DELTA ? p.kk + ((long long)c * p.Hk + kh) * (C * C) + j0 + 2 * t : nullptr;
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(qk + (r0 + (lane & 15)) * C));
+    if (DELTA) asm volatile("prefetch.global.L2 [%0];" ::"l"(kk + (r0 + (lane & 15)) * C));
     auto wwait = [&](uint64_t* b, uint32_t parity, int detail) {
       wait(b, parity, detail);
       __syncwarp();
@@ -381,9 +405,7 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
     const uint32_t a_hi = ((su + (lane >> 4)) ^ (sa_r & 7)) << 4, a_lo = ((su + (lane >> 4) + 4) ^ (sa_r & 7)) << 4;
     const uint32_t b_hi = ((su + ((lane >> 3) & 1)) ^ (sb_r & 7)) << 4, b_lo = ((su + ((lane >> 3) & 1) + 4) ^ (sb_r & 7)) << 4;
     wwait(&bars->qk_full, 0, 40);
-    const float rq = rqk[row], rk = rqk[C + row];
-    const float* qk = p.qk + ((long long)c * p.Hk + kh) * (C * C) + row * C + j0;
-    const float* kk = DELTA ? p.kk + ((long long)c * p.Hk + kh) * (C * C) + row * C + j0 : nullptr;
+    const float rq[2] = {rqk[row[0]], rqk[row[1]]}, rk[2] = {rqk[C + row[0]], rqk[C + row[1]]};
     int n = 0, m = 0;
     for (int hh = 0; hh < rep; ++hh) {
       Red& r = red[hh & 1];
@@ -467,70 +489,72 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
           dst[8] = d0 ? rv[1][2] : rv[1][3];
         }
       }
-      const float b = ldsf(hd + (2 * C + row) * 4), gam = ex2_sum(hd, row), dec = ex2_diff(hd, C - 1, row);
+      float f1[2], f2[2], f3[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const bool on = row[h] < len;                                 // rows behind the end hold other documents' products
+        const float b = ldsf(hd + (2 * C + row[h]) * 4), gam = ex2_sum(hd, row[h]), dec = ex2_diff(hd, C - 1, row[h]);
+        f1[h] = on ? gam * rq[h] : 0.f, f2[h] = on ? -b * gam * rk[h] : 0.f, f3[h] = on ? dec * rk[h] * (DELTA ? 1.f : b) : 0.f;
+      }
       wwait(&bars->acc_full, hh & 1, 43);
       tc_fence_after();
-      const bool on = row < len;                                      // rows behind the end hold other documents' products
-      const float f1 = on ? gam * rq : 0.f, f2 = on ? -b * gam * rk : 0.f, f3 = on ? dec * rk * (DELTA ? 1.f : b) : 0.f;
-      const float d3 = add_rows(base + COL_T3 + hf * 16 * WIDE, sm + L::SM_K, row, cu, f3, ak);
+      const float d3 = add_rows(base + COL_T3 + w0, sm + L::SM_K, r0, w0, f3, ak);
       if (!DELTA) {
         tc_fence_before();
         arrive(&bars->t3_empty);
       }
-      const float d1 = add_rows(base + COL_T1 + set * 128 + hf * 16 * WIDE, sm + L::SM_Q, row, cu, f1, aq);
-      const float d2 = DELTA ? add_rows(base + COL_T2 + hf * 16 * WIDE, sm + L::SM_K, row, cu, f2, ak) : 0.f;
-      if (act) r.rd[0][hf][row] = d1, r.rd[1][hf][row] = d2, r.rd[2][hf][row] = d3;
+      const float d1 = add_rows(base + COL_T1 + set * 128 + w0, sm + L::SM_Q, r0, w0, f1, aq);
+      const float d2 = DELTA ? add_rows(base + COL_T2 + w0, sm + L::SM_K, r0, w0, f2, ak) : 0.f;
+      if (t < 2) r.rd[0][hf][sum_row] = d1, r.rd[1][hf][sum_row] = d2, r.rd[2][hf][sum_row] = d3;
       {
-        float er = 0.f, fr = 0.f;
-        const float gi = ldsf(hd + row * 4), gl = ldsf(hd + (C + row) * 4);
-        const int last = row < len ? row : -1;                        // the row's last column; none behind the end
+        uint32_t x[8], xl[8];
+        float2 qr[2][2], kr[2][2];
+        tmem_ld_frag(base + COL_P + set * 64 + j0, x);
+        if (DELTA) tmem_ld_frag(base + COL_L + j0, xl);
 #pragma unroll
-        for (int i = 0; i < SQUARE; ++i) {
-          const int j = j0 + 16 * i;
-          float hi[8], lo[8], kj[8], bj[8], qr[8], kr[8], x[8], v[8];
-          uint32_t t[16], tl[16];
-          auto eight = [&](const float* src, float (&dst)[8]) {
-            const float4 a = reinterpret_cast<const float4*>(src)[0], c4 = reinterpret_cast<const float4*>(src)[1];
-            dst[0] = a.x, dst[1] = a.y, dst[2] = a.z, dst[3] = a.w, dst[4] = c4.x, dst[5] = c4.y, dst[6] = c4.z, dst[7] = c4.w;
-          };
-          auto eight_s = [&](uint32_t src, float (&dst)[8]) {
-            const float4 a = ldsf4(src), c4 = ldsf4(src + 16);
-            dst[0] = a.x, dst[1] = a.y, dst[2] = a.z, dst[3] = a.w, dst[4] = c4.x, dst[5] = c4.y, dst[6] = c4.z, dst[7] = c4.w;
-          };
-          tmem_ld_32x16(base + COL_P + set * 64 + hf * 16 * SQUARE + 16 * i, t);
-          if (DELTA) tmem_ld_32x16(base + COL_L + hf * 16 * SQUARE + 16 * i, tl);
-          eight(qk + 16 * i, qr);
-          if (DELTA) eight(kk + 16 * i, kr);
-          eight_s(hd + j * 4, hi), eight_s(hd + (C + j) * 4, lo), eight_s(srqk + (C + j) * 4, kj);
-          if (!DELTA) eight_s(hd + (2 * C + j) * 4, bj);
+        for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) hi[e] = xb_ex2((gi - hi[e]) + (gl - lo[e]));
-          tc_wait_ld();
-          spread<8>(t, x);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float y = j + e <= last ? hi[e] * x[e] : 0.f, w = j + e <= last ? y * qr[e] : 0.f;
-            er += DELTA ? w : bj[e] * w;
-            v[e] = w;
-            az[8 * i + e] += y * (rq * kj[e]) * (DELTA ? 1.f : bj[e]);
+          for (int h = 0; h < 2; ++h) {
+            qr[n][h] = *reinterpret_cast<const float2*>(qk + row[h] * C + 8 * n);
+            if (DELTA) kr[n][h] = *reinterpret_cast<const float2*>(kk + row[h] * C + 8 * n);
           }
-          const float es = col_sum(v);
-          if ((lane & 8) == 0) r.ec[q4][j + (lane & 7)] = es;
-          if (DELTA) {
-            spread<8>(tl, x);
+        float er[2] = {}, fr[2] = {}, ec[2][2] = {}, fc[2][2] = {}, b[2], gi[2], gl[2];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float y = j + e < last ? -hi[e] * x[e] : 0.f, w = j + e < last ? y * kr[e] : 0.f;
-              fr += w;
-              v[e] = b * w;
-              aw[DELTA ? 8 * i + e : 0] += b * y * (rk * kj[e]);
+        for (int h = 0; h < 2; ++h)
+          b[h] = DELTA ? ldsf(hd + (2 * C + row[h]) * 4) : 0.f, gi[h] = ldsf(hd + row[h] * 4), gl[h] = ldsf(hd + (C + row[h]) * 4);
+        tc_wait_ld();
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const int j = j0 + 8 * n + 2 * t;
+          const float2 hi = lds2(hd + j * 4), lo = lds2(hd + (C + j) * 4), kj = lds2(srqk + (C + j) * 4);
+          const float2 bj = DELTA ? make_float2(1.f, 1.f) : lds2(hd + (2 * C + j) * 4);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int last = row[h] < len ? row[h] : -1;              // the row's last column; none behind the end
+            const float e0 = xb_ex2((gi[h] - hi.x) + (gl[h] - lo.x)), e1 = xb_ex2((gi[h] - hi.y) + (gl[h] - lo.y));
+            {
+              const float y0 = j <= last ? e0 * __uint_as_float(x[4 * n + 2 * h]) : 0.f, w0 = j <= last ? y0 * qr[n][h].x : 0.f;
+              const float y1 = j < last ? e1 * __uint_as_float(x[4 * n + 2 * h + 1]) : 0.f, w1 = j < last ? y1 * qr[n][h].y : 0.f;
+              er[h] += DELTA ? w0 + w1 : bj.x * w0 + bj.y * w1;
+              ec[n][0] += w0, ec[n][1] += w1;
+              const Pair f = pair(rq[h] * kj.x, rq[h] * kj.y) * pair(y0, y1);
+              az[n][h] = DELTA ? az[n][h] + f : fma2(f, pair(bj.x, bj.y), az[n][h]);
             }
-            const float fs = col_sum(v);
-            if ((lane & 8) == 0) r.fc[q4][j + (lane & 7)] = fs;
+            if (DELTA) {
+              const float y0 = j < last ? -e0 * __uint_as_float(xl[4 * n + 2 * h]) : 0.f, w0 = j < last ? y0 * kr[n][h].x : 0.f;
+              const float y1 = j + 1 < last ? -e1 * __uint_as_float(xl[4 * n + 2 * h + 1]) : 0.f, w1 = j + 1 < last ? y1 * kr[n][h].y : 0.f;
+              fr[h] += w0 + w1;
+              fc[n][0] += b[h] * w0, fc[n][1] += b[h] * w1;
+              const float f = b[h] * rk[h];
+              aw[n][h] = fma2(pair(f * kj.x, f * kj.y), pair(y0, y1), aw[n][h]);
+            }
           }
         }
-        er += __shfl_xor_sync(0xffffffffu, er, 16), fr += __shfl_xor_sync(0xffffffffu, fr, 16);
-        if (act) r.er[hf][row] = er, r.fr[hf][row] = fr;
+        const int col = j0 + 8 * (g & 1) + 2 * t + ((g >> 1) & 1);
+        const float es = col_sum(ec), fs = DELTA ? col_sum(fc) : 0.f;
+        if (g < 4) r.ec[q4][col] = es, r.fc[q4][col] = fs;
+        const float rs = row_sum2(er, fr);
+        (t < 2 ? r.er : r.fr)[hf][sum_row] = rs;
       }
       tc_fence_before();
       arrive(DELTA ? &bars->t3_empty : &bars->set_empty[set]);
@@ -538,23 +562,16 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
       arrive(&bars->hd_empty[hh & 1]);
     }
     // Z and W as operand tiles over the ring, whose last tiles have been read; K and Q without rows behind the end
-    {
-      const uint32_t t = sm + L::SM_RING + row * 128;
 #pragma unroll
-      for (int part = 0; part < (DELTA ? 2 : 1); ++part) {
+    for (int part = 0; part < (DELTA ? 2 : 1); ++part) {
+      uint32_t hi[4], lo[4];
 #pragma unroll
-        for (int u = 0; u < SQUARE; ++u) {
-          uint32_t hi[4], lo[4];
+      for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int i = 8 * u + 2 * e;
-            split2(part ? aw[DELTA ? i : 0] : az[i], part ? aw[DELTA ? i + 1 : 0] : az[i + 1], hi[e], lo[e]);
-          }
-          const int off = part * 2 * T64 + ((((j0 >> 3) + 2 * u) ^ (row & 7)) << 4);
-          sts128(t + off, hi[0], hi[1], hi[2], hi[3]);
-          sts128(t + off + T64, lo[0], lo[1], lo[2], lo[3]);
-        }
-      }
+        for (int h = 0; h < 2; ++h) split2(part ? aw[n][h] : az[n][h], hi[2 * n + h], lo[2 * n + h]);
+      const uint32_t at = block_addr(sm + L::SM_RING + part * 2 * T64, r0, j0);
+      stsm4(at, hi[0], hi[1], hi[2], hi[3]);
+      stsm4(at + T64, lo[0], lo[1], lo[2], lo[3]);
     }
     for (int i = tid; i < 4 * (C - len) * 8; i += WORKERS) {
       const int part = i / ((C - len) * 8), rr = len + (i % ((C - len) * 8)) / 8;
@@ -565,43 +582,65 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
     arrive(&bars->z_full);
     wwait(&bars->last, 0, 44);
     tc_fence_after();
-    add_rows(base + COL_T1 + hf * 16 * WIDE, sm + L::SM_Q, row, cu, 1.f, aq);
-    add_rows(base + COL_T2 + hf * 16 * WIDE, sm + L::SM_K, row, cu, 1.f, ak);
+    const float one[2] = {1.f, 1.f};
+    add_rows(base + COL_T1 + w0, sm + L::SM_Q, r0, w0, one, aq);
+    add_rows(base + COL_T2 + w0, sm + L::SM_K, r0, w0, one, ak);
     // gradient through the L2 norms: dq - q^ (q^ . dq), rows of norm below 1e-12 excepted
-    float fq = 0.f, fk = 0.f;
+    float fq[2] = {}, fk[2] = {};
     if (p.l2norm) {
-      float sq = 0.f, sk = 0.f;
+      Pair sq[2], sk[2];
+      sq[0] = sq[1] = sk[0] = sk[1] = pair(0.f, 0.f);
 #pragma unroll
       for (int i = 0; i < WIDE; ++i) {
-        const int unit = cu + 2 * i;
-        float x[8], y[8];
-        floats8(tile_unit(sm + L::SM_Q, row, unit), x), floats8(tile_unit(sm + L::SM_K, row, unit), y);
+        uint32_t x[4], y[4];
+        ldsm4(x, block_addr(sm + L::SM_Q, r0, w0 + 16 * i)), ldsm4(y, block_addr(sm + L::SM_K, r0, w0 + 16 * i));
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sq += x[e] * aq[8 * i + e], sk += y[e] * ak[8 * i + e];
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            sq[h] = fma2(bf16_pair(x[2 * n + h]), aq[i][n][h], sq[h]), sk[h] = fma2(bf16_pair(y[2 * n + h]), ak[i][n][h], sk[h]);
       }
-      sq += __shfl_xor_sync(0xffffffffu, sq, 16), sk += __shfl_xor_sync(0xffffffffu, sk, 16);
+      const float2 q0 = both(sq[0]), q1 = both(sq[1]), k0 = both(sk[0]), k1 = both(sk[1]);
+      const float a[2] = {q0.x + q0.y, q1.x + q1.y}, b[2] = {k0.x + k0.y, k1.x + k1.y};
       Red& r = red[rep & 1];
       wwait(&bars->red_empty[rep & 1], ((rep >> 1) & 1) ^ 1, 46);
-      if (act) r.rd[0][hf][row] = sq, r.rd[1][hf][row] = sk;
+      const float s = row_sum2(a, b);
+      (t < 2 ? r.rd[0] : r.rd[1])[hf][sum_row] = s;
       wbar();
-      const float nq = rq / p.scale;
-      if (nq < 0.99e12f) fq = nq * nq * parts(r.rd[0], row);
-      if (rk < 0.99e12f) fk = rk * rk * parts(r.rd[1], row);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float nq = rq[h] / p.scale;
+        if (nq < 0.99e12f) fq[h] = nq * nq * parts(r.rd[0], row[h]);
+        if (rk[h] < 0.99e12f) fk[h] = rk[h] * rk[h] * parts(r.rd[1], row[h]);
+      }
     }
-    if (row < len)
+    // in the places of this warp's blocks of Q and K, and from there in 16-byte pieces
+#pragma unroll
+    for (int i = 0; i < WIDE; ++i)
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+        const uint32_t at = block_addr(sm + (part ? L::SM_K : L::SM_Q), r0, w0 + 16 * i);
+        uint32_t x[4];
+        ldsm4(x, at);
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float f = part ? -fk[h] : -fq[h];
+            const float2 y = both(fma2(pair(f, f), bf16_pair(x[2 * n + h]), part ? ak[i][n][h] : aq[i][n][h]));
+            x[2 * n + h] = pack_bf16x2(y.x, y.y);
+          }
+        stsm4(at, x[0], x[1], x[2], x[3]);
+      }
+    __syncwarp();
+    const int out = r0 + (lane & 15);
+    if (out < len)
 #pragma unroll
       for (int i = 0; i < WIDE; ++i) {
-        const int unit = cu + 2 * i, col = unit * 8;
+        const int unit = hf * 2 * WIDE + 2 * i + (lane >> 4), col = unit * 8;
         if (col < p.dk) {
-          float x[8], y[8];
-          floats8(tile_unit(sm + L::SM_Q, row, unit), x), floats8(tile_unit(sm + L::SM_K, row, unit), y);
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            x[e] = aq[8 * i + e] - fq * x[e], y[e] = ak[8 * i + e] - fk * y[e];
-          *reinterpret_cast<uint4*>(dq + row * d_t + col) =
-              make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
-          *reinterpret_cast<uint4*>(dk + row * d_t + col) =
-              make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7]));
+          *reinterpret_cast<uint4*>(dq + out * d_t + col) = tile_unit(sm + L::SM_Q, out, unit);
+          *reinterpret_cast<uint4*>(dk + out * d_t + col) = tile_unit(sm + L::SM_K, out, unit);
         }
       }
   }
