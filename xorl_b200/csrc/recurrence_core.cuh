@@ -81,6 +81,9 @@ __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint3
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 __device__ __forceinline__ float ldsf(uint32_t a) { return __uint_as_float(lds32(a)); }
+__device__ __forceinline__ void stsf(uint32_t a, float v) {
+  asm volatile("st.shared.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory");
+}
 __device__ __forceinline__ float4 ldsf4(uint32_t a) {
   float4 v;
   asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
@@ -145,9 +148,21 @@ __device__ __forceinline__ float ex2_diff(uint32_t hd, int i, int j) {
 __device__ __forceinline__ float ex2_sum(uint32_t hd, int i) { return xb_ex2(ldsf(hd + i * 4)) * (1.f + 0.6931472f * ldsf(hd + (C + i) * 4)); }
 
 // A bounded wait whose slow path stays out of line: a wait that runs out raises a flag and reports; from then on waits
-// return at once and every role walks to its end.
-__device__ __noinline__ void rec_wait_slow(uint64_t* bar, uint32_t parity, int* abort_flag, int* status, int detail) {
-  mbar_wait(bar, parity, abort_flag, status, XB_K_RECURRENCE, detail);
+// return at once and every role walks to its end.  Warps that wait sleep up to 20 us at a time, so that they leave the
+// issue slots to those that work.
+__device__ __noinline__ void rec_wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int detail) {
+  const uint64_t t0 = xb_globaltimer();
+  for (;;) {
+    uint32_t ok;
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(ok) : "r"(xb_smem_u32(bar)), "r"(parity), "r"(20000u) : "memory");
+    if (ok || *abort_flag) return;
+    if (xb_globaltimer() - t0 > XB_WAIT_LIMIT_NS) {
+      *abort_flag = 1;
+      xb_report(status, XB_ERR_MBAR_TIMEOUT, XB_K_RECURRENCE, detail);
+      return;
+    }
+  }
 }
 __device__ __forceinline__ void rec_wait(uint64_t* bar, uint32_t parity, int* abort_flag, int* status, int detail) {
   if (!mbar_try_wait(bar, parity)) rec_wait_slow(bar, parity, abort_flag, status, detail);

@@ -86,8 +86,9 @@ __global__ void __launch_bounds__(128) scan_prep(const XbRecArgs p) {
 constexpr int T64 = HALF / 2;
 // warps: 16 add up the state and write outputs, 6 make P (a block of 32 rows and 16 columns each), 4 the other operand
 constexpr int ADDERS = 512, PMAKERS = 192, XMAKERS = 128, MAKERS = PMAKERS + XMAKERS, THREADS = ADDERS + MAKERS + 64;
-// K and Q: [64 rows][128 bytes] twice each; v or dO: [64][64 columns]; Q K^T: [64][32 fp32] twice; decays and b
-constexpr int ST_K = 0, ST_Q = 2 * T64, ST_X = 4 * T64, ST_QK = 5 * T64, ST_HD = 7 * T64, STAGE = 7 * T64 + 1024;
+// K and Q: [64 rows][128 bytes] twice each; v or dO: [64][64 columns]; Q K^T: [64][32 fp32] twice; decays and b; the row
+// factors of the outputs
+constexpr int ST_K = 0, ST_Q = 2 * T64, ST_X = 4 * T64, ST_QK = 5 * T64, ST_HD = 7 * T64, ST_ROW = ST_HD + HD * 4, STAGE = ST_ROW + C * 4;
 constexpr int SM_S = 2 * STAGE, SM_P = SM_S + 2 * HALF, SM_D = SM_P + 2 * HALF, SM_BAR = SM_D + 2 * HALF;
 constexpr int SMEM = SM_BAR + 256 + 1024;
 constexpr int D1 = 0, D2 = 128, DSTEP = 192, D3 = 384;      // D1, D2 of even and odd steps; D3
@@ -231,7 +232,8 @@ scan_seq(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtenso
         }
         asm volatile("bar.sync 1, %0;" ::"n"(XMAKERS) : "memory");
       }
-      const float f = BWD ? ex2_sum(hd, row) : ex2_diff(hd, C - 1, row) * ldsf(hd + (2 * C + row) * 4);
+      const float gam = ex2_sum(hd, row), db = ex2_diff(hd, C - 1, row) * ldsf(hd + (2 * C + row) * 4), f = BWD ? gam : db;
+      if (OUT && half == 0) stsf(st + ST_ROW + row * 4, BWD ? db : gam);
       uint4 v[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) v[u] = lds128(st + ST_X + row * 128 + (((half * 4 + u) ^ (row & 7)) << 4));
@@ -297,9 +299,8 @@ scan_seq(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtenso
     }
   } else {
     // ------------------------------------ the state, and the outputs -------------------------------------------------
-    // a row of the state and 16 of its columns; 16 lanes of each warp hold the rows of the 64-row accumulators, the other
-    // 16 take half of their columns
-    const int q4 = warp & 3, sl = warp >> 3, part = (warp >> 2) & 1, r = q4 * 32 + lane, orow = q4 * 16 + (lane & 15);
+    // a row of the state and 16 of its columns; of the 64-row accumulators 16 rows and 16 columns per warp, as fragments
+    const int q4 = warp & 3, sl = warp >> 3, part = (warp >> 2) & 1, r = q4 * 32 + lane, r0 = q4 * 16, g = lane >> 2, t = lane & 3;
     const uint32_t base = tmem + ((uint32_t)(q4 * 32) << 16);
     const int col = v0 + sl * NV + part * 16, cols = p.dv - col;
     const long long soff = ((long long)doc * p.Hv + h) * p.dk * p.dv + col * p.s_v + r * p.s_k;
@@ -331,16 +332,21 @@ scan_seq(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtenso
     split_row();
     if (steps > 0) put();
     const float skip = p.D[h];
-    const int u0 = sl * 4 + part * 2 + (lane >> 4), ocol = v0 + u0 * 8;
+    const int xrow = r0 + (lane & 15), xunit = sl * 4 + part * 2 + (lane >> 4), ocol = col + 8 * (t & 1) + 4 * (t >> 1);
     bf16* out = (bf16*)(BWD ? p.dv_out : p.o) + (long long)h * p.dv + ocol;
     for (int n = 0; n < steps; ++n) {
       const int s = n & 1;
       const int4 ch = chunks[chunk_of(n)];
       const uint32_t st = sm + s * STAGE, hd = st + ST_HD;
       wwait(&bars->full[s], (n >> 1) & 1, 30);
-      const float f = BWD ? ex2_diff(hd, C - 1, orow) * ldsf(hd + (2 * C + orow) * 4) : ex2_sum(hd, orow), last = ex2_sum(hd, C - 1);
-      uint4 xv = make_uint4(0, 0, 0, 0);
-      if (OUT) xv = lds128(st + ST_X + orow * 128 + ((u0 ^ (orow & 7)) << 4));
+      const float last = ex2_sum(hd, C - 1);
+      float f[2] = {};
+      uint32_t xv[4];
+      if (OUT) {
+        wwait(&bars->pd_full[s], (n >> 1) & 1, 34);                    // the row factors
+        f[0] = ldsf(st + ST_ROW + (r0 + g) * 4), f[1] = ldsf(st + ST_ROW + (r0 + g + 8) * 4);
+        ldsm4(xv, st + ST_X + xrow * 128 + ((xunit ^ (xrow & 7)) << 4));
+      }
       arrive(&bars->empty[s]);
       wwait(&bars->d3_full, n & 1, 31);
       tc_fence_after();
@@ -363,33 +369,25 @@ scan_seq(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtenso
       if (OUT) {
         if (n + 1 == steps) wwait(&bars->out_full[s], (n >> 1) & 1, 33);   // else: the wait above was for the same products
         tc_fence_after();
-        uint32_t a[16], b[16], d[16];
-        tmem_ld_32x16(base + D1 + s * DSTEP + sl * 64 + part * 16, a);
-        tmem_ld_32x16(base + D1 + s * DSTEP + sl * 64 + 32 + part * 16, b);
-        tmem_ld_32x16(base + D2 + s * DSTEP + sl * 32 + part * 16, d);
+        uint32_t a[8], b[8], d[8], w[4];
+        tmem_ld_frag(base + D1 + s * DSTEP + sl * 64 + part * 16, a);
+        tmem_ld_frag(base + D1 + s * DSTEP + sl * 64 + 32 + part * 16, b);
+        tmem_ld_frag(base + D2 + s * DSTEP + sl * 32 + part * 16, d);
         tc_wait_ld();
         tc_fence_before();
         arrive(&bars->out_empty[s]);
-        float y[8];
 #pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-          const float2 z = both(fma2(pair(f, f), pair(a[e], a[e + 1]) + pair(b[e], b[e + 1]), pair(d[e], d[e + 1])));
-          a[e] = __float_as_uint(z.x), a[e + 1] = __float_as_uint(z.y);
+        for (int e = 0; e < 4; ++e) {        // e = 2 n + h: row g + 8 h, columns 8 n + 2 t, 8 n + 2 t + 1
+          const Pair z = fma2(pair(f[e & 1], f[e & 1]), pair(a[2 * e], a[2 * e + 1]) + pair(b[2 * e], b[2 * e + 1]), pair(d[2 * e], d[2 * e + 1]));
+          const float2 y = both(fma2(pair(skip, skip), pair(xv[e] << 16, xv[e] & 0xffff0000u), z));
+          w[e] = pack_bf16x2(y.x, y.y);
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t far = __shfl_sync(0xffffffffu, a[8 + e], lane & 15);
-          y[e] = __uint_as_float(lane & 16 ? far : a[e]);
-        }
-        if (orow < ch.y && ocol < p.dv) {
-          const uint32_t w[4] = {xv.x, xv.y, xv.z, xv.w};
-          uint32_t z[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 v = unpack_bf16x2(w[e]);
-            z[e] = pack_bf16x2(y[2 * e] + skip * v.x, y[2 * e + 1] + skip * v.y);
-          }
-          *reinterpret_cast<uint4*>(out + (long long)(ch.x + orow) * p.Hv * p.dv) = make_uint4(z[0], z[1], z[2], z[3]);
+        for (int h = 0; h < 2; ++h) {        // lanes t and t ^ 1 trade, for four neighbouring columns each
+          const uint32_t other = __shfl_xor_sync(0xffffffffu, t & 1 ? w[h] : w[2 + h], 1);
+          const int row = r0 + g + 8 * h;
+          if (row < ch.y && ocol < p.dv)
+            *reinterpret_cast<uint2*>(out + (long long)(ch.x + row) * p.Hv * p.dv) = t & 1 ? make_uint2(other, w[2 + h]) : make_uint2(w[h], other);
         }
       }
     }
