@@ -330,9 +330,13 @@ struct Lay {
   static constexpr int SM_S = STAGES * STAGE, SM_B2 = SM_S + HALF, SM_B3 = SM_B2 + ROWS, SM_U = SM_B3 + ROWS, SM_BAR = SM_U + HALF / 2;
   static constexpr int SMEM = SM_BAR + 128 + 1024;
 };
-constexpr int WORKERS = 256, ISSUER = WORKERS / 32, LOADER = ISSUER + 1, THREADS = WORKERS + 64;
+constexpr int NB = 2;                        // units of 8 columns per worker
+constexpr int WORKERS = 128 * (NV / 8 / NB), ISSUER = WORKERS / 32, LOADER = ISSUER + 1, THREADS = WORKERS + 64;
 constexpr int MEET = WORKERS + 32;           // workers and the issuing warp
-constexpr int TMEM_COLS = 256, D1 = 0, D2 = 64, D3 = 128, D4 = 192;     // accumulators, 64 columns each
+// Accumulators, 64 columns each: those of the three products of the chain and Q S, or P^T dO.  Forward with one CTA per SM,
+// Q S of the next step and P U have their own, and O is written behind R; else P U takes the place of T R, which has been
+// read by then, and O is written before R.
+constexpr int D1 = 0, D2 = 64, D3 = 128, D4 = 192, D5 = 256, D6 = 320;
 
 struct __align__(8) Bars {
   uint64_t full[2], done[4], kept;
@@ -394,70 +398,89 @@ __device__ __forceinline__ void clear_rows(uint32_t st, int len) {
   }
 }
 
-// 16 values of a row as [hi | lo] of a [rows][128 bytes] operand tile; columns 16 * half ..
-__device__ __forceinline__ void put_row(uint32_t tile, int row, int half, const float (&x)[16], uint32_t (&hi)[8], uint32_t (&lo)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) split2(x[2 * i], x[2 * i + 1], hi[i], lo[i]);
+// Workers: of the state a row and 8 NB columns per thread (warp w: rows 32 (w % 4) .., columns 8 NB (w / 4) ..), of what has
+// 64 rows 16 rows and 8 NB columns per warp, as fragments: of every 8 columns rows g and g + 8, columns 2 t and 2 t + 1,
+// element 4 n + 2 h + column.  An operand tile's row is 128 bytes, [hi 32 | lo 32]; u0 is the warp's first unit of it.
+__device__ __forceinline__ void put_row(uint32_t tile, int row, int u0, const float (&x)[8 * NB]) {
   const uint32_t r = tile + row * 128;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int u = half * 2 + i;
-    sts128(r + ((u ^ (row & 7)) << 4), hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
-    sts128(r + (((u + 4) ^ (row & 7)) << 4), lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
+  for (int n = 0; n < NB; ++n) {
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) split2(x[8 * n + 2 * i], x[8 * n + 2 * i + 1], hi[i], lo[i]);
+    sts128(r + (((u0 + n) ^ (row & 7)) << 4), hi[0], hi[1], hi[2], hi[3]);
+    sts128(r + (((u0 + n + 4) ^ (row & 7)) << 4), lo[0], lo[1], lo[2], lo[3]);
   }
 }
-// the sum of an accumulator's two halves, 16 columns of this thread's row
-__device__ __forceinline__ void read_acc(uint32_t addr, float (&x)[16]) {
-  uint32_t a[16], b[16];
-  tmem_ld_32x16(addr, a);
-  tmem_ld_32x16(addr + 32, b);
-  tc_wait_ld();
+// this lane's address of a warp's 16 rows and first 8 columns, hi and lo; a unit further is the address ^ 16 (u0 is even)
+__device__ __forceinline__ uint32_t frag_addr(uint32_t tile, int r0, int u0) {
+  const int l = xb_lane(), row = r0 + (l & 15), u = u0 + (l >> 4) * 4;
+  return tile + row * 128 + ((u ^ (row & 7)) << 4);
+}
+__device__ __forceinline__ void put_frag(uint32_t addr, const float (&x)[4 * NB]) {
 #pragma unroll
-  for (int i = 0; i < 16; i += 2) {
+  for (int n = 0; n < NB; ++n) {
+    uint32_t hi[2], lo[2];
+    split2(x[4 * n], x[4 * n + 1], hi[0], lo[0]), split2(x[4 * n + 2], x[4 * n + 3], hi[1], lo[1]);
+    stsm4(addr ^ (n << 4), hi[0], hi[1], lo[0], lo[1]);
+  }
+}
+// the sum of an accumulator's two halves
+template <int N>
+__device__ __forceinline__ void add_halves(const uint32_t (&a)[N], const uint32_t (&b)[N], float (&x)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
     const float2 f = both(pair(a[i], a[i + 1]) + pair(b[i], b[i + 1]));
     x[i] = f.x, x[i + 1] = f.y;
   }
 }
-// 16 bf16 values of a row of the [64][64 bytes] tile of v or dO
-__device__ __forceinline__ void read_x(uint32_t tile, int row, int half, bool on, uint4 (&v)[2]) {
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    v[i] = on ? lds128(tile + swz<4>(row, half * 2 + i)) : make_uint4(0, 0, 0, 0);
+__device__ __forceinline__ void read_rows(uint32_t addr, float (&x)[8 * NB]) {
+  uint32_t a[8 * NB], b[8 * NB];
+  tmem_ld_rows(addr, a);
+  tmem_ld_rows(addr + 32, b);
+  tc_wait_ld();
+  add_halves(a, b, x);
 }
-__device__ __forceinline__ void floats(const uint4 (&v)[2], float (&x)[16]) {
+__device__ __forceinline__ void read_frag(uint32_t addr, float (&x)[4 * NB]) {
+  uint32_t a[4 * NB], b[4 * NB];
+  tmem_ld_frag(addr, a);
+  tmem_ld_frag(addr + 32, b);
+  tc_wait_ld();
+  add_halves(a, b, x);
+}
+// A warp's 16 rows to global memory as bf16: lanes t and t ^ 1 trade, for four columns of one row each.  `dst` is row
+// frag_row() at the warp's first column; `cols` are left from there.
+__device__ __forceinline__ int frag_row() { return (xb_lane() >> 2) + 8 * (xb_lane() & 1); }
+__device__ __forceinline__ void store_frag(bf16* dst, bool on, int cols, const float (&x)[4 * NB]) {
+  const bool odd = xb_lane() & 1;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 f = unpack_bf16x2(w[j]);
-      x[8 * i + 2 * j] = f.x, x[8 * i + 2 * j + 1] = f.y;
-    }
+  for (int n = 0; n < NB; ++n) {
+    const uint32_t w0 = pack_bf16x2(x[4 * n], x[4 * n + 1]), w1 = pack_bf16x2(x[4 * n + 2], x[4 * n + 3]);
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, odd ? w0 : w1, 1);
+    if (on && 8 * n < cols) *reinterpret_cast<uint2*>(dst + 8 * n + 4 * ((xb_lane() >> 1) & 1)) = odd ? make_uint2(other, w1) : make_uint2(w0, other);
   }
 }
-// 16 fp32 values of a state row in global memory
-__device__ __forceinline__ void state_row(float* base, long long sk, long long sv, int row, int dk, int col, int cols, bool store, float (&s)[16]) {
-  if (sv == 1 && row < dk && col + 16 <= cols) {                     // rows of a multiple of 8 values
-    float4* at = reinterpret_cast<float4*>(base + row * sk + col);
+// a thread's part of a state row in global memory
+__device__ __forceinline__ void state_row(float* base, long long sk, long long sv, int row, int dk, int col, int cols, bool store, float (&s)[8 * NB]) {
+  if (row >= dk) return;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 2 * NB; ++i) {
+    if (col + 4 * i >= cols) return;                                 // columns come in multiples of 8
+    if (sv == 1) {
+      float4* at = reinterpret_cast<float4*>(base + row * sk + col) + i;
       if (store) {
-        at[i] = make_float4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
+        *at = make_float4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
       } else {
-        const float4 v = at[i];
+        const float4 v = *at;
         s[4 * i] = v.x, s[4 * i + 1] = v.y, s[4 * i + 2] = v.z, s[4 * i + 3] = v.w;
       }
-    }
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    float* at = base + row * sk + (col + i) * sv;
-    const bool on = row < dk && col + i < cols;
-    if (store) {
-      if (on) *at = s[i];
     } else {
-      s[i] = on ? *at : 0.f;
+#pragma unroll
+      for (int j = 4 * i; j < 4 * i + 4; ++j) {
+        float* at = base + row * sk + (col + j) * sv;
+        if (store) *at = s[j];
+        else s[j] = *at;
+      }
     }
   }
 }
@@ -477,6 +500,7 @@ __device__ __forceinline__ bool cta_setup(const XbRecArgs& p, Cta& a, uint8_t* r
   a.status = p.status;
   return a.doc >= 0 && a.doc < p.n_docs;
 }
+template <int COLS>
 __device__ __forceinline__ void cta_begin(Cta& a) {
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) mbar_init(&a.bars->full[i], 1);
@@ -486,7 +510,7 @@ __device__ __forceinline__ void cta_begin(Cta& a) {
     mbar_fence_init();
   }
   if (threadIdx.x / 32 == ISSUER) {
-    tmem_alloc(&a.bars->tmem, TMEM_COLS);
+    tmem_alloc(&a.bars->tmem, COLS);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -494,6 +518,7 @@ __device__ __forceinline__ void cta_begin(Cta& a) {
   tc_fence_after();
   a.tmem = a.bars->tmem;
 }
+template <int COLS>
 __device__ __forceinline__ void cta_end(Cta& a) {
   // after a wait that ran out, loads and products may still be on their way: give them 0.2 s
   if (*(volatile int*)&a.bars->abort_flag && threadIdx.x == 0)
@@ -502,7 +527,7 @@ __device__ __forceinline__ void cta_end(Cta& a) {
   __syncthreads();
   if (threadIdx.x / 32 == ISSUER) {
     tc_fence_after();
-    tmem_dealloc(a.tmem, TMEM_COLS);
+    tmem_dealloc(a.tmem, COLS);
   }
 }
 // rows outside the documents: zeros
@@ -533,7 +558,9 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
     if (OUT) zero_rows(p, a, o, o_t);
     return;
   }
-  cta_begin(a);
+  constexpr bool LATE = STAGES == 2;         // where O is written
+  constexpr int COLS = LATE ? 512 : 256, DPU = LATE ? D5 : D2;
+  cta_begin<COLS>(a);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int4* chunks = reinterpret_cast<const int4*>(p.chunks);
   constexpr int FIRST = MEET + (SAVE ? 32 : 0);    // whom barrier 1 brings together
@@ -559,6 +586,7 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
     }
   } else if (warp == ISSUER) {
     const bool one = xb_elect_one();
+    constexpr uint32_t id = xb_idesc(1, 1, 64, 64, 0, 1);
     for (int n = 0; n < a.c1 - a.c0; ++n) {
       const uint32_t st = xb_smem_u32(a.smem + (n % STAGES) * STAGE), b1 = xb_smem_u32(a.smem + L::SM_S), b2 = xb_smem_u32(a.smem + L::SM_B2),
                      b3 = xb_smem_u32(a.smem + L::SM_B3);
@@ -566,7 +594,6 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       if (one) {
         a.wait1(&a.bars->full[n % STAGES], (n / STAGES) & 1, 1);
         tc_fence_after();
-        constexpr uint32_t id = xb_idesc(1, 1, 128, 64, 0, 1);
 #pragma unroll
         for (int k = 0; k < 8; ++k)
           tc_mma_f16_ss(a.tmem + D1, xb_smem_desc(KMAJ, st + ST_KQ + (k >> 2) * HALF + (k & 3) * 32), xb_smem_desc(MNMAJ, b1 + k * 2048), id, k > 0);
@@ -575,30 +602,33 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       bar(2, MEET);
       if (one) {
         tc_fence_after();
-        constexpr uint32_t id = xb_idesc(1, 1, 128, 64, 0, 1);
 #pragma unroll
         for (int k = 0; k < 8; ++k)
           tc_mma_f16_ss(a.tmem + D2, xb_smem_desc(KMAJ, st + ST_TP + (k >> 2) * TP_PLANE + (k & 3) * 32), xb_smem_desc(MNMAJ, b2 + (k & 3) * 2048), id, k > 0);
         tc_commit(&a.bars->done[1]);
+        if (OUT) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)        // Q S: nobody waits for it
+            tc_mma_f16_ss(a.tmem + (LATE && (n & 1) ? D6 : D4), xb_smem_desc(KMAJ, st + ST_KQ + HALF / 2 + (k >> 2) * HALF + (k & 3) * 32), xb_smem_desc(MNMAJ, b1 + k * 2048), id, k > 0);
+        }
       }
       bar(3, MEET);
       if (one) {
         tc_fence_after();
-        constexpr uint32_t id = xb_idesc(1, 1, 128, 64, 1, 1);
+        constexpr uint32_t id3 = xb_idesc(1, 1, 128, 64, 1, 1);
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          tc_mma_f16_ss(a.tmem + D3, xb_smem_desc(MNMAJ, st + ST_KQ + k * 2048), xb_smem_desc(MNMAJ, b3 + k * 2048), id, k > 0);
+          tc_mma_f16_ss(a.tmem + D3, xb_smem_desc(MNMAJ, st + ST_KQ + k * 2048), xb_smem_desc(MNMAJ, b3 + k * 2048), id3, k > 0);
         tc_commit(&a.bars->done[2]);
       }
       if (OUT) {
         bar(4, MEET);
         if (one) {
           tc_fence_after();
-          constexpr uint32_t id = xb_idesc(1, 1, 128, 64, 0, 1);
           const uint32_t u = xb_smem_u32(a.smem + L::SM_U);
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            tc_mma_f16_ss(a.tmem + D4, xb_smem_desc(KMAJ, st + ST_TP + (k >> 2) * TP_PLANE + (k & 3) * 32), xb_smem_desc(MNMAJ, u + (k & 3) * 2048), id, k > 0);
+            tc_mma_f16_ss(a.tmem + DPU, xb_smem_desc(KMAJ, st + ST_TP + HALF / 2 + (k >> 2) * TP_PLANE + (k & 3) * 32), xb_smem_desc(MNMAJ, u + (k & 3) * 2048), id, k > 0);
           tc_commit(&a.bars->done[3]);
         }
       }
@@ -606,94 +636,98 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
     }
     if (SAVE && a.c0 < a.c1) bar(1, FIRST);
   } else {
-    const int q4 = warp & 3, half = warp >> 2, r = q4 * 32 + lane, i = r & 63;
-    const bool krow = r < C;
-    const uint32_t acc = a.tmem + ((uint32_t)(q4 * 32) << 16) + half * 16;
+    const int q4 = warp & 3, part = warp >> 2, r = q4 * 32 + lane, r0 = q4 * 16, g = lane >> 2;
+    const int row[2] = {r0 + g, r0 + g + 8}, u0 = part * NB, fcol = u0 * 8, orow = r0 + frag_row();
+    const uint32_t quad = a.tmem + ((uint32_t)(q4 * 32) << 16) + fcol;
+    const uint32_t f2 = frag_addr(a.sm + L::SM_B2, r0, u0), f3 = frag_addr(a.sm + L::SM_B3, r0, u0), fu = frag_addr(a.sm + L::SM_U, r0, u0);
     const long long soff = ((long long)a.doc * p.Hv + a.h) * p.dk * p.dv + a.v0 * p.s_v;
-    float s[16] = {}, y[16];
-    uint32_t hi[8], lo[8];
-    if (p.s_in != nullptr) state_row(const_cast<float*>(p.s_in) + soff, p.s_k, p.s_v, r, p.dk, half * 16, a.vcols, false, s);
-    // O = gamma rq Q S + P U of a chunk, whose Q S waits in y (threads of Q's rows)
-    auto finish = [&](int n, int4 ch, float f) {
+    float s[8 * NB] = {};
+    if (p.s_in != nullptr) state_row(const_cast<float*>(p.s_in) + soff, p.s_k, p.s_v, r, p.dk, fcol, a.vcols, false, s);
+    // O = gamma rq Q S + P U of a chunk
+    auto finish = [&](int n, int4 ch, const float (&f)[2]) {
       a.wait(&a.bars->done[3], n & 1, 7);
       tc_fence_after();
-      float x[16];
-      read_acc(acc + D4, x);
-      if (!krow && i < ch.y) {
-        bf16* dst = o + (long long)(ch.x + i) * o_t + half * 16;
+      uint32_t v[4][4 * NB];
+      float y[4 * NB], x[4 * NB];
+      const uint32_t qs = quad + (LATE && (n & 1) ? D6 : D4);
+      tmem_ld_frag(qs, v[0]), tmem_ld_frag(qs + 32, v[1]);
+      tmem_ld_frag(quad + DPU, v[2]), tmem_ld_frag(quad + DPU + 32, v[3]);
+      tc_wait_ld();
+      add_halves(v[0], v[1], y), add_halves(v[2], v[3], x);
 #pragma unroll
-        for (int e = 0; e < 16; e += 8)
-          if (half * 16 + e < a.vcols)
-            *reinterpret_cast<uint4*>(dst + e) =
-                make_uint4(pack_bf16x2(f * y[e] + x[e], f * y[e + 1] + x[e + 1]), pack_bf16x2(f * y[e + 2] + x[e + 2], f * y[e + 3] + x[e + 3]),
-                           pack_bf16x2(f * y[e + 4] + x[e + 4], f * y[e + 5] + x[e + 5]), pack_bf16x2(f * y[e + 6] + x[e + 6], f * y[e + 7] + x[e + 7]));
-      }
+      for (int e = 0; e < 4 * NB; ++e) x[e] += f[(e >> 1) & 1] * y[e];
+      store_frag(o + (long long)(ch.x + orow) * o_t + fcol, orow < ch.y, a.vcols - fcol, x);
       tc_fence_before();
       __syncwarp();
     };
     const int steps = a.c1 - a.c0;
     int4 ch = steps > 0 ? chunks[a.c0] : make_int4(0, 0, 0, 0), old = ch;
-    float fo = 0.f;                          // gamma rq of the chunk before
+    float fo[2] = {};                        // gamma rq of the chunk before
     for (int n = 0; n < steps; ++n) {
       const uint32_t st = a.sm + (n % STAGES) * STAGE, hd = st + ST_HD, rqk = st + ST_RQK;
-      put_row(a.sm + L::SM_S, r, half, s, hi, lo);
+      put_row(a.sm + L::SM_S, r, u0, s);
       a.wait(&a.bars->full[n % STAGES], (n / STAGES) & 1, 3);
       if (ch.y < C) clear_rows(st, ch.y);
       fence_proxy_async_smem();
       tc_fence_before();
       bar_arrive(1, FIRST);
-      if (OUT && q4 >= 2 && n > 0) finish(n - 1, old, fo);
+      if (OUT && !LATE && n > 0) finish(n - 1, old, fo);
       // row factors, and v, while the first product runs
-      const float gam = ex2_sum(hd, i), dec = ex2_diff(hd, C - 1, i), last = ex2_sum(hd, C - 1), b = ldsf(hd + (2 * C + i) * 4);
-      const float rq = ldsf(rqk + i * 4), rk = ldsf(rqk + (C + i) * 4);
-      const int len = ch.y;
-      uint4 xv[2];
-      read_x(st + ST_X, i, half, krow && i < len, xv);
-      old = ch, fo = gam * rq;
+      const float last = ex2_sum(hd, C - 1);
+      float f[2], b[2], dec[2], fn[2];
+      uint32_t v[NB][2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int i = row[h];
+        const float gam = ex2_sum(hd, i), rk = ldsf(rqk + (C + i) * 4);
+        f[h] = gam * rk, b[h] = ldsf(hd + (2 * C + i) * 4), dec[h] = ex2_diff(hd, C - 1, i) * rk;
+        fn[h] = gam * ldsf(rqk + i * 4);
+#pragma unroll
+        for (int m = 0; m < NB; ++m) v[m][h] = i < ch.y ? lds32(st + ST_X + swz<4>(i, u0 + m) + (lane & 3) * 4) : 0u;
+      }
+      const int4 now = ch;
       if (n + 1 < steps) ch = chunks[a.c0 + n + 1];
-      float x[16];
+      float x[4 * NB], z[4 * NB];
       a.wait(&a.bars->done[0], n & 1, 4);
       tc_fence_after();
-      read_acc(acc + D1, y);
-      if (krow) {                            // R = b (V - gamma rk K S)
-        floats(xv, x);
-        const float f = gam * rk;
+      read_frag(quad + D1, x);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = b * (x[e] - f * y[e]);
-        put_row(a.sm + L::SM_B2, i, half, x, hi, lo);
+      for (int e = 0; e < 4 * NB; e += 2) {  // R = b (V - gamma rk K S)
+        const int h = (e >> 1) & 1;
+        const float2 w = unpack_bf16x2(v[e >> 2][h]);
+        x[e] = b[h] * (w.x - f[h] * x[e]), x[e + 1] = b[h] * (w.y - f[h] * x[e + 1]);
       }
+      put_frag(f2, x);
       fence_proxy_async_smem();
       tc_fence_before();
       bar_arrive(2, MEET);
+      if (OUT && LATE && n > 0) finish(n - 1, old, fo);
+      old = now, fo[0] = fn[0], fo[1] = fn[1];
       a.wait(&a.bars->done[1], n & 1, 5);
       tc_fence_after();
-      if (krow) {                            // d rk U, then U itself
-        read_acc(acc + D2, x);
-        float z[16];
-        const float f = dec * rk;
+      read_frag(quad + D2, x);               // d rk U, then U itself
 #pragma unroll
-        for (int e = 0; e < 16; ++e) z[e] = f * x[e];
-        put_row(a.sm + L::SM_B3, i, half, z, hi, lo);
-      }
+      for (int e = 0; e < 4 * NB; ++e) z[e] = dec[(e >> 1) & 1] * x[e];
+      put_frag(f3, z);
       fence_proxy_async_smem();
       tc_fence_before();
       bar_arrive(3, MEET);
       if (SAVE) a.wait(&a.bars->kept, n & 1, 8);          // the tiles on their way out have been read
-      if (krow) put_row(a.sm + L::SM_U, i, half, x, hi, lo);
+      put_frag(fu, x);
       fence_proxy_async_smem();
       if (OUT) bar_arrive(4, MEET);
       a.wait(&a.bars->done[2], n & 1, 6);
       tc_fence_after();
-      float z[16];
-      read_acc(acc + D3, z);
+      float d[8 * NB];
+      read_rows(quad + D3, d);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] = last * s[e] + z[e];
+      for (int e = 0; e < 8 * NB; ++e) s[e] = last * s[e] + d[e];
     }
-    if (OUT && q4 >= 2 && steps > 0) finish(steps - 1, old, fo);
+    if (OUT && steps > 0) finish(steps - 1, old, fo);
     if (SAVE && steps > 0) bar_arrive(1, FIRST);
-    if (p.s_out != nullptr) state_row(p.s_out + soff, p.s_k, p.s_v, r, p.dk, half * 16, a.vcols, true, s);
+    if (p.s_out != nullptr) state_row(p.s_out + soff, p.s_k, p.s_v, r, p.dk, fcol, a.vcols, true, s);
   }
-  cta_end(a);
+  cta_end<COLS>(a);
 }
 
 // dS through one document, last chunk first.
@@ -710,7 +744,7 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
     zero_rows(p, a, dv, dv_t);
     return;
   }
-  cta_begin(a);
+  cta_begin<256>(a);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, steps = a.c1 - a.c0;
   const int4* chunks = reinterpret_cast<const int4*>(p.chunks);
   constexpr int FIRST = MEET + 32;
@@ -778,14 +812,14 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
     }
     if (steps > 0) bar(1, FIRST);
   } else {
-    const int q4 = warp & 3, half = warp >> 2, r = q4 * 32 + lane, i = r & 63;
+    const int q4 = warp & 3, part = warp >> 2, r = q4 * 32 + lane, i = r & 63, r0 = q4 * 16, g = lane >> 2;
+    const int row[2] = {r0 + g, r0 + g + 8}, u0 = part * NB, fcol = u0 * 8, orow = r0 + frag_row();
     const bool krow = r < C;
-    const int ri = q4 * 16 + (lane & 15);    // row of a 64-row accumulator: 16 lanes of every warp
-    const uint32_t acc = a.tmem + ((uint32_t)(q4 * 32) << 16) + half * 16;
+    const uint32_t quad = a.tmem + ((uint32_t)(q4 * 32) << 16) + fcol;
+    const uint32_t f2 = frag_addr(a.sm + L::SM_B2, r0, u0), f3 = frag_addr(a.sm + L::SM_B3, r0, u0), fu = frag_addr(a.sm + L::SM_U, r0, u0);
     const long long soff = ((long long)a.doc * p.Hv + a.h) * p.dk * p.dv + a.v0 * p.s_v;
-    float s[16] = {}, x[16];
-    uint32_t hi[8], lo[8];
-    if (p.ds_out != nullptr) state_row(const_cast<float*>(p.ds_out) + soff, p.s_k, p.s_v, r, p.dk, half * 16, a.vcols, false, s);
+    float s[8 * NB] = {};
+    if (p.ds_out != nullptr) state_row(const_cast<float*>(p.ds_out) + soff, p.s_k, p.s_v, r, p.dk, fcol, a.vcols, false, s);
     // operands that need dO alone: dO beside Y's tile, gamma rq dO of the third product (threads of Q's rows)
     auto put_dy = [&](int n) {
       const int len = chunks[a.c1 - 1 - n].y;
@@ -793,16 +827,20 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       a.wait(&a.bars->full[n & 1], (n >> 1) & 1, 3);
       if (len < C) clear_rows(st, len);
       if (krow) return;
-      uint4 v[2];
-      read_x(st + ST_X, i, half, i < len, v);
-      const uint32_t row = a.sm + L::SM_B2 + r * 128;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) sts128(row + (((half * 2 + e) ^ (r & 7)) << 4), v[e].x, v[e].y, v[e].z, v[e].w);
       const float f = ex2_sum(st + ST_HD, i) * ldsf(st + ST_RQK + i * 4);
-      floats(v, x);
+      float x[8 * NB];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) x[e] *= f;
-      put_row(a.sm + L::SM_B3, r, half, x, hi, lo);
+      for (int m = 0; m < NB; ++m) {
+        const uint4 v = i < len ? lds128(st + ST_X + swz<4>(i, u0 + m)) : make_uint4(0, 0, 0, 0);
+        sts128(a.sm + L::SM_B2 + r * 128 + (((u0 + m) ^ (r & 7)) << 4), v.x, v.y, v.z, v.w);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 y = unpack_bf16x2(w[e]);
+          x[8 * m + 2 * e] = f * y.x, x[8 * m + 2 * e + 1] = f * y.y;
+        }
+      }
+      put_row(a.sm + L::SM_B3, r, u0, x);
     };
     if (steps > 0) {
       put_dy(0);
@@ -814,50 +852,44 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       const int len = ch.y;
       const long long t0 = ch.x;
       const uint32_t st = a.sm + (n & 1) * STAGE, hd = st + ST_HD, rqk = st + ST_RQK;
-      put_row(a.sm + L::SM_S, r, half, s, hi, lo);
+      put_row(a.sm + L::SM_S, r, u0, s);
       fence_proxy_async_smem();
       tc_fence_before();
       bar_arrive(1, FIRST);
-      const float last = ex2_sum(hd, C - 1), rk = ldsf(rqk + (C + ri) * 4), f1 = ex2_diff(hd, C - 1, ri) * rk;
-      const float b = ldsf(hd + (2 * C + ri) * 4), f2 = -b * ex2_sum(hd, ri) * rk;
+      const float last = ex2_sum(hd, C - 1);
+      float w1[2], w2[2], b[2], x[4 * NB], y[4 * NB];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float rk = ldsf(rqk + (C + row[h]) * 4);
+        b[h] = ldsf(hd + (2 * C + row[h]) * 4), w1[h] = ex2_diff(hd, C - 1, row[h]) * rk, w2[h] = -b[h] * ex2_sum(hd, row[h]) * rk;
+      }
       a.wait(&a.bars->done[0], n & 1, 4);
       tc_fence_after();
       {                                      // Y = d rk K dS' + P^T dO
-        uint32_t v[16];
-        tmem_ld_32x16(acc + D4, v);
-        read_acc(acc + D1, x);
+        uint32_t v[4 * NB];
+        tmem_ld_frag(quad + D4, v);
+        read_frag(quad + D1, x);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = f1 * x[e] + __uint_as_float(v[e]);
-        if (lane < 16) put_row(a.sm + L::SM_B2, ri, half, x, hi, lo);
+        for (int e = 0; e < 4 * NB; ++e) x[e] = w1[(e >> 1) & 1] * x[e] + __uint_as_float(v[e]);
+        put_frag(f2, x);
       }
       fence_proxy_async_smem();
       tc_fence_before();
       bar_arrive(2, MEET);
       a.wait(&a.bars->done[1], n & 1, 5);
       tc_fence_after();
-      float dr[16];
-      read_acc(acc + D2, dr);
-      if (lane < 16) {                       // -b gamma rk dR
+      read_frag(quad + D2, x);               // -b gamma rk dR
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = f2 * dr[e];
-        put_row(a.sm + L::SM_B3, ri, half, x, hi, lo);
-      }
+      for (int e = 0; e < 4 * NB; ++e) y[e] = w2[(e >> 1) & 1] * x[e];
+      put_frag(f3, y);
       fence_proxy_async_smem();
       tc_fence_before();
       bar_arrive(3, MEET);
       a.wait(&a.bars->kept, n & 1, 8);       // the tiles on their way out have been read
-      if (lane < 16) {
-        put_row(a.sm + L::SM_U, ri, half, dr, hi, lo);
-        if (ri < len) {
-          bf16* dst = dv + (t0 + ri) * dv_t + half * 16;
+      put_frag(fu, x);
 #pragma unroll
-          for (int e = 0; e < 16; e += 8)
-            if (half * 16 + e < a.vcols)
-              *reinterpret_cast<uint4*>(dst + e) = make_uint4(pack_bf16x2(b * dr[e], b * dr[e + 1]), pack_bf16x2(b * dr[e + 2], b * dr[e + 3]),
-                                                              pack_bf16x2(b * dr[e + 4], b * dr[e + 5]), pack_bf16x2(b * dr[e + 6], b * dr[e + 7]));
-        }
-      }
-      __syncwarp();
+      for (int e = 0; e < 4 * NB; ++e) x[e] *= b[(e >> 1) & 1];
+      store_frag(dv + (t0 + orow) * dv_t + fcol, orow < len, a.vcols - fcol, x);
       if (n + 1 < steps) {                   // beside the third product: the first two have read these rows
         ch = chunks[a.c1 - 2 - n];
         put_dy(n + 1);
@@ -866,15 +898,16 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       }
       a.wait(&a.bars->done[2], n & 1, 6);
       tc_fence_after();
-      read_acc(acc + D3, x);
+      float d[8 * NB];
+      read_rows(quad + D3, d);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] = last * s[e] + x[e];
+      for (int e = 0; e < 8 * NB; ++e) s[e] = last * s[e] + d[e];
     }
     fence_proxy_async_smem();
     if (steps > 0) bar_arrive(1, FIRST);
-    if (p.ds_in != nullptr) state_row(p.ds_in + soff, p.s_k, p.s_v, r, p.dk, half * 16, a.vcols, true, s);
+    if (p.ds_in != nullptr) state_row(p.ds_in + soff, p.s_k, p.s_v, r, p.dk, fcol, a.vcols, true, s);
   }
-  cta_end(a);
+  cta_end<256>(a);
 }
 
 template <auto KERNEL, int SMEM>
