@@ -530,6 +530,8 @@ __device__ __forceinline__ void cta_end(Cta& a) {
     tmem_dealloc(a.tmem, COLS);
   }
 }
+// A descriptor `bytes` further on.
+__device__ __forceinline__ uint64_t ahead(uint64_t desc, int bytes) { return desc + (uint64_t)(bytes >> 4); }
 // rows outside the documents: zeros
 __device__ __forceinline__ void zero_rows(const XbRecArgs& p, const Cta& a, bf16* out, long long ld) {
   const int4* chunks = reinterpret_cast<const int4*>(p.chunks);
@@ -587,16 +589,19 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
   } else if (warp == ISSUER) {
     const bool one = xb_elect_one();
     constexpr uint32_t id = xb_idesc(1, 1, 64, 64, 0, 1);
+    const uint64_t b1 = xb_smem_desc(MNMAJ, a.sm + L::SM_S), b2 = xb_smem_desc(MNMAJ, a.sm + L::SM_B2), b3 = xb_smem_desc(MNMAJ, a.sm + L::SM_B3),
+                   u = xb_smem_desc(MNMAJ, a.sm + L::SM_U);
+    const int ksteps = (p.dk + 15) / 16;           // columns of K and Q behind dk are zeros
     for (int n = 0; n < a.c1 - a.c0; ++n) {
-      const uint32_t st = xb_smem_u32(a.smem + (n % STAGES) * STAGE), b1 = xb_smem_u32(a.smem + L::SM_S), b2 = xb_smem_u32(a.smem + L::SM_B2),
-                     b3 = xb_smem_u32(a.smem + L::SM_B3);
+      const uint32_t st = a.sm + (n % STAGES) * STAGE;
+      const uint64_t kq = xb_smem_desc(KMAJ, st + ST_KQ), kt = xb_smem_desc(MNMAJ, st + ST_KQ), tp = xb_smem_desc(KMAJ, st + ST_TP);
+      if (one) a.wait1(&a.bars->full[n % STAGES], (n / STAGES) & 1, 1);
       bar(1, FIRST);
       if (one) {
-        a.wait1(&a.bars->full[n % STAGES], (n / STAGES) & 1, 1);
         tc_fence_after();
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          tc_mma_f16_ss(a.tmem + D1, xb_smem_desc(KMAJ, st + ST_KQ + (k >> 2) * HALF + (k & 3) * 32), xb_smem_desc(MNMAJ, b1 + k * 2048), id, k > 0);
+          if (k < ksteps) tc_mma_f16_ss(a.tmem + D1, ahead(kq, (k >> 2) * HALF + (k & 3) * 32), ahead(b1, k * 2048), id, k > 0);
         tc_commit(&a.bars->done[0]);
       }
       bar(2, MEET);
@@ -604,12 +609,13 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
         tc_fence_after();
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          tc_mma_f16_ss(a.tmem + D2, xb_smem_desc(KMAJ, st + ST_TP + (k >> 2) * TP_PLANE + (k & 3) * 32), xb_smem_desc(MNMAJ, b2 + (k & 3) * 2048), id, k > 0);
+          tc_mma_f16_ss(a.tmem + D2, ahead(tp, (k >> 2) * TP_PLANE + (k & 3) * 32), ahead(b2, (k & 3) * 2048), id, k > 0);
         tc_commit(&a.bars->done[1]);
         if (OUT) {
 #pragma unroll
           for (int k = 0; k < 8; ++k)        // Q S: nobody waits for it
-            tc_mma_f16_ss(a.tmem + (LATE && (n & 1) ? D6 : D4), xb_smem_desc(KMAJ, st + ST_KQ + HALF / 2 + (k >> 2) * HALF + (k & 3) * 32), xb_smem_desc(MNMAJ, b1 + k * 2048), id, k > 0);
+            if (k < ksteps)
+              tc_mma_f16_ss(a.tmem + (LATE && (n & 1) ? D6 : D4), ahead(kq, HALF / 2 + (k >> 2) * HALF + (k & 3) * 32), ahead(b1, k * 2048), id, k > 0);
         }
       }
       bar(3, MEET);
@@ -618,17 +624,16 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
         constexpr uint32_t id3 = xb_idesc(1, 1, 128, 64, 1, 1);
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          tc_mma_f16_ss(a.tmem + D3, xb_smem_desc(MNMAJ, st + ST_KQ + k * 2048), xb_smem_desc(MNMAJ, b3 + k * 2048), id3, k > 0);
+          tc_mma_f16_ss(a.tmem + D3, ahead(kt, k * 2048), ahead(b3, k * 2048), id3, k > 0);
         tc_commit(&a.bars->done[2]);
       }
       if (OUT) {
         bar(4, MEET);
         if (one) {
           tc_fence_after();
-          const uint32_t u = xb_smem_u32(a.smem + L::SM_U);
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            tc_mma_f16_ss(a.tmem + DPU, xb_smem_desc(KMAJ, st + ST_TP + HALF / 2 + (k >> 2) * TP_PLANE + (k & 3) * 32), xb_smem_desc(MNMAJ, u + (k & 3) * 2048), id, k > 0);
+            tc_mma_f16_ss(a.tmem + DPU, ahead(tp, HALF / 2 + (k >> 2) * TP_PLANE + (k & 3) * 32), ahead(u, (k & 3) * 2048), id, k > 0);
           tc_commit(&a.bars->done[3]);
         }
       }
@@ -767,37 +772,38 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
     }
   } else if (warp == ISSUER) {
     const bool one = xb_elect_one();
+    const uint64_t b1 = xb_smem_desc(MNMAJ, a.sm + L::SM_S), b2 = xb_smem_desc(MNMAJ, a.sm + L::SM_B2), b3 = xb_smem_desc(MNMAJ, a.sm + L::SM_B3);
+    const int ksteps = (p.dk + 15) / 16;
     for (int n = 0; n < steps; ++n) {
-      const uint32_t st = xb_smem_u32(a.smem + (n & 1) * STAGE), b1 = xb_smem_u32(a.smem + L::SM_S), b2 = xb_smem_u32(a.smem + L::SM_B2),
-                     b3 = xb_smem_u32(a.smem + L::SM_B3);
+      const uint32_t st = a.sm + (n & 1) * STAGE;
+      const uint64_t kq = xb_smem_desc(KMAJ, st + ST_KQ), kt = xb_smem_desc(MNMAJ, st + ST_KQ), tp = xb_smem_desc(MNMAJ, st + ST_TP);
       constexpr uint32_t id3 = xb_idesc(1, 1, 128, 64, 1, 1);
       constexpr uint32_t id1 = xb_idesc(1, 1, 64, 64, 0, 1), id2 = xb_idesc(1, 1, 64, 64, 1, 1), id4 = xb_idesc(1, 1, 64, 32, 1, 1);
+      if (one) a.wait1(&a.bars->full[n & 1], (n >> 1) & 1, 1);
       bar(4, MEET);
       if (one) {
-        a.wait1(&a.bars->full[n & 1], (n >> 1) & 1, 1);
         tc_fence_after();
 #pragma unroll
         for (int k = 0; k < 8; ++k)          // P^T dO
-          tc_mma_f16_ss(a.tmem + D4, xb_smem_desc(MNMAJ, st + ST_TP + (k >> 2) * TP_PLANE + HALF / 2 + (k & 3) * 2048),
-                        xb_smem_desc(MNMAJ, b2 + HALF / 2 + (k & 3) * 2048), id4, k > 0);
+          tc_mma_f16_ss(a.tmem + D4, ahead(tp, (k >> 2) * TP_PLANE + HALF / 2 + (k & 3) * 2048), ahead(b2, HALF / 2 + (k & 3) * 2048), id4, k > 0);
       }
       bar(1, FIRST);
       if (one) {
         tc_fence_after();
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          tc_mma_f16_ss(a.tmem + D1, xb_smem_desc(KMAJ, st + ST_KQ + (k >> 2) * HALF + (k & 3) * 32), xb_smem_desc(MNMAJ, b1 + k * 2048), id1, k > 0);
+          if (k < ksteps) tc_mma_f16_ss(a.tmem + D1, ahead(kq, (k >> 2) * HALF + (k & 3) * 32), ahead(b1, k * 2048), id1, k > 0);
         tc_commit(&a.bars->done[0]);
 #pragma unroll
         for (int k = 4; k < 8; ++k)          // rows of Q
-          tc_mma_f16_ss(a.tmem + D3, xb_smem_desc(MNMAJ, st + ST_KQ + k * 2048), xb_smem_desc(MNMAJ, b3 + k * 2048), id3, k > 4);
+          tc_mma_f16_ss(a.tmem + D3, ahead(kt, k * 2048), ahead(b3, k * 2048), id3, k > 4);
       }
       bar(2, MEET);
       if (one) {
         tc_fence_after();
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          tc_mma_f16_ss(a.tmem + D2, xb_smem_desc(MNMAJ, st + ST_TP + (k >> 2) * TP_PLANE + (k & 3) * 2048), xb_smem_desc(MNMAJ, b2 + (k & 3) * 2048), id2, k > 0);
+          tc_mma_f16_ss(a.tmem + D2, ahead(tp, (k >> 2) * TP_PLANE + (k & 3) * 2048), ahead(b2, (k & 3) * 2048), id2, k > 0);
         tc_commit(&a.bars->done[1]);
       }
       bar(3, MEET);
@@ -805,7 +811,7 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
         tc_fence_after();
 #pragma unroll
         for (int k = 0; k < 4; ++k)          // rows of K
-          tc_mma_f16_ss(a.tmem + D3, xb_smem_desc(MNMAJ, st + ST_KQ + k * 2048), xb_smem_desc(MNMAJ, b3 + k * 2048), id3, 1);
+          tc_mma_f16_ss(a.tmem + D3, ahead(kt, k * 2048), ahead(b3, k * 2048), id3, 1);
         tc_commit(&a.bars->done[2]);
       }
       __syncwarp();
