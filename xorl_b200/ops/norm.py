@@ -140,7 +140,7 @@ class _GatedRMSNorm(torch.autograd.Function):
         x2, z2 = _norm_rows(x2), _norm_rows(z2)
         wc = w if w.is_contiguous() else w.contiguous()
         T, groups, dev = x2.shape[0], W // group_size, x.device
-        y = torch.empty((T, W), dtype=x.dtype, device=dev)
+        y = torch.empty_like(x2, memory_format=torch.contiguous_format)
         rstd = torch.empty((T, groups), dtype=torch.float32, device=dev) if True in ctx.needs_input_grad else None
         shared, wide = int(w.numel() == group_size), int(w.dtype == torch.float32)
         _lib.call_on(dev, "xb_gated_norm_fwd", x2.data_ptr(), x2.stride(0), z2.data_ptr(), z2.stride(0), wc.data_ptr(), wide,
@@ -159,7 +159,7 @@ class _GatedRMSNorm(torch.autograd.Function):
         T, W = x.shape
         dev = x.device
         dy = _norm_rows(dy if dy.dim() == 2 else dy.reshape(T, W))
-        dx, dz = torch.empty((T, W), dtype=x.dtype, device=dev), torch.empty((T, W), dtype=x.dtype, device=dev)
+        dx, dz = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (x, z))
         part = dw = None
         want, out_wide = ctx.needs_input_grad[2], 0
         if want:

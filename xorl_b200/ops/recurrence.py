@@ -13,8 +13,8 @@ read strided inputs in place when the last dimension is contiguous and rows star
 others.  A call allocates its workspace; it does not synchronise and may be captured into a CUDA graph."""
 from __future__ import annotations
 
-import ctypes
 import functools
+import struct
 from typing import Optional
 
 import torch
@@ -40,14 +40,15 @@ def launch_count() -> int:
     return _launches
 
 
-_Words = ctypes.c_longlong * 56      # the fields of XbRecArgs (csrc/recurrence.cu)
+_pack = struct.Struct("56q").pack      # the fields of XbRecArgs (csrc/recurrence.cu)
+_CONTIGUOUS = torch.contiguous_format
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """``x`` [T, heads, dim] as the kernels read it: itself, or a copy where its strides do not suit 16-byte loads."""
     t, h, d = x.stride()
     if d != 1 or t % 8 or h % 8 or t <= 0 or h <= 0 or x.data_ptr() % 16:
-        return x.clone(memory_format=torch.contiguous_format)
+        return x.clone(memory_format=_CONTIGUOUS)
     return x
 
 
@@ -55,7 +56,7 @@ def _state(x: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     """A state as the kernels read it: contiguous, on a 16-byte boundary."""
     if x is None or (x.is_contiguous() and x.data_ptr() % 16 == 0):
         return x
-    return x.clone(memory_format=torch.contiguous_format)
+    return x.clone(memory_format=_CONTIGUOUS)
 
 
 @functools.lru_cache(maxsize=256)
@@ -97,7 +98,7 @@ def _words(q, k, v, g, b, A, D, cu, s_in, s_out, ds_out, ds_in, dy, outs, ws, tm
         back = [base + o if o >= 0 else 0 for o in later]
     # state and U tiles come from the forward pass or are made again; dS and dR tiles and partial sums are the backward's
     work += back[3:] + back[:3] if not keep else back[:3]
-    return _Words(q.data_ptr(), k.data_ptr(), v.data_ptr(), 0 if dy is None else dy.data_ptr(), qs[0], qs[1], ks[0], ks[1],
+    return _pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), 0 if dy is None else dy.data_ptr(), qs[0], qs[1], ks[0], ks[1],
                   vs[0], vs[1], *((0, 0) if dy is None else dy.stride()[:2]),
                   0 if g is None else g.data_ptr(), b.data_ptr(), *((0, 0) if g is None else g.stride()), bs[0], bs[1],
                   _ptr(A), _ptr(D), cu.data_ptr(), _ptr(s_in), _ptr(s_out), _ptr(ds_out), _ptr(ds_in),
@@ -124,7 +125,7 @@ class _Recurrence(torch.autograd.Function):
         step = STEP if not train and T <= STEP * max(docs, 1) else 0
         lay = _layout(T, docs, Hk, Hv, dk, dv, delta, train, step)
         ws = torch.empty(lay[1], dtype=torch.uint8, device=dev)
-        o = torch.empty((T, Hv, dv), dtype=v.dtype, device=dev)
+        o = torch.empty_like(v, memory_format=_CONTIGUOUS)
         s_out = torch.empty((docs, Hv, dk, dv) if delta else (docs, Hv, dv, dk), dtype=torch.float32, device=dev) if final else None
         _lib.call_on(dev, "xb_recurrence_fwd", _words(q, k, v, g, b, A, D, cu, s_in, s_out, None, None, None,
                                                       (o.data_ptr(), 0, 0, 0, 0, 0, 0, 0), ws, None, lay, delta, l2norm, step),
@@ -141,21 +142,16 @@ class _Recurrence(torch.autograd.Function):
         global _launches
         q, k, v, g, b, A, D, s_in, cu, ws = ctx.saved_tensors
         delta, scale, l2norm, lay = ctx.conf
-        T, Hk, dk = q.shape
-        _, Hv, dv = v.shape
         dev = q.device
-        dy = torch.zeros((T, Hv, dv), dtype=v.dtype, device=dev) if dy is None else _rows(dy)
+        dy = torch.zeros_like(v, memory_format=_CONTIGUOUS) if dy is None else _rows(dy)
         ds_out = _state(ds_out)
         ds_in = torch.empty_like(s_in) if ctx.needs_input_grad[7] else None
-        dq = torch.empty((T, Hk, dk), dtype=q.dtype, device=dev)
-        dkk = torch.empty((T, Hk, dk), dtype=q.dtype, device=dev)
-        dvv = torch.empty((T, Hv, dv), dtype=v.dtype, device=dev)
-        db = torch.empty((T, Hv), dtype=torch.float32, device=dev)
+        dq, dkk, dvv = (torch.empty_like(t, memory_format=_CONTIGUOUS) for t in (q, k, v))
+        db = torch.empty_like(b, memory_format=_CONTIGUOUS)
         if delta:
-            dg, dA, dD = torch.empty((T, Hv), dtype=torch.float32, device=dev), None, None
+            dg, dA, dD = torch.empty_like(b, memory_format=_CONTIGUOUS), None, None
         else:
-            dg = None
-            dA, dD = (torch.empty(Hv, dtype=torch.float32, device=dev) for _ in range(2))
+            dg, dA, dD = None, torch.empty_like(A), torch.empty_like(D)
         tmp = torch.empty(lay[2], dtype=torch.uint8, device=dev)
         _lib.call_on(dev, "xb_recurrence_bwd", _words(q, k, v, g, b, A, D, cu, s_in, None, ds_out, ds_in, dy,
                                                (0, dq.data_ptr(), dkk.data_ptr(), dvv.data_ptr(), _ptr(dg), db.data_ptr(),
