@@ -3,12 +3,12 @@
 //
 // A chunk's chain  K S -> R -> U = T R -> S' = gamma S + K^T d U  is sequential, and with one long document there are
 // only heads x column slices of them (32 x 4 for 32 heads of 128), less than one per SM: the time of a step is what
-// counts.  A CTA carries 32 state columns through three products per step, all of them 128 rows high:
+// counts.  A CTA carries 32 state columns through three products per step that wait for one another:
 //
-//   forward   [K; Q] S      -> R (rows of K), gamma Q S (rows of Q)
-//             [T; P] R      -> U
+//   forward   K S           -> R
+//             T R           -> U
 //             K^T (d U)     -> added to the state, whose 128 rows live in the registers of 128 x 2 threads
-//             [T; P] U      -> P U, beside the next step
+//             Q S, P U      -> O, beside the chain
 //   backward  P^T dO        -> beside the step before
 //             K dS'         -> Y = d K dS' + P^T dO
 //             T^T Y         -> dR
@@ -16,9 +16,15 @@
 //
 // A computed operand enters as two bf16 parts side by side, [hi | lo], 64 columns of one product; the parts of T and
 // P are two products into the same accumulator.  P = tril(D o Q K^T) and T = (I + L)^-1 depend on the chunk alone and
-// come from the prepare kernel as operand tiles.  Eight warps work on the accumulators, one row and 16
-// columns per thread (row factors are scalars there), one issues the products, one moves tiles in and out.  mma.sync spent 5800
-// cycles on a forward step (1100 of them on cp.async, 2300 in the tensor pipe): 789 us for 16384 tokens of 32 heads.
+// come from the prepare kernel as operand tiles.  Products with 64 rows lie in half of each warp's lanes and are read as
+// fragments, which gives every lane values.  Eight warps work on the accumulators, one issues the products, one moves
+// tiles in and out.
+//
+// A forward step takes 2800 cycles: three times about 450 of products and their latency, the rest on the way from
+// accumulator to operand (four or sixteen warps on it: 2 % and 13 % more; mma.sync instead of tcgen05: 5800 cycles).  32
+// heads of 128 x 128: forward 376 us for a document of 16384 tokens and 128 us for 4096 tokens in five documents with
+// their tiles kept (0.4 GB written), backward 116 us; prepare 143 and 46 us (268 and 67 MB written: latencies of small
+// steps, three CTAs per SM).
 #include "recurrence_core.cuh"
 
 namespace {

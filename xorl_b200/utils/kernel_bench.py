@@ -8,6 +8,9 @@
     python -m xorl_b200.utils.kernel_bench conv1d --tokens 32768 --hidden 8192 --doc-len 4096
     python -m xorl_b200.utils.kernel_bench dequant4 --n 12288 --k 4096
     python -m xorl_b200.utils.kernel_bench symgemm --m 4096 --k 12288 --block 1024
+    python -m xorl_b200.utils.kernel_bench delta_rule --tokens 4096 --heads 32 --kv-heads 16 --doc-len 1024
+    python -m xorl_b200.utils.kernel_bench ssd_scan --tokens 4096 --heads 128 --kv-heads 8
+    python -m xorl_b200.utils.kernel_bench gated_norm --tokens 16384 --hidden 8192 --block 1024
     python -m xorl_b200.utils.kernel_bench grouped --experts 16 --m 32768 --k 2048 --n 1536
 
 Timing: CUDA events on the launching stream around each run, ``--warmup`` untimed runs, the median
@@ -373,7 +376,54 @@ def bench_mx_quant(a) -> Dict:
     return {"kernel": "quant_mx_rows", "m": a.m, "k": a.k, "ms": ms, "gbs": a.m * a.k * 3 / ms / 1e6}
 
 
+def _forward_and_both(fn, leaves, a) -> Dict:
+    """Milliseconds without gradients, and of a forward and backward pass."""
+    with torch.no_grad():
+        ms = _time(lambda: fn(*leaves), a.warmup, a.iters, a.flush)
+    live = [t.requires_grad_() for t in leaves]
+    dy = torch.randn_like(fn(*live))
+    return {"fwd_ms": ms, "fwd_bwd_ms": _time(lambda: torch.autograd.grad(fn(*live), live, dy), a.warmup, a.iters, a.flush)}
+
+
+def _documents(a) -> torch.Tensor:
+    return torch.tensor([*range(0, a.tokens, a.doc_len or a.tokens), a.tokens], device="cuda", dtype=torch.int32)
+
+
+def bench_delta_rule(a) -> Dict:
+    """Gated delta rule over packed documents, states of 128 x 128, ``--kv-heads`` heads of q and k."""
+    from ..ops.recurrence import gated_delta_rule
+    r = lambda *s: torch.randn(*s, device="cuda")  # noqa: E731
+    T, H, Hk, cu = a.tokens, a.heads, a.kv_heads, _documents(a)
+    leaves = [r(T, Hk, 128).bfloat16(), r(T, Hk, 128).bfloat16(), r(T, H, 128).bfloat16(),
+              -torch.nn.functional.softplus(r(T, H)), torch.sigmoid(r(T, H))]
+    fn = lambda q, k, v, g, b: gated_delta_rule(q, k, v, g, b, cu, scale=128 ** -0.5, qk_l2norm=True)  # noqa: E731
+    return {"kernel": "gated_delta_rule", "tokens": T, "heads": H, "qk_heads": Hk, "documents": cu.numel() - 1,
+            **_forward_and_both(fn, leaves, a)}
+
+
+def bench_ssd_scan(a) -> Dict:
+    """State-space scan over packed documents, states of 64 x 128, ``--kv-heads`` groups."""
+    from ..ops.recurrence import ssd_scan
+    r = lambda *s: torch.randn(*s, device="cuda")  # noqa: E731
+    T, H, G, cu = a.tokens, a.heads, a.kv_heads, _documents(a)
+    leaves = [r(T, H, 64).bfloat16(), 0.1 * torch.nn.functional.softplus(r(T, H)), -1 - torch.rand(H, device="cuda"),
+              r(T, G, 128).bfloat16(), r(T, G, 128).bfloat16(), r(H)]
+    return {"kernel": "ssd_scan", "tokens": T, "heads": H, "groups": G, "documents": cu.numel() - 1,
+            **_forward_and_both(lambda *t: ssd_scan(*t, cu), leaves, a)}
+
+
+def bench_gated_norm(a) -> Dict:
+    """RMS norm over groups of ``--block`` columns behind a SiLU gate."""
+    from ..ops.norm import gated_rms_norm
+    x, z = (torch.randn(a.tokens, a.hidden, device="cuda").bfloat16() for _ in range(2))
+    w = torch.ones(a.hidden, device="cuda").bfloat16()
+    t = _forward_and_both(lambda *s: gated_rms_norm(*s, a.block, norm_first=False), [x, z, w], a)
+    return {"kernel": "gated_rms_norm", "tokens": a.tokens, "hidden": a.hidden, "group": a.block, **t,
+            "fwd_gbs": a.tokens * a.hidden * 6 / t["fwd_ms"] / 1e6}
+
+
 BENCHES["grouped"] = bench_grouped
+BENCHES.update(delta_rule=bench_delta_rule, ssd_scan=bench_ssd_scan, gated_norm=bench_gated_norm)
 BENCHES.update(ce=bench_ce, route=bench_route, qk_norm_rope=bench_qk_norm_rope, permute=bench_permute,
                mx_quant=bench_mx_quant)
 
