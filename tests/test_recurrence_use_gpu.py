@@ -107,6 +107,59 @@ def test_captured_and_replayed(op):
 
 
 @pytest.mark.parametrize("op", OPS)
+def test_captured_without_gradients(op):
+    """A captured call of short documents, replayed with boundaries that make long ones too."""
+    ts = inputs(op, T=128, docs=8)
+    cu = boundaries(list(range(0, 129, 16)))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.no_grad():
+        with torch.cuda.stream(side):
+            call(op, ts, cu)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call(op, ts, cu)
+        for cuts in ([0, 1, 2, 3, 100, 101, 102, 103, 128], [0, 0, 128, 128, 128, 128, 128, 128, 128], [5, 6, 7, 8, 9, 10, 11, 12, 90]):
+            cu.copy_(boundaries(cuts))
+            graph.replay()
+            got = [t.clone() for t in out]
+            same(got, call(op, ts, boundaries(cuts)))
+            us = [t.double() for t in ts]
+            ref = oracle_delta(*us[:5], cuts, 0.125, True, us[5]) if op == "delta" else oracle_scan(*us[:6], cuts, us[6])
+            check(got[0], ref[0], "o")
+            check(got[1], ref[1], "S")
+
+
+@pytest.mark.parametrize("op", OPS)
+def test_entry_points_refuse(op):
+    """What the Python side never hands over is refused before anything is launched: pointers and strides off 16 bytes, sizes
+    beyond the kernels', too few chunks."""
+    from xorl_b200.ops import _lib, recurrence as R
+    ts, cu = inputs(op, T=64, docs=1, state=False), boundaries([0, 64])
+    q, k, v = ts[:3] if op == "delta" else (ts[4], ts[3], ts[0])
+    g, b = (ts[3], ts[4]) if op == "delta" else (None, ts[1])
+    A, D = (None, None) if op == "delta" else (ts[2], ts[5])
+    lay = R._layout(64, 1, 2, 4, 64, 64, op == "delta", False, 0)
+    ws, o = torch.empty(lay[1], dtype=torch.uint8, device="cuda"), torch.empty_like(v)
+
+    def run(q=q, k=k, v=v, lay=lay, step=0, s_in=None):
+        words = R._words(q, k, v, g, b, A, D, cu, s_in, None, None, None, None, (o.data_ptr(), 0, 0, 0, 0, 0, 0, 0), ws, None, lay,
+                         op == "delta", 0, step)
+        _lib.call_on(v.device, "xb_recurrence_fwd", words, 1.0, op == "delta")
+
+    run()
+    wide = torch.zeros(64, 2, 80, dtype=torch.bfloat16, device="cuda")
+    odd = torch.zeros(64 * 4 * 64 + 8, dtype=torch.bfloat16, device="cuda")[1:1 + 64 * 4 * 64].view(64, 4, 64)
+    flat = torch.zeros(64 * 4 * 64 + 4, device="cuda")
+    for bad in (dict(q=wide[:, :, 1:65]), dict(k=torch.zeros(64, 2, 65, device="cuda").bfloat16()[:, :, :64]), dict(v=odd),
+                dict(q=wide[:, :, :60]), dict(lay=(lay[0] - 3, *lay[1:])), dict(step=64), dict(step=-1),
+                dict(s_in=flat[1:1 + 4 * 64 * 64].view(1, 4, 64, 64))):
+        with pytest.raises(RuntimeError, match="xb_recurrence_fwd failed with code -1"):
+            run(**bad)
+
+
+@pytest.mark.parametrize("op", OPS)
 def test_strides_and_alignment(op):
     """Slices of a fused projection, rows off 16 bytes, shared (expanded) heads, other orders, states off 16 bytes."""
     cu = boundaries([0, 70, 71, 300])

@@ -11,7 +11,7 @@
 // Sixteen worker warps, a loading and an issuing warp, and one that turns the heads' sums into gradients of the decay.
 //
 // It reads the tiles that the two sequential passes keep (48 KB per head and 32 columns; scan 32 KB).  4096 tokens of 32
-// heads of 128 x 128: 209 us, 0.43 GB of tiles at 2.1 TB/s; 4095 tokens of 128 heads of 64 x 128: 244 us, 0.56 GB at 2.3
+// heads of 128 x 128: 209 us, 0.45 GB of tiles at 2.1 TB/s; 4095 tokens of 128 heads of 64 x 128: 244 us, 0.58 GB at 2.4
 // TB/s.  All of tensor memory holds one head's five products (scan: two heads' dP and t1), so that loads overlap the
 // workers' turn and products do not; with two heads per CTA a third of the time is its way in and out.
 #include "recurrence_core.cuh"
@@ -63,7 +63,10 @@ __device__ __forceinline__ float2 lds2(uint32_t a) {
   asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
   return v;
 }
-__device__ __forceinline__ void wbar() { asm volatile("bar.sync 1, %0;" ::"n"(WORKERS) : "memory"); }
+__device__ __forceinline__ void wbar() {
+  __syncwarp();
+  asm volatile("bar.sync 1, %0;" ::"n"(WORKERS) : "memory");
+}
 
 // D (64 x N) += A (64 x 16 of a row of 16-column steps) B^T: one step each
 __device__ __forceinline__ void step(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool first) {

@@ -11,7 +11,7 @@
 // outputs, one loads and one issues.  Computed operands are [hi 32 | lo 32] tiles (P: two planes).  Per step and CTA 20
 // products, about 1100 cycles of the tensor pipe of 3500: issue slots (66 % taken) and latencies of the warps that add and
 // split bound it.  128 heads of 64 x 128: forward 473 us for a document of 16384 tokens and 146 us for 4095 tokens in five
-// documents with their states kept (0.28 GB written), backward 148 us; prepare 37 and 11 us.  Eight adding warps instead
+// documents with their states kept (0.29 GB written), backward 148 us; prepare 37 and 11 us.  Eight adding warps instead
 // of sixteen: 1.7 times the time.
 #include "recurrence_core.cuh"
 
@@ -233,6 +233,7 @@ scan_seq(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtenso
           const int part = i / ((C - len) * 8), r = len + (i % ((C - len) * 8)) / 8;
           sts128(st + ST_K + part * T64 + r * 128 + (i & 7) * 16, 0, 0, 0, 0);
         }
+        __syncwarp();                        // named barriers want whole warps
         asm volatile("bar.sync 1, %0;" ::"n"(XMAKERS) : "memory");
       }
       const float gam = ex2_sum(hd, row), db = ex2_diff(hd, C - 1, row) * ldsf(hd + (2 * C + row) * 4), f = BWD ? gam : db;
