@@ -7,6 +7,8 @@ zero-centred ``(1 + w)`` variant.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
@@ -130,6 +132,11 @@ def _norm_rows(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
+@functools.lru_cache(maxsize=256)
+def _gated_norm_partial(T: int, groups: int, group_size: int, shared: int) -> int:
+    return max(_lib.cuda_lib().xb_gated_norm_partial(T, groups, group_size, shared), 1)
+
+
 class _GatedRMSNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate, w, group_size, eps, norm_first):
@@ -161,13 +168,12 @@ class _GatedRMSNorm(torch.autograd.Function):
         dy = _norm_rows(dy if dy.dim() == 2 else dy.reshape(T, W))
         dx, dz = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (x, z))
         part = dw = None
-        want, out_wide = ctx.needs_input_grad[2], 0
+        want, sink, out_wide = ctx.needs_input_grad[2], False, 0
         if want:
-            floats = _lib.cuda_lib().xb_gated_norm_partial(T, groups, group_size, shared)
-            part = torch.empty(max(floats, 1), dtype=torch.float32, device=dev)
+            part = torch.empty(_gated_norm_partial(T, groups, group_size, shared), dtype=torch.float32, device=dev)
             # an engine's buffer takes fp32 sums; a gradient that autograd gets is rounded where it is summed
             sink = grad_target(ctx.w)[0] is not None
-            dw = torch.empty(wc.shape, dtype=torch.float32 if sink else wc.dtype, device=dev)
+            dw = torch.empty_like(wc, dtype=torch.float32) if sink else torch.empty_like(wc)
             out_wide = int(sink or wide)
         _lib.call_on(dev, "xb_gated_norm_bwd", dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), z.data_ptr(), z.stride(0),
                      wc.data_ptr(), wide, shared, rstd.data_ptr(), dx.data_ptr(), dz.data_ptr(), _lib.ptr(part), _lib.ptr(dw),
@@ -175,7 +181,7 @@ class _GatedRMSNorm(torch.autograd.Function):
         _launches += 1 + int(want)
         if len(shape) != 2:
             dx, dz = dx.reshape(shape), dz.reshape(shape)
-        return dx, dz, deliver_param_grad(ctx.w, dw) if want else None, None, None, None
+        return dx, dz, deliver_param_grad(ctx.w, dw) if sink else dw, None, None, None
 
 
 GATED_NORM_MAX_GROUP = 8192
