@@ -22,7 +22,7 @@
 //
 // A forward step takes 2800 cycles: three times about 450 of products and their latency, the rest on the way from
 // accumulator to operand (four or sixteen warps on it: 2 % and 13 % more; mma.sync instead of tcgen05: 5800 cycles).  32
-// heads of 128 x 128: forward 376 us for a document of 16384 tokens and 128 us for 4096 tokens in five documents with
+// heads of 128 x 128: forward 371 us for a document of 16384 tokens and 128 us for 4096 tokens in five documents with
 // their tiles kept (0.22 GB written), backward 116 us; prepare 143 and 46 us (268 and 67 MB written: latencies of small
 // steps, three CTAs per SM).
 #include "recurrence_core.cuh"
@@ -407,13 +407,13 @@ __device__ __forceinline__ void clear_rows(uint32_t st, int len) {
 // Workers: of the state a row and 8 NB columns per thread (warp w: rows 32 (w % 4) .., columns 8 NB (w / 4) ..), of what has
 // 64 rows 16 rows and 8 NB columns per warp, as fragments: of every 8 columns rows g and g + 8, columns 2 t and 2 t + 1,
 // element 4 n + 2 h + column.  An operand tile's row is 128 bytes, [hi 32 | lo 32]; u0 is the warp's first unit of it.
-__device__ __forceinline__ void put_row(uint32_t tile, int row, int u0, const float (&x)[8 * NB]) {
+__device__ __forceinline__ void put_row(uint32_t tile, int row, int u0, const Pair (&x)[4 * NB]) {
   const uint32_t r = tile + row * 128;
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
     uint32_t hi[4], lo[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) split2(x[8 * n + 2 * i], x[8 * n + 2 * i + 1], hi[i], lo[i]);
+    for (int i = 0; i < 4; ++i) split2(x[4 * n + i], hi[i], lo[i]);
     sts128(r + (((u0 + n) ^ (row & 7)) << 4), hi[0], hi[1], hi[2], hi[3]);
     sts128(r + (((u0 + n + 4) ^ (row & 7)) << 4), lo[0], lo[1], lo[2], lo[3]);
   }
@@ -423,70 +423,63 @@ __device__ __forceinline__ uint32_t frag_addr(uint32_t tile, int r0, int u0) {
   const int l = xb_lane(), row = r0 + (l & 15), u = u0 + (l >> 4) * 4;
   return tile + row * 128 + ((u ^ (row & 7)) << 4);
 }
-__device__ __forceinline__ void put_frag(uint32_t addr, const float (&x)[4 * NB]) {
+__device__ __forceinline__ void put_frag(uint32_t addr, const Pair (&x)[2 * NB]) {
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
     uint32_t hi[2], lo[2];
-    split2(x[4 * n], x[4 * n + 1], hi[0], lo[0]), split2(x[4 * n + 2], x[4 * n + 3], hi[1], lo[1]);
+    split2(x[2 * n], hi[0], lo[0]), split2(x[2 * n + 1], hi[1], lo[1]);
     stsm4(addr ^ (n << 4), hi[0], hi[1], lo[0], lo[1]);
   }
 }
 // the sum of an accumulator's two halves
 template <int N>
-__device__ __forceinline__ void add_halves(const uint32_t (&a)[N], const uint32_t (&b)[N], float (&x)[N]) {
+__device__ __forceinline__ void add_halves(const uint32_t (&a)[2 * N], const uint32_t (&b)[2 * N], Pair (&x)[N]) {
 #pragma unroll
-  for (int i = 0; i < N; i += 2) {
-    const float2 f = both(pair(a[i], a[i + 1]) + pair(b[i], b[i + 1]));
-    x[i] = f.x, x[i + 1] = f.y;
-  }
+  for (int i = 0; i < N; ++i) x[i] = pair(a[2 * i], a[2 * i + 1]) + pair(b[2 * i], b[2 * i + 1]);
 }
-__device__ __forceinline__ void read_rows(uint32_t addr, float (&x)[8 * NB]) {
+__device__ __forceinline__ void read_rows(uint32_t addr, Pair (&x)[4 * NB]) {
   uint32_t a[8 * NB], b[8 * NB];
   tmem_ld_rows(addr, a);
   tmem_ld_rows(addr + 32, b);
   tc_wait_ld();
   add_halves(a, b, x);
 }
-__device__ __forceinline__ void read_frag(uint32_t addr, float (&x)[4 * NB]) {
+__device__ __forceinline__ void read_frag(uint32_t addr, Pair (&x)[2 * NB]) {
   uint32_t a[4 * NB], b[4 * NB];
   tmem_ld_frag(addr, a);
   tmem_ld_frag(addr + 32, b);
   tc_wait_ld();
   add_halves(a, b, x);
 }
+__device__ __forceinline__ Pair twice(float x) { return pair(x, x); }
+__device__ __forceinline__ Pair bf16_pair(uint32_t v) { return pair(v << 16, v & 0xffff0000u); }
 // A warp's 16 rows to global memory as bf16: lanes t and t ^ 1 trade, for four columns of one row each.  `dst` is row
 // frag_row() at the warp's first column; `cols` are left from there.
 __device__ __forceinline__ int frag_row() { return (xb_lane() >> 2) + 8 * (xb_lane() & 1); }
-__device__ __forceinline__ void store_frag(bf16* dst, bool on, int cols, const float (&x)[4 * NB]) {
+__device__ __forceinline__ void store_frag(bf16* dst, bool on, int cols, const Pair (&x)[2 * NB]) {
   const bool odd = xb_lane() & 1;
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
-    const uint32_t w0 = pack_bf16x2(x[4 * n], x[4 * n + 1]), w1 = pack_bf16x2(x[4 * n + 2], x[4 * n + 3]);
+    const float2 r0 = both(x[2 * n]), r1 = both(x[2 * n + 1]);
+    const uint32_t w0 = pack_bf16x2(r0.x, r0.y), w1 = pack_bf16x2(r1.x, r1.y);
     const uint32_t other = __shfl_xor_sync(0xffffffffu, odd ? w0 : w1, 1);
     if (on && 8 * n < cols) *reinterpret_cast<uint2*>(dst + 8 * n + 4 * ((xb_lane() >> 1) & 1)) = odd ? make_uint2(other, w1) : make_uint2(w0, other);
   }
 }
 // a thread's part of a state row in global memory
-__device__ __forceinline__ void state_row(float* base, long long sk, long long sv, int row, int dk, int col, int cols, bool store, float (&s)[8 * NB]) {
+__device__ __forceinline__ void state_row(float* base, long long sk, long long sv, int row, int dk, int col, int cols, bool store, Pair (&s)[4 * NB]) {
   if (row >= dk) return;
 #pragma unroll
   for (int i = 0; i < 2 * NB; ++i) {
     if (col + 4 * i >= cols) return;                                 // columns come in multiples of 8
-    if (sv == 1) {
-      float4* at = reinterpret_cast<float4*>(base + row * sk + col) + i;
-      if (store) {
-        *at = make_float4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
-      } else {
-        const float4 v = *at;
-        s[4 * i] = v.x, s[4 * i + 1] = v.y, s[4 * i + 2] = v.z, s[4 * i + 3] = v.w;
-      }
+    float* at = base + row * sk + (col + 4 * i) * sv;
+    if (store) {
+      const float2 a = both(s[2 * i]), b = both(s[2 * i + 1]);
+      if (sv == 1) *reinterpret_cast<float4*>(at) = make_float4(a.x, a.y, b.x, b.y);
+      else at[0] = a.x, at[sv] = a.y, at[2 * sv] = b.x, at[3 * sv] = b.y;
     } else {
-#pragma unroll
-      for (int j = 4 * i; j < 4 * i + 4; ++j) {
-        float* at = base + row * sk + (col + j) * sv;
-        if (store) *at = s[j];
-        else s[j] = *at;
-      }
+      const float4 v = sv == 1 ? *reinterpret_cast<const float4*>(at) : make_float4(at[0], at[sv], at[2 * sv], at[3 * sv]);
+      s[2 * i] = pair(v.x, v.y), s[2 * i + 1] = pair(v.z, v.w);
     }
   }
 }
@@ -652,21 +645,23 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
     const uint32_t quad = a.tmem + ((uint32_t)(q4 * 32) << 16) + fcol;
     const uint32_t f2 = frag_addr(a.sm + L::SM_B2, r0, u0), f3 = frag_addr(a.sm + L::SM_B3, r0, u0), fu = frag_addr(a.sm + L::SM_U, r0, u0);
     const long long soff = ((long long)a.doc * p.Hv + a.h) * p.dk * p.dv + a.v0 * p.s_v;
-    float s[8 * NB] = {};
+    Pair s[4 * NB];
+#pragma unroll
+    for (int e = 0; e < 4 * NB; ++e) s[e] = twice(0.f);
     if (p.s_in != nullptr) state_row(const_cast<float*>(p.s_in) + soff, p.s_k, p.s_v, r, p.dk, fcol, a.vcols, false, s);
     // O = gamma rq Q S + P U of a chunk
     auto finish = [&](int n, int4 ch, const float (&f)[2]) {
       a.wait(&a.bars->done[3], n & 1, 7);
       tc_fence_after();
       uint32_t v[4][4 * NB];
-      float y[4 * NB], x[4 * NB];
+      Pair y[2 * NB], x[2 * NB];
       const uint32_t qs = quad + (LATE && (n & 1) ? D6 : D4);
       tmem_ld_frag(qs, v[0]), tmem_ld_frag(qs + 32, v[1]);
       tmem_ld_frag(quad + DPU, v[2]), tmem_ld_frag(quad + DPU + 32, v[3]);
       tc_wait_ld();
       add_halves(v[0], v[1], y), add_halves(v[2], v[3], x);
 #pragma unroll
-      for (int e = 0; e < 4 * NB; ++e) x[e] += f[(e >> 1) & 1] * y[e];
+      for (int e = 0; e < 2 * NB; ++e) x[e] = fma2(twice(f[e & 1]), y[e], x[e]);
       store_frag(o + (long long)(ch.x + orow) * o_t + fcol, orow < ch.y, a.vcols - fcol, x);
       tc_fence_before();
       __syncwarp();
@@ -677,11 +672,14 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
     for (int n = 0; n < steps; ++n) {
       const uint32_t st = a.sm + (n % STAGES) * STAGE, hd = st + ST_HD, rqk = st + ST_RQK;
       put_row(a.sm + L::SM_S, r, u0, s);
-      a.wait(&a.bars->full[n % STAGES], (n / STAGES) & 1, 3);
-      if (ch.y < C) clear_rows(st, ch.y);
+      if (ch.y < C) {
+        a.wait(&a.bars->full[n % STAGES], (n / STAGES) & 1, 3);
+        clear_rows(st, ch.y);
+      }
       fence_proxy_async_smem();
       tc_fence_before();
       bar_arrive(1, FIRST);
+      a.wait(&a.bars->full[n % STAGES], (n / STAGES) & 1, 3);
       if (OUT && !LATE && n > 0) finish(n - 1, old, fo);
       // row factors, and v, while the first product runs
       const float last = ex2_sum(hd, C - 1);
@@ -698,16 +696,13 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       }
       const int4 now = ch;
       if (n + 1 < steps) ch = chunks[a.c0 + n + 1];
-      float x[4 * NB], z[4 * NB];
+      Pair x[2 * NB], z[2 * NB];
       a.wait(&a.bars->done[0], n & 1, 4);
       tc_fence_after();
       read_frag(quad + D1, x);
 #pragma unroll
-      for (int e = 0; e < 4 * NB; e += 2) {  // R = b (V - gamma rk K S)
-        const int h = (e >> 1) & 1;
-        const float2 w = unpack_bf16x2(v[e >> 2][h]);
-        x[e] = b[h] * (w.x - f[h] * x[e]), x[e + 1] = b[h] * (w.y - f[h] * x[e + 1]);
-      }
+      for (int e = 0; e < 2 * NB; ++e)       // R = b (V - gamma rk K S)
+        x[e] = twice(b[e & 1]) * fma2(twice(-f[e & 1]), x[e], bf16_pair(v[e >> 1][e & 1]));
       put_frag(f2, x);
       fence_proxy_async_smem();
       tc_fence_before();
@@ -718,7 +713,7 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       tc_fence_after();
       read_frag(quad + D2, x);               // d rk U, then U itself
 #pragma unroll
-      for (int e = 0; e < 4 * NB; ++e) z[e] = dec[(e >> 1) & 1] * x[e];
+      for (int e = 0; e < 2 * NB; ++e) z[e] = twice(dec[e & 1]) * x[e];
       put_frag(f3, z);
       fence_proxy_async_smem();
       tc_fence_before();
@@ -729,10 +724,10 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       if (OUT) bar_arrive(4, MEET);
       a.wait(&a.bars->done[2], n & 1, 6);
       tc_fence_after();
-      float d[8 * NB];
+      Pair d[4 * NB];
       read_rows(quad + D3, d);
 #pragma unroll
-      for (int e = 0; e < 8 * NB; ++e) s[e] = last * s[e] + d[e];
+      for (int e = 0; e < 4 * NB; ++e) s[e] = fma2(twice(last), s[e], d[e]);
     }
     if (OUT && steps > 0) finish(steps - 1, old, fo);
     if (SAVE && steps > 0) bar_arrive(1, FIRST);
@@ -830,7 +825,9 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
     const uint32_t quad = a.tmem + ((uint32_t)(q4 * 32) << 16) + fcol;
     const uint32_t f2 = frag_addr(a.sm + L::SM_B2, r0, u0), f3 = frag_addr(a.sm + L::SM_B3, r0, u0), fu = frag_addr(a.sm + L::SM_U, r0, u0);
     const long long soff = ((long long)a.doc * p.Hv + a.h) * p.dk * p.dv + a.v0 * p.s_v;
-    float s[8 * NB] = {};
+    Pair s[4 * NB];
+#pragma unroll
+    for (int e = 0; e < 4 * NB; ++e) s[e] = twice(0.f);
     if (p.ds_out != nullptr) state_row(const_cast<float*>(p.ds_out) + soff, p.s_k, p.s_v, r, p.dk, fcol, a.vcols, false, s);
     // operands that need dO alone: dO beside Y's tile, gamma rq dO of the third product (threads of Q's rows)
     auto put_dy = [&](int n) {
@@ -840,17 +837,14 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       if (len < C) clear_rows(st, len);
       if (krow) return;
       const float f = ex2_sum(st + ST_HD, i) * ldsf(st + ST_RQK + i * 4);
-      float x[8 * NB];
+      Pair x[4 * NB];
 #pragma unroll
       for (int m = 0; m < NB; ++m) {
         const uint4 v = i < len ? lds128(st + ST_X + swz<4>(i, u0 + m)) : make_uint4(0, 0, 0, 0);
         sts128(a.sm + L::SM_B2 + r * 128 + (((u0 + m) ^ (r & 7)) << 4), v.x, v.y, v.z, v.w);
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 y = unpack_bf16x2(w[e]);
-          x[8 * m + 2 * e] = f * y.x, x[8 * m + 2 * e + 1] = f * y.y;
-        }
+        for (int e = 0; e < 4; ++e) x[4 * m + e] = twice(f) * bf16_pair(w[e]);
       }
       put_row(a.sm + L::SM_B3, r, u0, x);
     };
@@ -869,7 +863,8 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       tc_fence_before();
       bar_arrive(1, FIRST);
       const float last = ex2_sum(hd, C - 1);
-      float w1[2], w2[2], b[2], x[4 * NB], y[4 * NB];
+      float w1[2], w2[2], b[2];
+      Pair x[2 * NB], y[2 * NB];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const float rk = ldsf(rqk + (C + row[h]) * 4);
@@ -882,7 +877,7 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
         tmem_ld_frag(quad + D4, v);
         read_frag(quad + D1, x);
 #pragma unroll
-        for (int e = 0; e < 4 * NB; ++e) x[e] = w1[(e >> 1) & 1] * x[e] + __uint_as_float(v[e]);
+        for (int e = 0; e < 2 * NB; ++e) x[e] = fma2(twice(w1[e & 1]), x[e], pair(v[2 * e], v[2 * e + 1]));
         put_frag(f2, x);
       }
       fence_proxy_async_smem();
@@ -892,7 +887,7 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       tc_fence_after();
       read_frag(quad + D2, x);               // -b gamma rk dR
 #pragma unroll
-      for (int e = 0; e < 4 * NB; ++e) y[e] = w2[(e >> 1) & 1] * x[e];
+      for (int e = 0; e < 2 * NB; ++e) y[e] = twice(w2[e & 1]) * x[e];
       put_frag(f3, y);
       fence_proxy_async_smem();
       tc_fence_before();
@@ -900,7 +895,7 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       a.wait(&a.bars->kept, n & 1, 8);       // the tiles on their way out have been read
       put_frag(fu, x);
 #pragma unroll
-      for (int e = 0; e < 4 * NB; ++e) x[e] *= b[(e >> 1) & 1];
+      for (int e = 0; e < 2 * NB; ++e) x[e] = twice(b[e & 1]) * x[e];
       store_frag(dv + (t0 + orow) * dv_t + fcol, orow < len, a.vcols - fcol, x);
       if (n + 1 < steps) {                   // beside the third product: the first two have read these rows
         ch = chunks[a.c1 - 2 - n];
@@ -910,10 +905,10 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       }
       a.wait(&a.bars->done[2], n & 1, 6);
       tc_fence_after();
-      float d[8 * NB];
+      Pair d[4 * NB];
       read_rows(quad + D3, d);
 #pragma unroll
-      for (int e = 0; e < 8 * NB; ++e) s[e] = last * s[e] + d[e];
+      for (int e = 0; e < 4 * NB; ++e) s[e] = fma2(twice(last), s[e], d[e]);
     }
     fence_proxy_async_smem();
     if (steps > 0) bar_arrive(1, FIRST);

@@ -10,7 +10,9 @@ floating input.
 On a GPU with bf16 inputs whose head dims are multiples of 8 (state rows at most 128) the CUDA kernels run; they keep
 every computed value in 32 bits and round outputs once.  Elsewhere the same arithmetic runs as tensor ops.  The kernels
 read strided inputs in place when the last dimension is contiguous and rows start on 16-byte boundaries, and copy
-others.  A call allocates its workspace; it does not synchronise and may be captured into a CUDA graph."""
+others.  A call allocates its workspace; it does not synchronise and may be captured into a CUDA graph (a backward pass:
+while no graph of the same leaves that was built outside the capture is alive, since torch would wait for its stream and end
+the process)."""
 from __future__ import annotations
 
 import functools
