@@ -147,7 +147,7 @@ static XbRecArgs unpack(const long long* w, float scale) {
   ptr(a.A), ptr(a.D), ptr(a.cu), ptr(a.s_in), ptr(a.s_out), ptr(a.ds_out), ptr(a.ds_in), num(a.s_k), num(a.s_v);
   ptr(a.o), ptr(a.dq), ptr(a.dk_out), ptr(a.dv_out), ptr(a.dg), ptr(a.db), ptr(a.dA), ptr(a.dD);
   ptr(a.chunks), ptr(a.doc_off), ptr(a.hd), ptr(a.rqk), ptr(a.qk), ptr(a.kk), ptr(a.pt);
-  ptr(a.s_tiles), ptr(a.u_tiles), ptr(a.ds_tiles), ptr(a.dr_tiles), ptr(a.part);
+  ptr(a.s_tiles), ptr(a.u_tiles), ptr(a.r_tiles), ptr(a.ds_tiles), ptr(a.dr_tiles), ptr(a.part);
   num(a.T), num(a.n_docs), num(a.Hk), num(a.Hv), num(a.dk), num(a.dv), num(a.nc_max), num(a.l2norm), num(a.step);
   a.doc_list = a.doc_off + a.n_docs + 3;
   a.dvp = (a.dv + 63) / 64 * 64;

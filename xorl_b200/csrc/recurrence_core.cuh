@@ -66,6 +66,18 @@ __device__ __forceinline__ void split2(Pair x, uint32_t& hi, uint32_t& lo) {
   const float2 r = both(fma2(pair(hi << 16, hi & 0xffff0000u), pair(-1.f, -1.f), x));
   lo = pack_bf16x2(r.x, r.y);
 }
+// two fp32 values as the sums of three bf16 values each: all 24 bits
+__device__ __forceinline__ void split3(Pair x, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
+  const Pair minus = pair(-1.f, -1.f);
+  const float2 f = both(x);
+  hi = pack_bf16x2(f.x, f.y);
+  const Pair r = fma2(pair(hi << 16, hi & 0xffff0000u), minus, x);
+  const float2 g = both(r);
+  mid = pack_bf16x2(g.x, g.y);
+  const float2 h = both(fma2(pair(mid << 16, mid & 0xffff0000u), minus, r));
+  lo = pack_bf16x2(h.x, h.y);
+}
+
 // A tile is rows of U 16-byte units; unit u of a row lies at u ^ f(row), so that the eight rows that ldmatrix reads
 // at one unit fall into eight different banks.
 template <int U>

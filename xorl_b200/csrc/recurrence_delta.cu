@@ -6,17 +6,18 @@
 // counts.  A CTA carries 32 state columns through three products per step that wait for one another:
 //
 //   forward   K S           -> R
-//             T R           -> U
+//             (T - I) R     -> U = R + (T - I) R
 //             K^T (d U)     -> added to the state, whose 128 rows live in the registers of 128 x 2 threads
 //             Q S, P U      -> O, beside the chain
 //   backward  P^T dO        -> beside the step before
 //             K dS'         -> Y = d K dS' + P^T dO
-//             T^T Y         -> dR
+//             (T - I)^T Y   -> dR = Y + (T - I)^T Y
 //             [K; Q]^T [-b gamma dR; gamma dO] -> added to dS  (the dO part is issued early)
 //
 // A computed operand enters as two bf16 parts side by side, [hi | lo], 64 columns of one product; the parts of T and
 // P are two products into the same accumulator.  P = tril(D o Q K^T) and T = (I + L)^-1 depend on the chunk alone and
-// come from the prepare kernel as operand tiles.  Products with 64 rows lie in half of each warp's lanes and are read as
+// come from the prepare kernel as operand tiles, T without its diagonal of ones: what they pass on stays in 32 bits, which
+// takes a fifth off the error of the decay's gradient.  Products with 64 rows lie in half of each warp's lanes and are read as
 // fragments, which gives every lane values.  Eight warps work on the accumulators, one issues the products, one moves
 // tiles in and out.
 //
@@ -54,7 +55,7 @@ struct DPrepSmem {
   float rq[C], rk[C], part[2][2 * C];
 };
 
-// 64 x 64 values per head to the upper half of its operand tile: two planes of [128 rows][128 bytes] whose 16-byte
+// T - I, 64 x 64 values per head, to the upper half of its operand tile: two planes of [128 rows][128 bytes] whose 16-byte
 // units are swizzled as the tensor core reads them
 constexpr int TP_PLANE = 128 * 128;
 __device__ __forceinline__ void put_tile(const XbRecArgs& p, const float (&l)[2][C * LS], int c, int h, int heads) {
@@ -63,7 +64,13 @@ __device__ __forceinline__ void put_tile(const XbRecArgs& p, const float (&l)[2]
     if (mm >= heads) break;
     const float4* src = reinterpret_cast<const float4*>(&l[mm][r * LS + u * 8]);
     const bool above = (u >> 1) > (r >> 4);            // blocks above the diagonal are not written by anybody
-    const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f), a = above ? zero : src[0], b = above ? zero : src[1];
+    const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+    float4 a = above ? zero : src[0], b = above ? zero : src[1];
+    if (u == r >> 3) {                                 // the ones of the diagonal
+      const int e = r & 7;
+      a.x = e == 0 ? 0.f : a.x, a.y = e == 1 ? 0.f : a.y, a.z = e == 2 ? 0.f : a.z, a.w = e == 3 ? 0.f : a.w;
+      b.x = e == 4 ? 0.f : b.x, b.y = e == 5 ? 0.f : b.y, b.z = e == 6 ? 0.f : b.z, b.w = e == 7 ? 0.f : b.w;
+    }
     uint4 hi, lo;
     split2(a.x, a.y, hi.x, lo.x), split2(a.z, a.w, hi.y, lo.y), split2(b.x, b.y, hi.z, lo.z), split2(b.z, b.w, hi.w, lo.w);
     uint8_t* dst = (uint8_t*)p.pt + ((long long)c * p.Hv + h + mm) * (2 * TP_PLANE) + r * 128 + ((u ^ (r & 7)) << 4);
@@ -711,7 +718,9 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       old = now, fo[0] = fn[0], fo[1] = fn[1];
       a.wait(&a.bars->done[1], n & 1, 5);
       tc_fence_after();
-      read_frag(quad + D2, x);               // d rk U, then U itself
+      read_frag(quad + D2, z);               // d rk U, then U itself
+#pragma unroll
+      for (int e = 0; e < 2 * NB; ++e) x[e] = x[e] + z[e];
 #pragma unroll
       for (int e = 0; e < 2 * NB; ++e) z[e] = twice(dec[e & 1]) * x[e];
       put_frag(f3, z);
@@ -885,7 +894,9 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       bar_arrive(2, MEET);
       a.wait(&a.bars->done[1], n & 1, 5);
       tc_fence_after();
-      read_frag(quad + D2, x);               // -b gamma rk dR
+      read_frag(quad + D2, y);               // -b gamma rk dR
+#pragma unroll
+      for (int e = 0; e < 2 * NB; ++e) x[e] = x[e] + y[e];
 #pragma unroll
       for (int e = 0; e < 2 * NB; ++e) y[e] = twice(w2[e & 1]) * x[e];
       put_frag(f3, y);

@@ -25,9 +25,9 @@ constexpr int WIDE = 8 / PARTS;                     // pieces of 16 columns of a
 constexpr int T64 = HALF / 2;                       // 8 KB: [64 rows][128 bytes]
 template <bool DELTA>
 struct Lay {
-  static constexpr int RING = DELTA ? 3 : 4;
-  static constexpr int ST_S = 0, ST_DS = HALF, ST_U = 2 * HALF, ST_R = 2 * HALF + T64;
-  static constexpr int STAGE = 2 * HALF + (DELTA ? 2 * T64 : 0);
+  static constexpr int RING = 3;
+  static constexpr int ST_S = 0, ST_DS = HALF, ST_U = 2 * HALF, ST_R = 2 * HALF + T64, ST_3 = 2 * HALF;
+  static constexpr int STAGE = 3 * HALF;
   // dO and V of a pass: 128 columns each in one buffer, which the next head's loads wait for; scan: 64 columns in two.
   // The decays of two heads.
   static constexpr int SL = DELTA ? 4 : 2, NB = DELTA ? 1 : 2, DOV = SL * T64;
@@ -238,6 +238,8 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
             if (DELTA) {
               bulk_load(st + L::ST_U, (const uint8_t*)p.u_tiles + at * T64, T64, &bars->full[s]);
               bulk_load(st + L::ST_R, (const uint8_t*)p.dr_tiles + at * T64, T64, &bars->full[s]);
+            } else {
+              bulk_load(st + L::ST_3, (const uint8_t*)p.r_tiles + at * HALF, HALF, &bars->full[s]);
             }
             bulk_load(st + L::ST_DS, (const uint8_t*)p.ds_tiles + at * HALF, HALF, &bars->full[s]);
           }
@@ -274,7 +276,11 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
               step(tmem + COL_P + set * 64, y, x, id64, first);
               step(tmem + COL_P + set * 64, y + 32, x + 32, id64, false);
               product<true>(tmem + COL_T1 + set * 128, y, st + L::ST_S, id128, first);
+              step(tmem + COL_T1 + set * 128, y, st + L::ST_3, id128, false);
+              step(tmem + COL_T1 + set * 128, y + 32, st + L::ST_3 + 32, id128, false);
               product<true>(tmem + COL_T3, x, st + L::ST_DS, id128, first);
+              step(tmem + COL_T3, x, st + L::ST_3 + 64, id128, false);
+              step(tmem + COL_T3, x + 32, st + L::ST_3 + 96, id128, false);
             }
             tc_commit(&bars->empty[s]);
           }
@@ -449,10 +455,13 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
             // and its tensor pipe has no room: 209 us this way, 221 us with diagonals.)
             {
               const uint32_t sa = st + L::ST_S + a_off, da = st + L::ST_DS + b_off;
-              uint32_t ah[4], al[4], bh[4], bl[4];
+              uint32_t ah[4], al[4], bh[4], bl[4], a3[4], b3[4];
               ldsm4(ah, sa + a_hi), ldsm4(al, sa + a_lo), ldsm4(bh, da + b_hi), ldsm4(bl, da + b_lo);
+              ldsm4(a3, st + L::ST_3 + a_off + a_hi), ldsm4(b3, st + L::ST_3 + b_off + b_lo);
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
+                mma(sd[e], a3, bh[2 * e], bh[2 * e + 1]);
+                mma(sd[e], ah, b3[2 * e], b3[2 * e + 1]);
                 mma(sd[e], al, bl[2 * e], bl[2 * e + 1]);
                 mma(sd[e], al, bh[2 * e], bh[2 * e + 1]);
                 mma(sd[e], ah, bl[2 * e], bl[2 * e + 1]);

@@ -89,10 +89,10 @@ __global__ void __launch_bounds__(128) scan_prep(const XbRecArgs p) {
 constexpr int T64 = HALF / 2;
 // warps: 16 add up the state and write outputs, 6 make P (a block of 32 rows and 16 columns each), 4 the other operand
 constexpr int ADDERS = 512, PMAKERS = 192, XMAKERS = 128, MAKERS = PMAKERS + XMAKERS, THREADS = ADDERS + MAKERS + 64;
-// K and Q: [64 rows][128 bytes] twice each; v or dO: [64][64 columns]; Q K^T: [64][32 fp32] twice; decays and b; the row
-// factors of the outputs
-constexpr int ST_K = 0, ST_Q = 2 * T64, ST_X = 4 * T64, ST_QK = 5 * T64, ST_HD = 7 * T64, ST_ROW = ST_HD + HD * 4, STAGE = ST_ROW + C * 4;
-constexpr int SM_S = 2 * STAGE, SM_P = SM_S + 2 * HALF, SM_D = SM_P + 2 * HALF, SM_BAR = SM_D + 2 * HALF;
+// K and Q: [64 rows][128 bytes] twice each; v or dO: [64][64 columns]; Q K^T: [64][32 fp32] and, of the
+// right half, the lower 32 rows; decays and b; the row factors of the outputs
+constexpr int ST_K = 0, ST_Q = 2 * T64, ST_X = 4 * T64, ST_QK = 5 * T64, ST_HD = ST_QK + T64 + T64 / 2, ST_ROW = ST_HD + HD * 4, STAGE = ST_ROW + C * 4;
+constexpr int SM_S = 2 * STAGE, SM_P = SM_S + 2 * HALF, SM_D = SM_P + 2 * HALF, SM_BAR = SM_D + 6 * T64;
 constexpr int SMEM = SM_BAR + 256 + 1024;
 constexpr int D1 = 0, D2 = 128, DSTEP = 192, D3 = 384;      // D1, D2 of even and odd steps; D3
 
@@ -156,12 +156,13 @@ scan_seq(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtenso
         uint8_t* st = smem + s * STAGE;
         uint64_t* full = &bars->full[s];
         wait(&bars->empty[s], ((n >> 1) & 1) ^ 1, 1);
-        mbar_expect_tx(full, T64 * (OUT ? 7 : 3) + HD * 4);
+        mbar_expect_tx(full, (OUT ? ST_HD : 3 * T64) + HD * 4);
         for (int i = 0; i < 2; ++i) {
           if (OUT || !BWD) tma_load_3d(st + ST_K + i * T64, &mk, full, i * 64, kh, t0);
           if (OUT || BWD) tma_load_3d(st + ST_Q + i * T64, &mq, full, i * 64, kh, t0);
-          if (OUT) tma_load_2d(st + ST_QK + i * T64, &mqk, full, i * 32, (c * p.Hk + kh) * C);
         }
+        for (int i = 0; OUT && i < 3; ++i)   // blocks of 32 x 32 on and below the diagonal
+          tma_load_2d(st + ST_QK + i * (T64 / 2), &mqk, full, i == 2 ? 32 : 0, (c * p.Hk + kh) * C + (i ? 32 : 0));
         tma_load_3d(st + ST_X, &mx, full, v0, h, t0);
         bulk_load(st + ST_HD, p.hd + ((long long)c * p.Hv + h) * HD, HD * 4, full);
       }
@@ -171,12 +172,12 @@ scan_seq(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtenso
     if (xb_elect_one()) {
       constexpr uint64_t kmaj = xb_smem_desc_base_sw128(16, 1024), mn64 = xb_smem_desc_base_sw128(T64, 1024),
                          mn128 = xb_smem_desc_base_sw128(HALF, 1024);
-      constexpr uint32_t id1 = xb_idesc(1, 1, 64, 128, 0, 1), id2 = xb_idesc(1, 1, 64, 64, BWD ? 1 : 0, 1), id3 = xb_idesc(1, 1, 128, 128, 1, 1);
+      constexpr uint32_t id1 = xb_idesc(1, 1, 64, 128, 0, 1), id2 = xb_idesc(1, 1, 64, 64, BWD ? 1 : 0, 1), id3 = xb_idesc(1, 1, 128, 128, 1, 1), id4 = xb_idesc(1, 1, 128, 64, 1, 1);
       const uint32_t bs = xb_smem_u32(smem + SM_S);
       for (int n = 0; n < steps; ++n) {
         const int s = n & 1;
         const uint32_t ph = (n >> 1) & 1, st = xb_smem_u32(smem + s * STAGE);
-        const uint32_t pt = xb_smem_u32(smem + SM_P + s * HALF), dt = xb_smem_u32(smem + SM_D + s * HALF);
+        const uint32_t pt = xb_smem_u32(smem + SM_P + s * HALF), dt = xb_smem_u32(smem + SM_D + s * 3 * T64);
         const uint32_t row = st + (BWD ? ST_K : ST_Q), col = st + (BWD ? ST_Q : ST_K);
         wait(&bars->full[s], ph, 10);
         wait(&bars->pd_full[s], ph, 11);
@@ -185,6 +186,9 @@ scan_seq(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtenso
 #pragma unroll
         for (int k = 0; k < 4; ++k)          // K^T (d b V), Q^T (gamma dO)
           tc_mma_f16_ss(tmem + D3, xb_smem_desc(mn64, col + k * 2048), xb_smem_desc(mn64, dt + k * 2048), id3, k > 0);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)          // the third parts, added to the second's
+          tc_mma_f16_ss(tmem + D3 + 64, xb_smem_desc(mn64, col + k * 2048), xb_smem_desc(mn64, dt + 2 * T64 + k * 2048), id4, 1);
         tc_commit(&bars->d3_full);
         if (OUT) {
           wait(&bars->out_empty[s], ph ^ 1, 13);
@@ -242,17 +246,17 @@ scan_seq(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtenso
 #pragma unroll
       for (int u = 0; u < 4; ++u) v[u] = lds128(st + ST_X + row * 128 + (((half * 4 + u) ^ (row & 7)) << 4));
       wwait(&bars->pd_empty[s], ((n >> 1) & 1) ^ 1, 21);
-      const uint32_t dst = sm + SM_D + s * HALF + half * T64 + row * 128;
+      const uint32_t dst = sm + SM_D + s * 3 * T64 + row * 128;
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const uint32_t x[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
-        uint32_t hi[4], lo[4];
+        uint32_t hi[4], mid[4], lo[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          split2(pair(f, f) * pair(x[e] << 16, x[e] & 0xffff0000u), hi[e], lo[e]);
-        }
-        sts128(dst + ((u ^ (row & 7)) << 4), hi[0], hi[1], hi[2], hi[3]);
-        sts128(dst + (((u + 4) ^ (row & 7)) << 4), lo[0], lo[1], lo[2], lo[3]);
+        for (int e = 0; e < 4; ++e) split3(pair(f, f) * pair(x[e] << 16, x[e] & 0xffff0000u), hi[e], mid[e], lo[e]);
+        const uint32_t at = dst + (((half * 4 + u) ^ (row & 7)) << 4);
+        sts128(at, hi[0], hi[1], hi[2], hi[3]);
+        sts128(at + T64, mid[0], mid[1], mid[2], mid[3]);
+        sts128(at + 2 * T64, lo[0], lo[1], lo[2], lo[3]);
       }
       fence_proxy_async_smem();
       arrive(&bars->pd_full[s]);
@@ -273,7 +277,7 @@ scan_seq(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtenso
       const uint32_t st = sm + s * STAGE, hd = st + ST_HD;
       wwait(&bars->full[s], (n >> 1) & 1, 22);
       const float gi = ldsf(hd + row * 4), gl = ldsf(hd + (C + row) * 4);
-      const uint32_t src = st + ST_QK + (j0 >> 5) * T64 + row * 128;
+      const uint32_t src = st + ST_QK + (j0 >> 5) * (T64 / 2) + row * 128;
       float y[16];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -317,9 +321,27 @@ scan_seq(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtenso
       x[e] = pair(at(2 * e), at(2 * e + 1));
     }
     uint32_t hi[8], lo[8];
-    auto split_row = [&]() {
+    // the state of chunk `c`; the third parts of a kept one go to global memory from here
+    auto split_row = [&](int c) {
+      if constexpr (KEEP) {
+        uint32_t third[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) split2(x[e], hi[e], lo[e]);
+        for (int e = 0; e < 8; ++e) split3(x[e], hi[e], lo[e], third[e]);
+        // units 2 part and 2 part + 1 trade places in odd rows and stay 32 bytes side by side
+        uint8_t* dst = (uint8_t*)p.r_tiles + (((long long)c * p.Hv + h) * (p.dvp / NV) + 2 * cb + sl) * HALF + r * 128 +
+                       (((part * 2 + (BWD ? 4 : 0)) ^ (r & 6)) << 4);
+        const bool odd = r & 1;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t a = third[e], b = third[4 + e];
+          third[e] = odd ? b : a, third[4 + e] = odd ? a : b;
+        }
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(third[0]), "r"(third[1]), "r"(third[2]),
+                     "r"(third[3]), "r"(third[4]), "r"(third[5]), "r"(third[6]), "r"(third[7]) : "memory");
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) split2(x[e], hi[e], lo[e]);
+      }
     };
     auto put = [&]() {                       // the state's row as [hi | lo]
       const uint32_t dst = sm + SM_S + sl * HALF + r * 128;
@@ -333,8 +355,10 @@ scan_seq(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtenso
       tc_fence_before();
       arrive(&bars->s_full);
     };
-    split_row();
-    if (steps > 0) put();
+    if (steps > 0) {
+      split_row(chunk_of(0));
+      put();
+    }
     const float skip = p.D[h];
     const int xrow = r0 + (lane & 15), xunit = sl * 4 + part * 2 + (lane >> 4), ocol = col + 8 * (t & 1) + 4 * (t >> 1);
     bf16* out = (bf16*)(BWD ? p.dv_out : p.o) + (long long)h * p.dv + ocol;
@@ -356,8 +380,8 @@ scan_seq(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtenso
       tc_fence_after();
       {
         uint32_t a[16], b[16];
-        tmem_ld_32x16(base + D3 + sl * 64 + part * 16, a);
-        tmem_ld_32x16(base + D3 + sl * 64 + 32 + part * 16, b);
+        tmem_ld_32x16(base + D3 + sl * NV + part * 16, a);
+        tmem_ld_32x16(base + D3 + 64 + sl * NV + part * 16, b);
         tc_wait_ld();
         tc_fence_before();
         arrive(&bars->d3_empty);
@@ -366,7 +390,7 @@ scan_seq(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtenso
           x[e] = fma2(pair(last, last), x[e], pair(a[2 * e], a[2 * e + 1]) + pair(b[2 * e], b[2 * e + 1]));
       }
       if (n + 1 < steps) {
-        split_row();
+        split_row(chunk_of(n + 1));
         wwait(&bars->s_empty, n & 1, 32);    // the tile's readers are done
         put();
       }
@@ -422,7 +446,7 @@ int run(const XbRecArgs& a, const void* x, long long x_t, long long x_h, cudaStr
   if (a.T > 0 && (rec_tile_map(&mk, a.k, a.T, a.Hk, a.dk, a.k_t, a.k_h, 64, CU_TENSOR_MAP_SWIZZLE_128B) ||
                   rec_tile_map(&mq, a.q, a.T, a.Hk, a.dk, a.q_t, a.q_h, 64, CU_TENSOR_MAP_SWIZZLE_128B) ||
                   rec_tile_map(&mx, x, a.T, a.Hv, a.dv, x_t, x_h, 64, CU_TENSOR_MAP_SWIZZLE_128B) ||
-                  xb_make_tmap_2d(&mqk, a.qk, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, (uint64_t)a.nc_max * a.Hk * C, C, C, C, 32, CU_TENSOR_MAP_SWIZZLE_128B)))
+                  xb_make_tmap_2d(&mqk, a.qk, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, (uint64_t)a.nc_max * a.Hk * C, C, C, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B)))
     return -2;
   if (!rec_configure<scan_seq<BWD, OUT, KEEP>>(SMEM)) return -5;
   scan_seq<BWD, OUT, KEEP><<<(unsigned)blocks, THREADS, SMEM, st>>>(mk, mq, mx, mqk, a);

@@ -42,7 +42,7 @@ def launch_count() -> int:
     return _launches
 
 
-_pack = struct.Struct("56q").pack      # the fields of XbRecArgs (csrc/recurrence.cu)
+_pack = struct.Struct("57q").pack      # the fields of XbRecArgs (csrc/recurrence.cu)
 _CONTIGUOUS = torch.contiguous_format
 
 
@@ -70,7 +70,7 @@ def _layout(T: int, docs: int, Hk: int, Hv: int, dk: int, dv: int, delta: bool, 
     work = [nc * 16, 2 * (docs + 3) * 4, nc * Hv * 3 * CHUNK * 4, nc * Hk * 2 * CHUNK * 4,
             Hk * square if train or not delta else 0, Hk * square if train and delta else 0, nc * Hv * OPERANDS if delta else 0]
     tiles = nc * Hv * (-(-dv // 64) * 2) * TILE
-    first = [tiles, tiles // 2 if delta else 0]
+    first = [tiles, tiles // 2 if delta else 0, 0 if delta else tiles]
     second = [tiles, tiles // 2 if delta else 0, 0 if delta else nc * Hv * 2 * 4]
     keep = train and sum(first) <= KEEP_BYTES
 
@@ -82,7 +82,7 @@ def _layout(T: int, docs: int, Hk: int, Hv: int, dk: int, dv: int, delta: bool, 
         return out, at
 
     kept, kept_bytes = place(work + (first if keep else []))
-    later, later_bytes = place(second if keep else second + (first if train else [0, 0]))
+    later, later_bytes = place(second if keep else second + (first if train else [0, 0, 0]))
     return nc, kept_bytes, later_bytes, keep, tuple(kept), tuple(later)
 
 
@@ -94,11 +94,11 @@ def _words(q, k, v, g, b, A, D, cu, s_in, s_out, ds_out, ds_in, dy, outs, ws, tm
     nc, _, _, keep, kept, later = lay
     base = ws.data_ptr()
     work = [base + o if o >= 0 else 0 for o in kept]
-    back = [0] * 5
+    back = [0] * 6
     if tmp is not None:
         base = tmp.data_ptr()
         back = [base + o if o >= 0 else 0 for o in later]
-    # state and U tiles come from the forward pass or are made again; dS and dR tiles and partial sums are the backward's
+    # state tiles (U and third parts with them) come from the forward pass or are made again; dS and dR tiles and partial sums are the backward's
     work += back[3:] + back[:3] if not keep else back[:3]
     return _pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), 0 if dy is None else dy.data_ptr(), qs[0], qs[1], ks[0], ks[1],
                   vs[0], vs[1], *((0, 0) if dy is None else dy.stride()[:2]),
