@@ -31,9 +31,10 @@ struct XbRecArgs {
   // operand tiles of [rows][hi 32 | lo 32] bf16, [nc_max, Hv, dvp / 32]: states entering and gradients of those leaving
   // the chunks (16 KB), U and dR (8 KB, delta rule only)
   void *s_tiles, *u_tiles, *ds_tiles, *dr_tiles;
-  // third bf16 parts of the states (columns 0 .. 31 of a row) and of the gradients (32 ..), 16 KB (scan only)
+  // third bf16 parts: scan, of the states (columns 0 .. 31 of a row) and of the gradients (32 ..), 16 KB per 32 columns;
+  // delta rule, of U, 8 KB per 64 columns
   void* r_tiles;
-  float* part;                   // [nc_max, Hv, 2] (scan only)
+  float* part;                   // scan: [nc_max, Hv, 2]; delta rule: dR.v by 16 columns, [nc_max, Hv, dvp / 16, 64]
   int* status;                   // filled in by the entry points
   int T, n_docs, Hk, Hv, dk, dv, dvp, nc_max, l2norm, step;   // step: documents of so many tokens at most go token by token; dvp: dv rounded up to 64
   float scale;

@@ -333,13 +333,13 @@ __global__ void __launch_bounds__(PT, 3) delta_prep(const XbRecArgs p) {
 // ---- the step of both directions ------------------------------------------------------------------------------------
 // HALF: [128 rows][64 bf16], K rows 0 .. 63, Q rows 64 .. 127
 constexpr int ST_KQ = 0, ST_TP = 2 * HALF, ST_X = ST_TP + 2 * TP_PLANE, ST_HD = ST_X + C * NV * 2, ST_RQK = ST_HD + HD * 4;
-constexpr int STAGE = (ST_RQK + RQK * 4 + 1023) / 1024 * 1024;
-constexpr int STAGE_BYTES = ST_RQK + RQK * 4;      // what the loads bring, boxes outside a tensor included
+constexpr int ST_V = (ST_RQK + RQK * 4 + 1023) / 1024 * 1024;        // v beside dO, backward
+constexpr int STAGE_BYTES = ST_RQK + RQK * 4;      // what the loads bring, boxes outside a tensor included (and v)
 // Shared memory.  Backward: two stages, operand tiles of 128 rows.  Forward: tiles of 64 rows; two stages, or one and two
 // CTAs per SM.
 template <bool BWD, int STAGES>
 struct Lay {
-  static constexpr int ROWS = BWD ? HALF : HALF / 2;
+  static constexpr int ROWS = BWD ? HALF : HALF / 2, STAGE = ST_V + (BWD ? C * NV * 2 : 0);
   static constexpr int SM_S = STAGES * STAGE, SM_B2 = SM_S + HALF, SM_B3 = SM_B2 + ROWS, SM_U = SM_B3 + ROWS, SM_BAR = SM_U + HALF / 2;
   static constexpr int SMEM = SM_BAR + 128 + 1024;
 };
@@ -377,11 +377,12 @@ struct Cta {
 
 // The loads of one chunk, by one thread.
 __device__ __forceinline__ void load_stage(const XbRecArgs& p, const Cta& a, const CUtensorMap* mk, const CUtensorMap* mq,
-                                           const CUtensorMap* mx, int c, int s) {
-  uint8_t* st = a.smem + s * STAGE;
+                                           const CUtensorMap* mx, const CUtensorMap* mv, int c, int s) {
+  uint8_t* st = a.smem + s * (mv ? Lay<true, 2>::STAGE : Lay<false, 2>::STAGE);
   uint64_t* full = &a.bars->full[s];
   const int t0 = reinterpret_cast<const int4*>(p.chunks)[c].x;
-  mbar_expect_tx(full, STAGE_BYTES);
+  mbar_expect_tx(full, STAGE_BYTES + (mv ? C * NV * 2 : 0));
+  if (mv) tma_load_3d(st + ST_V, mv, full, a.v0, a.h, t0);
   for (int i = 0; i < 2; ++i) {
     tma_load_3d(st + ST_KQ + i * HALF, mk, full, i * 64, a.kh, t0);
     tma_load_3d(st + ST_KQ + i * HALF + HALF / 2, mq, full, i * 64, a.kh, t0);
@@ -555,7 +556,7 @@ __device__ __forceinline__ void zero_rows(const XbRecArgs& p, const Cta& a, bf16
 template <bool OUT, bool SAVE, int STAGES>
 __global__ void __launch_bounds__(THREADS, 3 - STAGES)
 delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mv,
-          const __grid_constant__ XbRecArgs p) {
+          const __grid_constant__ CUtensorMap, const __grid_constant__ XbRecArgs p) {
   using L = Lay<false, STAGES>;
   extern __shared__ uint8_t smem_raw[];
   Cta a;
@@ -576,7 +577,7 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
     const bool one = xb_elect_one();
     const int steps = a.c1 - a.c0;
     for (int n = 0; n < STAGES; ++n)
-      if (one && n < steps) load_stage(p, a, &mk, &mq, &mv, a.c0 + n, n);
+      if (one && n < steps) load_stage(p, a, &mk, &mq, &mv, nullptr, a.c0 + n, n);
     for (int n = 0; n < steps; ++n) {
       if (SAVE) {
         bar(1, FIRST);
@@ -584,7 +585,7 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       }
       if (one && n + STAGES < steps) {         // the stage is free when the chunk's last product has read it
         a.wait1(&a.bars->done[OUT ? 3 : 2], n & 1, 2);
-        load_stage(p, a, &mk, &mq, &mv, a.c0 + n + STAGES, n % STAGES);
+        load_stage(p, a, &mk, &mq, &mv, nullptr, a.c0 + n + STAGES, n % STAGES);
       }
       __syncwarp();
     }
@@ -599,7 +600,7 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
                    u = xb_smem_desc(MNMAJ, a.sm + L::SM_U);
     const int ksteps = (p.dk + 15) / 16;           // columns of K and Q behind dk are zeros
     for (int n = 0; n < a.c1 - a.c0; ++n) {
-      const uint32_t st = a.sm + (n % STAGES) * STAGE;
+      const uint32_t st = a.sm + (n % STAGES) * L::STAGE;
       const uint64_t kq = xb_smem_desc(KMAJ, st + ST_KQ), kt = xb_smem_desc(MNMAJ, st + ST_KQ), tp = xb_smem_desc(KMAJ, st + ST_TP);
       if (one) a.wait1(&a.bars->full[n % STAGES], (n / STAGES) & 1, 1);
       bar(1, FIRST);
@@ -677,7 +678,7 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
     int4 ch = steps > 0 ? chunks[a.c0] : make_int4(0, 0, 0, 0), old = ch;
     float fo[2] = {};                        // gamma rq of the chunk before
     for (int n = 0; n < steps; ++n) {
-      const uint32_t st = a.sm + (n % STAGES) * STAGE, hd = st + ST_HD, rqk = st + ST_RQK;
+      const uint32_t st = a.sm + (n % STAGES) * L::STAGE, hd = st + ST_HD, rqk = st + ST_RQK;
       put_row(a.sm + L::SM_S, r, u0, s);
       if (ch.y < C) {
         a.wait(&a.bars->full[n % STAGES], (n / STAGES) & 1, 3);
@@ -728,7 +729,23 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       tc_fence_before();
       bar_arrive(3, MEET);
       if (SAVE) a.wait(&a.bars->kept, n & 1, 8);          // the tiles on their way out have been read
-      put_frag(fu, x);
+      if (SAVE) {
+        // the third parts: 8 KB tiles of 64 columns, lanes t and t ^ 1 trade as in store_frag
+        const int c = a.c0 + n, ur = r0 + frag_row();
+        uint8_t* dst = (uint8_t*)p.r_tiles + (((long long)c * p.Hv + a.h) * (p.dvp / 64) + (a.v0 >> 6)) * (HALF / 2) + ur * 128;
+#pragma unroll
+        for (int m = 0; m < NB; ++m) {
+          uint32_t hi[2], lo[2], third[2];
+          split3(x[2 * m], hi[0], lo[0], third[0]), split3(x[2 * m + 1], hi[1], lo[1], third[1]);
+          stsm4(fu ^ (m << 4), hi[0], hi[1], lo[0], lo[1]);
+          const bool odd = lane & 1;
+          const uint32_t other = __shfl_xor_sync(0xffffffffu, odd ? third[0] : third[1], 1);
+          const int u = ((a.v0 >> 3) & 7) + u0 + m;
+          *reinterpret_cast<uint2*>(dst + ((u ^ (ur & 7)) << 4) + 8 * ((lane >> 1) & 1)) = odd ? make_uint2(other, third[1]) : make_uint2(third[0], other);
+        }
+      } else {
+        put_frag(fu, x);
+      }
       fence_proxy_async_smem();
       if (OUT) bar_arrive(4, MEET);
       a.wait(&a.bars->done[2], n & 1, 6);
@@ -748,7 +765,7 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
 // dS through one document, last chunk first.
 __global__ void __launch_bounds__(THREADS, 1)
 delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap my,
-          const __grid_constant__ XbRecArgs p) {
+          const __grid_constant__ CUtensorMap mv, const __grid_constant__ XbRecArgs p) {
   using L = Lay<true, 2>;
   extern __shared__ uint8_t smem_raw[];
   Cta a;
@@ -766,13 +783,13 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
   if (warp == LOADER) {
     const bool one = xb_elect_one();
     for (int n = 0; n < 2; ++n)
-      if (one && n < steps) load_stage(p, a, &mk, &mq, &my, a.c1 - 1 - n, n);
+      if (one && n < steps) load_stage(p, a, &mk, &mq, &my, &mv, a.c1 - 1 - n, n);
     for (int n = 0; n < steps; ++n) {
       bar(1, FIRST);
       if (one) keep_tiles(p, a, p.ds_tiles, p.dr_tiles, a.c1 - 1 - n, n > 0 ? a.c1 - n : -1);
       if (one && n + 2 < steps) {
         a.wait1(&a.bars->done[2], n & 1, 2);
-        load_stage(p, a, &mk, &mq, &my, a.c1 - 1 - (n + 2), n & 1);
+        load_stage(p, a, &mk, &mq, &my, &mv, a.c1 - 1 - (n + 2), n & 1);
       }
       __syncwarp();
     }
@@ -785,7 +802,7 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
     const uint64_t b1 = xb_smem_desc(MNMAJ, a.sm + L::SM_S), b2 = xb_smem_desc(MNMAJ, a.sm + L::SM_B2), b3 = xb_smem_desc(MNMAJ, a.sm + L::SM_B3);
     const int ksteps = (p.dk + 15) / 16;
     for (int n = 0; n < steps; ++n) {
-      const uint32_t st = a.sm + (n & 1) * STAGE;
+      const uint32_t st = a.sm + (n & 1) * L::STAGE;
       const uint64_t kq = xb_smem_desc(KMAJ, st + ST_KQ), kt = xb_smem_desc(MNMAJ, st + ST_KQ), tp = xb_smem_desc(MNMAJ, st + ST_TP);
       constexpr uint32_t id3 = xb_idesc(1, 1, 128, 64, 1, 1);
       constexpr uint32_t id1 = xb_idesc(1, 1, 64, 64, 0, 1), id2 = xb_idesc(1, 1, 64, 64, 1, 1), id4 = xb_idesc(1, 1, 64, 32, 1, 1);
@@ -841,7 +858,7 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
     // operands that need dO alone: dO beside Y's tile, gamma rq dO of the third product (threads of Q's rows)
     auto put_dy = [&](int n) {
       const int len = chunks[a.c1 - 1 - n].y;
-      const uint32_t st = a.sm + (n & 1) * STAGE;
+      const uint32_t st = a.sm + (n & 1) * L::STAGE;
       a.wait(&a.bars->full[n & 1], (n >> 1) & 1, 3);
       if (len < C) clear_rows(st, len);
       if (krow) return;
@@ -866,27 +883,30 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
     for (int n = 0; n < steps; ++n) {
       const int len = ch.y;
       const long long t0 = ch.x;
-      const uint32_t st = a.sm + (n & 1) * STAGE, hd = st + ST_HD, rqk = st + ST_RQK;
+      const uint32_t st = a.sm + (n & 1) * L::STAGE, hd = st + ST_HD, rqk = st + ST_RQK;
       put_row(a.sm + L::SM_S, r, u0, s);
       fence_proxy_async_smem();
       tc_fence_before();
       bar_arrive(1, FIRST);
       const float last = ex2_sum(hd, C - 1);
       float w1[2], w2[2], b[2];
+      uint32_t v[NB][2];                     // the loads that take this stage next wait for the third product only
       Pair x[2 * NB], y[2 * NB];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const float rk = ldsf(rqk + (C + row[h]) * 4);
+#pragma unroll
+        for (int m = 0; m < NB; ++m) v[m][h] = row[h] < len ? lds32(st + ST_V + swz<4>(row[h], u0 + m) + (lane & 3) * 4) : 0u;
         b[h] = ldsf(hd + (2 * C + row[h]) * 4), w1[h] = ex2_diff(hd, C - 1, row[h]) * rk, w2[h] = -b[h] * ex2_sum(hd, row[h]) * rk;
       }
       a.wait(&a.bars->done[0], n & 1, 4);
       tc_fence_after();
       {                                      // Y = d rk K dS' + P^T dO
-        uint32_t v[4 * NB];
-        tmem_ld_frag(quad + D4, v);
+        uint32_t d[4 * NB];
+        tmem_ld_frag(quad + D4, d);
         read_frag(quad + D1, x);
 #pragma unroll
-        for (int e = 0; e < 2 * NB; ++e) x[e] = fma2(twice(w1[e & 1]), x[e], pair(v[2 * e], v[2 * e + 1]));
+        for (int e = 0; e < 2 * NB; ++e) x[e] = fma2(twice(w1[e & 1]), x[e], pair(d[2 * e], d[2 * e + 1]));
         put_frag(f2, x);
       }
       fence_proxy_async_smem();
@@ -905,6 +925,23 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       bar_arrive(3, MEET);
       a.wait(&a.bars->kept, n & 1, 8);       // the tiles on their way out have been read
       put_frag(fu, x);
+      {                                      // dR.v for the gradient of b
+        float d[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          Pair w = twice(0.f);
+#pragma unroll
+          for (int m = 0; m < NB; ++m) {
+            w = fma2(x[2 * m + h], bf16_pair(v[m][h]), w);
+          }
+          const float2 e = both(w);
+          d[h] = e.x + e.y;
+          d[h] += __shfl_xor_sync(0xffffffffu, d[h], 1);
+          d[h] += __shfl_xor_sync(0xffffffffu, d[h], 2);
+        }
+        if ((lane & 3) < 2)
+          p.part[(((long long)(a.c1 - 1 - n) * p.Hv + a.h) * (p.dvp / 16) + (a.v0 >> 4) + part) * C + ((lane & 1) ? row[1] : row[0])] = (lane & 1) ? d[1] : d[0];
+      }
 #pragma unroll
       for (int e = 0; e < 2 * NB; ++e) x[e] = twice(b[e & 1]) * x[e];
       store_frag(dv + (t0 + orow) * dv_t + fcol, orow < len, a.vcols - fcol, x);
@@ -933,13 +970,14 @@ int run(const XbRecArgs& a, const void* x, long long x_t, long long x_h, cudaStr
   const long long blocks = (long long)rec_docs(a) * a.Hv * (a.dvp / NV);
   if (blocks > 0x7fffffffLL) return -4;
   if (blocks == 0) return 0;
-  CUtensorMap mk{}, mq{}, mx{};
+  CUtensorMap mk{}, mq{}, mx{}, mv{};
   if (a.T > 0 && (rec_tile_map(&mk, a.k, a.T, a.Hk, a.dk, a.k_t, a.k_h, 64, CU_TENSOR_MAP_SWIZZLE_128B) ||
                   rec_tile_map(&mq, a.q, a.T, a.Hk, a.dk, a.q_t, a.q_h, 64, CU_TENSOR_MAP_SWIZZLE_128B) ||
-                  rec_tile_map(&mx, x, a.T, a.Hv, a.dv, x_t, x_h, NV, CU_TENSOR_MAP_SWIZZLE_64B)))
+                  rec_tile_map(&mx, x, a.T, a.Hv, a.dv, x_t, x_h, NV, CU_TENSOR_MAP_SWIZZLE_64B) ||
+                  rec_tile_map(&mv, a.v, a.T, a.Hv, a.dv, a.v_t, a.v_h, NV, CU_TENSOR_MAP_SWIZZLE_64B)))
     return -2;
   if (!rec_configure<KERNEL>(SMEM)) return -5;
-  KERNEL<<<(unsigned)blocks, THREADS, SMEM, st>>>(mk, mq, mx, a);
+  KERNEL<<<(unsigned)blocks, THREADS, SMEM, st>>>(mk, mq, mx, mv, a);
   return cudaGetLastError() == cudaSuccess ? 0 : -11;
 }
 

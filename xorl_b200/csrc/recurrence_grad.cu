@@ -28,7 +28,7 @@ struct Lay {
   static constexpr int RING = 3;
   static constexpr int ST_S = 0, ST_DS = HALF, ST_U = 2 * HALF, ST_R = 2 * HALF + T64, ST_3 = 2 * HALF;
   static constexpr int STAGE = 3 * HALF;
-  // dO and V of a pass: 128 columns each in one buffer, which the next head's loads wait for; scan: 64 columns in two.
+  // dO and V (delta rule: U's third parts) of a pass: 128 columns each in one buffer, which the next head's loads wait for; scan: 64 columns in two.
   // The decays of two heads.
   static constexpr int SL = DELTA ? 4 : 2, NB = DELTA ? 1 : 2, DOV = SL * T64;
   static constexpr int SM_Q = 0, SM_K = 2 * T64, SM_RING = 4 * T64, SM_DOV = SM_RING + RING * STAGE, SM_HD = SM_DOV + NB * DOV,
@@ -38,7 +38,7 @@ struct Red {                                        // what meets across warps, 
   float rd[3][PARTS][C];                            // q.t1, k.t2, k.t3 by column part
   float er[PARTS][C], fr[PARTS][C];                 // row sums of dP o P and dL o A by column part (scan: dP o P)
   float ec[4][C], fc[4][C];                         // column sums by row block
-  float rv[2][C], sdot[WORKERS / 32];                // dR.v (scan: dO.v) by column half of every slice; <S, dS'> by warp
+  float rv[2][C], sdot[WORKERS / 32];                // scan: dO.v by column half of every slice; <S, dS'> by warp
 };
 struct __align__(8) Bars {
   uint64_t full[4], empty[4], dov_full[2], dov_empty[2], hd_full[2], hd_empty[2], red_full[2], red_empty[2];
@@ -223,10 +223,14 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
           const int d = m % L::NB;
           uint8_t* dov = smem + L::SM_DOV + d * L::DOV;
           wait(&bars->dov_empty[d], ((m / L::NB) & 1) ^ 1, 20);
-          mbar_expect_tx(&bars->dov_full[d], L::DOV);
+          mbar_expect_tx(&bars->dov_full[d], DELTA ? T64 * (2 + min(2, slices / 2 - pass * 2)) : L::DOV);
           for (int i = 0; i < L::SL / 2; ++i) {
             tma_load_3d(dov + i * T64, &my, &bars->dov_full[d], pass * L::SL * NV + i * 64, h, ch.x);
-            tma_load_3d(dov + (L::SL / 2 + i) * T64, &mv, &bars->dov_full[d], pass * L::SL * NV + i * 64, h, ch.x);
+            if (!DELTA) {
+              tma_load_3d(dov + (L::SL / 2 + i) * T64, &mv, &bars->dov_full[d], pass * L::SL * NV + i * 64, h, ch.x);
+            } else if (pass * 2 + i < slices / 2) {
+              bulk_load(dov + (L::SL / 2 + i) * T64, (const uint8_t*)p.r_tiles + (ch_h * (slices / 2) + pass * 2 + i) * T64, T64, &bars->dov_full[d]);
+            }
           }
           for (int sl = pass * L::SL; sl < min(slices, pass * L::SL + L::SL); ++sl, ++n) {
             const int s = n % L::RING;
@@ -268,6 +272,8 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
             tc_fence_after();
             if (DELTA) {
               product<true>(tmem + COL_P, y, st + L::ST_U, id64, first);
+              step(tmem + COL_P, y, x, id64, false);             // U's third part
+              step(tmem + COL_P, y + 32, x + 32, id64, false);
               product<false>(tmem + COL_L, st + L::ST_R, st + L::ST_U, id64, first);
               product<true>(tmem + COL_T1, y, st + L::ST_S, id128, first);
               product<false>(tmem + COL_T2, st + L::ST_R, st + L::ST_S, id128, first);
@@ -335,7 +341,9 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
         if (DELTA) {
           x[i] = (double)q1 + (double)e1 - (double)e2 + (double)(bt * g1) - (double)g2 - (double)(bt * k2) - (double)k3;
           tail += k3;
-          db[i] = (r.rv[0][t] + r.rv[1][t]) - k2 + g1;
+          float dot = 0.f;                             // dR.v, from the walk
+          for (int e = 0; e < p.dvp / 16; ++e) dot += p.part[(ch_h * (p.dvp / 16) + e) * C + t];
+          db[i] = dot - k2 + g1;
         } else {
           x[i] = (double)q1 + (double)e1 - (double)(bt * e2) - (double)(bt * k3);
           tail += (double)(bt * k3);
@@ -440,15 +448,6 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
 #pragma unroll
               for (int e = 0; e < 8; ++e) sd[0][0] += (a[e] + al[e]) * (b[e] + bl[e]);
             }
-            if (tid < 4 * C) {  // dR.v
-              const int sr = tid >> 2, u = tid & 3;
-              float v[8], a[8], al[8];
-              floats8(tile_unit(dov + L::DOV / 2, sr, (sl % L::SL) * 4 + u), v);
-              floats8(lds128(st + L::ST_R + sr * 128 + ((u ^ (sr & 7)) << 4)), a);
-              floats8(lds128(st + L::ST_R + sr * 128 + (((u + 4) ^ (sr & 7)) << 4)), al);
-#pragma unroll
-              for (int e = 0; e < 8; ++e) rv[0][0] += (a[e] + al[e]) * v[e];
-            }
           } else {
             // <S, dS'> and the rows' dO.v are diagonals of products of 16 x 16 blocks: a block per warp.  (Here the state
             // tiles are most of what a head reads and the workers' time counts; the delta rule's products take longer
@@ -488,10 +487,6 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
       if (DELTA) {
         const float sum = warp_sum(sd[0][0]);
         if (lane == 0) r.sdot[warp] = sum;
-        float v = rv[0][0];
-        v += __shfl_xor_sync(0xffffffffu, v, 1);
-        v += __shfl_xor_sync(0xffffffffu, v, 2);
-        if (tid < 4 * C && (tid & 3) == 0) r.rv[0][tid >> 2] = v, r.rv[1][tid >> 2] = 0.f;
       } else {
         // rows 0 .. 7 of a block from the first column tile, 8 .. 15 from the second
         const int g = lane >> 2, t = lane & 3;

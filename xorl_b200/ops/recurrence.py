@@ -70,8 +70,8 @@ def _layout(T: int, docs: int, Hk: int, Hv: int, dk: int, dv: int, delta: bool, 
     work = [nc * 16, 2 * (docs + 3) * 4, nc * Hv * 3 * CHUNK * 4, nc * Hk * 2 * CHUNK * 4,
             Hk * square if train or not delta else 0, Hk * square if train and delta else 0, nc * Hv * OPERANDS if delta else 0]
     tiles = nc * Hv * (-(-dv // 64) * 2) * TILE
-    first = [tiles, tiles // 2 if delta else 0, 0 if delta else tiles]
-    second = [tiles, tiles // 2 if delta else 0, 0 if delta else nc * Hv * 2 * 4]
+    first = [tiles, tiles // 2 if delta else 0, tiles // 4 if delta else tiles]
+    second = [tiles, tiles // 2 if delta else 0, nc * Hv * (-(-dv // 64) * 4 * CHUNK if delta else 2) * 4]
     keep = train and sum(first) <= KEEP_BYTES
 
     def place(sizes):
