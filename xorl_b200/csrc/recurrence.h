@@ -27,12 +27,12 @@ struct XbRecArgs {
   float* hd;                     // [nc_max, Hv, 192]
   float* rqk;                    // [nc_max, Hk, 128]
   float *qk, *kk;                // [nc_max, Hk, 64, 64] (delta rule: for the backward pass, null without one)
-  void* pt;                      // [nc_max, Hv]: operand tile [T; P], two planes, 32768 bytes (delta rule only)
+  void* pt;                      // [nc_max, Hv]: operand tile [T; P], two planes, and a third of T: 40960 bytes (delta rule only)
   // operand tiles of [rows][hi 32 | lo 32] bf16, [nc_max, Hv, dvp / 32]: states entering and gradients of those leaving
   // the chunks (16 KB), U and dR (8 KB, delta rule only)
   void *s_tiles, *u_tiles, *ds_tiles, *dr_tiles;
   // third bf16 parts: scan, of the states (columns 0 .. 31 of a row) and of the gradients (32 ..), 16 KB per 32 columns;
-  // delta rule, of U, 8 KB per 64 columns
+  // delta rule, of U and of dR, 8 KB each per 64 columns
   void* r_tiles;
   float* part;                   // scan: [nc_max, Hv, 2]; delta rule: dR.v by 16 columns, [nc_max, Hv, dvp / 16, 64]
   int* status;                   // filled in by the entry points

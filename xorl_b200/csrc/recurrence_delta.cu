@@ -57,7 +57,7 @@ struct DPrepSmem {
 
 // T - I, 64 x 64 values per head, to the upper half of its operand tile: two planes of [128 rows][128 bytes] whose 16-byte
 // units are swizzled as the tensor core reads them
-constexpr int TP_PLANE = 128 * 128;
+constexpr int TP_PLANE = 128 * 128, T3 = 64 * 128, TP = 2 * TP_PLANE + T3;     // the third plane has T alone, for training
 __device__ __forceinline__ void put_tile(const XbRecArgs& p, const float (&l)[2][C * LS], int c, int h, int heads) {
   for (int it = threadIdx.x; it < 2 * C * 8; it += PT) {
     const int mm = it / (C * 8), r = (it >> 3) % C, u = it & 7;
@@ -71,11 +71,13 @@ __device__ __forceinline__ void put_tile(const XbRecArgs& p, const float (&l)[2]
       a.x = e == 0 ? 0.f : a.x, a.y = e == 1 ? 0.f : a.y, a.z = e == 2 ? 0.f : a.z, a.w = e == 3 ? 0.f : a.w;
       b.x = e == 4 ? 0.f : b.x, b.y = e == 5 ? 0.f : b.y, b.z = e == 6 ? 0.f : b.z, b.w = e == 7 ? 0.f : b.w;
     }
-    uint4 hi, lo;
-    split2(a.x, a.y, hi.x, lo.x), split2(a.z, a.w, hi.y, lo.y), split2(b.x, b.y, hi.z, lo.z), split2(b.z, b.w, hi.w, lo.w);
-    uint8_t* dst = (uint8_t*)p.pt + ((long long)c * p.Hv + h + mm) * (2 * TP_PLANE) + r * 128 + ((u ^ (r & 7)) << 4);
+    uint4 hi, lo, third;
+    split3(pair(a.x, a.y), hi.x, lo.x, third.x), split3(pair(a.z, a.w), hi.y, lo.y, third.y);
+    split3(pair(b.x, b.y), hi.z, lo.z, third.z), split3(pair(b.z, b.w), hi.w, lo.w, third.w);
+    uint8_t* dst = (uint8_t*)p.pt + ((long long)c * p.Hv + h + mm) * TP + r * 128 + ((u ^ (r & 7)) << 4);
     *reinterpret_cast<uint4*>(dst) = hi;
     *reinterpret_cast<uint4*>(dst + TP_PLANE) = lo;
+    if (p.kk != nullptr) *reinterpret_cast<uint4*>(dst + 2 * TP_PLANE) = third;
   }
 }
 
@@ -298,7 +300,7 @@ __global__ void __launch_bounds__(PT, 3) delta_prep(const XbRecArgs p) {
     if (on) {
       const float* hd = sm.hd[m][0];
       // P as the lower half of the operand tile, L for the inverse
-      uint8_t* tile = (uint8_t*)p.pt + ((long long)c * p.Hv + kh * rep + h0 + m) * (2 * TP_PLANE) + C * 128;
+      uint8_t* tile = (uint8_t*)p.pt + ((long long)c * p.Hv + kh * rep + h0 + m) * TP + C * 128;
       float gh[2], gl[2], bb[2];
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh) gh[hh] = hd[r0 + hh * 8], gl[hh] = hd[C + r0 + hh * 8], bb[hh] = hd[2 * C + r0 + hh * 8];
@@ -333,13 +335,13 @@ __global__ void __launch_bounds__(PT, 3) delta_prep(const XbRecArgs p) {
 // ---- the step of both directions ------------------------------------------------------------------------------------
 // HALF: [128 rows][64 bf16], K rows 0 .. 63, Q rows 64 .. 127
 constexpr int ST_KQ = 0, ST_TP = 2 * HALF, ST_X = ST_TP + 2 * TP_PLANE, ST_HD = ST_X + C * NV * 2, ST_RQK = ST_HD + HD * 4;
-constexpr int ST_V = (ST_RQK + RQK * 4 + 1023) / 1024 * 1024;        // v beside dO, backward
-constexpr int STAGE_BYTES = ST_RQK + RQK * 4;      // what the loads bring, boxes outside a tensor included (and v)
+constexpr int ST_T3 = (ST_RQK + RQK * 4 + 1023) / 1024 * 1024, ST_V = ST_T3 + T3;      // T's third plane; v beside dO, backward
+constexpr int STAGE_BYTES = ST_RQK + RQK * 4;      // what the loads bring, boxes outside a tensor included; T3 and v besides
 // Shared memory.  Backward: two stages, operand tiles of 128 rows.  Forward: tiles of 64 rows; two stages, or one and two
 // CTAs per SM.
 template <bool BWD, int STAGES>
 struct Lay {
-  static constexpr int ROWS = BWD ? HALF : HALF / 2, STAGE = ST_V + (BWD ? C * NV * 2 : 0);
+  static constexpr int ROWS = BWD ? HALF : HALF / 2, STAGE = BWD ? ST_V + C * NV * 2 : STAGES == 2 ? ST_V : ST_T3;
   static constexpr int SM_S = STAGES * STAGE, SM_B2 = SM_S + HALF, SM_B3 = SM_B2 + ROWS, SM_U = SM_B3 + ROWS, SM_BAR = SM_U + HALF / 2;
   static constexpr int SMEM = SM_BAR + 128 + 1024;
 };
@@ -377,18 +379,18 @@ struct Cta {
 
 // The loads of one chunk, by one thread.
 __device__ __forceinline__ void load_stage(const XbRecArgs& p, const Cta& a, const CUtensorMap* mk, const CUtensorMap* mq,
-                                           const CUtensorMap* mx, const CUtensorMap* mv, int c, int s) {
-  uint8_t* st = a.smem + s * (mv ? Lay<true, 2>::STAGE : Lay<false, 2>::STAGE);
-  uint64_t* full = &a.bars->full[s];
+                                           const CUtensorMap* mx, const CUtensorMap* mv, bool third, int c, uint8_t* st, uint64_t* full) {
   const int t0 = reinterpret_cast<const int4*>(p.chunks)[c].x;
-  mbar_expect_tx(full, STAGE_BYTES + (mv ? C * NV * 2 : 0));
+  const uint8_t* tp = (const uint8_t*)p.pt + ((long long)c * p.Hv + a.h) * TP;
+  mbar_expect_tx(full, STAGE_BYTES + (third ? T3 : 0) + (mv ? C * NV * 2 : 0));
   if (mv) tma_load_3d(st + ST_V, mv, full, a.v0, a.h, t0);
+  if (third) bulk_load(st + ST_T3, tp + 2 * TP_PLANE, T3, full);
   for (int i = 0; i < 2; ++i) {
     tma_load_3d(st + ST_KQ + i * HALF, mk, full, i * 64, a.kh, t0);
     tma_load_3d(st + ST_KQ + i * HALF + HALF / 2, mq, full, i * 64, a.kh, t0);
   }
   tma_load_3d(st + ST_X, mx, full, a.v0, a.h, t0);
-  bulk_load(st + ST_TP, (const uint8_t*)p.pt + ((long long)c * p.Hv + a.h) * (2 * TP_PLANE), 2 * TP_PLANE, full);
+  bulk_load(st + ST_TP, tp, 2 * TP_PLANE, full);
   bulk_load(st + ST_HD, p.hd + ((long long)c * p.Hv + a.h) * HD, HD * 4, full);
   bulk_load(st + ST_RQK, p.rqk + ((long long)c * p.Hk + a.kh) * RQK, RQK * 4, full);
 }
@@ -439,6 +441,30 @@ __device__ __forceinline__ void put_frag(uint32_t addr, const Pair (&x)[2 * NB])
     stsm4(addr ^ (n << 4), hi[0], hi[1], lo[0], lo[1]);
   }
 }
+// Three parts: the first two as above, the third as an operand tile of its own (units 0 .. 3) or to global memory.
+__device__ __forceinline__ void put_frag3(uint32_t addr, const Pair (&x)[2 * NB], uint32_t (&third)[2 * NB]) {
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    uint32_t hi[2], lo[2];
+    split3(x[2 * n], hi[0], lo[0], third[2 * n]), split3(x[2 * n + 1], hi[1], lo[1], third[2 * n + 1]);
+    stsm4(addr ^ (n << 4), hi[0], hi[1], lo[0], lo[1]);
+  }
+}
+__device__ __forceinline__ uint32_t third_addr(uint32_t tile, int r0, int u0) {
+  const int l = xb_lane(), row = r0 + (l & 15);
+  return tile + row * 128 + (((u0 + (l >> 4)) ^ (row & 7)) << 4);
+}
+// 8 KB tiles of 64 columns; lanes t and t ^ 1 trade as in store_frag.  `row`: r0 + frag_row(), u: the warp's first unit.
+__device__ __forceinline__ void keep_third(uint8_t* tile, int row, int u, const uint32_t (&third)[2 * NB]) {
+  const bool odd = xb_lane() & 1;
+#pragma unroll
+  for (int m = 0; m < NB; ++m) {
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, odd ? third[2 * m] : third[2 * m + 1], 1);
+    *reinterpret_cast<uint2*>(tile + row * 128 + (((u + m) ^ (row & 7)) << 4) + 8 * ((xb_lane() >> 1) & 1)) =
+        odd ? make_uint2(other, third[2 * m + 1]) : make_uint2(third[2 * m], other);
+  }
+}
+static_assert(NB == 2, "one stmatrix for a warp's third parts");
 // the sum of an accumulator's two halves
 template <int N>
 __device__ __forceinline__ void add_halves(const uint32_t (&a)[2 * N], const uint32_t (&b)[2 * N], Pair (&x)[N]) {
@@ -552,8 +578,9 @@ __device__ __forceinline__ void zero_rows(const XbRecArgs& p, const Cta& a, bf16
 // product is complete.  A wait that runs out raises a flag; everybody then walks through the remaining steps without
 // waiting, so that no barrier is left with a thread missing.
 
-// OUT: outputs are wanted.  SAVE: the tiles of the states and of U go to global memory.
-template <bool OUT, bool SAVE, int STAGES>
+// OUT: outputs are wanted.  SAVE: the tiles of the states and of U go to global memory.  THIRD: a backward pass follows, T R
+// is made with three parts.
+template <bool OUT, bool SAVE, int STAGES, bool THIRD = SAVE>
 __global__ void __launch_bounds__(THREADS, 3 - STAGES)
 delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mv,
           const __grid_constant__ CUtensorMap, const __grid_constant__ XbRecArgs p) {
@@ -577,7 +604,7 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
     const bool one = xb_elect_one();
     const int steps = a.c1 - a.c0;
     for (int n = 0; n < STAGES; ++n)
-      if (one && n < steps) load_stage(p, a, &mk, &mq, &mv, nullptr, a.c0 + n, n);
+      if (one && n < steps) load_stage(p, a, &mk, &mq, &mv, nullptr, THIRD, a.c0 + n, a.smem + n * L::STAGE, &a.bars->full[n]);
     for (int n = 0; n < steps; ++n) {
       if (SAVE) {
         bar(1, FIRST);
@@ -585,7 +612,7 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       }
       if (one && n + STAGES < steps) {         // the stage is free when the chunk's last product has read it
         a.wait1(&a.bars->done[OUT ? 3 : 2], n & 1, 2);
-        load_stage(p, a, &mk, &mq, &mv, nullptr, a.c0 + n + STAGES, n % STAGES);
+        load_stage(p, a, &mk, &mq, &mv, nullptr, THIRD, a.c0 + n + STAGES, a.smem + (n % STAGES) * L::STAGE, &a.bars->full[n % STAGES]);
       }
       __syncwarp();
     }
@@ -595,7 +622,7 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
     }
   } else if (warp == ISSUER) {
     const bool one = xb_elect_one();
-    constexpr uint32_t id = xb_idesc(1, 1, 64, 64, 0, 1);
+    constexpr uint32_t id = xb_idesc(1, 1, 64, 64, 0, 1), idh = xb_idesc(1, 1, 64, 32, 0, 1);
     const uint64_t b1 = xb_smem_desc(MNMAJ, a.sm + L::SM_S), b2 = xb_smem_desc(MNMAJ, a.sm + L::SM_B2), b3 = xb_smem_desc(MNMAJ, a.sm + L::SM_B3),
                    u = xb_smem_desc(MNMAJ, a.sm + L::SM_U);
     const int ksteps = (p.dk + 15) / 16;           // columns of K and Q behind dk are zeros
@@ -617,6 +644,13 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
 #pragma unroll
         for (int k = 0; k < 8; ++k)
           tc_mma_f16_ss(a.tmem + D2, ahead(tp, (k >> 2) * TP_PLANE + (k & 3) * 32), ahead(b2, (k & 3) * 2048), id, k > 0);
+        if (THIRD) {                         // the third parts, with the first ones of the other operand
+          const uint64_t t3 = xb_smem_desc(KMAJ, st + ST_T3);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) tc_mma_f16_ss(a.tmem + D2, ahead(t3, k * 32), ahead(b2, k * 2048), idh, 1);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) tc_mma_f16_ss(a.tmem + D2, ahead(tp, k * 32), ahead(b3, k * 2048), idh, 1);
+        }
         tc_commit(&a.bars->done[1]);
         if (OUT) {
 #pragma unroll
@@ -651,7 +685,8 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
     const int q4 = warp & 3, part = warp >> 2, r = q4 * 32 + lane, r0 = q4 * 16, g = lane >> 2;
     const int row[2] = {r0 + g, r0 + g + 8}, u0 = part * NB, fcol = u0 * 8, orow = r0 + frag_row();
     const uint32_t quad = a.tmem + ((uint32_t)(q4 * 32) << 16) + fcol;
-    const uint32_t f2 = frag_addr(a.sm + L::SM_B2, r0, u0), f3 = frag_addr(a.sm + L::SM_B3, r0, u0), fu = frag_addr(a.sm + L::SM_U, r0, u0);
+    const uint32_t f2 = frag_addr(a.sm + L::SM_B2, r0, u0), f3 = frag_addr(a.sm + L::SM_B3, r0, u0), fu = frag_addr(a.sm + L::SM_U, r0, u0),
+                   t3 = third_addr(a.sm + L::SM_B3, r0, u0);
     const long long soff = ((long long)a.doc * p.Hv + a.h) * p.dk * p.dv + a.v0 * p.s_v;
     Pair s[4 * NB];
 #pragma unroll
@@ -711,7 +746,13 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
 #pragma unroll
       for (int e = 0; e < 2 * NB; ++e)       // R = b (V - gamma rk K S)
         x[e] = twice(b[e & 1]) * fma2(twice(-f[e & 1]), x[e], bf16_pair(v[e >> 1][e & 1]));
-      put_frag(f2, x);
+      uint32_t third[2 * NB];
+      if (THIRD) {                           // R's third part where d U comes afterwards
+        put_frag3(f2, x, third);
+        stsm4(t3, third[0], third[1], third[2], third[3]);
+      } else {
+        put_frag(f2, x);
+      }
       fence_proxy_async_smem();
       tc_fence_before();
       bar_arrive(2, MEET);
@@ -730,19 +771,9 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       bar_arrive(3, MEET);
       if (SAVE) a.wait(&a.bars->kept, n & 1, 8);          // the tiles on their way out have been read
       if (SAVE) {
-        // the third parts: 8 KB tiles of 64 columns, lanes t and t ^ 1 trade as in store_frag
-        const int c = a.c0 + n, ur = r0 + frag_row();
-        uint8_t* dst = (uint8_t*)p.r_tiles + (((long long)c * p.Hv + a.h) * (p.dvp / 64) + (a.v0 >> 6)) * (HALF / 2) + ur * 128;
-#pragma unroll
-        for (int m = 0; m < NB; ++m) {
-          uint32_t hi[2], lo[2], third[2];
-          split3(x[2 * m], hi[0], lo[0], third[0]), split3(x[2 * m + 1], hi[1], lo[1], third[1]);
-          stsm4(fu ^ (m << 4), hi[0], hi[1], lo[0], lo[1]);
-          const bool odd = lane & 1;
-          const uint32_t other = __shfl_xor_sync(0xffffffffu, odd ? third[0] : third[1], 1);
-          const int u = ((a.v0 >> 3) & 7) + u0 + m;
-          *reinterpret_cast<uint2*>(dst + ((u ^ (ur & 7)) << 4) + 8 * ((lane >> 1) & 1)) = odd ? make_uint2(other, third[1]) : make_uint2(third[0], other);
-        }
+        put_frag3(fu, x, third);
+        keep_third((uint8_t*)p.r_tiles + (((long long)(a.c0 + n) * p.Hv + a.h) * (p.dvp / 64) + (a.v0 >> 6)) * HALF, orow,
+                   ((a.v0 >> 3) & 7) + u0, third);
       } else {
         put_frag(fu, x);
       }
@@ -783,13 +814,13 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
   if (warp == LOADER) {
     const bool one = xb_elect_one();
     for (int n = 0; n < 2; ++n)
-      if (one && n < steps) load_stage(p, a, &mk, &mq, &my, &mv, a.c1 - 1 - n, n);
+      if (one && n < steps) load_stage(p, a, &mk, &mq, &my, &mv, true, a.c1 - 1 - n, a.smem + n * L::STAGE, &a.bars->full[n]);
     for (int n = 0; n < steps; ++n) {
       bar(1, FIRST);
       if (one) keep_tiles(p, a, p.ds_tiles, p.dr_tiles, a.c1 - 1 - n, n > 0 ? a.c1 - n : -1);
       if (one && n + 2 < steps) {
         a.wait1(&a.bars->done[2], n & 1, 2);
-        load_stage(p, a, &mk, &mq, &my, &mv, a.c1 - 1 - (n + 2), n & 1);
+        load_stage(p, a, &mk, &mq, &my, &mv, true, a.c1 - 1 - (n + 2), a.smem + (n & 1) * L::STAGE, &a.bars->full[n & 1]);
       }
       __syncwarp();
     }
@@ -831,6 +862,11 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
 #pragma unroll
         for (int k = 0; k < 8; ++k)
           tc_mma_f16_ss(a.tmem + D2, ahead(tp, (k >> 2) * TP_PLANE + (k & 3) * 2048), ahead(b2, (k & 3) * 2048), id2, k > 0);
+        const uint64_t t3 = xb_smem_desc(MNMAJ, st + ST_T3);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) tc_mma_f16_ss(a.tmem + D2, ahead(t3, k * 2048), ahead(b2, k * 2048), id4, 1);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) tc_mma_f16_ss(a.tmem + D2, ahead(tp, k * 2048), ahead(b3, k * 2048), id4, 1);
         tc_commit(&a.bars->done[1]);
       }
       bar(3, MEET);
@@ -849,7 +885,8 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
     const int row[2] = {r0 + g, r0 + g + 8}, u0 = part * NB, fcol = u0 * 8, orow = r0 + frag_row();
     const bool krow = r < C;
     const uint32_t quad = a.tmem + ((uint32_t)(q4 * 32) << 16) + fcol;
-    const uint32_t f2 = frag_addr(a.sm + L::SM_B2, r0, u0), f3 = frag_addr(a.sm + L::SM_B3, r0, u0), fu = frag_addr(a.sm + L::SM_U, r0, u0);
+    const uint32_t f2 = frag_addr(a.sm + L::SM_B2, r0, u0), f3 = frag_addr(a.sm + L::SM_B3, r0, u0), fu = frag_addr(a.sm + L::SM_U, r0, u0),
+                   t3 = third_addr(a.sm + L::SM_B3, r0, u0);
     const long long soff = ((long long)a.doc * p.Hv + a.h) * p.dk * p.dv + a.v0 * p.s_v;
     Pair s[4 * NB];
 #pragma unroll
@@ -892,6 +929,7 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       float w1[2], w2[2], b[2];
       uint32_t v[NB][2];                     // the loads that take this stage next wait for the third product only
       Pair x[2 * NB], y[2 * NB];
+      uint32_t third[2 * NB];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const float rk = ldsf(rqk + (C + row[h]) * 4);
@@ -907,7 +945,8 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
         read_frag(quad + D1, x);
 #pragma unroll
         for (int e = 0; e < 2 * NB; ++e) x[e] = fma2(twice(w1[e & 1]), x[e], pair(d[2 * e], d[2 * e + 1]));
-        put_frag(f2, x);
+        put_frag3(f2, x, third);             // Y's third part where -b gamma dR comes afterwards
+        stsm4(t3, third[0], third[1], third[2], third[3]);
       }
       fence_proxy_async_smem();
       tc_fence_before();
@@ -924,7 +963,9 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       tc_fence_before();
       bar_arrive(3, MEET);
       a.wait(&a.bars->kept, n & 1, 8);       // the tiles on their way out have been read
-      put_frag(fu, x);
+      put_frag3(fu, x, third);
+      keep_third((uint8_t*)p.r_tiles + (((long long)(a.c1 - 1 - n) * p.Hv + a.h) * (p.dvp / 64) + (a.v0 >> 6)) * HALF + HALF / 2, orow,
+                 ((a.v0 >> 3) & 7) + u0, third);
       {                                      // dR.v for the gradient of b
         float d[2];
 #pragma unroll
@@ -992,6 +1033,7 @@ int prep(const XbRecArgs& a, cudaStream_t st) {
 int xb_delta_fwd(const XbRecArgs& a, cudaStream_t st) {
   if (int rc = a.dk <= 64 ? prep<64>(a, st) : prep<128>(a, st)) return rc;
   if (a.s_tiles != nullptr) return run<delta_fwd<true, true, 2>, Lay<false, 2>::SMEM>(a, a.v, a.v_t, a.v_h, st);
+  if (a.kk != nullptr) return run<delta_fwd<true, false, 2, true>, Lay<false, 2>::SMEM>(a, a.v, a.v_t, a.v_h, st);
   // Documents of one chunk on average spend their time on the way in and out: two CTAs per SM, one stage each (48
   // documents of 2 tokens, 32 heads of 128 x 128: 388 us with one, 164 us with two).  Longer ones want the next chunk's loads ahead of them.
   if ((long long)a.n_docs * C >= a.T) return run<delta_fwd<true, false, 1>, Lay<false, 1>::SMEM>(a, a.v, a.v_t, a.v_h, st);

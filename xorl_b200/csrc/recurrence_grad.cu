@@ -25,12 +25,12 @@ constexpr int WIDE = 8 / PARTS;                     // pieces of 16 columns of a
 constexpr int T64 = HALF / 2;                       // 8 KB: [64 rows][128 bytes]
 template <bool DELTA>
 struct Lay {
-  static constexpr int RING = 3;
+  static constexpr int RING = DELTA ? 2 : 3;
   static constexpr int ST_S = 0, ST_DS = HALF, ST_U = 2 * HALF, ST_R = 2 * HALF + T64, ST_3 = 2 * HALF;
   static constexpr int STAGE = 3 * HALF;
-  // dO and V (delta rule: U's third parts) of a pass: 128 columns each in one buffer, which the next head's loads wait for; scan: 64 columns in two.
+  // dO and V (delta rule: third parts of U and of dR) of a pass: 128 columns each in one buffer, which the next head's loads wait for; scan: 64 columns in two.
   // The decays of two heads.
-  static constexpr int SL = DELTA ? 4 : 2, NB = DELTA ? 1 : 2, DOV = SL * T64;
+  static constexpr int SL = DELTA ? 4 : 2, NB = DELTA ? 1 : 2, DOV = DELTA ? 6 * T64 : SL * T64;
   static constexpr int SM_Q = 0, SM_K = 2 * T64, SM_RING = 4 * T64, SM_DOV = SM_RING + RING * STAGE, SM_HD = SM_DOV + NB * DOV,
                        SM_RED = SM_HD + 2 * 1024;
 };
@@ -73,7 +73,7 @@ __device__ __forceinline__ void step(uint32_t d, uint32_t a, uint32_t b, uint32_
   constexpr uint64_t kmaj = xb_smem_desc_base_sw128(16, 1024);
   tc_mma_f16_ss(d, xb_smem_desc(kmaj, a), xb_smem_desc(kmaj, b), idesc, first ? 0u : 1u);
 }
-// hi hi, hi lo, lo hi of two [hi | lo] tiles; EXACT: a is 32 plain columns
+// all four products of the parts of two [hi | lo] tiles; EXACT: a is 32 plain columns
 template <bool EXACT>
 __device__ __forceinline__ void product(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool first) {
   step(d, a, b, idesc, first);
@@ -83,6 +83,8 @@ __device__ __forceinline__ void product(uint32_t d, uint32_t a, uint32_t b, uint
   if (!EXACT) {
     step(d, a + 64, b, idesc, false);
     step(d, a + 96, b + 32, idesc, false);
+    step(d, a + 64, b + 64, idesc, false);
+    step(d, a + 96, b + 96, idesc, false);
   }
 }
 // Fragments: a thread has rows g and g + 8 of its warp's 16 and, of every 8 columns, 2 t and 2 t + 1.
@@ -223,13 +225,15 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
           const int d = m % L::NB;
           uint8_t* dov = smem + L::SM_DOV + d * L::DOV;
           wait(&bars->dov_empty[d], ((m / L::NB) & 1) ^ 1, 20);
-          mbar_expect_tx(&bars->dov_full[d], DELTA ? T64 * (2 + min(2, slices / 2 - pass * 2)) : L::DOV);
+          mbar_expect_tx(&bars->dov_full[d], DELTA ? T64 * (2 + 2 * min(2, slices / 2 - pass * 2)) : L::DOV);
           for (int i = 0; i < L::SL / 2; ++i) {
             tma_load_3d(dov + i * T64, &my, &bars->dov_full[d], pass * L::SL * NV + i * 64, h, ch.x);
             if (!DELTA) {
               tma_load_3d(dov + (L::SL / 2 + i) * T64, &mv, &bars->dov_full[d], pass * L::SL * NV + i * 64, h, ch.x);
             } else if (pass * 2 + i < slices / 2) {
-              bulk_load(dov + (L::SL / 2 + i) * T64, (const uint8_t*)p.r_tiles + (ch_h * (slices / 2) + pass * 2 + i) * T64, T64, &bars->dov_full[d]);
+              const uint8_t* third = (const uint8_t*)p.r_tiles + (ch_h * (slices / 2) + pass * 2 + i) * HALF;
+              bulk_load(dov + (2 + i) * T64, third, T64, &bars->dov_full[d]);
+              bulk_load(dov + (4 + i) * T64, third + T64, T64, &bars->dov_full[d]);
             }
           }
           for (int sl = pass * L::SL; sl < min(slices, pass * L::SL + L::SL); ++sl, ++n) {
@@ -261,7 +265,7 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
         if (!DELTA) wait(&bars->set_empty[hh & 1], ((hh >> 1) & 1) ^ 1, 34);
         const uint32_t set = DELTA ? 0 : hh & 1;
         for (int pass = 0; pass < passes; ++pass, ++m) {
-          const uint32_t y0 = sm + L::SM_DOV + (m % L::NB) * L::DOV, x0 = y0 + L::DOV / 2;
+          const uint32_t y0 = sm + L::SM_DOV + (m % L::NB) * L::DOV, x0 = y0 + 2 * T64 / L::NB;
           wait(&bars->dov_full[m % L::NB], (m / L::NB) & 1, 31);
           for (int sl = pass * L::SL; sl < min(slices, pass * L::SL + L::SL); ++sl, ++n) {
             const int s = n % L::RING, q = sl % L::SL;
@@ -275,6 +279,10 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
               step(tmem + COL_P, y, x, id64, false);             // U's third part
               step(tmem + COL_P, y + 32, x + 32, id64, false);
               product<false>(tmem + COL_L, st + L::ST_R, st + L::ST_U, id64, first);
+              step(tmem + COL_L, st + L::ST_R, x, id64, false);
+              step(tmem + COL_L, st + L::ST_R + 32, x + 32, id64, false);
+              step(tmem + COL_L, x + 2 * T64, st + L::ST_U, id64, false);
+              step(tmem + COL_L, x + 2 * T64 + 32, st + L::ST_U + 32, id64, false);
               product<true>(tmem + COL_T1, y, st + L::ST_S, id128, first);
               product<false>(tmem + COL_T2, st + L::ST_R, st + L::ST_S, id128, first);
               product<false>(tmem + COL_T3, st + L::ST_U, st + L::ST_DS, id128, first);

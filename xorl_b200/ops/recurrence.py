@@ -35,7 +35,7 @@ KEEP_BYTES = 1 << 30
 # Without gradients and with at most so many tokens per document on average, documents of at most so many go token by
 # token (csrc/recurrence_step.cu, which gives the times of both ways), the others through the chunked kernels.
 STEP = 16
-OPERANDS = 32768        # bytes of the operand tile that the delta rule prepares per chunk and head
+OPERANDS = 40960        # bytes of the operand tile that the delta rule prepares per chunk and head
 
 
 def launch_count() -> int:
@@ -70,7 +70,7 @@ def _layout(T: int, docs: int, Hk: int, Hv: int, dk: int, dv: int, delta: bool, 
     work = [nc * 16, 2 * (docs + 3) * 4, nc * Hv * 3 * CHUNK * 4, nc * Hk * 2 * CHUNK * 4,
             Hk * square if train or not delta else 0, Hk * square if train and delta else 0, nc * Hv * OPERANDS if delta else 0]
     tiles = nc * Hv * (-(-dv // 64) * 2) * TILE
-    first = [tiles, tiles // 2 if delta else 0, tiles // 4 if delta else tiles]
+    first = [tiles, tiles // 2 if delta else 0, tiles // 2 if delta else tiles]
     second = [tiles, tiles // 2 if delta else 0, nc * Hv * (-(-dv // 64) * 4 * CHUNK if delta else 2) * 4]
     keep = train and sum(first) <= KEEP_BYTES
 
