@@ -23,8 +23,8 @@
 //
 // A forward step takes 2800 cycles: three times about 450 of products and their latency, the rest on the way from
 // accumulator to operand (four or sixteen warps on it: 2 % and 13 % more; mma.sync instead of tcgen05: 5800 cycles).  32
-// heads of 128 x 128: forward 371 us for a document of 16384 tokens and 128 us for 4096 tokens in five documents with
-// their tiles kept (0.22 GB written), backward 116 us; prepare 143 and 46 us (268 and 67 MB written: latencies of small
+// heads of 128 x 128: forward 370 us for a document of 16384 tokens and 135 us for 4096 tokens in five documents with
+// their tiles kept (0.26 GB written; with two parts 125), backward 136 us (118); prepare 144 and 49 us (268 and 90 MB written: latencies of small
 // steps, three CTAs per SM).
 #include "recurrence_core.cuh"
 

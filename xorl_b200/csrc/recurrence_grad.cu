@@ -5,14 +5,14 @@
 // 32 at a time, and forms five products in tensor memory, all with 64 rows of tokens:
 //   dP = dO U^T,  dL = dR U^T  [64 x 64];   t1 = dO S^T,  t2 = dR S^T,  t3 = U dS'^T  [64 x 128]
 // (scan: U = V, no dL and t2.)  A computed operand is a tile of [hi 32 | lo 32] columns; the parts of a product are the
-// pairs of 16-column steps hi hi, hi lo, lo hi.  Behind each head the rows of t1 .. t3 are scaled and added up in
+// pairs of 16-column steps; third parts are tiles of their own.  Behind each head the rows of t1 .. t3 are scaled and added up in
 // registers, their dot products with q and k give the gradient of the decay and of b, and D o dP, D o dL are added up;
 // the products with K and Q are the same for all heads of the group and are made once, from the sums.
 // Sixteen worker warps, a loading and an issuing warp, and one that turns the heads' sums into gradients of the decay.
 //
-// It reads the tiles that the two sequential passes keep (48 KB per head and 32 columns; scan 32 KB).  4096 tokens of 32
-// heads of 128 x 128: 209 us, 0.45 GB of tiles at 2.1 TB/s; 4095 tokens of 128 heads of 64 x 128: 244 us, 0.58 GB at 2.4
-// TB/s.  All of tensor memory holds one head's five products (scan: two heads' dP and t1), so that loads overlap the
+// It reads the tiles that the two sequential passes keep (56 KB per head and 32 columns; scan 48 KB).  4096 tokens of 32
+// heads of 128 x 128: 217 us, 0.52 GB of tiles at 2.4 TB/s; 4095 tokens of 128 heads of 64 x 128: 269 us, 0.87 GB at 3.2
+// TB/s (without third parts 208 and 244 us).  All of tensor memory holds one head's five products (scan: two heads' dP and t1), so that loads overlap the
 // workers' turn and products do not; with two heads per CTA a third of the time is its way in and out.
 #include "recurrence_core.cuh"
 
@@ -462,13 +462,10 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
             // and its tensor pipe has no room: 209 us this way, 221 us with diagonals.)
             {
               const uint32_t sa = st + L::ST_S + a_off, da = st + L::ST_DS + b_off;
-              uint32_t ah[4], al[4], bh[4], bl[4], a3[4], b3[4];
+              uint32_t ah[4], al[4], bh[4], bl[4];
               ldsm4(ah, sa + a_hi), ldsm4(al, sa + a_lo), ldsm4(bh, da + b_hi), ldsm4(bl, da + b_lo);
-              ldsm4(a3, st + L::ST_3 + a_off + a_hi), ldsm4(b3, st + L::ST_3 + b_off + b_lo);
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
-                mma(sd[e], a3, bh[2 * e], bh[2 * e + 1]);
-                mma(sd[e], ah, b3[2 * e], b3[2 * e + 1]);
                 mma(sd[e], al, bl[2 * e], bl[2 * e + 1]);
                 mma(sd[e], al, bh[2 * e], bh[2 * e + 1]);
                 mma(sd[e], ah, bl[2 * e], bl[2 * e + 1]);

@@ -8,10 +8,11 @@
 // walked the other way.  The state does not feed back into what is added to it, so the products of a step need not wait
 // for one another: a CTA carries 64 state columns of one head through one document, ten warps make the operands that
 // depend on the chunk alone (P, and d b V or gamma dO) ahead of the products, sixteen add up the state and write the
-// outputs, one loads and one issues.  Computed operands are [hi 32 | lo 32] tiles (P: two planes).  Per step and CTA 20
-// products, about 1100 cycles of the tensor pipe of 3500: issue slots (66 % taken) and latencies of the warps that add and
-// split bound it.  128 heads of 64 x 128: forward 473 us for a document of 16384 tokens and 146 us for 4095 tokens in five
-// documents with their states kept (0.29 GB written), backward 148 us; prepare 37 and 11 us.  Eight adding warps instead
+// outputs, one loads and one issues.  Computed operands are [hi 32 | lo 32] tiles (P: two planes, the other operand three;
+// kept states go with their third parts, straight from the registers).  Per step and CTA 24
+// products, about 1300 cycles of the tensor pipe of 3700: issue slots (66 % taken) and latencies of the warps that add and
+// split bound it.  128 heads of 64 x 128: forward 500 us for a document of 16384 tokens (with two parts 470) and 181 us for 4095
+// tokens in five documents with their states kept (0.43 GB written; with two parts and 0.29 GB 146), backward 183 us; prepare 37 and 11 us.  Eight adding warps instead
 // of sixteen: 1.7 times the time.
 #include "recurrence_core.cuh"
 
