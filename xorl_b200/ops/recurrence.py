@@ -29,9 +29,10 @@ _launches = 0
 CHUNK = 64              # tokens of a chunk of the kernels (csrc/recurrence.cu)
 TILE = 16384            # bytes of an operand tile of the state
 MAX_STATE_ROWS = 128
-# The state tiles of all chunks (and U of the delta rule) are kept for the backward pass up to this size (4096 tokens of 32
-# heads of 128 x 128: 0.2 GB); a longer call makes them again, which is the forward pass without its outputs once more.
-KEEP_BYTES = 1 << 30
+# The state tiles of all chunks, and what goes with them, are kept for the backward pass up to this size (4096 tokens of 32
+# heads of 128 x 128: 0.3 GB); a longer call makes them again, which is the forward pass without its outputs once more
+# (16384 tokens of such heads, forward and backward: 2.0 ms kept, 2.3 ms made again).
+KEEP_BYTES = 3 << 29
 # Without gradients and with at most so many tokens per document on average, documents of at most so many go token by
 # token (csrc/recurrence_step.cu, which gives the times of both ways), the others through the chunked kernels.
 STEP = 16
