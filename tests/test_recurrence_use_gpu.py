@@ -72,6 +72,22 @@ def test_two_calls_at_once_and_two_backward_passes(op):
     same(ga, torch.autograd.grad(oa, la, do))
 
 
+def test_both_operators_on_two_streams():
+    """Passes of both, of different lengths, side by side on two streams: the bits of one after the other."""
+    cases = [(op, inputs(op, T=T, docs=3, seed=T), boundaries([0, 70, 71, T])) for T in (300, 1500) for op in OPS]
+    want = [both_ways(*c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = []
+    for i in range(12):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(both_ways(*cases[(i * 3 + i // 2) % len(cases)]))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        same(g, want[(i * 3 + i // 2) % len(cases)])
+
+
 @pytest.mark.parametrize("op", OPS)
 def test_captured_and_replayed(op):
     """Two captured passes over the same buffers, replayed in turn with new values in them (boundaries too)."""
