@@ -1034,9 +1034,11 @@ int xb_delta_fwd(const XbRecArgs& a, cudaStream_t st) {
   if (int rc = a.dk <= 64 ? prep<64>(a, st) : prep<128>(a, st)) return rc;
   if (a.s_tiles != nullptr) return run<delta_fwd<true, true, 2>, Lay<false, 2>::SMEM>(a, a.v, a.v_t, a.v_h, st);
   if (a.kk != nullptr) return run<delta_fwd<true, false, 2, true>, Lay<false, 2>::SMEM>(a, a.v, a.v_t, a.v_h, st);
-  // Documents of one chunk on average spend their time on the way in and out: two CTAs per SM, one stage each (48
-  // documents of 2 tokens, 32 heads of 128 x 128: 388 us with one, 164 us with two).  Longer ones want the next chunk's loads ahead of them.
-  if ((long long)a.n_docs * C >= a.T) return run<delta_fwd<true, false, 1>, Lay<false, 1>::SMEM>(a, a.v, a.v_t, a.v_h, st);
+  // Documents of four chunks on average or fewer: two CTAs per SM, one stage each, hide one another's way in and out (40
+  // documents of 64, 100, 200 and 400 tokens, 32 heads of 128 x 128: 128, 182, 295, 455 us; with two stages 195, 261, 368,
+  // 512).  Longer ones, of which there are fewer CTAs, want the next chunk's loads ahead of them (one document of 1000
+  // tokens: 46 us and 29 us).
+  if (4ll * C * a.n_docs >= a.T) return run<delta_fwd<true, false, 1>, Lay<false, 1>::SMEM>(a, a.v, a.v_t, a.v_h, st);
   return run<delta_fwd<true, false, 2>, Lay<false, 2>::SMEM>(a, a.v, a.v_t, a.v_h, st);
 }
 int xb_delta_bwd(const XbRecArgs& a, int tiles, cudaStream_t st) {
