@@ -118,16 +118,6 @@ __device__ __forceinline__ void tmem_ld_frag(uint32_t addr, uint32_t (&r)[8]) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(addr) : "memory");
 }
 
-__device__ __forceinline__ void tmem_ld_frag(uint32_t addr, uint32_t (&r)[4]) {       // 8 columns
-  asm volatile("tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void tmem_ld_rows(uint32_t addr, uint32_t (&r)[8]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void tmem_ld_rows(uint32_t addr, uint32_t (&r)[16]) { tmem_ld_32x16(addr, r); }
-
 // fragment addresses of this lane; m0, n0, k0 are multiples of 8 (16 for the wide ones)
 template <int U>  // A[m][k], k contiguous
 __device__ __forceinline__ uint32_t addr_a(int m0, int k0) {

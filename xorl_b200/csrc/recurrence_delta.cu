@@ -15,7 +15,8 @@
 //             [K; Q]^T [-b gamma dR; gamma dO] -> added to dS  (the dO part is issued early)
 //
 // A computed operand enters as two bf16 parts side by side, [hi | lo], 64 columns of one product; the parts of T and
-// P are two products into the same accumulator.  P = tril(D o Q K^T) and T = (I + L)^-1 depend on the chunk alone and
+// P are two products into the same accumulator.  In calls with gradients the third parts of T - I, R and Y take part too,
+// as products of 32 columns with the first parts of the other operand.  P = tril(D o Q K^T) and T = (I + L)^-1 depend on the chunk alone and
 // come from the prepare kernel as operand tiles, T without its diagonal of ones: what they pass on stays in 32 bits, which
 // takes a fifth off the error of the decay's gradient.  Products with 64 rows lie in half of each warp's lanes and are read as
 // fragments, which gives every lane values.  Eight warps work on the accumulators, one issues the products, one moves
@@ -473,8 +474,8 @@ __device__ __forceinline__ void add_halves(const uint32_t (&a)[2 * N], const uin
 }
 __device__ __forceinline__ void read_rows(uint32_t addr, Pair (&x)[4 * NB]) {
   uint32_t a[8 * NB], b[8 * NB];
-  tmem_ld_rows(addr, a);
-  tmem_ld_rows(addr + 32, b);
+  tmem_ld_32x16(addr, a);
+  tmem_ld_32x16(addr + 32, b);
   tc_wait_ld();
   add_halves(a, b, x);
 }
