@@ -1,0 +1,28 @@
+"""Calls of the gated linear recurrences that have to give the same bits: repeated beside other work on the GPU, with and
+without gradients, and whatever a call keeps for its backward pass."""
+import pytest
+import torch
+
+from test_recurrence_gpu import _need_cuda, delta_inputs, scan_inputs  # noqa: F401
+from test_recurrence_use_gpu import OPS, both_ways, boundaries, same
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("op,hk,hv,dk,dv", [("delta", 2, 2, 128, 32), ("delta", 1, 3, 128, 64), ("delta", 1, 8, 64, 128),
+                                            ("scan", 2, 2, 128, 64), ("scan", 1, 3, 128, 64), ("scan", 1, 16, 64, 96)])
+def test_gradients_repeat_beside_other_work(op, hk, hv, dk, dv):
+    """Few slices and few heads, so that the gradient kernel's last head is soon behind its first, and products on another
+    stream that take issue slots and memory from its warps in ever different places."""
+    cuts = [0, 70, 71, 135, 700]
+    ts = list((delta_inputs if op == "delta" else scan_inputs)(700, hk, hv, dk, dv, len(cuts) - 1, seed=11, state=True))
+    cu = boundaries(cuts)
+    want = both_ways(op, ts, cu)
+    side, m = torch.cuda.Stream(), torch.randn(1024, 1024, device="cuda").bfloat16()
+    side.wait_stream(torch.cuda.current_stream())
+    for i in range(40):
+        with torch.cuda.stream(side):
+            for _ in range(i % 4):
+                m @ m
+        same(want, both_ways(op, ts, cu))
+    torch.cuda.current_stream().wait_stream(side)

@@ -576,7 +576,9 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
       arrive(&bars->red_full[hh & 1]);
       arrive(&bars->hd_empty[hh & 1]);
     }
-    // Z and W as operand tiles over the ring, whose last tiles have been read; K and Q without rows behind the end
+    // Z and W as operand tiles over the ring: the products have read its last tiles (acc_full), the other warps' own reads of S
+    // and dS' end at this barrier; K and Q without rows behind the end
+    wbar();
 #pragma unroll
     for (int part = 0; part < (DELTA ? 2 : 1); ++part) {
       uint32_t hi[4], lo[4];
