@@ -26,3 +26,23 @@ def test_gradients_repeat_beside_other_work(op, hk, hv, dk, dv):
                 m @ m
         same(want, both_ways(op, ts, cu))
     torch.cuda.current_stream().wait_stream(side)
+
+
+def test_long_walks_without_gradients_beside_other_work():
+    """Several hundred chunks in a row through the two-stage walk that keeps nothing, with products on another stream that
+    hold up its warps: the bits of the first call, and no wait that ran out (the fixture reads the status words)."""
+    from xorl_b200.ops.recurrence import gated_delta_rule
+    q, k, v, g, beta, s = delta_inputs(20000, 1, 2, 64, 64, 1, seed=13, state=True)
+    cu = boundaries([0, 20000])
+    side, m = torch.cuda.Stream(), torch.randn(2048, 2048, device="cuda").bfloat16()
+    with torch.no_grad():
+        run = lambda: gated_delta_rule(q, k, v, g, beta, cu, scale=0.125, qk_l2norm=True, initial_state=s,  # noqa: E731
+                                       return_final_state=True)
+        want = run()
+        side.wait_stream(torch.cuda.current_stream())
+        for _ in range(10):
+            with torch.cuda.stream(side):
+                for _ in range(8):
+                    m @ m
+            same(want, run())
+    torch.cuda.current_stream().wait_stream(side)

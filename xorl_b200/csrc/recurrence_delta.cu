@@ -355,7 +355,7 @@ constexpr int MEET = WORKERS + 32;           // workers and the issuing warp
 constexpr int D1 = 0, D2 = 64, D3 = 128, D4 = 192, D5 = 256, D6 = 320;
 
 struct __align__(8) Bars {
-  uint64_t full[2], done[4], kept;
+  uint64_t full[2], done[4], free[2], kept;
   uint32_t tmem;
   int abort_flag;
 };
@@ -537,7 +537,7 @@ __device__ __forceinline__ bool cta_setup(const XbRecArgs& p, Cta& a, uint8_t* r
 template <int COLS>
 __device__ __forceinline__ void cta_begin(Cta& a) {
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) mbar_init(&a.bars->full[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&a.bars->full[i], 1), mbar_init(&a.bars->free[i], 1);
     for (int i = 0; i < 4; ++i) mbar_init(&a.bars->done[i], 1);
     mbar_init(&a.bars->kept, 1);
     a.bars->abort_flag = 0;
@@ -611,8 +611,10 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
         bar(1, FIRST);
         if (one) keep_tiles(p, a, p.s_tiles, p.u_tiles, a.c0 + n, n > 0 ? a.c0 + n - 1 : -1);
       }
-      if (one && n + STAGES < steps) {         // the stage is free when the chunk's last product has read it
-        a.wait1(&a.bars->done[OUT ? 3 : 2], n & 1, 2);
+      // The stage is free when the chunk's last product has read it.  A barrier per stage: without tiles to keep nothing else
+      // holds this warp to the walk's pace, and of one barrier for all chunks it could miss a phase.
+      if (one && n + STAGES < steps) {
+        a.wait1(&a.bars->free[n % STAGES], (n / STAGES) & 1, 2);
         load_stage(p, a, &mk, &mq, &mv, nullptr, THIRD, a.c0 + n + STAGES, a.smem + (n % STAGES) * L::STAGE, &a.bars->full[n % STAGES]);
       }
       __syncwarp();
@@ -668,6 +670,7 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
         for (int k = 0; k < 4; ++k)
           tc_mma_f16_ss(a.tmem + D3, ahead(kt, k * 2048), ahead(b3, k * 2048), id3, k > 0);
         tc_commit(&a.bars->done[2]);
+        if (!OUT && n + STAGES < a.c1 - a.c0) tc_commit(&a.bars->free[n % STAGES]);
       }
       if (OUT) {
         bar(4, MEET);
@@ -677,6 +680,7 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
           for (int k = 0; k < 8; ++k)
             tc_mma_f16_ss(a.tmem + DPU, ahead(tp, HALF / 2 + (k >> 2) * TP_PLANE + (k & 3) * 32), ahead(u, (k & 3) * 2048), id, k > 0);
           tc_commit(&a.bars->done[3]);
+          if (n + STAGES < a.c1 - a.c0) tc_commit(&a.bars->free[n % STAGES]);
         }
       }
       __syncwarp();
