@@ -338,7 +338,7 @@ bool bad(const Args& a) {
 
 }  // namespace
 
-// fp32 values of the buffer that the backward pass needs for the weight's gradient.
+// fp32 values of the buffer that the backward pass needs on the current device for the weight's gradient.
 XB_API int xb_gated_norm_partial(int T, int groups, int d, int w_shared) {
   if (T <= 0 || groups <= 0 || d <= 0 || d % 8) return 0;
   const dim3 g = grid_of(T, groups, d, true);
@@ -356,15 +356,15 @@ XB_API int xb_gated_norm_fwd(const void* x, long long ldx, const void* z, long l
   return norm_first ? run<false, true>(a, (cudaStream_t)stream) : run<false, false>(a, (cudaStream_t)stream);
 }
 
-// dw: [d] (shared weight) or [groups * d], fp32 or bf16; with part null it is not computed.
+// dw: [d] (shared weight) or [groups * d], fp32 or bf16; with part null it is not computed.  part_n: values that part holds.
 XB_API int xb_gated_norm_bwd(const void* dy, long long lddy, const void* x, long long ldx, const void* z, long long ldz,
                              const void* w, int w_f32, int w_shared, const float* rstd, void* dx, void* dz, float* part,
-                             void* dw, int dw_f32, int T, int groups, int d, int norm_first, void* stream) {
+                             long long part_n, void* dw, int dw_f32, int T, int groups, int d, int norm_first, void* stream) {
   Args a{};
   a.dy = (const bf16*)dy, a.lddy = lddy;
   a.x = (const bf16*)x, a.z = (const bf16*)z, a.ldx = ldx, a.ldz = ldz, a.w = w, a.w_f32 = w_f32, a.w_shared = w_shared;
   a.rstd = const_cast<float*>(rstd), a.dx = (bf16*)dx, a.dz = (bf16*)dz, a.part = part, a.T = T, a.groups = groups, a.d = d;
-  if (bad(a) || (part != nullptr && dw == nullptr)) return -1;
+  if (bad(a) || (part != nullptr && (dw == nullptr || part_n < xb_gated_norm_partial(T, groups, d, w_shared)))) return -1;
   cudaStream_t st = (cudaStream_t)stream;
   if (T > 0) {
     const int rc = norm_first ? run<true, true>(a, st) : run<true, false>(a, st);

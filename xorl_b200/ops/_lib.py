@@ -114,7 +114,7 @@ _SIGNATURES = {
     "xb_causal_conv1d_bwd": [P, L, P, L, P, P, P, P, P, L, P, I, I, I, I, P],
     "xb_gated_norm_partial": [I, I, I, I],
     "xb_gated_norm_fwd": [P, L, P, L, P, I, I, P, P, I, I, I, F, I, P],
-    "xb_gated_norm_bwd": [P, L, P, L, P, L, P, I, I, P, P, P, P, P, I, I, I, I, I, P],
+    "xb_gated_norm_bwd": [P, L, P, L, P, L, P, I, I, P, P, P, P, L, P, I, I, I, I, I, P],
     "xb_recurrence_fwd": [P, F, I, P],
     "xb_recurrence_bwd": [P, F, I, I, P],
     "xb_dequant4": [P, P, P, P, L, I, I, P],

@@ -133,8 +133,10 @@ def _norm_rows(t: torch.Tensor) -> torch.Tensor:
 
 
 @functools.lru_cache(maxsize=256)
-def _gated_norm_partial(T: int, groups: int, group_size: int, shared: int) -> int:
-    return max(_lib.cuda_lib().xb_gated_norm_partial(T, groups, group_size, shared), 1)
+def _gated_norm_partial(T: int, groups: int, group_size: int, shared: int, device: int) -> int:
+    """Size of the weight gradient's partial sums: a matter of the device's SMs, so of the device."""
+    with torch.cuda.device(device):
+        return max(_lib.cuda_lib().xb_gated_norm_partial(T, groups, group_size, shared), 1)
 
 
 class _GatedRMSNorm(torch.autograd.Function):
@@ -170,14 +172,14 @@ class _GatedRMSNorm(torch.autograd.Function):
         part = dw = None
         want, sink, out_wide = ctx.needs_input_grad[2], False, 0
         if want:
-            part = torch.empty(_gated_norm_partial(T, groups, group_size, shared), dtype=torch.float32, device=dev)
+            part = torch.empty(_gated_norm_partial(T, groups, group_size, shared, dev.index), dtype=torch.float32, device=dev)
             # an engine's buffer takes fp32 sums; a gradient that autograd gets is rounded where it is summed
             sink = grad_target(ctx.w)[0] is not None
             dw = torch.empty_like(wc, dtype=torch.float32) if sink else torch.empty_like(wc)
             out_wide = int(sink or wide)
         _lib.call_on(dev, "xb_gated_norm_bwd", dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), z.data_ptr(), z.stride(0),
-                     wc.data_ptr(), wide, shared, rstd.data_ptr(), dx.data_ptr(), dz.data_ptr(), _lib.ptr(part), _lib.ptr(dw),
-                     out_wide, T, groups, group_size, norm_first)
+                     wc.data_ptr(), wide, shared, rstd.data_ptr(), dx.data_ptr(), dz.data_ptr(), _lib.ptr(part),
+                     0 if part is None else part.numel(), _lib.ptr(dw), out_wide, T, groups, group_size, norm_first)
         _launches += 1 + int(want)
         if len(shape) != 2:
             dx, dz = dx.reshape(shape), dz.reshape(shape)
