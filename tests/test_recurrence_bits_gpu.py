@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from test_recurrence_gpu import _need_cuda, delta_inputs, scan_inputs  # noqa: F401
-from test_recurrence_use_gpu import OPS, both_ways, boundaries, same
+from test_recurrence_use_gpu import OPS, both_ways, boundaries, call, same
 
 pytestmark = pytest.mark.gpu
 
@@ -46,3 +46,26 @@ def test_long_walks_without_gradients_beside_other_work():
                     m @ m
             same(want, run())
     torch.cuda.current_stream().wait_stream(side)
+
+
+def call_both(op, ts, cu):
+    """The call with gradients and without: outputs and states."""
+    with torch.no_grad():
+        plain = call(op, ts, cu)
+    return plain, [t.detach() for t in call(op, [None if t is None else t.detach().requires_grad_() for t in ts], cu)]
+
+
+CUTS = {"one": [0, 300], "two chunks": [0, 128], "long and short": [0, 1, 2, 3, 4, 5, 6, 7, 8, 9, 300], "outside": [40, 40, 101, 250],
+        "many": list(range(0, 2001, 50))}
+
+
+@pytest.mark.parametrize("op", OPS)
+@pytest.mark.parametrize("cuts", CUTS.values(), ids=CUTS.keys())
+@pytest.mark.parametrize("hk,hv,dk,dv", [(2, 4, 64, 64), (1, 4, 128, 128), (4, 8, 32, 40)])
+@pytest.mark.parametrize("state", [False, True])
+def test_calls_with_and_without_gradients(op, cuts, hk, hv, dk, dv, state):
+    """A pass without gradients that is repeated with them (recomputed activations), or whose scores are compared with those of
+    training, has the same bits."""
+    T = max(cuts[-1] + 3, 128)
+    ts = list((delta_inputs if op == "delta" else scan_inputs)(T, hk, hv, dk, dv, len(cuts) - 1, seed=17, state=state))
+    same(*call_both(op, ts, boundaries(cuts)))

@@ -29,8 +29,8 @@
 // their gradients) is kept in 32 bits and enters a product as the sum of two bf16 values, which keeps 17 bits of its
 // significand: one bf16 value (9 bits) would cost the fp32 gradients of the decay three decimal digits.  Where these
 // gradients are differences of large sums a third bf16 value keeps all 24: what is added to the scan's states, the
-// scan's kept states and their gradients, and in calls of the delta rule with gradients T - I, R, Y, U and dR in
-// T R, T^T Y, dO U^T and dR U^T.  Measured against 64 bits (with two parts everywhere in brackets): gradients of A 5e-7 to
+// scan's kept states and their gradients, and the delta rule's T - I, R, Y, U and dR in T R, T^T Y, dO U^T and
+// dR U^T.  A call without gradients does the same arithmetic as one with them: their outputs have the same bits.  Measured against 64 bits (with two parts everywhere in brackets): gradients of A 5e-7 to
 // 3e-6 of their norm (1e-6 to 1.2e-5), of dt 1e-7 to 5e-7, final states of the scan 7e-8 (3e-6); gradient of the delta rule's
 // decay 1e-6 to 7e-6 (4e-6 to 1.6e-5), of beta 4e-6, its states 4e-6; bf16 outputs by their rounding.  Decays are sums in
 // fp64 of log2 units, kept as two floats, so that differences of large sums stay exact.  L2 norms of q and k are row

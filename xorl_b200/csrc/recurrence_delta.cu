@@ -15,8 +15,9 @@
 //             [K; Q]^T [-b gamma dR; gamma dO] -> added to dS  (the dO part is issued early)
 //
 // A computed operand enters as two bf16 parts side by side, [hi | lo], 64 columns of one product; the parts of T and
-// P are two products into the same accumulator.  In calls with gradients the third parts of T - I, R and Y take part too,
-// as products of 32 columns with the first parts of the other operand.  P = tril(D o Q K^T) and T = (I + L)^-1 depend on the chunk alone and
+// P are two products into the same accumulator.  The third parts of T - I, R and Y take part too, as products of 32 columns
+// with the first parts of the other operand; of a call without gradients as well, so that its outputs are those of the
+// call that a backward pass follows, to the bit.  P = tril(D o Q K^T) and T = (I + L)^-1 depend on the chunk alone and
 // come from the prepare kernel as operand tiles, T without its diagonal of ones: what they pass on stays in 32 bits, which
 // takes a fifth off the error of the decay's gradient.  Products with 64 rows lie in half of each warp's lanes and are read as
 // fragments, which gives every lane values.  Eight warps work on the accumulators, one issues the products, one moves
@@ -58,7 +59,7 @@ struct DPrepSmem {
 
 // T - I, 64 x 64 values per head, to the upper half of its operand tile: two planes of [128 rows][128 bytes] whose 16-byte
 // units are swizzled as the tensor core reads them
-constexpr int TP_PLANE = 128 * 128, T3 = 64 * 128, TP = 2 * TP_PLANE + T3;     // the third plane has T alone, for training
+constexpr int TP_PLANE = 128 * 128, T3 = 64 * 128, TP = 2 * TP_PLANE + T3;     // the third plane has T alone
 __device__ __forceinline__ void put_tile(const XbRecArgs& p, const float (&l)[2][C * LS], int c, int h, int heads) {
   for (int it = threadIdx.x; it < 2 * C * 8; it += PT) {
     const int mm = it / (C * 8), r = (it >> 3) % C, u = it & 7;
@@ -78,7 +79,7 @@ __device__ __forceinline__ void put_tile(const XbRecArgs& p, const float (&l)[2]
     uint8_t* dst = (uint8_t*)p.pt + ((long long)c * p.Hv + h + mm) * TP + r * 128 + ((u ^ (r & 7)) << 4);
     *reinterpret_cast<uint4*>(dst) = hi;
     *reinterpret_cast<uint4*>(dst + TP_PLANE) = lo;
-    if (p.kk != nullptr) *reinterpret_cast<uint4*>(dst + 2 * TP_PLANE) = third;
+    *reinterpret_cast<uint4*>(dst + 2 * TP_PLANE) = third;
   }
 }
 
@@ -339,11 +340,12 @@ constexpr int ST_KQ = 0, ST_TP = 2 * HALF, ST_X = ST_TP + 2 * TP_PLANE, ST_HD = 
 constexpr int ST_T3 = (ST_RQK + RQK * 4 + 1023) / 1024 * 1024, ST_V = ST_T3 + T3;      // T's third plane; v beside dO, backward
 constexpr int STAGE_BYTES = ST_RQK + RQK * 4;      // what the loads bring, boxes outside a tensor included; T3 and v besides
 // Shared memory.  Backward: two stages, operand tiles of 128 rows.  Forward: tiles of 64 rows; two stages, or one and two
-// CTAs per SM.
+// CTAs per SM, where U takes the place of R, which T R has read by then (P U is complete before the next R).
 template <bool BWD, int STAGES>
 struct Lay {
-  static constexpr int ROWS = BWD ? HALF : HALF / 2, STAGE = BWD ? ST_V + C * NV * 2 : STAGES == 2 ? ST_V : ST_T3;
-  static constexpr int SM_S = STAGES * STAGE, SM_B2 = SM_S + HALF, SM_B3 = SM_B2 + ROWS, SM_U = SM_B3 + ROWS, SM_BAR = SM_U + HALF / 2;
+  static constexpr int ROWS = BWD ? HALF : HALF / 2, STAGE = BWD ? ST_V + C * NV * 2 : ST_V;
+  static constexpr int SM_S = STAGES * STAGE, SM_B2 = SM_S + HALF, SM_B3 = SM_B2 + ROWS, SM_U = STAGES == 2 ? SM_B3 + ROWS : SM_B2,
+                       SM_BAR = STAGES == 2 ? SM_U + HALF / 2 : SM_B3 + ROWS;
   static constexpr int SMEM = SM_BAR + 128 + 1024;
 };
 constexpr int NB = 2;                        // units of 8 columns per worker
@@ -380,12 +382,12 @@ struct Cta {
 
 // The loads of one chunk, by one thread.
 __device__ __forceinline__ void load_stage(const XbRecArgs& p, const Cta& a, const CUtensorMap* mk, const CUtensorMap* mq,
-                                           const CUtensorMap* mx, const CUtensorMap* mv, bool third, int c, uint8_t* st, uint64_t* full) {
+                                           const CUtensorMap* mx, const CUtensorMap* mv, int c, uint8_t* st, uint64_t* full) {
   const int t0 = reinterpret_cast<const int4*>(p.chunks)[c].x;
   const uint8_t* tp = (const uint8_t*)p.pt + ((long long)c * p.Hv + a.h) * TP;
-  mbar_expect_tx(full, STAGE_BYTES + (third ? T3 : 0) + (mv ? C * NV * 2 : 0));
+  mbar_expect_tx(full, STAGE_BYTES + T3 + (mv ? C * NV * 2 : 0));
   if (mv) tma_load_3d(st + ST_V, mv, full, a.v0, a.h, t0);
-  if (third) bulk_load(st + ST_T3, tp + 2 * TP_PLANE, T3, full);
+  bulk_load(st + ST_T3, tp + 2 * TP_PLANE, T3, full);
   for (int i = 0; i < 2; ++i) {
     tma_load_3d(st + ST_KQ + i * HALF, mk, full, i * 64, a.kh, t0);
     tma_load_3d(st + ST_KQ + i * HALF + HALF / 2, mq, full, i * 64, a.kh, t0);
@@ -579,9 +581,8 @@ __device__ __forceinline__ void zero_rows(const XbRecArgs& p, const Cta& a, bf16
 // product is complete.  A wait that runs out raises a flag; everybody then walks through the remaining steps without
 // waiting, so that no barrier is left with a thread missing.
 
-// OUT: outputs are wanted.  SAVE: the tiles of the states and of U go to global memory.  THIRD: a backward pass follows, T R
-// is made with three parts.
-template <bool OUT, bool SAVE, int STAGES, bool THIRD = SAVE>
+// OUT: outputs are wanted.  SAVE: the tiles of the states and of U go to global memory.
+template <bool OUT, bool SAVE, int STAGES>
 __global__ void __launch_bounds__(THREADS, 3 - STAGES)
 delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mv,
           const __grid_constant__ CUtensorMap, const __grid_constant__ XbRecArgs p) {
@@ -605,7 +606,7 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
     const bool one = xb_elect_one();
     const int steps = a.c1 - a.c0;
     for (int n = 0; n < STAGES; ++n)
-      if (one && n < steps) load_stage(p, a, &mk, &mq, &mv, nullptr, THIRD, a.c0 + n, a.smem + n * L::STAGE, &a.bars->full[n]);
+      if (one && n < steps) load_stage(p, a, &mk, &mq, &mv, nullptr, a.c0 + n, a.smem + n * L::STAGE, &a.bars->full[n]);
     for (int n = 0; n < steps; ++n) {
       if (SAVE) {
         bar(1, FIRST);
@@ -615,7 +616,7 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       // holds this warp to the walk's pace, and of one barrier for all chunks it could miss a phase.
       if (one && n + STAGES < steps) {
         a.wait1(&a.bars->free[n % STAGES], (n / STAGES) & 1, 2);
-        load_stage(p, a, &mk, &mq, &mv, nullptr, THIRD, a.c0 + n + STAGES, a.smem + (n % STAGES) * L::STAGE, &a.bars->full[n % STAGES]);
+        load_stage(p, a, &mk, &mq, &mv, nullptr, a.c0 + n + STAGES, a.smem + (n % STAGES) * L::STAGE, &a.bars->full[n % STAGES]);
       }
       __syncwarp();
     }
@@ -647,13 +648,12 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
 #pragma unroll
         for (int k = 0; k < 8; ++k)
           tc_mma_f16_ss(a.tmem + D2, ahead(tp, (k >> 2) * TP_PLANE + (k & 3) * 32), ahead(b2, (k & 3) * 2048), id, k > 0);
-        if (THIRD) {                         // the third parts, with the first ones of the other operand
-          const uint64_t t3 = xb_smem_desc(KMAJ, st + ST_T3);
+        // the third parts, with the first ones of the other operand
+        const uint64_t t3 = xb_smem_desc(KMAJ, st + ST_T3);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) tc_mma_f16_ss(a.tmem + D2, ahead(t3, k * 32), ahead(b2, k * 2048), idh, 1);
+        for (int k = 0; k < 4; ++k) tc_mma_f16_ss(a.tmem + D2, ahead(t3, k * 32), ahead(b2, k * 2048), idh, 1);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) tc_mma_f16_ss(a.tmem + D2, ahead(tp, k * 32), ahead(b3, k * 2048), idh, 1);
-        }
+        for (int k = 0; k < 4; ++k) tc_mma_f16_ss(a.tmem + D2, ahead(tp, k * 32), ahead(b3, k * 2048), idh, 1);
         tc_commit(&a.bars->done[1]);
         if (OUT) {
 #pragma unroll
@@ -752,12 +752,8 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
       for (int e = 0; e < 2 * NB; ++e)       // R = b (V - gamma rk K S)
         x[e] = twice(b[e & 1]) * fma2(twice(-f[e & 1]), x[e], bf16_pair(v[e >> 1][e & 1]));
       uint32_t third[2 * NB];
-      if (THIRD) {                           // R's third part where d U comes afterwards
-        put_frag3(f2, x, third);
-        stsm4(t3, third[0], third[1], third[2], third[3]);
-      } else {
-        put_frag(f2, x);
-      }
+      put_frag3(f2, x, third);               // R's third part where d U comes afterwards
+      stsm4(t3, third[0], third[1], third[2], third[3]);
       fence_proxy_async_smem();
       tc_fence_before();
       bar_arrive(2, MEET);
@@ -819,13 +815,13 @@ delta_bwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
   if (warp == LOADER) {
     const bool one = xb_elect_one();
     for (int n = 0; n < 2; ++n)
-      if (one && n < steps) load_stage(p, a, &mk, &mq, &my, &mv, true, a.c1 - 1 - n, a.smem + n * L::STAGE, &a.bars->full[n]);
+      if (one && n < steps) load_stage(p, a, &mk, &mq, &my, &mv, a.c1 - 1 - n, a.smem + n * L::STAGE, &a.bars->full[n]);
     for (int n = 0; n < steps; ++n) {
       bar(1, FIRST);
       if (one) keep_tiles(p, a, p.ds_tiles, p.dr_tiles, a.c1 - 1 - n, n > 0 ? a.c1 - n : -1);
       if (one && n + 2 < steps) {
         a.wait1(&a.bars->done[2], n & 1, 2);
-        load_stage(p, a, &mk, &mq, &my, &mv, true, a.c1 - 1 - (n + 2), a.smem + (n & 1) * L::STAGE, &a.bars->full[n & 1]);
+        load_stage(p, a, &mk, &mq, &my, &mv, a.c1 - 1 - (n + 2), a.smem + (n & 1) * L::STAGE, &a.bars->full[n & 1]);
       }
       __syncwarp();
     }
@@ -1038,7 +1034,6 @@ int prep(const XbRecArgs& a, cudaStream_t st) {
 int xb_delta_fwd(const XbRecArgs& a, cudaStream_t st) {
   if (int rc = a.dk <= 64 ? prep<64>(a, st) : prep<128>(a, st)) return rc;
   if (a.s_tiles != nullptr) return run<delta_fwd<true, true, 2>, Lay<false, 2>::SMEM>(a, a.v, a.v_t, a.v_h, st);
-  if (a.kk != nullptr) return run<delta_fwd<true, false, 2, true>, Lay<false, 2>::SMEM>(a, a.v, a.v_t, a.v_h, st);
   // Documents of four chunks on average or fewer: two CTAs per SM, one stage each, hide one another's way in and out (40
   // documents of 64, 100, 200 and 400 tokens, 32 heads of 128 x 128: 128, 182, 295, 455 us; with two stages 195, 261, 368,
   // 512).  Longer ones, of which there are fewer CTAs, want the next chunk's loads ahead of them (one document of 1000
