@@ -132,9 +132,11 @@ bool bad_args(const XbRecArgs& a) {
          a.dv % 8 || a.step < 0 || a.step >= C || a.nc_max < a.T / C + rec_docs(a);
 }
 
-int plan(const XbRecArgs& a, cudaStream_t st) {
+// plan, and the operands of the chunks
+int prepare(const XbRecArgs& a, int delta, cudaStream_t st) {
   rec_plan<<<1, 1024, 0, st>>>(a.cu, a.n_docs, a.T, a.nc_max, a.step, (int4*)a.chunks, a.doc_off, a.doc_list, a.status);
-  return cudaGetLastError() == cudaSuccess ? 0 : -11;
+  if (cudaGetLastError() != cudaSuccess) return -11;
+  return delta ? xb_delta_prep(a, st) : xb_scan_prep(a, st);
 }
 
 }  // namespace
@@ -167,17 +169,20 @@ XB_API int xb_recurrence_fwd(const long long* words, float scale, int delta, voi
   if (a.step > 0)
     if (int rc = xb_recurrence_step(a, delta, st)) return rc;
   if (a.step > 0 && a.T <= a.step) return 0;                  // no document can be longer
-  if (int rc = plan(a, st)) return rc;
+  if (int rc = prepare(a, delta, st)) return rc;
   return delta ? xb_delta_fwd(a, st) : xb_scan_fwd(a, st);
 }
 
-// tiles: the forward pass has left its tiles in s_tiles (and u_tiles); else they are made again.
-XB_API int xb_recurrence_bwd(const long long* words, float scale, int delta, int tiles, void* stream) {
+// kept: what the forward pass has left, 2: the operands of the chunks and the state tiles, 1: the operands, 0: nothing.
+// The rest is made again.
+XB_API int xb_recurrence_bwd(const long long* words, float scale, int delta, int kept, void* stream) {
   if (words == nullptr) return -1;
   const XbRecArgs a = unpack(words, scale);
   if (bad_args(a) || a.step > 0) return -1;
   cudaStream_t st = (cudaStream_t)stream;
-  if (int rc = delta ? xb_delta_bwd(a, tiles, st) : xb_scan_bwd(a, tiles, st)) return rc;
+  if (kept == 0)
+    if (int rc = prepare(a, delta, st)) return rc;
+  if (int rc = delta ? xb_delta_bwd(a, kept == 2, st) : xb_scan_bwd(a, kept == 2, st)) return rc;
   if (int rc = xb_recurrence_grad(a, delta, st)) return rc;
   return delta ? 0 : rec_launch(rec_reduce, a.Hv, 128, 0, a, st);
 }

@@ -223,13 +223,15 @@ int rec_launch(K kernel, long long blocks, int threads, size_t smem, const XbRec
 
 }  // namespace
 
-// recurrence_delta.cu: prepare and forward (keeping tiles where it is given room for them); forward again for the tiles
+// recurrence_delta.cu: prepare; forward (keeping tiles where it is given room for them); forward again for the tiles
 // unless they are there, and the state's gradient
+int xb_delta_prep(const XbRecArgs& a, cudaStream_t st);
 int xb_delta_fwd(const XbRecArgs& a, cudaStream_t st);
 int xb_delta_bwd(const XbRecArgs& a, int tiles, cudaStream_t st);
 // recurrence_step.cu: documents of at most `step` tokens, forward only
 int xb_recurrence_step(const XbRecArgs& a, int delta, cudaStream_t st);
 // recurrence_scan.cu: the same for the scan
+int xb_scan_prep(const XbRecArgs& a, cudaStream_t st);
 int xb_scan_fwd(const XbRecArgs& a, cudaStream_t st);
 int xb_scan_bwd(const XbRecArgs& a, int tiles, cudaStream_t st);
 // recurrence_grad.cu: gradients of q, k, the decay and b from the kept tiles

@@ -1031,8 +1031,8 @@ int prep(const XbRecArgs& a, cudaStream_t st) {
 
 }  // namespace
 
+int xb_delta_prep(const XbRecArgs& a, cudaStream_t st) { return a.dk <= 64 ? prep<64>(a, st) : prep<128>(a, st); }
 int xb_delta_fwd(const XbRecArgs& a, cudaStream_t st) {
-  if (int rc = a.dk <= 64 ? prep<64>(a, st) : prep<128>(a, st)) return rc;
   if (a.s_tiles != nullptr) return run<delta_fwd<true, true, 2>, Lay<false, 2>::SMEM>(a, a.v, a.v_t, a.v_h, st);
   // Documents of four chunks on average or fewer: two CTAs per SM, one stage each, hide one another's way in and out (40
   // documents of 64, 100, 200 and 400 tokens, 32 heads of 128 x 128: 128, 182, 295, 455 us; with two stages 195, 261, 368,

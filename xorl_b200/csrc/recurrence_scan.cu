@@ -456,9 +456,11 @@ int run(const XbRecArgs& a, const void* x, long long x_t, long long x_h, cudaStr
 
 }  // namespace
 
-int xb_scan_fwd(const XbRecArgs& a, cudaStream_t st) {
+int xb_scan_prep(const XbRecArgs& a, cudaStream_t st) {
   const long long blocks = (long long)a.nc_max * a.Hk;
-  if (int rc = a.dk <= 64 ? rec_launch(scan_prep<64>, blocks, 128, 0, a, st) : rec_launch(scan_prep<128>, blocks, 128, 0, a, st)) return rc;
+  return a.dk <= 64 ? rec_launch(scan_prep<64>, blocks, 128, 0, a, st) : rec_launch(scan_prep<128>, blocks, 128, 0, a, st);
+}
+int xb_scan_fwd(const XbRecArgs& a, cudaStream_t st) {
   return a.s_tiles != nullptr ? run<false, true, true>(a, a.v, a.v_t, a.v_h, st) : run<false, true, false>(a, a.v, a.v_t, a.v_h, st);
 }
 int xb_scan_bwd(const XbRecArgs& a, int tiles, cudaStream_t st) {

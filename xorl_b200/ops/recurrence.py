@@ -33,8 +33,10 @@ MAX_STATE_ROWS = 128
 # heads of 128 x 128: 0.3 GB); a longer call makes them again, which is the forward pass without its outputs once more
 # (16384 tokens of such heads, forward and backward: 2.0 ms kept, 2.3 ms made again).
 KEEP_BYTES = 3 << 29
-# Without gradients and with at most so many tokens per document on average, documents of at most so many go token by
-# token (csrc/recurrence_step.cu, which gives the times of both ways), the others through the chunked kernels.
+# With at most so many tokens per document on average, documents of at most so many go token by token
+# (csrc/recurrence_step.cu, which gives the times of both ways), the others through the chunked kernels.  The same with and
+# without gradients, so that a forward pass that is run again for its gradients has the bits of the first one; a backward
+# pass works on chunks, and makes theirs itself behind such a call.
 STEP = 16
 OPERANDS = 40960        # bytes of the operand tile that the delta rule prepares per chunk and head
 
@@ -65,7 +67,8 @@ def _state(x: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
 @functools.lru_cache(maxsize=256)
 def _layout(T: int, docs: int, Hk: int, Hv: int, dk: int, dv: int, delta: bool, train: bool, step: int):
     """Where the workspaces of a call of these sizes lie: (chunks, bytes kept from the forward pass, bytes of the backward
-    pass, whether the state tiles are kept, offsets of chunks .. pt, of the kept tiles, of the backward pass's buffers)."""
+    pass, whether the state tiles are kept, offsets of chunks .. pt, of the kept tiles, of the backward pass's buffers).
+    ``step``: of the forward pass; a backward pass's own layout has none."""
     nc = T // CHUNK + (T // (step + 1) if step else docs + 2)
     square = nc * CHUNK * CHUNK * 4
     work = [nc * 16, 2 * (docs + 3) * 4, nc * Hv * 3 * CHUNK * 4, nc * Hk * 2 * CHUNK * 4,
@@ -125,8 +128,8 @@ class _Recurrence(torch.autograd.Function):
         dev = v.device
         docs = cu.shape[0] - 1
         train = True in ctx.needs_input_grad
-        step = STEP if not train and T <= STEP * max(docs, 1) else 0
-        lay = _layout(T, docs, Hk, Hv, dk, dv, delta, train, step)
+        step = STEP if T <= STEP * max(docs, 1) else 0
+        lay = _layout(T, docs, Hk, Hv, dk, dv, delta, train and not step, step)
         ws = torch.empty(lay[1], dtype=torch.uint8, device=dev)
         o = torch.empty_like(v, memory_format=_CONTIGUOUS)
         s_out = torch.empty((docs, Hv, dk, dv) if delta else (docs, Hv, dv, dk), dtype=torch.float32, device=dev) if final else None
@@ -134,7 +137,7 @@ class _Recurrence(torch.autograd.Function):
                                                       (o.data_ptr(), 0, 0, 0, 0, 0, 0, 0), ws, None, lay, delta, l2norm, step),
                      scale, delta)
         _launches += 3 if not step else 4 if T > step else 1
-        ctx.save_for_backward(q, k, v, g, b, A, D, s_in, cu, ws)
+        ctx.save_for_backward(q, k, v, g, b, A, D, s_in, cu, None if step else ws)
         ctx.conf = (delta, scale, l2norm, lay)
         ctx.set_materialize_grads(False)
         return o, s_out
@@ -146,6 +149,11 @@ class _Recurrence(torch.autograd.Function):
         q, k, v, g, b, A, D, s_in, cu, ws = ctx.saved_tensors
         delta, scale, l2norm, lay = ctx.conf
         dev = q.device
+        kept = 1 + lay[3]                                        # the operands, and the tiles too
+        if ws is None:
+            kept = 0
+            lay = _layout(q.shape[0], cu.shape[0] - 1, q.shape[1], v.shape[1], q.shape[2], v.shape[2], delta, True, 0)
+            ws = torch.empty(lay[1], dtype=torch.uint8, device=dev)
         dy = torch.zeros_like(v, memory_format=_CONTIGUOUS) if dy is None else _rows(dy)
         ds_out = _state(ds_out)
         ds_in = torch.empty_like(s_in) if ctx.needs_input_grad[7] else None
@@ -159,8 +167,8 @@ class _Recurrence(torch.autograd.Function):
         _lib.call_on(dev, "xb_recurrence_bwd", _words(q, k, v, g, b, A, D, cu, s_in, None, ds_out, ds_in, dy,
                                                (0, dq.data_ptr(), dkk.data_ptr(), dvv.data_ptr(), _ptr(dg), db.data_ptr(),
                                                 _ptr(dA), _ptr(dD)), ws, tmp, lay, delta, l2norm),
-              scale, delta, lay[3])
-        _launches += (2 if delta else 3) + (not lay[3])
+              scale, delta, kept)
+        _launches += (2 if delta else 3) + (kept < 2) + 2 * (kept == 0)
         return dq, dkk, dvv, dg, db, dA, dD, ds_in, None, None, None, None, None
 
 
