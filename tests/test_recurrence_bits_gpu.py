@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from test_recurrence_gpu import _need_cuda, delta_inputs, run_delta, run_scan, scan_inputs  # noqa: F401
-from test_recurrence_use_gpu import OPS, both_ways, boundaries, call, same
+from test_recurrence_use_gpu import OPS, both_ways, boundaries, call, inputs, same
 
 pytestmark = pytest.mark.gpu
 
@@ -90,3 +90,25 @@ def test_gradients_behind_documents_of_few_tokens(op, cuts, hk, hv, dk, dv):
     o, S = call(op, leaves, boundaries(cuts))
     d = [torch.randn_like(o), torch.randn_like(S)]
     same(torch.autograd.grad([o, S], leaves, d, retain_graph=True), torch.autograd.grad([o, S], leaves, d))
+
+
+@pytest.mark.parametrize("op", OPS)
+@pytest.mark.parametrize("cuts", [[0, 70, 71, 300], list(range(0, 301, 10))], ids=["chunks", "few tokens"])
+@pytest.mark.parametrize("keep", [True, False])
+def test_boundaries_are_the_callers_again_behind_the_forward_pass(op, cuts, keep, monkeypatch):
+    """A buffer of boundaries that takes the next batch's before the backward pass of this one, whatever the call keeps."""
+    from xorl_b200.ops import recurrence as R
+    if not keep:
+        monkeypatch.setattr(R, "KEEP_BYTES", 0)
+        R._layout.cache_clear()
+    try:
+        ts, cu = inputs(op, docs=len(cuts) - 1), boundaries(cuts)
+        want = both_ways(op, ts, cu)
+        leaves = [t.detach().requires_grad_() for t in ts]
+        o, S = call(op, leaves, cu)
+        cu.copy_(torch.arange(len(cuts)))
+        gen = torch.Generator(device="cuda").manual_seed(9)
+        do, dS = torch.randn(o.shape, generator=gen, device="cuda").bfloat16(), torch.randn(S.shape, generator=gen, device="cuda")
+        same(want, [o.detach(), S.detach(), *torch.autograd.grad([o, S], leaves, [do, dS])])
+    finally:
+        R._layout.cache_clear()

@@ -90,8 +90,8 @@ def _layout(T: int, docs: int, Hk: int, Hv: int, dk: int, dv: int, delta: bool, 
     return nc, kept_bytes, later_bytes, keep, tuple(kept), tuple(later)
 
 
-def _words(q, k, v, g, b, A, D, cu, s_in, s_out, ds_out, ds_in, dy, outs, ws, tmp, lay, delta, l2norm, step=0):
-    """The arguments of the C entry points."""
+def _words(q, k, v, g, b, A, D, cu, s_in, s_out, ds_out, ds_in, dy, outs, ws, tmp, lay, delta, l2norm, step=0, docs=None):
+    """The arguments of the C entry points; ``docs`` where there are no boundaries."""
     T, Hk, dk = q.shape
     _, Hv, dv = v.shape
     qs, ks, vs, bs = q.stride(), k.stride(), v.stride(), b.stride()
@@ -107,9 +107,9 @@ def _words(q, k, v, g, b, A, D, cu, s_in, s_out, ds_out, ds_in, dy, outs, ws, tm
     return _pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), 0 if dy is None else dy.data_ptr(), qs[0], qs[1], ks[0], ks[1],
                   vs[0], vs[1], *((0, 0) if dy is None else dy.stride()[:2]),
                   0 if g is None else g.data_ptr(), b.data_ptr(), *((0, 0) if g is None else g.stride()), bs[0], bs[1],
-                  _ptr(A), _ptr(D), cu.data_ptr(), _ptr(s_in), _ptr(s_out), _ptr(ds_out), _ptr(ds_in),
+                  _ptr(A), _ptr(D), _ptr(cu), _ptr(s_in), _ptr(s_out), _ptr(ds_out), _ptr(ds_in),
                   *((dv, 1) if delta else (1, dk)), *outs, *work,
-                  T, cu.shape[0] - 1, Hk, Hv, dk, dv, nc, l2norm, step)
+                  T, cu.shape[0] - 1 if docs is None else docs, Hk, Hv, dk, dv, nc, l2norm, step)
 
 
 def _ptr(t) -> int:
@@ -137,8 +137,9 @@ class _Recurrence(torch.autograd.Function):
                                                       (o.data_ptr(), 0, 0, 0, 0, 0, 0, 0), ws, None, lay, delta, l2norm, step),
                      scale, delta)
         _launches += 3 if not step else 4 if T > step else 1
-        ctx.save_for_backward(q, k, v, g, b, A, D, s_in, cu, None if step else ws)
-        ctx.conf = (delta, scale, l2norm, lay)
+        # boundaries are read again only where the plan is made again, from a copy: the caller's may hold the next batch's by then
+        ctx.save_for_backward(q, k, v, g, b, A, D, s_in, cu.clone() if step and train else None, None if step else ws)
+        ctx.conf = (delta, scale, l2norm, docs, lay)
         ctx.set_materialize_grads(False)
         return o, s_out
 
@@ -147,12 +148,12 @@ class _Recurrence(torch.autograd.Function):
     def backward(ctx, dy, ds_out):
         global _launches
         q, k, v, g, b, A, D, s_in, cu, ws = ctx.saved_tensors
-        delta, scale, l2norm, lay = ctx.conf
+        delta, scale, l2norm, docs, lay = ctx.conf
         dev = q.device
         kept = 1 + lay[3]                                        # the operands, and the tiles too
         if ws is None:
             kept = 0
-            lay = _layout(q.shape[0], cu.shape[0] - 1, q.shape[1], v.shape[1], q.shape[2], v.shape[2], delta, True, 0)
+            lay = _layout(q.shape[0], docs, q.shape[1], v.shape[1], q.shape[2], v.shape[2], delta, True, 0)
             ws = torch.empty(lay[1], dtype=torch.uint8, device=dev)
         dy = torch.zeros_like(v, memory_format=_CONTIGUOUS) if dy is None else _rows(dy)
         ds_out = _state(ds_out)
@@ -166,7 +167,7 @@ class _Recurrence(torch.autograd.Function):
         tmp = torch.empty(lay[2], dtype=torch.uint8, device=dev)
         _lib.call_on(dev, "xb_recurrence_bwd", _words(q, k, v, g, b, A, D, cu, s_in, None, ds_out, ds_in, dy,
                                                (0, dq.data_ptr(), dkk.data_ptr(), dvv.data_ptr(), _ptr(dg), db.data_ptr(),
-                                                _ptr(dA), _ptr(dD)), ws, tmp, lay, delta, l2norm),
+                                                _ptr(dA), _ptr(dD)), ws, tmp, lay, delta, l2norm, docs=docs),
               scale, delta, kept)
         _launches += (2 if delta else 3) + (kept < 2) + 2 * (kept == 0)
         return dq, dkk, dvv, dg, db, dA, dD, ds_in, None, None, None, None, None
