@@ -112,3 +112,27 @@ def test_boundaries_are_the_callers_again_behind_the_forward_pass(op, cuts, keep
         same(want, [o.detach(), S.detach(), *torch.autograd.grad([o, S], leaves, [do, dS])])
     finally:
         R._layout.cache_clear()
+
+
+@pytest.mark.parametrize("op", OPS)
+def test_what_a_call_keeps_is_bounded(op, monkeypatch):
+    """Nothing, the operands, or the tiles too: within the bound, which a program may set at any time, with the same bits."""
+    from xorl_b200.ops import recurrence as R
+    ts, cu = inputs(op, T=2000, docs=2), boundaries([0, 700, 2000])
+    want = both_ways(op, ts, cu)
+    hk, hv, d = 2, 4, 64
+    full = R._layout(2000, 2, hk, hv, d, d, op == "delta", True, 0, 1 << 40)
+    part = R._layout(2000, 2, hk, hv, d, d, op == "delta", True, 0, full[1] - 1)
+    assert (full[3], part[3]) == (2, 1) and part[1] < full[1]
+    out = ts[2 if op == "delta" else 0].numel() * 2 + ts[-1].numel() * 4          # outputs and states
+    for limit, bound in ((full[1], full[1]), (full[1] - 1, part[1]), (part[1], part[1]), (part[1] - 1, 0), (0, 0)):
+        monkeypatch.setattr(R, "KEEP_BYTES", limit)
+        leaves = [t.detach().requires_grad_() for t in ts]
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        o, S = call(op, leaves, cu)
+        assert torch.cuda.memory_allocated() - before <= out + bound + 8192       # the allocator rounds up
+        gen = torch.Generator(device="cuda").manual_seed(9)
+        do, dS = torch.randn(o.shape, generator=gen, device="cuda").bfloat16(), torch.randn(S.shape, generator=gen, device="cuda")
+        same(want, [o.detach(), S.detach(), *torch.autograd.grad([o, S], leaves, [do, dS])])
+        del o, S, do, dS, leaves

@@ -29,9 +29,12 @@ _launches = 0
 CHUNK = 64              # tokens of a chunk of the kernels (csrc/recurrence.cu)
 TILE = 16384            # bytes of an operand tile of the state
 MAX_STATE_ROWS = 128
-# The state tiles of all chunks, and what goes with them, are kept for the backward pass up to this size (4096 tokens of 32
-# heads of 128 x 128: 0.3 GB); a longer call makes them again, which is the forward pass without its outputs once more
-# (16384 tokens of such heads, forward and backward: 2.0 ms kept, 2.3 ms made again).
+# What a call may keep from its forward pass for its backward pass besides its inputs, in bytes; a program may set it.  It keeps
+# the operands and the state tiles of all chunks if both fit (4096 tokens of 32 heads of 128 x 128: 0.4 GB), or the operands
+# alone, and makes the rest again: the tiles are the forward pass without its outputs once more, the operands its prepare
+# kernel.  Forward and backward, kept, operands alone, nothing: 4096 tokens of such heads 0.52, 0.61, 0.67 ms; 16384 tokens (1.6
+# GB) 1.92, 2.27, 2.43 ms; the scan of 128 heads of 64 x 128, 4096 tokens (0.6 GB) 0.64, 0.72, 0.74 ms.  The bound is about a
+# hundredth of the GPU's memory, so that some tens of such layers which recompute nothing leave room for the rest.
 KEEP_BYTES = 3 << 29
 # With at most so many tokens per document on average, documents of at most so many go token by token
 # (csrc/recurrence_step.cu, which gives the times of both ways), the others through the chunked kernels.  The same with and
@@ -65,10 +68,10 @@ def _state(x: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
 
 
 @functools.lru_cache(maxsize=256)
-def _layout(T: int, docs: int, Hk: int, Hv: int, dk: int, dv: int, delta: bool, train: bool, step: int):
-    """Where the workspaces of a call of these sizes lie: (chunks, bytes kept from the forward pass, bytes of the backward
-    pass, whether the state tiles are kept, offsets of chunks .. pt, of the kept tiles, of the backward pass's buffers).
-    ``step``: of the forward pass; a backward pass's own layout has none."""
+def _layout(T: int, docs: int, Hk: int, Hv: int, dk: int, dv: int, delta: bool, train: bool, step: int, limit: int = 0):
+    """Where the workspaces of a call of these sizes lie: (chunks, bytes of the forward pass's, bytes of the backward pass's,
+    what is kept in between (2: operands and state tiles, 1: operands, 0: nothing), offsets of chunks .. pt and of the tiles
+    among them, of the backward pass's buffers).  ``step``: of the forward pass; a backward pass's own layout has none."""
     nc = T // CHUNK + (T // (step + 1) if step else docs + 2)
     square = nc * CHUNK * CHUNK * 4
     work = [nc * 16, 2 * (docs + 3) * 4, nc * Hv * 3 * CHUNK * 4, nc * Hk * 2 * CHUNK * 4,
@@ -76,7 +79,6 @@ def _layout(T: int, docs: int, Hk: int, Hv: int, dk: int, dv: int, delta: bool, 
     tiles = nc * Hv * (-(-dv // 64) * 2) * TILE
     first = [tiles, tiles // 2 if delta else 0, tiles // 2 if delta else tiles]
     second = [tiles, tiles // 2 if delta else 0, nc * Hv * (-(-dv // 64) * 4 * CHUNK if delta else 2) * 4]
-    keep = train and sum(first) <= KEEP_BYTES
 
     def place(sizes):
         at, out = 0, []
@@ -85,9 +87,13 @@ def _layout(T: int, docs: int, Hk: int, Hv: int, dk: int, dv: int, delta: bool, 
             at += (s + 255) // 256 * 256
         return out, at
 
-    kept, kept_bytes = place(work + (first if keep else []))
-    later, later_bytes = place(second if keep else second + (first if train else [0, 0, 0]))
-    return nc, kept_bytes, later_bytes, keep, tuple(kept), tuple(later)
+    kept, kept_bytes = place(work + first)
+    if train and kept_bytes <= limit:
+        later, later_bytes = place(second)
+        return nc, kept_bytes, later_bytes, 2, tuple(kept), tuple(later)
+    kept, kept_bytes = place(work)
+    later, later_bytes = place(second + (first if train else [0, 0, 0]))
+    return nc, kept_bytes, later_bytes, int(train and kept_bytes <= limit), tuple(kept), tuple(later)
 
 
 def _words(q, k, v, g, b, A, D, cu, s_in, s_out, ds_out, ds_in, dy, outs, ws, tmp, lay, delta, l2norm, step=0, docs=None):
@@ -103,7 +109,7 @@ def _words(q, k, v, g, b, A, D, cu, s_in, s_out, ds_out, ds_in, dy, outs, ws, tm
         base = tmp.data_ptr()
         back = [base + o if o >= 0 else 0 for o in later]
     # state tiles (U and third parts with them) come from the forward pass or are made again; dS and dR tiles and partial sums are the backward's
-    work += back[3:] + back[:3] if not keep else back[:3]
+    work += back[:3] if keep == 2 else back[3:] + back[:3]
     return _pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), 0 if dy is None else dy.data_ptr(), qs[0], qs[1], ks[0], ks[1],
                   vs[0], vs[1], *((0, 0) if dy is None else dy.stride()[:2]),
                   0 if g is None else g.data_ptr(), b.data_ptr(), *((0, 0) if g is None else g.stride()), bs[0], bs[1],
@@ -129,7 +135,7 @@ class _Recurrence(torch.autograd.Function):
         docs = cu.shape[0] - 1
         train = True in ctx.needs_input_grad
         step = STEP if T <= STEP * max(docs, 1) else 0
-        lay = _layout(T, docs, Hk, Hv, dk, dv, delta, train and not step, step)
+        lay = _layout(T, docs, Hk, Hv, dk, dv, delta, train and not step, step, KEEP_BYTES)
         ws = torch.empty(lay[1], dtype=torch.uint8, device=dev)
         o = torch.empty_like(v, memory_format=_CONTIGUOUS)
         s_out = torch.empty((docs, Hv, dk, dv) if delta else (docs, Hv, dv, dk), dtype=torch.float32, device=dev) if final else None
@@ -138,7 +144,7 @@ class _Recurrence(torch.autograd.Function):
                      scale, delta)
         _launches += 3 if not step else 4 if T > step else 1
         # boundaries are read again only where the plan is made again, from a copy: the caller's may hold the next batch's by then
-        ctx.save_for_backward(q, k, v, g, b, A, D, s_in, cu.clone() if step and train else None, None if step else ws)
+        ctx.save_for_backward(q, k, v, g, b, A, D, s_in, cu.clone() if train and not lay[3] else None, ws if lay[3] else None)
         ctx.conf = (delta, scale, l2norm, docs, lay)
         ctx.set_materialize_grads(False)
         return o, s_out
@@ -150,9 +156,8 @@ class _Recurrence(torch.autograd.Function):
         q, k, v, g, b, A, D, s_in, cu, ws = ctx.saved_tensors
         delta, scale, l2norm, docs, lay = ctx.conf
         dev = q.device
-        kept = 1 + lay[3]                                        # the operands, and the tiles too
-        if ws is None:
-            kept = 0
+        kept = lay[3]
+        if not kept:
             lay = _layout(q.shape[0], docs, q.shape[1], v.shape[1], q.shape[2], v.shape[2], delta, True, 0)
             ws = torch.empty(lay[1], dtype=torch.uint8, device=dev)
         dy = torch.zeros_like(v, memory_format=_CONTIGUOUS) if dy is None else _rows(dy)
