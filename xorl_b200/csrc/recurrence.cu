@@ -57,6 +57,7 @@ __global__ void __launch_bounds__(1024) rec_plan(const int* __restrict__ cu, int
     if (d < nd) {
       const int2 r = doc_range(cu, n, T, d);
       v = r.y - r.x > step ? (r.y - r.x + C - 1) / C + DOC : 0;
+      if (bad_bounds(cu, n, T, d)) xb_report(status, XB_ERR_BAD_ARG, XB_K_RECURRENCE, d);
     }
     const bool some = v != 0;
 #pragma unroll
@@ -77,12 +78,11 @@ __global__ void __launch_bounds__(1024) rec_plan(const int* __restrict__ cu, int
     }
     __syncthreads();
     const long long all = carry + v + (w ? warp_tot[w - 1] : 0), incl = all & (DOC - 1);
-    // boundaries that overlap would need more chunks than the rows have: what does not fit is left out and reported
+    // boundaries that overlap may need more chunks than there is room for: what does not fit is left out
     if (d < nd) {
       doc_off[d + 1] = (int)min(incl, (long long)nc_max);
       if (some) doc_list[all / DOC] = d;
       if (d == nd - 1) doc_list[0] = (int)(all / DOC);
-      if (incl > nc_max) xb_report(status, XB_ERR_BAD_ARG, XB_K_RECURRENCE, d);
     }
     __syncthreads();
     if (tid == 0) carry += warp_tot[31];

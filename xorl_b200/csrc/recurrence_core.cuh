@@ -193,6 +193,11 @@ __device__ __forceinline__ int2 doc_range(const int* cu, int n, int T, int d) {
   const int s = cut(d);
   return make_int2(s, max(s, cut(d + 1)));
 }
+// Boundaries ascend from 0 or more to T or less.  What does not is clamped, so that nothing outside the rows is touched, and
+// reported: by the plan for all documents, by the token-by-token kernels for each of theirs.
+__device__ __forceinline__ bool bad_bounds(const int* cu, int n, int T, int d) {
+  return d < n ? cu[d] < 0 || cu[d + 1] < cu[d] || cu[d + 1] > T : d == n && (cu[n] < 0 || cu[n] > T);
+}
 // Documents that the grids of the chunked kernels cover: all, or at most those that are too long to go token by token.
 __host__ __device__ inline int rec_docs(const XbRecArgs& a) { return a.step > 0 ? a.T / (a.step + 1) : a.n_docs + 2; }
 // The document of a grid's `i`-th; -1: none.

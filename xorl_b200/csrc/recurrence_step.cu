@@ -79,6 +79,7 @@ __global__ void __launch_bounds__(THREADS, 7) delta_step(const __grid_constant__
   const int col = sl * NV + cg * 4, row = rg * R;
   const int2 r = doc_range(p.cu, p.n_docs, p.T, doc);
   const int len = r.y - r.x;
+  if (sl == 0 && h == 0 && threadIdx.x == 0 && bad_bounds(p.cu, p.n_docs, p.T, doc)) xb_report(p.status, XB_ERR_BAD_ARG, XB_K_RECURRENCE, doc);
   if (len > p.step) return;
   const bool vok = col < p.dv, kok = row < p.dk, first = rg == 0 && vok;
   bf16* o = (bf16*)p.o + ((long long)r.x * p.Hv + h) * p.dv + col;
@@ -161,6 +162,7 @@ __global__ void __launch_bounds__(THREADS, 5) scan_step(const __grid_constant__ 
   const int kh = h / (p.Hv / p.Hk), cg = threadIdx.x & 7, row = cb * ROWS + (threadIdx.x >> 3);
   const int2 r = doc_range(p.cu, p.n_docs, p.T, doc);
   const int len = r.y - r.x;
+  if (cb == 0 && h == 0 && threadIdx.x == 0 && bad_bounds(p.cu, p.n_docs, p.T, doc)) xb_report(p.status, XB_ERR_BAD_ARG, XB_K_RECURRENCE, doc);
   if (len > p.step) return;
   const bool state = doc < p.n_docs;
   __shared__ Inputs in;

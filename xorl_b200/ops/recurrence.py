@@ -3,8 +3,8 @@
 ``gated_delta_rule``  the recurrence of the GatedDeltaNet layers
 (src/xorl/ops/linear_attention/ops/gated_delta_rule/chunk.py), ``ssd_scan`` the one of the Mamba2 layers
 (src/xorl/ops/ssm/layers/mamba2_mixer.py).  Both carry one matrix state per head from token to token, restart it at
-every document of ``cu_seqlens`` (int32 or int64 [documents + 1] on the inputs' device, ascending; read on the device
-only), can take the states that enter the documents and return those that leave them, and are differentiable in every
+every document of ``cu_seqlens`` (int32 or int64 [documents + 1] on the inputs' device, ascending within the rows; read on
+the device only, where other boundaries are clamped and reported: ``_lib.raise_on_status``), can take the states that enter the documents and return those that leave them, and are differentiable in every
 floating input.
 
 On a GPU with bf16 inputs whose head dims are multiples of 8 (state rows at most 128) the CUDA kernels run; they keep
