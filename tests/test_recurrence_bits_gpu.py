@@ -136,3 +136,13 @@ def test_what_a_call_keeps_is_bounded(op, monkeypatch):
         do, dS = torch.randn(o.shape, generator=gen, device="cuda").bfloat16(), torch.randn(S.shape, generator=gen, device="cuda")
         same(want, [o.detach(), S.detach(), *torch.autograd.grad([o, S], leaves, [do, dS])])
         del o, S, do, dS, leaves
+
+
+@pytest.mark.parametrize("docs,length", [(1, 100), (2, 256), (3, 520), (40, 64), (10, 300), (3, 700)])
+@pytest.mark.parametrize("heads", [2, 20])
+def test_stages_of_the_walk(docs, length, heads):
+    """Few and many CTAs, short and long documents, on both sides of the walk's choice: without gradients the bits of the call
+    with them, which always has two stages."""
+    T = docs * length
+    ts = list(delta_inputs(T, heads // 2, heads, 128, 128, docs, seed=23, state=True))
+    same(*call_both("delta", ts, boundaries(list(range(0, T + 1, length)))))

@@ -1034,11 +1034,13 @@ int prep(const XbRecArgs& a, cudaStream_t st) {
 int xb_delta_prep(const XbRecArgs& a, cudaStream_t st) { return a.dk <= 64 ? prep<64>(a, st) : prep<128>(a, st); }
 int xb_delta_fwd(const XbRecArgs& a, cudaStream_t st) {
   if (a.s_tiles != nullptr) return run<delta_fwd<true, true, 2>, Lay<false, 2>::SMEM>(a, a.v, a.v_t, a.v_h, st);
-  // Documents of four chunks on average or fewer: two CTAs per SM, one stage each, hide one another's way in and out (40
-  // documents of 64, 100, 200 and 400 tokens, 32 heads of 128 x 128: 128, 182, 295, 455 us; with two stages 195, 261, 368,
-  // 512).  Longer ones, of which there are fewer CTAs, want the next chunk's loads ahead of them (one document of 1000
-  // tokens: 46 us and 29 us).
-  if (4ll * C * a.n_docs >= a.T) return run<delta_fwd<true, false, 1>, Lay<false, 1>::SMEM>(a, a.v, a.v_t, a.v_h, st);
+  // Two CTAs per SM, one stage each, hide one another's way in and out, but a chunk's loads wait for the chunk before.  They pay
+  // where there are more CTAs than SMs and a document has eight chunks or fewer on average.  One stage and two stages, heads of
+  // 128 x 128 without gradients, us: 32 heads, 40 documents of 64 tokens 131 and 192, of 128 212 and 272, of 256 371 and 422, of
+  // 400 611 and 655; 16 documents of 1000 537 and 542, three of 1000 150 and 129, two of 4000 310 and 287.  At most one CTA per
+  // SM, 4 heads: one document of 128 tokens 25 and 23, of 256 29 and 26, of 1000 60 and 43; eight of 400 38 and 31.
+  if ((long long)a.n_docs * a.Hv * (a.dvp / NV) > xb_sm_count() && 8ll * C * a.n_docs >= a.T)
+    return run<delta_fwd<true, false, 1>, Lay<false, 1>::SMEM>(a, a.v, a.v_t, a.v_h, st);
   return run<delta_fwd<true, false, 2>, Lay<false, 2>::SMEM>(a, a.v, a.v_t, a.v_h, st);
 }
 int xb_delta_bwd(const XbRecArgs& a, int tiles, cudaStream_t st) {
