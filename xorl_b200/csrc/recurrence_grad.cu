@@ -35,9 +35,11 @@ struct Lay {
                        SM_RED = SM_HD + 2 * 1024;
 };
 struct Red {                                        // what meets across warps, one set per head in turn
-  float rd[3][PARTS][C];                            // q.t1, k.t2, k.t3 by column part
-  float er[PARTS][C], fr[PARTS][C];                 // row sums of dP o P and dL o A by column part (scan: dP o P)
-  float ec[4][C], fc[4][C];                         // column sums by row block
+  float rd[3][PARTS][C];                            // q.t1, k.t2, k.t3 by column part (scan: the second holds the diagonal of dP o P)
+  // Row sums of dP o P and dL o A by column part (scan: dP o P), column sums by row block.  Without the diagonal: it carries no
+  // decay and would cancel in the decay's gradient, but as two roundings of what strong decays leave as the largest term.
+  float er[PARTS][C], fr[PARTS][C];
+  float ec[4][C], fc[4][C];
   float rv[2][C], sdot[WORKERS / 32];                // scan: dO.v by column half of every slice; <S, dS'> by warp
 };
 struct __align__(8) Bars {
@@ -355,7 +357,7 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
         } else {
           x[i] = (double)q1 + (double)e1 - (double)(bt * e2) - (double)(bt * k3);
           tail += (double)(bt * k3);
-          db[i] = e2 + k3;
+          db[i] = e2 + r.rd[1][0][t] + k3;
           if (on) dsum += r.rv[0][t] + r.rv[1][t];
         }
       }
@@ -520,7 +522,10 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
       }
       const float d1 = add_rows(base + COL_T1 + set * 128 + w0, sm + L::SM_Q, r0, w0, f1, aq);
       const float d2 = DELTA ? add_rows(base + COL_T2 + w0, sm + L::SM_K, r0, w0, f2, ak) : 0.f;
-      if (t < 2) r.rd[0][hf][sum_row] = d1, r.rd[1][hf][sum_row] = d2, r.rd[2][hf][sum_row] = d3;
+      if (t < 2) {
+        r.rd[0][hf][sum_row] = d1, r.rd[2][hf][sum_row] = d3;
+        if (DELTA) r.rd[1][hf][sum_row] = d2;
+      }
       {
         uint32_t x[8], xl[8];
         float2 qr[2][2], kr[2][2];
@@ -550,8 +555,10 @@ rec_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
             {
               const float y0 = j <= last ? e0 * __uint_as_float(x[4 * n + 2 * h]) : 0.f, w0 = j <= last ? y0 * qr[n][h].x : 0.f;
               const float y1 = j < last ? e1 * __uint_as_float(x[4 * n + 2 * h + 1]) : 0.f, w1 = j < last ? y1 * qr[n][h].y : 0.f;
-              er[h] += DELTA ? w0 + w1 : bj.x * w0 + bj.y * w1;
-              ec[n][0] += w0, ec[n][1] += w1;
+              const float s0 = j < row[h] ? w0 : 0.f, s1 = j + 1 < row[h] ? w1 : 0.f;
+              if (!DELTA && (j == row[h] || j + 1 == row[h])) r.rd[1][0][row[h]] = j == row[h] ? w0 : w1;
+              er[h] += DELTA ? s0 + s1 : bj.x * s0 + bj.y * s1;
+              ec[n][0] += s0, ec[n][1] += s1;
               const Pair f = pair(rq[h] * kj.x, rq[h] * kj.y) * pair(y0, y1);
               az[n][h] = DELTA ? az[n][h] + f : fma2(f, pair(bj.x, bj.y), az[n][h]);
             }
