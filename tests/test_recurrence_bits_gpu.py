@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from test_recurrence_gpu import _need_cuda, delta_inputs, run_delta, run_scan, scan_inputs  # noqa: F401
-from test_recurrence_use_gpu import OPS, both_ways, boundaries, call, inputs, same
+from test_recurrence_use_gpu import OPS, both_ways, boundaries, call, inputs, layer, same
 
 pytestmark = pytest.mark.gpu
 
@@ -146,3 +146,17 @@ def test_stages_of_the_walk(docs, length, heads):
     T = docs * length
     ts = list(delta_inputs(T, heads // 2, heads, 128, 128, docs, seed=23, state=True))
     same(*call_both("delta", ts, boundaries(list(range(0, T + 1, length)))))
+
+
+@pytest.mark.parametrize("kind", OPS)
+@pytest.mark.parametrize("cuts", [[0, 33, 34, 200], list(range(0, 201, 8))], ids=["chunks", "few tokens"])
+def test_layers_recomputed(kind, cuts):
+    """A layer's first pass without gradients and the one that is run again for them."""
+    from xorl_b200.models.context import StepContext
+    m = layer(kind)
+    ctx = StepContext(cu_seqlens=boundaries(cuts), position_ids=torch.cat([torch.arange(b - a) for a, b in zip(cuts, cuts[1:])]).cuda(),
+                      max_seqlen=max(b - a for a, b in zip(cuts, cuts[1:])))
+    x = torch.randn(200, 256, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).bfloat16()
+    with torch.no_grad():
+        first = m(x, ctx)
+    assert torch.equal(first, m(x.requires_grad_(), ctx).detach())
