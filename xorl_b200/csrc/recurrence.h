@@ -26,7 +26,7 @@ struct XbRecArgs {
   int* doc_list;                 // [n_docs + 3], behind doc_off: how many documents have chunks, and which
   float* hd;                     // [nc_max, Hv, 192]
   float* rqk;                    // [nc_max, Hk, 128]
-  float *qk, *kk;                // [nc_max, Hk, 64, 64] (delta rule: for the backward pass, null without one)
+  float *qk, *kk;                // [nc_max, Hk, 64, 64] (delta rule: for the backward pass, null in calls without gradients)
   void* pt;                      // [nc_max, Hv]: operand tile [T; P], two planes, and a third of T: 40960 bytes (delta rule only)
   // operand tiles of [rows][hi 32 | lo 32] bf16, [nc_max, Hv, dvp / 32]: states entering and gradients of those leaving
   // the chunks (16 KB), U and dR (8 KB, delta rule only)

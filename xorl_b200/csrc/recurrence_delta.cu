@@ -23,11 +23,11 @@
 // fragments, which gives every lane values.  Eight warps work on the accumulators, one issues the products, one moves
 // tiles in and out.
 //
-// A forward step takes 2800 cycles: three times about 450 of products and their latency, the rest on the way from
-// accumulator to operand (four or sixteen warps on it: 2 % and 13 % more; mma.sync instead of tcgen05: 5800 cycles).  32
-// heads of 128 x 128: forward 370 us for a document of 16384 tokens and 135 us for 4096 tokens in five documents with
-// their tiles kept (0.26 GB written; with two parts 125), backward 136 us (118); prepare 144 and 49 us (268 and 90 MB written: latencies of small
-// steps, three CTAs per SM).
+// A forward step takes 3000 cycles (with two parts 2800): three times about 450 to 500 of products and their latency, the rest
+// on the way from accumulator to operand (four or sixteen warps on it: 2 % and 13 % more; mma.sync instead of tcgen05: 5800
+// cycles).  32 heads of 128 x 128: forward 397 us for a document of 16384 tokens (370) and 136 us for 4096 tokens in five
+// documents with their tiles kept (0.26 GB written; 125), backward 136 us (118); prepare 151 and 50 us (0.34 and 0.11 GB
+// written: latencies of small steps, three CTAs per SM).
 #include "recurrence_core.cuh"
 
 namespace {

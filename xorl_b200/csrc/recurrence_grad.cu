@@ -11,7 +11,7 @@
 // Sixteen worker warps, a loading and an issuing warp, and one that turns the heads' sums into gradients of the decay.
 //
 // It reads the tiles that the two sequential passes keep (56 KB per head and 32 columns; scan 48 KB).  4096 tokens of 32
-// heads of 128 x 128: 217 us, 0.52 GB of tiles at 2.4 TB/s; 4095 tokens of 128 heads of 64 x 128: 269 us, 0.87 GB at 3.2
+// heads of 128 x 128: 217 us, 0.52 GB of tiles at 2.4 TB/s; 4095 tokens of 128 heads of 64 x 128: 276 us, 0.87 GB at 3.2
 // TB/s (without third parts 208 and 244 us).  All of tensor memory holds one head's five products (scan: two heads' dP and t1), so that loads overlap the
 // workers' turn and products do not; with two heads per CTA a third of the time is its way in and out.
 #include "recurrence_core.cuh"

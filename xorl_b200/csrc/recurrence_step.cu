@@ -1,5 +1,5 @@
-// Gated linear recurrences, documents of a few tokens (single ones when a model answers): token by token, the state in
-// registers (the formulas stand in recurrence.cu).
+// Gated linear recurrences, documents of a few tokens, down to single ones whose states come from the call before: token by
+// token, the state in registers (the formulas stand in recurrence.cu).  Forward only: a backward pass works on chunks.
 //
 // What counts is the state: 64 KB read and written per head of 128 x 128, next to nothing to compute.  A CTA holds 16 KB
 // of one head's state, each row segment 128 bytes; all its loads, and those of the document's inputs, are issued before the
@@ -10,10 +10,10 @@
 // so that one round of sums per token serves both products.
 //
 // 48 documents of one token, 32 heads of 128 x 128 (201 MB): 35 us, 5.7 TB/s; 200 documents: 131 us, 6.4 TB/s.  Scan, 48
-// documents, 128 heads of 64 x 128 (403 MB): 64 us, 6.3 TB/s.  Further tokens cost about 8 and 14 us each; their inputs
-// come from shared memory, since one at a time from global memory each cost another 7 and 12 us.  At 16 tokens the
-// chunked kernels take as long: 48 documents of 16, delta rule 150 us (chunks: 222), scan 279 us (chunks: 339), with 45
-// and 58 us for chunked kernels that find nothing to do.
+// documents, 128 heads of 64 x 128 (403 MB): 64 us, 6.3 TB/s (L2 full of other data to be written back: 38, 140 and 70 us).
+// Further tokens cost about 8 and 14 us each; their inputs come from shared memory, since one at a time from global memory
+// each cost another 7 and 12 us.  At 16 tokens the chunked kernels take about as long: 48 documents of 16, delta rule 150 us
+// (chunks: 222), scan 279 us (chunks: 339), with 45 and 59 us for chunked kernels that find nothing to do.
 #include "recurrence_core.cuh"
 
 namespace {
