@@ -57,7 +57,7 @@ def call_both(op, ts, cu):
 
 CUTS = {"one": [0, 300], "two chunks": [0, 128], "long and short": [0, 1, 2, 3, 4, 5, 6, 7, 8, 9, 300], "outside": [40, 40, 101, 250],
         "many": list(range(0, 2001, 50)), "tokens": list(range(0, 120)), "short and long": [5, 6, 7, 8, 9, 9, 10, 30, 31, 47, 48, 112],
-        "short and outside": [20, 21, 22, 37, 54, 55, 55, 56, 57]}
+        "padded": [0, 100, 290] + [300] * 30, "short and outside": [20, 21, 22, 37, 54, 55, 55, 56, 57]}
 
 
 @pytest.mark.parametrize("op", OPS)
@@ -76,9 +76,9 @@ def test_calls_with_and_without_gradients(op, cuts, hk, hv, dk, dv, state):
 @pytest.mark.parametrize("cuts", [[0, 1, 2, 3, 40, 41, 41, 57, 70], [18, 19, 20, 36, 53, 60, 61, 62], list(range(0, 65))],
                          ids=["mixed", "outside", "ones"])
 @pytest.mark.parametrize("hk,hv,dk,dv", [(2, 4, 64, 64), (1, 3, 128, 72), (4, 4, 24, 8)])
-def test_gradients_behind_documents_of_few_tokens(op, cuts, hk, hv, dk, dv):
-    """The forward pass goes token by token and keeps nothing; the backward pass makes the chunks' operands and tiles, twice in a
-    row with the same bits."""
+def test_gradients_behind_documents_of_few_tokens(op, cuts, hk, hv, dk, dv, monkeypatch):
+    """The forward pass goes token by token, the backward pass works on chunks, from kept tiles or from ones that it makes itself,
+    twice in a row with the same bits."""
     T, docs = cuts[-1] + 5, len(cuts) - 1
     if op == "delta":
         run_delta(delta_inputs(T, hk, hv, dk, dv, docs, seed=19, state=True), cuts, scale=dk ** -0.5)
@@ -89,7 +89,13 @@ def test_gradients_behind_documents_of_few_tokens(op, cuts, hk, hv, dk, dv):
     leaves = [t.detach().requires_grad_() for t in ts]
     o, S = call(op, leaves, boundaries(cuts))
     d = [torch.randn_like(o), torch.randn_like(S)]
-    same(torch.autograd.grad([o, S], leaves, d, retain_graph=True), torch.autograd.grad([o, S], leaves, d))
+    want = torch.autograd.grad([o, S], leaves, d, retain_graph=True)
+    same(want, torch.autograd.grad([o, S], leaves, d))
+    from xorl_b200.ops import recurrence as R
+    monkeypatch.setattr(R, "KEEP_BYTES", 0)
+    again = call(op, leaves, boundaries(cuts))
+    same([o, S], again)
+    same(want, torch.autograd.grad(again, leaves, d))
 
 
 @pytest.mark.parametrize("op", OPS)

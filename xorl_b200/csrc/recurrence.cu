@@ -166,13 +166,16 @@ static XbRecArgs unpack(const long long* w, float scale) {
 XB_API int xb_recurrence_fwd(const long long* words, float scale, int delta, void* stream) {
   if (words == nullptr) return -1;
   const XbRecArgs a = unpack(words, scale);
-  if (bad_args(a)) return -1;
+  XbRecArgs chunked = a;
+  if (a.s_tiles != nullptr) chunked.step = 0;                 // tiles are kept of all documents
+  if (bad_args(chunked) || a.step < 0 || a.step >= C) return -1;
   cudaStream_t st = (cudaStream_t)stream;
-  if (a.step > 0)
-    if (int rc = xb_recurrence_step(a, delta, st)) return rc;
-  if (a.step > 0 && a.T <= a.step) return 0;                  // no document can be longer
-  if (int rc = prepare(a, delta, st)) return rc;
-  return delta ? xb_delta_fwd(a, st) : xb_scan_fwd(a, st);
+  if (chunked.step == 0 || a.T > a.step) {                    // else no document has chunks
+    if (int rc = prepare(chunked, delta, st)) return rc;
+    if (int rc = delta ? xb_delta_fwd(chunked, st) : xb_scan_fwd(chunked, st)) return rc;
+  }
+  // behind the walk: with tiles it has written outputs and states of these documents too
+  return a.step > 0 ? xb_recurrence_step(a, delta, st) : 0;
 }
 
 // kept: what the forward pass has left, 2: the operands of the chunks and the state tiles, 1: the operands, 0: nothing.

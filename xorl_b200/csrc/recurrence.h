@@ -36,6 +36,6 @@ struct XbRecArgs {
   void* r_tiles;
   float* part;                   // scan: [nc_max, Hv, 2]; delta rule: dR.v by 16 columns, [nc_max, Hv, dvp / 16, 64]
   int* status;                   // filled in by the entry points
-  int T, n_docs, Hk, Hv, dk, dv, dvp, nc_max, l2norm, step;   // step: documents of so many tokens at most go token by token; dvp: dv rounded up to 64
+  int T, n_docs, Hk, Hv, dk, dv, dvp, nc_max, l2norm, step;   // step: documents of so many tokens at most go token by token (0 in the chunked kernels where they take all); dvp: dv rounded up to 64
   float scale;
 };

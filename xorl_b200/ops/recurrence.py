@@ -41,8 +41,9 @@ MAX_STATE_ROWS = 128
 KEEP_BYTES = 3 << 29
 # With at most so many tokens per document on average, documents of at most so many go token by token
 # (csrc/recurrence_step.cu, which gives the times of both ways), the others through the chunked kernels.  The same with and
-# without gradients, so that a forward pass that is run again for its gradients has the bits of the first one; a backward
-# pass works on chunks, and makes theirs itself behind such a call.
+# without gradients, so that a forward pass that is run again for its gradients has the bits of the first one.  A backward
+# pass works on chunks: where their tiles may be kept all documents go through the chunked kernels too, else the backward
+# pass makes what it needs.
 STEP = 16
 OPERANDS = 40960        # bytes of the operand tile that the delta rule prepares per chunk and head
 
@@ -138,14 +139,16 @@ class _Recurrence(torch.autograd.Function):
         docs = cu.shape[0] - 1
         train = True in ctx.needs_input_grad
         step = STEP if T <= STEP * max(docs, 1) else 0
-        lay = _layout(T, docs, Hk, Hv, dk, dv, delta, train and not step, step, KEEP_BYTES)
+        lay = _layout(T, docs, Hk, Hv, dk, dv, delta, train, 0, KEEP_BYTES)
+        if step and lay[3] < 2:
+            lay = _layout(T, docs, Hk, Hv, dk, dv, delta, False, step)
         ws = torch.empty(lay[1], dtype=torch.uint8, device=dev)
         o = torch.empty_like(v, memory_format=_CONTIGUOUS)
         s_out = torch.empty((docs, Hv, dk, dv) if delta else (docs, Hv, dv, dk), dtype=torch.float32, device=dev) if final else None
         _lib.call_on(dev, "xb_recurrence_fwd", _words(q, k, v, g, b, A, D, cu, s_in, s_out, None, None, None,
                                                       (o.data_ptr(), 0, 0, 0, 0, 0, 0, 0), ws, None, lay, delta, l2norm, step),
                      scale, delta)
-        _launches += 3 if not step else 4 if T > step else 1
+        _launches += 3 if not step else 4 if T > step or lay[3] else 1
         # boundaries are read again only where the plan is made again, from a copy: the caller's may hold the next batch's by then
         ctx.save_for_backward(q, k, v, g, b, A, D, s_in, cu.clone() if train and not lay[3] else None, ws if lay[3] else None)
         ctx.conf = (delta, scale, l2norm, docs, lay)
