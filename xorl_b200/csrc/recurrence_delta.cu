@@ -596,6 +596,7 @@ delta_fwd(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtens
     if (OUT) zero_rows(p, a, o, o_t);
     return;
   }
+  static_assert(STAGES == 2 || (OUT && !SAVE), "one stage: U lies over R, and the wait for P U frees both");
   constexpr bool LATE = STAGES == 2;         // where O is written
   constexpr int COLS = LATE ? 512 : 256, DPU = LATE ? D5 : D2;
   cta_begin<COLS>(a);
