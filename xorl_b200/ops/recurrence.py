@@ -4,8 +4,8 @@
 (src/xorl/ops/linear_attention/ops/gated_delta_rule/chunk.py), ``ssd_scan`` the one of the Mamba2 layers
 (src/xorl/ops/ssm/layers/mamba2_mixer.py).  Both carry one matrix state per head from token to token, restart it at
 every document of ``cu_seqlens`` (int32 or int64 [documents + 1] on the inputs' device, ascending within the rows; read on
-the device only, where other boundaries are clamped and reported: ``_lib.raise_on_status``), can take the states that enter the documents and return those that leave them, and are differentiable in every
-floating input.
+the device only, where other boundaries are clamped and reported: ``_lib.raise_on_status``), can take the states that
+enter the documents and return those that leave them, and are differentiable in every floating input.
 
 On a GPU with bf16 inputs whose head dims are multiples of 8 (state rows at most 128) the CUDA kernels run.  They add up
 states, sums and gradients in 32 bits and round outputs once; a computed value that enters a product of the tensor cores
@@ -13,9 +13,9 @@ states, sums and gradients in 32 bits and round outputs once; a computed value t
 outputs off by up to 7e-6 of their norm.  Elsewhere, and in the ``_reference`` forms for who wants fp32 throughout, the same
 arithmetic runs as tensor ops.  Outputs have the same bits with and without gradients, so that a recomputed pass repeats the
 first one.  The kernels read strided inputs in place when the last dimension is contiguous and rows start on 16-byte
-boundaries, and copy others.  A call allocates its workspace; it does not synchronise and may be captured into a CUDA graph (a backward pass:
-while no graph of the same leaves that was built outside the capture is alive, since torch would wait for its stream and end
-the process)."""
+boundaries, and copy others.  A call allocates its workspace; it does not synchronise and may be captured into a CUDA
+graph (a backward pass: while no graph of the same leaves that was built outside the capture is alive, since torch would
+wait for its stream and end the process)."""
 from __future__ import annotations
 
 import functools
